@@ -21,6 +21,10 @@ reference (noetic crate)               here
 ``Lm::loss`` (model.rs:228-234)        :meth:`Model.loss`
 =====================================  ===========================================
 
+Beyond the reference (:mod:`noetic_b200.head`, ``include/noetic/head.h``):
+:func:`token_logprobs`, :func:`distill` and :func:`layer_norm` with their
+gradients, and :meth:`Model.score`.
+
 Every computation runs on the GPU through hand-written sm_100a kernels.  There
 is no CPU fallback: importing works without a GPU, but every call that needs
 the library raises :class:`NoeticError` when the extension or a device is
@@ -35,6 +39,9 @@ import os
 from dataclasses import dataclass
 
 import numpy as np
+
+from . import head
+from .head import (NO_TOKEN, distill, layer_norm, layer_norm_backward, token_logprobs, token_logprobs_backward)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnoetic_gpu.so")
@@ -143,7 +150,7 @@ def lib():
             raise NoeticError(NK_ERR_UNSUPPORTED,
                               f"{LIB_PATH} is not built; run python noetic_b200/make_lib.py")
         L = C.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (*SIGNATURES.items(), *head.SIGNATURES.items()):
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args
@@ -295,6 +302,12 @@ class Model:
         _check(lib().nk_model_loss(self.h, _ptr(ids), _ptr(targets), batch, t, C.byref(loss),
                                    _ptr(out) if out is not None else None))
         return (float(loss.value), out) if want_logits else float(loss.value)
+
+    def score(self, ids, targets, batch: int, t: int, top: int = 0) -> dict:
+        """Log probability and entropy of every position of `batch` sequences of
+        `t` tokens ([batch, t]; targets 0xFFFFFFFF have none), and with `top` the
+        most probable tokens there (`top_ids`, `top_logprobs` [batch, t, top])."""
+        return head.model_score(self, ids, targets, batch, t, top)
 
     def close(self):
         if getattr(self, "h", None):

@@ -23,7 +23,9 @@
 #include <fcntl.h>
 #include <unistd.h>
 
+#include "../../include/noetic/head.h"
 #include "../../include/noetic_gpu.h"
+#include "nk_head.h"
 #include "nk_kernels.h"
 #include "nk_tc.h"
 
@@ -2191,6 +2193,114 @@ nk_status nk_model_loss(nk_model *model, const uint32_t *ids, const uint32_t *ta
         prefill_device(dec, dec->p_ids, dec->p_lens, lv, t, nullptr, per_chunk);
         launch_ok(dec, nk::ce_mean(d_nll, d_cnt, n, d_loss, dec->stream), "loss mean");
         cuda_check(cudaMemcpyAsync(loss_out, d_loss, sizeof(float), cudaMemcpyDeviceToHost, dec->stream), "download loss");
+        check_err_flag(dec);
+    });
+    nk_decoder_destroy(tmp);
+    return st;
+}
+
+nk_status nk_model_score(nk_model *model, const uint32_t *ids, const uint32_t *targets, uint32_t batch, uint32_t t,
+                         uint32_t top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprobs) {
+    nk_decoder *tmp = nullptr;
+    nk_status st = guard([&] {
+        if (!model || !ids || !targets) fail(NK_ERR_INVALID, "null argument");
+        if (batch == 0 || t == 0) fail(NK_ERR_INVALID, "batch and sequence length must be positive");
+        if (top > NK_MAX_TOP) fail(NK_ERR_INVALID, "score: top is limited to NK_MAX_TOP");
+        if (top == 0 && (top_ids || top_logprobs)) fail(NK_ERR_INVALID, "score: top is 0 and its arrays are not null");
+        const size_t n = (size_t)batch * t;
+        validate_tokens(model, ids, n);
+        const uint64_t V = model->cfg.vocab;
+        if (V >= (1ull << 31)) fail(NK_ERR_UNSUPPORTED, "score: vocabulary too large");
+        for (size_t i = 0; i < n; ++i)
+            if (targets[i] != 0xFFFFFFFFu && targets[i] >= V) fail(NK_ERR_INVALID, "score: target out of range");
+    });
+    if (st != NK_OK) return st;
+    st = nk_decoder_create(model, batch, &tmp);
+    if (st != NK_OK) return st;
+    st = guard([&] {
+        nk_decoder *dec = tmp;
+        nk_model *m = model;
+        const int S = (int)batch, d = (int)m->d();
+        const size_t V = m->cfg.vocab;
+        ensure_ready(dec);
+        std::vector<uint32_t> lv(batch, t);
+        upload_prompts(dec, ids, lv.data(), t);
+        struct Free {
+            std::vector<void *> p;
+            ~Free() {
+                for (void *q : p) cudaFree(q);
+            }
+        } fr;
+        fr.p.reserve(8);
+        // Logits in blocks of at most 512 MiB, their rows' results beside them.
+        const int block_rows = (int)std::max<size_t>(1, std::min<size_t>(((size_t)512 << 20) / (4 * V), 1u << 16));
+        float *d_lg = nullptr, *d_lp = nullptr, *d_en = nullptr, *d_tl = nullptr;
+        uint32_t *d_tg = nullptr, *d_ti = nullptr;
+        auto room = [&](auto **p, size_t count, const char *what) {
+            dalloc(p, count, what);
+            fr.p.push_back(*p);
+        };
+        room(&d_lg, (size_t)block_rows * V, "logits block");
+        room(&d_tg, block_rows, "targets");
+        room(&d_lp, block_rows, "log probabilities");
+        room(&d_en, block_rows, "entropies");
+        room(&d_ti, (size_t)block_rows * std::max(top, 1u), "alternatives");
+        room(&d_tl, (size_t)block_rows * std::max(top, 1u), "alternatives' log probabilities");
+        std::vector<uint32_t> h_tg(block_rows);
+        const nk::TcOperand *w_lg = tc_op(m, 4 * m->cfg.n_layer);
+        auto per_chunk = [&](uint32_t t0, int tcc) {
+            const int R = S * tcc;
+            for (int r0 = 0; r0 < R; r0 += block_rows) {
+                const int rr = std::min(block_rows, R - r0);
+                const bool t_lg = use_tc(dec, rr, (int)V, d, w_lg);
+                const Act nrm{dec->p_n, dec->p_ahi, dec->p_alo};
+                launch_ok(dec, nk::rmsnorm_rows(dec->p_x + (size_t)r0 * d, m->dp(m->norm_f), m->cfg.eps, nrm.out(t_lg),
+                                                rr, d, dec->stream),
+                          "rmsnorm");
+                project(dec, t_lg, nrm, rr, d, m->dp(m->emb), w_lg, (int)V, nullptr, d_lg, nullptr);
+                // Rows of one stream are consecutive positions: one copy per run.
+                auto runs = [&](auto &&f) {
+                    for (int r = 0; r < rr;) {
+                        const int g = r0 + r, s = g / tcc, tt = g - s * tcc;
+                        const int run = std::min(rr - r, tcc - tt);
+                        f((size_t)r, (size_t)s * t + t0 + tt, (size_t)run);
+                        r += run;
+                    }
+                };
+                // The copies below wait for the block, so h_tg is free again here.
+                runs([&](size_t r, size_t pos, size_t run) { std::copy_n(targets + pos, run, h_tg.data() + r); });
+                cuda_check(cudaMemcpyAsync(d_tg, h_tg.data(), rr * sizeof(uint32_t), cudaMemcpyHostToDevice, dec->stream),
+                           "upload targets");
+                nk::LogprobsArgs a{};
+                a.logits = d_lg;
+                a.rows = rr;
+                a.stride = (int64_t)V;
+                a.vocab = (int)V;
+                a.targets = d_tg;
+                a.scale = 1.44269504088896341f;
+                a.inv_t = 1.0f;
+                a.top = (int)top;
+                a.logprob = d_lp;
+                a.entropy = d_en;
+                a.top_ids = d_ti;
+                a.top_logprobs = d_tl;
+                launch_ok(dec, nk::token_logprobs(a, NK_F32, dec->stream), "token log probabilities");
+                auto down = [&](auto *host, const auto *dev, size_t per_row) {
+                    if (!host || per_row == 0) return;
+                    runs([&](size_t r, size_t pos, size_t run) {
+                        cuda_check(cudaMemcpyAsync(host + pos * per_row, dev + r * per_row, run * per_row * 4,
+                                                   cudaMemcpyDeviceToHost, dec->stream),
+                                   "download scores");
+                    });
+                };
+                down(logprob, d_lp, 1);
+                down(entropy, d_en, 1);
+                down(top_ids, d_ti, top);
+                down(top_logprobs, d_tl, top);
+                cuda_check(cudaStreamSynchronize(dec->stream), "score");
+            }
+        };
+        prefill_device(dec, dec->p_ids, dec->p_lens, lv, t, nullptr, per_chunk);
         check_err_flag(dec);
     });
     nk_decoder_destroy(tmp);

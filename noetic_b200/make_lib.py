@@ -3,7 +3,8 @@
 Each ``.cu`` file is compiled with nvcc to an object under
 ``noetic_b200/_build`` (in parallel, skipped when up to date) and the objects
 are linked into one shared library that exports the C ABI declared in
-``include/noetic_gpu.h``.  nvcc cross-compiles for sm_100a without a GPU.
+``include/noetic_gpu.h`` and ``include/noetic/head.h``.  nvcc cross-compiles
+for sm_100a without a GPU.
 """
 
 from __future__ import annotations
@@ -32,6 +33,7 @@ def _sources():
 def _headers():
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh", ".inc"))]
     hs.append(os.path.join(ROOT, "include", "noetic_gpu.h"))
+    hs.append(os.path.join(ROOT, "include", "noetic", "head.h"))
     return hs
 
 
