@@ -26,9 +26,9 @@
  *   - Results do not depend on scheduling: the same call gives the same bits.
  *   - NK_ERR_INVALID: a null array with a non-zero size, a pointer that is not
  *     device memory, a misaligned one, a stride below the width, a size beyond
- *     the limits (rows <= 2^26, vocab < 2^31, width < 2^31, rows * stride <= 2^37), a
- *     temperature that is not finite and positive, an eps that is negative or
- *     not finite.
+ *     the limits (rows <= 2^26, vocab and width <= 2^30, rows * stride <=
+ *     2^37), a temperature outside [1e-30, 1e30], an eps that is negative or not
+ *     finite, an output that overlaps an input other than as said below.
  */
 #ifndef NOETIC_HEAD_H
 #define NOETIC_HEAD_H
@@ -104,7 +104,8 @@ nk_status nk_token_logprobs_backward(const void *logits, int dtype, uint64_t row
  * which is the gradient of grad_scale sum_r row_weight[r] loss[r].  row_weight
  * null: 1.  dlogits null: the loss alone; loss null: the gradient alone.  The
  * logits are read once for both.  A row without entries is not read: its loss
- * and gradient are 0.  A row of weight 0 has gradient 0.  An id may stand in a
+ * and gradient are 0.  A row of weight 0 has gradient 0.  Where the student has
+ * no logit above -infinity the loss is infinity and the gradient 0.  An id may stand in a
  * row more than once (its shares add up).  dlogits has the type of the logits
  * and can be the same array with the same stride. */
 nk_status nk_distill_device(const void *logits, int dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,

@@ -53,6 +53,7 @@ nk_status guard(const char *name, F &&f) {
 }
 
 constexpr uint64_t MAX_ROWS = 1ull << 26;
+constexpr uint64_t MAX_WIDTH = 1ull << 30;
 constexpr uint32_t NO_TOKEN = 0xFFFFFFFFu;
 
 int elem_size(int dtype) { return dtype == NK_F32 ? 4 : 2; }
@@ -61,7 +62,7 @@ void check_dtype(int dtype) { need(dtype == NK_F32 || dtype == NK_F16 || dtype =
 
 void check_matrix(uint64_t rows, uint64_t width, uint64_t stride, const char *what) {
     uint64_t n = 0;
-    if (rows > MAX_ROWS || width >= (1ull << 31)) fail(NK_ERR_INVALID, std::string(what) + ": rows are limited to 2^26, the width to 2^31 - 1");
+    if (rows > MAX_ROWS || width > MAX_WIDTH) fail(NK_ERR_INVALID, std::string(what) + ": rows are limited to 2^26, the width to 2^30");
     if (stride < width) fail(NK_ERR_INVALID, std::string(what) + ": the row stride is below the width");
     if (!nk::checked_mul(rows, stride, n)) fail(NK_ERR_INVALID, std::string(what) + ": rows * stride is limited to 2^37 elements");
 }
@@ -73,7 +74,8 @@ void check_f32(std::initializer_list<const void *> ps) {
     for (const void *p : ps) check_aligned(p, 4, "an f32 or u32 array");
 }
 
-void check_temperature(float t) { need(std::isfinite(t) && t > 0.0f, "temperature must be finite and positive"); }
+// Its reciprocal has to be a normal f32 too.
+void check_temperature(float t) { need(t >= 1e-30f && t <= 1e30f, "temperature must be within [1e-30, 1e30]"); }
 
 // Whether two matrices of `rows` rows share an element without being the same
 // array at the same stride (columns of one wide array are apart).

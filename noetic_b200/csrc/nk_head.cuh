@@ -7,6 +7,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "nk_common.cuh"
 
 namespace nk {
@@ -76,11 +78,127 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// Running softmax sums of one thread: the maximum m of what it has seen, and
-// relative to it s = sum 2^y and t = sum 2^y y with y = (z - m) scale, scale =
-// log2(e) / temperature.  The difference z - m is taken before the product, so
-// a common offset of the logits costs no accuracy.  y is held at -256 in t, where 2^y is 0: masked
-// logits (-infinity, or a type's lowest value) add 0 and not 0 * infinity.
+// ---------------------------------------------------------------- 16-byte vectors
+// A row of n elements is `head` elements up to a 16-byte boundary, n_vec
+// vectors, and `tail` elements, so that any row start gets wide loads.
+template <class T>
+struct Vec {
+    static constexpr int N = 16 / (int)sizeof(T);
+};
+
+struct RowSpan {
+    int head, n_vec, tail;
+};
+template <class T>
+__device__ __forceinline__ RowSpan row_span(const T *row, int n) {
+    const int off = (int)((uintptr_t)row & 15);
+    RowSpan s;
+    s.head = off ? (16 - off) / (int)sizeof(T) : 0;
+    if (s.head > n) s.head = n;
+    s.n_vec = (n - s.head) / Vec<T>::N;
+    s.tail = n - s.head - s.n_vec * Vec<T>::N;
+    return s;
+}
+
+__device__ __forceinline__ uint4 load16(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+// For arrays that the same kernel writes (in place).
+__device__ __forceinline__ uint4 load16_rw(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void store16(void *p, uint4 v) {
+    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+template <class T>
+__device__ __forceinline__ void unpack(uint4 v, float (&x)[Vec<T>::N]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack(const float (&x)[Vec<T>::N]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __float_as_uint(x[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// A vector of -infinity.
+template <class T>
+__device__ __forceinline__ uint4 masked16() {
+    const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+    return make_uint4(w, w, w, w);
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; "
+        "fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// ---------------------------------------------------------------- softmax sums
+// Running softmax sums of one thread: the maximum m of what it has seen (a
+// NaN is passed over), and relative to it s = sum 2^y and t = sum 2^y y with y
+// = (z - m) scale, scale = log2(e) / temperature.  The difference z - m is
+// taken before the product, so a common offset of the logits costs no
+// accuracy.  y is held at -256, where 2^y is 0: masked logits (-infinity, or a
+// type's lowest value) then add 0 to t and not 0 * infinity.  A NaN or
+// +infinity makes s NaN.
 struct SoftSums {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
 
@@ -95,12 +213,63 @@ struct SoftSums {
     }
     // What z is measured from: the maximum, or 0 while there is none.
     __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.0f : m; }
-    __device__ __forceinline__ void add(float z, float base, float scale) {
-        const float y = (z - base) * scale, e = ex2(y);
+    // One logit (the maximum counts it already).
+    __device__ __forceinline__ void add(float z, float scale) {
+        const float y = max_nan((z - base()) * scale, -256.0f), e = ex2(y);
         s += e;
-        t = fmaf(e, fmaxf(y, -256.0f), t);
+        t = fmaf(e, y, t);
     }
 };
+
+// The largest of U vectors' elements; a NaN is passed over.  16-bit types are
+// compared in pairs.
+template <class T, int U>
+__device__ __forceinline__ float batch_max(const uint4 (&raw)[U]) {
+    if constexpr (sizeof(T) == 4) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(raw[u].x), __uint_as_float(raw[u].y)),
+                               fmaxf(__uint_as_float(raw[u].z), __uint_as_float(raw[u].w))));
+        return m;
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        auto as = [](uint32_t w) { return *reinterpret_cast<T2 *>(&w); };
+        T2 m = as(masked16<T>().x);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            m = __hmax2(m, __hmax2(__hmax2(as(raw[u].x), as(raw[u].y)), __hmax2(as(raw[u].z), as(raw[u].w))));
+        return fmaxf(to_f32(m.x), to_f32(m.y));
+    }
+}
+
+// Adds U vectors to a thread's sums; returns their maximum.  Two partial sums
+// each, one of a vector's even elements and one of its odd ones, in pairs of
+// f32 operations.
+template <class T, int U>
+__device__ __forceinline__ float add_batch(const uint4 (&raw)[U], SoftSums &a, float scale) {
+    const float bm = batch_max<T, U>(raw);
+    a.raise(bm, scale);
+    const float base = a.base();
+    const float2 nb = make_float2(-base, -base), sc = make_float2(scale, scale);
+    float2 s = make_float2(0.0f, 0.0f), t = s;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float x[Vec<T>::N];
+        unpack<T>(raw[u], x);
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; i += 2) {
+            float2 y = mul2(add2(make_float2(x[i], x[i + 1]), nb), sc);
+            y = make_float2(max_nan(y.x, -256.0f), max_nan(y.y, -256.0f));
+            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+            s = add2(s, e);
+            t = fma2(e, y, t);
+        }
+    }
+    a.s += s.x + s.y;
+    a.t += t.x + t.y;
+    return bm;
+}
 
 // Every thread's sums joined over the block in a fixed order; all threads get
 // the result.
@@ -108,10 +277,9 @@ __device__ __forceinline__ SoftSums block_join(SoftSums a, float scale, float *r
     SoftSums r;
     r.m = block_max(a.m, red);
     // A thread without a logit above -infinity holds s = 0, or NaN.
-    const float keep_s = a.s, keep_t = a.t;
     if (a.m != -INFINITY) a.raise(r.m, scale);
-    r.s = block_sum(a.m == -INFINITY ? keep_s : a.s, red);
-    r.t = block_sum(a.m == -INFINITY ? keep_t : a.t, red);
+    r.s = block_sum(a.s, red);
+    r.t = block_sum(a.t, red);
     return r;
 }
 

@@ -2210,7 +2210,7 @@ nk_status nk_model_score(nk_model *model, const uint32_t *ids, const uint32_t *t
         const size_t n = (size_t)batch * t;
         validate_tokens(model, ids, n);
         const uint64_t V = model->cfg.vocab;
-        if (V >= (1ull << 31)) fail(NK_ERR_UNSUPPORTED, "score: vocabulary too large");
+        if (V > (1ull << 30)) fail(NK_ERR_UNSUPPORTED, "score: vocabulary too large");
         for (size_t i = 0; i < n; ++i)
             if (targets[i] != 0xFFFFFFFFu && targets[i] >= V) fail(NK_ERR_INVALID, "score: target out of range");
     });

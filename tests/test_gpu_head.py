@@ -162,7 +162,7 @@ def test_logprobs_over_sizes(gpu, torch, dtype, rows, V, pad, shift):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("V", [40, 2048, 40001, 131072])
+@pytest.mark.parametrize("V", [40, 2048, 40001, 131072, 700000])
 def test_logprobs_alternatives_in_awkward_orders(gpu, torch, dtype, V):
     # Sorted rows, constant rows, few values, the largest side by side, zeros
     # of both signs: ties go to the lower id.
@@ -404,6 +404,10 @@ def test_distill_special_rows(gpu, torch):
     assert torch.isnan(loss[2]) and torch.isnan(dz[2]).all()
     assert torch.isnan(loss[4]) and (dz[4] == 0).all()
     assert loss[5] == INF and torch.isfinite(dz[5]).all()
+    # A student that can say nothing: infinity, and no direction to go.
+    z[1] = -INF
+    loss, dz = _distill(gpu, torch, z[1:2], ids[1:2], t[1:2], 1.0, None, 1.0, "f32", "f32")
+    assert loss[0] == INF and (dz == 0).all()
     # A teacher without any places.
     none = torch.empty(6, 0, device="cuda", dtype=torch.int32)
     loss, dz = _distill(gpu, torch, z, none, none.float(), 1.0, w, 1.0, "f32", "f32")
