@@ -493,7 +493,9 @@ def test_norm_over_sizes(gpu, torch, rms, dtype, rows, d, pad, shift):
     tol1 = hh.abs() * (r_rel + 4 * U) + r * (mean_tol + U * xd.abs())
     assert ((plain.double() - hh).abs() <= tol1 + _out_tol(torch, dtype, hh)).all()
     out, around = _matrix(torch, rows, d, dtype, pad + 3, shift + 1)
-    assert torch.equal(_norm(gpu, torch, x, gain, bias, eps, rms, dtype, out)[0], y)
+    # (Rows of another alignment are summed in another order: the same bound, not the same bits.)
+    other = _norm(gpu, torch, x, gain, bias, eps, rms, dtype, out)[0]
+    assert ((other.double() - ref).abs() <= tol + _out_tol(torch, dtype, ref)).all()
     gaps = torch.ones(around.numel(), dtype=torch.bool, device="cuda")
     gaps[shift + 1:shift + 1 + rows * (d + pad + 3)].view(rows, -1)[:, :d] = False
     assert torch.isnan(around[gaps]).all()
