@@ -15,6 +15,7 @@ namespace {
 constexpr int DS_NT = 256;
 constexpr int TEACHER_MAX = 256;  // one entry per thread
 constexpr int DS_U = 4;
+constexpr int DS_DEPTH = 4;
 constexpr int DS_CLUSTER = 8;
 constexpr int DS_PART = 68 << 10;   // bytes of a part: three to an SM
 constexpr int DS_MOST = 216 << 10;  // the most that a CTA keeps
@@ -86,23 +87,31 @@ __global__ void __launch_bounds__(DS_NT) distill_k(DistillArgs a, int cs, int ke
     const float z_my = mine ? to_f32(row[my]) : 0.0f;
 
     SoftSums sums;
-    int batch = 0;
-    for (int v = v0 + tid; v < v1; v += DS_NT * DS_U, ++batch) {
-        uint4 raw[DS_U];
-        if (v + (DS_U - 1) * DS_NT < v1) {
-#pragma unroll
-            for (int u = 0; u < DS_U; ++u) raw[u] = load16_rw(body + (int64_t)(v + u * DS_NT) * N);
-        } else {
+    if (out) {
+        // Groups of DS_U vectors per thread, DS_DEPTH groups on their way.
+        constexpr int STEP = DS_NT * DS_U;
+        auto fetch = [&](int v) {
 #pragma unroll
             for (int u = 0; u < DS_U; ++u)
-                raw[u] = v + u * DS_NT < v1 ? load16_rw(body + (int64_t)(v + u * DS_NT) * N) : masked16<T>();
-        }
-        if (out) {
+                if (v + u * DS_NT < keep && v0 + v + u * DS_NT < v1)
+                    copy_async16(&kept[v + u * DS_NT], body + (int64_t)(v0 + v + u * DS_NT) * N);
+            copy_commit();
+        };
 #pragma unroll
-            for (int u = 0; u < DS_U; ++u)
-                if (v - v0 + u * DS_NT < keep) kept[v - v0 + u * DS_NT] = raw[u];
+        for (int g = 0; g < DS_DEPTH; ++g) fetch(tid + g * STEP);
+        const int n_kept = min(keep, v1 - v0);
+        for (int v = tid; v < n_kept; v += STEP) {
+            copy_wait<DS_DEPTH - 1>();
+            uint4 raw[DS_U];
+#pragma unroll
+            for (int u = 0; u < DS_U; ++u) raw[u] = v + u * DS_NT < n_kept ? kept[v + u * DS_NT] : masked16<T>();
+            fetch(v + DS_DEPTH * STEP);
+            add_batch<T, DS_U>(raw, sums, scale);
         }
-        add_batch<T, DS_U>(raw, sums, scale);
+        copy_wait<0>();
+        if (v0 + keep < v1) stream_sums<T, DS_NT, DS_U>(body, v0 + keep, v1, scale, sums, [](int, float) {});
+    } else {
+        stream_sums<T, DS_NT, DS_U>(body, v0, v1, scale, sums, [](int, float) {});
     }
     float z_head = 0.0f, z_tail = 0.0f;
     if (tid < n_head) {

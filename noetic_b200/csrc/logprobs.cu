@@ -164,24 +164,13 @@ __global__ void __launch_bounds__(LP_NT) token_logprobs_k(LogprobsArgs a, int cs
     const float scale = a.scale;
     SoftSums sums;
     float tmax = -INFINITY, gmax = -INFINITY;
-    int batch = 0;
-    for (int v = v0 + tid; v < v1; v += LP_NT * LP_U, ++batch) {
-        uint4 raw[LP_U];
-        if (v + (LP_U - 1) * LP_NT < v1) {
-#pragma unroll
-            for (int u = 0; u < LP_U; ++u) raw[u] = load16(body + (int64_t)(v + u * LP_NT) * N);
-        } else {
-#pragma unroll
-            for (int u = 0; u < LP_U; ++u)
-                raw[u] = v + u * LP_NT < v1 ? load16(body + (int64_t)(v + u * LP_NT) * N) : masked16<T>();
-        }
-        const float bm = add_batch<T, LP_U>(raw, sums, scale);
+    const int batch = stream_sums<T, LP_NT, LP_U>(body, v0, v1, scale, sums, [&](int b, float bm) {
         if (a.top) {
-            gmax = (batch & ((1 << slot_shift) - 1)) == 0 ? bm : fmaxf(gmax, bm);
-            group_max[(batch >> slot_shift) * LP_NT + tid] = gmax;
+            gmax = (b & ((1 << slot_shift) - 1)) == 0 ? bm : fmaxf(gmax, bm);
+            group_max[(b >> slot_shift) * LP_NT + tid] = gmax;
             tmax = fmaxf(tmax, bm);
         }
-    }
+    });
     // The ends that no vector covers, one element per thread and end.
     auto single = [&](int e) {
         const float z = to_f32(row[e]);

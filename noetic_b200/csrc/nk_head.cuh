@@ -271,6 +271,41 @@ __device__ __forceinline__ float add_batch(const uint4 (&raw)[U], SoftSums &a, f
     return bm;
 }
 
+// Adds the vectors v0 <= v < v1 of `body` to the sums of a block of NT threads,
+// U to a thread at a time, the next U on their way while the present ones are
+// added.  each(batch, maximum) is called for every U.  Returns their number.
+template <class T, int NT, int U, class F>
+__device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, float scale, SoftSums &sums, F &&each) {
+    uint4 next[U];
+    auto fetch = [&](int v) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            next[u] = v + u * NT < v1 ? load16_rw(body + (int64_t)(v + u * NT) * Vec<T>::N) : masked16<T>();
+    };
+    int batch = 0, v = v0 + (int)threadIdx.x;
+    fetch(v);
+    for (; v < v1; ++batch) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = next[u];
+        v += NT * U;
+        fetch(v);
+        each(batch, add_batch<T, U>(raw, sums, scale));
+    }
+    return batch;
+}
+
+// Asynchronous copies to shared memory: 16 bytes, a group of them, and the
+// wait until at most N groups of this thread are still on their way.
+__device__ __forceinline__ void copy_async16(void *to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Every thread's sums joined over the block in a fixed order; all threads get
 // the result.
 __device__ __forceinline__ SoftSums block_join(SoftSums a, float scale, float *red) {

@@ -23,6 +23,8 @@ namespace {
 constexpr int NM_NT = 256;
 constexpr int NM_VALS = 16;
 constexpr int NM_WIDE = 8192;
+constexpr int FWD_DEPTH = 4;  // rows on their way to each group
+constexpr int BWD_DEPTH = 3;
 constexpr int PARTIAL_ROWS = 1024;  // most partial sums of dgain and dbias
 
 // ---------------------------------------------------------------- groups of threads
@@ -124,6 +126,48 @@ struct RowPart {
     }
 };
 
+// The rows that a thread will work on next: with VEC in its own places of a
+// ring in shared memory, DEPTH rows on their way by asynchronous copies (no
+// barrier: a thread reads only what it copied); else one row in registers.
+template <class T, int G, bool VEC, int NT, int DEPTH, int ARRAYS>
+struct RowQueue {
+    using P = Place<T, G, VEC>;
+    static constexpr int BYTES = VEC ? DEPTH * ARRAYS * P::LOADS * NT * 16 : 0;
+    RowPart<T, G, VEC> next[ARRAYS];
+    uint4 *ring;  // [DEPTH][ARRAYS][LOADS][NT]
+    int at = 0;
+
+    __device__ __forceinline__ void push(const T *const (&rows)[ARRAYS], int slot, int lane, int width, bool real) {
+#pragma unroll
+        for (int k = 0; k < ARRAYS; ++k) {
+            if constexpr (VEC) {
+#pragma unroll
+                for (int l = 0; l < P::LOADS; ++l)
+                    if (real && P::at(lane, l) < width)
+                        copy_async16(ring + ((slot * ARRAYS + k) * P::LOADS + l) * NT + threadIdx.x, rows[k] + P::at(lane, l));
+            } else {
+                next[k].load(rows[k], lane, width, real);
+            }
+        }
+        if constexpr (VEC) copy_commit();
+    }
+    // The row pushed DEPTH pushes ago (VEC) or last.
+    __device__ __forceinline__ void front(int k, int lane, int width, bool real, float (&x)[NM_VALS]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int l = 0; l < P::LOADS; ++l) {
+                float v[P::N];
+                unpack<T>(real && P::at(lane, l) < width ? ring[((at * ARRAYS + k) * P::LOADS + l) * NT + threadIdx.x]
+                                                         : make_uint4(0, 0, 0, 0), v);
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) x[l * P::N + i] = v[i];
+            }
+        } else {
+            next[k].get(x);
+        }
+    }
+};
+
 // A thread's part of an f32 vector of the width (null: `other`).
 template <class T, int G, bool VEC>
 __device__ __forceinline__ void column_part(const float *p, float other, int lane, int width, float (&x)[NM_VALS]) {
@@ -138,26 +182,37 @@ __device__ __forceinline__ void column_part(const float *p, float other, int lan
 
 // ---------------------------------------------------------------- forward
 template <class T, int G, bool VEC>
-__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT) norm_rows_k(NormArgs a) {
+__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 3) norm_rows_k(NormArgs a) {
     using P = Place<T, G, VEC>;
     constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
     __shared__ float red[2][32];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_n = 1.0f / (float)a.width;
     float gain[NM_VALS], bias[NM_VALS];
-    RowPart<T, G, VEC> next;
+    extern __shared__ uint4 ring[];
+    RowQueue<T, G, VEC, NT, FWD_DEPTH, 1> queue;
+    queue.ring = ring;
+    constexpr int AHEAD = VEC ? FWD_DEPTH : 1;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-    next.load((const T *)a.x + r * a.x_stride, lane, a.width, r < a.rows);
-    column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
-    column_part<T, G, VEC>(a.bias, 0.0f, lane, a.width, bias);
+    auto push = [&](int64_t q, int slot) {
+        const T *const rows[1] = {(const T *)a.x + q * a.x_stride};
+        queue.push(rows, slot, lane, a.width, q < a.rows);
+    };
+    for (int k = 0; k < AHEAD; ++k) push(r + k * step, k);
+    if constexpr (VEC) {
+        column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
+        column_part<T, G, VEC>(a.bias, 0.0f, lane, a.width, bias);
+    }
     // Every group takes the same number of turns: the reductions hold barriers.
     const int64_t turns = (a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step;
     for (int64_t i = 0; i < turns; ++i, r += step) {
         const bool real = r < a.rows;
         float x[NM_VALS];
-        next.get(x);
-        if (i + 1 < turns) next.load((const T *)a.x + (r + step) * a.x_stride, lane, a.width, r + step < a.rows);
+        if constexpr (VEC) copy_wait<FWD_DEPTH - 1>();
+        queue.front(0, lane, a.width, real, x);
+        push(r + AHEAD * step, queue.at);
+        queue.at = queue.at + 1 == AHEAD ? 0 : queue.at + 1;
         float mean = 0.0f;
         if (!a.rms) {
             float s = 0.0f;
@@ -179,6 +234,10 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT) norm_rows_k(NormArgs a)
         const float rstd = 1.0f / sqrtf(fmaf(group_sum<G>(v, red[1]), inv_n, a.eps));
         if (G > 32 && a.rms) __syncthreads();  // red[1] again in the next turn
         if (!real) continue;
+        if constexpr (!VEC) {  // from L1 for every row: the loads' sixteen registers are taken
+            column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
+            column_part<T, G, VEC>(a.bias, 0.0f, lane, a.width, bias);
+        }
 #pragma unroll
         for (int j = 0; j < NM_VALS; ++j) x[j] = fmaf(x[j] * rstd, gain[j], bias[j]);
         RowPart<T, G, VEC>::store((T *)a.y + r * a.y_stride, lane, a.width, x);
@@ -224,36 +283,45 @@ __global__ void __launch_bounds__(NM_NT) norm_wide_rows_k(NormArgs a) {
 // groups' registers joined in shared memory in their order, then one row of
 // the workspace per block.
 template <class T, int G, bool VEC, bool PARAMS>
-__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT) norm_backward_k(NormGradArgs a) {
+__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_backward_k(NormGradArgs a) {
     using P = Place<T, G, VEC>;
     constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
     __shared__ float2 red[2][32];
-    extern __shared__ float joined[];  // [2][width], with more than one group
+    extern __shared__ uint4 ring[];
+    float *joined = (float *)ring;  // [2][width], when the rows are done
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_n = 1.0f / (float)a.width;
     float gain[NM_VALS], dg[NM_VALS], db[NM_VALS];
 #pragma unroll
     for (int j = 0; j < NM_VALS; ++j) dg[j] = db[j] = 0.0f;
-    RowPart<T, G, VEC> nx, ndy;
+    RowQueue<T, G, VEC, NT, BWD_DEPTH, 2> queue;
+    queue.ring = ring;
+    constexpr int AHEAD = VEC ? BWD_DEPTH : 1;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-    auto fetch = [&](int64_t q, float &m, float &rs) {
-        const bool real = q < a.rows;
-        nx.load((const T *)a.x + q * a.x_stride, lane, a.width, real);
-        ndy.load((const T *)a.dy + q * a.dy_stride, lane, a.width, real);
-        m = real && !a.rms ? a.mean[q] : 0.0f;
-        rs = real ? a.rstd[q] : 0.0f;
+    auto push = [&](int64_t q, int slot) {
+        const T *const rows[2] = {(const T *)a.x + q * a.x_stride, (const T *)a.dy + q * a.dy_stride};
+        queue.push(rows, slot, lane, a.width, q < a.rows);
     };
     float next_mean, next_rstd;
-    fetch(r, next_mean, next_rstd);
-    column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
+    auto stats = [&](int64_t q) {
+        next_mean = q < a.rows && !a.rms ? a.mean[q] : 0.0f;
+        next_rstd = q < a.rows ? a.rstd[q] : 0.0f;
+    };
+    for (int k = 0; k < AHEAD; ++k) push(r + k * step, k);
+    stats(r);
+    if constexpr (VEC) column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
     const int64_t turns = (a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step;
     for (int64_t i = 0; i < turns; ++i, r += step) {
         float h[NM_VALS], c[NM_VALS];
-        nx.get(h);
-        ndy.get(c);
+        if constexpr (VEC) copy_wait<BWD_DEPTH - 1>();
+        queue.front(0, lane, a.width, r < a.rows, h);
+        queue.front(1, lane, a.width, r < a.rows, c);
         const float mean = next_mean, rstd = next_rstd;
-        if (i + 1 < turns) fetch(r + step, next_mean, next_rstd);
+        push(r + AHEAD * step, queue.at);
+        queue.at = queue.at + 1 == AHEAD ? 0 : queue.at + 1;
+        stats(r + step);
+        if constexpr (!VEC) column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < NM_VALS; ++j) {
@@ -278,6 +346,7 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT) norm_backward_k(NormGra
     }
     if constexpr (PARAMS) {
         float *w = a.workspace + (int64_t)blockIdx.x * 2 * a.width;
+        if (GROUPS > 1) __syncthreads();
         for (int g = 0; g < GROUPS; ++g) {
             if (group == g) {
                 float *to = g == GROUPS - 1 ? w : joined;
@@ -365,11 +434,21 @@ int64_t blocks(int64_t rows, int groups, int per_sm) {
     return std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, 148 * per_sm));
 }
 
+template <class Args>
+cudaError_t launch(void (*kern)(Args), const Args &a, int64_t grid, int nt, int smem, cudaStream_t st) {
+    if (smem > 40000) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
+    kern<<<(unsigned)grid, nt, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
 template <class T, int G, bool VEC>
 cudaError_t forward_g(const NormArgs &a, cudaStream_t st) {
     constexpr int NT = G > NM_NT ? G : NM_NT;
-    norm_rows_k<T, G, VEC><<<(unsigned)blocks(a.rows, NT / G, NT > 256 ? 2 : 4), NT, 0, st>>>(a);
-    return cudaGetLastError();
+    constexpr int smem = RowQueue<T, G, VEC, NT, FWD_DEPTH, 1>::BYTES;
+    return launch(norm_rows_k<T, G, VEC>, a, blocks(a.rows, NT / G, NT > NM_NT ? 1 : 3), NT, smem, st);
 }
 template <class T, bool VEC>
 cudaError_t forward_v(const NormArgs &a, cudaStream_t st) {
@@ -396,12 +475,10 @@ template <class T, int G, bool VEC>
 cudaError_t backward_g(const NormGradArgs &a, bool params, int64_t &parts, cudaStream_t st) {
     constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
     parts = blocks(a.rows, GROUPS, NT > 256 ? 1 : 2);
-    const size_t smem = params && GROUPS > 1 ? 2 * (size_t)a.width * sizeof(float) : 0;
-    if (params)
-        norm_backward_k<T, G, VEC, true><<<(unsigned)parts, NT, smem, st>>>(a);
-    else
-        norm_backward_k<T, G, VEC, false><<<(unsigned)parts, NT, 0, st>>>(a);
-    return cudaGetLastError();
+    const int join = params && GROUPS > 1 ? 2 * a.width * (int)sizeof(float) : 0;
+    const int smem = std::max(join, RowQueue<T, G, VEC, NT, BWD_DEPTH, 2>::BYTES);
+    return params ? launch(norm_backward_k<T, G, VEC, true>, a, parts, NT, smem, st)
+                  : launch(norm_backward_k<T, G, VEC, false>, a, parts, NT, smem, st);
 }
 template <class T, bool VEC>
 cudaError_t backward_v(const NormGradArgs &a, bool params, int64_t &parts, cudaStream_t st) {
