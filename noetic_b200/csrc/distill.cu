@@ -12,13 +12,22 @@ namespace nk {
 
 namespace {
 
-constexpr int DS_NT = 256;
-constexpr int TEACHER_MAX = 256;  // one entry per thread
+constexpr int TEACHER_MAX = 256;
 constexpr int DS_U = 4;
-constexpr int DS_DEPTH = 4;
+#ifndef DS_NT_
+#define DS_NT_ 192
+#define DS_PART_ 68
+#define DS_ROWS_ 8
+#define DS_FILL_ 4
+#define DS_MINB_ 3
+#define DS_WVEC_ 1024
+#define DS_WMIN_ 512
+#endif
+constexpr int DS_NT = DS_NT_;
 constexpr int DS_CLUSTER = 8;
-constexpr int DS_PART = 68 << 10;   // bytes of a part: three to an SM
-constexpr int DS_MOST = 216 << 10;  // the most that a CTA keeps
+constexpr int DS_PART = DS_PART_ << 10;  // bytes of a part: three to an SM
+constexpr int DS_MOST = (208 << 10) / (DS_NT * DS_U * 16) * (DS_NT * DS_U * 16);  // the most that a CTA keeps, in whole batches
+constexpr int DS_ROWS = DS_ROWS_;        // rows of a cluster, at most
 
 __device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t i) {
     return dtype == 0   ? ((const float *)p)[i]
@@ -26,204 +35,578 @@ __device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t
                         : to_f32(((const __nv_bfloat16 *)p)[i]);
 }
 
-// One row by a cluster of `cs` CTAs, each with a contiguous part of it that
-// stays in shared memory between the two passes: the logits are read from HBM
-// once, for the softmax sums, and the gradient is made from the copy.  A
-// thread keeps the vectors that it loaded itself, so the copy needs no
-// barrier.  Bound by HBM (one read, one write).
+// Waits until at most n of this thread's groups of copies are on their way
+// (from 8 on: until at most 7 are).
+__device__ __forceinline__ void copy_wait_for(int n) {
+    switch (n) {
+        case 0: copy_wait<0>(); break;
+        case 1: copy_wait<1>(); break;
+        case 2: copy_wait<2>(); break;
+        case 3: copy_wait<3>(); break;
+        case 4: copy_wait<4>(); break;
+        case 5: copy_wait<5>(); break;
+        case 6: copy_wait<6>(); break;
+        default: copy_wait<7>(); break;
+    }
+}
+
+// The entries of one row in the lanes of a warp, lane l with l, l + 32, ...;
+// an entry that does not count has no token.  q holds the teacher's logits, then
+// the shares.  ENTRIES is 2 for teachers of up to 64 entries, else 8: these
+// registers are every warp's.
+template <int ENTRIES>
+struct Entries {
+    uint32_t id[ENTRIES];
+    float q[ENTRIES];
+
+    __device__ __forceinline__ void load(const DistillArgs &a, int64_t r, int lane) {
+#pragma unroll
+        for (int k = 0; k < ENTRIES; ++k) {
+            const int i = k * 32 + lane;
+            id[k] = i < a.n ? a.ids[r * a.n + i] : NO_TOKEN;
+            q[k] = i < a.n ? teacher_value(a.teacher, a.teacher_dtype, r * a.n + i) : -INFINITY;
+        }
+    }
+    // Drops what does not count; whether anything is left.
+    __device__ __forceinline__ bool settle(const DistillArgs &a) {
+        bool any = false;
+#pragma unroll
+        for (int k = 0; k < ENTRIES; ++k) {
+            if (id[k] >= (uint32_t)a.vocab) q[k] = -INFINITY;
+            if (q[k] == -INFINITY) id[k] = NO_TOKEN;
+            any |= id[k] != NO_TOKEN;
+        }
+        return __any_sync(0xffffffffu, any);
+    }
+    // q = softmax(q / temperature); returns the maximum and the logarithm of the sum that log q takes.
+    __device__ __forceinline__ void share(float inv_t, int n, float (&log_q)[ENTRIES]) {
+        float m = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < ENTRIES; ++k) m = fmaxf(m, q[k]);
+        m = warp_max1(m);
+#pragma unroll
+        for (int k = 0; k < ENTRIES; ++k) {
+            log_q[k] = (q[k] - m) * inv_t;
+            q[k] = k * 32 < n && id[k] != NO_TOKEN ? expf(log_q[k]) : 0.0f;
+            s += q[k];
+        }
+        s = warp_sum(s);
+        const float log_s = logf(s), inv_s = 1.0f / s;
+#pragma unroll
+        for (int k = 0; k < ENTRIES; ++k) {
+            log_q[k] -= log_s;
+            q[k] *= inv_s;
+        }
+    }
+};
+
+// Rows by a cluster of CTAs, each with a contiguous part of every row that
+// stays in shared memory between the two passes over it: the logits are read
+// from HBM once, for the softmax sums, and the gradient is made from the copy.
+// A thread keeps the vectors that it copied itself, so the copy needs no
+// barrier; as it takes a vector for the gradient it sends for the same vector
+// of the cluster's next row, so that reads and writes run side by side.
 //
-// The teacher's entries lie one per thread; each CTA answers for the entries
-// whose ids are in its part: their terms of the loss, and their places in the
-// gradient, which it writes after a barrier over the dense gradient's values.
+// What a row costs beside its elements is kept off the NT threads that stream
+// it.  They meet once per row, to join their sums.  A warp of its own sees to
+// the teacher: it reads the next row's entries a row ahead, softmaxes this
+// row's while the logits stream in, exchanges the sums with the cluster's other
+// CTAs, and after the streaming threads have passed (they do not wait for it)
+// puts the gradient's values in the entries' places.  Each CTA answers for the
+// entries in its part.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The streaming threads' mark and the teacher warp's wait for it.
+template <int THREADS>
+__device__ __forceinline__ void mark_arrive() {
+    asm volatile("bar.arrive 1, %0;" ::"n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void mark_wait() {
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
+
+// What the two sides of a CTA share, by a row's or a turn's parity (a turn is a
+// row that is read).
+template <int NT>
+struct DistillShared {
+    float4 warps[2][NT / 32];    // the streaming warps' sums
+    float4 parts[2][DS_CLUSTER]; // the cluster's CTAs'
+    float kl[2][DS_CLUSTER];     // their terms of the loss (rank 0's)
+    float weight[2];
+    int any[2];  // whether the row has entries
+    uint32_t id[TEACHER_MAX];
+    float q[TEACHER_MAX];
+};
+
+// A part of one row.
 template <class T>
-__global__ void __launch_bounds__(DS_NT) distill_k(DistillArgs a, int cs, int keep) {
+struct RowOfPart {
+    const T *row;
+    const uint4 *from;  // the part's first vector
+    int head, v0, n_vec, tail;
+    __device__ __forceinline__ RowOfPart(const DistillArgs &a, int64_t r, int rank, int log_cs) {
+        row = (const T *)a.logits + r * a.stride;
+        const RowSpan span = row_span(row, a.vocab);
+        v0 = (int)((int64_t)span.n_vec * rank >> log_cs);
+        n_vec = (int)((int64_t)span.n_vec * (rank + 1) >> log_cs) - v0;
+        from = (const uint4 *)(row + span.head) + v0;
+        head = span.head;
+        tail = span.tail;
+    }
+};
+
+// The sums of the whole row from a CTA's warps, through the cluster; the
+// teacher warp (`speaks`) carries the exchange.
+template <int NT>
+__device__ __forceinline__ SoftSums row_sums(DistillShared<NT> &sh, int turn, int log_cs, int rank, float scale, bool speaks) {
     namespace cg = cooperative_groups;
-    extern __shared__ uint4 kept[];  // keep vectors
-    __shared__ float red[32], sums_out[2], kl_part[DS_CLUSTER];
-    __shared__ uint32_t id[TEACHER_MAX];
-    __shared__ float q[TEACHER_MAX];
+    const int lane = threadIdx.x & 31, cs = 1 << log_cs;
+    SoftSums sums;
+    if (log_cs == 0 || speaks) sums = join_places(sh.warps[turn & 1], NT / 32, scale);
+    if (log_cs) {
+        if (speaks) {
+            if (lane < cs)
+                *cg::this_cluster().map_shared_rank(&sh.parts[turn & 1][rank], lane) = make_float4(sums.m, sums.s, 0.0f, 0.0f);
+            cluster_arrive();
+        } else {
+            cluster_arrive_relaxed();
+        }
+        cluster_wait();
+        sums = join_places(sh.parts[turn & 1], cs, scale);
+    }
+    return sums;
+}
+
+// What does not fit the part's shared memory, from global memory.
+template <class T, int NT>
+__device__ __noinline__ SoftSums stream_rest(const uint4 *from, int v0, int v1, float scale, SoftSums sums) {
+    stream_sums<T, NT, DS_U, false>((const T *)from, v0, v1, threadIdx.x, scale, sums, [](int, float) {});
+    return sums;
+}
+
+template <class T, int NT, int ENTRIES>
+__global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, int log_cs, int keep, int rows_per) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint4 kept[];  // [keep]
+    __shared__ DistillShared<NT> sh;
+    constexpr int N = Vec<T>::N, STEP = NT * DS_U;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int cs = 1 << log_cs, rank = blockIdx.x & (cs - 1);
+    const int64_t r0 = (int64_t)(blockIdx.x >> log_cs) * rows_per;
+    const int n_rows = (int)min((int64_t)rows_per, a.rows - r0);
+    const float scale = a.scale;
+    int turn = 0;
+    if (log_cs) {  // every CTA has to run before its shared memory is written
+        cluster_arrive_relaxed();
+        cluster_wait();
+    }
+
+    if (tid >= NT) {
+        // ---- the teacher
+        Entries<ENTRIES> now, next;
+        float next_weight = 1.0f;
+        auto read_ahead = [&](int i) {
+            next.load(a, r0 + i, lane);
+            if (a.row_weight) next_weight = a.row_weight[r0 + i];
+        };
+        auto tell = [&](int i) {
+            const bool some = next.settle(a);
+            if (lane == 0) {
+                sh.any[i & 1] = some;
+                sh.weight[i & 1] = next_weight;
+            }
+            return some;
+        };
+        int64_t loss_row = -1;  // whose terms the cluster's next barrier brings
+        auto write_loss = [&](int t) {
+            if (loss_row >= 0 && rank == 0 && lane == 0 && a.loss) {
+                float all = 0.0f;
+                for (int c = 0; c < cs; ++c) all += sh.kl[t & 1][c];
+                a.loss[loss_row] = a.temperature * a.temperature * all;
+            }
+        };
+        read_ahead(0);
+        bool any = tell(0);
+        __syncthreads();
+        for (int i = 0; i < n_rows; ++i) {
+            const int64_t r = r0 + i;
+            const bool more = i + 1 < n_rows, live = any;
+            const float w = next_weight;
+            now = next;
+            if (more) read_ahead(i + 1);
+            float z[ENTRIES], log_q[ENTRIES];
+            uint32_t mine = 0;  // which of this lane's entries are in the part
+            if (live) {
+                const RowOfPart<T> here(a, r, rank, log_cs);
+                const int e0 = rank == 0 ? 0 : here.head + here.v0 * N;
+                const int e1 = rank == cs - 1 ? a.vocab : here.head + (here.v0 + here.n_vec) * N;
+#pragma unroll
+                for (int k = 0; k < ENTRIES; ++k) {
+                    z[k] = 0.0f;
+                    if (now.id[k] != NO_TOKEN && (int)now.id[k] >= e0 && (int)now.id[k] < e1) {
+                        mine |= 1u << k;
+                        z[k] = to_f32(here.row[now.id[k]]);
+                    }
+                }
+                now.share(a.inv_t, a.n, log_q);
+                if (a.dlogits) {
+#pragma unroll
+                    for (int k = 0; k < ENTRIES; ++k)
+                        if (k * 32 + lane < a.n) {
+                            sh.id[k * 32 + lane] = now.id[k];
+                            sh.q[k * 32 + lane] = now.q[k];
+                        }
+                }
+            }
+            any = more && tell(i + 1);
+            __syncthreads();
+            if (!live) {
+                if (rank == 0 && lane == 0 && a.loss) a.loss[r] = 0.0f;
+                continue;
+            }
+            const SoftSums sums = row_sums<NT>(sh, turn, log_cs, rank, scale, true);
+            write_loss(turn - 1);
+            const float log_s = logf(sums.s), log2_s = log_s * LOG2E;
+            const bool empty = sums.m == -INFINITY && sums.s == 0.0f;  // a student that can say nothing
+            float kl = 0.0f;
+#pragma unroll
+            for (int k = 0; k < ENTRIES; ++k)
+                if ((mine >> k & 1) && now.q[k] != 0.0f)
+                    kl += empty ? INFINITY : now.q[k] * (log_q[k] - ((z[k] - sums.m) * a.inv_t - log_s));
+            kl = warp_sum(kl);
+            if (log_cs) {
+                if (lane == 0) cg::this_cluster().map_shared_rank(&sh.kl[turn & 1][0], 0)[rank] = kl;
+            } else if (lane == 0 && a.loss) {
+                a.loss[r] = a.temperature * a.temperature * kl;
+            }
+            loss_row = r;
+            ++turn;
+            if (!a.dlogits || w == 0.0f || empty) continue;
+            // What stands at an entry: p less the shares of its id.
+            const float gs = a.grad_scale * w * a.temperature;
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < ENTRIES; ++k)
+                if (mine >> k & 1) {
+                    float share = 0.0f;
+                    for (int j = 0; j < a.n; ++j) share += sh.id[j] == now.id[k] ? sh.q[j] : 0.0f;
+                    z[k] = gs * (ex2(fmaf(z[k] - sums.m, scale, -log2_s)) - share);
+                }
+            mark_wait<NT + 32>();
+            // (An id that stands here more than once gets the same value each time.)
+            T *out = (T *)a.dlogits + r * a.dstride;
+#pragma unroll
+            for (int k = 0; k < ENTRIES; ++k)
+                if (mine >> k & 1) out[now.id[k]] = from_f32<T>(z[k]);
+        }
+        if (log_cs) {
+            cluster_arrive();
+            cluster_wait();
+            write_loss(turn - 1);
+        }
+        return;
+    }
+
+    // ---- the stream
+    const int groups = (keep + STEP - 1) / STEP;
+    auto fetch = [&](const RowOfPart<T> &p, int g) {  // group g of this thread's vectors
+        const int v = g * STEP + tid, n = min(keep, p.n_vec);
+        const uint4 *from = p.from + v;
+#pragma unroll
+        for (int u = 0; u < DS_U; ++u)
+            if (v + u * NT < n) copy_async16(&kept[v + u * NT], from + u * NT);
+        copy_commit();
+    };
+    auto fetch_all = [&](const RowOfPart<T> &p) {
+        for (int g = 0; g < groups; ++g) fetch(p, g);
+    };
+    RowOfPart<T> part(a, r0, rank, log_cs);
+    __syncthreads();
+    // A row without entries is not read, in no CTA of the cluster.
+    bool any = sh.any[0];
+    if (any) fetch_all(part);
+    for (int i = 0; i < n_rows; ++i) {
+        const int64_t r = r0 + i;
+        const RowOfPart<T> here = part;
+        const bool more = i + 1 < n_rows, live = any;
+        const float w = sh.weight[i & 1];
+        if (more) part = RowOfPart<T>(a, r + 1, rank, log_cs);
+        const int n_kept = min(keep, here.n_vec);
+        const int n_head = rank == 0 ? here.head : 0, n_tail = rank == cs - 1 ? here.tail : 0;
+        const int e_tail = a.vocab - here.tail + tid;
+
+        SoftSums sums;
+        float z_head = 0.0f, z_tail = 0.0f;
+        if (live) {
+            for (int g = 0; g < groups; ++g) {
+                copy_wait_for(groups - 1 - g);
+                const int v = tid + g * STEP;
+                uint4 raw[DS_U];
+#pragma unroll
+                for (int u = 0; u < DS_U; ++u) raw[u] = v + u * NT < n_kept ? kept[v + u * NT] : masked16<T>();
+                add_batch<T, DS_U, false>(raw, sums, scale);
+            }
+            if (n_kept < here.n_vec) sums = stream_rest<T, NT>(here.from, n_kept, here.n_vec, scale, sums);
+            if (tid < n_head) {
+                z_head = to_f32(here.row[tid]);
+                sums.raise(z_head, scale);
+                sums.add(z_head, scale);
+            }
+            if (tid < n_tail) {
+                z_tail = to_f32(here.row[e_tail]);
+                sums.raise(z_tail, scale);
+                sums.add(z_tail, scale);
+            }
+            sums.t = 0.0f;
+            sums = warp_join(sums, scale);
+            if (lane == 0) sh.warps[turn & 1][tid >> 5] = make_float4(sums.m, sums.s, 0.0f, 0.0f);
+        }
+        __syncthreads();
+        any = more && sh.any[(i + 1) & 1];
+        bool nothing = !live || w == 0.0f;
+        if (live) {
+            sums = row_sums<NT>(sh, turn, log_cs, rank, scale, false);
+            ++turn;
+            nothing |= sums.m == -INFINITY && sums.s == 0.0f;
+        }
+        if (!a.dlogits) {
+            if (any) fetch_all(part);
+            continue;
+        }
+        T *out = (T *)a.dlogits + r * a.dstride;
+        uint4 *to = (uint4 *)(out + here.head) + here.v0;  // the part's first vector
+        const bool wide = ((uintptr_t)to & 15) == 0;
+        auto put = [&](int v, float (&x)[N]) {
+            if (wide) {
+                store16(to + v, pack<T>(x));
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) ((T *)(to + v))[k] = from_f32<T>(x[k]);
+            }
+        };
+        if (nothing) {
+            float x[N] = {};
+            for (int v = tid; v < here.n_vec; v += NT) put(v, x);
+            if (tid < n_head) out[tid] = from_f32<T>(0.0f);
+            if (tid < n_tail) out[e_tail] = from_f32<T>(0.0f);
+            if (any) fetch_all(part);
+            continue;
+        }
+        const float gs = a.grad_scale * w * a.temperature, log2_s = logf(sums.s) * LOG2E;
+        const float2 nm = make_float2(-sums.m, -sums.m), sc2 = make_float2(scale, scale), nl = make_float2(-log2_s, -log2_s),
+                     g2 = make_float2(gs, gs);
+        auto dense = [&](float z) { return gs * ex2(fmaf(z - sums.m, scale, -log2_s)); };
+        auto vec = [&](int v, uint4 raw) {
+            float x[N];
+            unpack<T>(raw, x);
+#pragma unroll
+            for (int k = 0; k < N; k += 2) {
+                const float2 y = fma2(add2(make_float2(x[k], x[k + 1]), nm), sc2, nl);
+                const float2 p = mul2(make_float2(ex2(y.x), ex2(y.y)), g2);
+                x[k] = p.x;
+                x[k + 1] = p.y;
+            }
+            put(v, x);
+        };
+        for (int g = 0; g < groups; ++g) {
+            const int v = tid + g * STEP;
+#pragma unroll
+            for (int u = 0; u < DS_U; ++u)
+                if (v + u * NT < n_kept) vec(v + u * NT, kept[v + u * NT]);
+            if (any) fetch(part, g);
+        }
+        for (int v = n_kept + tid; v < here.n_vec; v += NT) vec(v, load16_rw(here.from + v));
+        if (tid < n_head) out[tid] = from_f32<T>(dense(z_head));
+        if (tid < n_tail) out[e_tail] = from_f32<T>(dense(z_tail));
+        mark_arrive<NT + 32>();
+    }
+    if (log_cs) {  // the others' shared memory is written until here
+        cluster_arrive_relaxed();
+        cluster_wait();
+    }
+}
+
+// ---------------------------------------------------------------- short rows: a warp each
+// The same in a warp, without a barrier but its own: 12 rows of 16 KB in the air per SM.
+constexpr int WARP_ROWS = 4;
+
+template <class T, int ENTRIES>
+__global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, int keep) {
+    extern __shared__ uint4 shared[];  // WARP_ROWS of: [keep] vectors, [n] ids, [n] shares
     constexpr int N = Vec<T>::N;
-    const int tid = threadIdx.x;
-    const int64_t r = blockIdx.x / cs;
-    const int rank = blockIdx.x % cs;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = (int64_t)blockIdx.x * WARP_ROWS + warp;
+    if (r >= a.rows) return;
+    uint4 *kept = shared + warp * (keep + (2 * a.n + 3) / 4);
+    uint32_t *id = (uint32_t *)(kept + keep);
+    float *q = (float *)(id + a.n);
     const T *row = (const T *)a.logits + r * a.stride;
-    T *out = a.dlogits ? (T *)a.dlogits + r * a.dstride : nullptr;
     const RowSpan span = row_span(row, a.vocab);
-    const T *body = row + span.head;
+    const uint4 *body = (const uint4 *)(row + span.head);
+    const int n_vec = span.n_vec, e_tail = a.vocab - span.tail + lane;
+    const float scale = a.scale;
+    T *out = a.dlogits ? (T *)a.dlogits + r * a.dstride : nullptr;
     T *obody = out + span.head;
     const bool wide = ((uintptr_t)obody & 15) == 0;
-    const int v0 = (int)((int64_t)span.n_vec * rank / cs), v1 = (int)((int64_t)span.n_vec * (rank + 1) / cs);
-    const int n_head = rank == 0 ? span.head : 0, n_tail = rank == cs - 1 ? span.tail : 0;
-    // The elements of this part.
-    const int e0 = rank == 0 ? 0 : span.head + v0 * N, e1 = rank == cs - 1 ? a.vocab : span.head + v1 * N;
-    const float scale = a.scale;
-
     auto put = [&](int v, float (&x)[N]) {
+        T *to = obody + (int64_t)v * N;
         if (wide) {
-            store16(obody + (int64_t)v * N, pack<T>(x));
+            store16(to, pack<T>(x));
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) obody[(int64_t)v * N + i] = from_f32<T>(x[i]);
+            for (int i = 0; i < N; ++i) to[i] = from_f32<T>(x[i]);
         }
     };
     auto zeros = [&] {
         float x[N] = {};
-        for (int v = v0 + tid; v < v1; v += DS_NT) put(v, x);
-        if (tid < n_head) out[tid] = from_f32<T>(0.0f);
-        if (tid < n_tail) out[a.vocab - span.tail + tid] = from_f32<T>(0.0f);
+        for (int v = lane; v < n_vec; v += 32) put(v, x);
+        if (lane < span.head) out[lane] = from_f32<T>(0.0f);
+        if (lane < span.tail) out[e_tail] = from_f32<T>(0.0f);
     };
 
-    // The teacher's entry of this thread: q = softmax(teacher / temperature).
-    const uint32_t my = tid < a.n ? a.ids[r * a.n + tid] : NO_TOKEN;
-    const float t = my < (uint32_t)a.vocab ? teacher_value(a.teacher, a.teacher_dtype, r * a.n + tid) : -INFINITY;
+    Entries<ENTRIES> now;
+    now.load(a, r, lane);
+    const bool any = now.settle(a);
     const float w = a.row_weight ? a.row_weight[r] : 1.0f;
-    const bool live = t != -INFINITY;
-    if (!__syncthreads_or(live)) {  // no entries: the row is not read, in no CTA of the cluster
-        if (rank == 0 && tid == 0 && a.loss) a.loss[r] = 0.0f;
+    if (!any) {
+        if (lane == 0 && a.loss) a.loss[r] = 0.0f;
         if (out) zeros();
         return;
     }
-    const bool mine = live && (int)my >= e0 && (int)my < e1;
-    const float z_my = mine ? to_f32(row[my]) : 0.0f;
-
+    float z_entry[ENTRIES];
+    auto entry_logits = [&] {
+#pragma unroll
+        for (int k = 0; k < ENTRIES; ++k) z_entry[k] = now.id[k] != NO_TOKEN ? to_f32(row[now.id[k]]) : 0.0f;
+    };
     SoftSums sums;
     if (out) {
-        // Groups of DS_U vectors per thread, DS_DEPTH groups on their way.
-        constexpr int STEP = DS_NT * DS_U;
-        auto fetch = [&](int v) {
+        const int half = n_vec / (64 * DS_U) * (32 * DS_U);  // in two groups, of whole batches
+        for (int v = lane; v < half; v += 32) copy_async16(&kept[v], body + v);
+        copy_commit();
+        for (int v = half + lane; v < n_vec; v += 32) copy_async16(&kept[v], body + v);
+        copy_commit();
+        entry_logits();
+        auto add = [&](int from, int to) {
+            for (int v = from + lane; v < to; v += 32 * DS_U) {
+                uint4 raw[DS_U];
 #pragma unroll
-            for (int u = 0; u < DS_U; ++u)
-                if (v + u * DS_NT < keep && v0 + v + u * DS_NT < v1)
-                    copy_async16(&kept[v + u * DS_NT], body + (int64_t)(v0 + v + u * DS_NT) * N);
-            copy_commit();
+                for (int u = 0; u < DS_U; ++u)
+                    if (v + u * 32 < to) raw[u] = kept[v + u * 32];
+                if (v + (DS_U - 1) * 32 < to)
+                    add_batch<T, DS_U, false>(raw, sums, scale);
+                else
+                    add_some<T, 32, DS_U, false>(raw, v, to, sums, scale);
+            }
         };
-#pragma unroll
-        for (int g = 0; g < DS_DEPTH; ++g) fetch(tid + g * STEP);
-        const int n_kept = min(keep, v1 - v0);
-        for (int v = tid; v < n_kept; v += STEP) {
-            copy_wait<DS_DEPTH - 1>();
-            uint4 raw[DS_U];
-#pragma unroll
-            for (int u = 0; u < DS_U; ++u) raw[u] = v + u * DS_NT < n_kept ? kept[v + u * DS_NT] : masked16<T>();
-            fetch(v + DS_DEPTH * STEP);
-            add_batch<T, DS_U>(raw, sums, scale);
-        }
+        copy_wait<1>();
+        add(0, half);
         copy_wait<0>();
-        if (v0 + keep < v1) stream_sums<T, DS_NT, DS_U>(body, v0 + keep, v1, scale, sums, [](int, float) {});
+        add(half, n_vec);
     } else {
-        stream_sums<T, DS_NT, DS_U>(body, v0, v1, scale, sums, [](int, float) {});
+        entry_logits();
+        stream_sums<T, 32, DS_U, false>(row + span.head, 0, n_vec, lane, scale, sums, [](int, float) {});
     }
     float z_head = 0.0f, z_tail = 0.0f;
-    if (tid < n_head) {
-        z_head = to_f32(row[tid]);
+    if (lane < span.head) {
+        z_head = to_f32(row[lane]);
         sums.raise(z_head, scale);
         sums.add(z_head, scale);
     }
-    if (tid < n_tail) {
-        z_tail = to_f32(row[a.vocab - span.tail + tid]);
+    if (lane < span.tail) {
+        z_tail = to_f32(row[e_tail]);
         sums.raise(z_tail, scale);
         sums.add(z_tail, scale);
     }
-
-    const float tm = block_max(t, red);
-    const float ty = (t - tm) * a.inv_t;
-    const float te = live ? expf(ty) : 0.0f;
-    const float ts = block_sum(te, red);
-    const float my_q = te / ts;
-    if (tid < a.n) {
-        id[tid] = live ? my : NO_TOKEN;
-        q[tid] = my_q;
-    }
-    sums = block_join(sums, scale, red);
-    if (cs > 1) {
-        cg::cluster_group cluster = cg::this_cluster();
-        if (tid == 0) {
-            sums_out[0] = sums.m;
-            sums_out[1] = sums.s;
-        }
-        cluster.sync();
-        // The parts in their order, the same in every CTA.
-        SoftSums all;
-        for (int c = 0; c < cs; ++c) all.m = fmaxf(all.m, cluster.map_shared_rank(sums_out, c)[0]);
-        for (int c = 0; c < cs; ++c) {
-            SoftSums part;
-            part.m = cluster.map_shared_rank(sums_out, c)[0];
-            part.s = cluster.map_shared_rank(sums_out, c)[1];
-            if (part.m != -INFINITY) part.raise(all.m, scale);
-            all.s += part.s;
-        }
-        sums = all;
-    }
-    const float log_s = logf(sums.s);
-    const bool empty = sums.m == -INFINITY && sums.s == 0.0f;  // a student that can say nothing
-    float part = 0.0f;
-    if (mine && my_q != 0.0f)
-        part = empty ? INFINITY : my_q * ((ty - logf(ts)) - ((z_my - sums.m) * a.inv_t - log_s));
-    const float kl = block_sum(part, red);
-    if (cs > 1) {
-        cg::cluster_group cluster = cg::this_cluster();
-        if (tid == 0) cluster.map_shared_rank(kl_part, 0)[rank] = kl;
-        cluster.barrier_arrive();
-    }
-
-    if (out && (w == 0.0f || empty)) {
-        zeros();
-    } else if (out) {
-        const float g = a.grad_scale * w * a.temperature, log2_s = log_s * LOG2E;
-        auto grad = [&](float z) { return g * ex2(fmaf(z - sums.m, scale, -log2_s)); };
-        for (int v = v0 + tid; v < v1; v += DS_NT) {
-            float x[N];
-            unpack<T>(v - v0 < keep ? kept[v - v0] : load16_rw(body + (int64_t)v * N), x);
+    sums.t = 0.0f;
+    const SoftSums all = warp_join(sums, scale);
+    const float log_s = logf(all.s), log2_s = log_s * LOG2E;
+    const bool empty = all.m == -INFINITY && all.s == 0.0f;  // a student that can say nothing
+    float log_q[ENTRIES], kl = 0.0f;
+    now.share(a.inv_t, a.n, log_q);
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = grad(x[i]);
-            put(v, x);
+    for (int k = 0; k < ENTRIES; ++k)
+        if (now.id[k] != NO_TOKEN && now.q[k] != 0.0f)
+            kl += empty ? INFINITY : now.q[k] * (log_q[k] - ((z_entry[k] - all.m) * a.inv_t - log_s));
+    kl = warp_sum(kl);
+    if (lane == 0 && a.loss) a.loss[r] = a.temperature * a.temperature * kl;
+    if (!out) return;
+    if (w == 0.0f || empty) {
+        zeros();
+        return;
+    }
+    const float gs = a.grad_scale * w * a.temperature;
+    auto dense = [&](float z) { return gs * ex2(fmaf(z - all.m, scale, -log2_s)); };
+    const float2 nm = make_float2(-all.m, -all.m), sc2 = make_float2(scale, scale), nl = make_float2(-log2_s, -log2_s),
+                 g2 = make_float2(gs, gs);
+#pragma unroll
+    for (int k = 0; k < ENTRIES; ++k)
+        if (k * 32 + lane < a.n) {
+            id[k * 32 + lane] = now.id[k];
+            q[k * 32 + lane] = now.q[k];
         }
-        if (tid < n_head) out[tid] = from_f32<T>(grad(z_head));
-        if (tid < n_tail) out[a.vocab - span.tail + tid] = from_f32<T>(grad(z_tail));
-        __syncthreads();
-        // The entries' own places, from the first of each id.
-        if (mine) {
+    __syncwarp();
+    for (int v = lane; v < n_vec; v += 32) {
+        float x[N];
+        unpack<T>(kept[v], x);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 y = fma2(add2(make_float2(x[i], x[i + 1]), nm), sc2, nl);
+            const float2 p = mul2(make_float2(ex2(y.x), ex2(y.y)), g2);
+            x[i] = p.x;
+            x[i + 1] = p.y;
+        }
+        put(v, x);
+    }
+    if (lane < span.head) out[lane] = from_f32<T>(dense(z_head));
+    if (lane < span.tail) out[e_tail] = from_f32<T>(dense(z_tail));
+    __syncwarp();
+    // What stands at an entry: p less the shares of its id.  (An id that stands
+    // here more than once gets the same value each time.)
+#pragma unroll
+    for (int k = 0; k < ENTRIES; ++k)
+        if (now.id[k] != NO_TOKEN) {
             float share = 0.0f;
-            bool first = true;
-            for (int i = 0; i < a.n; ++i)
-                if (id[i] == my) {
-                    share += q[i];
-                    first = first && i >= tid;
-                }
-            if (first) out[my] = from_f32<T>(g * (ex2(fmaf(z_my - sums.m, scale, -log2_s)) - share));
+            for (int j = 0; j < a.n; ++j) share += id[j] == now.id[k] ? q[j] : 0.0f;
+            out[now.id[k]] = from_f32<T>(gs * (ex2(fmaf(z_entry[k] - all.m, scale, -log2_s)) - share));
         }
-    }
-    if (cs > 1) {
-        cg::this_cluster().barrier_wait();
-        if (rank == 0 && tid == 0 && a.loss) {
-            float all = 0.0f;
-            for (int c = 0; c < cs; ++c) all += kl_part[c];
-            a.loss[r] = a.temperature * a.temperature * all;
-        }
-    } else if (tid == 0 && a.loss) {
-        a.loss[r] = a.temperature * a.temperature * kl;
-    }
 }
 
 template <class T>
 cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
     const int64_t n_vec = a.vocab / N;
+    if (n_vec <= DS_WVEC_ && a.rows >= DS_WMIN_) {
+        const int keep = a.dlogits ? (int)n_vec : 0;
+        const int smem = WARP_ROWS * (keep + (2 * a.n + 3) / 4) * 16;
+        auto kern = a.n <= 64 ? distill_warp_k<T, 2> : distill_warp_k<T, TEACHER_MAX / 32>;
+        if (smem > 48 << 10) {
+            cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e != cudaSuccess) return e;
+        }
+        kern<<<(unsigned)((a.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, smem, st>>>(a, keep);
+        return cudaGetLastError();
+    }
     // A row is split until a part and those of two more CTAs fit an SM's shared
-    // memory, and while the rows alone do not fill the GPU and every thread keeps a vector.
-    int cs = 1;
-    while (cs < DS_CLUSTER && ((a.dlogits && (n_vec + cs - 1) / cs * 16 > DS_PART) ||
-                               (a.rows * cs < 148 * 2 && n_vec / (2 * cs) >= DS_NT)))
-        cs *= 2;
+    // memory, and while the rows alone leave SMs idle and every thread keeps a vector.
+    int log_cs = 0;
+    while ((1 << log_cs) < DS_CLUSTER && ((a.dlogits && (n_vec >> log_cs) * 16 > DS_PART) ||
+                                          (a.rows << log_cs < 148 && n_vec >> (log_cs + 1) >= DS_NT)))
+        ++log_cs;
+    const int cs = 1 << log_cs;
     const int64_t keep = a.dlogits ? std::min<int64_t>((n_vec + cs - 1) / cs, DS_MOST / 16) : 0;
-    auto kern = distill_k<T>;
+    // Several rows to a cluster, as long as there are some turns of clusters left to even out.
+    const int64_t rows_per = std::max<int64_t>(1, std::min<int64_t>(DS_ROWS, a.rows * cs / (148 * 3 * DS_FILL_)));
+    const int64_t clusters = (a.rows + rows_per - 1) / rows_per;
+    auto kern = a.n <= 64 ? distill_k<T, DS_NT, 2> : distill_k<T, DS_NT, TEACHER_MAX / 32>;
     if (keep * 16 > 32768) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DS_MOST);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.rows * cs));
-    cfg.blockDim = dim3(DS_NT);
+    cfg.gridDim = dim3((unsigned)(clusters * cs));
+    cfg.blockDim = dim3(DS_NT + 32);
     cfg.dynamicSmemBytes = (size_t)keep * 16;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -232,7 +615,7 @@ cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cs > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, a, cs, (int)keep);
+    return cudaLaunchKernelEx(&cfg, kern, a, log_cs, (int)keep, (int)rows_per);
 }
 
 }  // namespace

@@ -161,28 +161,9 @@ __device__ __forceinline__ uint4 masked16() {
 }
 
 // Two f32 operations in one instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; "
-        "fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
 // Maximum that keeps a NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -243,10 +224,10 @@ __device__ __forceinline__ float batch_max(const uint4 (&raw)[U]) {
     }
 }
 
-// Adds U vectors to a thread's sums; returns their maximum.  Two partial sums
-// each, one of a vector's even elements and one of its odd ones, in pairs of
-// f32 operations.
-template <class T, int U>
+// Adds U vectors to a thread's sums (t only with ENT); returns their maximum.
+// Two partial sums each, one of a vector's even elements and one of its odd
+// ones, in pairs of f32 operations.
+template <class T, int U, bool ENT>
 __device__ __forceinline__ float add_batch(const uint4 (&raw)[U], SoftSums &a, float scale) {
     const float bm = batch_max<T, U>(raw);
     a.raise(bm, scale);
@@ -260,37 +241,58 @@ __device__ __forceinline__ float add_batch(const uint4 (&raw)[U], SoftSums &a, f
 #pragma unroll
         for (int i = 0; i < Vec<T>::N; i += 2) {
             float2 y = mul2(add2(make_float2(x[i], x[i + 1]), nb), sc);
-            y = make_float2(max_nan(y.x, -256.0f), max_nan(y.y, -256.0f));
+            if (ENT) y = make_float2(max_nan(y.x, -256.0f), max_nan(y.y, -256.0f));
             const float2 e = make_float2(ex2(y.x), ex2(y.y));
             s = add2(s, e);
-            t = fma2(e, y, t);
+            if (ENT) t = fma2(e, y, t);
         }
     }
     a.s += s.x + s.y;
-    a.t += t.x + t.y;
+    if (ENT) a.t += t.x + t.y;
+    return bm;
+}
+// The same for those of U vectors that lie at v, v + NT, ... below v1.
+template <class T, int NT, int U, bool ENT>
+__device__ __forceinline__ float add_some(const uint4 (&raw)[U], int v, int v1, SoftSums &a, float scale) {
+    float bm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (v + u * NT < v1) {
+            const uint4 one[1] = {raw[u]};
+            bm = fmaxf(bm, add_batch<T, 1, ENT>(one, a, scale));
+        }
     return bm;
 }
 
-// Adds the vectors v0 <= v < v1 of `body` to the sums of a block of NT threads,
-// U to a thread at a time, the next U on their way while the present ones are
-// added.  each(batch, maximum) is called for every U.  Returns their number.
-template <class T, int NT, int U, class F>
-__device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, float scale, SoftSums &sums, F &&each) {
+// Adds the vectors v0 <= v < v1 of `body` to the sums of a team of NT threads,
+// of which this is thread `tid`, U to a thread at a time, the next U on their
+// way while the present ones are added.  each(batch, maximum) is called for
+// every U.  Returns the number of these.
+template <class T, int NT, int U, bool ENT, class F>
+__device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int tid, float scale, SoftSums &sums, F &&each) {
     uint4 next[U];
-    auto fetch = [&](int v) {
+    int batch = 0, v = v0 + tid;
+    const uint4 *at = (const uint4 *)body + v;
+    auto fetch = [&] {
+        if (v + (U - 1) * NT < v1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            next[u] = v + u * NT < v1 ? load16_rw(body + (int64_t)(v + u * NT) * Vec<T>::N) : masked16<T>();
+            for (int u = 0; u < U; ++u) next[u] = load16_rw(at + u * NT);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (v + u * NT < v1) next[u] = load16_rw(at + u * NT);
+        }
+        at += U * NT;
     };
-    int batch = 0, v = v0 + (int)threadIdx.x;
-    fetch(v);
+    fetch();
     for (; v < v1; ++batch) {
         uint4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) raw[u] = next[u];
+        const int now = v;
         v += NT * U;
-        fetch(v);
-        each(batch, add_batch<T, U>(raw, sums, scale));
+        fetch();
+        each(batch, now + (U - 1) * NT < v1 ? add_batch<T, U, ENT>(raw, sums, scale) : add_some<T, NT, U, ENT>(raw, now, v1, sums, scale));
     }
     return batch;
 }
@@ -306,16 +308,45 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Every thread's sums joined over the block in a fixed order; all threads get
-// the result.
-__device__ __forceinline__ SoftSums block_join(SoftSums a, float scale, float *red) {
+// The largest of a warp's values; a NaN is passed over.
+__device__ __forceinline__ float warp_max1(float v) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// A warp's sums joined, in all its lanes.
+__device__ __forceinline__ SoftSums warp_join(SoftSums a, float scale) {
     SoftSums r;
-    r.m = block_max(a.m, red);
+    r.m = warp_max1(a.m);
     // A thread without a logit above -infinity holds s = 0, or NaN.
     if (a.m != -INFINITY) a.raise(r.m, scale);
-    r.s = block_sum(a.s, red);
-    r.t = block_sum(a.t, red);
+    r.s = warp_sum(a.s);
+    r.t = warp_sum(a.t);
     return r;
+}
+
+// The parts that n <= 32 places hold, joined in a fixed order in every lane of a warp.
+__device__ __forceinline__ SoftSums join_places(const float4 *places, int n, float scale) {
+    SoftSums a;
+    const int lane = threadIdx.x & 31;
+    if (lane < n) {
+        const float4 p = places[lane];
+        a.m = p.x;
+        a.s = p.y;
+        a.t = p.z;
+    }
+    return warp_join(a, scale);
+}
+
+// Every thread's sums joined over a block of NT with one barrier; all threads
+// get the result.  `places` holds a float4 per warp and must not be in use.
+template <int NT>
+__device__ __forceinline__ SoftSums block_join(const SoftSums &a, float scale, float4 *places) {
+    const SoftSums w = warp_join(a, scale);
+    if ((threadIdx.x & 31) == 0) places[threadIdx.x >> 5] = make_float4(w.m, w.s, w.t, 0.0f);
+    __syncthreads();
+    return join_places(places, NT / 32, scale);
 }
 
 }  // namespace nk
