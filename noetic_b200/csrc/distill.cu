@@ -17,7 +17,7 @@ constexpr int DS_U = 4;
 #ifndef DS_NT_
 #define DS_NT_ 192
 #define DS_PART_ 68
-#define DS_ROWS_ 8
+#define DS_ROWS_ 4
 #define DS_FILL_ 4
 #define DS_MINB_ 3
 #define DS_WVEC_ 1024
@@ -25,6 +25,7 @@ constexpr int DS_U = 4;
 #endif
 constexpr int DS_NT = DS_NT_;
 constexpr int DS_CLUSTER = 8;
+constexpr int DUP_BITS = 16384, WARP_DUP_BITS = 8192;
 constexpr int DS_PART = DS_PART_ << 10;  // bytes of a part: three to an SM
 constexpr int DS_MOST = (208 << 10) / (DS_NT * DS_U * 16) * (DS_NT * DS_U * 16);  // the most that a CTA keeps, in whole batches
 constexpr int DS_ROWS = DS_ROWS_;        // rows of a cluster, at most
@@ -100,6 +101,47 @@ struct Entries {
     }
 };
 
+// Whether two of a warp's entries have the same id, by a bitmap of DUP_BITS bits
+// in shared memory that is clear before and after; ids that far apart may pass
+// for the same one.  Walking all pairs costs a row more than its other teacher
+// work together, and ids are nearly always distinct.
+template <int DUP_BITS, int ENTRIES>
+__device__ __forceinline__ bool perhaps_twice(const uint32_t (&id)[ENTRIES], uint32_t *bits) {
+    bool twice = false;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < ENTRIES; ++k)
+        if (id[k] != NO_TOKEN) {
+            const uint32_t at = id[k] & (DUP_BITS - 1), bit = 1u << (at & 31);
+            twice |= atomicOr(&bits[at >> 5], bit) & bit;
+        }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < ENTRIES; ++k)
+        if (id[k] != NO_TOKEN) bits[(id[k] & (DUP_BITS - 1)) >> 5] = 0;
+    return __any_sync(0xffffffffu, twice);
+}
+
+// The shares of this lane's ids, over all entries that have them.
+template <int ENTRIES>
+__device__ __forceinline__ void total_shares(const Entries<ENTRIES> &e, int n, uint32_t *id, float *q, float (&share)[ENTRIES]) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < ENTRIES; ++k)
+        if (k * 32 + lane < n) {
+            id[k * 32 + lane] = e.id[k];
+            q[k * 32 + lane] = e.q[k];
+        }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < ENTRIES; ++k) {
+        share[k] = 0.0f;
+        for (int j = 0; j < n; ++j) share[k] += id[j] == e.id[k] ? q[j] : 0.0f;
+    }
+    __syncwarp();
+}
+
 // Rows by a cluster of CTAs, each with a contiguous part of every row that
 // stays in shared memory between the two passes over it: the logits are read
 // from HBM once, for the softmax sums, and the gradient is made from the copy.
@@ -136,7 +178,7 @@ struct DistillShared {
     float kl[2][DS_CLUSTER];     // their terms of the loss (rank 0's)
     float weight[2];
     int any[2];  // whether the row has entries
-    uint32_t id[TEACHER_MAX];
+    uint32_t id[TEACHER_MAX], bits[DUP_BITS / 32];
     float q[TEACHER_MAX];
 };
 
@@ -149,8 +191,9 @@ struct RowOfPart {
     __device__ __forceinline__ RowOfPart(const DistillArgs &a, int64_t r, int rank, int log_cs) {
         row = (const T *)a.logits + r * a.stride;
         const RowSpan span = row_span(row, a.vocab);
-        v0 = (int)((int64_t)span.n_vec * rank >> log_cs);
-        n_vec = (int)((int64_t)span.n_vec * (rank + 1) >> log_cs) - v0;
+        // (At most 2^28 vectors times 8.)
+        v0 = (int)((uint32_t)span.n_vec * (uint32_t)rank >> log_cs);
+        n_vec = (int)((uint32_t)span.n_vec * (uint32_t)(rank + 1) >> log_cs) - v0;
         from = (const uint4 *)(row + span.head) + v0;
         head = span.head;
         tail = span.tail;
@@ -158,13 +201,14 @@ struct RowOfPart {
 };
 
 // The sums of the whole row from a CTA's warps, through the cluster; the
-// teacher warp (`speaks`) carries the exchange.
-template <int NT>
-__device__ __forceinline__ SoftSums row_sums(DistillShared<NT> &sh, int turn, int log_cs, int rank, float scale, bool speaks) {
+// teacher warp (`speaks`) carries the exchange, and does `meanwhile` while it waits.
+template <int NT, class F>
+__device__ __forceinline__ SoftSums row_sums(DistillShared<NT> &sh, int turn, int log_cs, int rank, float scale, bool speaks,
+                                             F &&meanwhile) {
     namespace cg = cooperative_groups;
     const int lane = threadIdx.x & 31, cs = 1 << log_cs;
     SoftSums sums;
-    if (log_cs == 0 || speaks) sums = join_places(sh.warps[turn & 1], NT / 32, scale);
+    if (log_cs == 0 || speaks) sums = join_places<false>(sh.warps[turn & 1], NT / 32, scale);
     if (log_cs) {
         if (speaks) {
             if (lane < cs)
@@ -173,8 +217,11 @@ __device__ __forceinline__ SoftSums row_sums(DistillShared<NT> &sh, int turn, in
         } else {
             cluster_arrive_relaxed();
         }
+        meanwhile();
         cluster_wait();
-        sums = join_places(sh.parts[turn & 1], cs, scale);
+        sums = join_places<false>(sh.parts[turn & 1], cs, scale);
+    } else {
+        meanwhile();
     }
     return sums;
 }
@@ -182,7 +229,7 @@ __device__ __forceinline__ SoftSums row_sums(DistillShared<NT> &sh, int turn, in
 // What does not fit the part's shared memory, from global memory.
 template <class T, int NT>
 __device__ __noinline__ SoftSums stream_rest(const uint4 *from, int v0, int v1, float scale, SoftSums sums) {
-    stream_sums<T, NT, DS_U, false>((const T *)from, v0, v1, threadIdx.x, scale, sums, [](int, float) {});
+    stream_sums<T, NT, DS_U, false, true>((const T *)from, v0, v1, threadIdx.x, scale, sums, [](int, float) {});
     return sums;
 }
 
@@ -227,6 +274,7 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
                 a.loss[loss_row] = a.temperature * a.temperature * all;
             }
         };
+        for (int i = lane; i < DUP_BITS / 32; i += 32) sh.bits[i] = 0;
         read_ahead(0);
         bool any = tell(0);
         __syncthreads();
@@ -250,15 +298,6 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
                         z[k] = to_f32(here.row[now.id[k]]);
                     }
                 }
-                now.share(a.inv_t, a.n, log_q);
-                if (a.dlogits) {
-#pragma unroll
-                    for (int k = 0; k < ENTRIES; ++k)
-                        if (k * 32 + lane < a.n) {
-                            sh.id[k * 32 + lane] = now.id[k];
-                            sh.q[k * 32 + lane] = now.q[k];
-                        }
-                }
             }
             any = more && tell(i + 1);
             __syncthreads();
@@ -266,7 +305,7 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
                 if (rank == 0 && lane == 0 && a.loss) a.loss[r] = 0.0f;
                 continue;
             }
-            const SoftSums sums = row_sums<NT>(sh, turn, log_cs, rank, scale, true);
+            const SoftSums sums = row_sums<NT>(sh, turn, log_cs, rank, scale, true, [&] { now.share(a.inv_t, a.n, log_q); });
             write_loss(turn - 1);
             const float log_s = logf(sums.s), log2_s = log_s * LOG2E;
             const bool empty = sums.m == -INFINITY && sums.s == 0.0f;  // a student that can say nothing
@@ -286,14 +325,13 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
             if (!a.dlogits || w == 0.0f || empty) continue;
             // What stands at an entry: p less the shares of its id.
             const float gs = a.grad_scale * w * a.temperature;
-            __syncwarp();
+            float share[ENTRIES];
+#pragma unroll
+            for (int k = 0; k < ENTRIES; ++k) share[k] = now.q[k];
+            if (perhaps_twice<DUP_BITS>(now.id, sh.bits)) total_shares(now, a.n, sh.id, sh.q, share);
 #pragma unroll
             for (int k = 0; k < ENTRIES; ++k)
-                if (mine >> k & 1) {
-                    float share = 0.0f;
-                    for (int j = 0; j < a.n; ++j) share += sh.id[j] == now.id[k] ? sh.q[j] : 0.0f;
-                    z[k] = gs * (ex2(fmaf(z[k] - sums.m, scale, -log2_s)) - share);
-                }
+                if (mine >> k & 1) z[k] = gs * (ex2(fmaf(z[k] - sums.m, scale, -log2_s)) - share[k]);
             mark_wait<NT + 32>();
             // (An id that stands here more than once gets the same value each time.)
             T *out = (T *)a.dlogits + r * a.dstride;
@@ -314,9 +352,15 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
     auto fetch = [&](const RowOfPart<T> &p, int g) {  // group g of this thread's vectors
         const int v = g * STEP + tid, n = min(keep, p.n_vec);
         const uint4 *from = p.from + v;
+        uint4 *to = kept + v;
+        if ((g + 1) * STEP <= n) {
 #pragma unroll
-        for (int u = 0; u < DS_U; ++u)
-            if (v + u * NT < n) copy_async16(&kept[v + u * NT], from + u * NT);
+            for (int u = 0; u < DS_U; ++u) copy_async16(to + u * NT, from + u * NT);
+        } else {
+#pragma unroll
+            for (int u = 0; u < DS_U; ++u)
+                if (v + u * NT < n) copy_async16(to + u * NT, from + u * NT);
+        }
         copy_commit();
     };
     auto fetch_all = [&](const RowOfPart<T> &p) {
@@ -344,8 +388,13 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
                 copy_wait_for(groups - 1 - g);
                 const int v = tid + g * STEP;
                 uint4 raw[DS_U];
+                if ((g + 1) * STEP <= n_kept) {
 #pragma unroll
-                for (int u = 0; u < DS_U; ++u) raw[u] = v + u * NT < n_kept ? kept[v + u * NT] : masked16<T>();
+                    for (int u = 0; u < DS_U; ++u) raw[u] = kept[v + u * NT];
+                } else {
+#pragma unroll
+                    for (int u = 0; u < DS_U; ++u) raw[u] = v + u * NT < n_kept ? kept[v + u * NT] : masked16<T>();
+                }
                 add_batch<T, DS_U, false>(raw, sums, scale);
             }
             if (n_kept < here.n_vec) sums = stream_rest<T, NT>(here.from, n_kept, here.n_vec, scale, sums);
@@ -359,15 +408,14 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
                 sums.raise(z_tail, scale);
                 sums.add(z_tail, scale);
             }
-            sums.t = 0.0f;
-            sums = warp_join(sums, scale);
+            sums = warp_join<false>(sums, scale);
             if (lane == 0) sh.warps[turn & 1][tid >> 5] = make_float4(sums.m, sums.s, 0.0f, 0.0f);
         }
         __syncthreads();
         any = more && sh.any[(i + 1) & 1];
         bool nothing = !live || w == 0.0f;
         if (live) {
-            sums = row_sums<NT>(sh, turn, log_cs, rank, scale, false);
+            sums = row_sums<NT>(sh, turn, log_cs, rank, scale, false, [] {});
             ++turn;
             nothing |= sums.m == -INFINITY && sums.s == 0.0f;
         }
@@ -412,9 +460,13 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
         };
         for (int g = 0; g < groups; ++g) {
             const int v = tid + g * STEP;
+            if ((g + 1) * STEP <= n_kept) {
 #pragma unroll
-            for (int u = 0; u < DS_U; ++u)
-                if (v + u * NT < n_kept) vec(v + u * NT, kept[v + u * NT]);
+                for (int u = 0; u < DS_U; ++u) vec(v + u * NT, kept[v + u * NT]);
+            } else {
+                for (int u = 0; u < DS_U; ++u)
+                    if (v + u * NT < n_kept) vec(v + u * NT, kept[v + u * NT]);
+            }
             if (any) fetch(part, g);
         }
         for (int v = n_kept + tid; v < here.n_vec; v += NT) vec(v, load16_rw(here.from + v));
@@ -432,16 +484,20 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
 // The same in a warp, without a barrier but its own: 12 rows of 16 KB in the air per SM.
 constexpr int WARP_ROWS = 4;
 
+// 16-byte units of shared memory of one warp.
+__host__ __device__ inline int warp_vectors(int keep, int n) { return keep ? keep + (2 * n + 3) / 4 + WARP_DUP_BITS / 128 : 0; }
+
 template <class T, int ENTRIES>
 __global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, int keep) {
-    extern __shared__ uint4 shared[];  // WARP_ROWS of: [keep] vectors, [n] ids, [n] shares
+    extern __shared__ uint4 shared[];  // WARP_ROWS of: [keep] vectors, [n] ids, [n] shares, the bitmap
     constexpr int N = Vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r = (int64_t)blockIdx.x * WARP_ROWS + warp;
     if (r >= a.rows) return;
-    uint4 *kept = shared + warp * (keep + (2 * a.n + 3) / 4);
+    uint4 *kept = shared + warp * warp_vectors(keep, a.n);
     uint32_t *id = (uint32_t *)(kept + keep);
     float *q = (float *)(id + a.n);
+    uint32_t *bits = (uint32_t *)(kept + warp_vectors(keep, a.n)) - WARP_DUP_BITS / 32;
     const T *row = (const T *)a.logits + r * a.stride;
     const RowSpan span = row_span(row, a.vocab);
     const uint4 *body = (const uint4 *)(row + span.head);
@@ -488,6 +544,7 @@ __global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, 
         for (int v = half + lane; v < n_vec; v += 32) copy_async16(&kept[v], body + v);
         copy_commit();
         entry_logits();
+        for (int i = lane; i < WARP_DUP_BITS / 32; i += 32) bits[i] = 0;
         auto add = [&](int from, int to) {
             for (int v = from + lane; v < to; v += 32 * DS_U) {
                 uint4 raw[DS_U];
@@ -519,8 +576,7 @@ __global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, 
         sums.raise(z_tail, scale);
         sums.add(z_tail, scale);
     }
-    sums.t = 0.0f;
-    const SoftSums all = warp_join(sums, scale);
+    const SoftSums all = warp_join<false>(sums, scale);
     const float log_s = logf(all.s), log2_s = log_s * LOG2E;
     const bool empty = all.m == -INFINITY && all.s == 0.0f;  // a student that can say nothing
     float log_q[ENTRIES], kl = 0.0f;
@@ -540,12 +596,10 @@ __global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, 
     auto dense = [&](float z) { return gs * ex2(fmaf(z - all.m, scale, -log2_s)); };
     const float2 nm = make_float2(-all.m, -all.m), sc2 = make_float2(scale, scale), nl = make_float2(-log2_s, -log2_s),
                  g2 = make_float2(gs, gs);
+    float share[ENTRIES];
 #pragma unroll
-    for (int k = 0; k < ENTRIES; ++k)
-        if (k * 32 + lane < a.n) {
-            id[k * 32 + lane] = now.id[k];
-            q[k * 32 + lane] = now.q[k];
-        }
+    for (int k = 0; k < ENTRIES; ++k) share[k] = now.q[k];
+    if (perhaps_twice<WARP_DUP_BITS>(now.id, bits)) total_shares(now, a.n, id, q, share);
     __syncwarp();
     for (int v = lane; v < n_vec; v += 32) {
         float x[N];
@@ -566,11 +620,7 @@ __global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, 
     // here more than once gets the same value each time.)
 #pragma unroll
     for (int k = 0; k < ENTRIES; ++k)
-        if (now.id[k] != NO_TOKEN) {
-            float share = 0.0f;
-            for (int j = 0; j < a.n; ++j) share += id[j] == now.id[k] ? q[j] : 0.0f;
-            out[now.id[k]] = from_f32<T>(gs * (ex2(fmaf(z_entry[k] - all.m, scale, -log2_s)) - share));
-        }
+        if (now.id[k] != NO_TOKEN) out[now.id[k]] = from_f32<T>(gs * (ex2(fmaf(z_entry[k] - all.m, scale, -log2_s)) - share[k]));
 }
 
 template <class T>
@@ -579,7 +629,7 @@ cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     const int64_t n_vec = a.vocab / N;
     if (n_vec <= DS_WVEC_ && a.rows >= DS_WMIN_) {
         const int keep = a.dlogits ? (int)n_vec : 0;
-        const int smem = WARP_ROWS * (keep + (2 * a.n + 3) / 4) * 16;
+        const int smem = WARP_ROWS * warp_vectors(keep, a.n) * 16;
         auto kern = a.n <= 64 ? distill_warp_k<T, 2> : distill_warp_k<T, TEACHER_MAX / 32>;
         if (smem > 48 << 10) {
             cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(32 * WARP_ROWS, 4) token_logprobs_warp_k(Logpr
     }
     const RowSpan span = row_span(row, a.vocab);
     SoftSums sums = logprobs_part<T, 32>(a, row, span, 0, span.n_vec, true, true, slot_shift, w);
-    write_row<32>(a, r, warp_join(sums, a.scale), z_target, w.best);
+    write_row<32>(a, r, warp_join<true>(sums, a.scale), z_target, w.best);
 }
 
 // ---------------------------------------------------------------- long rows: a block or a cluster each
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(LP_NT, 4) token_logprobs_k(LogprobsArgs a, int
             // The parts in their order.
             if (tid < cs) sh.warps[tid] = *cluster.map_shared_rank(&sh.part, tid);
             __syncthreads();
-            sums = join_places(sh.warps, cs, a.scale);
+            sums = join_places<true>(sh.warps, cs, a.scale);
             if (a.top) {
                 for (int i = tid; i < cs * a.top; i += LP_NT)
                     sh.cand[i] = cluster.map_shared_rank(sh.best, i / a.top)[i % a.top];

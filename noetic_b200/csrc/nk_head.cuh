@@ -267,8 +267,9 @@ __device__ __forceinline__ float add_some(const uint4 (&raw)[U], int v, int v1, 
 // Adds the vectors v0 <= v < v1 of `body` to the sums of a team of NT threads,
 // of which this is thread `tid`, U to a thread at a time, the next U on their
 // way while the present ones are added.  each(batch, maximum) is called for
-// every U.  Returns the number of these.
-template <class T, int NT, int U, bool ENT, class F>
+// every U.  Returns the number of these.  With MASK a last batch that is not
+// full counts its missing vectors as masked ones.
+template <class T, int NT, int U, bool ENT, bool MASK = false, class F>
 __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int tid, float scale, SoftSums &sums, F &&each) {
     uint4 next[U];
     int batch = 0, v = v0 + tid;
@@ -280,7 +281,10 @@ __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int ti
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (v + u * NT < v1) next[u] = load16_rw(at + u * NT);
+                if (v + u * NT < v1)
+                    next[u] = load16_rw(at + u * NT);
+                else if (MASK)
+                    next[u] = masked16<T>();
         }
         at += U * NT;
     };
@@ -292,7 +296,7 @@ __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int ti
         const int now = v;
         v += NT * U;
         fetch();
-        each(batch, now + (U - 1) * NT < v1 ? add_batch<T, U, ENT>(raw, sums, scale) : add_some<T, NT, U, ENT>(raw, now, v1, sums, scale));
+        each(batch, MASK || now + (U - 1) * NT < v1 ? add_batch<T, U, ENT>(raw, sums, scale) : add_some<T, NT, U, ENT>(raw, now, v1, sums, scale));
     }
     return batch;
 }
@@ -315,18 +319,20 @@ __device__ __forceinline__ float warp_max1(float v) {
     return r;
 }
 
-// A warp's sums joined, in all its lanes.
+// A warp's sums joined, in all its lanes (t only with ENT).
+template <bool ENT>
 __device__ __forceinline__ SoftSums warp_join(SoftSums a, float scale) {
     SoftSums r;
     r.m = warp_max1(a.m);
     // A thread without a logit above -infinity holds s = 0, or NaN.
     if (a.m != -INFINITY) a.raise(r.m, scale);
     r.s = warp_sum(a.s);
-    r.t = warp_sum(a.t);
+    if (ENT) r.t = warp_sum(a.t);
     return r;
 }
 
 // The parts that n <= 32 places hold, joined in a fixed order in every lane of a warp.
+template <bool ENT>
 __device__ __forceinline__ SoftSums join_places(const float4 *places, int n, float scale) {
     SoftSums a;
     const int lane = threadIdx.x & 31;
@@ -336,17 +342,17 @@ __device__ __forceinline__ SoftSums join_places(const float4 *places, int n, flo
         a.s = p.y;
         a.t = p.z;
     }
-    return warp_join(a, scale);
+    return warp_join<ENT>(a, scale);
 }
 
 // Every thread's sums joined over a block of NT with one barrier; all threads
 // get the result.  `places` holds a float4 per warp and must not be in use.
 template <int NT>
 __device__ __forceinline__ SoftSums block_join(const SoftSums &a, float scale, float4 *places) {
-    const SoftSums w = warp_join(a, scale);
+    const SoftSums w = warp_join<true>(a, scale);
     if ((threadIdx.x & 31) == 0) places[threadIdx.x >> 5] = make_float4(w.m, w.s, w.t, 0.0f);
     __syncthreads();
-    return join_places(places, NT / 32, scale);
+    return join_places<true>(places, NT / 32, scale);
 }
 
 }  // namespace nk
