@@ -14,21 +14,12 @@ namespace {
 
 constexpr int TEACHER_MAX = 256;
 constexpr int DS_U = 4;
-#ifndef DS_NT_
-#define DS_NT_ 192
-#define DS_PART_ 68
-#define DS_ROWS_ 4
-#define DS_FILL_ 4
-#define DS_MINB_ 3
-#define DS_WVEC_ 1024
-#define DS_WMIN_ 512
-#endif
-constexpr int DS_NT = DS_NT_;
+constexpr int DS_NT = 192;
 constexpr int DS_CLUSTER = 8;
 constexpr int DUP_BITS = 16384, WARP_DUP_BITS = 8192;
-constexpr int DS_PART = DS_PART_ << 10;  // bytes of a part: three to an SM
+constexpr int DS_PART = 68 << 10;  // bytes of a part: three to an SM
 constexpr int DS_MOST = (208 << 10) / (DS_NT * DS_U * 16) * (DS_NT * DS_U * 16);  // the most that a CTA keeps, in whole batches
-constexpr int DS_ROWS = DS_ROWS_;        // rows of a cluster, at most
+constexpr int DS_ROWS = 4;         // rows of a cluster, at most
 
 __device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t i) {
     return dtype == 0   ? ((const float *)p)[i]
@@ -234,7 +225,7 @@ __device__ __noinline__ SoftSums stream_rest(const uint4 *from, int v0, int v1, 
 }
 
 template <class T, int NT, int ENTRIES>
-__global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, int log_cs, int keep, int rows_per) {
+__global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_cs, int keep, int rows_per) {
     namespace cg = cooperative_groups;
     extern __shared__ uint4 kept[];  // [keep]
     __shared__ DistillShared<NT> sh;
@@ -460,9 +451,12 @@ __global__ void __launch_bounds__(NT + 32, DS_MINB_) distill_k(DistillArgs a, in
         };
         for (int g = 0; g < groups; ++g) {
             const int v = tid + g * STEP;
+            uint4 raw[DS_U];
             if ((g + 1) * STEP <= n_kept) {
 #pragma unroll
-                for (int u = 0; u < DS_U; ++u) vec(v + u * NT, kept[v + u * NT]);
+                for (int u = 0; u < DS_U; ++u) raw[u] = kept[v + u * NT];
+#pragma unroll
+                for (int u = 0; u < DS_U; ++u) vec(v + u * NT, raw[u]);
             } else {
                 for (int u = 0; u < DS_U; ++u)
                     if (v + u * NT < n_kept) vec(v + u * NT, kept[v + u * NT]);
@@ -627,7 +621,7 @@ template <class T>
 cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
     const int64_t n_vec = a.vocab / N;
-    if (n_vec <= DS_WVEC_ && a.rows >= DS_WMIN_) {
+    if (n_vec <= 1024 && a.rows >= 512) {
         const int keep = a.dlogits ? (int)n_vec : 0;
         const int smem = WARP_ROWS * warp_vectors(keep, a.n) * 16;
         auto kern = a.n <= 64 ? distill_warp_k<T, 2> : distill_warp_k<T, TEACHER_MAX / 32>;
@@ -647,7 +641,7 @@ cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     const int cs = 1 << log_cs;
     const int64_t keep = a.dlogits ? std::min<int64_t>((n_vec + cs - 1) / cs, DS_MOST / 16) : 0;
     // Several rows to a cluster, as long as there are some turns of clusters left to even out.
-    const int64_t rows_per = std::max<int64_t>(1, std::min<int64_t>(DS_ROWS, a.rows * cs / (148 * 3 * DS_FILL_)));
+    const int64_t rows_per = std::max<int64_t>(1, std::min<int64_t>(DS_ROWS, a.rows * cs / (148 * 3 * 4)));
     const int64_t clusters = (a.rows + rows_per - 1) / rows_per;
     auto kern = a.n <= 64 ? distill_k<T, DS_NT, 2> : distill_k<T, DS_NT, TEACHER_MAX / 32>;
     if (keep * 16 > 32768) {

@@ -17,7 +17,7 @@ constexpr int LP_NT = 256;
 constexpr int TOP_MAX = 128;
 constexpr int LP_LOG_U = 2, LP_U = 1 << LP_LOG_U;
 constexpr int MAX_CLUSTER = 8;
-constexpr int MAXIMA = 256;  // that the bound on the alternatives is taken from
+constexpr int MAXIMA = 256;  // that a warp takes the bound on the alternatives from
 
 // The threads that share a row: a warp or a block of LP_NT.
 template <int NT>
@@ -40,7 +40,7 @@ struct TopTeam {
     uint64_t *cand;    // [cand_cap], shared with sc
     uint64_t *best;    // [top]
     float *group_max;  // [slots][team size]
-    float *thread_max; // [MAXIMA], a block's
+    float *thread_max; // [team size], a block's
     uint32_t *hits;    // [hit_cap]
     TopScratch *sc;
     uint32_t *word;    // [4]: candidates, hits, prefix, above
@@ -175,9 +175,10 @@ __device__ __forceinline__ SoftSums logprobs_part(const LogprobsArgs &a, const T
         // the range between the least and the greatest of them, sixteen times at
         // most.
         const float *maxima = NT == 32 ? w.group_max : w.thread_max;
-        uint32_t k[MAXIMA / 32], lo = 0xFFFFFFFFu, hi = 0;
+        constexpr int PER_LANE = (NT == 32 ? MAXIMA : NT) / 32;
+        uint32_t k[PER_LANE], lo = 0xFFFFFFFFu, hi = 0;
 #pragma unroll
-        for (int i = 0; i < MAXIMA / 32; ++i) {
+        for (int i = 0; i < PER_LANE; ++i) {
             k[i] = order_key(maxima[i * 32 + lane]);
             lo = min(lo, k[i]);
             hi = max(hi, k[i]);
@@ -189,7 +190,7 @@ __device__ __forceinline__ SoftSums logprobs_part(const LogprobsArgs &a, const T
             const uint32_t mid = lo + (hi - lo) / 2;
             int n = 0;
 #pragma unroll
-            for (int j = 0; j < MAXIMA / 32; ++j) n += k[j] >= mid;
+            for (int j = 0; j < PER_LANE; ++j) n += k[j] >= mid;
             n = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
             if (n < a.top) {
                 hi = mid;
@@ -345,14 +346,15 @@ constexpr int LP_SLOTS = 32;      // groups per thread
 constexpr int HITS = 512;
 constexpr int CANDIDATES = 1024;  // at least MAX_CLUSTER * TOP_MAX
 
+template <int NT>
 struct LogprobsShared {
-    float4 warps[LP_NT / 32], part;
+    float4 warps[NT / 32 > MAX_CLUSTER ? NT / 32 : MAX_CLUSTER], part;
     uint32_t word[4], hits[HITS];
     uint64_t cand[CANDIDATES];
     uint64_t best[TOP_MAX];
-    float thread_max[LP_NT];
+    float thread_max[NT];
 };
-static_assert(sizeof(TopScratch) <= CANDIDATES * 8 && LP_NT == MAXIMA && CANDIDATES >= MAX_CLUSTER * TOP_MAX && MAX_CLUSTER <= LP_NT / 32, "");
+static_assert(sizeof(TopScratch) <= CANDIDATES * 8 && CANDIDATES >= MAX_CLUSTER * TOP_MAX, "");
 
 // How many of list[0, n) (descending) are above key.
 __device__ __forceinline__ int count_above(const uint64_t *list, int n, uint64_t key) {
@@ -367,10 +369,10 @@ __device__ __forceinline__ int count_above(const uint64_t *list, int n, uint64_t
     return lo;
 }
 
-template <class T>
-__global__ void __launch_bounds__(LP_NT, 4) token_logprobs_k(LogprobsArgs a, int log_cs, int slot_shift) {
+template <class T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_k(LogprobsArgs a, int log_cs, int slot_shift) {
     extern __shared__ float group_max[];
-    __shared__ LogprobsShared sh;
+    __shared__ LogprobsShared<NT> sh;
     const int tid = threadIdx.x;
     const int cs = 1 << log_cs;
     const int64_t r = blockIdx.x >> log_cs;
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(LP_NT, 4) token_logprobs_k(LogprobsArgs a, int
     const T *row = (const T *)a.logits + r * a.stride;
     const uint32_t target = a.targets ? a.targets[r] : NO_TOKEN;
     if (a.targets && target >= (uint32_t)a.vocab) {
-        if (rank == 0) no_token_row<LP_NT>(a, r);
+        if (rank == 0) no_token_row<NT>(a, r);
         return;  // the whole cluster
     }
     const float z_target = a.targets && rank == 0 && tid == 0 ? to_f32(row[target]) : 0.0f;
@@ -394,8 +396,8 @@ __global__ void __launch_bounds__(LP_NT, 4) token_logprobs_k(LogprobsArgs a, int
     w.hit_cap = HITS;
     const RowSpan span = row_span(row, a.vocab);
     const int v0 = (int)((int64_t)span.n_vec * rank >> log_cs), v1 = (int)((int64_t)span.n_vec * (rank + 1) >> log_cs);
-    SoftSums sums = logprobs_part<T, LP_NT>(a, row, span, v0, v1, rank == 0, rank == cs - 1, slot_shift, w);
-    sums = block_join<LP_NT>(sums, a.scale, sh.warps);
+    SoftSums sums = logprobs_part<T, NT>(a, row, span, v0, v1, rank == 0, rank == cs - 1, slot_shift, w);
+    sums = block_join<NT>(sums, a.scale, sh.warps);
 
     if (cs > 1) {
         namespace cg = cooperative_groups;
@@ -408,12 +410,12 @@ __global__ void __launch_bounds__(LP_NT, 4) token_logprobs_k(LogprobsArgs a, int
             __syncthreads();
             sums = join_places<true>(sh.warps, cs, a.scale);
             if (a.top) {
-                for (int i = tid; i < cs * a.top; i += LP_NT)
+                for (int i = tid; i < cs * a.top; i += NT)
                     sh.cand[i] = cluster.map_shared_rank(sh.best, i / a.top)[i % a.top];
                 __syncthreads();
-                for (int i = tid; i < a.top; i += LP_NT) sh.best[i] = 0;
+                for (int i = tid; i < a.top; i += NT) sh.best[i] = 0;
                 __syncthreads();
-                for (int i = tid; i < cs * a.top; i += LP_NT) {
+                for (int i = tid; i < cs * a.top; i += NT) {
                     const uint64_t key = sh.cand[i];
                     if (key == 0) continue;
                     int rk = 0;
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(LP_NT, 4) token_logprobs_k(LogprobsArgs a, int
         cluster.sync();  // the others' shared memory is read until here
         if (rank != 0) return;
     }
-    write_row<LP_NT>(a, r, sums, z_target, sh.best);
+    write_row<NT>(a, r, sums, z_target, sh.best);
 }
 
 // The gradient, element by element: a CTA takes LP_NT * LP_U vectors of one
@@ -487,6 +489,32 @@ __global__ void __launch_bounds__(LP_NT) token_logprobs_backward_k(LogprobsGradA
 
 }  // namespace
 
+template <class T, int NT>
+cudaError_t launch_blocks(const LogprobsArgs &a, cudaStream_t st) {
+    const int64_t n_vec = a.vocab / Vec<T>::N;
+    // A row is split over a cluster while the rows alone leave SMs idle and
+    // every thread keeps a vector.
+    int log_cs = 0;
+    while ((1 << log_cs) < MAX_CLUSTER && a.rows << log_cs < 148 && n_vec >> (log_cs + 1) >= NT) ++log_cs;
+    const int cs = 1 << log_cs;
+    const int64_t batches = ((n_vec + cs - 1) / cs + NT * LP_U - 1) / (NT * LP_U);
+    int shift = 0;
+    while ((batches >> shift) >= LP_SLOTS) ++shift;
+    const size_t smem = a.top ? ((batches >> shift) + 1) * NT * sizeof(float) : 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.rows * cs));
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cs;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cs > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, token_logprobs_k<T, NT>, a, log_cs, shift);
+}
+
 template <class T>
 cudaError_t launch_logprobs(const LogprobsArgs &a, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
@@ -507,27 +535,14 @@ cudaError_t launch_logprobs(const LogprobsArgs &a, cudaStream_t st) {
         kern<<<(unsigned)((a.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, smem, st>>>(a, shift);
         return cudaGetLastError();
     }
-    // A row is split over a cluster while the rows alone leave SMs idle and
-    // every thread keeps a vector.
-    int log_cs = 0;
-    while ((1 << log_cs) < MAX_CLUSTER && a.rows << log_cs < 148 && n_vec >> (log_cs + 1) >= LP_NT) ++log_cs;
-    const int cs = 1 << log_cs;
-    const int64_t batches = ((n_vec + cs - 1) / cs + LP_NT * LP_U - 1) / (LP_NT * LP_U);
-    int shift = 0;
-    while ((batches >> shift) >= LP_SLOTS) ++shift;
-    const size_t smem = a.top ? ((batches >> shift) + 1) * LP_NT * sizeof(float) : 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.rows * cs));
-    cfg.blockDim = dim3(LP_NT);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cs;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cs > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_k<T>, a, log_cs, shift);
+    // A block of 128 threads, eight to an SM, or of 256, four: the smaller one
+    // where the larger would need a second round for few rows, and for rows of up to 128
+    // KB, whose search is a larger share.  Measured with 20 alternatives, 128
+    // against 256: 700 rows of 40 KB 16 and 23 us, of 256 KB 47 and 57; 3000 rows of
+    // 100 KB 74 and 82; but 1500 rows of 256 KB 96 and 86, 450 rows of 100 KB 23 and 20.
+    // With more than 64 alternatives 128 threads' maxima bound them loosely.
+    const bool small = a.rows > 592 && a.top <= 64 && (a.rows <= 1184 || n_vec <= 8192);
+    return small ? launch_blocks<T, 128>(a, st) : launch_blocks<T, 256>(a, st);
 }
 
 template <class T>

@@ -115,8 +115,9 @@ __device__ __forceinline__ uint4 load16_rw(const void *p) {
                  : "l"(p));
     return v;
 }
+// (Not a barrier to the compiler: loads of what it does not overwrite may pass.)
 __device__ __forceinline__ void store16(void *p, uint4 v) {
-    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
 }
 
 template <class T>
