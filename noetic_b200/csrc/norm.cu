@@ -1,15 +1,16 @@
 // norm.cu -- layer norm and RMSNorm of rows, and their gradients
 // (include/noetic/head.h).
 //
-// Rows of up to NM_WIDE elements are taken by groups of G threads (a warp to
-// 512 threads), NM_VALS elements to a thread, which stay in registers from the
-// one load of the row to its one store: the mean and then the sum of squared
-// differences from it are two reductions over registers, not two passes over
-// memory.  A block walks rows blockIdx, blockIdx + gridDim, ... so that the
-// gain, the bias and (backward) the sums for dgain and dbias stay in registers
-// too, and the next row is on its way while the present one is worked on.  All
-// of it is bound by HBM.  Wider rows take one block per row and read it again
-// from L2.
+// Rows are taken by groups of G threads (a warp to 512 threads), VALS elements to
+// a thread, which stay on the SM from the one load of the row to its one
+// store: the mean and then the sum of squared differences from it are two
+// reductions over registers, not two passes over memory.  A block walks rows
+// blockIdx, blockIdx + gridDim, ..., so that the gain, the bias and (backward)
+// the sums for dgain and dbias stay in registers too, and the next rows are on
+// their way while the present one is worked on.  All of it is bound by HBM,
+// as long as a row costs its threads few instructions beside its elements:
+// hence the f32 operations in pairs, and 64 bytes of a row to a thread where it has them.
+// Rows too wide for that take one block per row and read it again from L2.
 
 #include <algorithm>
 
@@ -21,8 +22,7 @@ namespace nk {
 namespace {
 
 constexpr int NM_NT = 256;
-constexpr int NM_VALS = 16;
-constexpr int NM_WIDE = 8192;
+constexpr int ONE_VALS = 16;  // of a thread, backward and where no vectors fit
 constexpr int FWD_DEPTH = 4;  // rows on their way to each group
 constexpr int BWD_DEPTH = 3;
 constexpr int PARTIAL_ROWS = 1024;  // most partial sums of dgain and dbias
@@ -70,177 +70,176 @@ __device__ __forceinline__ float2 group_sum2(float2 v, float2 *red) {
     return v;
 }
 
-// Where a thread's elements lie: with VEC, NM_VALS / N vectors of N elements, G
+// Where a thread's elements lie: with VEC, VALS / N vectors of N elements, G
 // vectors apart; else single elements, G apart.
-template <class T, int G, bool VEC>
+template <class T, int G, int VALS, bool VEC>
 struct Place {
     static constexpr int N = VEC ? Vec<T>::N : 1;
-    static constexpr int LOADS = NM_VALS / N;
+    static constexpr int LOADS = VALS / N;
     static __device__ __forceinline__ int at(int lane, int l) { return (l * G + lane) * N; }
 };
 
-// A thread's part of one row as it lies in memory.
-template <class T, int G, bool VEC>
-struct RowPart {
-    using P = Place<T, G, VEC>;
-    uint4 raw[VEC ? P::LOADS : 1];
-    T one[VEC ? 1 : P::LOADS];
-
-    __device__ __forceinline__ void load(const T *row, int lane, int width, bool real) {
-#pragma unroll
-        for (int l = 0; l < P::LOADS; ++l) {
-            const int e = P::at(lane, l);
-            if constexpr (VEC)
-                raw[l] = real && e < width ? load16_rw(row + e) : make_uint4(0, 0, 0, 0);
-            else
-                one[l] = real && e < width ? row[e] : from_f32<T>(0.0f);
-        }
-    }
-    __device__ __forceinline__ void get(float (&x)[NM_VALS]) const {
-#pragma unroll
-        for (int l = 0; l < P::LOADS; ++l) {
-            if constexpr (VEC) {
-                float v[P::N];
-                unpack<T>(raw[l], v);
-#pragma unroll
-                for (int i = 0; i < P::N; ++i) x[l * P::N + i] = v[i];
-            } else {
-                x[l] = to_f32(one[l]);
-            }
-        }
-    }
-    static __device__ __forceinline__ void store(T *row, int lane, int width, const float (&x)[NM_VALS]) {
-#pragma unroll
-        for (int l = 0; l < P::LOADS; ++l) {
-            const int e = P::at(lane, l);
-            if (e >= width) continue;
-            if constexpr (VEC) {
-                float v[P::N];
-#pragma unroll
-                for (int i = 0; i < P::N; ++i) v[i] = x[l * P::N + i];
-                store16(row + e, pack<T>(v));
-            } else {
-                row[e] = from_f32<T>(x[l]);
-            }
-        }
-    }
-};
-
-// The rows that a thread will work on next: with VEC in its own places of a
-// ring in shared memory, DEPTH rows on their way by asynchronous copies (no
-// barrier: a thread reads only what it copied); else one row in registers.
-template <class T, int G, bool VEC, int NT, int DEPTH, int ARRAYS>
+// The rows that a thread will work on next, ARRAYS of them at a time: with VEC
+// in its own places of a ring in shared memory, DEPTH rows on their way by
+// asynchronous copies (no barrier: a thread reads only what it copied); else
+// one row in registers, which the next push overwrites.
+template <class T, int G, int VALS, bool VEC, int NT, int DEPTH, int ARRAYS>
 struct RowQueue {
-    using P = Place<T, G, VEC>;
+    using P = Place<T, G, VALS, VEC>;
+    static constexpr int AHEAD = VEC ? DEPTH : 1;
     static constexpr int BYTES = VEC ? DEPTH * ARRAYS * P::LOADS * NT * 16 : 0;
-    RowPart<T, G, VEC> next[ARRAYS];
-    uint4 *ring;  // [DEPTH][ARRAYS][LOADS][NT]
-    int at = 0;
+    T next[ARRAYS][VEC ? 1 : VALS];
+    uint4 *ring;  // [DEPTH][ARRAYS][LOADS][NT], from this thread's place on
+    int slot = 0;
 
-    __device__ __forceinline__ void push(const T *const (&rows)[ARRAYS], int slot, int lane, int width, bool real) {
+    __device__ __forceinline__ uint4 *place(int at, int k) const { return ring + (at * ARRAYS + k) * P::LOADS * NT; }
+    __device__ __forceinline__ void push(const T *const (&rows)[ARRAYS], int at, int lane, int width, bool real) {
 #pragma unroll
         for (int k = 0; k < ARRAYS; ++k) {
-            if constexpr (VEC) {
+            const T *row = rows[k] + lane * P::N;
 #pragma unroll
-                for (int l = 0; l < P::LOADS; ++l)
-                    if (real && P::at(lane, l) < width)
-                        copy_async16(ring + ((slot * ARRAYS + k) * P::LOADS + l) * NT + threadIdx.x, rows[k] + P::at(lane, l));
-            } else {
-                next[k].load(rows[k], lane, width, real);
+            for (int l = 0; l < P::LOADS; ++l) {
+                const bool in = real && P::at(lane, l) < width;
+                if constexpr (VEC) {
+                    if (in) copy_async16(place(at, k) + l * NT, row + l * G * P::N);
+                } else {
+                    next[k][l] = in ? row[l * G] : from_f32<T>(0.0f);
+                }
             }
         }
         if constexpr (VEC) copy_commit();
     }
-    // The row pushed DEPTH pushes ago (VEC) or last.
-    __device__ __forceinline__ void front(int k, int lane, int width, bool real, float (&x)[NM_VALS]) {
+    // Waits for the row pushed first, which is then the present one.
+    __device__ __forceinline__ void wait() const {
+        if constexpr (VEC) copy_wait<DEPTH - 1>();
+    }
+    // Done with it: the next push goes to its slot.
+    __device__ __forceinline__ void pop() { slot = slot + 1 == AHEAD ? 0 : slot + 1; }
+    // Chunk c of the present row: a vector's elements (VEC) or two of the single
+    // ones, in pairs; zeros beyond the width.
+    static constexpr int CHUNK = VEC ? P::N / 2 : 1;
+    __device__ __forceinline__ void get(int k, int c, int lane, int width, bool real, float2 (&x)[CHUNK]) const {
         if constexpr (VEC) {
+            float v[P::N];
+            unpack<T>(real && P::at(lane, c) < width ? place(slot, k)[c * NT] : make_uint4(0, 0, 0, 0), v);
 #pragma unroll
-            for (int l = 0; l < P::LOADS; ++l) {
-                float v[P::N];
-                unpack<T>(real && P::at(lane, l) < width ? ring[((at * ARRAYS + k) * P::LOADS + l) * NT + threadIdx.x]
-                                                         : make_uint4(0, 0, 0, 0), v);
-#pragma unroll
-                for (int i = 0; i < P::N; ++i) x[l * P::N + i] = v[i];
-            }
+            for (int i = 0; i < CHUNK; ++i) x[i] = make_float2(v[2 * i], v[2 * i + 1]);
         } else {
-            next[k].get(x);
+            x[0] = make_float2(to_f32(next[k][2 * c]), to_f32(next[k][2 * c + 1]));
         }
+    }
+    // A pair of chunk c, 0 where it is beyond the width.
+    static __device__ __forceinline__ float2 keep(int c, int lane, int width, float2 v) {
+        if constexpr (VEC) return P::at(lane, c) < width ? v : make_float2(0.0f, 0.0f);
+        return make_float2(P::at(lane, 2 * c) < width ? v.x : 0.0f, P::at(lane, 2 * c + 1) < width ? v.y : 0.0f);
     }
 };
 
-// A thread's part of an f32 vector of the width (null: `other`).
-template <class T, int G, bool VEC>
-__device__ __forceinline__ void column_part(const float *p, float other, int lane, int width, float (&x)[NM_VALS]) {
-    using P = Place<T, G, VEC>;
+// Chunk c of a thread's part of a row, as RowQueue::get has it.
+template <class T, int G, int VALS, bool VEC, int CHUNK>
+__device__ __forceinline__ void store_chunk(T *row, int c, int lane, int width, const float2 (&x)[CHUNK]) {
+    using P = Place<T, G, VALS, VEC>;
+    if constexpr (VEC) {
+        if (P::at(lane, c) >= width) return;
+        float v[P::N];
 #pragma unroll
-    for (int l = 0; l < P::LOADS; ++l) {
-        const int e = P::at(lane, l);
-#pragma unroll
-        for (int i = 0; i < P::N; ++i) x[l * P::N + i] = e < width ? (p ? p[e + i] : other) : 0.0f;
+        for (int i = 0; i < CHUNK; ++i) {
+            v[2 * i] = x[i].x;
+            v[2 * i + 1] = x[i].y;
+        }
+        store16(row + P::at(lane, c), pack<T>(v));
+    } else {
+        if (P::at(lane, 2 * c) < width) row[P::at(lane, 2 * c)] = from_f32<T>(x[0].x);
+        if (P::at(lane, 2 * c + 1) < width) row[P::at(lane, 2 * c + 1)] = from_f32<T>(x[0].y);
     }
 }
 
+// A thread's part of an f32 vector of the width (null: `other`); 0 beyond it.
+template <class T, int G, int VALS, bool VEC>
+__device__ __forceinline__ void column_part(const float *p, float other, int lane, int width, float2 (&x)[VALS / 2]) {
+    using P = Place<T, G, VALS, VEC>;
+    auto one = [&](int k) {
+        const int e = P::at(lane, k / P::N) + k % P::N;
+        return e < width ? (p ? p[e] : other) : 0.0f;
+    };
+#pragma unroll
+    for (int k = 0; k < VALS / 2; ++k) x[k] = make_float2(one(2 * k), one(2 * k + 1));
+}
+
+// Elements e and e + step of a row, 0 beyond the width.
+template <class T>
+__device__ __forceinline__ float2 pair_of(const T *row, int e, int step, int width) {
+    return make_float2(e < width ? to_f32(row[e]) : 0.0f, e + step < width ? to_f32(row[e + step]) : 0.0f);
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // ---------------------------------------------------------------- forward
-template <class T, int G, bool VEC>
-__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 3) norm_rows_k(NormArgs a) {
-    using P = Place<T, G, VEC>;
-    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
+template <class T, int G, int VALS, bool VEC>
+__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_rows_k(NormArgs a) {
+    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G, H = VALS / 2;
+    using Queue = RowQueue<T, G, VALS, VEC, NT, FWD_DEPTH, 1>;
+    constexpr int C = Queue::CHUNK;
     __shared__ float red[2][32];
+    extern __shared__ uint4 ring[];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_n = 1.0f / (float)a.width;
-    float gain[NM_VALS], bias[NM_VALS];
-    extern __shared__ uint4 ring[];
-    RowQueue<T, G, VEC, NT, FWD_DEPTH, 1> queue;
-    queue.ring = ring;
-    constexpr int AHEAD = VEC ? FWD_DEPTH : 1;
+    float2 gain[H], bias[H];
+    Queue queue;
+    queue.ring = ring + threadIdx.x;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-    auto push = [&](int64_t q, int slot) {
+    auto push = [&](int64_t q, int at) {
         const T *const rows[1] = {(const T *)a.x + q * a.x_stride};
-        queue.push(rows, slot, lane, a.width, q < a.rows);
+        queue.push(rows, at, lane, a.width, q < a.rows);
     };
-    for (int k = 0; k < AHEAD; ++k) push(r + k * step, k);
+    for (int k = 0; k < Queue::AHEAD; ++k) push(r + k * step, k);
     if constexpr (VEC) {
-        column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
-        column_part<T, G, VEC>(a.bias, 0.0f, lane, a.width, bias);
+        column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
+        column_part<T, G, VALS, VEC>(a.bias, 0.0f, lane, a.width, bias);
     }
     // Every group takes the same number of turns: the reductions hold barriers.
-    const int64_t turns = (a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step;
-    for (int64_t i = 0; i < turns; ++i, r += step) {
+    const int turns = (int)((a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step);
+    for (int i = 0; i < turns; ++i, r += step) {
         const bool real = r < a.rows;
-        float x[NM_VALS];
-        if constexpr (VEC) copy_wait<FWD_DEPTH - 1>();
-        queue.front(0, lane, a.width, real, x);
-        push(r + AHEAD * step, queue.at);
-        queue.at = queue.at + 1 == AHEAD ? 0 : queue.at + 1;
+        float2 x[H];
+        queue.wait();
+#pragma unroll
+        for (int c = 0; c < H / C; ++c) {
+            float2 v[C];
+            queue.get(0, c, lane, a.width, real, v);
+#pragma unroll
+            for (int j = 0; j < C; ++j) x[c * C + j] = v[j];
+        }
+        push(r + Queue::AHEAD * step, queue.slot);
+        queue.pop();
         float mean = 0.0f;
         if (!a.rms) {
-            float s = 0.0f;
+            float2 s = x[0];
 #pragma unroll
-            for (int j = 0; j < NM_VALS; ++j) s += x[j];
-            mean = group_sum<G>(s, red[0]) * inv_n;
+            for (int j = 1; j < H; ++j) s = add2(s, x[j]);
+            mean = group_sum<G>(s.x + s.y, red[0]) * inv_n;
         }
-        float v = 0.0f;
+        float2 v = both(0.0f);
 #pragma unroll
-        for (int l = 0; l < P::LOADS; ++l)
-            if (P::at(lane, l) < a.width) {
-#pragma unroll
-                for (int j = 0; j < P::N; ++j) {
-                    float &d = x[l * P::N + j];
-                    d -= mean;
-                    v = fmaf(d, d, v);
-                }
-            }
-        const float rstd = 1.0f / sqrtf(fmaf(group_sum<G>(v, red[1]), inv_n, a.eps));
+        for (int j = 0; j < H; ++j) {
+            x[j] = Queue::keep(j / C, lane, a.width, add2(x[j], both(-mean)));
+            v = fma2(x[j], x[j], v);
+        }
+        const float rstd = 1.0f / sqrtf(fmaf(group_sum<G>(v.x + v.y, red[1]), inv_n, a.eps));
         if (G > 32 && a.rms) __syncthreads();  // red[1] again in the next turn
         if (!real) continue;
         if constexpr (!VEC) {  // from L1 for every row: the loads' sixteen registers are taken
-            column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
-            column_part<T, G, VEC>(a.bias, 0.0f, lane, a.width, bias);
+            column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
+            column_part<T, G, VALS, VEC>(a.bias, 0.0f, lane, a.width, bias);
         }
 #pragma unroll
-        for (int j = 0; j < NM_VALS; ++j) x[j] = fmaf(x[j] * rstd, gain[j], bias[j]);
-        RowPart<T, G, VEC>::store((T *)a.y + r * a.y_stride, lane, a.width, x);
+        for (int c = 0; c < H / C; ++c) {
+            float2 v[C];
+#pragma unroll
+            for (int j = 0; j < C; ++j) v[j] = fma2(mul2(x[c * C + j], both(rstd)), gain[c * C + j], bias[c * C + j]);
+            store_chunk<T, G, VALS, VEC>((T *)a.y + r * a.y_stride, c, lane, a.width, v);
+        }
         if (lane == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
@@ -248,30 +247,78 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 3) norm
     }
 }
 
-// Rows wider than NM_WIDE.
-template <class T>
-__global__ void __launch_bounds__(NM_NT) norm_wide_rows_k(NormArgs a) {
+// Rows that are too wide for a group: a block each, the first `keep` vectors
+// (16 bytes with VEC) waiting in shared memory, the others read again from L2.
+constexpr int WIDE_NT = 512;
+constexpr int WIDE_KEEP = 64 << 10;  // bytes: three blocks to an SM
+
+// f(pair of elements, index of the first) over a thread's part of a row, which
+// `at(v)` gives as 16 bytes of N elements (VEC) or one element.
+template <class T, bool VEC, class At, class F>
+__device__ __forceinline__ void wide_each(int width, At &&at, F &&f) {
+    if constexpr (VEC) {
+        constexpr int N = Vec<T>::N;
+#pragma unroll 4
+        for (int v = threadIdx.x; v < width / N; v += WIDE_NT) {
+            float x[N];
+            unpack<T>(at(v), x);
+            f(v, x);
+        }
+    } else {
+#pragma unroll 4
+        for (int v = threadIdx.x; v < width; v += WIDE_NT) {
+            float x[1] = {to_f32(at(v))};
+            f(v, x);
+        }
+    }
+}
+
+template <class T, bool VEC>
+__global__ void __launch_bounds__(WIDE_NT) norm_wide_rows_k(NormArgs a, int keep) {
     __shared__ float red[32];
+    extern __shared__ uint4 kept[];
+    constexpr int N = VEC ? Vec<T>::N : 1;
     const int64_t r = blockIdx.x;
     const T *x = (const T *)a.x + r * a.x_stride;
     T *y = (T *)a.y + r * a.y_stride;
+    if constexpr (VEC) {
+        for (int v = threadIdx.x; v < min(keep, a.width / N); v += WIDE_NT) copy_async16(&kept[v], x + v * N);
+        copy_commit();
+        copy_wait<0>();
+    }
+    auto at = [&](int v) {
+        if constexpr (VEC)
+            return v < keep ? kept[v] : load16_rw(x + (int64_t)v * N);
+        else
+            return x[v];
+    };
     const float n = (float)a.width;
     float mean = 0.0f;
     if (!a.rms) {
         float s = 0.0f;
-        for (int e = threadIdx.x; e < a.width; e += NM_NT) s += to_f32(x[e]);
+        wide_each<T, VEC>(a.width, at, [&](int, float (&z)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s += z[i];
+        });
         mean = block_sum(s, red) / n;
     }
     float v = 0.0f;
-    for (int e = threadIdx.x; e < a.width; e += NM_NT) {
-        const float d = to_f32(x[e]) - mean;
-        v = fmaf(d, d, v);
-    }
+    wide_each<T, VEC>(a.width, at, [&](int, float (&z)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v = fmaf(z[i] - mean, z[i] - mean, v);
+    });
     const float rstd = 1.0f / sqrtf(block_sum(v, red) / n + a.eps);
-    for (int e = threadIdx.x; e < a.width; e += NM_NT) {
-        const float h = (to_f32(x[e]) - mean) * rstd;
-        y[e] = from_f32<T>(fmaf(h, a.gain ? a.gain[e] : 1.0f, a.bias ? a.bias[e] : 0.0f));
-    }
+    wide_each<T, VEC>(a.width, at, [&](int w, float (&z)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = w * N + i;
+            z[i] = fmaf((z[i] - mean) * rstd, a.gain ? a.gain[e] : 1.0f, a.bias ? a.bias[e] : 0.0f);
+        }
+        if constexpr (VEC)
+            store16(y + (int64_t)w * N, pack<T>(z));
+        else
+            y[w] = from_f32<T>(z[0]);
+    });
     if (threadIdx.x == 0) {
         if (a.mean) a.mean[r] = mean;
         if (a.rstd) a.rstd[r] = rstd;
@@ -280,127 +327,210 @@ __global__ void __launch_bounds__(NM_NT) norm_wide_rows_k(NormArgs a) {
 
 // ---------------------------------------------------------------- backward
 // dx of the rows, and with PARAMS this block's sums for dgain and dbias: its
-// groups' registers joined in shared memory in their order, then one row of
-// the workspace per block.
-template <class T, int G, bool VEC, bool PARAMS>
+// groups' registers joined in shared memory in their order, one row of
+// the workspace per block.  The row is unpacked twice, once for the sums and
+// once for dx: it waits in shared memory (without VEC in L1), not in registers.
+template <class T, int G, int VALS, bool VEC, bool PARAMS>
 __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_backward_k(NormGradArgs a) {
-    using P = Place<T, G, VEC>;
-    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
+    using P = Place<T, G, VALS, VEC>;
+    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G, H = VALS / 2;
+    using Queue = RowQueue<T, G, VALS, VEC, NT, BWD_DEPTH, 2>;
+    constexpr int C = Queue::CHUNK;
     __shared__ float2 red[2][32];
     extern __shared__ uint4 ring[];
-    float *joined = (float *)ring;  // [2][width], when the rows are done
+    float *joined = (float *)ring;  // [GROUPS][2][width], when the rows are done
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_n = 1.0f / (float)a.width;
-    float gain[NM_VALS], dg[NM_VALS], db[NM_VALS];
+    float2 gain[H], dg[H], db[H];
 #pragma unroll
-    for (int j = 0; j < NM_VALS; ++j) dg[j] = db[j] = 0.0f;
-    RowQueue<T, G, VEC, NT, BWD_DEPTH, 2> queue;
-    queue.ring = ring;
-    constexpr int AHEAD = VEC ? BWD_DEPTH : 1;
+    for (int j = 0; j < H; ++j) dg[j] = db[j] = both(0.0f);
+    Queue queue;
+    queue.ring = ring + threadIdx.x;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-    auto push = [&](int64_t q, int slot) {
+    auto push = [&](int64_t q, int at) {
         const T *const rows[2] = {(const T *)a.x + q * a.x_stride, (const T *)a.dy + q * a.dy_stride};
-        queue.push(rows, slot, lane, a.width, q < a.rows);
+        queue.push(rows, at, lane, a.width, q < a.rows);
     };
     float next_mean, next_rstd;
     auto stats = [&](int64_t q) {
         next_mean = q < a.rows && !a.rms ? a.mean[q] : 0.0f;
         next_rstd = q < a.rows ? a.rstd[q] : 0.0f;
     };
-    for (int k = 0; k < AHEAD; ++k) push(r + k * step, k);
+    for (int k = 0; k < Queue::AHEAD; ++k) push(r + k * step, k);
     stats(r);
-    if constexpr (VEC) column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
-    const int64_t turns = (a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step;
-    for (int64_t i = 0; i < turns; ++i, r += step) {
-        float h[NM_VALS], c[NM_VALS];
-        if constexpr (VEC) copy_wait<BWD_DEPTH - 1>();
-        queue.front(0, lane, a.width, r < a.rows, h);
-        queue.front(1, lane, a.width, r < a.rows, c);
+    if constexpr (VEC) column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
+    const int turns = (int)((a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step);
+    for (int i = 0; i < turns; ++i, r += step) {
+        const bool real = r < a.rows;
         const float mean = next_mean, rstd = next_rstd;
-        push(r + AHEAD * step, queue.at);
-        queue.at = queue.at + 1 == AHEAD ? 0 : queue.at + 1;
+        queue.wait();
+        if constexpr (!VEC) column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
         stats(r + step);
-        if constexpr (!VEC) column_part<T, G, VEC>(a.gain, 1.0f, lane, a.width, gain);
-        float2 s = make_float2(0.0f, 0.0f);
+        float2 sc = both(0.0f), sch = sc;
+        // Beyond the width dy and the gain are 0, and h does not count.
 #pragma unroll
-        for (int j = 0; j < NM_VALS; ++j) {
-            // Beyond the width c is 0, and h does not count.
-            h[j] = (h[j] - mean) * rstd;
-            if (PARAMS) {
-                dg[j] = fmaf(c[j], h[j], dg[j]);
-                db[j] += c[j];
+        for (int q = 0; q < H / C; ++q) {
+            float2 h[C], c[C];
+            queue.get(0, q, lane, a.width, real, h);
+            queue.get(1, q, lane, a.width, real, c);
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
+                if (PARAMS) {
+                    dg[q * C + j] = fma2(c[j], h[j], dg[q * C + j]);
+                    db[q * C + j] = add2(db[q * C + j], c[j]);
+                }
+                c[j] = mul2(c[j], gain[q * C + j]);
+                sc = add2(sc, c[j]);
+                sch = fma2(c[j], h[j], sch);
             }
-            c[j] *= gain[j];
-            s.x += c[j];
-            s.y = fmaf(c[j], h[j], s.y);
         }
-        if (!a.dx) continue;
-        s = group_sum2<G>(s, red[i & 1]);
-        const float mc = a.rms ? 0.0f : s.x * inv_n, mch = s.y * inv_n;
-        if (r < a.rows) {
+        if constexpr (!VEC) push(r + step, 0);
+        if (a.dx) {
+            const float2 s = group_sum2<G>(make_float2(sc.x + sc.y, sch.x + sch.y), red[i & 1]);
+            const float mc = a.rms ? 0.0f : s.x * inv_n, mch = s.y * inv_n;
+            T *to = (T *)a.dx + r * a.dx_stride;
+            if (real) {
 #pragma unroll
-            for (int j = 0; j < NM_VALS; ++j) h[j] = rstd * (c[j] - mc - h[j] * mch);
-            RowPart<T, G, VEC>::store((T *)a.dx + r * a.dx_stride, lane, a.width, h);
+                for (int q = 0; q < H / C; ++q) {
+                    float2 h[C], c[C];
+                    if constexpr (VEC) {
+                        queue.get(0, q, lane, a.width, real, h);
+                        queue.get(1, q, lane, a.width, real, c);
+                    } else {  // from L1
+                        h[0] = pair_of((const T *)a.x + r * a.x_stride, P::at(lane, 2 * q), G, a.width);
+                        c[0] = pair_of((const T *)a.dy + r * a.dy_stride, P::at(lane, 2 * q), G, a.width);
+                    }
+#pragma unroll
+                    for (int j = 0; j < C; ++j) {
+                        h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
+                        c[j] = fma2(c[j], gain[q * C + j], both(-mc));
+                        h[j] = mul2(both(rstd), fma2(h[j], both(-mch), c[j]));
+                    }
+                    store_chunk<T, G, VALS, VEC>(to, q, lane, a.width, h);
+                }
+            }
+        }
+        if constexpr (VEC) {
+            push(r + Queue::AHEAD * step, queue.slot);
+            queue.pop();
         }
     }
     if constexpr (PARAMS) {
         float *w = a.workspace + (int64_t)blockIdx.x * 2 * a.width;
+        float *to = GROUPS > 1 ? joined + group * 2 * a.width : w;
         if (GROUPS > 1) __syncthreads();
-        for (int g = 0; g < GROUPS; ++g) {
-            if (group == g) {
-                float *to = g == GROUPS - 1 ? w : joined;
 #pragma unroll
-                for (int l = 0; l < P::LOADS; ++l)
+        for (int j = 0; j < VALS; ++j) {
+            const int e = P::at(lane, j / P::N) + j % P::N;
+            if (e >= a.width) continue;
+            to[e] = j & 1 ? dg[j / 2].y : dg[j / 2].x;
+            to[a.width + e] = j & 1 ? db[j / 2].y : db[j / 2].x;
+        }
+        if (GROUPS > 1) {
+            __syncthreads();
+            for (int e = threadIdx.x; e < 2 * a.width; e += NT) {
+                float sum = joined[e];
 #pragma unroll
-                    for (int j = 0; j < P::N; ++j) {
-                        const int e = P::at(lane, l) + j;
-                        if (e >= a.width) continue;
-                        to[e] = g ? joined[e] + dg[l * P::N + j] : dg[l * P::N + j];
-                        to[a.width + e] = g ? joined[a.width + e] + db[l * P::N + j] : db[l * P::N + j];
-                    }
+                for (int g = 1; g < GROUPS; ++g) sum += joined[g * 2 * a.width + e];
+                w[e] = sum;
             }
-            if (g + 1 < GROUPS) __syncthreads();
         }
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(NM_NT) norm_wide_dx_k(NormGradArgs a) {
+template <class T, bool VEC>
+__global__ void __launch_bounds__(WIDE_NT) norm_wide_dx_k(NormGradArgs a, int keep) {
     __shared__ float red[32];
+    extern __shared__ uint4 kept[];  // [keep] of x, [keep] of dy
+    constexpr int N = VEC ? Vec<T>::N : 1;
     const int64_t r = blockIdx.x;
     const T *x = (const T *)a.x + r * a.x_stride, *dy = (const T *)a.dy + r * a.dy_stride;
     T *dx = (T *)a.dx + r * a.dx_stride;
-    const float n = (float)a.width, mean = a.rms ? 0.0f : a.mean[r], rstd = a.rstd[r];
-    float sc = 0.0f, sch = 0.0f;
-    for (int e = threadIdx.x; e < a.width; e += NM_NT) {
-        const float c = to_f32(dy[e]) * (a.gain ? a.gain[e] : 1.0f), h = (to_f32(x[e]) - mean) * rstd;
-        sc += c;
-        sch = fmaf(c, h, sch);
+    if constexpr (VEC) {
+        for (int v = threadIdx.x; v < min(keep, a.width / N); v += WIDE_NT) {
+            copy_async16(&kept[v], x + v * N);
+            copy_async16(&kept[keep + v], dy + v * N);
+        }
+        copy_commit();
+        copy_wait<0>();
     }
+    // The gradient's vector (element) v beside x's.
+    auto x_at = [&](int v) {
+        if constexpr (VEC)
+            return v < keep ? kept[v] : load16_rw(x + (int64_t)v * N);
+        else
+            return x[v];
+    };
+    const float n = (float)a.width, mean = a.rms ? 0.0f : a.mean[r], rstd = a.rstd[r];
+    auto both_of = [&](int v, float (&h)[N], float (&c)[N]) {
+        if constexpr (VEC)
+            unpack<T>(v < keep ? kept[keep + v] : load16_rw(dy + (int64_t)v * N), c);
+        else
+            c[0] = to_f32(dy[v]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            c[i] *= a.gain ? a.gain[v * N + i] : 1.0f;
+            h[i] = (h[i] - mean) * rstd;
+        }
+    };
+    float sc = 0.0f, sch = 0.0f;
+    wide_each<T, VEC>(a.width, x_at, [&](int v, float (&h)[N]) {
+        float c[N];
+        both_of(v, h, c);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            sc += c[i];
+            sch = fmaf(c[i], h[i], sch);
+        }
+    });
     sc = a.rms ? 0.0f : block_sum(sc, red) / n;
     sch = block_sum(sch, red) / n;
-    for (int e = threadIdx.x; e < a.width; e += NM_NT) {
-        const float c = to_f32(dy[e]) * (a.gain ? a.gain[e] : 1.0f), h = (to_f32(x[e]) - mean) * rstd;
-        dx[e] = from_f32<T>(rstd * (c - sc - h * sch));
-    }
+    wide_each<T, VEC>(a.width, x_at, [&](int v, float (&h)[N]) {
+        float c[N];
+        both_of(v, h, c);
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] = rstd * (c[i] - sc - h[i] * sch);
+        if constexpr (VEC)
+            store16(dx + (int64_t)v * N, pack<T>(h));
+        else
+            dx[v] = from_f32<T>(h[0]);
+    });
 }
 
-// Partial sums over the rows p, p + P, ... of one column per thread.
-template <class T>
+// Partial sums over the rows p, p + P, ... of N columns (one without VEC) per
+// thread.
+template <class T, bool VEC>
 __global__ void __launch_bounds__(NM_NT) norm_wide_param_k(NormGradArgs a) {
-    const int e = blockIdx.x * NM_NT + threadIdx.x;
+    constexpr int N = VEC ? Vec<T>::N : 1;
+    const int e = (blockIdx.x * NM_NT + threadIdx.x) * N;
     if (e >= a.width) return;
-    float dg = 0.0f, db = 0.0f;
+    float dg[N] = {}, db[N] = {};
+#pragma unroll 2
     for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const float dy = to_f32(((const T *)a.dy)[r * a.dy_stride + e]);
-        const float h = (to_f32(((const T *)a.x)[r * a.x_stride + e]) - (a.rms ? 0.0f : a.mean[r])) * a.rstd[r];
-        dg = fmaf(dy, h, dg);
-        db += dy;
+        const T *x = (const T *)a.x + r * a.x_stride + e, *dy = (const T *)a.dy + r * a.dy_stride + e;
+        const float mean = a.rms ? 0.0f : a.mean[r], rstd = a.rstd[r];
+        float h[N], c[N];
+        if constexpr (VEC) {
+            unpack<T>(load16_rw(x), h);
+            unpack<T>(load16_rw(dy), c);
+        } else {
+            h[0] = to_f32(*x);
+            c[0] = to_f32(*dy);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            dg[i] = fmaf(c[i], (h[i] - mean) * rstd, dg[i]);
+            db[i] += c[i];
+        }
     }
     float *w = a.workspace + (int64_t)blockIdx.y * 2 * a.width;
-    w[e] = dg;
-    w[a.width + e] = db;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        w[e + i] = dg[i];
+        w[a.width + e + i] = db[i];
+    }
 }
 
 // The partial rows' sum: 32 columns to a block, SUM_LANES threads to a column,
@@ -434,79 +564,105 @@ int64_t blocks(int64_t rows, int groups, int per_sm) {
     return std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, 148 * per_sm));
 }
 
-template <class Args>
-cudaError_t launch(void (*kern)(Args), const Args &a, int64_t grid, int nt, int smem, cudaStream_t st) {
+template <class Args, class... More>
+cudaError_t launch(void (*kern)(Args, More...), const Args &a, int64_t grid, int nt, int smem, cudaStream_t st, More... more) {
     if (smem > 40000) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
     }
-    kern<<<(unsigned)grid, nt, smem, st>>>(a);
+    kern<<<(unsigned)grid, nt, smem, st>>>(a, more...);
     return cudaGetLastError();
 }
 
-template <class T, int G, bool VEC>
-cudaError_t forward_g(const NormArgs &a, cudaStream_t st) {
-    constexpr int NT = G > NM_NT ? G : NM_NT;
-    constexpr int smem = RowQueue<T, G, VEC, NT, FWD_DEPTH, 1>::BYTES;
-    return launch(norm_rows_k<T, G, VEC>, a, blocks(a.rows, NT / G, NT > NM_NT ? 1 : 3), NT, smem, st);
+// The group and the elements per thread for a width: as few threads as hold it
+// with MOST elements each, a warp at least.  Forward MOST is 64 bytes with VEC
+// (16384 x 4096 bf16: 45 us, with 32 bytes 49); backward 16 elements, whose
+// gain and sums take 48 registers (65536 x 1024 bf16: 32 elements take 95 us, 16 73).
+template <class T>
+constexpr int forward_vals(bool vec) {
+    return vec ? 64 / (int)sizeof(T) : ONE_VALS;
 }
+template <class T, bool VEC, int MOST, class F>
+cudaError_t with_group(int width, F &&f) {
+    constexpr int N = Vec<T>::N;
+    using std::integral_constant;
+    auto go = [&](auto g, auto vals) { return f(g, vals); };
+    if constexpr (VEC) {
+        if (width <= 32 * N) return go(integral_constant<int, 32>(), integral_constant<int, N>());
+        if (2 * N < MOST && width <= 64 * N) return go(integral_constant<int, 32>(), integral_constant<int, 2 * N>());
+    }
+    integral_constant<int, MOST> vals;
+    if (width <= 32 * MOST) return go(integral_constant<int, 32>(), vals);
+    if (width <= 64 * MOST) return go(integral_constant<int, 64>(), vals);
+    if (width <= 128 * MOST) return go(integral_constant<int, 128>(), vals);
+    if (width <= 256 * MOST) return go(integral_constant<int, 256>(), vals);
+    return go(integral_constant<int, 512>(), vals);
+}
+
 template <class T, bool VEC>
 cudaError_t forward_v(const NormArgs &a, cudaStream_t st) {
-    if (a.width <= 32 * NM_VALS) return forward_g<T, 32, VEC>(a, st);
-    if (a.width <= 64 * NM_VALS) return forward_g<T, 64, VEC>(a, st);
-    if (a.width <= 128 * NM_VALS) return forward_g<T, 128, VEC>(a, st);
-    if (a.width <= 256 * NM_VALS) return forward_g<T, 256, VEC>(a, st);
-    return forward_g<T, 512, VEC>(a, st);
+    return with_group<T, VEC, forward_vals<T>(VEC)>(a.width, [&](auto g, auto vals) {
+        constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT;
+        constexpr int smem = RowQueue<T, G, VALS, VEC, NT, FWD_DEPTH, 1>::BYTES;
+        return launch(norm_rows_k<T, G, VALS, VEC>, a, blocks(a.rows, NT / G, NT > NM_NT ? 1 : 2), NT, smem, st);
+    });
 }
 template <class T>
 cudaError_t forward(const NormArgs &a, cudaStream_t st) {
-    if (a.width > NM_WIDE) {
-        norm_wide_rows_k<T><<<(unsigned)a.rows, NM_NT, 0, st>>>(a);
-        return cudaGetLastError();
-    }
     const bool vec = a.width % Vec<T>::N == 0 && aligned16(a.x, a.x_stride, sizeof(T)) && aligned16(a.y, a.y_stride, sizeof(T));
+    if (a.width > 512 * forward_vals<T>(vec)) {
+        if (!vec) {
+            norm_wide_rows_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a, 0);
+            return cudaGetLastError();
+        }
+        const int keep = std::min(a.width / Vec<T>::N, WIDE_KEEP / 16);
+        return launch(norm_wide_rows_k<T, true>, a, a.rows, WIDE_NT, keep * 16, st, keep);
+    }
     return vec ? forward_v<T, true>(a, st) : forward_v<T, false>(a, st);
 }
 
 // The partial rows of dgain and dbias: what `blocks` gives at most.
 int partial_rows(int64_t rows) { return (int)std::min<int64_t>(std::max<int64_t>(rows, 1), PARTIAL_ROWS); }
 
-template <class T, int G, bool VEC>
-cudaError_t backward_g(const NormGradArgs &a, bool params, int64_t &parts, cudaStream_t st) {
-    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
-    parts = blocks(a.rows, GROUPS, NT > 256 ? 1 : 2);
-    const int join = params && GROUPS > 1 ? 2 * a.width * (int)sizeof(float) : 0;
-    const int smem = std::max(join, RowQueue<T, G, VEC, NT, BWD_DEPTH, 2>::BYTES);
-    return params ? launch(norm_backward_k<T, G, VEC, true>, a, parts, NT, smem, st)
-                  : launch(norm_backward_k<T, G, VEC, false>, a, parts, NT, smem, st);
-}
 template <class T, bool VEC>
 cudaError_t backward_v(const NormGradArgs &a, bool params, int64_t &parts, cudaStream_t st) {
-    if (a.width <= 32 * NM_VALS) return backward_g<T, 32, VEC>(a, params, parts, st);
-    if (a.width <= 64 * NM_VALS) return backward_g<T, 64, VEC>(a, params, parts, st);
-    if (a.width <= 128 * NM_VALS) return backward_g<T, 128, VEC>(a, params, parts, st);
-    if (a.width <= 256 * NM_VALS) return backward_g<T, 256, VEC>(a, params, parts, st);
-    return backward_g<T, 512, VEC>(a, params, parts, st);
+    return with_group<T, VEC, ONE_VALS>(a.width, [&](auto g, auto vals) {
+        constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
+        parts = blocks(a.rows, GROUPS, NT > NM_NT ? 1 : 2);
+        const int join = params && GROUPS > 1 ? GROUPS * 2 * a.width * (int)sizeof(float) : 0;
+        const int smem = std::max(join, RowQueue<T, G, VALS, VEC, NT, BWD_DEPTH, 2>::BYTES);
+        return params ? launch(norm_backward_k<T, G, VALS, VEC, true>, a, parts, NT, smem, st)
+                      : launch(norm_backward_k<T, G, VALS, VEC, false>, a, parts, NT, smem, st);
+    });
 }
 
 template <class T>
 cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
     const bool params = a.dgain || a.dbias;
     int64_t parts = 0;
-    if (a.rows && a.width <= NM_WIDE) {
-        bool vec = a.width % Vec<T>::N == 0 && aligned16(a.x, a.x_stride, sizeof(T)) &&
-                   aligned16(a.dy, a.dy_stride, sizeof(T)) && (!a.dx || aligned16(a.dx, a.dx_stride, sizeof(T)));
+    const bool vec = a.width % Vec<T>::N == 0 && aligned16(a.x, a.x_stride, sizeof(T)) &&
+                       aligned16(a.dy, a.dy_stride, sizeof(T)) && (!a.dx || aligned16(a.dx, a.dx_stride, sizeof(T)));
+    if (a.rows && a.width <= 512 * ONE_VALS) {
         cudaError_t e = vec ? backward_v<T, true>(a, params, parts, st) : backward_v<T, false>(a, params, parts, st);
         if (e != cudaSuccess) return e;
     } else if (a.rows) {
         // The parameters' sums first: dx may be the array of dy.
         if (params) {
             parts = std::min<int64_t>(a.rows, 64);
-            norm_wide_param_k<T><<<dim3((unsigned)((a.width + NM_NT - 1) / NM_NT), (unsigned)parts), NM_NT, 0, st>>>(a);
+            const unsigned cols = (unsigned)((a.width / (vec ? Vec<T>::N : 1) + NM_NT - 1) / NM_NT);
+            if (vec)
+                norm_wide_param_k<T, true><<<dim3(cols, (unsigned)parts), NM_NT, 0, st>>>(a);
+            else
+                norm_wide_param_k<T, false><<<dim3(cols, (unsigned)parts), NM_NT, 0, st>>>(a);
             if (cudaError_t e = cudaGetLastError()) return e;
         }
-        if (a.dx) norm_wide_dx_k<T><<<(unsigned)a.rows, NM_NT, 0, st>>>(a);
-        if (cudaError_t e = cudaGetLastError()) return e;
+        if (a.dx && vec) {
+            const int keep = std::min(a.width / Vec<T>::N, WIDE_KEEP / 16);
+            if (cudaError_t e = launch(norm_wide_dx_k<T, true>, a, a.rows, WIDE_NT, 2 * keep * 16, st, keep)) return e;
+        } else if (a.dx) {
+            norm_wide_dx_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a, 0);
+            if (cudaError_t e = cudaGetLastError()) return e;
+        }
     }
     if (params) {
         norm_param_sum_k<<<(unsigned)((2 * (int64_t)a.width + 31) / 32), 32 * SUM_LANES, 0, st>>>(a, (int)parts);
