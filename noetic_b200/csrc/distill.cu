@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_c
                 continue;
             }
             const SoftSums sums = row_sums<NT>(sh, turn, log_cs, rank, scale, true, [&] { now.share(a.inv_t, a.n, log_q); });
-            write_loss(turn - 1);
+            if (log_cs) write_loss(turn - 1);
             const float log_s = logf(sums.s), log2_s = log_s * LOG2E;
             const bool empty = sums.m == -INFINITY && sums.s == 0.0f;  // a student that can say nothing
             float kl = 0.0f;

@@ -134,7 +134,7 @@ __device__ __noinline__ void exact_top(const T *row, int e0, int e1, int top, To
 // ranked by counting.  Where more groups or candidates reach it than fit (many
 // equal logits, an order that gives one thread all the large ones), exact_top
 // takes over.
-template <class T, int NT>
+template <class T, int NT, bool FINE>
 __device__ __forceinline__ SoftSums logprobs_part(const LogprobsArgs &a, const T *row, RowSpan span, int v0, int v1, bool first,
                                                   bool last, int slot_shift, const TopTeam &w) {
     constexpr int N = Vec<T>::N;
@@ -144,7 +144,7 @@ __device__ __forceinline__ SoftSums logprobs_part(const LogprobsArgs &a, const T
     const float scale = a.scale;
     SoftSums sums;
     float tmax = -INFINITY, gmax = -INFINITY;
-    const int batches = stream_sums<T, NT, LP_U, true>(body, v0, v1, tid, scale, sums, [&](int b, float bm) {
+    const int batches = stream_sums<T, NT, LP_U, true, false, FINE>(body, v0, v1, tid, scale, sums, [&](int b, float bm) {
         if (a.top) {
             gmax = (b & ((1 << slot_shift) - 1)) == 0 ? bm : fmaxf(gmax, bm);
             w.group_max[(b >> slot_shift) * NT + tid] = gmax;
@@ -155,7 +155,7 @@ __device__ __forceinline__ SoftSums logprobs_part(const LogprobsArgs &a, const T
     auto single = [&](int e) {
         const float z = to_f32(row[e]);
         sums.raise(z, scale);
-        sums.add(z, scale);
+        sums.template add<FINE>(z, scale);
         tmax = fmaxf(tmax, z);
     };
     if (tid < n_head) single(tid);
@@ -266,16 +266,16 @@ __device__ __forceinline__ void no_token_row(const LogprobsArgs &a, int64_t r) {
 }
 
 // The row's results from its whole sums and its best keys.
-template <int NT>
+template <int NT, bool FINE>
 __device__ __forceinline__ void write_row(const LogprobsArgs &a, int64_t r, const SoftSums &sums, float z_target,
                                           const uint64_t *best) {
     const int tid = threadIdx.x % NT;
-    const float log_s = logf(sums.s);
+    const float log_s = sums.log_sum<FINE>(), total = sums.s + sums.n;
     const bool empty = sums.m == -INFINITY && sums.s == 0.0f;
     if (tid == 0) {
         if (a.logprob) a.logprob[r] = empty ? -INFINITY : (z_target - sums.m) * a.inv_t - log_s;
         if (a.entropy) {
-            const float h = log_s - LN2 * (sums.t / sums.s);
+            const float h = log_s - LN2 * (sums.t / total);
             a.entropy[r] = empty || h < 0.0f ? 0.0f : h;
         }
         if (a.stats) {
@@ -333,8 +333,8 @@ __global__ void __launch_bounds__(32 * WARP_ROWS, 4) token_logprobs_warp_k(Logpr
         w.word = w.hits + w.hit_cap;
     }
     const RowSpan span = row_span(row, a.vocab);
-    SoftSums sums = logprobs_part<T, 32>(a, row, span, 0, span.n_vec, true, true, slot_shift, w);
-    write_row<32>(a, r, warp_join<true>(sums, a.scale), z_target, w.best);
+    SoftSums sums = logprobs_part<T, 32, false>(a, row, span, 0, span.n_vec, true, true, slot_shift, w);
+    write_row<32, false>(a, r, warp_join<true>(sums, a.scale), z_target, w.best);
 }
 
 // ---------------------------------------------------------------- long rows: a block or a cluster each
@@ -369,7 +369,7 @@ __device__ __forceinline__ int count_above(const uint64_t *list, int n, uint64_t
     return lo;
 }
 
-template <class T, int NT>
+template <class T, int NT, bool FINE>
 __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_k(LogprobsArgs a, int log_cs, int slot_shift) {
     extern __shared__ float group_max[];
     __shared__ LogprobsShared<NT> sh;
@@ -396,19 +396,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_k(LogprobsArgs a
     w.hit_cap = HITS;
     const RowSpan span = row_span(row, a.vocab);
     const int v0 = (int)((int64_t)span.n_vec * rank >> log_cs), v1 = (int)((int64_t)span.n_vec * (rank + 1) >> log_cs);
-    SoftSums sums = logprobs_part<T, NT>(a, row, span, v0, v1, rank == 0, rank == cs - 1, slot_shift, w);
-    sums = block_join<NT>(sums, a.scale, sh.warps);
+    SoftSums sums = logprobs_part<T, NT, FINE>(a, row, span, v0, v1, rank == 0, rank == cs - 1, slot_shift, w);
+    sums = block_join<NT, FINE>(sums, a.scale, sh.warps);
 
     if (cs > 1) {
         namespace cg = cooperative_groups;
         cg::cluster_group cluster = cg::this_cluster();
-        if (tid == 0) sh.part = make_float4(sums.m, sums.s, sums.t, 0.0f);
+        if (tid == 0) sh.part = make_float4(sums.m, sums.s, sums.t, sums.n);
         cluster.sync();
         if (rank == 0) {
             // The parts in their order.
             if (tid < cs) sh.warps[tid] = *cluster.map_shared_rank(&sh.part, tid);
             __syncthreads();
-            sums = join_places<true>(sh.warps, cs, a.scale);
+            sums = join_places<true, FINE>(sh.warps, cs, a.scale);
             if (a.top) {
                 for (int i = tid; i < cs * a.top; i += NT)
                     sh.cand[i] = cluster.map_shared_rank(sh.best, i / a.top)[i % a.top];
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_k(LogprobsArgs a
         cluster.sync();  // the others' shared memory is read until here
         if (rank != 0) return;
     }
-    write_row<NT>(a, r, sums, z_target, sh.best);
+    write_row<NT, FINE>(a, r, sums, z_target, sh.best);
 }
 
 // The gradient, element by element: a CTA takes LP_NT * LP_U vectors of one
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(LP_NT) token_logprobs_backward_k(LogprobsGradA
 
 }  // namespace
 
-template <class T, int NT>
+template <class T, int NT, bool FINE>
 cudaError_t launch_blocks(const LogprobsArgs &a, cudaStream_t st) {
     const int64_t n_vec = a.vocab / Vec<T>::N;
     // A row is split over a cluster while the rows alone leave SMs idle and
@@ -512,7 +512,7 @@ cudaError_t launch_blocks(const LogprobsArgs &a, cudaStream_t st) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cs > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_k<T, NT>, a, log_cs, shift);
+    return cudaLaunchKernelEx(&cfg, token_logprobs_k<T, NT, FINE>, a, log_cs, shift);
 }
 
 template <class T>
@@ -542,7 +542,10 @@ cudaError_t launch_logprobs(const LogprobsArgs &a, cudaStream_t st) {
     // 100 KB 74 and 82; but 1500 rows of 256 KB 96 and 86, 450 rows of 100 KB 23 and 20.
     // With more than 64 alternatives 128 threads' maxima bound them loosely.
     const bool small = a.rows > 592 && a.top <= 64 && (a.rows <= 1184 || n_vec <= 8192);
-    return small ? launch_blocks<T, 128>(a, st) : launch_blocks<T, 256>(a, st);
+    if (small) return launch_blocks<T, 128, false>(a, st);
+    // With few rows the SMs wait for memory, and a single row's log probability
+    // may be all that is looked at: fine sums (one row of 32768 f32: 12.3 us with and without).
+    return a.rows <= 148 ? launch_blocks<T, 256, true>(a, st) : launch_blocks<T, 256, false>(a, st);
 }
 
 template <class T>

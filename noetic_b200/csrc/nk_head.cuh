@@ -181,25 +181,40 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // accuracy.  y is held at -256, where 2^y is 0: masked logits (-infinity, or a
 // type's lowest value) then add 0 to t and not 0 * infinity.  A NaN or
 // +infinity makes s NaN.
+//
+// FINE sums count the logits that equal the maximum in n and leave their ones
+// out of s: beside a sure token (log s near 0) the small rest then keeps its
+// own 24 bits instead of those that 1 + rest leaves it.  It costs two
+// instructions per logit; n is 0 otherwise.
 struct SoftSums {
-    float m = -INFINITY, s = 0.0f, t = 0.0f;
+    float m = -INFINITY, s = 0.0f, t = 0.0f, n = 0.0f;
 
     // Makes v the maximum if it is above the present one.
     __device__ __forceinline__ void raise(float v, float scale) {
         if (v > m) {
-            const float dy = fmaxf((m - v) * scale, -256.0f), f = ex2(dy);
-            t = f * fmaf(dy, s, t);
-            s *= f;
+            const float dy = fmaxf((m - v) * scale, -256.0f), f = ex2(dy), all = s + n;
+            t = f * fmaf(dy, all, t);
+            s = all * f;
+            n = 0.0f;
             m = v;
         }
     }
     // What z is measured from: the maximum, or 0 while there is none.
     __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.0f : m; }
     // One logit (the maximum counts it already).
+    template <bool FINE = false>
     __device__ __forceinline__ void add(float z, float scale) {
         const float y = max_nan((z - base()) * scale, -256.0f), e = ex2(y);
-        s += e;
+        if (FINE && y == 0.0f)
+            n += 1.0f;
+        else
+            s += e;
         t = fmaf(e, y, t);
+    }
+    // log(s + n).
+    template <bool FINE = false>
+    __device__ __forceinline__ float log_sum() const {
+        return FINE ? (float)log((double)n + (double)s) : logf(s);
     }
 };
 
@@ -226,9 +241,10 @@ __device__ __forceinline__ float batch_max(const uint4 (&raw)[U]) {
 }
 
 // Adds U vectors to a thread's sums (t only with ENT); returns their maximum.
-// Two partial sums each, one of a vector's even elements and one of its odd
+// (Masked logits are not counted in n: y is not 0 there, as base is 0 while
+// there is no maximum.)  Two partial sums each, one of a vector's even elements and one of its odd
 // ones, in pairs of f32 operations.
-template <class T, int U, bool ENT>
+template <class T, int U, bool ENT, bool FINE = false>
 __device__ __forceinline__ float add_batch(const uint4 (&raw)[U], SoftSums &a, float scale) {
     const float bm = batch_max<T, U>(raw);
     a.raise(bm, scale);
@@ -243,9 +259,13 @@ __device__ __forceinline__ float add_batch(const uint4 (&raw)[U], SoftSums &a, f
         for (int i = 0; i < Vec<T>::N; i += 2) {
             float2 y = mul2(add2(make_float2(x[i], x[i + 1]), nb), sc);
             if (ENT) y = make_float2(max_nan(y.x, -256.0f), max_nan(y.y, -256.0f));
-            const float2 e = make_float2(ex2(y.x), ex2(y.y));
-            s = add2(s, e);
+            float2 e = make_float2(ex2(y.x), ex2(y.y));
             if (ENT) t = fma2(e, y, t);
+            if (FINE) {
+                a.n += (y.x == 0.0f ? 1.0f : 0.0f) + (y.y == 0.0f ? 1.0f : 0.0f);
+                e = make_float2(y.x == 0.0f ? 0.0f : e.x, y.y == 0.0f ? 0.0f : e.y);
+            }
+            s = add2(s, e);
         }
     }
     a.s += s.x + s.y;
@@ -253,14 +273,14 @@ __device__ __forceinline__ float add_batch(const uint4 (&raw)[U], SoftSums &a, f
     return bm;
 }
 // The same for those of U vectors that lie at v, v + NT, ... below v1.
-template <class T, int NT, int U, bool ENT>
+template <class T, int NT, int U, bool ENT, bool FINE = false>
 __device__ __forceinline__ float add_some(const uint4 (&raw)[U], int v, int v1, SoftSums &a, float scale) {
     float bm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (v + u * NT < v1) {
             const uint4 one[1] = {raw[u]};
-            bm = fmaxf(bm, add_batch<T, 1, ENT>(one, a, scale));
+            bm = fmaxf(bm, add_batch<T, 1, ENT, FINE>(one, a, scale));
         }
     return bm;
 }
@@ -270,7 +290,7 @@ __device__ __forceinline__ float add_some(const uint4 (&raw)[U], int v, int v1, 
 // way while the present ones are added.  each(batch, maximum) is called for
 // every U.  Returns the number of these.  With MASK a last batch that is not
 // full counts its missing vectors as masked ones.
-template <class T, int NT, int U, bool ENT, bool MASK = false, class F>
+template <class T, int NT, int U, bool ENT, bool MASK = false, bool FINE = false, class F>
 __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int tid, float scale, SoftSums &sums, F &&each) {
     uint4 next[U];
     int batch = 0, v = v0 + tid;
@@ -297,7 +317,7 @@ __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int ti
         const int now = v;
         v += NT * U;
         fetch();
-        each(batch, MASK || now + (U - 1) * NT < v1 ? add_batch<T, U, ENT>(raw, sums, scale) : add_some<T, NT, U, ENT>(raw, now, v1, sums, scale));
+        each(batch, MASK || now + (U - 1) * NT < v1 ? add_batch<T, U, ENT, FINE>(raw, sums, scale) : add_some<T, NT, U, ENT, FINE>(raw, now, v1, sums, scale));
     }
     return batch;
 }
@@ -306,6 +326,14 @@ __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int ti
 // wait until at most N groups of this thread are still on their way.
 __device__ __forceinline__ void copy_async16(void *to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+// The first `bytes` of 16, the rest zeros (none of it is read); 4 bytes.
+__device__ __forceinline__ void copy_async16_part(void *to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_async4(void *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -320,8 +348,8 @@ __device__ __forceinline__ float warp_max1(float v) {
     return r;
 }
 
-// A warp's sums joined, in all its lanes (t only with ENT).
-template <bool ENT>
+// A warp's sums joined, in all its lanes (t only with ENT, n only with FINE).
+template <bool ENT, bool FINE = false>
 __device__ __forceinline__ SoftSums warp_join(SoftSums a, float scale) {
     SoftSums r;
     r.m = warp_max1(a.m);
@@ -329,11 +357,12 @@ __device__ __forceinline__ SoftSums warp_join(SoftSums a, float scale) {
     if (a.m != -INFINITY) a.raise(r.m, scale);
     r.s = warp_sum(a.s);
     if (ENT) r.t = warp_sum(a.t);
+    if (FINE) r.n = warp_sum(a.n);
     return r;
 }
 
 // The parts that n <= 32 places hold, joined in a fixed order in every lane of a warp.
-template <bool ENT>
+template <bool ENT, bool FINE = false>
 __device__ __forceinline__ SoftSums join_places(const float4 *places, int n, float scale) {
     SoftSums a;
     const int lane = threadIdx.x & 31;
@@ -342,18 +371,19 @@ __device__ __forceinline__ SoftSums join_places(const float4 *places, int n, flo
         a.m = p.x;
         a.s = p.y;
         a.t = p.z;
+        a.n = p.w;
     }
-    return warp_join<ENT>(a, scale);
+    return warp_join<ENT, FINE>(a, scale);
 }
 
 // Every thread's sums joined over a block of NT with one barrier; all threads
 // get the result.  `places` holds a float4 per warp and must not be in use.
-template <int NT>
+template <int NT, bool FINE>
 __device__ __forceinline__ SoftSums block_join(const SoftSums &a, float scale, float4 *places) {
-    const SoftSums w = warp_join<true>(a, scale);
-    if ((threadIdx.x & 31) == 0) places[threadIdx.x >> 5] = make_float4(w.m, w.s, w.t, 0.0f);
+    const SoftSums w = warp_join<true, FINE>(a, scale);
+    if ((threadIdx.x & 31) == 0) places[threadIdx.x >> 5] = make_float4(w.m, w.s, w.t, w.n);
     __syncthreads();
-    return join_places<true>(places, NT / 32, scale);
+    return join_places<true, FINE>(places, NT / 32, scale);
 }
 
 }  // namespace nk

@@ -11,6 +11,11 @@
 // as long as a row costs its threads few instructions beside its elements:
 // hence the f32 operations in pairs, and 64 bytes of a row to a thread where it has them.
 // Rows too wide for that take one block per row and read it again from L2.
+//
+// Rows that do not start on 16-byte boundaries (an odd width) are read in the
+// same 16-byte units of memory.  Where a row starts in its first unit repeats
+// every 8 rows at most, so a group that steps by a multiple of 8 rows sees
+// every row start at the same place, and each thread's columns stay the same.
 
 #include <algorithm>
 
@@ -22,7 +27,7 @@ namespace nk {
 namespace {
 
 constexpr int NM_NT = 256;
-constexpr int ONE_VALS = 16;  // of a thread, backward and where no vectors fit
+constexpr int BWD_VALS = 16;  // elements of a thread
 constexpr int FWD_DEPTH = 4;  // rows on their way to each group
 constexpr int BWD_DEPTH = 3;
 constexpr int PARTIAL_ROWS = 1024;  // most partial sums of dgain and dbias
@@ -70,177 +75,237 @@ __device__ __forceinline__ float2 group_sum2(float2 v, float2 *red) {
     return v;
 }
 
-// Where a thread's elements lie: with VEC, VALS / N vectors of N elements, G
-// vectors apart; else single elements, G apart.
-template <class T, int G, int VALS, bool VEC>
+// Where a group's elements lie: 16-byte units of N elements, unit l * G + lane
+// the l-th of a thread.  With EDGE the row starts `shift` elements into unit 0
+// and may end inside the last one.
+template <class T, int G, int VALS, bool EDGE>
 struct Place {
-    static constexpr int N = VEC ? Vec<T>::N : 1;
-    static constexpr int LOADS = VALS / N;
-    static __device__ __forceinline__ int at(int lane, int l) { return (l * G + lane) * N; }
+    static constexpr int N = Vec<T>::N, LOADS = VALS / N, H = VALS / 2, C = N / 2;  // pairs in all, in a unit
+    int lane, width, shift, units, last;  // last: the load that holds the last unit
+
+    __device__ __forceinline__ Place(const void *row, int lane_, int width_) : lane(lane_), width(width_) {
+        shift = EDGE ? (int)((uintptr_t)row & 15) / (int)sizeof(T) : 0;
+        units = (shift + width + N - 1) / N;
+        last = (units - 1) / G;
+    }
+    __device__ __forceinline__ int unit(int l) const { return l * G + lane; }
+    __device__ __forceinline__ int column(int l) const { return unit(l) * N - shift; }
+    __device__ __forceinline__ bool has(int l) const { return unit(l) < units; }
+    // Whether one of the group's units of load l may reach out of the row; whether
+    // this thread's does.
+    __device__ __forceinline__ bool edgy(int l) const { return EDGE && (l == 0 || l == last); }
+    __device__ __forceinline__ bool on_edge(int l) const { return edgy(l) && (unit(l) == 0 || unit(l) == units - 1); }
+    __device__ __forceinline__ bool inside(int col) const { return (unsigned)col < (unsigned)width; }
+    // A pair of elements, 0 where it is not in the row.
+    __device__ __forceinline__ float2 keep(int l, int i, float2 v) const {
+        if (!has(l)) return make_float2(0.0f, 0.0f);
+        if (edgy(l)) v = make_float2(inside(column(l) + i) ? v.x : 0.0f, inside(column(l) + i + 1) ? v.y : 0.0f);
+        return v;
+    }
 };
 
-// The rows that a thread will work on next, ARRAYS of them at a time: with VEC
+// The rows that a thread will work on next, ARRAYS of them at a time: its units
 // in its own places of a ring in shared memory, DEPTH rows on their way by
-// asynchronous copies (no barrier: a thread reads only what it copied); else
-// one row in registers, which the next push overwrites.
-template <class T, int G, int VALS, bool VEC, int NT, int DEPTH, int ARRAYS>
+// asynchronous copies (no barrier: a thread reads only what it copied).
+template <class T, int G, int VALS, bool EDGE, int NT, int DEPTH, int ARRAYS>
 struct RowQueue {
-    using P = Place<T, G, VALS, VEC>;
-    static constexpr int AHEAD = VEC ? DEPTH : 1;
-    static constexpr int BYTES = VEC ? DEPTH * ARRAYS * P::LOADS * NT * 16 : 0;
-    T next[ARRAYS][VEC ? 1 : VALS];
+    using P = Place<T, G, VALS, EDGE>;
+    static constexpr int BYTES = DEPTH * ARRAYS * P::LOADS * NT * 16;
     uint4 *ring;  // [DEPTH][ARRAYS][LOADS][NT], from this thread's place on
     int slot = 0;
 
     __device__ __forceinline__ uint4 *place(int at, int k) const { return ring + (at * ARRAYS + k) * P::LOADS * NT; }
-    __device__ __forceinline__ void push(const T *const (&rows)[ARRAYS], int at, int lane, int width, bool real) {
+    // Sends for one row of each array (for nothing, if it is not `real`).
+    __device__ __forceinline__ void push(const P &p, const T *const (&rows)[ARRAYS], int at, bool real, bool first_row) {
 #pragma unroll
-        for (int k = 0; k < ARRAYS; ++k) {
-            const T *row = rows[k] + lane * P::N;
+        for (int k = 0; k < ARRAYS; ++k)
 #pragma unroll
             for (int l = 0; l < P::LOADS; ++l) {
-                const bool in = real && P::at(lane, l) < width;
-                if constexpr (VEC) {
-                    if (in) copy_async16(place(at, k) + l * NT, row + l * G * P::N);
+                if (!real || !p.has(l)) continue;
+                uint4 *to = place(at, k) + l * NT;
+                const T *from = rows[k] + p.column(l);
+                if (!EDGE) {
+                    copy_async16(to, from);
+                } else if (l > 0 || p.lane > 0 || p.shift == 0) {
+                    copy_async16_part(to, from, min(16, (p.width - p.column(l)) * (int)sizeof(T)));
+                } else if (p.units > 1 && !first_row) {
+                    // The unit that the row starts inside: by words, of which the first
+                    // may begin with the element before (there is one, but for the first row).
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        if ((w + 1) * 4 > p.shift * (int)sizeof(T)) copy_async4((char *)to + 4 * w, (const char *)from + 4 * w);
                 } else {
-                    next[k][l] = in ? row[l * G] : from_f32<T>(0.0f);
+                    for (int i = p.shift; i < min(P::N, p.shift + p.width); ++i) ((T *)to)[i] = from[i];
                 }
             }
-        }
-        if constexpr (VEC) copy_commit();
+        copy_commit();
     }
     // Waits for the row pushed first, which is then the present one.
-    __device__ __forceinline__ void wait() const {
-        if constexpr (VEC) copy_wait<DEPTH - 1>();
-    }
+    __device__ __forceinline__ void wait() const { copy_wait<DEPTH - 1>(); }
     // Done with it: the next push goes to its slot.
-    __device__ __forceinline__ void pop() { slot = slot + 1 == AHEAD ? 0 : slot + 1; }
-    // Chunk c of the present row: a vector's elements (VEC) or two of the single
-    // ones, in pairs; zeros beyond the width.
-    static constexpr int CHUNK = VEC ? P::N / 2 : 1;
-    __device__ __forceinline__ void get(int k, int c, int lane, int width, bool real, float2 (&x)[CHUNK]) const {
-        if constexpr (VEC) {
-            float v[P::N];
-            unpack<T>(real && P::at(lane, c) < width ? place(slot, k)[c * NT] : make_uint4(0, 0, 0, 0), v);
+    __device__ __forceinline__ void pop() { slot = slot + 1 == DEPTH ? 0 : slot + 1; }
+    // Load l of the present row, in pairs; zeros outside the row.
+    __device__ __forceinline__ void get(const P &p, int k, int l, bool real, float2 (&x)[P::C]) const {
+        float v[P::N];
+        unpack<T>(real && p.has(l) ? place(slot, k)[l * NT] : make_uint4(0, 0, 0, 0), v);
+        if (EDGE && l == 0) {
 #pragma unroll
-            for (int i = 0; i < CHUNK; ++i) x[i] = make_float2(v[2 * i], v[2 * i + 1]);
-        } else {
-            x[0] = make_float2(to_f32(next[k][2 * c]), to_f32(next[k][2 * c + 1]));
+            for (int i = 0; i < P::N; ++i) v[i] = p.inside(p.column(0) + i) ? v[i] : 0.0f;
         }
-    }
-    // A pair of chunk c, 0 where it is beyond the width.
-    static __device__ __forceinline__ float2 keep(int c, int lane, int width, float2 v) {
-        if constexpr (VEC) return P::at(lane, c) < width ? v : make_float2(0.0f, 0.0f);
-        return make_float2(P::at(lane, 2 * c) < width ? v.x : 0.0f, P::at(lane, 2 * c + 1) < width ? v.y : 0.0f);
+#pragma unroll
+        for (int i = 0; i < P::C; ++i) x[i] = make_float2(v[2 * i], v[2 * i + 1]);
     }
 };
 
-// Chunk c of a thread's part of a row, as RowQueue::get has it.
-template <class T, int G, int VALS, bool VEC, int CHUNK>
-__device__ __forceinline__ void store_chunk(T *row, int c, int lane, int width, const float2 (&x)[CHUNK]) {
-    using P = Place<T, G, VALS, VEC>;
-    if constexpr (VEC) {
-        if (P::at(lane, c) >= width) return;
-        float v[P::N];
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            v[2 * i] = x[i].x;
-            v[2 * i + 1] = x[i].y;
-        }
-        store16(row + P::at(lane, c), pack<T>(v));
+template <class P, class T>
+__device__ __forceinline__ void store_unit(const P &p, T *row, int col, bool whole, uint4 v) {
+    if (whole) {
+        store16(row + col, v);
     } else {
-        if (P::at(lane, 2 * c) < width) row[P::at(lane, 2 * c)] = from_f32<T>(x[0].x);
-        if (P::at(lane, 2 * c + 1) < width) row[P::at(lane, 2 * c + 1)] = from_f32<T>(x[0].y);
+        const T *x = (const T *)&v;
+#pragma unroll
+        for (int i = 0; i < P::N; ++i)
+            if (p.inside(col + i)) row[col + i] = x[i];
     }
 }
 
-// A thread's part of an f32 vector of the width (null: `other`); 0 beyond it.
-template <class T, int G, int VALS, bool VEC>
-__device__ __forceinline__ void column_part(const float *p, float other, int lane, int width, float2 (&x)[VALS / 2]) {
-    using P = Place<T, G, VALS, VEC>;
-    auto one = [&](int k) {
-        const int e = P::at(lane, k / P::N) + k % P::N;
-        return e < width ? (p ? p[e] : other) : 0.0f;
-    };
+// The 16 bytes that start d elements into a, b.
+template <class T>
+__device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int d) {
+    uint32_t o[5];
+    switch (d * (int)sizeof(T) / 4) {
+        case 0: o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x; break;
+        case 1: o[0] = a.y, o[1] = a.z, o[2] = a.w, o[3] = b.x, o[4] = b.y; break;
+        case 2: o[0] = a.z, o[1] = a.w, o[2] = b.x, o[3] = b.y, o[4] = b.z; break;
+        default: o[0] = a.w, o[1] = b.x, o[2] = b.y, o[3] = b.z, o[4] = b.w; break;
+    }
+    if (sizeof(T) == 2 && (d & 1)) {
 #pragma unroll
-    for (int k = 0; k < VALS / 2; ++k) x[k] = make_float2(one(2 * k), one(2 * k + 1));
+        for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(o[i], o[i + 1], 16);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Elements e and e + step of a row, 0 beyond the width.
-template <class T>
-__device__ __forceinline__ float2 pair_of(const T *row, int e, int step, int width) {
-    return make_float2(e < width ? to_f32(row[e]) : 0.0f, e + step < width ? to_f32(row[e + step]) : 0.0f);
+// A thread's part x(l) of a row that starts at `row`.  `same`: in the same place
+// of a unit as the rows read.  Otherwise the group hands the units over in
+// `stage` ([LOADS][NT] units, from the group's place on), where each thread
+// reads the two that its unit of the row written is cut from.  The caller's
+// reductions keep the stage of one row apart from the next.
+template <int G, int NT, class P, class T, class F>
+__device__ __forceinline__ void store_row(const P &p, T *row, bool same, uint4 *stage, F &&x) {
+    if (same) {
+#pragma unroll
+        for (int l = 0; l < P::LOADS; ++l)
+            if (p.has(l)) store_unit(p, row, p.column(l), !p.on_edge(l), x(l));
+        return;
+    }
+#pragma unroll
+    for (int l = 0; l < P::LOADS; ++l)
+        if (p.has(l)) stage[l * NT + p.lane] = x(l);
+    if constexpr (G == 32)
+        __syncwarp();
+    else
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / G), "n"(G) : "memory");
+    const int shift = (int)((uintptr_t)row & 15) / (int)sizeof(T), d = p.shift - shift;
+    const int units = (shift + p.width + P::N - 1) / P::N, first = d < 0 ? -1 : 0;
+    auto staged = [&](int u) {
+        return u >= 0 && u < p.units ? stage[u / G * NT + u % G] : make_uint4(0, 0, 0, 0);
+    };
+#pragma unroll
+    for (int l = 0; l < P::LOADS; ++l) {
+        const int u = p.unit(l);
+        if (u < units)
+            store_unit(p, row, u * P::N - shift, u > 0 && u < units - 1,
+                       shifted<T>(staged(u + first), staged(u + first + 1), d < 0 ? d + P::N : d));
+    }
+}
+
+template <class T, int C>
+__device__ __forceinline__ uint4 pack_pairs(const float2 (&x)[C]) {
+    float v[2 * C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        v[2 * i] = x[i].x;
+        v[2 * i + 1] = x[i].y;
+    }
+    return pack<T>(v);
+}
+
+// A thread's part of an f32 vector of the width (null: `other`); 0 outside it.
+template <class P>
+__device__ __forceinline__ void column_part(const P &p, const float *v, float other, float2 (&x)[P::H]) {
+    auto one = [&](int j) {
+        const int e = p.column(j / P::N) + j % P::N;
+        return p.inside(e) ? (v ? v[e] : other) : 0.0f;
+    };
+#pragma unroll
+    for (int j = 0; j < P::H; ++j) x[j] = make_float2(one(2 * j), one(2 * j + 1));
 }
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // ---------------------------------------------------------------- forward
-template <class T, int G, int VALS, bool VEC>
-__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_rows_k(NormArgs a) {
-    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G, H = VALS / 2;
-    using Queue = RowQueue<T, G, VALS, VEC, NT, FWD_DEPTH, 1>;
-    constexpr int C = Queue::CHUNK;
+template <class T, int G, int VALS, bool EDGE>
+__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_rows_k(NormArgs a, int same) {
+    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
+    using P = Place<T, G, VALS, EDGE>;
+    constexpr int C = P::C;
     __shared__ float red[2][32];
     extern __shared__ uint4 ring[];
-    const int lane = threadIdx.x % G, group = threadIdx.x / G;
+    const int group = threadIdx.x / G;
     const float inv_n = 1.0f / (float)a.width;
-    float2 gain[H], bias[H];
-    Queue queue;
+    float2 gain[P::H], bias[P::H];
+    RowQueue<T, G, VALS, EDGE, NT, FWD_DEPTH, 1> queue;
     queue.ring = ring + threadIdx.x;
+    uint4 *stage = ring + queue.BYTES / 16 + group * G;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
+    const P p((const T *)a.x + r * a.x_stride, threadIdx.x % G, a.width);
     auto push = [&](int64_t q, int at) {
         const T *const rows[1] = {(const T *)a.x + q * a.x_stride};
-        queue.push(rows, at, lane, a.width, q < a.rows);
+        queue.push(p, rows, at, q < a.rows, q == 0);
     };
-    for (int k = 0; k < Queue::AHEAD; ++k) push(r + k * step, k);
-    if constexpr (VEC) {
-        column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
-        column_part<T, G, VALS, VEC>(a.bias, 0.0f, lane, a.width, bias);
-    }
+    for (int k = 0; k < FWD_DEPTH; ++k) push(r + k * step, k);
+    column_part(p, a.gain, 1.0f, gain);
+    column_part(p, a.bias, 0.0f, bias);
     // Every group takes the same number of turns: the reductions hold barriers.
     const int turns = (int)((a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step);
     for (int i = 0; i < turns; ++i, r += step) {
         const bool real = r < a.rows;
-        float2 x[H];
+        float2 x[P::H];
         queue.wait();
 #pragma unroll
-        for (int c = 0; c < H / C; ++c) {
+        for (int l = 0; l < P::LOADS; ++l) {
             float2 v[C];
-            queue.get(0, c, lane, a.width, real, v);
+            queue.get(p, 0, l, real, v);
 #pragma unroll
-            for (int j = 0; j < C; ++j) x[c * C + j] = v[j];
+            for (int j = 0; j < C; ++j) x[l * C + j] = v[j];
         }
-        push(r + Queue::AHEAD * step, queue.slot);
+        push(r + FWD_DEPTH * step, queue.slot);
         queue.pop();
         float mean = 0.0f;
         if (!a.rms) {
             float2 s = x[0];
 #pragma unroll
-            for (int j = 1; j < H; ++j) s = add2(s, x[j]);
+            for (int j = 1; j < P::H; ++j) s = add2(s, x[j]);
             mean = group_sum<G>(s.x + s.y, red[0]) * inv_n;
         }
         float2 v = both(0.0f);
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            x[j] = Queue::keep(j / C, lane, a.width, add2(x[j], both(-mean)));
+        for (int j = 0; j < P::H; ++j) {
+            x[j] = p.keep(j / C, 2 * (j % C), add2(x[j], both(-mean)));
             v = fma2(x[j], x[j], v);
         }
         const float rstd = 1.0f / sqrtf(fmaf(group_sum<G>(v.x + v.y, red[1]), inv_n, a.eps));
         if (G > 32 && a.rms) __syncthreads();  // red[1] again in the next turn
         if (!real) continue;
-        if constexpr (!VEC) {  // from L1 for every row: the loads' sixteen registers are taken
-            column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
-            column_part<T, G, VALS, VEC>(a.bias, 0.0f, lane, a.width, bias);
-        }
+        store_row<G, NT>(p, (T *)a.y + r * a.y_stride, same, stage, [&](int l) {
+            float2 z[C];
 #pragma unroll
-        for (int c = 0; c < H / C; ++c) {
-            float2 v[C];
-#pragma unroll
-            for (int j = 0; j < C; ++j) v[j] = fma2(mul2(x[c * C + j], both(rstd)), gain[c * C + j], bias[c * C + j]);
-            store_chunk<T, G, VALS, VEC>((T *)a.y + r * a.y_stride, c, lane, a.width, v);
-        }
-        if (lane == 0) {
+            for (int j = 0; j < C; ++j) z[j] = fma2(mul2(x[l * C + j], both(rstd)), gain[l * C + j], bias[l * C + j]);
+            return pack_pairs<T>(z);
+        });
+        if (p.lane == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
         }
@@ -327,95 +392,85 @@ __global__ void __launch_bounds__(WIDE_NT) norm_wide_rows_k(NormArgs a, int keep
 
 // ---------------------------------------------------------------- backward
 // dx of the rows, and with PARAMS this block's sums for dgain and dbias: its
-// groups' registers joined in shared memory in their order, one row of
-// the workspace per block.  The row is unpacked twice, once for the sums and
-// once for dx: it waits in shared memory (without VEC in L1), not in registers.
-template <class T, int G, int VALS, bool VEC, bool PARAMS>
-__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_backward_k(NormGradArgs a) {
-    using P = Place<T, G, VALS, VEC>;
-    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G, H = VALS / 2;
-    using Queue = RowQueue<T, G, VALS, VEC, NT, BWD_DEPTH, 2>;
-    constexpr int C = Queue::CHUNK;
+// groups' registers joined in shared memory in their order, one row of the
+// workspace per block.  The row is unpacked twice, once for the sums and once
+// for dx: it waits in shared memory, not in registers.
+template <class T, int G, int VALS, bool EDGE, bool PARAMS>
+__global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_backward_k(NormGradArgs a, int same) {
+    constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
+    using P = Place<T, G, VALS, EDGE>;
+    constexpr int C = P::C;
     __shared__ float2 red[2][32];
     extern __shared__ uint4 ring[];
     float *joined = (float *)ring;  // [GROUPS][2][width], when the rows are done
-    const int lane = threadIdx.x % G, group = threadIdx.x / G;
+    const int group = threadIdx.x / G;
     const float inv_n = 1.0f / (float)a.width;
-    float2 gain[H], dg[H], db[H];
+    float2 gain[P::H], dg[P::H], db[P::H];
 #pragma unroll
-    for (int j = 0; j < H; ++j) dg[j] = db[j] = both(0.0f);
-    Queue queue;
+    for (int j = 0; j < P::H; ++j) dg[j] = db[j] = both(0.0f);
+    RowQueue<T, G, VALS, EDGE, NT, BWD_DEPTH, 2> queue;
     queue.ring = ring + threadIdx.x;
+    uint4 *stage = ring + queue.BYTES / 16 + group * G;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
+    const P p((const T *)a.x + r * a.x_stride, threadIdx.x % G, a.width);
     auto push = [&](int64_t q, int at) {
         const T *const rows[2] = {(const T *)a.x + q * a.x_stride, (const T *)a.dy + q * a.dy_stride};
-        queue.push(rows, at, lane, a.width, q < a.rows);
+        queue.push(p, rows, at, q < a.rows, q == 0);
     };
     float next_mean, next_rstd;
     auto stats = [&](int64_t q) {
         next_mean = q < a.rows && !a.rms ? a.mean[q] : 0.0f;
         next_rstd = q < a.rows ? a.rstd[q] : 0.0f;
     };
-    for (int k = 0; k < Queue::AHEAD; ++k) push(r + k * step, k);
+    for (int k = 0; k < BWD_DEPTH; ++k) push(r + k * step, k);
     stats(r);
-    if constexpr (VEC) column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
+    column_part(p, a.gain, 1.0f, gain);
+    if (PARAMS) pdl_trigger();  // norm_param_sum_k comes up, and waits for this grid's end
     const int turns = (int)((a.rows - (int64_t)blockIdx.x * GROUPS + step - 1) / step);
     for (int i = 0; i < turns; ++i, r += step) {
         const bool real = r < a.rows;
         const float mean = next_mean, rstd = next_rstd;
         queue.wait();
-        if constexpr (!VEC) column_part<T, G, VALS, VEC>(a.gain, 1.0f, lane, a.width, gain);
         stats(r + step);
         float2 sc = both(0.0f), sch = sc;
-        // Beyond the width dy and the gain are 0, and h does not count.
+        // Outside the row dy and the gain are 0, and h does not count.
 #pragma unroll
-        for (int q = 0; q < H / C; ++q) {
+        for (int l = 0; l < P::LOADS; ++l) {
             float2 h[C], c[C];
-            queue.get(0, q, lane, a.width, real, h);
-            queue.get(1, q, lane, a.width, real, c);
+            queue.get(p, 0, l, real, h);
+            queue.get(p, 1, l, real, c);
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
                 if (PARAMS) {
-                    dg[q * C + j] = fma2(c[j], h[j], dg[q * C + j]);
-                    db[q * C + j] = add2(db[q * C + j], c[j]);
+                    dg[l * C + j] = fma2(c[j], h[j], dg[l * C + j]);
+                    db[l * C + j] = add2(db[l * C + j], c[j]);
                 }
-                c[j] = mul2(c[j], gain[q * C + j]);
+                c[j] = mul2(c[j], gain[l * C + j]);
                 sc = add2(sc, c[j]);
                 sch = fma2(c[j], h[j], sch);
             }
         }
-        if constexpr (!VEC) push(r + step, 0);
         if (a.dx) {
             const float2 s = group_sum2<G>(make_float2(sc.x + sc.y, sch.x + sch.y), red[i & 1]);
             const float mc = a.rms ? 0.0f : s.x * inv_n, mch = s.y * inv_n;
-            T *to = (T *)a.dx + r * a.dx_stride;
-            if (real) {
-#pragma unroll
-                for (int q = 0; q < H / C; ++q) {
+            if (real)
+                store_row<G, NT>(p, (T *)a.dx + r * a.dx_stride, same, stage, [&](int l) {
                     float2 h[C], c[C];
-                    if constexpr (VEC) {
-                        queue.get(0, q, lane, a.width, real, h);
-                        queue.get(1, q, lane, a.width, real, c);
-                    } else {  // from L1
-                        h[0] = pair_of((const T *)a.x + r * a.x_stride, P::at(lane, 2 * q), G, a.width);
-                        c[0] = pair_of((const T *)a.dy + r * a.dy_stride, P::at(lane, 2 * q), G, a.width);
-                    }
+                    queue.get(p, 0, l, real, h);
+                    queue.get(p, 1, l, real, c);
 #pragma unroll
                     for (int j = 0; j < C; ++j) {
                         h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
-                        c[j] = fma2(c[j], gain[q * C + j], both(-mc));
+                        c[j] = fma2(c[j], gain[l * C + j], both(-mc));
                         h[j] = mul2(both(rstd), fma2(h[j], both(-mch), c[j]));
                     }
-                    store_chunk<T, G, VALS, VEC>(to, q, lane, a.width, h);
-                }
-            }
+                    return pack_pairs<T>(h);
+                });
         }
-        if constexpr (VEC) {
-            push(r + Queue::AHEAD * step, queue.slot);
-            queue.pop();
-        }
+        push(r + BWD_DEPTH * step, queue.slot);
+        queue.pop();
     }
     if constexpr (PARAMS) {
         float *w = a.workspace + (int64_t)blockIdx.x * 2 * a.width;
@@ -423,8 +478,8 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm
         if (GROUPS > 1) __syncthreads();
 #pragma unroll
         for (int j = 0; j < VALS; ++j) {
-            const int e = P::at(lane, j / P::N) + j % P::N;
-            if (e >= a.width) continue;
+            const int e = p.column(j / P::N) + j % P::N;
+            if (!p.inside(e)) continue;
             to[e] = j & 1 ? dg[j / 2].y : dg[j / 2].x;
             to[a.width + e] = j & 1 ? db[j / 2].y : db[j / 2].x;
         }
@@ -538,6 +593,7 @@ __global__ void __launch_bounds__(NM_NT) norm_wide_param_k(NormGradArgs a) {
 constexpr int SUM_LANES = 16;
 __global__ void __launch_bounds__(32 * SUM_LANES) norm_param_sum_k(NormGradArgs a, int parts) {
     __shared__ float sums[SUM_LANES][32];
+    pdl_wait();
     const int col = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t e = (int64_t)blockIdx.x * 32 + col, n = 2 * (int64_t)a.width;
     float s = 0.0f;
@@ -558,10 +614,15 @@ __global__ void __launch_bounds__(32 * SUM_LANES) norm_param_sum_k(NormGradArgs 
 
 // ---------------------------------------------------------------- launches
 bool aligned16(const void *p, int64_t stride, int es) { return ((uintptr_t)p & 15) == 0 && stride * es % 16 == 0; }
+// Whether every row of b starts at the same place of a 16-byte unit as that of a.
+bool same_place(const void *a, int64_t a_stride, const void *b, int64_t b_stride, int es) {
+    return (((uintptr_t)a ^ (uintptr_t)b) & 15) == 0 && (a_stride - b_stride) * es % 16 == 0;
+}
 
-// Blocks that the GPU holds at once, at most one per turn of rows.
+// Blocks that the GPU holds at once, at most one per turn of rows; a multiple
+// of 8 where they take several turns, for rows that start anywhere.
 int64_t blocks(int64_t rows, int groups, int per_sm) {
-    return std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, 148 * per_sm));
+    return std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, 148 * per_sm / 8 * 8));
 }
 
 template <class Args, class... More>
@@ -574,82 +635,95 @@ cudaError_t launch(void (*kern)(Args, More...), const Args &a, int64_t grid, int
     return cudaGetLastError();
 }
 
-// The group and the elements per thread for a width: as few threads as hold it
-// with MOST elements each, a warp at least.  Forward MOST is 64 bytes with VEC
-// (16384 x 4096 bf16: 45 us, with 32 bytes 49); backward 16 elements, whose
-// gain and sums take 48 registers (65536 x 1024 bf16: 32 elements take 95 us, 16 73).
+// The group and the elements per thread for a number of 16-byte units: as few
+// threads as hold it with MOST elements each, a warp at least.  Forward MOST is
+// 64 bytes (16384 x 4096 bf16: 45 us, with 32 bytes 49); backward 16 elements,
+// whose gain and sums take 48 registers (65536 x 1024 bf16: 32 elements take 95 us, 16 73).
 template <class T>
-constexpr int forward_vals(bool vec) {
-    return vec ? 64 / (int)sizeof(T) : ONE_VALS;
+constexpr int fwd_vals() {
+    return 64 / (int)sizeof(T);
 }
-template <class T, bool VEC, int MOST, class F>
-cudaError_t with_group(int width, F &&f) {
-    constexpr int N = Vec<T>::N;
+template <class T, int MOST, class F>
+cudaError_t with_group(int units, F &&f) {
+    constexpr int N = Vec<T>::N, L = MOST / N;
     using std::integral_constant;
-    auto go = [&](auto g, auto vals) { return f(g, vals); };
-    if constexpr (VEC) {
-        if (width <= 32 * N) return go(integral_constant<int, 32>(), integral_constant<int, N>());
-        if (2 * N < MOST && width <= 64 * N) return go(integral_constant<int, 32>(), integral_constant<int, 2 * N>());
-    }
+    if (units <= 32) return f(integral_constant<int, 32>(), integral_constant<int, N>());
+    if (2 < L && units <= 64) return f(integral_constant<int, 32>(), integral_constant<int, 2 * N>());
     integral_constant<int, MOST> vals;
-    if (width <= 32 * MOST) return go(integral_constant<int, 32>(), vals);
-    if (width <= 64 * MOST) return go(integral_constant<int, 64>(), vals);
-    if (width <= 128 * MOST) return go(integral_constant<int, 128>(), vals);
-    if (width <= 256 * MOST) return go(integral_constant<int, 256>(), vals);
-    return go(integral_constant<int, 512>(), vals);
+    integral_constant<int, (L > 3 ? 3 * N : MOST)> fewer;
+    if (units <= 32 * L) return f(integral_constant<int, 32>(), vals);
+    if (L > 3 && units <= 64 * 3) return f(integral_constant<int, 64>(), fewer);
+    if (units <= 64 * L) return f(integral_constant<int, 64>(), vals);
+    if (L > 3 && units <= 128 * 3) return f(integral_constant<int, 128>(), fewer);
+    if (units <= 128 * L) return f(integral_constant<int, 128>(), vals);
+    if (L > 3 && units <= 256 * 3) return f(integral_constant<int, 256>(), fewer);
+    if (units <= 256 * L) return f(integral_constant<int, 256>(), vals);
+    return f(integral_constant<int, 512>(), vals);
+}
+// The units that a row can cover.
+template <class T, bool EDGE>
+int units_of(int width) {
+    return (width + (EDGE ? 2 : 1) * (Vec<T>::N - 1)) / Vec<T>::N;
 }
 
-template <class T, bool VEC>
-cudaError_t forward_v(const NormArgs &a, cudaStream_t st) {
-    return with_group<T, VEC, forward_vals<T>(VEC)>(a.width, [&](auto g, auto vals) {
+template <class T, bool EDGE>
+cudaError_t forward_g(const NormArgs &a, int same, cudaStream_t st) {
+    return with_group<T, fwd_vals<T>()>(units_of<T, EDGE>(a.width), [&](auto g, auto vals) {
         constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT;
-        constexpr int smem = RowQueue<T, G, VALS, VEC, NT, FWD_DEPTH, 1>::BYTES;
-        return launch(norm_rows_k<T, G, VALS, VEC>, a, blocks(a.rows, NT / G, NT > NM_NT ? 1 : 2), NT, smem, st);
+        const int smem = RowQueue<T, G, VALS, EDGE, NT, FWD_DEPTH, 1>::BYTES + (same ? 0 : NT * VALS * (int)sizeof(T));
+        return launch(norm_rows_k<T, G, VALS, EDGE>, a, blocks(a.rows, NT / G, NT > NM_NT ? 1 : 2), NT, smem, st, same);
     });
 }
 template <class T>
 cudaError_t forward(const NormArgs &a, cudaStream_t st) {
-    const bool vec = a.width % Vec<T>::N == 0 && aligned16(a.x, a.x_stride, sizeof(T)) && aligned16(a.y, a.y_stride, sizeof(T));
-    if (a.width > 512 * forward_vals<T>(vec)) {
-        if (!vec) {
-            norm_wide_rows_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a, 0);
-            return cudaGetLastError();
-        }
-        const int keep = std::min(a.width / Vec<T>::N, WIDE_KEEP / 16);
-        return launch(norm_wide_rows_k<T, true>, a, a.rows, WIDE_NT, keep * 16, st, keep);
+    constexpr int N = Vec<T>::N, ES = sizeof(T);
+    const bool whole = a.width % N == 0 && aligned16(a.x, a.x_stride, ES);
+    const bool same = same_place(a.x, a.x_stride, a.y, a.y_stride, ES);
+    const int most = 512 * fwd_vals<T>() / N;
+    if (whole && same && a.width / N <= most) return forward_g<T, false>(a, 1, st);
+    if (units_of<T, true>(a.width) <= most) return forward_g<T, true>(a, same, st);
+    if (!whole || !same) {
+        norm_wide_rows_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a, 0);
+        return cudaGetLastError();
     }
-    return vec ? forward_v<T, true>(a, st) : forward_v<T, false>(a, st);
+    const int keep = std::min(a.width / N, WIDE_KEEP / 16);
+    return launch(norm_wide_rows_k<T, true>, a, a.rows, WIDE_NT, keep * 16, st, keep);
 }
 
 // The partial rows of dgain and dbias: what `blocks` gives at most.
 int partial_rows(int64_t rows) { return (int)std::min<int64_t>(std::max<int64_t>(rows, 1), PARTIAL_ROWS); }
 
-template <class T, bool VEC>
-cudaError_t backward_v(const NormGradArgs &a, bool params, int64_t &parts, cudaStream_t st) {
-    return with_group<T, VEC, ONE_VALS>(a.width, [&](auto g, auto vals) {
+template <class T, bool EDGE>
+cudaError_t backward_g(const NormGradArgs &a, int same, bool params, int64_t &parts, cudaStream_t st) {
+    return with_group<T, BWD_VALS>(units_of<T, EDGE>(a.width), [&](auto g, auto vals) {
         constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
         parts = blocks(a.rows, GROUPS, NT > NM_NT ? 1 : 2);
         const int join = params && GROUPS > 1 ? GROUPS * 2 * a.width * (int)sizeof(float) : 0;
-        const int smem = std::max(join, RowQueue<T, G, VALS, VEC, NT, BWD_DEPTH, 2>::BYTES);
-        return params ? launch(norm_backward_k<T, G, VALS, VEC, true>, a, parts, NT, smem, st)
-                      : launch(norm_backward_k<T, G, VALS, VEC, false>, a, parts, NT, smem, st);
+        const int smem = std::max(join, RowQueue<T, G, VALS, EDGE, NT, BWD_DEPTH, 2>::BYTES + (same ? 0 : NT * VALS * (int)sizeof(T)));
+        return params ? launch(norm_backward_k<T, G, VALS, EDGE, true>, a, parts, NT, smem, st, same)
+                      : launch(norm_backward_k<T, G, VALS, EDGE, false>, a, parts, NT, smem, st, same);
     });
 }
 
 template <class T>
 cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
+    constexpr int N = Vec<T>::N, ES = sizeof(T);
     const bool params = a.dgain || a.dbias;
     int64_t parts = 0;
-    const bool vec = a.width % Vec<T>::N == 0 && aligned16(a.x, a.x_stride, sizeof(T)) &&
-                       aligned16(a.dy, a.dy_stride, sizeof(T)) && (!a.dx || aligned16(a.dx, a.dx_stride, sizeof(T)));
-    if (a.rows && a.width <= 512 * ONE_VALS) {
-        cudaError_t e = vec ? backward_v<T, true>(a, params, parts, st) : backward_v<T, false>(a, params, parts, st);
-        if (e != cudaSuccess) return e;
+    const bool whole = a.width % N == 0 && aligned16(a.x, a.x_stride, ES);
+    const bool like = same_place(a.x, a.x_stride, a.dy, a.dy_stride, ES);
+    const bool same = !a.dx || same_place(a.x, a.x_stride, a.dx, a.dx_stride, ES);
+    const int most = 512 * BWD_VALS / N;
+    if (a.rows && like && whole && same && a.width / N <= most) {
+        if (cudaError_t e = backward_g<T, false>(a, 1, params, parts, st)) return e;
+    } else if (a.rows && like && units_of<T, true>(a.width) <= most) {
+        if (cudaError_t e = backward_g<T, true>(a, same, params, parts, st)) return e;
     } else if (a.rows) {
+        const bool vec = whole && like && same;
         // The parameters' sums first: dx may be the array of dy.
         if (params) {
             parts = std::min<int64_t>(a.rows, 64);
-            const unsigned cols = (unsigned)((a.width / (vec ? Vec<T>::N : 1) + NM_NT - 1) / NM_NT);
+            const unsigned cols = (unsigned)((a.width / (vec ? N : 1) + NM_NT - 1) / NM_NT);
             if (vec)
                 norm_wide_param_k<T, true><<<dim3(cols, (unsigned)parts), NM_NT, 0, st>>>(a);
             else
@@ -657,7 +731,7 @@ cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
             if (cudaError_t e = cudaGetLastError()) return e;
         }
         if (a.dx && vec) {
-            const int keep = std::min(a.width / Vec<T>::N, WIDE_KEEP / 16);
+            const int keep = std::min(a.width / N, WIDE_KEEP / 16);
             if (cudaError_t e = launch(norm_wide_dx_k<T, true>, a, a.rows, WIDE_NT, 2 * keep * 16, st, keep)) return e;
         } else if (a.dx) {
             norm_wide_dx_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a, 0);
@@ -665,8 +739,7 @@ cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
         }
     }
     if (params) {
-        norm_param_sum_k<<<(unsigned)((2 * (int64_t)a.width + 31) / 32), 32 * SUM_LANES, 0, st>>>(a, (int)parts);
-        return cudaGetLastError();
+        return pdl_launch(norm_param_sum_k, dim3((unsigned)((2 * (int64_t)a.width + 31) / 32)), dim3(32 * SUM_LANES), 0, st, a, (int)parts);
     }
     return cudaSuccess;
 }

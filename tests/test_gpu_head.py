@@ -385,6 +385,60 @@ def test_distill_over_sizes(gpu, torch, dtype, t_dtype, rows, V, pad, shift):
     assert torch.equal(same, dz) and torch.equal(ls, loss)
 
 
+@pytest.mark.parametrize("rows,V,dtype,K", [(3700, 4200, "f32", 20), (7500, 4997, "f32", 70), (1900, 17600, "f32", 5),
+                                            (3600, 8800, "bf16", 33), (1000, 70001, "bf16", 64)])
+def test_distill_of_many_rows(gpu, torch, rows, V, dtype, K):
+    # More rows than the GPU works on at once, among them rows without entries, side by
+    # side, at the ends and scattered, and rows of weight 0.
+    z, _ = _matrix(torch, rows, V, dtype, seed=rows)
+    ids = torch.randint(0, V, (rows, K), device="cuda", dtype=torch.int32)
+    for gone in (slice(0, 1), slice(5, 12), slice(rows - 3, rows), torch.randperm(rows, device="cuda")[:rows // 6]):
+        ids[gone] = NONE
+    t = torch.randn(rows, K, device="cuda")
+    w = torch.rand(rows, device="cuda") + 0.5
+    w[20:30] = 0.0
+    w[torch.randperm(rows, device="cuda")[:rows // 10]] = 0.0
+    loss, dz = _distill(gpu, torch, z, ids, t, 1.5, w, 0.5, dtype, "f32")
+    alone = _distill(gpu, torch, z, ids, t, 1.5, w, 0.5, dtype, "f32", grad=False)[0]
+    for r in range(0, rows, 500):
+        b = slice(r, r + 500)
+        ref, tol, rdz, ztol = _ref_distill(torch, z[b], ids[b], t[b], 1.5, w[b], 0.5)
+        for got in (loss, alone):
+            assert ((got[b].double() - ref).abs() <= tol).all()
+        assert ((dz[b].double() - rdz).abs() <= ztol + _out_tol(torch, dtype, rdz)).all()
+    assert (dz[w == 0] == 0).all()
+    _, same = _distill(gpu, torch, z, ids, t, 1.5, w, 0.5, dtype, "f32", dz=z)
+    assert torch.equal(same, dz)
+
+
+@pytest.mark.parametrize("rows,V,dtype,top", [(5000, 300, "f32", 5), (3000, 4100, "bf16", 20), (1100, 9001, "f16", 40),
+                                              (1500, 20000, "f32", 70), (700, 40000, "bf16", 3)])
+def test_logprobs_of_many_rows(gpu, torch, rows, V, dtype, top):
+    z, _ = _matrix(torch, rows, V, dtype, seed=rows)
+    t = torch.randint(0, V, (rows,), device="cuda", dtype=torch.int32)
+    t[torch.randperm(rows, device="cuda")[:rows // 5]] = NONE
+    out = _logprobs(gpu, torch, z, t, 0.9, top, dtype)
+    for r in range(0, rows, 500):
+        b = slice(r, r + 500)
+        _check_logprobs(torch, {k: v[b] for k, v in out.items()}, z[b], t[b], 0.9, top)
+
+
+def test_logprobs_of_sure_tokens_keep_their_digits(gpu, torch):
+    # log p = -log(1 + rest) of a rest down to 1e-5: with few rows the rest is summed by
+    # itself, so the result is good to a relative 1e-5 at 16384 terms (each exponential 4 U
+    # and 4 |y| U, the sum below 112 U, the logarithm's rounding), not to 2^-24 absolutely.
+    for V, gap in [(16384, 12.0), (16384, 20.0), (300, 9.0), (40001, 16.0)]:
+        z = torch.randn(3, V, device="cuda")
+        z[:, 7] = z.amax() + gap
+        t = torch.full((3,), 7, device="cuda", dtype=torch.int32)
+        out = _logprobs(gpu, torch, z, t, 1.0, 2, "f32")
+        zd = z.double()
+        rest = torch.exp(zd - zd[:, 7:8])
+        rest[:, 7] = 0
+        want = -torch.log1p(rest.sum(-1))
+        assert ((out["logprob"].double() - want).abs() <= 1e-5 * want.abs()).all()
+
+
 def test_distill_special_rows(gpu, torch):
     z = torch.randn(6, 500, device="cuda")
     z[0] = NAN                       # a row without entries is not read
