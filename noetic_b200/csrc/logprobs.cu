@@ -15,7 +15,7 @@ namespace {
 
 constexpr int LP_NT = 256;
 constexpr int TOP_MAX = 128;
-constexpr int LP_LOG_U = 2, LP_U = 1 << LP_LOG_U;
+constexpr int LP_U = 4;  // vectors of a thread in the gradient
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAXIMA = 256;  // that a warp takes the bound on the alternatives from
 
@@ -120,10 +120,16 @@ __device__ __noinline__ void exact_top(const T *row, int e0, int e1, int top, To
     team_sync<NT>();
 }
 
+// Vectors that a thread of a team takes at a time.
+template <int NT>
+constexpr int log_batch() {
+    return NT == 32 ? 2 : 3;
+}
+
 // One team's part of one row: the softmax sums, and with a.top its best
-// alternatives in w.best.  The part is read once: a thread takes LP_U 16-byte
-// vectors at a time, the next ones on their way, raises its running maximum by
-// theirs and adds their exponentials.
+// alternatives in w.best.  The part is read once: a thread takes a batch of
+// 16-byte vectors at a time, raises its running maximum by theirs and adds
+// their exponentials.
 //
 // Alternatives.  Threads keep the maximum of each group of their vectors in
 // shared memory.  The top-th largest of MAXIMA of these (a block: of its
@@ -144,7 +150,7 @@ __device__ __forceinline__ SoftSums logprobs_part(const LogprobsArgs &a, const T
     const float scale = a.scale;
     SoftSums sums;
     float tmax = -INFINITY, gmax = -INFINITY;
-    const int batches = stream_sums<T, NT, LP_U, true, false, FINE>(body, v0, v1, tid, scale, sums, [&](int b, float bm) {
+    const int batches = stream_sums<T, NT, 1 << log_batch<NT>(), true, false, FINE>(body, v0, v1, tid, scale, sums, [&](int b, float bm) {
         if (a.top) {
             gmax = (b & ((1 << slot_shift) - 1)) == 0 ? bm : fmaxf(gmax, bm);
             w.group_max[(b >> slot_shift) * NT + tid] = gmax;
@@ -220,7 +226,7 @@ __device__ __forceinline__ SoftSums logprobs_part(const LogprobsArgs &a, const T
         if (tid < n_tail) offer(to_f32(row[a.vocab - span.tail + tid]), a.vocab - span.tail + tid);
     }
     team_sync<NT>();
-    const int log_group = LP_LOG_U + slot_shift, n_hits = (int)w.word[1];
+    const int log_group = log_batch<NT>() + slot_shift, n_hits = (int)w.word[1];
     if (n_hits <= w.hit_cap) {
         for (int i = tid; i < (n_hits << log_group); i += NT) {
             const uint32_t hit = w.hits[i >> log_group];
@@ -497,7 +503,8 @@ cudaError_t launch_blocks(const LogprobsArgs &a, cudaStream_t st) {
     int log_cs = 0;
     while ((1 << log_cs) < MAX_CLUSTER && a.rows << log_cs < 148 && n_vec >> (log_cs + 1) >= NT) ++log_cs;
     const int cs = 1 << log_cs;
-    const int64_t batches = ((n_vec + cs - 1) / cs + NT * LP_U - 1) / (NT * LP_U);
+    constexpr int step = NT << log_batch<NT>();
+    const int64_t batches = ((n_vec + cs - 1) / cs + step - 1) / step;
     int shift = 0;
     while ((batches >> shift) >= LP_SLOTS) ++shift;
     const size_t smem = a.top ? ((batches >> shift) + 1) * NT * sizeof(float) : 0;
@@ -525,7 +532,8 @@ cudaError_t launch_logprobs(const LogprobsArgs &a, cudaStream_t st) {
     // 160, of 64 KB 257 and 216; 1024 rows of 32 KB 27 and 22.
     if (n_vec <= 2048 && a.rows >= std::max<int64_t>(512, n_vec)) {
         int shift = 0;
-        while (((n_vec + 32 * LP_U - 1) / (32 * LP_U) + (1 << shift) - 1) >> shift > MAXIMA / 32) ++shift;
+        constexpr int step = 32 << log_batch<32>();
+        while (((n_vec + step - 1) / step + (1 << shift) - 1) >> shift > MAXIMA / 32) ++shift;
         const int smem = WARP_ROWS * warp_team_bytes(a.top);
         auto kern = token_logprobs_warp_k<T>;
         if (smem > 48 << 10) {

@@ -286,38 +286,32 @@ __device__ __forceinline__ float add_some(const uint4 (&raw)[U], int v, int v1, 
 }
 
 // Adds the vectors v0 <= v < v1 of `body` to the sums of a team of NT threads,
-// of which this is thread `tid`, U to a thread at a time, the next U on their
-// way while the present ones are added.  each(batch, maximum) is called for
-// every U.  Returns the number of these.  With MASK a last batch that is not
-// full counts its missing vectors as masked ones.
+// of which this is thread `tid`, U to a thread at a time.  each(batch, maximum)
+// is called for every U; returns the number of these.  With MASK a last batch
+// that is not full counts its missing vectors as masked ones.  (Other warps'
+// work covers the loads: fetching the next batch ahead measured 213 us a pass
+// over 4096 rows of 131072 bf16, eight vectors at a time without it 207.)
 template <class T, int NT, int U, bool ENT, bool MASK = false, bool FINE = false, class F>
 __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int tid, float scale, SoftSums &sums, F &&each) {
-    uint4 next[U];
     int batch = 0, v = v0 + tid;
     const uint4 *at = (const uint4 *)body + v;
-    auto fetch = [&] {
+    for (; v < v1; ++batch) {
+        uint4 raw[U];
         if (v + (U - 1) * NT < v1) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) next[u] = load16_rw(at + u * NT);
+            for (int u = 0; u < U; ++u) raw[u] = load16_rw(at + u * NT);
+            each(batch, add_batch<T, U, ENT, FINE>(raw, sums, scale));
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (v + u * NT < v1)
-                    next[u] = load16_rw(at + u * NT);
+                    raw[u] = load16_rw(at + u * NT);
                 else if (MASK)
-                    next[u] = masked16<T>();
+                    raw[u] = masked16<T>();
+            each(batch, MASK ? add_batch<T, U, ENT, FINE>(raw, sums, scale) : add_some<T, NT, U, ENT, FINE>(raw, v, v1, sums, scale));
         }
         at += U * NT;
-    };
-    fetch();
-    for (; v < v1; ++batch) {
-        uint4 raw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = next[u];
-        const int now = v;
-        v += NT * U;
-        fetch();
-        each(batch, MASK || now + (U - 1) * NT < v1 ? add_batch<T, U, ENT, FINE>(raw, sums, scale) : add_some<T, NT, U, ENT, FINE>(raw, now, v1, sums, scale));
+        v += U * NT;
     }
     return batch;
 }
