@@ -12,8 +12,9 @@
  *   - Entry points whose name ends in _device take device pointers and a CUDA
  *     stream (cudaStream_t, NULL for the legacy default stream), do not
  *     synchronise or allocate, and can be captured into a CUDA graph after a
- *     first call on that device.  They run on the device that owns their first
- *     pointer, whichever is current; the stream has to belong to it.
+ *     first call on that device.  They run on the device that owns their arrays,
+ *     whichever is current (managed memory alone: the current one); the stream
+ *     has to belong to it.
  *     The others take contiguous host arrays and run on `device`.
  *   - dtype is an nk_dtype.  Sums, maxima and statistics are f32 at least;
  *     results are rounded once, on the way out.
@@ -25,10 +26,11 @@
  *     those).
  *   - Results do not depend on scheduling: the same call gives the same bits.
  *   - NK_ERR_INVALID: a null array with a non-zero size, a pointer that is not
- *     device memory, a misaligned one, a stride below the width, a size beyond
- *     the limits (rows <= 2^26, vocab and width <= 2^30, rows * stride <=
- *     2^37), a temperature outside [1e-30, 1e30], an eps that is negative or not
- *     finite, an output that overlaps an input other than as said below.
+ *     device memory or not on the same device as the others, a misaligned one, a
+ *     stride below the width, a size beyond the limits (rows <= 2^26, vocab and
+ *     width <= 2^30, rows * stride <= 2^37), a temperature outside [1e-30, 1e30],
+ *     an eps that is negative or not finite; on the device also an output that
+ *     overlaps an input, other than as said below, or another output.
  */
 #ifndef NOETIC_HEAD_H
 #define NOETIC_HEAD_H
@@ -97,17 +99,18 @@ nk_status nk_token_logprobs_backward(const void *logits, int dtype, uint64_t row
 /* Distillation from a teacher's top logits.  A row of the teacher is n_teacher
  * (<= NK_MAX_TEACHER) ids and their logits or log probabilities (they are
  * normalised here: q = softmax(teacher / temperature) over the row's entries;
- * an id that is no token, or a logit of -infinity, is no entry).  With p the student's softmax(logits /
- * temperature) over the vocabulary,
+ * an id that is no token, or a logit of -infinity, is no entry).  With p the
+ * student's softmax(logits / temperature) over the vocabulary,
  *   loss[r] = temperature^2 sum_i q_i (log q_i - log p[id_i])
  *   dlogits[r][j] = grad_scale row_weight[r] temperature (p_j - sum_{i: id_i = j} q_i)
  * which is the gradient of grad_scale sum_r row_weight[r] loss[r].  row_weight
  * null: 1.  dlogits null: the loss alone; loss null: the gradient alone.  The
  * logits are read once for both.  A row without entries is not read: its loss
  * and gradient are 0.  A row of weight 0 has gradient 0.  Where the student has
- * no logit above -infinity the loss is infinity and the gradient 0.  An id may stand in a
- * row more than once (its shares add up).  dlogits has the type of the logits
- * and can be the same array with the same stride. */
+ * no logit above -infinity the loss is infinity and the gradient 0.  An id may
+ * stand in a row more than once (its shares add up).  dlogits has the type of
+ * the logits and can be the same array with the same stride.  The temperature is
+ * limited to [1e-4, 1e4] (the loss comes with an error of about 1e-7 temperature^2). */
 nk_status nk_distill_device(const void *logits, int dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
                             const uint32_t *teacher_ids, const void *teacher_logits, int teacher_dtype,
                             uint32_t n_teacher, float temperature, float *loss, const float *row_weight,
@@ -135,8 +138,8 @@ nk_status nk_layer_norm(const void *x, int dtype, uint64_t rows, uint64_t width,
  * the same stride; accumulate != 0 adds to dgain and dbias instead of setting
  * them (dx is set).  The sums over rows are split and joined in a fixed order
  * through `workspace` (of nk_layer_norm_backward_workspace bytes, 16-byte
- * aligned; not needed without dgain and dbias): calls that overlap on the GPU, replays of
- * captured graphs among them, need a workspace each. */
+ * aligned; not needed without dgain and dbias): calls that overlap on the GPU,
+ * replays of captured graphs among them, need a workspace each. */
 nk_status nk_layer_norm_backward_workspace(uint64_t rows, uint64_t width, uint64_t *bytes);
 nk_status nk_layer_norm_backward_device(const void *x, int dtype, uint64_t rows, uint64_t width, uint64_t x_stride,
                                         const float *gain, const float *mean, const float *rstd, int rms,

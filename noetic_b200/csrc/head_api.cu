@@ -89,18 +89,45 @@ bool overlap(const void *a, uint64_t as, const void *b, uint64_t bs, uint64_t ro
     return at < width * es || at + width * es > row;
 }
 
-// The device that owns the call's first array, current for the call.
+// An array from its first byte to its last.
+struct Span {
+    const void *p;
+    uint64_t bytes;
+};
+Span matrix_span(const void *p, uint64_t rows, uint64_t width, uint64_t stride, int es) {
+    return {p, rows ? ((rows - 1) * stride + width) * es : 0};
+}
+// No output shares a byte with another one or with an input.  (Matrices among
+// each other: `overlap`.)
+void check_apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+    auto meet = [](const Span &a, const Span &b) {
+        return a.p && b.p && a.bytes && b.bytes && (uintptr_t)a.p < (uintptr_t)b.p + b.bytes && (uintptr_t)b.p < (uintptr_t)a.p + a.bytes;
+    };
+    for (const Span *a = outs.begin(); a != outs.end(); ++a) {
+        for (const Span *b = a + 1; b != outs.end(); ++b) need(!meet(*a, *b), "two outputs overlap");
+        for (const Span &b : ins) need(!meet(*a, b), "an output overlaps an input");
+    }
+}
+
+// The device that owns the call's first array, current for the call.  All of its
+// arrays that are not null have to be there, or managed.
 struct OnDevice {
     int before = -1;
-    explicit OnDevice(const void *p) {
-        cudaPointerAttributes at{};
-        cuda_check(cudaPointerGetAttributes(&at, p), "cudaPointerGetAttributes");
-        need(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, "the arrays must be in device memory");
-        if (at.type == cudaMemoryTypeManaged) return;
-        int now = 0;
+    explicit OnDevice(std::initializer_list<const void *> arrays) {
+        int device = -1, now = 0;
+        for (const void *p : arrays) {
+            if (!p) continue;
+            cudaPointerAttributes at{};
+            cuda_check(cudaPointerGetAttributes(&at, p), "cudaPointerGetAttributes");
+            if (at.type == cudaMemoryTypeManaged) continue;
+            need(at.type == cudaMemoryTypeDevice, "the arrays must be in device memory");
+            if (device < 0) device = at.device;
+            need(device == at.device, "the arrays are on different devices");
+        }
+        if (device < 0) return;
         cuda_check(cudaGetDevice(&now), "cudaGetDevice");
-        if (now != at.device) {
-            cuda_check(cudaSetDevice(at.device), "cudaSetDevice");
+        if (now != device) {
+            cuda_check(cudaSetDevice(device), "cudaSetDevice");
             before = now;
         }
     }
@@ -186,10 +213,12 @@ void check_logprobs_grad(uint64_t rows, const uint32_t *targets, const float *st
 }
 
 void check_distill(uint64_t rows, const uint32_t *ids, const void *teacher, int teacher_dtype, uint32_t n,
-                   const float *loss, const float *row_weight, float grad_scale, const void *dlogits) {
+                   float temperature, const float *loss, const float *row_weight, float grad_scale, const void *dlogits) {
     check_dtype(teacher_dtype);
     need(n <= NK_MAX_TEACHER, "n_teacher is limited to NK_MAX_TEACHER");
     need(std::isfinite(grad_scale), "grad_scale must be finite");
+    // Beyond these temperature^2 leaves the loss no digits of an f32.
+    need(temperature >= 1e-4f && temperature <= 1e4f, "temperature must be within [1e-4, 1e4]");
     if (rows == 0) return;
     need(n == 0 || (ids && teacher), "null teacher arrays");
     need(loss || dlogits, "loss and dlogits are both null");
@@ -235,7 +264,9 @@ nk_status nk_token_logprobs_device(const void *logits, int dtype, uint64_t rows,
         check_logits(logits, dtype, rows, vocab, row_stride, temperature);
         check_logprobs(rows, targets, top, logprob, entropy, stats, top_ids, top_logprobs);
         if (rows == 0 || !(logprob || entropy || stats || top_ids || top_logprobs)) return;
-        OnDevice on(logits);
+        check_apart({{logprob, rows * 4}, {entropy, rows * 4}, {stats, rows * 8}, {top_ids, rows * top * 4}, {top_logprobs, rows * top * 4}},
+                    {matrix_span(logits, rows, vocab, row_stride, elem_size(dtype)), {targets, rows * 4}});
+        OnDevice on({logits, targets, logprob, entropy, stats, top_ids, top_logprobs});
         nk::LogprobsArgs a{};
         a.logits = logits;
         a.rows = (int64_t)rows;
@@ -290,7 +321,9 @@ nk_status nk_token_logprobs_backward_device(const void *logits, int dtype, uint6
         check_aligned(dlogits, elem_size(dtype), "dlogits");
         need(!overlap(logits, row_stride, dlogits, dlogits_stride, rows, vocab, elem_size(dtype)),
              "dlogits overlaps the logits");
-        OnDevice on(logits);
+        check_apart({matrix_span(dlogits, rows, vocab, dlogits_stride, elem_size(dtype))},
+                    {{targets, rows * 4}, {stats, rows * 8}, {entropy, rows * 4}, {g_logprob, rows * 4}, {g_entropy, rows * 4}});
+        OnDevice on({logits, targets, stats, entropy, g_logprob, g_entropy, dlogits});
         nk::LogprobsGradArgs a{};
         a.logits = logits;
         a.dlogits = dlogits;
@@ -336,7 +369,7 @@ nk_status nk_distill_device(const void *logits, int dtype, uint64_t rows, uint64
                             float grad_scale, void *dlogits, uint64_t dlogits_stride, void *stream) {
     return guard("nk_distill", [&] {
         check_logits(logits, dtype, rows, vocab, row_stride, temperature);
-        check_distill(rows, teacher_ids, teacher_logits, teacher_dtype, n_teacher, loss, row_weight, grad_scale, dlogits);
+        check_distill(rows, teacher_ids, teacher_logits, teacher_dtype, n_teacher, temperature, loss, row_weight, grad_scale, dlogits);
         if (rows == 0) return;
         if (dlogits) {
             check_matrix(rows, vocab, dlogits_stride, "dlogits");
@@ -344,7 +377,12 @@ nk_status nk_distill_device(const void *logits, int dtype, uint64_t rows, uint64
             need(!overlap(logits, row_stride, dlogits, dlogits_stride, rows, vocab, elem_size(dtype)),
                  "dlogits overlaps the logits");
         }
-        OnDevice on(logits);
+        const Span z = matrix_span(logits, rows, vocab, row_stride, elem_size(dtype));
+        const Span ids{teacher_ids, rows * n_teacher * 4}, q{teacher_logits, rows * n_teacher * elem_size(teacher_dtype)};
+        check_apart({{loss, rows * 4}}, {z});
+        check_apart({{loss, rows * 4}, matrix_span(dlogits, rows, vocab, dlogits_stride, elem_size(dtype))},
+                    {ids, q, {row_weight, rows * 4}});
+        OnDevice on({logits, n_teacher ? teacher_ids : nullptr, n_teacher ? teacher_logits : nullptr, loss, row_weight, dlogits});
         nk::DistillArgs a{};
         a.logits = logits;
         a.dlogits = dlogits;
@@ -371,7 +409,7 @@ nk_status nk_distill(const void *logits, int dtype, uint64_t rows, uint64_t voca
                      float *loss, const float *row_weight, float grad_scale, void *dlogits, int device) {
     return guard("nk_distill", [&] {
         check_logits(logits, dtype, rows, vocab, vocab, temperature);
-        check_distill(rows, teacher_ids, teacher_logits, teacher_dtype, n_teacher, loss, row_weight, grad_scale, dlogits);
+        check_distill(rows, teacher_ids, teacher_logits, teacher_dtype, n_teacher, temperature, loss, row_weight, grad_scale, dlogits);
         if (rows == 0) return;
         check_ids(teacher_ids, rows * n_teacher, vocab);
         HostCall h(device);
@@ -397,7 +435,10 @@ nk_status nk_layer_norm_device(const void *x, int dtype, uint64_t rows, uint64_t
         check_matrix(rows, width, y_stride, "y");
         if (rows == 0) return;
         need(!overlap(x, x_stride, y, y_stride, rows, width, elem_size(dtype)), "y overlaps x");
-        OnDevice on(x);
+        const int es = elem_size(dtype);
+        check_apart({{mean, rows * 4}, {rstd, rows * 4}}, {matrix_span(x, rows, width, x_stride, es)});
+        check_apart({{mean, rows * 4}, {rstd, rows * 4}, matrix_span(y, rows, width, y_stride, es)}, {{gain, width * 4}, {bias, width * 4}});
+        OnDevice on({x, gain, bias, y, mean, rstd});
         nk::NormArgs a{};
         a.x = x;
         a.y = y;
@@ -464,7 +505,13 @@ nk_status nk_layer_norm_backward_device(const void *x, int dtype, uint64_t rows,
             need(!overlap(dy, dy_stride, dx, dx_stride, rows, width, elem_size(dtype)), "dx overlaps dy");
             need(dx != x && !overlap(x, x_stride, dx, dx_stride, rows, width, elem_size(dtype)), "dx overlaps x");
         }
-        OnDevice on(rows ? x : (const void *)(dgain ? dgain : dbias));
+        const int es = elem_size(dtype);
+        const Span dg{dgain, width * 4}, db{dbias, width * 4}, ws{dgain || dbias ? workspace : nullptr, nk::norm_backward_workspace_bytes((int64_t)rows, (int)width)};
+        check_apart({dg, db, ws}, {matrix_span(x, rows, width, x_stride, es), matrix_span(dy, rows, width, dy_stride, es)});
+        check_apart({dg, db, ws, matrix_span(dx, rows, width, dx_stride, es)}, {{gain, width * 4}, {mean, rows * 4}, {rstd, rows * 4}});
+        const bool some = rows != 0;
+        OnDevice on({some ? x : nullptr, some ? gain : nullptr, some ? mean : nullptr, some ? rstd : nullptr, some ? dy : nullptr,
+                     some ? dx : nullptr, ws.p, dgain, dbias});
         nk::NormGradArgs a{};
         a.x = x;
         a.dy = dy;

@@ -54,21 +54,6 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return warp_sum(lane < (int)(blockDim.x >> 5) ? red[lane] : 0.0f);
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-
-__device__ __forceinline__ float block_max(float v, float *red) {
-    v = warp_max(v);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    __syncthreads();
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    return warp_max(lane < (int)(blockDim.x >> 5) ? red[lane] : -INFINITY);
-}
-
 // Order-preserving u32 of a float; -0 counts as +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);

@@ -30,7 +30,6 @@ constexpr int NM_NT = 256;
 constexpr int BWD_VALS = 16;  // elements of a thread
 constexpr int FWD_DEPTH = 4;  // rows on their way to each group
 constexpr int BWD_DEPTH = 3;
-constexpr int PARTIAL_ROWS = 1024;  // most partial sums of dgain and dbias
 
 // ---------------------------------------------------------------- groups of threads
 // Sum over the G threads of a group, the same in all of them, in a fixed
@@ -189,8 +188,8 @@ __device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int d) {
 // A thread's part x(l) of a row that starts at `row`.  `same`: in the same place
 // of a unit as the rows read.  Otherwise the group hands the units over in
 // `stage` ([LOADS][NT] units, from the group's place on), where each thread
-// reads the two that its unit of the row written is cut from.  The caller's
-// reductions keep the stage of one row apart from the next.
+// reads the two that its unit of the row written is cut from.  (Groups of several
+// warps: the barriers of the caller's reductions keep one row's stage from the next.)
 template <int G, int NT, class P, class T, class F>
 __device__ __forceinline__ void store_row(const P &p, T *row, bool same, uint4 *stage, F &&x) {
     if (same) {
@@ -199,6 +198,7 @@ __device__ __forceinline__ void store_row(const P &p, T *row, bool same, uint4 *
             if (p.has(l)) store_unit(p, row, p.column(l), !p.on_edge(l), x(l));
         return;
     }
+    if (G == 32) __syncwarp();
 #pragma unroll
     for (int l = 0; l < P::LOADS; ++l)
         if (p.has(l)) stage[l * NT + p.lane] = x(l);
@@ -690,8 +690,12 @@ cudaError_t forward(const NormArgs &a, cudaStream_t st) {
     return launch(norm_wide_rows_k<T, true>, a, a.rows, WIDE_NT, keep * 16, st, keep);
 }
 
-// The partial rows of dgain and dbias: what `blocks` gives at most.
-int partial_rows(int64_t rows) { return (int)std::min<int64_t>(std::max<int64_t>(rows, 1), PARTIAL_ROWS); }
+// The partial rows of dgain and dbias, at most: what `blocks` gives, or in rows
+// that are too wide for any group WIDE_PARTS.
+constexpr int WIDE_PARTS = 64;
+int partial_rows(int64_t rows, int width) {
+    return (int)std::min<int64_t>(std::max<int64_t>(rows, 1), width > 512 * BWD_VALS ? WIDE_PARTS : 2 * 148);
+}
 
 template <class T, bool EDGE>
 cudaError_t backward_g(const NormGradArgs &a, int same, bool params, int64_t &parts, cudaStream_t st) {
@@ -722,7 +726,7 @@ cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
         const bool vec = whole && like && same;
         // The parameters' sums first: dx may be the array of dy.
         if (params) {
-            parts = std::min<int64_t>(a.rows, 64);
+            parts = std::min<int64_t>(a.rows, WIDE_PARTS);
             const unsigned cols = (unsigned)((a.width / (vec ? N : 1) + NM_NT - 1) / NM_NT);
             if (vec)
                 norm_wide_param_k<T, true><<<dim3(cols, (unsigned)parts), NM_NT, 0, st>>>(a);
@@ -755,7 +759,7 @@ cudaError_t norm_rows(const NormArgs &a, int dtype, cudaStream_t st) {
 }
 
 size_t norm_backward_workspace_bytes(int64_t rows, int width) {
-    return (size_t)partial_rows(rows) * 2 * (size_t)width * sizeof(float);
+    return (size_t)partial_rows(rows, width) * 2 * (size_t)width * sizeof(float);
 }
 
 cudaError_t norm_backward(const NormGradArgs &a, int dtype, cudaStream_t st) {

@@ -761,6 +761,14 @@ def test_host_memory_is_refused(gpu, torch):
     L = gpu.lib()
     assert L.nk_token_logprobs_device(p, 0, 2, 8, 8, None, 1.0, 0, None, _p(d), None, None, None, None) == gpu.NK_ERR_INVALID
     assert L.nk_layer_norm_device(p, 0, 2, 8, 8, None, None, 1e-5, 1, _p(d), 8, None, None, None) == gpu.NK_ERR_INVALID
+    # Any array, not the first alone.
+    e = torch.zeros(64, device="cuda")
+    assert L.nk_token_logprobs_device(_p(d), 0, 2, 8, 8, p, 1.0, 0, _p(e), None, None, None, None, None) == gpu.NK_ERR_INVALID
+    assert L.nk_token_logprobs_device(_p(d), 0, 2, 8, 8, None, 1.0, 0, None, p, None, None, None, None) == gpu.NK_ERR_INVALID
+    assert L.nk_distill_device(_p(d), 0, 2, 8, 8, p, _p(e), 0, 1, 1.0, _p(e[32:]), None, 1.0, None, 8, None) == gpu.NK_ERR_INVALID
+    assert L.nk_layer_norm_device(_p(d), 0, 2, 8, 8, p, None, 1e-5, 1, _p(e), 8, None, None, None) == gpu.NK_ERR_INVALID
+    assert L.nk_layer_norm_backward_device(_p(d), 0, 2, 8, 8, None, None, p, 1, _p(d), 8, _p(e), 8, None, None, 0, None, 0,
+                                           None) == gpu.NK_ERR_INVALID
     torch.cuda.synchronize()
 
 

@@ -37,19 +37,21 @@ def test_header_library_and_mirror_agree(nb):
 # Arguments of a call that would be taken, by name; p is some address.
 def _calls(p):
     return {
-        "nk_token_logprobs_device": dict(logits=p, dtype=0, rows=2, vocab=8, row_stride=8, targets=p, temperature=1.0,
-                                         top=2, logprob=p, entropy=p, stats=p, top_ids=p, top_logprobs=p, stream=None),
-        "nk_token_logprobs_backward_device": dict(logits=p, dtype=0, rows=2, vocab=8, row_stride=8, targets=p,
-                                                  temperature=1.0, stats=p, entropy=p, g_logprob=p, g_entropy=p,
-                                                  dlogits=p, dlogits_stride=8, stream=None),
-        "nk_distill_device": dict(logits=p, dtype=0, rows=2, vocab=8, row_stride=8, teacher_ids=p, teacher_logits=p,
-                                  teacher_dtype=0, n_teacher=2, temperature=1.0, loss=p, row_weight=p, grad_scale=1.0,
-                                  dlogits=p, dlogits_stride=8, stream=None),
-        "nk_layer_norm_device": dict(x=p, dtype=0, rows=2, width=8, x_stride=8, gain=p, bias=p, eps=1e-5, rms=0, y=p,
-                                     y_stride=8, mean=p, rstd=p, stream=None),
-        "nk_layer_norm_backward_device": dict(x=p, dtype=0, rows=2, width=8, x_stride=8, gain=p, mean=p, rstd=p, rms=0,
-                                              dy=p + 1024, dy_stride=8, dx=p + 2048, dx_stride=8, dgain=p, dbias=p,
-                                              accumulate=0, workspace=p, workspace_bytes=1 << 20, stream=None),
+        "nk_token_logprobs_device": dict(logits=p, dtype=0, rows=2, vocab=8, row_stride=8, targets=p + 1024,
+                                         temperature=1.0, top=2, logprob=p + 1280, entropy=p + 1536, stats=p + 1792,
+                                         top_ids=p + 2048, top_logprobs=p + 2304, stream=None),
+        "nk_token_logprobs_backward_device": dict(logits=p, dtype=0, rows=2, vocab=8, row_stride=8, targets=p + 1024,
+                                                  temperature=1.0, stats=p + 1280, entropy=p + 1536, g_logprob=p + 1792,
+                                                  g_entropy=p + 1792, dlogits=p, dlogits_stride=8, stream=None),
+        "nk_distill_device": dict(logits=p, dtype=0, rows=2, vocab=8, row_stride=8, teacher_ids=p + 1024,
+                                  teacher_logits=p + 1280, teacher_dtype=0, n_teacher=2, temperature=1.0, loss=p + 1536,
+                                  row_weight=p + 1792, grad_scale=1.0, dlogits=p, dlogits_stride=8, stream=None),
+        "nk_layer_norm_device": dict(x=p, dtype=0, rows=2, width=8, x_stride=8, gain=p + 1024, bias=p + 1024, eps=1e-5,
+                                     rms=0, y=p, y_stride=8, mean=p + 1280, rstd=p + 1536, stream=None),
+        "nk_layer_norm_backward_device": dict(x=p, dtype=0, rows=2, width=8, x_stride=8, gain=p + 256, mean=p + 512,
+                                              rstd=p + 768, rms=0, dy=p + 1024, dy_stride=8, dx=p + 2048, dx_stride=8,
+                                              dgain=p + 1280, dbias=p + 1536, accumulate=0, workspace=p + 2304,
+                                              workspace_bytes=1 << 20, stream=None),
     }
 
 
@@ -110,13 +112,39 @@ def test_columns_of_one_wide_array_do_not_overlap(nb, buf):
     assert b"overlap" in nb.lib().nk_last_error()
 
 
+# An output on an input's place, or on another output's, other than in place.
+@pytest.mark.parametrize("name,out,on", [
+    ("nk_token_logprobs_device", "logprob", "targets"), ("nk_token_logprobs_device", "stats", "logits"),
+    ("nk_token_logprobs_device", "entropy", "logprob"), ("nk_token_logprobs_device", "top_ids", "top_logprobs"),
+    ("nk_token_logprobs_backward_device", "dlogits", "stats"), ("nk_token_logprobs_backward_device", "dlogits", "g_entropy"),
+    ("nk_distill_device", "loss", "row_weight"), ("nk_distill_device", "loss", "dlogits"),
+    ("nk_distill_device", "dlogits", "teacher_ids"), ("nk_layer_norm_device", "y", "gain"),
+    ("nk_layer_norm_device", "mean", "x"), ("nk_layer_norm_device", "mean", "rstd"),
+    ("nk_layer_norm_backward_device", "dgain", "gain"), ("nk_layer_norm_backward_device", "dbias", "dgain"),
+    ("nk_layer_norm_backward_device", "workspace", "dy"), ("nk_layer_norm_backward_device", "dx", "rstd")])
+def test_outputs_on_top_of_other_arrays_are_refused(nb, buf, name, out, on):
+    args = _calls(C.addressof(buf))[name]
+    getattr(nb.lib(), name)(*args.values())
+    assert b"overlap" not in nb.lib().nk_last_error()
+    for shift in (0, 4):
+        assert getattr(nb.lib(), name)(*dict(args, **{out: args[on] + (0 if out == "workspace" else shift)}).values()) == nb.NK_ERR_INVALID
+        assert b"overlap" in nb.lib().nk_last_error()
+
+
+@pytest.mark.parametrize("temperature", [9e-5, 1.1e4, 1e30])
+def test_distillation_refuses_temperatures_that_leave_the_loss_no_digits(nb, buf, temperature):
+    args = _calls(C.addressof(buf))["nk_distill_device"]
+    args["temperature"] = temperature
+    assert nb.lib().nk_distill_device(*args.values()) == nb.NK_ERR_INVALID
+    assert b"temperature" in nb.lib().nk_last_error()
+
+
 @pytest.mark.parametrize("name", list(REFUSALS))
 def test_no_rows_is_no_work(nb, name):
     args = _calls(0)[name]
-    args = {k: (None if v in (0, 1024, 2048) and k in ("logits", "targets", "stats", "entropy", "logprob", "g_logprob",
-                                                       "g_entropy", "dlogits", "top_ids", "top_logprobs", "teacher_ids",
-                                                       "teacher_logits", "loss", "row_weight", "x", "y", "gain", "bias",
-                                                       "mean", "rstd", "dy", "dx", "dgain", "dbias", "workspace") else v)
+    args = {k: (None if k in ("logits", "targets", "stats", "entropy", "logprob", "g_logprob", "g_entropy", "dlogits",
+                              "top_ids", "top_logprobs", "teacher_ids", "teacher_logits", "loss", "row_weight", "x", "y",
+                              "gain", "bias", "mean", "rstd", "dy", "dx", "dgain", "dbias", "workspace") else v)
             for k, v in args.items()}
     args["rows"] = 0
     assert getattr(nb.lib(), name)(*args.values()) == 0, nb.lib().nk_last_error()
@@ -163,3 +191,6 @@ def test_workspace_grows_no_further_than_its_limit(nb):
         assert nb.lib().nk_layer_norm_backward_workspace(rows, 100, C.byref(n)) == 0
         sizes.append(n.value)
     assert sizes == sorted(sizes) and 0 < sizes[0] and sizes[-1] <= 2048 * 100 * 4
+    # Nor do wide rows ask for more than a few sums of the parameters.
+    assert nb.lib().nk_layer_norm_backward_workspace(1 << 10, 1 << 20, C.byref(n)) == 0
+    assert n.value <= 64 * 2 * (1 << 20) * 4
