@@ -147,9 +147,6 @@ __device__ __forceinline__ void total_shares(const Entries<ENTRIES> &e, int n, u
 // CTAs, and after the streaming threads have passed (they do not wait for it)
 // puts the gradient's values in the entries' places.  Each CTA answers for the
 // entries in its part.
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The streaming threads' mark and the teacher warp's wait for it.
 template <int THREADS>
 __device__ __forceinline__ void mark_arrive() {

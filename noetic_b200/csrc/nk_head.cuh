@@ -320,6 +320,12 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// The cluster's barrier; what a thread wrote before cluster_arrive is seen after the
+// wait, the relaxed one promises nothing.  Every thread of the cluster takes part.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // The largest of a warp's values; a NaN is passed over.
 __device__ __forceinline__ float warp_max1(float v) {
     float r;

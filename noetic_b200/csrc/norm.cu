@@ -9,13 +9,20 @@
 // the sums for dgain and dbias stay in registers too, and the next rows are on
 // their way while the present one is worked on.  All of it is bound by HBM,
 // as long as a row costs its threads few instructions beside its elements:
-// hence the f32 operations in pairs, and 64 bytes of a row to a thread where it has them.
-// Rows too wide for that take one block per row and read it again from L2.
+// hence the f32 operations in pairs, and 64 bytes of a row to a thread where it
+// has them.  Rows too wide for that are shared by a cluster of CTAs in the same
+// way; wider ones still, or wide ones that start anywhere, take a block per row
+// that reads them again from L2.
 //
 // Rows that do not start on 16-byte boundaries (an odd width) are read in the
 // same 16-byte units of memory.  Where a row starts in its first unit repeats
 // every 8 rows at most, so a group that steps by a multiple of 8 rows sees
 // every row start at the same place, and each thread's columns stay the same.
+//
+// Times below are of calls back to back on inputs beyond L2, HBM's copy rate
+// being 6.55 TB/s.
+
+#include <cooperative_groups.h>
 
 #include <algorithm>
 
@@ -51,13 +58,17 @@ __device__ __forceinline__ float group_sum(float v, float *red) {
     }
     return v;
 }
-template <int G>
-__device__ __forceinline__ float2 group_sum2(float2 v, float2 *red) {
+__device__ __forceinline__ float2 warp_sum2(float2 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
         v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float2 group_sum2(float2 v, float2 *red) {
+    v = warp_sum2(v);
     if constexpr (G > 32) {
         constexpr int W = G / 32;
         const int warp = threadIdx.x >> 5;
@@ -74,27 +85,34 @@ __device__ __forceinline__ float2 group_sum2(float2 v, float2 *red) {
     return v;
 }
 
-// Where a group's elements lie: 16-byte units of N elements, unit l * G + lane
-// the l-th of a thread.  With EDGE the row starts `shift` elements into unit 0
-// and may end inside the last one.
-template <class T, int G, int VALS, bool EDGE>
+// Where a group's elements lie: 16-byte units of N elements, unit base + l * G +
+// lane the l-th of a thread, up to `end`.  With EDGE the row starts `shift` elements
+// into unit 0 and may end inside the last one.  A row that a cluster shares (CL,
+// without EDGE) is cut into even parts.
+template <class T, int G, int VALS, bool EDGE, bool CL>
 struct Place {
     static constexpr int N = Vec<T>::N, LOADS = VALS / N, H = VALS / 2, C = N / 2;  // pairs in all, in a unit
-    int lane, width, shift, units, last;  // last: the load that holds the last unit
+    static constexpr bool whole = !EDGE;
+    int lane, width, shift, units, base, end, last;  // last: the load that holds the part's last unit
 
-    __device__ __forceinline__ Place(const void *row, int lane_, int width_) : lane(lane_), width(width_) {
+    __device__ __forceinline__ Place(const void *row, int lane_, int width_, int rank = 0, int cs = 1) : lane(lane_), width(width_) {
         shift = EDGE ? (int)((uintptr_t)row & 15) / (int)sizeof(T) : 0;
         units = (shift + width + N - 1) / N;
-        last = (units - 1) / G;
+        const int share = CL ? (units + cs - 1) / cs : units;
+        base = CL ? min(units, rank * share) : 0;
+        end = CL ? min(units, base + share) : units;
+        last = (end - base - 1) / G;
     }
-    __device__ __forceinline__ int unit(int l) const { return l * G + lane; }
+    __device__ __forceinline__ int unit(int l) const { return base + l * G + lane; }
     __device__ __forceinline__ int column(int l) const { return unit(l) * N - shift; }
-    __device__ __forceinline__ bool has(int l) const { return unit(l) < units; }
+    __device__ __forceinline__ bool has(int l) const { return unit(l) < end; }
     // Whether one of the group's units of load l may reach out of the row; whether
     // this thread's does.
     __device__ __forceinline__ bool edgy(int l) const { return EDGE && (l == 0 || l == last); }
     __device__ __forceinline__ bool on_edge(int l) const { return edgy(l) && (unit(l) == 0 || unit(l) == units - 1); }
     __device__ __forceinline__ bool inside(int col) const { return (unsigned)col < (unsigned)width; }
+    // Elements of a part (of a row without EDGE).
+    __device__ __forceinline__ int count() const { return (end - base) * N; }
     // A pair of elements, 0 where it is not in the row.
     __device__ __forceinline__ float2 keep(int l, int i, float2 v) const {
         if (!has(l)) return make_float2(0.0f, 0.0f);
@@ -106,9 +124,8 @@ struct Place {
 // The rows that a thread will work on next, ARRAYS of them at a time: its units
 // in its own places of a ring in shared memory, DEPTH rows on their way by
 // asynchronous copies (no barrier: a thread reads only what it copied).
-template <class T, int G, int VALS, bool EDGE, int NT, int DEPTH, int ARRAYS>
+template <class T, class P, bool EDGE, int NT, int DEPTH, int ARRAYS>
 struct RowQueue {
-    using P = Place<T, G, VALS, EDGE>;
     static constexpr int BYTES = DEPTH * ARRAYS * P::LOADS * NT * 16;
     uint4 *ring;  // [DEPTH][ARRAYS][LOADS][NT], from this thread's place on
     int slot = 0;
@@ -125,7 +142,7 @@ struct RowQueue {
                 const T *from = rows[k] + p.column(l);
                 if (!EDGE) {
                     copy_async16(to, from);
-                } else if (l > 0 || p.lane > 0 || p.shift == 0) {
+                } else if (p.unit(l) > 0 || p.shift == 0) {
                     copy_async16_part(to, from, min(16, (p.width - p.column(l)) * (int)sizeof(T)));
                 } else if (p.units > 1 && !first_row) {
                     // The unit that the row starts inside: by words, of which the first
@@ -139,14 +156,19 @@ struct RowQueue {
             }
         copy_commit();
     }
-    // Waits for the row pushed first, which is then the present one.
-    __device__ __forceinline__ void wait() const { copy_wait<DEPTH - 1>(); }
+    // Waits until the first n rows that were pushed, from the present one on, are there.
+    template <int n = 1>
+    __device__ __forceinline__ void wait() const {
+        copy_wait<DEPTH - n>();
+    }
     // Done with it: the next push goes to its slot.
-    __device__ __forceinline__ void pop() { slot = slot + 1 == DEPTH ? 0 : slot + 1; }
-    // Load l of the present row, in pairs; zeros outside the row.
-    __device__ __forceinline__ void get(const P &p, int k, int l, bool real, float2 (&x)[P::C]) const {
+    __device__ __forceinline__ void pop() { slot = ahead(1); }
+    // The slot of the k-th row behind the present one.
+    __device__ __forceinline__ int ahead(int k) const { return slot + k < DEPTH ? slot + k : slot + k - DEPTH; }
+    // Load l of the row in a slot, in pairs; zeros outside the row.
+    __device__ __forceinline__ void get(const P &p, int at, int k, int l, bool real, float2 (&x)[P::C]) const {
         float v[P::N];
-        unpack<T>(real && p.has(l) ? place(slot, k)[l * NT] : make_uint4(0, 0, 0, 0), v);
+        unpack<T>(real && p.has(l) ? place(at, k)[l * NT] : make_uint4(0, 0, 0, 0), v);
         if (EDGE && l == 0) {
 #pragma unroll
             for (int i = 0; i < P::N; ++i) v[i] = p.inside(p.column(0) + i) ? v[i] : 0.0f;
@@ -186,13 +208,13 @@ __device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int d) {
 }
 
 // A thread's part x(l) of a row that starts at `row`.  `same`: in the same place
-// of a unit as the rows read.  Otherwise the group hands the units over in
+// of a unit as the rows read (without EDGE always).  Otherwise the group hands the units over in
 // `stage` ([LOADS][NT] units, from the group's place on), where each thread
 // reads the two that its unit of the row written is cut from.  (Groups of several
 // warps: the barriers of the caller's reductions keep one row's stage from the next.)
 template <int G, int NT, class P, class T, class F>
 __device__ __forceinline__ void store_row(const P &p, T *row, bool same, uint4 *stage, F &&x) {
-    if (same) {
+    if (P::whole || same) {
 #pragma unroll
         for (int l = 0; l < P::LOADS; ++l)
             if (p.has(l)) store_unit(p, row, p.column(l), !p.on_edge(l), x(l));
@@ -236,7 +258,7 @@ template <class P>
 __device__ __forceinline__ void column_part(const P &p, const float *v, float other, float2 (&x)[P::H]) {
     auto one = [&](int j) {
         const int e = p.column(j / P::N) + j % P::N;
-        return p.inside(e) ? (v ? v[e] : other) : 0.0f;
+        return p.has(j / P::N) && p.inside(e) ? (v ? v[e] : other) : 0.0f;
     };
 #pragma unroll
     for (int j = 0; j < P::H; ++j) x[j] = make_float2(one(2 * j), one(2 * j + 1));
@@ -245,17 +267,20 @@ __device__ __forceinline__ void column_part(const P &p, const float *v, float ot
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // ---------------------------------------------------------------- forward
+// 16384 rows of 4096 bf16 in 49 us (5.5 TB/s, 0.83 of the copy rate); 8192 rows of
+// 8192 the same.  Four rows on their way to each group, since a block's own
+// reductions leave memory idle otherwise.  Rows of 64 x 1024 f32 cost their launch.
 template <class T, int G, int VALS, bool EDGE>
 __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_rows_k(NormArgs a, int same) {
     constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
-    using P = Place<T, G, VALS, EDGE>;
+    using P = Place<T, G, VALS, EDGE, false>;
     constexpr int C = P::C;
     __shared__ float red[2][32];
     extern __shared__ uint4 ring[];
     const int group = threadIdx.x / G;
     const float inv_n = 1.0f / (float)a.width;
     float2 gain[P::H], bias[P::H];
-    RowQueue<T, G, VALS, EDGE, NT, FWD_DEPTH, 1> queue;
+    RowQueue<T, P, EDGE, NT, FWD_DEPTH, 1> queue;
     queue.ring = ring + threadIdx.x;
     uint4 *stage = ring + queue.BYTES / 16 + group * G;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
@@ -277,7 +302,7 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm
 #pragma unroll
         for (int l = 0; l < P::LOADS; ++l) {
             float2 v[C];
-            queue.get(p, 0, l, real, v);
+            queue.get(p, queue.slot, 0, l, real, v);
 #pragma unroll
             for (int j = 0; j < C; ++j) x[l * C + j] = v[j];
         }
@@ -312,10 +337,189 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm
     }
 }
 
-// Rows that are too wide for a group: a block each, the first `keep` vectors
-// (16 bytes with VEC) waiting in shared memory, the others read again from L2.
+template <class T>
+constexpr int fwd_vals() {
+    return 64 / (int)sizeof(T);
+}
+
+// ---------------------------------------------------------------- rows that a cluster shares
+// Of R rows at a time (a turn), which share an exchange.  What a cluster's CTAs
+// tell each other: the NM_NT streaming threads leave two sums per warp and row in
+// `warps`; a warp of its own, the speaker, joins these, writes them to every CTA of
+// the cluster and carries the barrier's release: the streaming threads' arrival
+// promises nothing, or it would wait for their stores to the rows before.  They
+// send the next turn's sums off before they finish the present one's rows, which
+// covers the exchange.  (Two turns' places, by parity.)  Bound by that exchange, about
+// 2 us a turn with two CTAs to an SM, where the parts are small: 2048 rows of 32768
+// bf16 84 us (3.2 TB/s; 96 with one row to a turn, 161 by a block per row), 4096 of
+// 16384 f32 107 (124, 132).
+constexpr int CL_MOST = 8;  // CTAs of a cluster
+template <int R>
+struct RowExchange {
+    float2 warps[2][R][NM_NT / 32], parts[2][R][CL_MOST];
+    float counts[NM_NT / 32];  // elements of a warp
+
+    // The streaming threads' side: a warp's sums for a turn; after the exchange the
+    // parts', one to a lane.
+    __device__ __forceinline__ void send(const float2 (&v)[R], int turn) {
+        if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+            for (int k = 0; k < R; ++k) warps[turn & 1][k][threadIdx.x >> 5] = v[k];
+        }
+        __syncthreads();
+        cluster_arrive_relaxed();
+    }
+    __device__ __forceinline__ void receive(float2 (&v)[R], int turn, int cs) const {
+        cluster_wait();
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int k = 0; k < R; ++k) v[k] = lane < cs ? parts[turn & 1][k][lane] : make_float2(0.0f, 0.0f);
+    }
+    // The speaker's; join(a warp's sums in each lane) gives the CTA's in all.
+    template <class F>
+    __device__ __forceinline__ void speak(int turns, int rank, int cs, F &&join) {
+        namespace cg = cooperative_groups;
+        const int lane = threadIdx.x & 31;
+        for (int i = 0; i < turns; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const float2 all = join(lane < NM_NT / 32 ? warps[i & 1][k][lane] : make_float2(0.0f, 0.0f));
+                if (lane < cs) *cg::this_cluster().map_shared_rank(&parts[i & 1][k][rank], lane) = all;
+            }
+            cluster_arrive();
+            cluster_wait();
+        }
+    }
+};
+
+// Sums (of elements; of squared differences from the own mean) over parts of n
+// elements each, one part to a lane, joined.
+__device__ __forceinline__ float2 join_moments(float2 v, float n, float inv_all) {
+    const float s = warp_sum(v.x), off = (n > 0.0f ? v.x / n : 0.0f) - s * inv_all;
+    return make_float2(s, warp_sum(fmaf(n * off, off, v.y)));
+}
+
+constexpr int CL_FWD_ROWS = 2;
+template <class T>
+__global__ void __launch_bounds__(NM_NT + 32, 2) norm_cluster_rows_k(NormArgs a, int cs) {
+    constexpr int R = CL_FWD_ROWS;
+    using P = Place<T, NM_NT, fwd_vals<T>(), false, true>;
+    constexpr int C = P::C;
+    __shared__ RowExchange<R> ex;
+    extern __shared__ uint4 ring[];
+    const int rank = blockIdx.x % cs, lane = threadIdx.x & 31;
+    const int64_t step = gridDim.x / cs;
+    int64_t r = blockIdx.x / cs;
+    const int turns = (int)((a.rows - r + R * step - 1) / (R * step));
+    const T *row = (const T *)a.x + r * a.x_stride;
+    const float inv_n = 1.0f / (float)a.width;
+    cluster_arrive_relaxed();  // every CTA has to run before its shared memory is written
+    cluster_wait();
+    if (threadIdx.x >= NM_NT) {
+        const P p(row, 0, a.width, rank, cs);
+        const float inv_part = 1.0f / (float)max(1, p.count());
+        ex.speak(turns, rank, cs, [&](float2 v) { return join_moments(v, lane < NM_NT / 32 ? ex.counts[lane] : 0.0f, inv_part); });
+        return;
+    }
+    float2 gain[P::H], bias[P::H];
+    RowQueue<T, P, false, NM_NT, 3 * R, 1> queue;
+    queue.ring = ring + threadIdx.x;
+    const P p(row, threadIdx.x, a.width, rank, cs);
+    auto push = [&](int64_t q, int at) {
+        const T *const rows[1] = {(const T *)a.x + q * a.x_stride};
+        queue.push(p, rows, at, q < a.rows, q == 0);
+    };
+    for (int k = 0; k < 3 * R; ++k) push(r + k * step, k);
+    column_part(p, a.gain, 1.0f, gain);
+    column_part(p, a.bias, 0.0f, bias);
+    float count = 0.0f;
+#pragma unroll
+    for (int l = 0; l < P::LOADS; ++l) count += p.has(l) ? P::N : 0.0f;
+    count = warp_sum(count);
+    if (lane == 0) ex.counts[threadIdx.x >> 5] = count;
+    const float inv_count = count > 0.0f ? 1.0f / count : 0.0f;
+    const P of(row, 0, a.width, min(lane, cs - 1), cs);  // the part that this lane receives
+    const float n_part = lane < cs ? (float)of.count() : 0.0f;
+    // A turn's sums, of the rows that start at q, `first` slots on.
+    auto send = [&](int turn, int first, int64_t q) {
+        queue.template wait<2 * R>();
+        float2 own[R], v[R];  // the warp's means; the sums
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            own[k] = v[k] = both(0.0f);
+            if (a.rms) continue;
+            float2 s = both(0.0f), x[C];
+#pragma unroll
+            for (int l = 0; l < P::LOADS; ++l) {
+                queue.get(p, queue.ahead(first + k), 0, l, q + k * step < a.rows, x);
+#pragma unroll
+                for (int j = 0; j < C; ++j) s = add2(s, x[j]);
+            }
+            v[k].x = s.x + s.y;
+        }
+        if (!a.rms) {
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                v[k].x = warp_sum(v[k].x);
+                own[k] = both(-v[k].x * inv_count);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            float2 s = both(0.0f), x[C];
+#pragma unroll
+            for (int l = 0; l < P::LOADS; ++l) {
+                queue.get(p, queue.ahead(first + k), 0, l, q + k * step < a.rows, x);
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    x[j] = p.keep(l, 2 * j, add2(x[j], own[k]));
+                    s = fma2(x[j], x[j], s);
+                }
+            }
+            v[k].y = s.x + s.y;
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) v[k].y = warp_sum(v[k].y);
+        ex.send(v, turn);
+    };
+    send(0, 0, r);
+    for (int i = 0; i < turns; ++i) {
+        float2 all[R];
+        ex.receive(all, i, cs);
+        if (i + 1 < turns) send(i + 1, R, r + R * step);
+#pragma unroll
+        for (int k = 0; k < R; ++k) all[k] = join_moments(all[k], n_part, inv_n);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            if (r < a.rows) {
+                const float mean = all[k].x * inv_n, rstd = 1.0f / sqrtf(fmaf(all[k].y, inv_n, a.eps));
+                store_row<NM_NT, NM_NT>(p, (T *)a.y + r * a.y_stride, true, nullptr, [&](int l) {
+                    float2 x[C];
+                    queue.get(p, queue.slot, 0, l, true, x);
+#pragma unroll
+                    for (int j = 0; j < C; ++j) x[j] = fma2(mul2(add2(x[j], both(-mean)), both(rstd)), gain[l * C + j], bias[l * C + j]);
+                    return pack_pairs<T>(x);
+                });
+                if (rank == 0 && threadIdx.x == 0) {
+                    if (a.mean) a.mean[r] = mean;
+                    if (a.rstd) a.rstd[r] = rstd;
+                }
+            }
+            push(r + 3 * R * step, queue.slot);
+            queue.pop();
+            r += step;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- wider rows
+// A block each, in 16-byte vectors (VEC) or element by element, read again from L2
+// for each pass over them (kept in shared memory instead, fewer blocks share an SM:
+// 2048 rows of 40000 bf16 205 us with 64 KB of each kept, 193 so).  The f32 gain
+// and bias, read once per row, are most of what passes L2: 4096 rows of 16381 bf16
+// take 124 us, a third of HBM's rate.
 constexpr int WIDE_NT = 512;
-constexpr int WIDE_KEEP = 64 << 10;  // bytes: three blocks to an SM
 
 // f(pair of elements, index of the first) over a thread's part of a row, which
 // `at(v)` gives as 16 bytes of N elements (VEC) or one element.
@@ -339,21 +543,15 @@ __device__ __forceinline__ void wide_each(int width, At &&at, F &&f) {
 }
 
 template <class T, bool VEC>
-__global__ void __launch_bounds__(WIDE_NT) norm_wide_rows_k(NormArgs a, int keep) {
+__global__ void __launch_bounds__(WIDE_NT) norm_wide_rows_k(NormArgs a) {
     __shared__ float red[32];
-    extern __shared__ uint4 kept[];
     constexpr int N = VEC ? Vec<T>::N : 1;
     const int64_t r = blockIdx.x;
     const T *x = (const T *)a.x + r * a.x_stride;
     T *y = (T *)a.y + r * a.y_stride;
-    if constexpr (VEC) {
-        for (int v = threadIdx.x; v < min(keep, a.width / N); v += WIDE_NT) copy_async16(&kept[v], x + v * N);
-        copy_commit();
-        copy_wait<0>();
-    }
     auto at = [&](int v) {
         if constexpr (VEC)
-            return v < keep ? kept[v] : load16_rw(x + (int64_t)v * N);
+            return load16_rw(x + (int64_t)v * N);
         else
             return x[v];
     };
@@ -394,11 +592,13 @@ __global__ void __launch_bounds__(WIDE_NT) norm_wide_rows_k(NormArgs a, int keep
 // dx of the rows, and with PARAMS this block's sums for dgain and dbias: its
 // groups' registers joined in shared memory in their order, one row of the
 // workspace per block.  The row is unpacked twice, once for the sums and once
-// for dx: it waits in shared memory, not in registers.
+// for dx: it waits in shared memory, not in registers.  65536 rows of 1024 bf16 with
+// the parameters' sums in 79 us (5.1 TB/s); then the instructions per element
+// (about 10, two unpackings) are near to binding.
 template <class T, int G, int VALS, bool EDGE, bool PARAMS>
 __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_backward_k(NormGradArgs a, int same) {
     constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
-    using P = Place<T, G, VALS, EDGE>;
+    using P = Place<T, G, VALS, EDGE, false>;
     constexpr int C = P::C;
     __shared__ float2 red[2][32];
     extern __shared__ uint4 ring[];
@@ -408,7 +608,7 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm
     float2 gain[P::H], dg[P::H], db[P::H];
 #pragma unroll
     for (int j = 0; j < P::H; ++j) dg[j] = db[j] = both(0.0f);
-    RowQueue<T, G, VALS, EDGE, NT, BWD_DEPTH, 2> queue;
+    RowQueue<T, P, EDGE, NT, BWD_DEPTH, 2> queue;
     queue.ring = ring + threadIdx.x;
     uint4 *stage = ring + queue.BYTES / 16 + group * G;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
@@ -438,8 +638,8 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm
 #pragma unroll
         for (int l = 0; l < P::LOADS; ++l) {
             float2 h[C], c[C];
-            queue.get(p, 0, l, real, h);
-            queue.get(p, 1, l, real, c);
+            queue.get(p, queue.slot, 0, l, real, h);
+            queue.get(p, queue.slot, 1, l, real, c);
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
@@ -458,8 +658,8 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm
             if (real)
                 store_row<G, NT>(p, (T *)a.dx + r * a.dx_stride, same, stage, [&](int l) {
                     float2 h[C], c[C];
-                    queue.get(p, 0, l, real, h);
-                    queue.get(p, 1, l, real, c);
+                    queue.get(p, queue.slot, 0, l, real, h);
+                    queue.get(p, queue.slot, 1, l, real, c);
 #pragma unroll
                     for (int j = 0; j < C; ++j) {
                         h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
@@ -495,33 +695,150 @@ __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm
     }
 }
 
+// Rows of a turn: f32 rows leave shared memory for two CTAs with one only.  4096 rows
+// of 16384 bf16 with the parameters' sums: 133 us, 141 with one row to a turn, 231 by
+// the kernels for wider rows, which read everything twice; f32 168 and 311.
+template <class T>
+constexpr int cl_bwd_rows() {
+    return sizeof(T) == 4 ? 1 : 2;
+}
+template <class T, bool PARAMS>
+__global__ void __launch_bounds__(NM_NT + 32, 2) norm_cluster_backward_k(NormGradArgs a, int cs) {
+    constexpr int R = cl_bwd_rows<T>();
+    using P = Place<T, NM_NT, BWD_VALS, false, true>;
+    constexpr int C = P::C;
+    __shared__ RowExchange<R> ex;
+    extern __shared__ uint4 ring[];
+    const int rank = blockIdx.x % cs;
+    const int64_t step = gridDim.x / cs;
+    int64_t r = blockIdx.x / cs;
+    const int turns = (int)((a.rows - r + R * step - 1) / (R * step));
+    const float inv_n = 1.0f / (float)a.width;
+    if (PARAMS) pdl_trigger();  // norm_param_sum_k comes up, and waits for this grid's end
+    cluster_arrive_relaxed();   // every CTA has to run before its shared memory is written
+    cluster_wait();
+    if (threadIdx.x >= NM_NT) {
+        if (a.dx) ex.speak(turns, rank, cs, [](float2 v) { return warp_sum2(v); });
+        return;
+    }
+    float2 gain[P::H], dg[P::H], db[P::H];
+#pragma unroll
+    for (int j = 0; j < P::H; ++j) dg[j] = db[j] = both(0.0f);
+    RowQueue<T, P, false, NM_NT, 3 * R, 2> queue;
+    queue.ring = ring + threadIdx.x;
+    const P p((const T *)a.x + r * a.x_stride, threadIdx.x, a.width, rank, cs);
+    auto push = [&](int64_t q, int at) {
+        const T *const rows[2] = {(const T *)a.x + q * a.x_stride, (const T *)a.dy + q * a.dy_stride};
+        queue.push(p, rows, at, q < a.rows, q == 0);
+    };
+    for (int k = 0; k < 3 * R; ++k) push(r + k * step, k);
+    column_part(p, a.gain, 1.0f, gain);
+    float next_mean[R], next_rstd[R];  // of the rows that are sent next
+    auto stats = [&](int64_t q) {
+#pragma unroll
+        for (int k = 0; k < R; ++k, q += step) {
+            next_mean[k] = q < a.rows && !a.rms ? a.mean[q] : 0.0f;
+            next_rstd[k] = q < a.rows ? a.rstd[q] : 0.0f;
+        }
+    };
+    stats(r);
+    // A turn's share in the parameters' sums, and its rows' own sums.
+    auto send = [&](int turn, int first, int64_t q) {
+        queue.template wait<2 * R>();
+        float2 v[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const bool real = q + k * step < a.rows;
+            float2 sc = both(0.0f), sch = sc;
+#pragma unroll
+            for (int l = 0; l < P::LOADS; ++l) {
+                float2 h[C], c[C];
+                queue.get(p, queue.ahead(first + k), 0, l, real, h);
+                queue.get(p, queue.ahead(first + k), 1, l, real, c);
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    h[j] = mul2(add2(h[j], both(-next_mean[k])), both(next_rstd[k]));
+                    if (PARAMS) {
+                        dg[l * C + j] = fma2(c[j], h[j], dg[l * C + j]);
+                        db[l * C + j] = add2(db[l * C + j], c[j]);
+                    }
+                    c[j] = mul2(c[j], gain[l * C + j]);
+                    sc = add2(sc, c[j]);
+                    sch = fma2(c[j], h[j], sch);
+                }
+            }
+            v[k] = make_float2(sc.x + sc.y, sch.x + sch.y);
+        }
+        if (!a.dx) return;
+#pragma unroll
+        for (int k = 0; k < R; ++k) v[k] = warp_sum2(v[k]);
+        ex.send(v, turn);
+    };
+    send(0, 0, r);
+    for (int i = 0; i < turns; ++i) {
+        float mean[R], rstd[R];
+        float2 s[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            mean[k] = next_mean[k];
+            rstd[k] = next_rstd[k];
+        }
+        if (a.dx) ex.receive(s, i, cs);
+        stats(r + R * step);
+        if (i + 1 < turns) send(i + 1, R, r + R * step);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            if (a.dx && r < a.rows) {
+                const float2 all = warp_sum2(s[k]);
+                const float mc = a.rms ? 0.0f : all.x * inv_n, mch = all.y * inv_n;
+                store_row<NM_NT, NM_NT>(p, (T *)a.dx + r * a.dx_stride, true, nullptr, [&](int l) {
+                    float2 h[C], c[C];
+                    queue.get(p, queue.slot, 0, l, true, h);
+                    queue.get(p, queue.slot, 1, l, true, c);
+#pragma unroll
+                    for (int j = 0; j < C; ++j) {
+                        h[j] = mul2(add2(h[j], both(-mean[k])), both(rstd[k]));
+                        c[j] = fma2(c[j], gain[l * C + j], both(-mc));
+                        h[j] = mul2(both(rstd[k]), fma2(h[j], both(-mch), c[j]));
+                    }
+                    return pack_pairs<T>(h);
+                });
+            }
+            push(r + 3 * R * step, queue.slot);
+            queue.pop();
+            r += step;
+        }
+    }
+    if constexpr (PARAMS) {
+        float *w = a.workspace + (int64_t)(blockIdx.x / cs) * 2 * a.width;
+#pragma unroll
+        for (int j = 0; j < BWD_VALS; ++j) {
+            const int e = p.column(j / P::N) + j % P::N;
+            if (!p.has(j / P::N) || !p.inside(e)) continue;
+            w[e] = j & 1 ? dg[j / 2].y : dg[j / 2].x;
+            w[a.width + e] = j & 1 ? db[j / 2].y : db[j / 2].x;
+        }
+    }
+}
+
 template <class T, bool VEC>
-__global__ void __launch_bounds__(WIDE_NT) norm_wide_dx_k(NormGradArgs a, int keep) {
+__global__ void __launch_bounds__(WIDE_NT) norm_wide_dx_k(NormGradArgs a) {
     __shared__ float red[32];
-    extern __shared__ uint4 kept[];  // [keep] of x, [keep] of dy
     constexpr int N = VEC ? Vec<T>::N : 1;
     const int64_t r = blockIdx.x;
     const T *x = (const T *)a.x + r * a.x_stride, *dy = (const T *)a.dy + r * a.dy_stride;
     T *dx = (T *)a.dx + r * a.dx_stride;
-    if constexpr (VEC) {
-        for (int v = threadIdx.x; v < min(keep, a.width / N); v += WIDE_NT) {
-            copy_async16(&kept[v], x + v * N);
-            copy_async16(&kept[keep + v], dy + v * N);
-        }
-        copy_commit();
-        copy_wait<0>();
-    }
     // The gradient's vector (element) v beside x's.
     auto x_at = [&](int v) {
         if constexpr (VEC)
-            return v < keep ? kept[v] : load16_rw(x + (int64_t)v * N);
+            return load16_rw(x + (int64_t)v * N);
         else
             return x[v];
     };
     const float n = (float)a.width, mean = a.rms ? 0.0f : a.mean[r], rstd = a.rstd[r];
     auto both_of = [&](int v, float (&h)[N], float (&c)[N]) {
         if constexpr (VEC)
-            unpack<T>(v < keep ? kept[keep + v] : load16_rw(dy + (int64_t)v * N), c);
+            unpack<T>(load16_rw(dy + (int64_t)v * N), c);
         else
             c[0] = to_f32(dy[v]);
 #pragma unroll
@@ -588,7 +905,7 @@ __global__ void __launch_bounds__(NM_NT) norm_wide_param_k(NormGradArgs a) {
     }
 }
 
-// The partial rows' sum: 32 columns to a block, SUM_LANES threads to a column,
+// The partial rows' sum, from L2 (it starts while the rows' kernel ends): 32 columns to a block, SUM_LANES threads to a column,
 // each over every SUM_LANES-th row; their sums are added in order.
 constexpr int SUM_LANES = 16;
 __global__ void __launch_bounds__(32 * SUM_LANES) norm_param_sum_k(NormGradArgs a, int parts) {
@@ -619,30 +936,40 @@ bool same_place(const void *a, int64_t a_stride, const void *b, int64_t b_stride
     return (((uintptr_t)a ^ (uintptr_t)b) & 15) == 0 && (a_stride - b_stride) * es % 16 == 0;
 }
 
-// Blocks that the GPU holds at once, at most one per turn of rows; a multiple
-// of 8 where they take several turns, for rows that start anywhere.
-int64_t blocks(int64_t rows, int groups, int per_sm) {
-    return std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, 148 * per_sm / 8 * 8));
+// Blocks (or clusters) that the GPU holds at once, at most one per turn of
+// rows; a multiple of 8 where rows that start anywhere take several turns.
+// (More clusters than fit would run all their turns after the others.)
+constexpr int MOST_CLUSTERS[] = {0, 2 * 148, 148, 92, 68, 55, 44, 36, 32};  // of that many CTAs, two to an SM
+int64_t blocks(int64_t rows, int groups, int most, bool edge) {
+    return std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, edge ? most / 8 * 8 : most));
 }
 
-template <class Args, class... More>
-cudaError_t launch(void (*kern)(Args, More...), const Args &a, int64_t grid, int nt, int smem, cudaStream_t st, More... more) {
+template <class... Params, class... Args>
+cudaError_t launch(void (*kern)(Params...), int64_t grid, int nt, int smem, int cs, cudaStream_t st, Args... args) {
     if (smem > 40000) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
     }
-    kern<<<(unsigned)grid, nt, smem, st>>>(a, more...);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(grid * cs));
+    cfg.blockDim = dim3(nt);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cs;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cs > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
 }
 
 // The group and the elements per thread for a number of 16-byte units: as few
-// threads as hold it with MOST elements each, a warp at least.  Forward MOST is
-// 64 bytes (16384 x 4096 bf16: 45 us, with 32 bytes 49); backward 16 elements,
-// whose gain and sums take 48 registers (65536 x 1024 bf16: 32 elements take 95 us, 16 73).
-template <class T>
-constexpr int fwd_vals() {
-    return 64 / (int)sizeof(T);
-}
+// threads as hold it with MOST elements each, a warp at least; three quarters of
+// them where that is enough (16384 rows of 2560 bf16 34 us, with the unused places 41).
+// Forward MOST is 64 bytes (16384 rows of 4096 bf16 cold: 45 us, with 32 bytes 49);
+// backward 16 elements, whose gain and sums take 48 registers (65536 rows of 1024
+// bf16 cold: 73 us, with 32 elements 95).
 template <class T, int MOST, class F>
 cudaError_t with_group(int units, F &&f) {
     constexpr int N = Vec<T>::N, L = MOST / N;
@@ -660,6 +987,15 @@ cudaError_t with_group(int units, F &&f) {
     if (units <= 256 * L) return f(integral_constant<int, 256>(), vals);
     return f(integral_constant<int, 512>(), vals);
 }
+// The most units of a part of a row that a cluster shares, and its CTAs: as few as hold it.
+template <class T, int MOST>
+constexpr int part_units() {
+    return NM_NT * MOST / Vec<T>::N;
+}
+template <class T, int MOST>
+int cluster_of(int units) {
+    return (units + part_units<T, MOST>() - 1) / part_units<T, MOST>();
+}
 // The units that a row can cover.
 template <class T, bool EDGE>
 int units_of(int width) {
@@ -670,60 +1006,70 @@ template <class T, bool EDGE>
 cudaError_t forward_g(const NormArgs &a, int same, cudaStream_t st) {
     return with_group<T, fwd_vals<T>()>(units_of<T, EDGE>(a.width), [&](auto g, auto vals) {
         constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT;
-        const int smem = RowQueue<T, G, VALS, EDGE, NT, FWD_DEPTH, 1>::BYTES + (same ? 0 : NT * VALS * (int)sizeof(T));
-        return launch(norm_rows_k<T, G, VALS, EDGE>, a, blocks(a.rows, NT / G, NT > NM_NT ? 1 : 2), NT, smem, st, same);
+        const int smem = RowQueue<T, Place<T, G, VALS, EDGE, false>, EDGE, NT, FWD_DEPTH, 1>::BYTES + (same ? 0 : NT * VALS * (int)sizeof(T));
+        return launch(norm_rows_k<T, G, VALS, EDGE>, blocks(a.rows, NT / G, NT > NM_NT ? 148 : 2 * 148, EDGE), NT, smem, 1, st, a, same);
     });
 }
 template <class T>
 cudaError_t forward(const NormArgs &a, cudaStream_t st) {
-    constexpr int N = Vec<T>::N, ES = sizeof(T);
-    const bool whole = a.width % N == 0 && aligned16(a.x, a.x_stride, ES);
+    constexpr int N = Vec<T>::N, ES = sizeof(T), MOST = fwd_vals<T>(), most = 512 * MOST / N;
     const bool same = same_place(a.x, a.x_stride, a.y, a.y_stride, ES);
-    const int most = 512 * fwd_vals<T>() / N;
-    if (whole && same && a.width / N <= most) return forward_g<T, false>(a, 1, st);
+    const bool whole = same && a.width % N == 0 && aligned16(a.x, a.x_stride, ES);
+    const int units = a.width / N;
+    if (whole && units <= most) return forward_g<T, false>(a, 1, st);
     if (units_of<T, true>(a.width) <= most) return forward_g<T, true>(a, same, st);
-    if (!whole || !same) {
-        norm_wide_rows_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a, 0);
-        return cudaGetLastError();
+    if (whole && units <= CL_MOST * part_units<T, MOST>()) {
+        const int cs = cluster_of<T, MOST>(units), smem = RowQueue<T, Place<T, NM_NT, MOST, false, true>, false, NM_NT, 3 * CL_FWD_ROWS, 1>::BYTES;
+        return launch(norm_cluster_rows_k<T>, blocks(a.rows, 1, MOST_CLUSTERS[cs], false), NM_NT + 32, smem, cs, st, a, cs);
     }
-    const int keep = std::min(a.width / N, WIDE_KEEP / 16);
-    return launch(norm_wide_rows_k<T, true>, a, a.rows, WIDE_NT, keep * 16, st, keep);
+    if (whole)
+        norm_wide_rows_k<T, true><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a);
+    else
+        norm_wide_rows_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a);
+    return cudaGetLastError();
 }
 
 // The partial rows of dgain and dbias, at most: what `blocks` gives, or in rows
 // that are too wide for any group WIDE_PARTS.
 constexpr int WIDE_PARTS = 64;
 int partial_rows(int64_t rows, int width) {
-    return (int)std::min<int64_t>(std::max<int64_t>(rows, 1), width > 512 * BWD_VALS ? WIDE_PARTS : 2 * 148);
+    return (int)std::min<int64_t>(std::max<int64_t>(rows, 1), width > CL_MOST * NM_NT * BWD_VALS ? WIDE_PARTS : 2 * 148);
 }
 
 template <class T, bool EDGE>
 cudaError_t backward_g(const NormGradArgs &a, int same, bool params, int64_t &parts, cudaStream_t st) {
     return with_group<T, BWD_VALS>(units_of<T, EDGE>(a.width), [&](auto g, auto vals) {
         constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
-        parts = blocks(a.rows, GROUPS, NT > NM_NT ? 1 : 2);
+        parts = blocks(a.rows, GROUPS, NT > NM_NT ? 148 : 2 * 148, EDGE);
         const int join = params && GROUPS > 1 ? GROUPS * 2 * a.width * (int)sizeof(float) : 0;
-        const int smem = std::max(join, RowQueue<T, G, VALS, EDGE, NT, BWD_DEPTH, 2>::BYTES + (same ? 0 : NT * VALS * (int)sizeof(T)));
-        return params ? launch(norm_backward_k<T, G, VALS, EDGE, true>, a, parts, NT, smem, st, same)
-                      : launch(norm_backward_k<T, G, VALS, EDGE, false>, a, parts, NT, smem, st, same);
+        const int smem = std::max(join, RowQueue<T, Place<T, G, VALS, EDGE, false>, EDGE, NT, BWD_DEPTH, 2>::BYTES +
+                                            (same ? 0 : NT * VALS * (int)sizeof(T)));
+        return params ? launch(norm_backward_k<T, G, VALS, EDGE, true>, parts, NT, smem, 1, st, a, same)
+                      : launch(norm_backward_k<T, G, VALS, EDGE, false>, parts, NT, smem, 1, st, a, same);
     });
 }
 
 template <class T>
 cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
-    constexpr int N = Vec<T>::N, ES = sizeof(T);
+    constexpr int N = Vec<T>::N, ES = sizeof(T), most = 512 * BWD_VALS / N;
     const bool params = a.dgain || a.dbias;
     int64_t parts = 0;
-    const bool whole = a.width % N == 0 && aligned16(a.x, a.x_stride, ES);
     const bool like = same_place(a.x, a.x_stride, a.dy, a.dy_stride, ES);
     const bool same = !a.dx || same_place(a.x, a.x_stride, a.dx, a.dx_stride, ES);
-    const int most = 512 * BWD_VALS / N;
-    if (a.rows && like && whole && same && a.width / N <= most) {
+    const bool vec = like && same && a.width % N == 0 && aligned16(a.x, a.x_stride, ES);
+    const int units = a.width / N;
+    if (a.rows && vec && units <= most) {
         if (cudaError_t e = backward_g<T, false>(a, 1, params, parts, st)) return e;
     } else if (a.rows && like && units_of<T, true>(a.width) <= most) {
         if (cudaError_t e = backward_g<T, true>(a, same, params, parts, st)) return e;
+    } else if (a.rows && vec && units <= CL_MOST * part_units<T, BWD_VALS>()) {
+        const int cs = cluster_of<T, BWD_VALS>(units);
+        const int smem = RowQueue<T, Place<T, NM_NT, BWD_VALS, false, true>, false, NM_NT, 3 * cl_bwd_rows<T>(), 2>::BYTES;
+        parts = blocks(a.rows, 1, MOST_CLUSTERS[cs], false);
+        cudaError_t e = params ? launch(norm_cluster_backward_k<T, true>, parts, NM_NT + 32, smem, cs, st, a, cs)
+                               : launch(norm_cluster_backward_k<T, false>, parts, NM_NT + 32, smem, cs, st, a, cs);
+        if (e) return e;
     } else if (a.rows) {
-        const bool vec = whole && like && same;
         // The parameters' sums first: dx may be the array of dy.
         if (params) {
             parts = std::min<int64_t>(a.rows, WIDE_PARTS);
@@ -734,11 +1080,11 @@ cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
                 norm_wide_param_k<T, false><<<dim3(cols, (unsigned)parts), NM_NT, 0, st>>>(a);
             if (cudaError_t e = cudaGetLastError()) return e;
         }
-        if (a.dx && vec) {
-            const int keep = std::min(a.width / N, WIDE_KEEP / 16);
-            if (cudaError_t e = launch(norm_wide_dx_k<T, true>, a, a.rows, WIDE_NT, 2 * keep * 16, st, keep)) return e;
-        } else if (a.dx) {
-            norm_wide_dx_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a, 0);
+        if (a.dx) {
+            if (vec)
+                norm_wide_dx_k<T, true><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a);
+            else
+                norm_wide_dx_k<T, false><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a);
             if (cudaError_t e = cudaGetLastError()) return e;
         }
     }

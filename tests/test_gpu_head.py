@@ -486,7 +486,9 @@ def test_distill_gradient_against_differences(gpu, torch):
 # ---------------------------------------------------------------- norms
 NORM_SHAPES = [(1, 1, 0, 0), (3, 2, 0, 1), (5, 19, 3, 0), (64, 192, 0, 0), (33, 255, 0, 1), (16, 512, 8, 0),
                (9, 767, 1, 0), (300, 768, 0, 0), (70, 1024, 0, 0), (5, 1025, 0, 1), (40, 2048, 0, 0), (7, 4099, 0, 2),
-               (12, 8192, 0, 0), (3, 8193, 0, 0), (6, 16384, 8, 0), (2, 40000, 0, 0), (1200, 96, 0, 0), (2500, 40, 0, 0)]
+               (12, 8192, 0, 0), (3, 8193, 0, 0), (6, 16384, 8, 0), (2, 40000, 0, 0), (1200, 96, 0, 0), (2500, 40, 0, 0),
+               (310, 10240, 0, 0), (301, 12289, 0, 1), (9, 16383, 1, 1), (160, 20001, 0, 0), (75, 33000, 8, 4), (41, 65520, 0, 0),
+               (39, 65497, 0, 2), (3, 65535, 0, 0), (2, 131075, 0, 0)]
 
 
 def _norm(nb, torch, x, gain, bias, eps, rms, dtype, y=None):
