@@ -13,11 +13,11 @@ namespace nk {
 namespace {
 
 constexpr int TEACHER_MAX = 256;
-constexpr int DS_U = 4;
-constexpr int DS_NT = 192;
+constexpr int DS_U = 4;       // vectors of a thread at a time
+constexpr int DS_NT = 192;    // streaming threads of a CTA
 constexpr int DS_CLUSTER = 8;
 constexpr int DUP_BITS = 16384, WARP_DUP_BITS = 8192;
-constexpr int DS_PART = 68 << 10;  // bytes of a part: three to an SM
+constexpr int DS_PART = 68 << 10;  // bytes of a part
 constexpr int DS_MOST = (208 << 10) / (DS_NT * DS_U * 16) * (DS_NT * DS_U * 16);  // the most that a CTA keeps, in whole batches
 constexpr int DS_ROWS = 4;         // rows of a cluster, at most
 
@@ -147,6 +147,15 @@ __device__ __forceinline__ void total_shares(const Entries<ENTRIES> &e, int n, u
 // CTAs, and after the streaming threads have passed (they do not wait for it)
 // puts the gradient's values in the entries' places.  Each CTA answers for the
 // entries in its part.
+//
+// 4096 rows of 16384 f32 with 32 entries take 92 us (5.5 TB/s, 0.83 of HBM's copy
+// rate), 8192 of 131072 bf16 with 64 take 980 us (4.4 TB/s, 0.67).  16-bit rows cost
+// the special-function unit two exponentials per element, one for the sum and one for the
+// gradient, which is half of what HBM leaves time for, and their instructions issue in turns
+// with the copies: without the exponentials the same rows measured 770 us, without
+// the cluster's exchange 872, without both 725.  Taking the exponentials of half of the
+// elements by a polynomial instead gained nothing, reading the row a second time from
+// L2 in place of shared memory cost 1084 us.
 // The streaming threads' mark and the teacher warp's wait for it.
 template <int THREADS>
 __device__ __forceinline__ void mark_arrive() {
@@ -472,7 +481,8 @@ __global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_c
 }
 
 // ---------------------------------------------------------------- short rows: a warp each
-// The same in a warp, without a barrier but its own: 12 rows of 16 KB in the air per SM.
+// The same in a warp, without a barrier but its own: 12 rows of 16 KB in the air
+// per SM.  16384 rows of 1024 f32 take 31 us (4.3 TB/s).
 constexpr int WARP_ROWS = 4;
 
 // 16-byte units of shared memory of one warp.
@@ -618,6 +628,10 @@ template <class T>
 cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
     const int64_t n_vec = a.vocab / N;
+    // A warp per row for rows of up to 16 KB, when there are enough to fill the GPU.
+    // Measured, a warp against a cluster's CTA per row: 16384 rows of 4 KB 31 and
+    // 217 us, 8192 of 16 KB 74 and 175, 1000 of 16 KB 16 and 25; but 8192 rows of 32 KB
+    // 230 and 135 (few fit an SM), 256 rows of 4 KB 14 and 12.
     if (n_vec <= 1024 && a.rows >= 512) {
         const int keep = a.dlogits ? (int)n_vec : 0;
         const int smem = WARP_ROWS * warp_vectors(keep, a.n) * 16;
@@ -631,13 +645,19 @@ cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     }
     // A row is split until a part and those of two more CTAs fit an SM's shared
     // memory, and while the rows alone leave SMs idle and every thread keeps a vector.
+    // (8192 rows of 131072 bf16: parts of at most 68 KB 982 us, of 36 KB 1225, of 104 KB
+    // 954; 4096 rows of 16384 f32 93, 112 and 92; 1500 rows of 50000 bf16 80, 99 and 80:
+    // with larger parts two CTAs share an SM, which then differs little, and leaves it
+    // idle where rows end unevenly.  192 threads against 128 and 256: 982, 983 and 945 us;
+    // 93, 97 and 96; 80, 74 and 78.)
     int log_cs = 0;
     while ((1 << log_cs) < DS_CLUSTER && ((a.dlogits && (n_vec >> log_cs) * 16 > DS_PART) ||
                                           (a.rows << log_cs < 148 && n_vec >> (log_cs + 1) >= DS_NT)))
         ++log_cs;
     const int cs = 1 << log_cs;
     const int64_t keep = a.dlogits ? std::min<int64_t>((n_vec + cs - 1) / cs, DS_MOST / 16) : 0;
-    // Several rows to a cluster, as long as there are some turns of clusters left to even out.
+    // Several rows to a cluster, as long as there are some turns of clusters left to
+    // even out.  (8192 rows of 131072 bf16: four 982 us, one 1072, sixteen 995.)
     const int64_t rows_per = std::max<int64_t>(1, std::min<int64_t>(DS_ROWS, a.rows * cs / (148 * 3 * 4)));
     const int64_t clusters = (a.rows + rows_per - 1) / rows_per;
     auto kern = a.n <= 64 ? distill_k<T, DS_NT, 2> : distill_k<T, DS_NT, TEACHER_MAX / 32>;
