@@ -485,8 +485,9 @@ __global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_c
 // per SM.  16384 rows of 1024 f32 take 31 us (4.3 TB/s).
 constexpr int WARP_ROWS = 4;
 
-// 16-byte units of shared memory of one warp.
-__host__ __device__ inline int warp_vectors(int keep, int n) { return keep ? keep + (2 * n + 3) / 4 + WARP_DUP_BITS / 128 : 0; }
+// 16-byte units of shared memory of one warp that makes a gradient: `keep` vectors
+// (none in rows shorter than a vector), ids and shares, the bitmap.
+__host__ __device__ inline int warp_vectors(int keep, int n) { return keep + (2 * n + 3) / 4 + WARP_DUP_BITS / 128; }
 
 template <class T, int ENTRIES>
 __global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, int keep) {
@@ -633,8 +634,8 @@ cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     // 217 us, 8192 of 16 KB 74 and 175, 1000 of 16 KB 16 and 25; but 8192 rows of 32 KB
     // 230 and 135 (few fit an SM), 256 rows of 4 KB 14 and 12.
     if (n_vec <= 1024 && a.rows >= 512) {
-        const int keep = a.dlogits ? (int)n_vec : 0;
-        const int smem = WARP_ROWS * warp_vectors(keep, a.n) * 16;
+        const int keep = (int)n_vec;
+        const int smem = a.dlogits ? WARP_ROWS * warp_vectors(keep, a.n) * 16 : 0;
         auto kern = a.n <= 64 ? distill_warp_k<T, 2> : distill_warp_k<T, TEACHER_MAX / 32>;
         if (smem > 48 << 10) {
             cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

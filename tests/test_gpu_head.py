@@ -147,7 +147,7 @@ SHAPES = [(1, 1, 0, 0), (3, 2, 0, 1), (2, 19, 5, 0), (5, 255, 0, 1), (4, 256, 0,
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,V,pad,shift", SHAPES)
+@pytest.mark.parametrize("rows,V,pad,shift", SHAPES + [(600, 3, 0, 0), (700, 1, 2, 1), (900, 9, 1, 0)])
 def test_logprobs_over_sizes(gpu, torch, dtype, rows, V, pad, shift):
     z, whole = _matrix(torch, rows, V, dtype, pad, shift, seed=V + rows)
     before = whole.clone()
@@ -347,7 +347,8 @@ def _ref_distill(torch, z, ids, t, T, w, scale):
 
 
 @pytest.mark.parametrize("dtype,t_dtype", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("f32", "f16")])
-@pytest.mark.parametrize("rows,V,pad,shift", SHAPES)
+@pytest.mark.parametrize("rows,V,pad,shift", SHAPES + [(600, 3, 0, 0), (700, 1, 2, 1), (513, 7, 0, 0), (900, 9, 1, 0),
+                                                       (512, 8, 0, 0), (3, 4, 0, 1)])
 def test_distill_over_sizes(gpu, torch, dtype, t_dtype, rows, V, pad, shift):
     z, _ = _matrix(torch, rows, V, dtype, pad, shift, seed=7 * V + rows)
     for K, T, weighted in [(1, 1.0, False), (8, 2.0, True), (min(V, 33), 0.8, True), (256, 1.0, True)]:
