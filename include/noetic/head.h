@@ -104,8 +104,9 @@ nk_status nk_token_logprobs_backward(const void *logits, int dtype, uint64_t row
  *   loss[r] = temperature^2 sum_i q_i (log q_i - log p[id_i])
  *   dlogits[r][j] = grad_scale row_weight[r] temperature (p_j - sum_{i: id_i = j} q_i)
  * which is the gradient of grad_scale sum_r row_weight[r] loss[r].  row_weight
- * null: 1.  dlogits null: the loss alone; loss null: the gradient alone.  The
- * logits are read once for both.  A row without entries is not read: its loss
+ * null: 1.  dlogits null: the loss alone (summed in another order in long rows,
+ * so its last bits can differ); loss null: the gradient alone.  The logits are
+ * read once for both.  A row without entries is not read: its loss
  * and gradient are 0.  A row of weight 0 has gradient 0.  Where the student has
  * no logit above -infinity the loss is infinity and the gradient 0.  An id may
  * stand in a row more than once (its shares add up).  dlogits has the type of
