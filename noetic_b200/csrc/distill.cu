@@ -484,6 +484,7 @@ __global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_c
 // The same in a warp, without a barrier but its own: 12 rows of 16 KB in the air
 // per SM.  16384 rows of 1024 f32 take 31 us (4.3 TB/s).
 constexpr int WARP_ROWS = 4;
+constexpr int WARP_VECTORS = 1024;  // of a row, at most
 
 // 16-byte units of shared memory of one warp that makes a gradient: `keep` vectors
 // (none in rows shorter than a vector), ids and shares, the bitmap.
@@ -633,12 +634,12 @@ cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     // Measured, a warp against a cluster's CTA per row: 16384 rows of 4 KB 31 and
     // 217 us, 8192 of 16 KB 74 and 175, 1000 of 16 KB 16 and 25; but 8192 rows of 32 KB
     // 230 and 135 (few fit an SM), 256 rows of 4 KB 14 and 12.
-    if (n_vec <= 1024 && a.rows >= 512) {
+    if (n_vec <= WARP_VECTORS && a.rows >= 512) {
         const int keep = (int)n_vec;
         const int smem = a.dlogits ? WARP_ROWS * warp_vectors(keep, a.n) * 16 : 0;
         auto kern = a.n <= 64 ? distill_warp_k<T, 2> : distill_warp_k<T, TEACHER_MAX / 32>;
         if (smem > 48 << 10) {
-            cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            cudaError_t e = allow_shared(kern, WARP_ROWS * warp_vectors(WARP_VECTORS, TEACHER_MAX) * 16);
             if (e != cudaSuccess) return e;
         }
         kern<<<(unsigned)((a.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, smem, st>>>(a, keep);
@@ -663,7 +664,7 @@ cudaError_t launch_distill(const DistillArgs &a, cudaStream_t st) {
     const int64_t clusters = (a.rows + rows_per - 1) / rows_per;
     auto kern = a.n <= 64 ? distill_k<T, DS_NT, 2> : distill_k<T, DS_NT, TEACHER_MAX / 32>;
     if (keep * 16 > 32768) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DS_MOST);
+        cudaError_t e = allow_shared(kern, DS_MOST);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};

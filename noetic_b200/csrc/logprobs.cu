@@ -544,7 +544,7 @@ cudaError_t launch_logprobs(const LogprobsArgs &a, cudaStream_t st) {
         const int smem = WARP_ROWS * warp_team_bytes(a.top);
         auto kern = token_logprobs_warp_k<T>;
         if (smem > 48 << 10) {
-            cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            cudaError_t e = allow_shared(kern, WARP_ROWS * warp_team_bytes(TOP_MAX));
             if (e != cudaSuccess) return e;
         }
         kern<<<(unsigned)((a.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, smem, st>>>(a, shift);

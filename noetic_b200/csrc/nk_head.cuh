@@ -63,6 +63,15 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
+// Lets a kernel be launched with `most` bytes of dynamic shared memory.  The limit
+// belongs to the function on its device, not to a call, so `most` is the most that
+// any call of this function asks for: set to the call's own need, a call of another
+// host thread could lower it between this and the launch.
+template <class K>
+inline cudaError_t allow_shared(K *kern, int most) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+}
+
 // ---------------------------------------------------------------- 16-byte vectors
 // A row of n elements is `head` elements up to a 16-byte boundary, n_vec
 // vectors, and `tail` elements, so that any row start gets wide loads.

@@ -944,10 +944,11 @@ int64_t blocks(int64_t rows, int groups, int most, bool edge) {
     return std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, edge ? most / 8 * 8 : most));
 }
 
+// With `smem` bytes of shared memory of the `most` that any call of this kernel takes.
 template <class... Params, class... Args>
-cudaError_t launch(void (*kern)(Params...), int64_t grid, int nt, int smem, int cs, cudaStream_t st, Args... args) {
+cudaError_t launch(void (*kern)(Params...), int64_t grid, int nt, int smem, int most, int cs, cudaStream_t st, Args... args) {
     if (smem > 40000) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t e = allow_shared(kern, most);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
@@ -1006,8 +1007,9 @@ template <class T, bool EDGE>
 cudaError_t forward_g(const NormArgs &a, int same, cudaStream_t st) {
     return with_group<T, fwd_vals<T>()>(units_of<T, EDGE>(a.width), [&](auto g, auto vals) {
         constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT;
-        const int smem = RowQueue<T, Place<T, G, VALS, EDGE, false>, EDGE, NT, FWD_DEPTH, 1>::BYTES + (same ? 0 : NT * VALS * (int)sizeof(T));
-        return launch(norm_rows_k<T, G, VALS, EDGE>, blocks(a.rows, NT / G, NT > NM_NT ? 148 : 2 * 148, EDGE), NT, smem, 1, st, a, same);
+        constexpr int queue = RowQueue<T, Place<T, G, VALS, EDGE, false>, EDGE, NT, FWD_DEPTH, 1>::BYTES, stage = NT * VALS * (int)sizeof(T);
+        return launch(norm_rows_k<T, G, VALS, EDGE>, blocks(a.rows, NT / G, NT > NM_NT ? 148 : 2 * 148, EDGE), NT, queue + (same ? 0 : stage),
+                      queue + (EDGE ? stage : 0), 1, st, a, same);
     });
 }
 template <class T>
@@ -1020,7 +1022,7 @@ cudaError_t forward(const NormArgs &a, cudaStream_t st) {
     if (units_of<T, true>(a.width) <= most) return forward_g<T, true>(a, same, st);
     if (whole && units <= CL_MOST * part_units<T, MOST>()) {
         const int cs = cluster_of<T, MOST>(units), smem = RowQueue<T, Place<T, NM_NT, MOST, false, true>, false, NM_NT, 3 * CL_FWD_ROWS, 1>::BYTES;
-        return launch(norm_cluster_rows_k<T>, blocks(a.rows, 1, MOST_CLUSTERS[cs], false), NM_NT + 32, smem, cs, st, a, cs);
+        return launch(norm_cluster_rows_k<T>, blocks(a.rows, 1, MOST_CLUSTERS[cs], false), NM_NT + 32, smem, smem, cs, st, a, cs);
     }
     if (whole)
         norm_wide_rows_k<T, true><<<(unsigned)a.rows, WIDE_NT, 0, st>>>(a);
@@ -1041,11 +1043,12 @@ cudaError_t backward_g(const NormGradArgs &a, int same, bool params, int64_t &pa
     return with_group<T, BWD_VALS>(units_of<T, EDGE>(a.width), [&](auto g, auto vals) {
         constexpr int G = decltype(g)::value, VALS = decltype(vals)::value, NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
         parts = blocks(a.rows, GROUPS, NT > NM_NT ? 148 : 2 * 148, EDGE);
-        const int join = params && GROUPS > 1 ? GROUPS * 2 * a.width * (int)sizeof(float) : 0;
-        const int smem = std::max(join, RowQueue<T, Place<T, G, VALS, EDGE, false>, EDGE, NT, BWD_DEPTH, 2>::BYTES +
-                                            (same ? 0 : NT * VALS * (int)sizeof(T)));
-        return params ? launch(norm_backward_k<T, G, VALS, EDGE, true>, parts, NT, smem, 1, st, a, same)
-                      : launch(norm_backward_k<T, G, VALS, EDGE, false>, parts, NT, smem, 1, st, a, same);
+        // (Where the parameters' sums are joined the rows were: two f32 for each of their elements.)
+        constexpr int queue = RowQueue<T, Place<T, G, VALS, EDGE, false>, EDGE, NT, BWD_DEPTH, 2>::BYTES, stage = NT * VALS * (int)sizeof(T);
+        static_assert(GROUPS == 1 || queue >= NT * VALS * 2 * (int)sizeof(float), "");
+        const int smem = queue + (same ? 0 : stage), most = queue + (EDGE ? stage : 0);
+        return params ? launch(norm_backward_k<T, G, VALS, EDGE, true>, parts, NT, smem, most, 1, st, a, same)
+                      : launch(norm_backward_k<T, G, VALS, EDGE, false>, parts, NT, smem, most, 1, st, a, same);
     });
 }
 
@@ -1066,8 +1069,8 @@ cudaError_t backward(const NormGradArgs &a, cudaStream_t st) {
         const int cs = cluster_of<T, BWD_VALS>(units);
         const int smem = RowQueue<T, Place<T, NM_NT, BWD_VALS, false, true>, false, NM_NT, 3 * cl_bwd_rows<T>(), 2>::BYTES;
         parts = blocks(a.rows, 1, MOST_CLUSTERS[cs], false);
-        cudaError_t e = params ? launch(norm_cluster_backward_k<T, true>, parts, NM_NT + 32, smem, cs, st, a, cs)
-                               : launch(norm_cluster_backward_k<T, false>, parts, NM_NT + 32, smem, cs, st, a, cs);
+        cudaError_t e = params ? launch(norm_cluster_backward_k<T, true>, parts, NM_NT + 32, smem, smem, cs, st, a, cs)
+                               : launch(norm_cluster_backward_k<T, false>, parts, NM_NT + 32, smem, smem, cs, st, a, cs);
         if (e) return e;
     } else if (a.rows) {
         // The parameters' sums first: dx may be the array of dy.

@@ -1,0 +1,81 @@
+"""Calls of include/noetic/head.h that the operators' own tests do not make: two
+host threads at once."""
+
+import ctypes as C
+import threading
+
+import pytest
+
+from test_gpu_head import CODE, _matrix, _norm, _p, torch  # noqa: F401  (torch: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def _both(gpu, torch, calls, times=4000):
+    """Each call by a host thread of its own on a stream of its own, again and
+    again; returns the messages of those that failed."""
+    torch.cuda.synchronize()
+    failed, start = [], threading.Barrier(len(calls))
+
+    def work(call):
+        st = torch.cuda.Stream()
+        s = C.c_void_p(st.cuda_stream)
+        start.wait()
+        for _ in range(times):
+            if call(s) != 0:
+                failed.append(gpu.lib().nk_last_error())
+        st.synchronize()
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return failed
+
+
+# Pairs of calls of one kernel that take different amounts of shared memory, both
+# more than every kernel may have: neither makes the other fail.
+def test_two_threads_with_teachers_of_other_lengths(gpu, torch):
+    L, R, V = gpu.lib(), 512, 4096
+    z, _ = _matrix(torch, R, V, "f32", seed=1)
+    z = z.contiguous()
+
+    def call(K):
+        ids = torch.arange(K, device="cuda", dtype=torch.int32).repeat(R, 1).contiguous()
+        t = torch.zeros(R, K, device="cuda")
+        dz = torch.empty_like(z)
+        return lambda s: L.nk_distill_device(_p(z), 0, R, V, V, _p(ids), _p(t), 0, K, 1.0, None, None, 1.0, _p(dz), V, s)
+
+    assert _both(gpu, torch, [call(1), call(64)]) == []
+
+
+def test_two_threads_with_other_numbers_of_alternatives(gpu, torch):
+    L, R, V = gpu.lib(), 512, 300
+    z, _ = _matrix(torch, R, V, "f32", seed=1)
+    z = z.contiguous()
+
+    def call(top):
+        ids = torch.empty(R, top, device="cuda", dtype=torch.int32)
+        return lambda s: L.nk_token_logprobs_device(_p(z), 0, R, V, V, None, 1.0, top, None, None, None, _p(ids), None, s)
+
+    assert _both(gpu, torch, [call(110), call(128)]) == []
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_two_threads_with_norms_into_other_layouts(gpu, torch, dtype):
+    L, R, d = gpu.lib(), 9000, 767 if dtype == "f32" else 1001
+    x, _ = _matrix(torch, R, d, dtype, seed=1)
+    code, gain = CODE[dtype], torch.ones(d, device="cuda")
+    _, mean, rstd = _norm(gpu, torch, x, gain, None, 1e-5, False, dtype)
+
+    def forward(out):
+        return lambda s: L.nk_layer_norm_device(_p(x), code, R, d, d, _p(gain), None, 1e-5, 0, _p(out), out.stride(0), None, None, s)
+
+    def backward(out):
+        return lambda s: L.nk_layer_norm_backward_device(_p(x), code, R, d, d, _p(gain), _p(mean), _p(rstd), 0, _p(x), d, _p(out),
+                                                         out.stride(0), None, None, 0, None, 0, s)
+
+    for call in (forward, backward):
+        alike, other = (_matrix(torch, R, d, dtype, shift=k)[0] for k in (0, 1))
+        assert _both(gpu, torch, [call(alike), call(other)]) == []
