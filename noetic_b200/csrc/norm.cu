@@ -872,36 +872,46 @@ __global__ void __launch_bounds__(WIDE_NT) norm_wide_dx_k(NormGradArgs a) {
 }
 
 // Partial sums over the rows p, p + P, ... of N columns (one without VEC) per
-// thread.
+// thread; of PARAM_ROWS at a time, joined in the workspace, so that with millions of
+// rows a term still passes through few additions (2^20 rows: 64 + 256 in place of
+// 16384).  (Two rows at once, four of single f32: 65536 rows of 1024 f32, dx included, 625
+// us, with two 816; of bf16, element by element, 658 and with four 1053.)
+constexpr int PARAM_ROWS = 64;
 template <class T, bool VEC>
 __global__ void __launch_bounds__(NM_NT) norm_wide_param_k(NormGradArgs a) {
     constexpr int N = VEC ? Vec<T>::N : 1;
     const int e = (blockIdx.x * NM_NT + threadIdx.x) * N;
     if (e >= a.width) return;
-    float dg[N] = {}, db[N] = {};
-#pragma unroll 2
-    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const T *x = (const T *)a.x + r * a.x_stride + e, *dy = (const T *)a.dy + r * a.dy_stride + e;
-        const float mean = a.rms ? 0.0f : a.mean[r], rstd = a.rstd[r];
-        float h[N], c[N];
-        if constexpr (VEC) {
-            unpack<T>(load16_rw(x), h);
-            unpack<T>(load16_rw(dy), c);
-        } else {
-            h[0] = to_f32(*x);
-            c[0] = to_f32(*dy);
+    float *w = a.workspace + (int64_t)blockIdx.y * 2 * a.width;
+    const T *x = (const T *)a.x + blockIdx.y * a.x_stride + e, *dy = (const T *)a.dy + blockIdx.y * a.dy_stride + e;
+    const int64_t x_step = gridDim.y * a.x_stride, dy_step = gridDim.y * a.dy_stride;
+    const int n = (int)((a.rows - blockIdx.y + gridDim.y - 1) / gridDim.y);
+    int r = blockIdx.y;
+    for (int done = 0; done < n; done += PARAM_ROWS) {
+        const int m = min(n - done, PARAM_ROWS);
+        float dg[N] = {}, db[N] = {};
+#pragma unroll (sizeof(T) == 4 && !VEC ? 4 : 2)
+        for (int k = 0; k < m; ++k, r += gridDim.y, x += x_step, dy += dy_step) {
+            const float mean = a.rms ? 0.0f : a.mean[r], rstd = a.rstd[r];
+            float h[N], c[N];
+            if constexpr (VEC) {
+                unpack<T>(load16_rw(x), h);
+                unpack<T>(load16_rw(dy), c);
+            } else {
+                h[0] = to_f32(*x);
+                c[0] = to_f32(*dy);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                dg[i] = fmaf(c[i], (h[i] - mean) * rstd, dg[i]);
+                db[i] += c[i];
+            }
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            dg[i] = fmaf(c[i], (h[i] - mean) * rstd, dg[i]);
-            db[i] += c[i];
+            w[e + i] = done == 0 ? dg[i] : w[e + i] + dg[i];
+            w[a.width + e + i] = done == 0 ? db[i] : w[a.width + e + i] + db[i];
         }
-    }
-    float *w = a.workspace + (int64_t)blockIdx.y * 2 * a.width;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        w[e + i] = dg[i];
-        w[a.width + e + i] = db[i];
     }
 }
 

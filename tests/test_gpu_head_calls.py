@@ -1,12 +1,12 @@
 """Calls of include/noetic/head.h that the operators' own tests do not make: two
-host threads at once."""
+host threads at once, sums over many rows."""
 
 import ctypes as C
 import threading
 
 import pytest
 
-from test_gpu_head import CODE, _matrix, _norm, _p, torch  # noqa: F401  (torch: the fixture)
+from test_gpu_head import CODE, _matrix, _norm, _norm_grad, _p, torch  # noqa: F401  (torch: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,22 @@ def test_two_threads_with_norms_into_other_layouts(gpu, torch, dtype):
     for call in (forward, backward):
         alike, other = (_matrix(torch, R, d, dtype, shift=k)[0] for k in (0, 1))
         assert _both(gpu, torch, [call(alike), call(other)]) == []
+
+
+def test_norm_gradient_sums_over_a_million_rows(gpu, torch):
+    # Rows of dy that start elsewhere than those of x.  A term passes through 64 additions, one for
+    # each 4096 rows, four over the partial rows of a lane, 16 at the end.  Column 0 is a constant
+    # of 1023.499 steps of the binade that a sum over every 64th row ends in: added one by one, half of
+    # these additions would round down by half a step, 4000 U in all.
+    U, rows, d = 2.0**-24, 2**20 + 37, 8
+    x, _ = _matrix(torch, rows, d, "f32", seed=1)
+    dy, _ = _matrix(torch, rows, d, "f32", pad=1, seed=2, offset=1.0)
+    dy[:, 0] = 1023.499 * 2.0**-13
+    gain = torch.ones(d, device="cuda")
+    _, mean, rstd = _norm(gpu, torch, x, gain, None, 1e-5, False, "f32")
+    dx, dg, db = _norm_grad(gpu, torch, x, dy, gain, mean, rstd, "f32")
+    hh = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    adds = (64 + rows / 4096 + 4 + 16) * U
+    g = dy.double()
+    assert ((db - g.sum(0)).abs() <= adds * g.abs().sum(0)).all()
+    assert ((dg - (g * hh).sum(0)).abs() <= (adds + 3 * U) * (g * hh).abs().sum(0)).all()
