@@ -92,6 +92,13 @@ struct Entries {
     }
 };
 
+// temperature q (log q - log p) of an entry, p = exp((z - m) / temperature - log_s).
+// Not divided by the temperature, so that a student's logit of f32's lowest value
+// stays in range at temperatures below 1.
+__device__ __forceinline__ float loss_term(float q, float log_q, float z, float m, float log_s, float temperature) {
+    return q * fmaf(temperature, log_q + log_s, m - z);
+}
+
 // Whether two of a warp's entries have the same id, by a bitmap of DUP_BITS bits
 // in shared memory that is clear before and after; ids that far apart may pass
 // for the same one.  Walking all pairs costs a row more than its other teacher
@@ -268,7 +275,7 @@ __global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_c
             if (loss_row >= 0 && rank == 0 && lane == 0 && a.loss) {
                 float all = 0.0f;
                 for (int c = 0; c < cs; ++c) all += sh.kl[t & 1][c];
-                a.loss[loss_row] = a.temperature * a.temperature * all;
+                a.loss[loss_row] = a.temperature * all;
             }
         };
         for (int i = lane; i < DUP_BITS / 32; i += 32) sh.bits[i] = 0;
@@ -310,12 +317,12 @@ __global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_c
 #pragma unroll
             for (int k = 0; k < ENTRIES; ++k)
                 if ((mine >> k & 1) && now.q[k] != 0.0f)
-                    kl += empty ? INFINITY : now.q[k] * (log_q[k] - ((z[k] - sums.m) * a.inv_t - log_s));
+                    kl += empty ? INFINITY : loss_term(now.q[k], log_q[k], z[k], sums.m, log_s, a.temperature);
             kl = warp_sum(kl);
             if (log_cs) {
                 if (lane == 0) cg::this_cluster().map_shared_rank(&sh.kl[turn & 1][0], 0)[rank] = kl;
             } else if (lane == 0 && a.loss) {
-                a.loss[r] = a.temperature * a.temperature * kl;
+                a.loss[r] = a.temperature * kl;
             }
             loss_row = r;
             ++turn;
@@ -587,9 +594,9 @@ __global__ void __launch_bounds__(32 * WARP_ROWS) distill_warp_k(DistillArgs a, 
 #pragma unroll
     for (int k = 0; k < ENTRIES; ++k)
         if (now.id[k] != NO_TOKEN && now.q[k] != 0.0f)
-            kl += empty ? INFINITY : now.q[k] * (log_q[k] - ((z_entry[k] - all.m) * a.inv_t - log_s));
+            kl += empty ? INFINITY : loss_term(now.q[k], log_q[k], z_entry[k], all.m, log_s, a.temperature);
     kl = warp_sum(kl);
-    if (lane == 0 && a.loss) a.loss[r] = a.temperature * a.temperature * kl;
+    if (lane == 0 && a.loss) a.loss[r] = a.temperature * kl;
     if (!out) return;
     if (w == 0.0f || empty) {
         zeros();

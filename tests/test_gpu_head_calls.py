@@ -1,12 +1,12 @@
 """Calls of include/noetic/head.h that the operators' own tests do not make: two
-host threads at once, sums over many rows."""
+host threads at once, sums over many rows, logits at the end of f32's range."""
 
 import ctypes as C
 import threading
 
 import pytest
 
-from test_gpu_head import CODE, _matrix, _norm, _norm_grad, _p, torch  # noqa: F401  (torch: the fixture)
+from test_gpu_head import CODE, _distill, _matrix, _norm, _norm_grad, _out_tol, _p, _ref_distill, torch  # noqa: F401  (torch: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,25 @@ def test_norm_gradient_sums_over_a_million_rows(gpu, torch):
     g = dy.double()
     assert ((db - g.sum(0)).abs() <= adds * g.abs().sum(0)).all()
     assert ((dg - (g * hh).sum(0)).abs() <= (adds + 3 * U) * (g * hh).abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("rows,V", [(4, 300), (600, 300), (3, 60000), (2000, 9000)])
+@pytest.mark.parametrize("T", [1.0, 0.5, 0.03])
+def test_distillation_of_a_student_masked_by_the_lowest_value(gpu, torch, rows, V, T):
+    # (z - m) / T is beyond f32's range where the teacher wants what the student's mask forbids and T is below 1;
+    # T^2 times it is not.
+    low = torch.finfo(torch.float32).min
+    z, _ = _matrix(torch, rows, V, "f32", seed=V)
+    z[:, 40:80] = low
+    z[:, V - 3:] = low
+    ids = torch.tensor([7, 50, V - 1, 79, 20], device="cuda", dtype=torch.int32).repeat(rows, 1)
+    ids[::2, 1:4] = torch.tensor([8, 9, 10], device="cuda", dtype=torch.int32)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    t = torch.randn(rows, 5, generator=g, device="cuda") * T
+    ref, tol, rdz, ztol = _ref_distill(torch, z, ids, t, T, None, 1.0)
+    for grad in (True, False):
+        loss, dz = _distill(gpu, torch, z, ids, t, T, None, 1.0, "f32", "f32", grad=grad)
+        assert torch.isfinite(loss).all() and (loss[1::2] > 1e30).all()
+        assert ((loss.double() - ref).abs() <= tol).all()
+        if grad:
+            assert ((dz.double() - rdz).abs() <= ztol + _out_tol(torch, "f32", rdz)).all()
