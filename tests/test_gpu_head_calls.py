@@ -1,12 +1,15 @@
 """Calls of include/noetic/head.h that the operators' own tests do not make: two
-host threads at once, sums over many rows, logits at the end of f32's range."""
+host threads at once, sums over many rows, logits at the end of f32's range, texts
+longer than a block of logits."""
 
 import ctypes as C
 import threading
 
+import numpy as np
 import pytest
 
-from test_gpu_head import CODE, _distill, _matrix, _norm, _norm_grad, _out_tol, _p, _ref_distill, torch  # noqa: F401  (torch: the fixture)
+from test_gpu_head import (CODE, U, _distill, _matrix, _norm, _norm_grad, _out_tol, _p, _ref_distill, _span,  # noqa: F401
+                           _sum_rel, torch)  # (torch: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -86,7 +89,7 @@ def test_norm_gradient_sums_over_a_million_rows(gpu, torch):
     # each 4096 rows, four over the partial rows of a lane, 16 at the end.  Column 0 is a constant
     # of 1023.499 steps of the binade that a sum over every 64th row ends in: added one by one, half of
     # these additions would round down by half a step, 4000 U in all.
-    U, rows, d = 2.0**-24, 2**20 + 37, 8
+    rows, d = 2**20 + 37, 8
     x, _ = _matrix(torch, rows, d, "f32", seed=1)
     dy, _ = _matrix(torch, rows, d, "f32", pad=1, seed=2, offset=1.0)
     dy[:, 0] = 1023.499 * 2.0**-13
@@ -120,3 +123,35 @@ def test_distillation_of_a_student_masked_by_the_lowest_value(gpu, torch, rows, 
         assert ((loss.double() - ref).abs() <= tol).all()
         if grad:
             assert ((dz.double() - rdz).abs() <= ztol + _out_tol(torch, "f32", rdz)).all()
+
+
+def test_scores_in_several_blocks_of_logits(gpu):
+    # A vocabulary of which a block of logits (512 MiB) holds fewer rows than the texts have, so
+    # that a block ends inside a text: every position against the logits of the loss call in 64 bits.
+    V, batch, t, top = 300007, 3, 210, 4
+    block = (512 << 20) // (4 * V)
+    assert block < batch * t and block % t != 0
+    gm = gpu.Model.new(gpu.LmConfig(vocab=V, d_model=16, n_layer=2, expand=2, conv_k=3, mlp_mult=2, eps=1e-5, tau_max=8.0), 4, device=0)
+    rng = np.random.default_rng(3)
+    ids = rng.integers(0, V, batch * t).astype(np.uint32)
+    tg = np.roll(ids, -1)
+    tg[::11] = 0xFFFFFFFF
+    out = gm.score(ids, tg, batch, t, top)
+    _, lg = gm.loss(ids, tg, batch, t, want_logits=True)
+    rel = _sum_rel(V, _span(V))
+    for r in range(batch * t):
+        lp, ent, ti, tl = (out[k].reshape(batch * t, -1)[r] for k in ("logprob", "entropy", "top_ids", "top_logprobs"))
+        if tg[r] == 0xFFFFFFFF:
+            assert lp == 0 and ent == 0 and (ti == 0xFFFFFFFF).all() and np.isneginf(tl).all()
+            continue
+        z = lg[r].astype(np.float64)
+        p = z - z.max() - np.log(np.exp(z - z.max()).sum())
+        best = np.argsort(-lg[r], kind="stable")[:top]
+        assert np.array_equal(ti, best.astype(np.uint32))
+        assert abs(lp[0] - p[tg[r]]) <= rel + 16 * U * abs(p[tg[r]]) and (abs(tl - p[best]) <= rel + 16 * U * abs(p[best])).all()
+        assert abs(ent[0] + (np.exp(p) * p).sum()) <= (rel + 8 * U) * (2 + 2 * np.log(V))
+    # Alternatives asked for and not taken: the same scores.
+    lp = np.empty(batch * t, np.float32)
+    as_p = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+    gpu._check(gpu.lib().nk_model_score(gm.h, as_p(ids), as_p(tg), batch, t, top, as_p(lp), None, None, None))
+    assert np.array_equal(lp, out["logprob"].reshape(-1))
