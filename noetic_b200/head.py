@@ -63,6 +63,10 @@ def _matrix(a, what: str):
 def _vector(a, n: int, what: str, dtype=np.float32):
     if a is None:
         return None
+    a = np.asarray(a)
+    # (-1 in a signed array is 0xFFFFFFFF; the library looks at what is left.)
+    if dtype == np.uint32 and a.dtype.itemsize > 4 and a.size and (a.max() > NO_TOKEN or a.min() < -(1 << 31)):
+        raise ValueError(f"{what} must fit 32 bits")
     a = np.ascontiguousarray(a, dtype=dtype).reshape(-1)
     if a.size != n:
         raise ValueError(f"{what} must hold {n} values")

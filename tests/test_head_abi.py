@@ -194,3 +194,16 @@ def test_workspace_grows_no_further_than_its_limit(nb):
     # Nor do wide rows ask for more than a few sums of the parameters.
     assert nb.lib().nk_layer_norm_backward_workspace(1 << 10, 1 << 20, C.byref(n)) == 0
     assert n.value <= 64 * 2 * (1 << 20) * 4
+
+
+def test_python_mirror_refuses_ids_beyond_32_bits(nb):
+    # 2^32 + 1 is not token 1.
+    z, far = np.zeros((2, 4), np.float32), np.array([0, (1 << 32) + 1])
+    with pytest.raises(ValueError, match="32 bits"):
+        nb.token_logprobs(z, far)
+    with pytest.raises(ValueError, match="32 bits"):
+        nb.token_logprobs_backward(z, -far, np.zeros((2, 2)), g_logprob=np.ones(2))
+    with pytest.raises(ValueError, match="32 bits"):
+        nb.distill(z, far[:, None], np.zeros((2, 1)))
+    with pytest.raises(ValueError, match="32 bits"):
+        nb.head.model_score(None, far, far, 1, 2)
