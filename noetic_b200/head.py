@@ -119,6 +119,8 @@ def distill(logits, teacher_ids, teacher_logits, temperature: float = 1.0, row_w
     rows, vocab = z.shape
     if tl.shape[0] != rows:
         raise ValueError("teacher_logits must have a row for each row of the logits")
+    if np.ndim(teacher_ids) > 1 and np.shape(teacher_ids) != tl.shape:
+        raise ValueError("teacher_ids must have the shape of teacher_logits")
     ids = _vector(teacher_ids, tl.size, "teacher_ids", np.uint32)
     w = _vector(row_weight, rows, "row_weight")
     loss = np.empty(rows, np.float32)

@@ -207,3 +207,9 @@ def test_python_mirror_refuses_ids_beyond_32_bits(nb):
         nb.distill(z, far[:, None], np.zeros((2, 1)))
     with pytest.raises(ValueError, match="32 bits"):
         nb.head.model_score(None, far, far, 1, 2)
+
+
+def test_python_mirror_refuses_transposed_teacher_ids(nb):
+    # As many ids as logits, but another row's.
+    with pytest.raises(ValueError, match="shape"):
+        nb.distill(np.zeros((2, 4), np.float32), np.zeros((3, 2), np.uint32), np.zeros((2, 3)))
