@@ -20,11 +20,19 @@
  *     results are rounded once, on the way out.
  *   - Matrices are row-major with a row stride in elements (>= the width); an
  *     array only has to be aligned to its element.  Rows that start on 16-byte
- *     boundaries are read fastest.  What lies between the rows is not touched.
+ *     boundaries are read fastest.  Matrices of one call (logits and dlogits; x
+ *     and y; x, dy and dx) should start their rows at the same places of 16
+ *     bytes: equal strides, or strides that differ by multiples of 16 bytes.
+ *     Otherwise 16-bit gradients take three times as long, and the norm's
+ *     gradient, where dy starts elsewhere than x, five to nine times.  What lies
+ *     between the rows is not touched.
  *   - A token id is a u32.  0xFFFFFFFF means "no token"; so does, on the device,
  *     every id that is not below the vocabulary size (the host forms refuse
  *     those).
  *   - Results do not depend on scheduling: the same call gives the same bits.
+ *     How a row's sum is split goes by the number of rows, their strides and
+ *     places and what is asked for, so the same row in another call can differ in
+ *     its last bits.
  *   - NK_ERR_INVALID: a null array with a non-zero size, a pointer that is not
  *     device memory or not on the same device as the others, a misaligned one, a
  *     stride below the width, a size beyond the limits (rows <= 2^26, vocab and
@@ -68,7 +76,9 @@ typedef enum nk_dtype { NK_F32 = 0, NK_F16 = 1, NK_BF16 = 2 } nk_dtype;
  * what fills the places beyond a row's logits above -infinity.  Masked logits
  * are -infinity.  In a row that has nothing else, logprob and stats are
  * -infinity and entropy is 0.  A NaN or +infinity makes the row's numbers NaN;
- * a NaN is no alternative. */
+ * a NaN is no alternative.
+ * In calls of up to 148 rows a sure token's log probability (near 0) keeps its
+ * digits; beyond, log p is good to about 2^-24 of 1, as the sum 1 + rest is. */
 nk_status nk_token_logprobs_device(const void *logits, int dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
                                    const uint32_t *targets, float temperature, uint32_t top, float *logprob,
                                    float *entropy, float *stats, uint32_t *top_ids, float *top_logprobs,
@@ -137,10 +147,11 @@ nk_status nk_layer_norm(const void *x, int dtype, uint64_t rows, uint64_t width,
  *   dgain = sum over rows of dy n,  dbias = sum over rows of dy
  * dx, dgain and dbias are each nullable; dx can be the same array as dy, with
  * the same stride; accumulate != 0 adds to dgain and dbias instead of setting
- * them (dx is set).  The sums over rows are split and joined in a fixed order
- * through `workspace` (of nk_layer_norm_backward_workspace bytes, 16-byte
- * aligned; not needed without dgain and dbias): calls that overlap on the GPU,
- * replays of captured graphs among them, need a workspace each. */
+ * them (dx is set).  The sums over rows, in f32 (a term passes through at most
+ * rows / 32 + 64 additions), are split and joined in a fixed order through
+ * `workspace` (of nk_layer_norm_backward_workspace bytes, 16-byte aligned; not
+ * needed without dgain and dbias): calls that overlap on the GPU, replays of
+ * captured graphs among them, need a workspace each. */
 nk_status nk_layer_norm_backward_workspace(uint64_t rows, uint64_t width, uint64_t *bytes);
 nk_status nk_layer_norm_backward_device(const void *x, int dtype, uint64_t rows, uint64_t width, uint64_t x_stride,
                                         const float *gain, const float *mean, const float *rstd, int rms,
@@ -156,6 +167,8 @@ nk_status nk_layer_norm_backward(const void *x, int dtype, uint64_t rows, uint64
  * temperature 1.  ids and targets: host [batch * t], sequence-major; logprob,
  * entropy [batch * t], top_ids and top_logprobs [batch * t, top]: host, each
  * nullable.  Positions whose target is 0xFFFFFFFF have no scores, as above.
+ * A text's scores beside other texts, or cut elsewhere, can differ in the last
+ * digits (see nk_token_logprobs; the logits' product, too, goes by its rows).
  * Runs on a scratch decoder, as nk_model_loss does. */
 nk_status nk_model_score(nk_model *model, const uint32_t *ids, const uint32_t *targets, uint32_t batch, uint32_t t,
                          uint32_t top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprobs);

@@ -306,7 +306,8 @@ class Model:
     def score(self, ids, targets, batch: int, t: int, top: int = 0) -> dict:
         """Log probability and entropy of every position of `batch` sequences of
         `t` tokens ([batch, t]; targets 0xFFFFFFFF have none), and with `top` the
-        most probable tokens there (`top_ids`, `top_logprobs` [batch, t, top])."""
+        most probable tokens there (`top_ids`, `top_logprobs` [batch, t, top]).
+        The same text in another batch can differ in its last digits."""
         return head.model_score(self, ids, targets, batch, t, top)
 
     def close(self):

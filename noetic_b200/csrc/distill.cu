@@ -155,14 +155,18 @@ __device__ __forceinline__ void total_shares(const Entries<ENTRIES> &e, int n, u
 // puts the gradient's values in the entries' places.  Each CTA answers for the
 // entries in its part.
 //
-// 4096 rows of 16384 f32 with 32 entries take 92 us (5.5 TB/s, 0.83 of HBM's copy
-// rate), 8192 of 131072 bf16 with 64 take 980 us (4.4 TB/s, 0.67).  16-bit rows cost
-// the special-function unit two exponentials per element, one for the sum and one for the
-// gradient, which is half of what HBM leaves time for, and their instructions issue in turns
-// with the copies: without the exponentials the same rows measured 770 us, without
-// the cluster's exchange 872, without both 725.  Taking the exponentials of half of the
-// elements by a polynomial instead gained nothing, reading the row a second time from
-// L2 in place of shared memory cost 1084 us.
+// 4096 rows of 16384 f32 with 32 entries take 90 us (5.6 TB/s, 0.86 of HBM's copy
+// rate), 8192 of 131072 bf16 with 64 take 932 us (4.6 TB/s, 0.70; 980 on the GPU of what
+// follows).  16-bit rows cost the special-function unit two exponentials per element,
+// one for the sum and one for the gradient, about 480 us of its time, and their
+// instructions issue in turns with the copies: without the exponentials the same rows
+// measured 770 us, without the cluster's exchange, which every row waits for, 872,
+// without both 725.  Taking the exponentials of half of the elements by a polynomial
+// instead gained nothing, reading the row a second time from L2 in place of shared
+// memory cost 1084 us.  The loss alone keeps nothing and reads in vectors (stream_rest):
+// 8192 of 131072 bf16 475 us (0.69).  Where the gradient's rows start elsewhere than the
+// logits' it is stored element by element: 8192 rows of 65537 bf16, stride 65544, into
+// dense ones 1130 us where equal strides take 436; f32 rows of 16384 106 and 87.
 // The streaming threads' mark and the teacher warp's wait for it.
 template <int THREADS>
 __device__ __forceinline__ void mark_arrive() {
@@ -489,7 +493,8 @@ __global__ void __launch_bounds__(NT + 32, 3) distill_k(DistillArgs a, int log_c
 
 // ---------------------------------------------------------------- short rows: a warp each
 // The same in a warp, without a barrier but its own: 12 rows of 16 KB in the air
-// per SM.  16384 rows of 1024 f32 take 31 us (4.3 TB/s).
+// per SM.  16384 rows of 1024 f32 take 31 us (4.3 TB/s, 0.68): a warp's loads, sums
+// and stores follow one another, and no other row's are fetched meanwhile.
 constexpr int WARP_ROWS = 4;
 constexpr int WARP_VECTORS = 1024;  // of a row, at most
 

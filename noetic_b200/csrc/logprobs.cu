@@ -349,8 +349,10 @@ __global__ void __launch_bounds__(32 * WARP_ROWS, 4) token_logprobs_warp_k(Logpr
 // the GPU), each with a contiguous part of it.  What bounds it: HBM; 16-bit
 // logits need one exponential per two bytes, 16 of which an SM's
 // special-function unit makes per clock, 1.4 times what HBM delivers.  4096 rows
-// of 131072 bf16 take 192 us with 20 alternatives (5.6 TB/s, 0.85 of the copy
-// rate) and 176 without (0.93), 2048 of f32 173 with them (0.95).
+// of 131072 bf16 take 180 us with 20 alternatives (6.0 TB/s, 0.91 of the copy rate)
+// and 159 without (as fast as it only reads, 1.03), 2048 of f32 170 with them (0.97):
+// two sets of inputs in turn.  Among passes over other inputs the first takes 195 to
+// 207.
 constexpr int LP_SLOTS = 32;      // groups per thread
 constexpr int HITS = 512;
 constexpr int CANDIDATES = 1024;  // at least MAX_CLUSTER * TOP_MAX
@@ -443,7 +445,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_k(LogprobsArgs a
 // The gradient, element by element: a CTA takes LP_NT * LP_U vectors of one
 // row, read once and written once.  Bound by HBM: 4096 rows of 32768 f32, an
 // eighth of them without a target (not read), take 152 us (6.6 TB/s), 2048 rows of
-// 65537 bf16, whose vectors start anywhere, 95 us (5.6 TB/s).
+// 65537 bf16, read and written in vectors that start at the same places, 93 us (5.8
+// TB/s).  Where the gradient's rows start elsewhere than the logits' it is stored
+// element by element: these rows of stride 65544 into dense ones 337 us, f32 rows,
+// whose stores still fill their sectors, 165 as dense.
 template <class T>
 __global__ void __launch_bounds__(LP_NT) token_logprobs_backward_k(LogprobsGradArgs a, int chunks) {
     // (A 32-bit division: rows * chunks is below 2^31.)
@@ -560,7 +565,8 @@ cudaError_t launch_logprobs(const LogprobsArgs &a, cudaStream_t st) {
     if (small) return launch_blocks<T, 128, false>(a, st);
     // With few rows the SMs wait for memory, and a single row's log probability
     // may be all that is looked at: fine sums (one row of 32768 f32 10 us with and
-    // without, 120 of 131072 23 and 21; but 4096 of 131072 bf16 243 and 192).
+    // without, 120 of 131072 23 and 21; but 4096 of 131072 bf16 243 and 192, one after
+    // the other on one GPU).
     return a.rows <= 148 ? launch_blocks<T, 256, true>(a, st) : launch_blocks<T, 256, false>(a, st);
 }
 

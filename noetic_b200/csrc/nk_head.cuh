@@ -284,7 +284,7 @@ __device__ __forceinline__ float add_some(const uint4 (&raw)[U], int v, int v1, 
 // is called for every U; returns the number of these.  With MASK a last batch
 // that is not full counts its missing vectors as masked ones.  (Other warps'
 // work covers the loads: fetching the next batch ahead measured 213 us a pass
-// over 4096 rows of 131072 bf16, eight vectors at a time without it 207.)
+// over 4096 rows of 131072 bf16, eight vectors at a time without it 207 in the same run.)
 template <class T, int NT, int U, bool ENT, bool MASK = false, bool FINE = false, class F>
 __device__ __forceinline__ int stream_sums(const T *body, int v0, int v1, int tid, float scale, SoftSums &sums, F &&each) {
     int batch = 0, v = v0 + tid;

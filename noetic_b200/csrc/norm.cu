@@ -267,7 +267,7 @@ __device__ __forceinline__ void column_part(const P &p, const float *v, float ot
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // ---------------------------------------------------------------- forward
-// 16384 rows of 4096 bf16 in 49 us (5.5 TB/s, 0.83 of the copy rate); 8192 rows of
+// 16384 rows of 4096 bf16 in 49 to 52 us (5.3 TB/s, 0.81 of the copy rate); 8192 rows of
 // 8192 the same.  Four rows on their way to each group, since a block's own
 // reductions leave memory idle otherwise.  Rows of 64 x 1024 f32 cost their launch.
 template <class T, int G, int VALS, bool EDGE>
@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(NM_NT + 32, 2) norm_cluster_rows_k(NormArgs a,
 // take 124 us, a third of HBM's rate.
 constexpr int WIDE_NT = 512;
 
-// f(pair of elements, index of the first) over a thread's part of a row, which
-// `at(v)` gives as 16 bytes of N elements (VEC) or one element.
+// f(v, the elements of unit v) over a thread's part of a row, whose units are 16 bytes
+// of N elements (VEC) or one element, as `at(v)` gives them.
 template <class T, bool VEC, class At, class F>
 __device__ __forceinline__ void wide_each(int width, At &&at, F &&f) {
     if constexpr (VEC) {
@@ -593,8 +593,10 @@ __global__ void __launch_bounds__(WIDE_NT) norm_wide_rows_k(NormArgs a) {
 // groups' registers joined in shared memory in their order, one row of the
 // workspace per block.  The row is unpacked twice, once for the sums and once
 // for dx: it waits in shared memory, not in registers.  65536 rows of 1024 bf16 with
-// the parameters' sums in 79 us (5.1 TB/s); then the instructions per element
-// (about 10, two unpackings) are near to binding.
+// the parameters' sums in 76 us (5.3 TB/s); then the instructions per element
+// (about 10, two unpackings) are near to binding.  With EDGE 65536 x 1001 bf16 105 us
+// (0.58 of the copy rate) and f32 141 (0.85); into rows that start elsewhere, by way of
+// the stage, 65536 x 1024 bf16 of stride 1025 into dense rows 203.
 template <class T, int G, int VALS, bool EDGE, bool PARAMS>
 __global__ void __launch_bounds__(G > NM_NT ? G : NM_NT, G > NM_NT ? 1 : 2) norm_backward_k(NormGradArgs a, int same) {
     constexpr int NT = G > NM_NT ? G : NM_NT, GROUPS = NT / G;
@@ -821,6 +823,9 @@ __global__ void __launch_bounds__(NM_NT + 32, 2) norm_cluster_backward_k(NormGra
     }
 }
 
+// Rows too wide for the kernels above, and those of which x and dy (VEC: dx too) start at
+// different places of a 16-byte unit, at any width: 65536 x 1024 bf16 with dy of stride
+// 1025 take 658 us, nine times what equal strides do (f32 625 us, five times).
 template <class T, bool VEC>
 __global__ void __launch_bounds__(WIDE_NT) norm_wide_dx_k(NormGradArgs a) {
     __shared__ float red[32];

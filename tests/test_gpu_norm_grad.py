@@ -16,6 +16,7 @@ Tolerances count roundings, U = 2^-24 being half a step of f32.
  - A result of a narrower type is off by half a step more.
 """
 
+import ctypes as C
 import math
 
 import pytest
@@ -180,3 +181,15 @@ def test_gradient_along_a_direction_against_differences(gpu, torch, rows, d, lay
     terms = (dx.double() * v).abs().sum() + (dg.double() * vg).abs().sum() + (0.0 if rms else (db.double() * vb).abs().sum())
     got = (dx.double() * v).sum() + (dg.double() * vg).sum() + (0.0 if rms else (db.double() * vb).sum())
     assert abs(num - got) <= (1e-6 + 4 * (d / 256 + 60) * U) * terms
+
+
+def test_the_workspace_holds_one_row_per_block_and_no_more(nb):
+    # 296 blocks, or for rows too wide for a cluster 64, of two f32 per column; never more than one per row.
+    n = C.c_uint64()
+    for rows in (0, 1, 63, 64, 65, 295, 296, 297, 1 << 20, 1 << 26):
+        for width, most in ((1, 296), (100, 296), (8192, 296), (32768, 296), (32769, 64), (1 << 20, 64)):
+            status = nb.lib().nk_layer_norm_backward_workspace(rows, width, C.byref(n))
+            if rows * width > 1 << 37:  # beyond what a matrix may hold
+                assert status == nb.NK_ERR_INVALID and n.value == 0
+                continue
+            assert status == 0 and n.value == min(max(rows, 1), most) * 2 * width * 4
