@@ -1,6 +1,6 @@
 """Calls of include/noetic/head.h that the operators' own tests do not make: two
-host threads at once, sums over many rows, logits at the end of f32's range, texts
-longer than a block of logits."""
+host threads at once, sums over many rows, logits at the end of f32's range,
+special rows in every kernel, texts longer than a block of logits."""
 
 import ctypes as C
 import threading
@@ -8,8 +8,8 @@ import threading
 import numpy as np
 import pytest
 
-from test_gpu_head import (CODE, U, _distill, _matrix, _norm, _norm_grad, _out_tol, _p, _ref_distill, _span,  # noqa: F401
-                           _sum_rel, torch)  # (torch: the fixture)
+from test_gpu_head import (CODE, INF, NAN, NONE, U, _check_logprobs, _distill, _dt, _grad, _logprobs, _matrix, _norm,  # noqa: F401
+                           _norm_grad, _out_tol, _p, _ref_distill, _ref_grad, _span, _sum_rel, torch)  # (torch: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,82 @@ def test_scores_in_several_blocks_of_logits(gpu):
     as_p = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
     gpu._check(gpu.lib().nk_model_score(gm.h, as_p(ids), as_p(tg), batch, t, top, as_p(lp), None, None, None))
     assert np.array_equal(lp, out["logprob"].reshape(-1))
+
+
+# Rows, vocabulary: one block or cluster to a row, a warp, blocks of 128 and of 256 threads, clusters.
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,V", [(9, 1000), (603, 1000), (603, 1003), (720, 40000), (1260, 70001), (5, 130000), (513, 9)])
+def test_special_rows_in_every_kernel_of_the_log_probabilities(gpu, torch, dtype, rows, V):
+    low, half = torch.finfo(_dt(torch, dtype)).min, V // 2
+    z, _ = _matrix(torch, rows, V, dtype, seed=V)
+    z = z.contiguous()
+    t = torch.randint(0, half, (rows,), device="cuda", dtype=torch.int32, generator=torch.Generator(device="cuda").manual_seed(V))
+    kind = torch.arange(rows, device="cuda") % 9
+    rest = slice(half, V)
+    z[kind == 0] = -INF                  # nothing left
+    z[kind == 1] = low                   # the lowest value alone: uniform
+    z[kind == 2, rest] = low
+    z[kind == 3, rest] = -INF
+    z[kind == 4, half - 1] = NAN
+    z[kind == 5, V - 1] = INF
+    z[kind == 6] = -INF                  # one token left, at the end
+    z[kind == 6, V - 1] = 1.0
+    t[kind == 6] = V - 1
+    z[kind == 7] = NAN                   # not read
+    t[kind == 7] = NONE
+    broken, plain = (kind == 4) | (kind == 5), (kind == 1) | (kind == 2) | (kind == 3) | (kind == 6) | (kind == 8)
+    for T, top in ((1.0, 0), (1.0, 20), (0.3, 5), (40.0, 128)):
+        out = _logprobs(gpu, torch, z, t, T, top, dtype)
+        _check_logprobs(torch, {k: None if v is None else v[plain] for k, v in out.items()}, z[plain], t[plain], T, top)
+        none, gone = kind == 0, kind == 7
+        assert (out["logprob"][none] == -INF).all() and (out["entropy"][none] == 0).all() and (out["stats"][none] == -INF).all()
+        assert torch.isnan(out["logprob"][broken]).all() and torch.isnan(out["entropy"][broken]).all()
+        for k in ("logprob", "entropy", "stats"):
+            assert (out[k][gone] == 0).all()
+        assert (out["logprob"][kind == 6] == 0).all() and (out["entropy"][kind == 6] == 0).all()
+        if top:
+            assert (out["top_ids"][none | gone] == NONE).all() and (out["top_logprobs"][none | gone] == -INF).all()
+            assert (out["top_ids"][kind == 4] != half - 1).all() and (out["top_ids"][kind == 5, 0] == V - 1).all()
+        gl = torch.ones(rows, device="cuda")
+        fw = out if T != 40.0 else _logprobs(gpu, torch, z, t, T, 0, dtype)
+        dz = _grad(gpu, torch, z, t, T, fw["stats"], fw["entropy"], gl, 0.5 * gl, dtype)
+        assert (dz[none | gone] == 0).all() and torch.isnan(dz[broken]).all()
+        ref, tol = _ref_grad(torch, z[plain], t[plain], T, fw["stats"][plain], fw["entropy"][plain], gl[plain], 0.5 * gl[plain])
+        # A probability below 2^-126 counts as 0: at most that is lost, times |g_logprob| + |g_entropy| (|log p| + H),
+        # log p = -126 log 2 there (the logarithm of a smaller one grows slower than it falls), over T.
+        lost = 2.0**-126 * (1 + 0.5 * (126 * np.log(2) + np.log(V))) / T
+        assert ((dz[plain].double() - ref).abs() <= tol + lost + _out_tol(torch, dtype, ref)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,V", [(8, 500), (1003, 500), (1003, 1001), (5, 130000), (700, 30000), (130, 200001), (515, 9)])
+def test_special_rows_in_every_kernel_of_the_distillation(gpu, torch, dtype, rows, V):
+    z, _ = _matrix(torch, rows, V, dtype, seed=V)
+    z = z.contiguous()
+    kind = torch.arange(rows, device="cuda") % 8
+    ids = torch.tensor([0, V // 2, V - 1, V // 2, 2], device="cuda", dtype=torch.int32).repeat(rows, 1)  # one of them twice
+    t = torch.randn(rows, 5, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+    w = torch.ones(rows, device="cuda")
+    z[kind == 0] = NAN                   # no entries: not read
+    ids[kind == 0] = NONE
+    z[kind == 1, 3:V // 2] = -INF        # masked where no entry is
+    z[kind == 2, V - 2] = NAN
+    t[kind == 3] = -INF                  # no entries either
+    z[kind == 4] = NAN                   # weight 0
+    w[kind == 4] = 0.0
+    z[kind == 5, V - 1] = -INF           # the teacher wants what the student cannot say
+    z[kind == 6] = -INF                  # a student that can say nothing
+    t[kind == 7, 0] = torch.finfo(torch.float32).min
+    for T in (1.0, 2.5):
+        loss, dz = _distill(gpu, torch, z, ids, t, T, w, 0.7, dtype, "f32")
+        alone = _distill(gpu, torch, z, ids, t, T, w, 0.7, dtype, "f32", grad=False)[0]
+        ref, tol, rdz, ztol = _ref_distill(torch, z, ids, t, T, w, 0.7)
+        plain = (kind == 1) | (kind == 7)
+        for got in (loss, alone):
+            assert ((got[plain].double() - ref[plain]).abs() <= tol[plain]).all()
+            assert (got[(kind == 0) | (kind == 3)] == 0).all()
+            assert torch.isnan(got[(kind == 2) | (kind == 4)]).all()
+            assert (got[(kind == 5) | (kind == 6)] == INF).all()
+        right = plain | (kind == 5)
+        assert ((dz[right].double() - rdz[right]).abs() <= ztol[right] + _out_tol(torch, dtype, rdz[right])).all()
+        assert (dz[(kind == 0) | (kind == 3) | (kind == 4) | (kind == 6)] == 0).all() and torch.isnan(dz[kind == 2]).all()
