@@ -193,3 +193,40 @@ def test_the_workspace_holds_one_row_per_block_and_no_more(nb):
                 assert status == nb.NK_ERR_INVALID and n.value == 0
                 continue
             assert status == 0 and n.value == min(max(rows, 1), most) * 2 * width * 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("rows,d", [(5003, 104), (5003, 41), (1301, 1401), (700, 2800), (331, 7001), (310, 8192), (301, 16384),
+                                    (130, 20000), (130, 32768), (70, 33000), (67, 9001)])
+def test_a_broken_row_stays_alone(gpu, torch, rows, d, layout, dtype):
+    # NaN and infinities in some rows: all other rows, and the parameters' sums that do not see
+    # them, have the bits that they have without.
+    (xp, xs), (yp, ys), (op, os_) = LAYOUTS[layout](16 // SIZE[dtype])
+    x, _ = _matrix(torch, rows, d, dtype, xp, xs, scale=1.5, seed=d, offset=0.7)
+    dy, _ = _matrix(torch, rows, d, dtype, yp, ys, scale=0.5, seed=d + 1)
+    out, _ = _matrix(torch, rows, d, dtype, op, os_)
+    gain = torch.linspace(0.5, 1.5, d, device="cuda")
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[[0, 1, rows // 2, rows - 1]] = True
+    c = d // 3
+    for rms in (False, True):
+        y, mean, rstd = _norm(gpu, torch, x, gain, None, 1e-5, rms, dtype, out)
+        y = y.clone()
+        dx, dg, db = _norm_grad(gpu, torch, x, dy, gain, mean, rstd, dtype, dx=out)
+        dx = dx.clone()
+        kept = x[bad].clone()
+        x[0, c], x[1, d - 1], x[rows // 2, 0], x[rows - 1, c] = float("nan"), float("inf"), -float("inf"), float("nan")
+        y2, mean2, rstd2 = _norm(gpu, torch, x, gain, None, 1e-5, rms, dtype, out)
+        assert torch.equal(y2[~bad], y[~bad]) and torch.equal(rstd2[~bad], rstd[~bad])
+        assert torch.isnan(y2[[0, rows - 1]]).all() and not torch.isfinite(y2[1, d - 1]) and not torch.isfinite(y2[rows // 2, 0])
+        x[bad] = kept
+        kept = dy[bad].clone()
+        dy[bad, c] = float("nan")
+        dx2, dg2, db2 = _norm_grad(gpu, torch, x, dy, gain, mean, rstd, dtype, dx=out)
+        assert torch.equal(dx2[~bad], dx[~bad]) and torch.isnan(dx2[bad]).all()
+        others = torch.arange(d, device="cuda") != c
+        for a, b in ((dg, dg2), (db, db2)):
+            assert a is None or (torch.equal(a[others], b[others]) and torch.isnan(b[c]))
+        dy[bad] = kept
