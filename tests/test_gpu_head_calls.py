@@ -1,6 +1,7 @@
 """Calls of include/noetic/head.h that the operators' own tests do not make: two
 host threads at once, sums over many rows, logits at the end of f32's range,
-special rows in every kernel, texts longer than a block of logits."""
+special rows in every kernel, texts longer than a block of logits, streams and
+graphs side by side."""
 
 import ctypes as C
 import threading
@@ -234,3 +235,96 @@ def test_special_rows_in_every_kernel_of_the_distillation(gpu, torch, dtype, row
         right = plain | (kind == 5)
         assert ((dz[right].double() - rdz[right]).abs() <= ztol[right] + _out_tol(torch, dtype, rdz[right])).all()
         assert (dz[(kind == 0) | (kind == 3) | (kind == 4) | (kind == 6)] == 0).all() and torch.isnan(dz[kind == 2]).all()
+
+
+def _mixed_calls(gpu, torch, seed):
+    """Calls of the kernels of short, long and wide rows on buffers of their own: (a function of the
+    stream, its outputs) each."""
+    L, g = gpu.lib(), torch.Generator(device="cuda").manual_seed(seed)
+    keep = []
+
+    def rn(*n, dtype="f32"):
+        keep.append(torch.randn(*n, generator=g, device="cuda").to(_dt(torch, dtype)))
+        return keep[-1]
+
+    def out(*n, dtype=None):
+        keep.append(torch.zeros(*n, device="cuda", dtype=dtype or torch.float32))
+        return keep[-1]
+
+    def ids(*n, V):
+        keep.append(torch.randint(0, V, n, generator=g, device="cuda", dtype=torch.int32))
+        return keep[-1]
+
+    calls = []
+    for R, V, dtype, top in ((700, 1024, "f32", 128), (5, 130000, "bf16", 20), (700, 40000, "f16", 7)):
+        z, t, lp, ti = 3 * rn(R, V, dtype=dtype), ids(R, V=V), out(R), out(R, top, dtype=torch.int32)
+        keep.append(z)
+        calls.append((lambda s, z=z, t=t, lp=lp, ti=ti, R=R, V=V, top=top, c=CODE[dtype]: L.nk_token_logprobs_device(
+            _p(z), c, R, V, V, _p(t), 1.0, top, _p(lp), None, None, _p(ti), None, s), (lp, ti)))
+    for R, V, dtype, K in ((600, 4000, "f32", 40), (300, 70000, "bf16", 33), (3, 131072, "f16", 200)):
+        z, i, q, ls, dz = rn(R, V, dtype=dtype), ids(R, K, V=V), rn(R, K), out(R), out(R, V, dtype=_dt(torch, dtype))
+        calls.append((lambda s, z=z, i=i, q=q, ls=ls, dz=dz, R=R, V=V, K=K, c=CODE[dtype]: L.nk_distill_device(
+            _p(z), c, R, V, V, _p(i), _p(q), 0, K, 2.0, _p(ls), None, 1.0, _p(dz), V, s), (ls, dz)))
+    for R, d, dtype in ((700, 1001, "bf16"), (200, 20000, "f32"), (300, 16384, "bf16"), (70, 33001, "f16"), (900, 104, "f16")):
+        x, dy, gain = rn(R, d, dtype=dtype), rn(R, d, dtype=dtype), rn(d)
+        y, dx = (out(R * d + 1, dtype=_dt(torch, dtype))[1:] for _ in range(2))
+        mean, rstd, dg, db = out(R), out(R), out(d), out(d)
+        n = C.c_uint64()
+        gpu._check(L.nk_layer_norm_backward_workspace(R, d, C.byref(n)))
+        ws = out(n.value // 4)
+
+        def both(s, x=x, dy=dy, gain=gain, y=y, dx=dx, mean=mean, rstd=rstd, dg=dg, db=db, ws=ws, n=n.value, R=R, d=d, c=CODE[dtype]):
+            return L.nk_layer_norm_device(_p(x), c, R, d, d, _p(gain), None, 1e-5, 0, _p(y), d, _p(mean), _p(rstd), s) or \
+                L.nk_layer_norm_backward_device(_p(x), c, R, d, d, _p(gain), _p(mean), _p(rstd), 0, _p(dy), d, _p(dx), d, _p(dg),
+                                                _p(db), 0, _p(ws), n, s)
+
+        calls.append((both, (y, dx, mean, rstd, dg, db)))
+    return calls, keep
+
+
+def test_large_calls_on_two_streams_and_in_graphs(gpu, torch):
+    sets = [_mixed_calls(gpu, torch, k) for k in (1, 2)]
+
+    def run(calls):
+        s = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        for f, _ in calls:
+            assert f(s) == 0, gpu.lib().nk_last_error()
+
+    want = []
+    for calls, _ in sets:
+        run(calls)
+        torch.cuda.synchronize()
+        want.append([o.clone() for _, outs in calls for o in outs])
+
+    def clear():
+        torch.cuda.synchronize()
+        for calls, _ in sets:
+            for _, outs in calls:
+                for o in outs:
+                    o.zero_()
+        torch.cuda.synchronize()
+
+    def same():
+        torch.cuda.synchronize()
+        return all(torch.equal(a, b) for (calls, _), w in zip(sets, want) for a, b in zip((o for _, outs in calls for o in outs), w))
+
+    streams = [torch.cuda.Stream() for _ in sets]
+    clear()
+    for _ in range(3):
+        for (calls, _), st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                run(calls)
+    assert same()
+    graphs = []
+    for calls, _ in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(calls)
+        graphs.append(g)
+    clear()
+    for _ in range(3):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    assert same()
+    del graphs
