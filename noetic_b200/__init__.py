@@ -23,7 +23,9 @@ reference (noetic crate)               here
 
 Beyond the reference (:mod:`noetic_b200.head`, ``include/noetic/head.h``):
 :func:`token_logprobs`, :func:`distill` and :func:`layer_norm` with their
-gradients, and :meth:`Model.score`.
+gradients, and :meth:`Model.score`; :mod:`noetic_b200.train`,
+``include/noetic/train.h``: :func:`linear_cross_entropy` with its gradients, and
+:func:`adamw_step_many`.
 
 Every computation runs on the GPU through hand-written sm_100a kernels.  There
 is no CPU fallback: importing works without a GPU, but every call that needs
@@ -41,7 +43,9 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import head
+from . import train
 from .head import (NO_TOKEN, distill, layer_norm, layer_norm_backward, token_logprobs, token_logprobs_backward)
+from .train import adamw_step_many, linear_cross_entropy, linear_cross_entropy_backward
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnoetic_gpu.so")
@@ -150,7 +154,7 @@ def lib():
             raise NoeticError(NK_ERR_UNSUPPORTED,
                               f"{LIB_PATH} is not built; run python noetic_b200/make_lib.py")
         L = C.CDLL(LIB_PATH)
-        for name, (res, args) in (*SIGNATURES.items(), *head.SIGNATURES.items()):
+        for name, (res, args) in (*SIGNATURES.items(), *head.SIGNATURES.items(), *train.SIGNATURES.items()):
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

@@ -1,0 +1,354 @@
+// adamw_many.cu -- one AdamW step (optim.rs:33-72) over all of a model's
+// tensors, with moments in 32 bits or in 8 bits and a scale for each block of
+// 256, and the gradients' norm that the step can clip them by.
+//
+//   g = grad c,  m' = b1 m + (1 - b1) g,  v' = b2 v + (1 - b2) g g,
+//   val' = val - lr (m' / (1 - b1^t) / (sqrt(v' / (1 - b2^t)) + eps) + wd val)
+//
+// Bound: HBM.  An element moves 8 bytes of val, 2 or 4 of gradient, 16 (32-bit)
+// or 4 (8-bit) of moments and 2 of the optional copy, and the norm reads the
+// gradients once more before.
+
+#include <algorithm>
+#include <cuda_fp8.h>
+
+#include "nk_head.cuh"
+#include "nk_train.h"
+
+namespace nk {
+
+namespace {
+
+constexpr float E4M3_MAX = 448.0f;
+constexpr float E4M3_TINY = 0.001953125f;  // 2^-9, the smallest number above 0
+// Blocks whose largest value is below this are stored as zeros: 448 / value
+// would leave f32's range (values like that come of gradients below 1e-30).
+constexpr float SCALE_MIN = 7.8886090522101181e-31f;  // 2^-100
+constexpr float ROOT_MAX = 1.8446742974197924e19f;    // the root of f32's largest value
+constexpr float MOMENT_MAX = 1.2676506002282294e30f;  // 2^100: m / (1 - b1^t) stays in range
+
+// Four gradients from element 4 i on.
+template <class G>
+__device__ __forceinline__ void load4(const G *p, float (&g)[4]) {
+    if constexpr (sizeof(G) == 4) {
+        const float4 q = __ldcs(reinterpret_cast<const float4 *>(p));
+        g[0] = q.x, g[1] = q.y, g[2] = q.z, g[3] = q.w;
+    } else {
+        const uint2 q = __ldcs(reinterpret_cast<const uint2 *>(p));
+        const G *h = reinterpret_cast<const G *>(&q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = to_f32(h[i]);
+    }
+}
+
+// ---------------------------------------------------------------- norm
+template <class G>
+__device__ __forceinline__ double chunk_squares(const G *grad, uint32_t n, bool vec) {
+    double s = 0.0;
+    uint32_t done = 0;
+    if (vec) {
+        done = n & ~3u;
+        for (uint32_t i = threadIdx.x * 4; i < done; i += blockDim.x * 4) {
+            float g[4];
+            load4(grad + i, g);
+            // (A group of four in f32, the groups in 64 bits.)
+            s += (double)(fmaf(g[0], g[0], g[1] * g[1]) + fmaf(g[2], g[2], g[3] * g[3]));
+        }
+    }
+    for (uint32_t i = done + threadIdx.x; i < n; i += blockDim.x) {
+        const float g = to_f32(grad[i]);
+        s += (double)(g * g);
+    }
+    return s;
+}
+
+__device__ __forceinline__ double block_sum_d(double v, double *red) {
+    v = warp_sum_d(v);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    return warp_sum_d(lane < (int)(blockDim.x >> 5) ? red[lane] : 0.0);
+}
+
+__device__ __forceinline__ bool aligned(const void *p, uint32_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// Each chunk's sum of squares to its own place; the block that finishes last
+// adds them in a fixed order, so the norm does not depend on scheduling.
+__global__ void __launch_bounds__(256) adamw_norm_k(AdamwMany p, float grad_scale, float max_norm, float *norm,
+                                                    uint32_t *bad) {
+    __shared__ double red[32];
+    __shared__ bool last;
+    for (uint32_t c = blockIdx.x; c < p.n_chunks; c += gridDim.x) {
+        const AdamwChunk ch = p.chunks[c];
+        const nk_adamw_tensor &t = p.tensors[ch.tensor];
+        double s;
+        if (t.grad_dtype == NK_F32) {
+            const float *g = (const float *)t.grad + ch.first;
+            s = chunk_squares(g, ch.n, aligned(g, 16));
+        } else if (t.grad_dtype == NK_F16) {
+            const __half *g = (const __half *)t.grad + ch.first;
+            s = chunk_squares(g, ch.n, aligned(g, 8));
+        } else {
+            const __nv_bfloat16 *g = (const __nv_bfloat16 *)t.grad + ch.first;
+            s = chunk_squares(g, ch.n, aligned(g, 8));
+        }
+        s = block_sum_d(s, red);
+        if (threadIdx.x == 0) p.partial[c] = s;
+    }
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double s = 0.0;
+    for (uint32_t c = threadIdx.x; c < p.n_chunks; c += blockDim.x) s += __ldcg(p.partial + c);
+    s = block_sum_d(s, red);
+    if (threadIdx.x == 0) {
+        const float all = (float)(sqrt(s) * fabs((double)grad_scale));
+        if (norm) *norm = all;
+        if (max_norm > 0.0f) {
+            const bool fine = isfinite(all);
+            p.clip[0] = all > max_norm ? grad_scale * __fdiv_rn(max_norm, all) : grad_scale;
+            p.clip[1] = fine ? 1.0f : 0.0f;
+            if (!fine && bad) *bad = 1u;
+        }
+        *p.ticket = 0u;
+    }
+}
+
+// ---------------------------------------------------------------- the step
+// The reference's operations, each correctly rounded, in its order.  False: the
+// element stays as it is.
+__device__ __forceinline__ bool adamw_element(float &val, float grad, float c, float &m, float &v, const AdamwParams &a,
+                                              bool decay) {
+    if (!isfinite(grad) || !isfinite(val)) return false;
+    const float g = __fmul_rn(grad, c);
+    m = __fadd_rn(__fmul_rn(a.b1, m), __fmul_rn(__fsub_rn(1.0f, a.b1), g));
+    v = __fadd_rn(__fmul_rn(a.b2, v), __fmul_rn(__fmul_rn(__fsub_rn(1.0f, a.b2), g), g));
+    const float mh = __fmul_rn(m, a.inv_bc1), vh = __fmul_rn(v, a.inv_bc2);
+    float upd = __fdiv_rn(mh, __fadd_rn(__fsqrt_rn(vh), a.eps));
+    if (decay) upd = __fadd_rn(upd, __fmul_rn(a.wd, val));
+    val = __fsub_rn(val, __fmul_rn(a.lr, upd));
+    return true;
+}
+
+__device__ __forceinline__ void store_copy(void *copy, int dtype, uint64_t i, float v) {
+    if (dtype == NK_F16)
+        ((__half *)copy)[i] = from_f32<__half>(v);
+    else
+        ((__nv_bfloat16 *)copy)[i] = from_f32<__nv_bfloat16>(v);
+}
+// Four values from element i on, a multiple of 4 of an 8-byte aligned copy.
+__device__ __forceinline__ void store_copy4(void *copy, int dtype, uint64_t i, const float (&v)[4]) {
+    uint2 q;
+    if (dtype == NK_F16) {
+        __half *h = reinterpret_cast<__half *>(&q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = from_f32<__half>(v[e]);
+    } else {
+        __nv_bfloat16 *h = reinterpret_cast<__nv_bfloat16 *>(&q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = from_f32<__nv_bfloat16>(v[e]);
+    }
+    __stcs(reinterpret_cast<uint2 *>((char *)copy + 2 * i), q);
+}
+
+template <class G>
+__device__ __forceinline__ bool chunk_step32(const nk_adamw_tensor &t, const AdamwChunk &ch, const AdamwParams &a,
+                                             float c, bool decay) {
+    float *val = t.val + ch.first, *m = (float *)t.m + ch.first, *v = (float *)t.v + ch.first;
+    const G *grad = (const G *)t.grad + ch.first;
+    bool ok = true;
+    uint32_t done = 0;
+    if (aligned(val, 16) && aligned(m, 16) && aligned(v, 16) && aligned(grad, 4 * sizeof(G)) &&
+        (!t.copy || aligned((char *)t.copy + 2 * ch.first, 8))) {
+        done = ch.n & ~3u;
+        for (uint32_t i = threadIdx.x * 4; i < done; i += blockDim.x * 4) {
+            float g[4];
+            load4(grad + i, g);
+            const float4 pq = __ldcs(reinterpret_cast<float4 *>(val + i)), mq = __ldcs(reinterpret_cast<float4 *>(m + i)),
+                         vq = __ldcs(reinterpret_cast<float4 *>(v + i));
+            float pv[4] = {pq.x, pq.y, pq.z, pq.w}, mv[4] = {mq.x, mq.y, mq.z, mq.w}, vv[4] = {vq.x, vq.y, vq.z, vq.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ok &= adamw_element(pv[e], g[e], c, mv[e], vv[e], a, decay);
+            __stcs(reinterpret_cast<float4 *>(val + i), make_float4(pv[0], pv[1], pv[2], pv[3]));
+            __stcs(reinterpret_cast<float4 *>(m + i), make_float4(mv[0], mv[1], mv[2], mv[3]));
+            __stcs(reinterpret_cast<float4 *>(v + i), make_float4(vv[0], vv[1], vv[2], vv[3]));
+            if (t.copy) store_copy4(t.copy, t.copy_dtype, ch.first + i, pv);
+        }
+    }
+    for (uint32_t i = done + threadIdx.x; i < ch.n; i += blockDim.x) {
+        float pv = val[i], mv = m[i], vv = v[i];
+        ok &= adamw_element(pv, to_f32(grad[i]), c, mv, vv, a, decay);
+        val[i] = pv;
+        m[i] = mv;
+        v[i] = vv;
+        if (t.copy) store_copy(t.copy, t.copy_dtype, ch.first + i, pv);
+    }
+    return ok;
+}
+
+__device__ __forceinline__ float from_e4m3(uint8_t b) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
+}
+__device__ __forceinline__ uint8_t to_e4m3(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// A warp steps one block of up to 256 elements: lane l holds elements 4 l .. + 3
+// and 128 + 4 l .. + 3, so the block's largest |m| and sqrt(v) are two shuffles'
+// reductions and nothing is read twice.
+template <class G>
+__device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t first, uint32_t n, const AdamwParams &a,
+                                            float c, bool decay, bool vec) {
+    const int lane = threadIdx.x & 31;
+    float *val = t.val + first;
+    uint8_t *m = (uint8_t *)t.m + first, *v = (uint8_t *)t.v + first;
+    const G *grad = (const G *)t.grad + first;
+    const float ms = t.m_scale[first / NK_ADAMW_BLOCK], vs = t.v_scale[first / NK_ADAMW_BLOCK];
+    float pv[2][4], g[2][4], mv[2][4], rv[2][4];
+    uint32_t mb[2], vb[2];
+    vec &= n == NK_ADAMW_BLOCK;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t at = h * 128 + lane * 4;
+        if (vec) {
+            const float4 q = __ldcs(reinterpret_cast<const float4 *>(val + at));
+            pv[h][0] = q.x, pv[h][1] = q.y, pv[h][2] = q.z, pv[h][3] = q.w;
+            load4(grad + at, g[h]);
+            mb[h] = __ldcs(reinterpret_cast<const uint32_t *>(m + at));
+            vb[h] = __ldcs(reinterpret_cast<const uint32_t *>(v + at));
+        } else {
+            mb[h] = vb[h] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = at + e < n;
+                pv[h][e] = in ? val[at + e] : 0.0f;
+                g[h][e] = in ? to_f32(grad[at + e]) : 0.0f;
+                mb[h] |= in ? (uint32_t)m[at + e] << (8 * e) : 0u;
+                vb[h] |= in ? (uint32_t)v[at + e] << (8 * e) : 0u;
+            }
+        }
+    }
+    bool ok = true;
+    float top_m = 0.0f, top_r = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float mm = __fmul_rn(from_e4m3((uint8_t)(mb[h] >> (8 * e))), ms);
+            const float r = __fmul_rn(from_e4m3((uint8_t)(vb[h] >> (8 * e))), vs);
+            float vv = __fmul_rn(r, r);
+            ok &= adamw_element(pv[h][e], g[h][e], c, mm, vv, a, decay);
+            mv[h][e] = fminf(fmaxf(mm, -MOMENT_MAX), MOMENT_MAX);
+            rv[h][e] = fminf(__fsqrt_rn(vv), ROOT_MAX);
+            top_m = fmaxf(top_m, fabsf(mv[h][e]));
+            top_r = fmaxf(top_r, rv[h][e]);
+        }
+    top_m = warp_max(top_m);
+    top_r = warp_max(top_r);
+    const float km = top_m >= SCALE_MIN ? __fdiv_rn(E4M3_MAX, top_m) : 0.0f;
+    const float kr = top_r >= SCALE_MIN ? __fdiv_rn(E4M3_MAX, top_r) : 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t at = h * 128 + lane * 4;
+        uint32_t mo = 0, vo = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float y = __fmul_rn(rv[h][e], kr);
+            mo |= (uint32_t)to_e4m3(__fmul_rn(mv[h][e], km)) << (8 * e);
+            // A root above 0 stays above 0: a later step divides by it.
+            vo |= (uint32_t)to_e4m3(rv[h][e] > 0.0f && kr > 0.0f ? fmaxf(y, E4M3_TINY) : 0.0f) << (8 * e);
+        }
+        if (vec) {
+            __stcs(reinterpret_cast<float4 *>(val + at), make_float4(pv[h][0], pv[h][1], pv[h][2], pv[h][3]));
+            __stcs(reinterpret_cast<uint32_t *>(m + at), mo);
+            __stcs(reinterpret_cast<uint32_t *>(v + at), vo);
+            if (t.copy) store_copy4(t.copy, t.copy_dtype, first + at, pv[h]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at + e < n) {
+                    val[at + e] = pv[h][e];
+                    m[at + e] = (uint8_t)(mo >> (8 * e));
+                    v[at + e] = (uint8_t)(vo >> (8 * e));
+                    if (t.copy) store_copy(t.copy, t.copy_dtype, first + at + e, pv[h][e]);
+                }
+        }
+    }
+    if (lane == 0) {
+        // (The scale of what was stored: 1 / k up to rounding, 0 for zeros.)
+        t.m_scale[first / NK_ADAMW_BLOCK] = km > 0.0f ? __fdiv_rn(top_m, E4M3_MAX) : 0.0f;
+        t.v_scale[first / NK_ADAMW_BLOCK] = kr > 0.0f ? __fdiv_rn(top_r, E4M3_MAX) : 0.0f;
+    }
+    return ok;
+}
+
+template <class G>
+__device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const AdamwChunk &ch, const AdamwParams &a,
+                                            float c, bool decay) {
+    const bool vec = aligned(t.val, 16) && aligned(t.m, 4) && aligned(t.v, 4) && aligned(t.grad, 4 * sizeof(G)) &&
+                     (!t.copy || aligned(t.copy, 8));
+    bool ok = true;
+    for (uint32_t b = (threadIdx.x >> 5) * NK_ADAMW_BLOCK; b < ch.n; b += (blockDim.x >> 5) * NK_ADAMW_BLOCK)
+        ok &= block_step8<G>(t, ch.first + b, min(ch.n - b, (uint32_t)NK_ADAMW_BLOCK), a, c, decay, vec);
+    return ok;
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(256) adamw_many_k(AdamwMany p, uint32_t from, uint32_t to, AdamwParams a,
+                                                    float grad_scale, bool with_clip, uint32_t *bad) {
+    float c = grad_scale;
+    if (with_clip) {
+        if (p.clip[1] == 0.0f) return;
+        c = p.clip[0];
+    }
+    bool ok = true;
+    for (uint32_t i = from + blockIdx.x; i < to; i += gridDim.x) {
+        const AdamwChunk ch = p.chunks[i];
+        const nk_adamw_tensor t = p.tensors[ch.tensor];
+        const bool decay = t.decay && a.wd != 0.0f;
+        if constexpr (BITS == 32) {
+            ok &= t.grad_dtype == NK_F32   ? chunk_step32<float>(t, ch, a, c, decay)
+                  : t.grad_dtype == NK_F16 ? chunk_step32<__half>(t, ch, a, c, decay)
+                                           : chunk_step32<__nv_bfloat16>(t, ch, a, c, decay);
+        } else {
+            ok &= t.grad_dtype == NK_F32   ? chunk_step8<float>(t, ch, a, c, decay)
+                  : t.grad_dtype == NK_F16 ? chunk_step8<__half>(t, ch, a, c, decay)
+                                           : chunk_step8<__nv_bfloat16>(t, ch, a, c, decay);
+        }
+    }
+    if (!ok && bad) *bad = 1u;
+}
+
+}  // namespace
+
+uint32_t adamw_chunk_elements(uint64_t total, int sms) {
+    // Enough chunks for eight blocks on every SM, of 1024 to 16384 elements.
+    const uint64_t want = total / ((uint64_t)sms * 8) / 1024 * 1024;
+    return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(want, 1024), 16384);
+}
+
+cudaError_t adamw_many_norm(const AdamwMany &p, float grad_scale, float max_norm, float *norm, uint32_t *bad, int sms,
+                            cudaStream_t st) {
+    const unsigned blocks = std::max(1u, std::min<unsigned>(p.n_chunks, (unsigned)sms * 8));
+    adamw_norm_k<<<blocks, 256, 0, st>>>(p, grad_scale, max_norm, norm, bad);
+    return cudaGetLastError();
+}
+
+cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, float grad_scale, bool with_clip, uint32_t *bad,
+                            int sms, cudaStream_t st) {
+    const uint32_t n32 = p.n_chunks32, n8 = p.n_chunks - n32;
+    if (n32) adamw_many_k<32><<<std::min<unsigned>(n32, (unsigned)sms * 8), 256, 0, st>>>(p, 0, n32, a, grad_scale, with_clip, bad);
+    if (n8) adamw_many_k<8><<<std::min<unsigned>(n8, (unsigned)sms * 8), 256, 0, st>>>(p, n32, p.n_chunks, a, grad_scale, with_clip, bad);
+    return cudaGetLastError();
+}
+
+}  // namespace nk

@@ -3,7 +3,8 @@
 Each ``.cu`` file is compiled with nvcc to an object under
 ``noetic_b200/_build`` (in parallel, skipped when up to date) and the objects
 are linked into one shared library that exports the C ABI declared in
-``include/noetic_gpu.h`` and ``include/noetic/head.h``.  nvcc cross-compiles
+``include/noetic_gpu.h``, ``include/noetic/head.h`` and
+``include/noetic/train.h``.  nvcc cross-compiles
 for sm_100a without a GPU.
 """
 
@@ -34,6 +35,7 @@ def _headers():
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh", ".inc"))]
     hs.append(os.path.join(ROOT, "include", "noetic_gpu.h"))
     hs.append(os.path.join(ROOT, "include", "noetic", "head.h"))
+    hs.append(os.path.join(ROOT, "include", "noetic", "train.h"))
     return hs
 
 

@@ -1,0 +1,332 @@
+"""AdamW over many tensors (include/noetic/train.h) on the GPU: bit for bit
+against nk_adamw_step and a restatement in torch, whose f32 operations are rounded
+one by one as the kernel's are."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+CODE = {"f32": 0, "f16": 1, "bf16": 2}
+SIZES = [1, 2, 255, 256, 257, 1000, 4096, 70001, 3, 513, 1 << 18]
+HYPER = dict(lr=3e-3, t=7, b1=0.9, b2=0.95, eps=1e-8, wd=0.1)
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    return torch
+
+
+def _dt(torch, name):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+class Tensors:
+    """Parameter tensors at places `shift` elements into their arrays."""
+
+    def __init__(self, torch, sizes, grad="f32", bits=32, copy=None, shift=0, seed=0):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.torch, self.bits, self.grad, self.copy = torch, bits, grad, copy
+        self.t = []
+
+        def array(n, dtype, v=None):
+            whole = torch.zeros(n + shift + 8, device="cuda", dtype=dtype)
+            a = whole[shift:shift + n]
+            if v is not None:
+                a.copy_(v)
+            return a
+
+        for i, n in enumerate(sizes):
+            nb = -(-n // 256)
+            size = torch.exp(2 * torch.randn(nb, generator=g, device="cuda") - 6).repeat_interleave(256)[:n]
+            gr = torch.randn(n, generator=g, device="cuda") * size
+            t = {"val": array(n, torch.float32, torch.randn(n, generator=g, device="cuda")),
+                 "grad": array(n, _dt(torch, grad), gr), "decay": i % 2, "n": n}
+            if bits == 32:
+                t["m"] = array(n, torch.float32, gr * 0.3)
+                t["v"] = array(n, torch.float32, gr.square() * torch.rand(n, generator=g, device="cuda"))
+            else:
+                t["m"] = array(n, torch.uint8, torch.randint(0, 127, (n,), generator=g, device="cuda") +
+                               128 * torch.randint(0, 2, (n,), generator=g, device="cuda"))
+                t["v"] = array(n, torch.uint8, torch.randint(0, 127, (n,), generator=g, device="cuda"))
+                t["m_scale"] = array(nb, torch.float32, torch.rand(nb, generator=g, device="cuda") * 1e-4)
+                t["v_scale"] = array(nb, torch.float32, torch.rand(nb, generator=g, device="cuda") * 1e-4)
+            if copy:
+                t["copy"] = array(n, _dt(torch, copy))
+            self.t.append(t)
+
+    def plan(self, nb):
+        def at(t, k):
+            return t[k].data_ptr() if k in t and t["n"] else None
+
+        return nb.train.AdamwMany([nb.train.AdamwTensor(
+            val=at(t, "val"), grad=at(t, "grad"), m=at(t, "m"), v=at(t, "v"), n=t["n"], m_scale=at(t, "m_scale"),
+            v_scale=at(t, "v_scale"), copy=at(t, "copy"), grad_dtype=CODE[self.grad],
+            copy_dtype=CODE[self.copy or "bf16"], state_bits=self.bits, decay=t["decay"]) for t in self.t])
+
+    def clone(self):
+        return [{k: v.clone() if hasattr(v, "clone") else v for k, v in t.items()} for t in self.t]
+
+
+def _bias(b, t):
+    """1 / (1 - b^t) with the C library's powf, as the host computes it."""
+    powf = C.CDLL("libm.so.6").powf
+    powf.restype, powf.argtypes = C.c_float, [C.c_float, C.c_float]
+    one = np.float32(1.0)
+    return float(one / (one - np.float32(powf(b, t))))
+
+
+def _want(torch, t, c, lr, t_step, b1, b2, eps, wd, bits):
+    """The step of one tensor, operation by operation in f32."""
+    f = lambda x: float(np.float32(x))  # noqa: E731
+    g = t["grad"].float()
+    n = t["n"]
+    blocks = -(-n // 256)
+    fine = torch.isfinite(g) & torch.isfinite(t["val"])
+    g = g * c
+    if bits == 8:
+        def per(s):
+            return s.repeat_interleave(256)[:n]
+
+        m = t["m"].view(torch.float8_e4m3fn).float() * per(t["m_scale"])
+        v = (t["v"].view(torch.float8_e4m3fn).float() * per(t["v_scale"])).square()
+    else:
+        m, v = t["m"], t["v"]
+    m1 = m * f(b1) + g * f(np.float32(1) - np.float32(b1))
+    v1 = v * f(b2) + (g * f(np.float32(1) - np.float32(b2))) * g
+    upd = (m1 * _bias(b1, t_step)) / (torch.sqrt(v1 * _bias(b2, t_step)) + f(eps))
+    if t["decay"] and wd:
+        upd = upd + t["val"] * f(wd)
+    val = torch.where(fine, t["val"] - upd * f(lr), t["val"])
+    m1, v1 = torch.where(fine, m1, m), torch.where(fine, v1, v)
+    out = {"val": val}
+    if bits == 32:
+        out.update(m=m1, v=v1)
+        return out
+    for k, x in (("m", m1), ("v", torch.sqrt(v1))):
+        rows = torch.zeros(blocks * 256, device="cuda")
+        rows[:n] = x
+        rows = rows.view(blocks, 256)
+        top = rows.abs().amax(1)
+        most = torch.full_like(top, 448.0)  # (A quotient of tensors is rounded once; one with a number need not be.)
+        y = rows * torch.where(top > 0, most / top, 0.0)[:, None]
+        if k == "v":
+            y = torch.where(rows > 0, y.clamp(min=2.0**-9), y)
+        out[k] = y.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8).reshape(-1)[:n]
+        out[k + "_scale"] = top / most
+    return out
+
+
+def _same(torch, got, want, copy=None):
+    for k, v in want.items():
+        assert torch.equal(got[k], v), (k, got["n"], (got[k].float() - v.float()).abs().max())
+    if copy:
+        assert torch.equal(got["copy"], want["val"].to(_dt(torch, copy)))
+
+
+@pytest.mark.parametrize("grad", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits,copy,shift", [(32, None, 0), (32, "f16", 0), (32, "bf16", 1), (8, None, 0), (8, "bf16", 0),
+                                             (8, "f16", 3)])
+def test_step(nb, torch, grad, bits, copy, shift):
+    s = Tensors(torch, SIZES, grad, bits, copy, shift)
+    before = s.clone()
+    plan = s.plan(nb)
+    plan.step(**HYPER)
+    torch.cuda.synchronize()
+    for t, b in zip(s.t, before):
+        _same(torch, t, _want(torch, b, 1.0, HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, bits), copy)
+
+
+def test_32_bits_are_nk_adamw_step(nb, torch):
+    s = Tensors(torch, SIZES, seed=3)
+    other = s.clone()
+    plan = s.plan(nb)
+    for step in range(1, 5):
+        plan.step(**{**HYPER, "t": step})
+        for t in other:
+            cfg = nb.NkAdamwCfg(HYPER["lr"], 0.9, 0.95, 1e-8, 0.1, step, t["decay"])
+            nb._check(nb.lib().nk_adamw_step_device(t["val"].data_ptr(), t["grad"].data_ptr(), t["m"].data_ptr(),
+                                                    t["v"].data_ptr(), t["n"], C.byref(cfg), None))
+    torch.cuda.synchronize()
+    for t, o in zip(s.t, other):
+        assert all(torch.equal(t[k], o[k]) for k in ("val", "m", "v"))
+
+
+@pytest.mark.parametrize("bits,grad", [(32, "f32"), (8, "bf16"), (8, "f16")])
+@pytest.mark.parametrize("scale", [1.0, 1 / 1024])
+def test_norm_and_clip(nb, torch, bits, grad, scale):
+    s = Tensors(torch, SIZES, grad, bits, seed=4)
+    before = s.clone()
+    plan = s.plan(nb)
+    norm = torch.zeros(1, device="cuda")
+    bad = torch.zeros(1, device="cuda", dtype=torch.int32)
+    exact = sum(float(t["grad"].double().square().sum()) for t in before) ** 0.5 * scale
+    for limit in (0.0, 2 * exact, exact / 3):
+        plan.step(**HYPER, grad_scale=scale, max_norm=limit, norm=norm.data_ptr(), bad=bad.data_ptr())
+        torch.cuda.synchronize()
+        # Squares, and sums of four of them, in f32: 3 roundings of a square, 2 of the result.
+        assert abs(float(norm) - exact) <= 4 * 2.0**-24 * exact and int(bad) == 0
+        c = np.float32(scale)
+        if limit and float(norm) > np.float32(limit):
+            c = np.float32(scale) * (np.float32(limit) / np.float32(norm.cpu().numpy()[0]))
+        for t, b in zip(s.t, before):
+            _same(torch, t, _want(torch, b, float(c), HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, bits))
+        before = s.clone()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_elements_that_are_not_finite_stay(nb, torch, bits):
+    s = Tensors(torch, [1000, 4096, 5], bits=bits, seed=5)
+    s.t[0]["grad"][3] = float("nan")
+    s.t[1]["grad"][4095] = float("inf")
+    s.t[2]["val"][0] = float("inf")
+    before = s.clone()
+    plan = s.plan(nb)
+    bad = torch.zeros(1, device="cuda", dtype=torch.int32)
+    plan.step(**HYPER, bad=bad.data_ptr())
+    torch.cuda.synchronize()
+    assert int(bad) == 1
+    for t, b in zip(s.t, before):
+        _same(torch, t, _want(torch, b, 1.0, HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, bits))
+    # With a clip nothing changes.
+    now = s.clone()
+    bad.zero_()
+    norm = torch.zeros(1, device="cuda")
+    plan.step(**HYPER, max_norm=1.0, norm=norm.data_ptr(), bad=bad.data_ptr())
+    torch.cuda.synchronize()
+    assert int(bad) == 1 and not torch.isfinite(norm).any()
+    for t, b in zip(s.t, now):
+        assert all(torch.equal(t[k].view(torch.uint8), b[k].view(torch.uint8)) for k in t if k in ("val", "m", "v"))
+
+
+def test_blocks_of_zeros_and_of_extremes(nb, torch):
+    """Zero gradients and moments stay zero; v stays above zero beside a large one; the largest values do not overflow."""
+    s = Tensors(torch, [1024], bits=8, seed=6)
+    t = s.t[0]
+    for k in ("m", "v", "m_scale", "v_scale"):
+        t[k].zero_()
+    t["grad"][:256] = 0.0
+    t["grad"][256:512] = 1e-9
+    t["grad"][300] = 1e3
+    t["grad"][512:768] = 1e-38
+    t["grad"][768:] = 3e38
+    before = s.clone()[0]
+    plan = s.plan(nb)
+    plan.step(**{**HYPER, "wd": 0.0})
+    torch.cuda.synchronize()
+    assert torch.equal(t["val"][:256], before["val"][:256]) and (t["m"][:256] == 0).all() and (t["v"][:256] == 0).all()
+    assert (t["v"][256:512] > 0).all() and float(t["v_scale"][0]) == 0.0
+    assert all(torch.isfinite(t[k]).all() for k in ("val", "m_scale", "v_scale"))
+    assert (t["m"] != 127).all() and (t["v"] != 127).all()
+    for _ in range(20):
+        plan.step(**{**HYPER, "wd": 0.0})
+    torch.cuda.synchronize()
+    # A step moves a value by lr |m^| / (sqrt(v^) + eps), and in this framework's moments m^2 <= 11 v
+    # (sum of the weights' squares ratio, (1 - b1)^2 / ((1 - b2)(1 - b1^2 / b2)) < 2) with rounding
+    # of 1/16 in each: far below 4 steps each.
+    assert (t["val"] - before["val"]).abs().max() <= 21 * 4 * HYPER["lr"]
+
+
+def test_8_bits_follow_32_bits(nb, torch):
+    """Thirty steps on noisy gradients: the values part by a small share of the way."""
+    a, b = Tensors(torch, [50000], seed=7), Tensors(torch, [50000], bits=8, seed=7)
+    for s in (a, b):
+        for k in ("m", "v", "m_scale", "v_scale"):
+            if k in s.t[0]:
+                s.t[0][k].zero_()
+    b.t[0]["val"].copy_(a.t[0]["val"])
+    start = a.t[0]["val"].clone()
+    pa, pb = a.plan(nb), b.plan(nb)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    base = a.t[0]["grad"].clone()
+    for step in range(1, 31):
+        now = base * (1 + 0.5 * torch.randn(50000, generator=g, device="cuda"))
+        for s in (a, b):
+            s.t[0]["grad"].copy_(now)
+        pa.step(**{**HYPER, "t": step, "wd": 0.0})
+        pb.step(**{**HYPER, "t": step, "wd": 0.0})
+    torch.cuda.synchronize()
+    way = (a.t[0]["val"] - start).norm()
+    # m is off by 2^-4 of itself at most after each step and forgets a tenth of that a step, the
+    # root of v by 2^-4 and half of a twentieth: independent errors of 2^-4 / sqrt(3) add to
+    # at most 0.036 sqrt(1 / (1 - 0.81)) = 0.08 and 0.036 sqrt(1 / (1 - 0.95)) = 0.16 of the update.
+    assert (a.t[0]["val"] - b.t[0]["val"]).norm() <= 0.25 * way
+
+
+def test_empty_tensors_and_empty_models(nb, torch):
+    s = Tensors(torch, [0, 300, 0])
+    before = s.clone()
+    s.plan(nb).step(**HYPER)
+    _same(torch, s.t[1], _want(torch, before[1], 1.0, HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, 32))
+    norm = torch.full((1,), 9.0, device="cuda")
+    nb.train.AdamwMany([]).step(**HYPER, max_norm=1.0, norm=norm.data_ptr())
+    torch.cuda.synchronize()
+    assert float(norm) == 0.0
+
+
+def test_both_kinds_of_moments_in_one_model(nb, torch):
+    a, b = Tensors(torch, [700, 5000], "bf16", 32, seed=8), Tensors(torch, [300, 9001], "bf16", 8, seed=9)
+    before = a.clone(), b.clone()
+    ta, tb = a.plan, b.plan
+    made = []
+
+    class Take:
+        train = type("t", (), {"AdamwTensor": nb.train.AdamwTensor, "AdamwMany": staticmethod(made.extend)})
+
+    ta(Take), tb(Take)
+    plan = nb.train.AdamwMany([made[2], made[0], made[3], made[1]])
+    plan.step(**HYPER)
+    torch.cuda.synchronize()
+    for s, was, bits in ((a, before[0], 32), (b, before[1], 8)):
+        for t, w in zip(s.t, was):
+            _same(torch, t, _want(torch, w, 1.0, HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, bits))
+
+
+def test_streams_and_graphs(nb, torch):
+    """Two models on two streams, and a captured step replayed: each replay is one more step."""
+    sets = [Tensors(torch, SIZES, "bf16", 8, "bf16", seed=10), Tensors(torch, SIZES, "f32", 32, seed=11)]
+    ref = [Tensors(torch, SIZES, "bf16", 8, "bf16", seed=10), Tensors(torch, SIZES, "f32", 32, seed=11)]
+    for r in ref:
+        p = r.plan(nb)
+        for _ in range(4):
+            p.step(**HYPER, max_norm=0.5)
+    torch.cuda.synchronize()
+    plans, streams, graphs = [s.plan(nb) for s in sets], [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for p, st in zip(plans, streams):
+        p.step(**HYPER, max_norm=0.5, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for p, st in zip(plans, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            p.step(**HYPER, max_norm=0.5, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for _ in range(3):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for s, r in zip(sets, ref):
+        for a, b in zip(s.t, r.t):
+            assert all(torch.equal(a[k], b[k]) for k in a if hasattr(a[k], "clone"))
+
+
+def test_host_form(nb, torch):
+    rng = np.random.default_rng(0)
+    val, grad = rng.standard_normal(600).astype(np.float32), rng.standard_normal(600).astype(np.float32)
+    zero = np.zeros(600, np.float32)
+    out, norm = nb.adamw_step_many([dict(val=val, grad=grad, m=zero, v=zero, copy="f16"),
+                                    dict(val=val, grad=grad, m=np.zeros(600), v=np.zeros(600), m_scale=np.zeros(3),
+                                         v_scale=np.zeros(3), decay=False)], lr=0.1, t=1, wd=0.01)
+    v, m, vv = nb.adamw_step(val, grad, zero, zero, 0.1, 1, True, wd=0.01)
+    assert np.array_equal(out[0]["val"], v) and np.array_equal(out[0]["m"], m) and np.array_equal(out[0]["v"], vv)
+    assert np.array_equal(out[0]["copy"], v.astype(np.float16))
+    assert np.array_equal(out[1]["val"], nb.adamw_step(val, grad, zero, zero, 0.1, 1, False)[0])
+    assert out[1]["m"].dtype == np.uint8 and out[1]["m_scale"].shape == (3,) and (out[1]["m_scale"] > 0).all()
+    assert abs(norm - np.sqrt(2 * (grad.astype(np.float64) ** 2).sum())) < 1e-5
+    grad[7] = np.nan
+    with pytest.raises(nb.NoeticError):
+        nb.adamw_step_many([dict(val=val, grad=grad, m=zero, v=zero)], lr=0.1, t=1)

@@ -1,0 +1,419 @@
+"""Cross entropy from hidden rows and its gradients (include/noetic/train.h) on
+the GPU against their definitions in 64 bits.
+
+Tolerances count roundings, U = 2^-24 being half a step of f32.  With A = sum_k
+|x_k w_k| of a logit:
+ - products of 16-bit elements are exact in f32.  A sum of d of them passes each
+   through at most d additions that round (U each), or d / 16 + 5 of the tensor
+   cores' that cut (2 U each): off by (d + 64) U A at most.
+ - f32 elements are taken with 22 bits (2^-22 of each factor, and 2^-40 of the
+   largest element of its matrix below that): 2^-21 A + 2^-39 d max|x| max|w|.
+ - loss = (m - z_t) + log s: two logits, the sum's own error (a mean of the
+   logits' errors, 2^-22 of the exponential, N / 32 + 64 additions) and the
+   rounding of differences of the size of the spread: 2 max dz + (N / 32 + 80 +
+   4 Y) U.
+ - p comes with dz, the 2 U (|m| + log s) of the statistics and 2^-22; G with half a
+   step of its type more (f32: 2^-22), and 2^-38 of the largest weight; the
+   products add (K + 64) U of sum |G| |w| and the output's rounding.
+"""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+INF, NAN = float("inf"), float("nan")
+CODE = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    return torch
+
+
+def _dt(torch, name):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def _p(t):
+    return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _st(torch):
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _matrix(torch, rows, width, dtype, pad=0, shift=0, scale=1.0, seed=0):
+    """A [rows, width] view whose rows start `shift` elements into an array of
+    row stride width + pad (NaN around the rows)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    whole = torch.full((shift + rows * (width + pad) + 8,), NAN, device="cuda", dtype=_dt(torch, dtype))
+    v = whole[shift:shift + rows * (width + pad)].view(rows, width + pad)[:, :width]
+    v.copy_(torch.randn(rows, width, generator=g, device="cuda") * scale)
+    return v
+
+
+class Case:
+    """Inputs, and what the definitions give for them in 64 bits."""
+
+    def __init__(self, torch, rows, width, vocab, dtype, ignored=0.0, pad=0, shift=0, seed=0, spread=2.0, weights=True):
+        g = torch.Generator(device="cuda").manual_seed(seed + 7)
+        self.torch, self.dtype, self.rows, self.width, self.vocab = torch, dtype, rows, width, vocab
+        self.x = _matrix(torch, rows, width, dtype, pad, shift, 1.0, seed)
+        self.w = _matrix(torch, vocab, width, dtype, pad, shift, spread / width**0.5, seed + 1)
+        self.targets = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+        dead = torch.rand(rows, generator=g, device="cuda") < ignored
+        self.targets[dead] = -1
+        self.x[dead] = NAN  # (What stands in a row that does not count can be anything.)
+        self.weight = torch.rand(rows, generator=g, device="cuda") + 0.5 if weights else None
+        self.live = ~dead
+
+    def workspace(self, nb, backward):
+        n = nb.train.linear_ce_workspace(CODE[self.dtype], self.rows, self.width, self.vocab, self.w.data_ptr(),
+                                         self.w.stride(0), backward)
+        return self.torch.full((n + 64,), 255, device="cuda", dtype=self.torch.uint8)  # (NaN in every type)
+
+    def forward(self, nb, room=None, targets=None):
+        torch = self.torch
+        room = self.workspace(nb, False) if room is None else room
+        loss = torch.full((self.rows,), 5.0, device="cuda")
+        stats = torch.full((self.rows, 2), 5.0, device="cuda")
+        nb._check(nb.lib().nk_linear_ce_device(
+            _p(self.x), CODE[self.dtype], self.rows, self.width, self.x.stride(0), _p(self.w), self.vocab,
+            self.w.stride(0), _p(self.targets if targets is None else targets), _p(loss), _p(stats), _p(room),
+            room.numel() - 64, _st(torch)))
+        return loss, stats
+
+    def backward(self, nb, stats, scale=1.0, dw_dtype=None, dw=None, dx=None, want_dx=True, want_dw=True, room=None):
+        torch = self.torch
+        room = self.workspace(nb, True) if room is None else room
+        add = dw is not None
+        dw_dtype = dw_dtype or self.dtype
+        if want_dx and dx is None:
+            dx = torch.full((self.rows, self.width), 5.0, device="cuda", dtype=_dt(torch, self.dtype))
+        if want_dw and dw is None:
+            dw = torch.full((self.vocab, self.width), 5.0, device="cuda", dtype=_dt(torch, dw_dtype))
+        nb._check(nb.lib().nk_linear_ce_backward_device(
+            _p(self.x), CODE[self.dtype], self.rows, self.width, self.x.stride(0), _p(self.w), self.vocab,
+            self.w.stride(0), _p(self.targets), _p(stats), _p(self.weight), scale, _p(dx),
+            0 if dx is None else dx.stride(0), _p(dw), CODE[dw_dtype], 0 if dw is None else dw.stride(0), int(add),
+            _p(room), room.numel() - 64, _st(torch)))
+        return dx, dw
+
+    # ---- 64 bits
+    def x64(self):
+        return self.torch.where(self.live[:, None], self.x.double(), 0.0)
+
+    def logits(self):
+        return self.x64() @ self.w.double().T
+
+    def dz(self):
+        """The most that a logit can be off, for each logit."""
+        x, w = self.x64().abs(), self.w.double().abs()
+        tol = (self.width + 64) * U * (x @ w.T)
+        if self.dtype == "f32":
+            tol = tol * (1 + 8 / (self.width + 64)) + 2.0**-39 * self.width * float(x.max()) * float(w.max())
+        return tol
+
+    def check_forward(self, loss, stats):
+        torch = self.torch
+        z, dz = self.logits(), self.dz().max(-1).values
+        lse, m = torch.logsumexp(z, -1), z.max(-1).values
+        at = z.gather(1, self.targets.long().clamp(min=0)[:, None])[:, 0]
+        y = (m - z.min(-1).values)
+        own = (self.vocab / 32 + 80 + 4 * y) * U
+        zero = torch.zeros((), device="cuda", dtype=torch.float64)
+        err = (loss.double() - torch.where(self.live, lse - at, zero)).abs()
+        assert (err <= torch.where(self.live, 2 * dz + own, zero)).all(), float(err.max())
+        err = (stats.double() - torch.stack([m, lse - m], 1) * self.live[:, None]).abs()
+        tol = torch.stack([dz + U * m.abs(), 2 * dz + own + U * (lse - m).abs()], 1) * self.live[:, None]
+        assert (err <= tol).all(), float(err.max())
+
+    def check_backward(self, stats, scale, dx=None, dw=None, base=None):
+        torch = self.torch
+        eps = {"f32": 2.0**-22, "f16": 2.0**-11, "bf16": 2.0**-8}[self.dtype]
+        h = self.weight.double() if self.weight is not None else torch.ones(self.rows, device="cuda", dtype=torch.float64)
+        h = torch.where(self.live, h * scale, 0.0)[:, None]
+        x, w, st = self.x64(), self.w.double(), stats.double()
+        p = torch.exp(self.logits() - st.sum(1, keepdim=True))
+        hot = torch.zeros_like(p).scatter_(1, self.targets.long().clamp(min=0)[:, None], 1.0)
+        G = h * (p - hot)
+        dG = h.abs() * p * torch.expm1(self.dz() + 2 * U * (st.abs().sum(1, keepdim=True) + 4)) + 4 * U * h.abs() * hot
+        dG = dG + eps * (G.abs() + dG) + 2.0**-38 * h.abs().max()
+        dG = dG * (h != 0)
+        for out, a, b, db in ((dx, G, w, dG), (dw, G.T, x, dG.T)):
+            if out is None:
+                continue
+            ref = a @ b
+            tol = db @ b.abs() + (b.shape[0] + 64) * U * (a.abs() @ b.abs()) * (1 + (8 / (b.shape[0] + 64) if self.dtype == "f32" else 0))
+            if self.dtype == "f32":
+                # The product's own factors: 2^-22 of each element, 2^-40 of the largest.
+                tol = tol + a.abs().sum(1, keepdim=True) * float(b.abs().max()) * 2.0**-39
+            if out is dw and base is not None:
+                ref = ref + base.double()
+            f = torch.finfo(out.dtype)
+            tol = tol + (f.eps / 2) * (ref.abs() + tol) + f.smallest_normal * f.eps / 2
+            err = (out.double() - ref).abs()
+            assert (err <= tol).all(), (float(err.max()), float((err / tol.clamp(min=1e-300)).max()))
+
+
+SIZES = [(1, 1, 1), (1, 64, 1000), (2, 3, 5), (7, 17, 300), (64, 192, 1024), (129, 100, 1003), (255, 72, 515),
+         (257, 136, 769), (300, 767, 2003), (513, 64, 33), (1, 1024, 32768), (5, 4096, 259), (17, 65, 8192)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,width,vocab", SIZES)
+def test_forward(nb, torch, rows, width, vocab, dtype):
+    c = Case(torch, rows, width, vocab, dtype)
+    c.check_forward(*c.forward(nb))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,width,vocab", SIZES)
+def test_backward(nb, torch, rows, width, vocab, dtype):
+    c = Case(torch, rows, width, vocab, dtype)
+    _, stats = c.forward(nb)
+    c.check_backward(stats, 0.25, *c.backward(nb, stats, 0.25))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad,shift,ignored", [(0, 0, 0.4), (1, 0, 0.0), (8, 0, 0.2), (3, 1, 0.2), (16, 5, 0.9)])
+def test_strides_places_and_padded_batches(nb, torch, dtype, pad, shift, ignored):
+    c = Case(torch, 333, 200, 1500, dtype, ignored=ignored, pad=pad, shift=shift, seed=3)
+    loss, stats = c.forward(nb)
+    c.check_forward(loss, stats)
+    # Outputs with strides of their own; what lies between their rows stays.
+    dx = torch.full((333, 207), 7.0, device="cuda", dtype=_dt(torch, dtype))
+    dw = torch.full((1500, 203), 7.0, device="cuda", dtype=_dt(torch, dtype))
+    room = c.workspace(nb, True)
+    nb._check(nb.lib().nk_linear_ce_backward_device(
+        _p(c.x), CODE[dtype], 333, 200, c.x.stride(0), _p(c.w), 1500, c.w.stride(0), _p(c.targets), _p(stats),
+        _p(c.weight), 1e-3, _p(dx), 207, _p(dw), CODE[dtype], 203, 0, _p(room), room.numel() - 64, _st(torch)))
+    c.check_backward(stats, 1e-3, dx[:, :200], dw[:, :200])
+    assert (dx[:, 200:] == 7).all() and (dw[:, 200:] == 7).all()
+    assert (dx[:, :200][~c.live] == 0).all()
+    assert (room[-64:] == 255).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_no_row_counts(nb, torch, dtype):
+    c = Case(torch, 70, 64, 300, dtype)
+    c.targets[:] = -1
+    c.live[:] = False
+    c.x[:] = NAN
+    loss, stats = c.forward(nb)
+    assert (loss == 0).all() and (stats == 0).all()
+    dx, dw = c.backward(nb, stats)
+    assert (dx == 0).all() and (dw == 0).all()
+    base = torch.ones(300, 64, device="cuda", dtype=_dt(torch, dtype))
+    _, dw = c.backward(nb, stats, dw=base.clone())
+    assert torch.equal(dw, base)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_ids_beyond_the_vocabulary_are_no_token_and_weights_of_zero_add_nothing(nb, torch, dtype):
+    c = Case(torch, 90, 96, 700, dtype, seed=5)
+    c.targets[::3] = 700
+    c.targets[1::7] = 2**31 - 1
+    c.live = (c.targets >= 0) & (c.targets < 700)
+    dead = ~c.live
+    loss, stats = c.forward(nb)
+    c.targets[dead] = -1
+    c.x[dead] = NAN
+    c.check_forward(loss, stats)
+    c.weight[::5] = 0.0
+    off = c.live & (c.weight == 0)
+    dx, dw = c.backward(nb, stats)
+    c.check_backward(stats, 1.0, dx, dw)
+    # Their rows are not read.
+    c.x[off] = INF
+    again = c.backward(nb, stats)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1]) and (dx[off] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_each_output_alone_f32_sums_and_accumulation(nb, torch, dtype):
+    c = Case(torch, 270, 130, 900, dtype, ignored=0.1, seed=6)
+    _, stats = c.forward(nb)
+    dx, dw = c.backward(nb, stats, 0.5)
+    alone_x, none = c.backward(nb, stats, 0.5, want_dw=False)
+    assert none is None and torch.equal(alone_x, dx)
+    none, alone_w = c.backward(nb, stats, 0.5, want_dx=False)
+    assert none is None and torch.equal(alone_w, dw)
+    _, wide = c.backward(nb, stats, 0.5, dw_dtype="f32")
+    c.check_backward(stats, 0.5, None, wide)
+    assert torch.equal(wide.to(dw.dtype), dw)
+    base = torch.randn(900, 130, device="cuda")
+    _, added = c.backward(nb, stats, 0.5, dw_dtype="f32", dw=base.clone())
+    c.check_backward(stats, 0.5, None, added, base)
+    low = base.to(_dt(torch, dtype))
+    _, added = c.backward(nb, stats, 0.5, dw=low.clone())
+    c.check_backward(stats, 0.5, None, added, low)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_several_pieces_of_the_vocabulary(nb, torch, dtype):
+    c = Case(torch, 5000, 48, 60001, dtype, ignored=0.05, seed=8)
+    loss, stats = c.forward(nb)
+    c.check_forward(loss, stats)
+    torch.cuda.empty_cache()
+    c.check_backward(stats, 1 / 5000, *c.backward(nb, stats, 1 / 5000))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_many_rows_of_a_tiny_vocabulary(nb, torch, dtype):
+    c = Case(torch, 70001, 24, 37, dtype, ignored=0.3, seed=9)
+    loss, stats = c.forward(nb)
+    c.check_forward(loss, stats)
+    c.check_backward(stats, 1 / 70001, *c.backward(nb, stats, 1 / 70001))
+
+
+def test_sure_tokens_and_far_logits(nb, torch):
+    """Logits in the thousands: p is 0 or 1, and nothing overflows."""
+    for dtype in ("f32", "f16", "bf16"):
+        c = Case(torch, 40, 64, 500, dtype, spread=500.0, seed=10)
+        loss, stats = c.forward(nb)
+        c.check_forward(loss, stats)
+        dx, dw = c.backward(nb, stats)
+        assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+        c.check_backward(stats, 1.0, dx, dw)
+
+
+@pytest.mark.parametrize("scale", [1e-20, 1e15])
+def test_f32_and_bf16_values_far_from_one(nb, torch, scale):
+    for dtype in ("f32", "bf16"):
+        c = Case(torch, 50, 80, 300, dtype, seed=11)
+        c.x.mul_(scale)
+        c.w.div_(scale)
+        loss, stats = c.forward(nb)
+        c.check_forward(loss, stats)
+        c.check_backward(stats, 1.0, *c.backward(nb, stats))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_broken_rows_leave_the_others_alone(nb, torch, dtype):
+    c = Case(torch, 300, 128, 600, dtype, seed=12)
+    loss, stats = c.forward(nb)
+    c.x[17, 3] = NAN
+    c.x[211, 0] = INF
+    bad = torch.zeros(300, dtype=torch.bool, device="cuda")
+    bad[[17, 211]] = True
+    broken, st = c.forward(nb)
+    assert torch.isnan(broken[bad]).all() and torch.isnan(st[bad]).all()
+    assert torch.equal(broken[~bad], loss[~bad]) and torch.equal(st[~bad], stats[~bad])
+    c.w[5, 9] = NAN
+    broken, _ = c.forward(nb)
+    assert torch.isnan(broken).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradients_against_differences(nb, torch, dtype):
+    """Along random directions, central differences of the 64-bit loss."""
+    c = Case(torch, 60, 40, 200, dtype, ignored=0.2, seed=13)
+    _, stats = c.forward(nb)
+    dx, dw = c.backward(nb, stats, 2.0, dw_dtype="f32")
+    x, w, t = c.x64(), c.w.double(), c.targets.long().clamp(min=0)[:, None]
+
+    def total(x, w):
+        z = x @ w.T
+        loss = torch.logsumexp(z, -1) - z.gather(1, t)[:, 0]
+        return float((2.0 * c.weight.double() * torch.where(c.live, loss, 0.0)).sum())
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    half = {"f32": 2.0**-20, "bf16": 2.0**-8}[dtype]
+    for out, v, f in ((dx, x, lambda u: total(x + u, w)), (dw, w, lambda u: total(x, w + u))):
+        u = torch.randn(v.shape, generator=g, device="cuda", dtype=torch.float64) * 1e-4
+        if out is dx:
+            u *= c.live[:, None]
+        want, got = (f(u) - f(-u)) / 2, float((out.double() * u).sum())
+        # Each element of the gradient: its own rounding and those of the 200 or 60
+        # terms of its sum; the differences: their second order, |u|^3.
+        bound = 4 * half * float((out.double() * u).abs().sum()) + half * float(u.abs().sum()) + 1e-9
+        assert abs(want - got) <= bound, (want, got, bound)
+
+
+def test_calls_on_streams_and_graphs_side_by_side(nb, torch):
+    cases = [Case(torch, 700, 256, 4000, "bf16", ignored=0.2, seed=20), Case(torch, 400, 192, 3000, "f32", seed=21)]
+    want = []
+    for c in cases:
+        loss, stats = c.forward(nb)
+        want.append((loss, stats, *c.backward(nb, stats, 0.1)))
+    torch.cuda.synchronize()
+    rooms = [(c.workspace(nb, False), c.workspace(nb, True)) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = []
+        for c, s, room in zip(cases, streams, rooms):
+            with torch.cuda.stream(s):
+                loss, stats = c.forward(nb, room[0])
+                got.append((loss, stats, *c.backward(nb, stats, 0.1, room=room[1])))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    graphs, outs = [], []
+    for c, s, room in zip(cases, streams, rooms):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            loss, stats = c.forward(nb, room[0])
+            outs.append((loss, stats, *c.backward(nb, stats, 0.1, room=room[1])))
+        graphs.append(g)
+    # Other inputs in the same arrays: the replay computes with them.
+    for c in cases:
+        c.targets.copy_(c.targets.flip(0))
+        c.x.copy_(c.x.flip(0))
+        c.live = c.live.flip(0)
+        c.weight.copy_(c.weight.flip(0))
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for c, (loss, stats, dx, dw) in zip(cases, outs):
+        c.check_forward(loss, stats)
+        c.check_backward(stats, 0.1, dx, dw)
+
+
+def test_host_form_and_python_mirror(nb):
+    rng = np.random.default_rng(0)
+    x, w = rng.standard_normal((30, 50), np.float32), rng.standard_normal((90, 50), np.float32) * 0.3
+    t = rng.integers(0, 90, 30)
+    t[4] = -1
+    out = nb.linear_cross_entropy(x, w, t)
+    z = x.astype(np.float64) @ w.T.astype(np.float64)
+    lse = np.log(np.exp(z).sum(1))
+    want = np.where(t >= 0, lse - z[np.arange(30), t], 0.0)
+    assert np.abs(out["loss"] - want).max() < 2e-5  # (114 U A of two logits, A about 20)
+    base = rng.standard_normal((90, 50)).astype(np.float32)
+    dx, dw = nb.linear_cross_entropy_backward(x, w, t, out["stats"], grad_scale=0.5)
+    dx2, dw2 = nb.linear_cross_entropy_backward(x, w, t, out["stats"], grad_scale=0.5, dw=base)
+    G = 0.5 * np.exp(z - lse[:, None])
+    G[np.arange(30), t] -= 0.5
+    G[4] = 0
+    assert np.abs(dx - G @ w).max() < 2e-5 and np.abs(dw - G.T @ x).max() < 4e-5
+    assert np.array_equal(dx, dx2) and np.abs(dw2 - base - dw).max() < 1e-6
+    with pytest.raises(nb.NoeticError):
+        nb.linear_cross_entropy(x, w, np.full(30, 90))
+    with pytest.raises(ValueError):
+        nb.linear_cross_entropy(x, w.astype(np.float16), t)
+    with pytest.raises(ValueError):
+        nb.linear_cross_entropy_backward(x, w, t, out["stats"], dw=base[:5])
+
+
+def test_the_loss_is_that_of_the_logits(nb, torch):
+    """Beside nk_token_logprobs of the same logits, and its gradient."""
+    c = Case(torch, 200, 64, 1000, "f32", seed=30, weights=False)
+    loss, stats = c.forward(nb)
+    z = c.logits().float()
+    lp = torch.empty(200, device="cuda")
+    nb._check(nb.lib().nk_token_logprobs_device(_p(z), 0, 200, 1000, 1000, _p(c.targets), 1.0, 0, _p(lp), None, None, None,
+                                                None, _st(torch)))
+    tol = 2 * c.dz().max() + (1000 / 32 + 200) * U + U * z.abs().max() * 4
+    assert (loss + lp).abs().max() <= tol
