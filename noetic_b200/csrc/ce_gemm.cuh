@@ -1,0 +1,512 @@
+// ce_gemm.cuh -- the matrix products of linear_ce.cu on the tensor cores: one
+// kernel, C = sum over pairs of parts (i, j) of A_i B_j^T in f32, whose epilogue
+// reduces a tile of logits to a maximum and a sum for each row, turns it into
+// the gradient's G, or stores it.
+//
+// Two CTAs (a cluster) make a 256 x 256 tile with tcgen05.mma.cta_group::2: each
+// holds half of A's and half of B's rows in shared memory and 128 x 256 sums in
+// TMEM, so an SM reads 64 bytes of operands a clock at full rate where a CTA
+// alone would read 96 and be bound by shared memory.  384 threads:
+//   warp 0      TMA: K-blocks of 64 into a ring of 6 stages (128-byte swizzle,
+//               zeros outside of the matrix).  An operand's rows run along K
+//               (K-major) or across it (MN-major: G and x in dw, w in dx), so
+//               nothing is transposed in memory;
+//   warp 1      the leader's issues the MMAs, 4 to a K-block;
+//   warps 4-11  epilogue, from one of two accumulators while the other fills.
+// Every wait is bounded (1 s); where one runs out, the kernel records it, every
+// role leaves its loop, copies in flight are waited for and TMEM is freed.
+#pragma once
+
+#include <cuda.h>
+
+#include "nk_head.cuh"
+
+namespace nk {
+namespace ce {
+
+constexpr int TM = 256, TN = 256, BK = 64;  // a pair's tile
+constexpr int STAGES = 6;
+constexpr int OPERAND_BYTES = 128 * BK * 2;          // a CTA's half of A or B
+constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int THREADS = 384, EPI_WARPS = 8;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint64_t WAIT_NS = 1000000000ull;
+
+// What the first kernel of a call finds out, for the others (the workspace's head).
+struct Head {
+    uint32_t err;
+    uint32_t live;     // rows that count
+    float weight_max;  // the largest |row_weight| of them
+    uint32_t x_max, w_max;  // f32: bits of the largest finite |x| and |w|
+};
+
+enum Mode { ROWS = 0, GRAD = 1, STORE = 2 };
+
+struct Gemm {
+    int M, N, K;  // at most: which of M and K is the number of rows that count (Head::live), `live_dim` says
+    int live_dim; // 0: M, 1: K, 2: neither
+    int segs;     // products of parts, small ones first
+    uint32_t sa, sb;  // bit s: which part of A and B product s takes
+    int b_row0;       // the first row of B (K-major) or the first of its K (MN-major)
+    uint32_t idesc;
+    int m_fast, group_m;  // tile order: m first within groups of group_m row blocks, else n first
+    int splits, kps;      // K-blocks (of all products) a piece of a tile takes
+    Head *head;
+    const float *x_scale, *w_scale;  // f32: exact powers of two that undo the parts' scales (nullable)
+    int n_valid;                     // columns of C that exist
+    // ROWS: part [2 tile + half][Mp] of (maximum, sum), zt [M]
+    float2 *part;
+    int64_t part_ld;
+    float *zt;
+    const uint32_t *target;  // of each row that counts
+    // GRAD: G [row][ldg], and its second part ldg * Mp elements behind
+    const float2 *stats;     // of each row that counts
+    const float *weight;     // of each row that counts, relative to the largest
+    void *g;
+    int64_t ldg, g_part;
+    int col0;                // the piece's first token
+    float g_scale;
+    // STORE
+    float *acc;              // [split][rows][ld_acc]
+    int64_t ld_acc, acc_split;
+    int add, keep;           // add what is there; keep the sum there (else it goes to out)
+    void *out;
+    int64_t out_ld, out_row0;
+    int out_dtype, out_add;
+    const uint32_t *out_row; // nullable: where a row goes
+    float out_scale;         // times Head::weight_max (and the scales)
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ uint64_t globaltimer() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t at_leader(uint32_t addr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    if (mbar_try(bar, parity)) return true;
+    const uint64_t t0 = globaltimer();
+    while (!mbar_try(bar, parity))
+        if (globaltimer() - t0 > WAIT_NS) return false;
+    return true;
+}
+
+// A box of a matrix into this CTA's shared memory, counted on the leader's barrier.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t leader_bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"((uint64_t)map), "r"(leader_bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+// Shared memory descriptors, 128-byte swizzle.  K-major: rows of 128 bytes (64
+// elements of K), groups of 8 rows 1024 bytes apart; 16 elements of K are 32
+// bytes on.  MN-major: boxes of 64 rows of K, each 128 bytes (64 elements of M or
+// N): groups of 8 K are 1024 bytes apart, the next 64 of M or N a box (8192
+// bytes); 16 of K are 2048 bytes on.
+template <bool MN>
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(MN ? 8192 >> 4 : 1) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+template <bool MN>
+constexpr uint64_t k_step() {
+    return (MN ? 2048 : 32) >> 4;
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// Arrives on the barrier at this place in both CTAs when all MMAs so far are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"((unsigned short)3)
+        : "memory");
+}
+
+// 32 columns of this warp's 32 rows; every lane takes part.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// A tile's piece: its row and column block and its K-blocks.
+struct Item {
+    int tm, tn, split, k0, k1;
+};
+
+struct Walk {
+    int mt, nt, total, kblocks, items;
+    __device__ __forceinline__ Walk(const Gemm &p, int M, int K) {
+        mt = (M + TM - 1) / TM;
+        nt = (p.N + TN - 1) / TN;
+        kblocks = (K + BK - 1) / BK;
+        total = kblocks * p.segs;
+        items = mt * nt * p.splits;
+    }
+    __device__ __forceinline__ Item at(const Gemm &p, int i) const {
+        Item it;
+        int t = i / p.splits;
+        it.split = i - t * p.splits;
+        it.k0 = min(total, it.split * p.kps);
+        it.k1 = min(total, it.k0 + p.kps);
+        if (p.m_fast) {
+            const int per = p.group_m * nt, g = t / per;
+            t -= g * per;
+            const int rows = min(p.group_m, mt - g * p.group_m);
+            it.tn = t / rows;
+            it.tm = g * p.group_m + t - it.tn * rows;
+        } else {
+            it.tm = t / nt;
+            it.tn = t - it.tm * nt;
+        }
+        return it;
+    }
+};
+
+// ---------------------------------------------------------------- epilogues
+// A warp has 32 rows (lane = row) and 128 columns of its CTA's 128 x 256 sums.
+// `row` counts rows that count (or tokens, in dw), `col` is the first column.
+
+// The maximum and the sum of exponentials of 128 logits of a row.
+template <bool SCALED>
+__device__ __forceinline__ void rows_epilogue(const Gemm &p, uint32_t tmem, int row, int live, int col, int slot) {
+    const uint32_t t = row < live ? p.target[row] : NO_TOKEN;
+    float m = -INFINITY, s = 0.0f;
+    const float xs = SCALED ? *p.x_scale : 1.0f, ws = SCALED ? *p.w_scale : 1.0f;
+#pragma unroll 1
+    for (int c = 0; c < 128; c += 32) {
+        if (col + c >= p.n_valid) break;  // warp-uniform
+        float v[32];
+        tmem_ld32(tmem + c, v);
+        if (SCALED)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = v[j] * xs * ws;
+        if (col + c + 32 > p.n_valid)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col + c + j >= p.n_valid) v[j] = -INFINITY;
+        if (t - (uint32_t)(col + c) < 32u)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (t == (uint32_t)(col + c + j)) p.zt[row] = v[j];
+        float top = v[0];
+#pragma unroll
+        for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+        const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
+        s *= ex2((m - base) * LOG2E);
+        float a[4] = {};
+#pragma unroll
+        for (int j = 0; j < 32; ++j) a[j & 3] += ex2((v[j] - base) * LOG2E);
+        s += (a[0] + a[1]) + (a[2] + a[3]);
+        m = now;
+    }
+    if (row < live) p.part[(int64_t)slot * p.part_ld + row] = make_float2(m, s);
+}
+
+// G = weight (exp(z - m - log s) - [t]) of 128 logits of a row; zeros where there
+// is no row or no token, since the products that follow read whole blocks.
+template <class T, bool SCALED>
+__device__ __forceinline__ void grad_epilogue(const Gemm &p, uint32_t tmem, int row, int live, int col) {
+    const bool in = row < live;
+    const uint32_t t = in ? p.target[row] - (uint32_t)p.col0 : NO_TOKEN;
+    const float2 st = in ? p.stats[row] : make_float2(0.0f, 0.0f);
+    const float h = in ? p.weight[row] * p.g_scale : 0.0f;
+    const float xs = SCALED ? *p.x_scale : 1.0f, ws = SCALED ? *p.w_scale : 1.0f;
+#pragma unroll 1
+    for (int c = 0; c < 128; c += 32) {
+        float v[32];
+        tmem_ld32(tmem + c, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            float z = v[j];
+            if (SCALED) z = z * xs * ws;
+            z = ex2(((z - st.x) - st.y) * LOG2E);
+            v[j] = in && col + c + j < p.n_valid ? z * h : 0.0f;
+        }
+        if (t - (uint32_t)(col + c) < 32u)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (t == (uint32_t)(col + c + j)) v[j] = fmaf(v[j], 1.0f, -h);
+        T *g = (T *)p.g + (int64_t)row * p.ldg + col + c;
+#pragma unroll
+        for (int part = 0; part < (SCALED ? 2 : 1); ++part) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+                uint4 q;
+                T *o = reinterpret_cast<T *>(&q);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    o[e] = from_f32<T>(v[j + e]);
+                    if (SCALED) v[j + e] -= to_f32(o[e]);
+                }
+                *reinterpret_cast<uint4 *>(g + part * p.g_part + j) = q;
+            }
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store_out(const Gemm &p, const float (&v)[32], int64_t at, int col) {
+    T *o = (T *)p.out + at + col;
+    constexpr int PER = 16 / sizeof(T);
+    if (col + 32 <= p.n_valid && ((uintptr_t)o & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < 32; j += PER) {
+            uint4 q;
+            T *e = reinterpret_cast<T *>(&q);
+            if (p.out_add) q = *reinterpret_cast<const uint4 *>(o + j);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) e[i] = from_f32<T>(p.out_add ? v[j + i] + to_f32(e[i]) : v[j + i]);
+            *reinterpret_cast<uint4 *>(o + j) = q;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (col + j < p.n_valid) o[j] = from_f32<T>(p.out_add ? v[j] + to_f32(o[j]) : v[j]);
+    }
+}
+
+__device__ __forceinline__ float out_factor(const Gemm &p) {
+    float f = p.out_scale * p.head->weight_max;
+    if (p.x_scale) f *= *p.x_scale;
+    if (p.w_scale) f *= *p.w_scale;
+    return f;
+}
+
+__device__ __forceinline__ void store_epilogue(const Gemm &p, uint32_t tmem, bool some, int row, int rows, int col,
+                                               int split, float factor) {
+#pragma unroll 1
+    for (int c = 0; c < 128; c += 32) {
+        if (col + c >= p.n_valid) break;  // warp-uniform
+        float v[32];
+        tmem_ld32(tmem + c, v);
+        if (!some)  // (No K at all: the accumulator holds nothing.)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+        if (row >= rows) continue;
+        float *a = p.acc ? p.acc + (int64_t)split * p.acc_split + (int64_t)row * p.ld_acc + col + c : nullptr;
+        if (p.add)
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const float4 q = *reinterpret_cast<const float4 *>(a + j);
+                v[j] += q.x, v[j + 1] += q.y, v[j + 2] += q.z, v[j + 3] += q.w;
+            }
+        if (p.keep) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(a + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= factor;
+        const int64_t at = (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld;
+        if (p.out_dtype == 0)
+            store_out<float>(p, v, at, col + c);
+        else if (p.out_dtype == 1)
+            store_out<__half>(p, v, at, col + c);
+        else
+            store_out<__nv_bfloat16>(p, v, at, col + c);
+    }
+}
+
+// ---------------------------------------------------------------- the kernel
+// T: the parts' type.  SCALED: f32 inputs, taken as two scaled f16 parts.
+template <int MODE, class T, bool SCALED, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
+       const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ Gemm p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = (uint64_t *)(smem + STAGES * STAGE_BYTES);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 4);
+    __shared__ int s_abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]);
+    const uint32_t acc_full0 = smem_u32(&bars[2 * STAGES]), acc_empty0 = smem_u32(&bars[2 * STAGES + 2]);
+
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full0 + 8 * b, 1);
+            mbar_init(acc_empty0 + 8 * b, 2 * EPI_WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&mapA0) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&mapB0) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    pair_sync();  // both CTAs' barriers exist before either signals the other
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    const int live = (int)p.head->live;
+    const int M = p.live_dim == 0 ? live : p.M, K = p.live_dim == 1 ? live : p.K;
+    const Walk walk(p, M, K);
+    auto aborted = [&] { return *(volatile int *)&s_abort != 0; };
+    auto give_up = [&](uint32_t code) {
+        atomicExch(&p.head->err, code);
+        s_abort = 1;
+    };
+
+    if (warp == 0 && lane == 0) {
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        const uint32_t leader_full = at_leader(full0);
+        for (int i = pair; i < walk.items && !aborted(); i += n_pairs) {
+            const Item it = walk.at(p, i);
+            const int m0 = it.tm * TM + (int)rank * 128, n0 = it.tn * TN + (int)rank * 128;
+            int seg = it.k0 / max(1, walk.kblocks), kb = it.k0 - seg * walk.kblocks;
+            for (int k = it.k0; k < it.k1; ++k) {
+                if (!mbar_wait(empty0 + 8 * stage, phase ^ 1)) give_up(201);
+                if (aborted()) break;
+                const uint32_t to = smem_u32(smem + stage * STAGE_BYTES), bar = leader_full + 8 * stage;
+                if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * STAGE_BYTES);
+                const CUtensorMap *ma = (p.sa >> seg) & 1 ? &mapA1 : &mapA0, *mb = (p.sb >> seg) & 1 ? &mapB1 : &mapB0;
+                if (A_MN) {
+                    tma_load(to, ma, bar, m0, kb * BK);
+                    tma_load(to + OPERAND_BYTES / 2, ma, bar, m0 + 64, kb * BK);
+                } else {
+                    tma_load(to, ma, bar, kb * BK, m0);
+                }
+                if (B_MN) {
+                    tma_load(to + OPERAND_BYTES, mb, bar, n0, p.b_row0 + kb * BK);
+                    tma_load(to + OPERAND_BYTES + OPERAND_BYTES / 2, mb, bar, n0 + 64, p.b_row0 + kb * BK);
+                } else {
+                    tma_load(to + OPERAND_BYTES, mb, bar, kb * BK, p.b_row0 + n0);
+                }
+                ++issued;
+                if (++stage == STAGES) stage = 0, phase ^= 1;
+                if (++kb == walk.kblocks) kb = 0, ++seg;
+            }
+        }
+        // A stage's copies have landed once its MMAs are done: wait for the last
+        // ones, so that none writes into shared memory after the CTA's end.
+        int s = 0;
+        uint32_t ph = 0;
+        for (int i = 0; i < issued; ++i) {
+            if (i >= issued - STAGES) mbar_wait(empty0 + 8 * s, ph);
+            if (++s == STAGES) s = 0, ph ^= 1;
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        int stage = 0, n = 0;
+        uint32_t phase = 0;
+        for (int i = pair; i < walk.items && !aborted(); i += n_pairs, ++n) {
+            const Item it = walk.at(p, i);
+            const int b = n & 1;
+            if (!mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1))) give_up(202);
+            if (aborted()) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t d = tmem + b * TN;
+            for (int k = it.k0; k < it.k1; ++k) {
+                if (!mbar_wait(full0 + 8 * stage, phase)) give_up(203);
+                if (aborted()) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at = smem_u32(smem + stage * STAGE_BYTES);
+                const uint64_t da = smem_desc<A_MN>(at), db = smem_desc<B_MN>(at + OPERAND_BYTES);
+#pragma unroll
+                for (int kk = 0; kk < BK / 16; ++kk)
+                    mma(d, da + kk * k_step<A_MN>(), db + kk * k_step<B_MN>(), p.idesc, k > it.k0 || kk ? 1u : 0u);
+                mma_commit(empty0 + 8 * stage);
+                if (++stage == STAGES) stage = 0, phase ^= 1;
+            }
+            mma_commit(acc_full0 + 8 * b);
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t leader_empty = at_leader(acc_empty0);
+        const float factor = MODE == STORE ? out_factor(p) : 1.0f;
+        int n = 0;
+        for (int i = pair; i < walk.items; i += n_pairs, ++n) {
+            const Item it = walk.at(p, i);
+            const int b = n & 1;
+            const bool ok = mbar_wait(acc_full0 + 8 * b, (uint32_t)((n >> 1) & 1)) && !aborted();
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) give_up(204);
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * TN + half * 128;
+            const int row = it.tm * TM + (int)rank * 128 + q * 32 + lane, col = it.tn * TN + half * 128;
+            if constexpr (MODE == ROWS)
+                rows_epilogue<SCALED>(p, at, row, live, col, 2 * it.tn + half);
+            else if constexpr (MODE == GRAD)
+                grad_epilogue<T, SCALED>(p, at, row, live, col);
+            else
+                store_epilogue(p, at, it.k1 > it.k0, row, M, col, it.split, factor);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_empty + 8 * b)
+                             : "memory");
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    pair_sync();  // the other CTA is done with this one's barriers and TMEM
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+}  // namespace ce
+}  // namespace nk

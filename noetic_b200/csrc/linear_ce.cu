@@ -10,270 +10,581 @@
 // the logits of a piece of the vocabulary are computed again and become G, from
 // which the two products take their part; G of one piece is all that is kept.
 
-#include <algorithm>
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
-#include "nk_head.cuh"
+#include <algorithm>
+#include <mutex>
+
+#include "ce_gemm.cuh"
 #include "nk_train.h"
 
 namespace nk {
 
 namespace {
 
-constexpr int TILE = 64, TILE_K = 16;
+using ce::Gemm;
+using ce::Head;
+
 constexpr uint64_t PIECE_BYTES = 256ull << 20;  // of G
+// G is at most 1 before its scale: f16 keeps it down to 2^-38.
+constexpr float G_SCALE = 16384.0f;
 
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+constexpr size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-// ---------------------------------------------------------------- logits in f32
-// A 64 x 64 tile of z per block of 256 threads, 4 x 4 to a thread, 16 columns of
-// x and w staged in shared memory at a time.
-template <class T>
-__device__ __forceinline__ void z_tile(const T *x, int64_t xs, const T *w, int64_t ws, const uint32_t *targets,
-                                       int64_t rows, int d, int vocab, int64_t r0, int c0, int c_end, float (&acc)[4][4]) {
-    __shared__ __align__(16) float As[TILE_K][TILE + 4];
-    __shared__ __align__(16) float Bs[TILE_K][TILE + 4];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    for (int k0 = 0; k0 < d; k0 += TILE_K) {
-#pragma unroll
-        for (int l = 0; l < TILE * TILE_K / 256; ++l) {
-            const int i = threadIdx.x + l * 256, k = i % TILE_K, r = i / TILE_K;
-            const bool kin = k0 + k < d;
-            // (A row without a target is not read.)
-            As[k][r] = kin && r0 + r < rows && targets[r0 + r] < (uint32_t)vocab ? to_f32(x[(r0 + r) * xs + k0 + k]) : 0.0f;
-            Bs[k][r] = kin && c0 + r < c_end ? to_f32(w[(int64_t)(c0 + r) * ws + k0 + k]) : 0.0f;
+// A block joins 32 rows' tiles, in a fixed order: lane = row, warps share the tiles.
+__global__ void __launch_bounds__(256) ce_join_k(LinearCeArgs a, const Head *head, const uint32_t *row_of, const float2 *part,
+                                                 int64_t part_ld, const float *zt, int tiles) {
+    __shared__ float red[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+    const int64_t n = head->live;
+    if ((int64_t)blockIdx.x * 32 >= n) return;
+    const bool in = i < n;
+    const float2 *p = part + i;
+    float m = -INFINITY, s = 0.0f;
+    if (in)
+        for (int t = warp; t < tiles; t += 8) {
+            const float2 q = p[t * part_ld];
+            const float now = fmaxf(m, q.x), base = now == -INFINITY ? 0.0f : now;
+            s = fmaf(q.y, ex2((q.x - base) * LOG2E), s * ex2((m - base) * LOG2E));
+            m = now;
         }
-        __syncthreads();
+    red[warp][lane] = m;
+    __syncthreads();
+    float top = red[0][lane];
 #pragma unroll
-        for (int k = 0; k < TILE_K; ++k) {
-            const float4 a4 = *reinterpret_cast<const float4 *>(&As[k][ty * 4]), b4 = *reinterpret_cast<const float4 *>(&Bs[k][tx * 4]);
-            const float a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+    for (int w = 1; w < 8; ++w) top = fmaxf(top, red[w][lane]);
+    __syncthreads();
+    red[warp][lane] = s * ex2((m - (top == -INFINITY ? 0.0f : top)) * LOG2E);
+    __syncthreads();
+    if (warp != 0 || !in) return;
+    s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
+    for (int w = 0; w < 8; ++w) s += red[w][lane];
+    float ls = logf(s), loss = (top - zt[i]) + ls;
+    // Not a number, or a wait in the product ran out.
+    if (!(isfinite(loss) && isfinite(ls)) || head->err) top = ls = loss = NAN;
+    const int64_t row = row_of[i];
+    if (a.loss) a.loss[row] = loss;
+    if (a.stats) a.stats[2 * row] = top, a.stats[2 * row + 1] = ls;
 }
 
-// part[row][tile] = the tile's maximum and its sum relative to it; zt[row] = the
-// target's logit.
-template <class T>
-__global__ void __launch_bounds__(256) ce_tile_k(LinearCeArgs a, float2 *part, float *zt, int tiles) {
-    float z[4][4];
-    const int64_t r0 = (int64_t)blockIdx.y * TILE;
-    const int c0 = blockIdx.x * TILE;
-    z_tile((const T *)a.x, a.x_stride, (const T *)a.w, a.w_stride, a.targets, a.rows, a.width, a.vocab, r0, c0, a.vocab, z);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = r0 + ty * 4 + i;
-        const uint32_t t = row < a.rows ? a.targets[row] : NO_TOKEN;
-        float m = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = c0 + tx * 4 + j;
-            if (col >= a.vocab) z[i][j] = -INFINITY;
-            if ((uint32_t)col == t && t < (uint32_t)a.vocab) zt[row] = z[i][j];
-            m = fmaxf(m, z[i][j]);
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float s = 0.0f;
-        const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += ex2((z[i][j] - base) * LOG2E);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (tx == 0 && row < a.rows) part[row * tiles + blockIdx.x] = make_float2(m, s);
-    }
-}
-
-// A warp joins a row's tiles, in a fixed order.
-__global__ void __launch_bounds__(256) ce_join_k(LinearCeArgs a, const float2 *part, const float *zt, int tiles) {
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= a.rows) return;
-    float loss = 0.0f, m = 0.0f, ls = 0.0f;
-    if (a.targets[row] < (uint32_t)a.vocab) {
-        const float2 *p = part + row * tiles;
-        m = -INFINITY;
-        for (int i = lane; i < tiles; i += 32) m = fmaxf(m, p[i].x);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float s = 0.0f;
-        for (int i = lane; i < tiles; i += 32) s = fmaf(p[i].y, ex2((p[i].x - m) * LOG2E), s);
-        s = warp_sum(s);
-        ls = logf(s);
-        loss = (m - zt[row]) + ls;
-        if (!isfinite(s)) m = ls = loss = NAN;
-    }
-    if (lane == 0) {
-        if (a.loss) a.loss[row] = loss;
-        if (a.stats) a.stats[2 * row] = m, a.stats[2 * row + 1] = ls;
-    }
-}
-
-// G of columns [v0, v0 + n) of the vocabulary, f32 [rows][n].
-template <class T>
-__global__ void __launch_bounds__(256) ce_grad_tile_k(LinearCeArgs a, float *g, int v0, int n) {
-    float z[4][4];
-    const int64_t r0 = (int64_t)blockIdx.y * TILE;
-    const int c0 = v0 + blockIdx.x * TILE;
-    z_tile((const T *)a.x, a.x_stride, (const T *)a.w, a.w_stride, a.targets, a.rows, a.width, a.vocab, r0, c0, v0 + n, z);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = r0 + ty * 4 + i;
-        if (row >= a.rows) continue;
-        const uint32_t t = a.targets[row];
-        float h = a.grad_scale * (a.row_weight ? a.row_weight[row] : 1.0f);
-        const bool live = t < (uint32_t)a.vocab && h != 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = c0 + tx * 4 + j;
-            if (col >= v0 + n) continue;
-            float v = 0.0f;
-            if (live) {
-                v = ex2(((z[i][j] - a.in_stats[2 * row]) - a.in_stats[2 * row + 1]) * LOG2E);
-                if ((uint32_t)col == t) v -= 1.0f;
-                v *= h;
-            }
-            g[row * n + col - v0] = v;
-        }
-    }
-}
-
-// C[i][j] = sum_k A(i, k) B[k][j], A(i, k) = a[i as + k ak].  A zero of A skips
-// its product: what stands in a row that does not count can be anything.
-// sum: added to (nullable: 0); out: f32, or rounded to T with out_t.
-template <class T>
-__global__ void __launch_bounds__(256) ce_product_k(const float *A, int64_t as, int64_t ak, const T *B, int64_t bs, int64_t M,
-                                                    int N, int64_t K, float *acc, bool add, T *out_t, float *out_f,
-                                                    int64_t os, bool out_add) {
-    __shared__ __align__(16) float As[TILE_K][TILE + 4];
-    __shared__ __align__(16) float Bs[TILE_K][TILE];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t m0 = (int64_t)blockIdx.y * TILE;
-    const int n0 = blockIdx.x * TILE;
-    float c[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += TILE_K) {
-#pragma unroll
-        for (int l = 0; l < TILE * TILE_K / 256; ++l) {
-            const int i = threadIdx.x + l * 256;
-            const int kk = ak == 1 ? i % TILE_K : i / TILE, r = ak == 1 ? i / TILE_K : i % TILE;
-            As[kk][r] = k0 + kk < K && m0 + r < M ? A[(m0 + r) * as + (k0 + kk) * ak] : 0.0f;
-            const int kb = i / TILE, n = i % TILE;
-            Bs[kb][n] = k0 + kb < K && n0 + n < N ? to_f32(B[(k0 + kb) * bs + n0 + n]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < TILE_K; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = As[k][ty * 4 + i];
-                if (x != 0.0f)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) c[i][j] = fmaf(x, Bs[k][tx * 4 + j], c[i][j]);
-            }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = m0 + ty * 4 + i;
-        if (row >= M) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = n0 + tx * 4 + j;
-            if (col >= N) continue;
-            float v = c[i][j];
-            if (acc) {
-                if (add) v += acc[row * N + col];
-                acc[row * N + col] = v;
-            }
-            if (out_t) out_t[row * os + col] = from_f32<T>(out_add ? v + to_f32(out_t[row * os + col]) : v);
-            if (out_f) out_f[row * os + col] = out_add ? v + out_f[row * os + col] : v;
-        }
-    }
-}
-
-struct Plan {
-    int tiles = 0;
-    int piece = 0;  // columns of G at a time
-    size_t part = 0, zt = 0, g = 0, dx = 0, bytes = 0;
+// ---------------------------------------------------------------- rows that count
+// What the rows that count have, in their order.
+struct Index {
+    Head *head;
+    uint32_t *row_of, *place;  // the row of each that counts; the place of each row, or NO_TOKEN
+    uint32_t *target;
+    float2 *stats;   // backward
+    float *weight;   // backward: relative to the largest
 };
 
-Plan make_plan(int64_t rows, int width, int vocab, bool backward) {
+// One block: each thread walks rows / 1024 of the rows, twice, around a prefix sum.
+__global__ void __launch_bounds__(1024) ce_index_k(LinearCeArgs a, Index ix, bool backward) {
+    __shared__ uint32_t sums[32];
+    __shared__ float tops[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t per = (a.rows + 1023) / 1024, r0 = min(a.rows, tid * per), r1 = min(a.rows, r0 + per);
+    auto weight = [&](int64_t r) { return a.row_weight ? a.row_weight[r] : 1.0f; };
+    auto counts = [&](int64_t r) { return a.targets[r] < (uint32_t)a.vocab && (!backward || weight(r) != 0.0f); };
+    uint32_t n = 0;
+    float top = 0.0f;
+    for (int64_t r = r0; r < r1; ++r)
+        if (counts(r)) {
+            ++n;
+            if (backward) top = fmaxf(top, fabsf(weight(r)));
+        }
+    uint32_t upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if (lane == 31) sums[warp] = upto;
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    top = 0.0f;
+    for (int w = 0; w < 32; ++w) {
+        if (w < warp) before += sums[w];
+        all += sums[w];
+        top = fmaxf(top, tops[w]);
+    }
+    uint32_t at = before + upto - n;
+    for (int64_t r = r0; r < r1; ++r) {
+        if (!counts(r)) {
+            ix.place[r] = NO_TOKEN;
+            if (!backward) {
+                if (a.loss) a.loss[r] = 0.0f;
+                if (a.stats) a.stats[2 * r] = a.stats[2 * r + 1] = 0.0f;
+            }
+            continue;
+        }
+        ix.place[r] = at;
+        ix.row_of[at] = (uint32_t)r;
+        ix.target[at] = a.targets[r];
+        if (backward) {
+            ix.stats[at] = make_float2(a.in_stats[2 * r], a.in_stats[2 * r + 1]);
+            ix.weight[at] = __fdiv_rn(weight(r), top);
+        }
+        ++at;
+    }
+    if (tid == 0) *ix.head = Head{0u, all, backward ? top : 1.0f, 0u, 0u};
+}
+
+// The largest finite |x| of the rows that count (place not null), or of all.
+__global__ void __launch_bounds__(256) ce_absmax_k(const float *x, int64_t stride, int64_t rows, int d, const uint32_t *place,
+                                                   uint32_t *out) {
+    float top = 0.0f;
+    const int lane = threadIdx.x & 31;
+    const int64_t step = (int64_t)gridDim.x * 8;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += step) {
+        if (place && place[r] == NO_TOKEN) continue;
+        const float *p = x + r * stride;
+        int c = 0;
+        if (((uintptr_t)p & 15) == 0) {
+            c = d & ~3;
+            for (int i = lane * 4; i < c; i += 128) {
+                const float4 q = *reinterpret_cast<const float4 *>(p + i);
+                const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (isfinite(v[e])) top = fmaxf(top, fabsf(v[e]));
+            }
+        }
+        for (int i = c + lane; i < d; i += 32)
+            if (isfinite(p[i])) top = fmaxf(top, fabsf(p[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // (Bits of numbers that are not negative are in their order; a maximum does not
+    // depend on who comes first.)
+    if (lane == 0 && top > 0.0f) atomicMax(out, __float_as_uint(top));
+}
+
+// The power of two that brings the largest of a matrix to [2^14, 2^15).
+__device__ __forceinline__ float part_scale(uint32_t top) {
+    if (top == 0) return 1.0f;
+    const int e = 14 - ilogbf(__uint_as_float(top));
+    return exp2f((float)min(max(e, -120), 120));
+}
+
+// Rows as the products take them, from 16-byte boundaries and with zeros up to a
+// multiple of 8 columns: 16-bit rows as they are, f32 rows as two scaled f16 parts,
+// high and low, 22 bits together.  place: where each row goes (null: its own
+// place); `fill` rows behind the last become zeros, within `room` rows.  zero: rows that have no place
+// become zeros there (dx).
+template <class T>
+__global__ void __launch_bounds__(256) ce_lay_out_k(const T *src, int64_t stride, int64_t rows, int d, const uint32_t *place,
+                                                    const Head *head, void *dst, int64_t ld, int64_t part, int fill, int64_t room,
+                                                    T *zero, int64_t zero_stride, const uint32_t *top, float *undo) {
+    const int lane = threadIdx.x & 31;
+    const float scale = top ? part_scale(*top) : 1.0f;
+    if (undo && blockIdx.x == 0 && threadIdx.x == 0) *undo = 1.0f / scale;
+    const int64_t step = (int64_t)gridDim.x * 8;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows + fill; r += step) {
+        const bool real = r < rows;
+        int64_t to = r;
+        if (place) {
+            if (real && place[r] == NO_TOKEN) {
+                if (zero)
+                    for (int i = lane; i < d; i += 32) zero[r * zero_stride + i] = from_f32<T>(0.0f);
+                continue;
+            }
+            to = real ? (int64_t)place[r] : (int64_t)head->live + (r - rows);
+            if (to >= room) continue;
+        }
+        const T *p = src + r * stride;
+        if constexpr (sizeof(T) == 2) {
+            T *o = (T *)dst + to * ld;
+            const bool vec = real && ((uintptr_t)p & 15) == 0;
+            for (int i = lane * 8; i < ld; i += 256) {
+                uint4 q = make_uint4(0, 0, 0, 0);
+                T *e = reinterpret_cast<T *>(&q);
+                if (vec && i + 8 <= d)
+                    q = *reinterpret_cast<const uint4 *>(p + i);
+                else if (real)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (i + j < d) e[j] = p[i + j];
+                *reinterpret_cast<uint4 *>(o + i) = q;
+            }
+        } else {
+            __half *o = (__half *)dst + to * ld;
+            const bool vec = real && ((uintptr_t)p & 15) == 0;
+            for (int i = lane * 8; i < ld; i += 256) {
+                float v[8] = {};
+                if (vec && i + 8 <= d) {
+                    const float4 a = *reinterpret_cast<const float4 *>(p + i), b = *reinterpret_cast<const float4 *>(p + i + 4);
+                    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+                } else if (real) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (i + j < d) v[j] = p[i + j];
+                }
+                uint4 hi, lo;
+                __half *h = reinterpret_cast<__half *>(&hi), *l = reinterpret_cast<__half *>(&lo);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = v[j] * scale;
+                    h[j] = __float2half_rn(y);
+                    l[j] = __float2half_rn(isfinite(y) ? y - __half2float(h[j]) : 0.0f);
+                }
+                *reinterpret_cast<uint4 *>(o + i) = hi;
+                *reinterpret_cast<uint4 *>(o + part + i) = lo;
+            }
+        }
+    }
+}
+
+// The sums of a product whose K was split, in their order, rounded on the way out.
+template <class T>
+__global__ void __launch_bounds__(256) ce_reduce_k(Gemm p, int rows_max, int splits) {
+    const int rows = p.live_dim == 0 ? (int)p.head->live : rows_max;
+    const float factor = ce::out_factor(p);
+    const int64_t n = (int64_t)rows * p.ld_acc / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i * 4 / p.ld_acc;
+        const int col = (int)(i * 4 - row * p.ld_acc);
+        if (col >= p.n_valid) continue;
+        const float *a = p.acc + row * p.ld_acc + col;
+        float4 v = *reinterpret_cast<const float4 *>(a);
+        for (int s = 1; s < splits; ++s) {
+            const float4 q = *reinterpret_cast<const float4 *>(a + s * p.acc_split);
+            v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
+        }
+        const float f[4] = {v.x * factor, v.y * factor, v.z * factor, v.w * factor};
+        T *o = (T *)p.out + (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < p.n_valid) o[j] = from_f32<T>(p.out_add ? f[j] + to_f32(o[j]) : f[j]);
+    }
+}
+
+// Where a wait in a product ran out, no gradient is right: NaN.
+template <class T, class W>
+__global__ void ce_check_k(const Head *head, T *dx, int64_t rows, int64_t dxs, W *dw, int64_t vocab, int64_t dws, int d) {
+    if (head->err == 0) return;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (rows + vocab) * d; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / d;
+        const int c = (int)(i - r * d);
+        if (r < rows) {
+            if (dx) dx[r * dxs + c] = from_f32<T>(NAN);
+        } else if (dw) {
+            dw[(r - rows) * dws + c] = from_f32<W>(NAN);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+    });
+    return fn;
+}
+
+// Boxes of 64 columns and box_rows rows of a 16-bit matrix, 128-byte swizzle.
+bool make_map(CUtensorMap *map, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    auto fn = encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, one[2] = {1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base),
+              dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Where everything is in the workspace, and how the work is cut.
+struct Plan {
+    int64_t mp = 0;      // rows, up to whole tiles
+    int64_t dp = 0;      // columns of laid out rows
+    bool split = false;  // f32: two parts
+    bool copy_w = false;
+    int tiles = 0;       // partial results of a row
+    int piece = 0;       // tokens of G at a time
+    int64_t ldg = 0, ld_acc = 0;
+    int dx_splits = 1, dw_splits = 1;
+    size_t head = 0, row_of = 0, place = 0, target = 0, stats = 0, weight = 0, scales = 0, x = 0, w = 0, part = 0, zt = 0, g = 0,
+           dx = 0, dw = 0, bytes = 0;
+};
+
+// Pieces of K for a product of few tiles: as many as fill the pairs, each of 8
+// K-blocks at least.
+int pick_splits(int64_t tiles, int64_t kblocks, int pairs) {
+    const int64_t s = std::min<int64_t>(pairs / std::max<int64_t>(1, tiles), kblocks / 8);
+    return (int)std::max<int64_t>(1, s);
+}
+
+Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride, bool backward) {
     Plan p;
     auto room = [&](size_t n) {
         const size_t at = p.bytes;
-        p.bytes += round256(n);
+        p.bytes += round_up(n, 256);
         return at;
     };
-    p.tiles = (vocab + TILE - 1) / TILE;
+    p.mp = (int64_t)round_up((size_t)std::max<int64_t>(rows, 1), ce::TM);
+    p.dp = (int64_t)round_up((size_t)width, 8);
+    p.split = dtype == NK_F32;
+    p.copy_w = p.split || ((uintptr_t)w & 15) != 0 || w_stride % 8 != 0;
+    const size_t parts = p.split ? 2 : 1;
+    p.head = room(sizeof(Head));
+    p.scales = room(8);
+    p.row_of = room((size_t)rows * 4);
+    p.place = room((size_t)rows * 4);
+    p.target = room((size_t)rows * 4);
+    p.x = room((size_t)p.mp * p.dp * 2 * parts);
+    if (p.copy_w) p.w = room((size_t)vocab * p.dp * 2 * parts);
     if (!backward) {
-        p.part = room((size_t)rows * p.tiles * 8);
+        p.tiles = 2 * ((vocab + ce::TN - 1) / ce::TN);
+        p.part = room((size_t)p.mp * p.tiles * 8);
         p.zt = room((size_t)rows * 4);
-    } else {
-        const uint64_t fit = PIECE_BYTES / 4 / std::max<uint64_t>(1, (uint64_t)rows) / TILE * TILE;
-        p.piece = (int)std::min<uint64_t>(std::max<uint64_t>(fit, 1024), (uint64_t)vocab);
-        p.g = room((size_t)rows * p.piece * 4);
-        p.dx = room((size_t)rows * width * 4);
+        return p;
     }
+    p.stats = room((size_t)rows * 8);
+    p.weight = room((size_t)rows * 4);
+    const uint64_t fit = PIECE_BYTES / 2 / parts / std::max<uint64_t>(1, (uint64_t)p.mp) / ce::TN * ce::TN;
+    p.piece = (int)std::min<uint64_t>(std::max<uint64_t>(fit, 4 * ce::TN), (uint64_t)vocab);
+    p.ldg = (int64_t)round_up((size_t)p.piece, ce::TN);
+    p.g = room((size_t)p.mp * p.ldg * 2 * parts);
+    p.ld_acc = (int64_t)round_up((size_t)width, ce::TN);
+    const int pairs = 74;
+    const int64_t nt = p.ld_acc / ce::TN, segs = p.split ? 3 : 1;
+    p.dx_splits = pick_splits(p.mp / ce::TM * nt, p.ldg / ce::BK * segs, pairs);
+    p.dw_splits = pick_splits(p.ldg / ce::TN * nt, p.mp / ce::BK * segs, pairs);
+    if (p.dx_splits > 1 || p.piece < vocab) p.dx = room((size_t)p.dx_splits * p.mp * p.ld_acc * 4);
+    if (p.dw_splits > 1) p.dw = room((size_t)p.dw_splits * p.ldg * p.ld_acc * 4);
     return p;
 }
 
-template <class T>
-cudaError_t forward(const LinearCeArgs &a, cudaStream_t st) {
-    const Plan p = make_plan(a.rows, a.width, a.vocab, false);
-    float2 *part = (float2 *)((char *)a.workspace + p.part);
-    float *zt = (float *)((char *)a.workspace + p.zt);
-    ce_tile_k<T><<<dim3((unsigned)p.tiles, (unsigned)((a.rows + TILE - 1) / TILE)), 256, 0, st>>>(a, part, zt, p.tiles);
-    ce_join_k<<<(unsigned)((a.rows + 7) / 8), 256, 0, st>>>(a, part, zt, p.tiles);
+// Instruction descriptor: f32 sums, f16 or bf16 factors, 256 x 256, majors.
+uint32_t instruction(bool bf16, bool a_mn, bool b_mn) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
+           ((uint32_t)(ce::TN >> 3) << 17) | ((uint32_t)(ce::TM >> 4) << 24);
+}
+
+struct Maps {
+    CUtensorMap a[2], b[2];
+};
+
+template <int MODE, class T, bool SCALED, bool A_MN, bool B_MN>
+cudaError_t launch(const Maps &m, const Gemm &g, int sms, cudaStream_t st) {
+    auto *k = ce::gemm_k<MODE, T, SCALED, A_MN, B_MN>;
+    cudaError_t e = allow_shared(k, ce::SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    const int64_t items = (int64_t)((g.M + ce::TM - 1) / ce::TM) * ((g.N + ce::TN - 1) / ce::TN) * g.splits;
+    const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(sms / 2, items));
+    k<<<2 * pairs, ce::THREADS, ce::SMEM_BYTES, st>>>(m.a[0], m.a[1], m.b[0], m.b[1], g);
     return cudaGetLastError();
 }
 
-template <class T>
-cudaError_t backward(const LinearCeArgs &a, cudaStream_t st) {
-    const Plan p = make_plan(a.rows, a.width, a.vocab, true);
-    float *g = (float *)((char *)a.workspace + p.g), *acc = (float *)((char *)a.workspace + p.dx);
-    const unsigned by = (unsigned)((a.rows + TILE - 1) / TILE), bd = (unsigned)((a.width + TILE - 1) / TILE);
-    for (int v0 = 0; v0 < a.vocab; v0 += p.piece) {
-        const int n = std::min(p.piece, a.vocab - v0);
-        const unsigned bv = (unsigned)((n + TILE - 1) / TILE);
-        if (a.rows) ce_grad_tile_k<T><<<dim3(bv, by), 256, 0, st>>>(a, g, v0, n);
-        if (a.dx && a.rows)
-            ce_product_k<T><<<dim3(bd, by), 256, 0, st>>>(g, n, 1, (const T *)a.w + v0 * a.w_stride, a.w_stride, a.rows,
-                                                          a.width, n, acc, v0 != 0,
-                                                          v0 + n == a.vocab ? (T *)a.dx : nullptr, nullptr, a.dx_stride, false);
-        if (a.dw) {
-            const bool f32 = a.dw_dtype == NK_F32;
-            ce_product_k<T><<<dim3(bd, bv), 256, 0, st>>>(g, 1, n, (const T *)a.x, a.x_stride, n, a.width, a.rows, nullptr,
-                                                          false, f32 ? nullptr : (T *)a.dw + v0 * a.dw_stride,
-                                                          f32 ? (float *)a.dw + v0 * a.dw_stride : nullptr, a.dw_stride,
-                                                          a.accumulate != 0);
-        }
+// T: the type of x and w; P: that of the parts the products take.
+template <class T, class P>
+struct Call {
+    static constexpr bool SPLIT = sizeof(T) == 4;
+    static constexpr bool BF16 = std::is_same_v<P, __nv_bfloat16>;
+    const LinearCeArgs &a;
+    Plan p;
+    int sms;
+    cudaStream_t st;
+    char *ws;
+    Index ix;
+    float *scales;
+    const P *w;      // as the products take it
+    int64_t w_ld, w_cols;
+
+    Call(const LinearCeArgs &args, bool backward, int n_sms, cudaStream_t stream)
+        : a(args), p(make_plan(args.dtype, args.rows, args.width, args.vocab, args.w, args.w_stride, backward)), sms(n_sms), st(stream),
+          ws((char *)args.workspace) {
+        ix = {at<Head>(p.head), at<uint32_t>(p.row_of), at<uint32_t>(p.place), at<uint32_t>(p.target), at<float2>(p.stats), at<float>(p.weight)};
+        scales = at<float>(p.scales);
+        w = p.copy_w ? at<P>(p.w) : (const P *)a.w;
+        w_ld = p.copy_w ? p.dp : a.w_stride;
+        w_cols = p.copy_w ? p.dp : a.width;
     }
-    return cudaGetLastError();
-}
+    template <class U>
+    U *at(size_t o) const {
+        return (U *)(ws + o);
+    }
+    unsigned blocks(int64_t rows) const { return (unsigned)std::min<int64_t>((rows + 7) / 8, (int64_t)sms * 8); }
+
+    // The index, x and, where it has to be, w laid out.
+    // (Zero rows follow the rows that count: up to a whole K-block of dw.)
+    cudaError_t begin(bool backward) {
+        ce_index_k<<<1, 1024, 0, st>>>(a, ix, backward);
+        uint32_t *tops = nullptr;
+        if (SPLIT) {
+            tops = &ix.head->x_max;
+            if (a.rows) ce_absmax_k<<<blocks(a.rows), 256, 0, st>>>((const float *)a.x, a.x_stride, a.rows, a.width, ix.place, tops);
+            ce_absmax_k<<<blocks(a.vocab), 256, 0, st>>>((const float *)a.w, a.w_stride, a.vocab, a.width, nullptr, tops + 1);
+        }
+        ce_lay_out_k<T><<<blocks(a.rows + ce::TM), 256, 0, st>>>((const T *)a.x, a.x_stride, a.rows, a.width, ix.place, ix.head,
+                                                                 at<void>(p.x), p.dp, p.mp * p.dp, ce::BK - 1, p.mp, (T *)a.dx, a.dx_stride,
+                                                                 tops, SPLIT ? scales : nullptr);
+        if (p.copy_w)
+            ce_lay_out_k<T><<<blocks(a.vocab), 256, 0, st>>>((const T *)a.w, a.w_stride, a.vocab, a.width, nullptr, nullptr,
+                                                             at<void>(p.w), p.dp, (int64_t)a.vocab * p.dp, 0, 0, nullptr, 0,
+                                                             tops ? tops + 1 : nullptr, SPLIT ? scales + 1 : nullptr);
+        return cudaGetLastError();
+    }
+
+    bool map_x(CUtensorMap (&m)[2], int box) const {
+        for (int i = 0; i < (SPLIT ? 2 : 1); ++i)
+            if (!make_map(&m[i], at<P>(p.x) + i * p.mp * p.dp, BF16, p.mp, p.dp, p.dp, box)) return false;
+        if (!SPLIT) m[1] = m[0];
+        return true;
+    }
+    bool map_w(CUtensorMap (&m)[2], int box) const {
+        for (int i = 0; i < (SPLIT ? 2 : 1); ++i)
+            if (!make_map(&m[i], w + i * (int64_t)a.vocab * p.dp, BF16, a.vocab, w_cols, w_ld, box)) return false;
+        if (!SPLIT) m[1] = m[0];
+        return true;
+    }
+    bool map_g(CUtensorMap (&m)[2], int box) const {
+        for (int i = 0; i < (SPLIT ? 2 : 1); ++i)
+            if (!make_map(&m[i], at<P>(p.g) + i * p.mp * p.ldg, BF16, p.mp, p.ldg, p.ldg, box)) return false;
+        if (!SPLIT) m[1] = m[0];
+        return true;
+    }
+    Gemm gemm(int M, int N, int K, int live_dim, bool a_mn, bool b_mn, int splits) const {
+        Gemm g{};
+        g.M = M;
+        g.N = g.n_valid = N;
+        g.K = K;
+        g.live_dim = live_dim;
+        // high * low, low * high, high * high: the small products first.
+        g.segs = SPLIT ? 3 : 1;
+        g.sa = SPLIT ? 2u : 0u;
+        g.sb = SPLIT ? 1u : 0u;
+        g.idesc = instruction(BF16, a_mn, b_mn);
+        g.m_fast = 0;
+        g.group_m = 32;
+        g.splits = splits;
+        const int total = (K + ce::BK - 1) / ce::BK * g.segs;
+        g.kps = std::max(1, (total + splits - 1) / splits);
+        g.head = ix.head;
+        return g;
+    }
+
+    cudaError_t forward() {
+        cudaError_t e = begin(false);
+        if (e != cudaSuccess) return e;
+        Maps m;
+        if (!map_x(m.a, 128) || !map_w(m.b, 128)) return cudaErrorInvalidValue;
+        Gemm g = gemm((int)a.rows, a.vocab, a.width, 0, false, false, 1);
+        g.m_fast = 1;
+        if (SPLIT) g.x_scale = scales, g.w_scale = scales + 1;
+        g.part = at<float2>(p.part);
+        g.part_ld = p.mp;
+        g.zt = at<float>(p.zt);
+        g.target = ix.target;
+        e = launch<ce::ROWS, P, SPLIT, false, false>(m, g, sms, st);
+        if (e != cudaSuccess) return e;
+        ce_join_k<<<(unsigned)((a.rows + 31) / 32), 256, 0, st>>>(a, ix.head, ix.row_of, g.part, p.mp, g.zt, p.tiles);
+        return cudaGetLastError();
+    }
+
+    template <class O>
+    cudaError_t reduce(const Gemm &g, int rows, int splits) const {
+        const int64_t n = (int64_t)rows * g.ld_acc / 4;
+        ce_reduce_k<O><<<(unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, (int64_t)sms * 8)), 256, 0, st>>>(g, rows, splits);
+        return cudaGetLastError();
+    }
+
+    cudaError_t backward() {
+        cudaError_t e = begin(true);
+        if (e != cudaSuccess) return e;
+        Maps mg, mx, mw;
+        if (!map_x(mg.a, 128) || !map_w(mg.b, 128) || !map_g(mx.a, 128) || !map_w(mx.b, 64) || !map_g(mw.a, 64) || !map_x(mw.b, 64))
+            return cudaErrorInvalidValue;
+        const float g_scale = BF16 ? 1.0f : G_SCALE;
+        for (int v0 = 0; v0 < a.vocab; v0 += p.piece) {
+            const int n = std::min(p.piece, a.vocab - v0);
+            const bool last = v0 + n == a.vocab;
+            Gemm g = gemm((int)a.rows, n, a.width, 0, false, false, 1);
+            g.m_fast = 1;
+            g.b_row0 = v0;
+            if (SPLIT) g.x_scale = scales, g.w_scale = scales + 1;
+            g.target = ix.target;
+            g.stats = ix.stats;
+            g.weight = ix.weight;
+            g.g = at<P>(p.g);
+            g.ldg = p.ldg;
+            g.g_part = p.mp * p.ldg;
+            g.col0 = v0;
+            g.g_scale = g_scale;
+            if (a.rows) e = launch<ce::GRAD, P, SPLIT, false, false>(mg, g, sms, st);
+            if (e != cudaSuccess) return e;
+            if (a.dx) {
+                Gemm c = gemm((int)a.rows, a.width, n, 0, false, true, p.dx_splits);
+                c.b_row0 = v0;
+                if (SPLIT) c.w_scale = scales + 1;
+                c.acc = p.dx ? at<float>(p.dx) : nullptr;
+                c.ld_acc = p.ld_acc;
+                c.acc_split = p.mp * p.ld_acc;
+                c.add = v0 != 0;
+                c.keep = !last || p.dx_splits > 1;
+                c.out = a.dx;
+                c.out_ld = a.dx_stride;
+                c.out_dtype = a.dtype;
+                c.out_row = ix.row_of;
+                c.out_scale = a.grad_scale / g_scale;
+                e = launch<ce::STORE, P, SPLIT, false, true>(mx, c, sms, st);
+                if (e == cudaSuccess && last && p.dx_splits > 1) e = reduce<T>(c, (int)a.rows, p.dx_splits);
+                if (e != cudaSuccess) return e;
+            }
+            if (a.dw) {
+                Gemm c = gemm(n, a.width, (int)a.rows, 1, true, true, p.dw_splits);
+                if (SPLIT) c.x_scale = scales;
+                c.acc = p.dw ? at<float>(p.dw) : nullptr;
+                c.ld_acc = p.ld_acc;
+                c.acc_split = p.ldg * p.ld_acc;
+                c.keep = p.dw_splits > 1;
+                c.out = a.dw;
+                c.out_ld = a.dw_stride;
+                c.out_row0 = v0;
+                c.out_dtype = a.dw_dtype;
+                c.out_add = a.accumulate;
+                c.out_scale = a.grad_scale / g_scale;
+                e = launch<ce::STORE, P, SPLIT, true, true>(mw, c, sms, st);
+                if (e == cudaSuccess && p.dw_splits > 1)
+                    e = a.dw_dtype == NK_F32 ? reduce<float>(c, n, p.dw_splits) : reduce<T>(c, n, p.dw_splits);
+                if (e != cudaSuccess) return e;
+            }
+        }
+        if (a.dw_dtype == NK_F32)
+            ce_check_k<T, float><<<(unsigned)sms, 256, 0, st>>>(ix.head, (T *)a.dx, a.rows, a.dx_stride, (float *)a.dw, a.vocab, a.dw_stride, a.width);
+        else
+            ce_check_k<T, T><<<(unsigned)sms, 256, 0, st>>>(ix.head, (T *)a.dx, a.rows, a.dx_stride, (T *)a.dw, a.vocab, a.dw_stride, a.width);
+        return cudaGetLastError();
+    }
+};
 
 }  // namespace
 
 size_t linear_ce_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
                                  bool backward) {
-    return make_plan(rows, width, vocab, backward).bytes;
+    return make_plan(dtype, rows, width, vocab, w, w_stride, backward).bytes;
 }
 
 cudaError_t linear_ce(const LinearCeArgs &a, int sms, cudaStream_t st) {
-    return a.dtype == NK_F32 ? forward<float>(a, st) : a.dtype == NK_F16 ? forward<__half>(a, st) : forward<__nv_bfloat16>(a, st);
+    if (a.dtype == NK_F32) return Call<float, __half>(a, false, sms, st).forward();
+    if (a.dtype == NK_F16) return Call<__half, __half>(a, false, sms, st).forward();
+    return Call<__nv_bfloat16, __nv_bfloat16>(a, false, sms, st).forward();
 }
 
 cudaError_t linear_ce_backward(const LinearCeArgs &a, int sms, cudaStream_t st) {
-    return a.dtype == NK_F32 ? backward<float>(a, st) : a.dtype == NK_F16 ? backward<__half>(a, st) : backward<__nv_bfloat16>(a, st);
+    if (a.dtype == NK_F32) return Call<float, __half>(a, true, sms, st).backward();
+    if (a.dtype == NK_F16) return Call<__half, __half>(a, true, sms, st).backward();
+    return Call<__nv_bfloat16, __nv_bfloat16>(a, true, sms, st).backward();
 }
 
 }  // namespace nk
