@@ -32,6 +32,12 @@ constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
 constexpr int THREADS = 384, EPI_WARPS = 8;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint64_t WAIT_NS = 1000000000ull;
+// The tensor cores cut, not round, when they add to a sum, so a chain of products
+// is off by half a step of the sum for each 16 of K, all one way (measured: 1.7e-8
+// of a logit each).  Where f32 results depend on it (the loss; f32 gradients), a
+// chain ends after CHAIN K-blocks and the epilogue's registers add the chains up.
+constexpr int CHAIN = 4;
+constexpr int REGS_FEW = 64, REGS_MANY = 216;  // 4 warps and 8 of 32: within 384 * 168
 
 // What the first kernel of a call finds out, for the others (the workspace's head).
 struct Head {
@@ -177,6 +183,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // A tile's piece: its row and column block and its K-blocks.
 struct Item {
     int tm, tn, split, k0, k1;
@@ -212,23 +231,27 @@ struct Walk {
 };
 
 // ---------------------------------------------------------------- epilogues
-// A warp has 32 rows (lane = row) and 128 columns of its CTA's 128 x 256 sums.
-// `row` counts rows that count (or tokens, in dw), `col` is the first column.
+// A warp has 32 rows (lane = row) and 128 columns of its CTA's 128 x 256 sums, which
+// come 32 at a time, from TMEM or (LONG) from the registers that added them up.
+// `row` counts rows that count (or tokens, in dw), `col` is the first column; every
+// lane of a warp calls chunk().
 
 // The maximum and the sum of exponentials of 128 logits of a row.
 template <bool SCALED>
-__device__ __forceinline__ void rows_epilogue(const Gemm &p, uint32_t tmem, int row, int live, int col, int slot) {
-    const uint32_t t = row < live ? p.target[row] : NO_TOKEN;
+struct RowsEpilogue {
+    const Gemm &p;
+    const int row, live, col, slot;
+    const uint32_t t;
     float m = -INFINITY, s = 0.0f;
-    const float xs = SCALED ? *p.x_scale : 1.0f, ws = SCALED ? *p.w_scale : 1.0f;
-#pragma unroll 1
-    for (int c = 0; c < 128; c += 32) {
-        if (col + c >= p.n_valid) break;  // warp-uniform
-        float v[32];
-        tmem_ld32(tmem + c, v);
-        if (SCALED)
+    __device__ __forceinline__ RowsEpilogue(const Gemm &g, int r, int n, int c, int at)
+        : p(g), row(r), live(n), col(c), slot(at), t(r < n ? g.target[r] : NO_TOKEN) {}
+    __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
+        if (col + c >= p.n_valid) return;  // warp-uniform
+        if (SCALED) {
+            const float xs = *p.x_scale, ws = *p.w_scale;
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = v[j] * xs * ws;
+        }
         if (col + c + 32 > p.n_valid)
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -248,34 +271,40 @@ __device__ __forceinline__ void rows_epilogue(const Gemm &p, uint32_t tmem, int 
         s += (a[0] + a[1]) + (a[2] + a[3]);
         m = now;
     }
-    if (row < live) p.part[(int64_t)slot * p.part_ld + row] = make_float2(m, s);
-}
+    __device__ __forceinline__ void end() const {
+        if (row < live) p.part[(int64_t)slot * p.part_ld + row] = make_float2(m, s);
+    }
+};
 
 // G = weight (exp(z - m - log s) - [t]) of 128 logits of a row; zeros where there
 // is no row or no token, since the products that follow read whole blocks.
 template <class T, bool SCALED>
-__device__ __forceinline__ void grad_epilogue(const Gemm &p, uint32_t tmem, int row, int live, int col) {
-    const bool in = row < live;
-    const uint32_t t = in ? p.target[row] - (uint32_t)p.col0 : NO_TOKEN;
-    const float2 st = in ? p.stats[row] : make_float2(0.0f, 0.0f);
-    const float h = in ? p.weight[row] * p.g_scale : 0.0f;
-    const float xs = SCALED ? *p.x_scale : 1.0f, ws = SCALED ? *p.w_scale : 1.0f;
-#pragma unroll 1
-    for (int c = 0; c < 128; c += 32) {
-        float v[32];
-        tmem_ld32(tmem + c, v);
+struct GradEpilogue {
+    const Gemm &p;
+    const bool in;
+    const int col;
+    const uint32_t t;
+    const float2 st;
+    const float h;
+    T *const g;
+    __device__ __forceinline__ GradEpilogue(const Gemm &q, int row, int live, int c)
+        : p(q), in(row < live), col(c), t(in ? q.target[row] - (uint32_t)q.col0 : NO_TOKEN),
+          st(in ? q.stats[row] : make_float2(0.0f, 0.0f)), h(in ? q.weight[row] * q.g_scale : 0.0f),
+          g((T *)q.g + (int64_t)row * q.ldg + c) {}
+    __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
+        const float xs = SCALED ? *p.x_scale : 1.0f, ws = SCALED ? *p.w_scale : 1.0f;
+        const bool whole = in && col + c + 32 <= p.n_valid;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
             float z = v[j];
             if (SCALED) z = z * xs * ws;
-            z = ex2(((z - st.x) - st.y) * LOG2E);
-            v[j] = in && col + c + j < p.n_valid ? z * h : 0.0f;
+            z = ex2(((z - st.x) - st.y) * LOG2E) * h;
+            v[j] = whole || (in && col + c + j < p.n_valid) ? z : 0.0f;
         }
         if (t - (uint32_t)(col + c) < 32u)
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-                if (t == (uint32_t)(col + c + j)) v[j] = fmaf(v[j], 1.0f, -h);
-        T *g = (T *)p.g + (int64_t)row * p.ldg + col + c;
+                if (t == (uint32_t)(col + c + j)) v[j] -= h;
 #pragma unroll
         for (int part = 0; part < (SCALED ? 2 : 1); ++part) {
 #pragma unroll
@@ -287,11 +316,12 @@ __device__ __forceinline__ void grad_epilogue(const Gemm &p, uint32_t tmem, int 
                     o[e] = from_f32<T>(v[j + e]);
                     if (SCALED) v[j + e] -= to_f32(o[e]);
                 }
-                *reinterpret_cast<uint4 *>(g + part * p.g_part + j) = q;
+                *reinterpret_cast<uint4 *>(g + part * p.g_part + c + j) = q;
             }
         }
     }
-}
+    __device__ __forceinline__ void end() const {}
+};
 
 template <class T>
 __device__ __forceinline__ void store_out(const Gemm &p, const float (&v)[32], int64_t at, int col) {
@@ -321,18 +351,23 @@ __device__ __forceinline__ float out_factor(const Gemm &p) {
     return f;
 }
 
-__device__ __forceinline__ void store_epilogue(const Gemm &p, uint32_t tmem, bool some, int row, int rows, int col,
-                                               int split, float factor) {
-#pragma unroll 1
-    for (int c = 0; c < 128; c += 32) {
-        if (col + c >= p.n_valid) break;  // warp-uniform
-        float v[32];
-        tmem_ld32(tmem + c, v);
-        if (!some)  // (No K at all: the accumulator holds nothing.)
+// F32: the output is always f32 (f32 inputs).
+template <bool F32>
+struct StoreEpilogue {
+    const Gemm &p;
+    const bool some;  // K has anything: else the accumulator holds nothing
+    const int row, rows, col;
+    const float factor;
+    float *const acc;
+    __device__ __forceinline__ StoreEpilogue(const Gemm &g, bool any, int r, int n, int c, int split, float f)
+        : p(g), some(any), row(r), rows(n), col(c), factor(f),
+          acc(g.acc ? g.acc + (int64_t)split * g.acc_split + (int64_t)r * g.ld_acc + c : nullptr) {}
+    __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
+        if (col + c >= p.n_valid || row >= rows) return;
+        if (!some)
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-        if (row >= rows) continue;
-        float *a = p.acc ? p.acc + (int64_t)split * p.acc_split + (int64_t)row * p.ld_acc + col + c : nullptr;
+        float *a = acc + c;
         if (p.add)
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
@@ -342,23 +377,34 @@ __device__ __forceinline__ void store_epilogue(const Gemm &p, uint32_t tmem, boo
         if (p.keep) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(a + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            continue;
+            return;
         }
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= factor;
         const int64_t at = (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld;
-        if (p.out_dtype == 0)
+        if (F32 || p.out_dtype == 0)
             store_out<float>(p, v, at, col + c);
         else if (p.out_dtype == 1)
             store_out<__half>(p, v, at, col + c);
         else
             store_out<__nv_bfloat16>(p, v, at, col + c);
     }
-}
+    __device__ __forceinline__ void end() const {}
+};
 
 // ---------------------------------------------------------------- the kernel
-// T: the parts' type.  SCALED: f32 inputs, taken as two scaled f16 parts.
-template <int MODE, class T, bool SCALED, bool A_MN, bool B_MN>
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// T: the parts' type.  SCALED: f32 inputs, taken as two scaled f16 parts.  LONG:
+// chains of CHAIN K-blocks, added up in registers.
+template <int MODE, class T, bool SCALED, bool LONG, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
        const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ Gemm p) {
@@ -407,6 +453,8 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
         s_abort = 1;
     };
 
+    if (warp < 4) {
+    if constexpr (LONG) fewer_registers<REGS_FEW>();
     if (warp == 0 && lane == 0) {
         int stage = 0, issued = 0;
         uint32_t phase = 0;
@@ -449,54 +497,103 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     } else if (warp == 1 && lane == 0 && rank == 0) {
         int stage = 0, n = 0;
         uint32_t phase = 0;
-        for (int i = pair; i < walk.items && !aborted(); i += n_pairs, ++n) {
+        for (int i = pair; i < walk.items && !aborted(); i += n_pairs) {
             const Item it = walk.at(p, i);
-            const int b = n & 1;
-            if (!mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1))) give_up(202);
-            if (aborted()) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t d = tmem + b * TN;
-            for (int k = it.k0; k < it.k1; ++k) {
-                if (!mbar_wait(full0 + 8 * stage, phase)) give_up(203);
+            for (int k = it.k0;;) {
+                const int end = LONG ? min(it.k1, k + CHAIN) : it.k1, first = k, b = n & 1;
+                if (!mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1))) give_up(202);
                 if (aborted()) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t at = smem_u32(smem + stage * STAGE_BYTES);
-                const uint64_t da = smem_desc<A_MN>(at), db = smem_desc<B_MN>(at + OPERAND_BYTES);
+                const uint32_t d = tmem + b * TN;
+                for (; k < end; ++k) {
+                    if (!mbar_wait(full0 + 8 * stage, phase)) give_up(203);
+                    if (aborted()) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = smem_u32(smem + stage * STAGE_BYTES);
+                    const uint64_t da = smem_desc<A_MN>(at), db = smem_desc<B_MN>(at + OPERAND_BYTES);
 #pragma unroll
-                for (int kk = 0; kk < BK / 16; ++kk)
-                    mma(d, da + kk * k_step<A_MN>(), db + kk * k_step<B_MN>(), p.idesc, k > it.k0 || kk ? 1u : 0u);
-                mma_commit(empty0 + 8 * stage);
-                if (++stage == STAGES) stage = 0, phase ^= 1;
+                    for (int kk = 0; kk < BK / 16; ++kk)
+                        mma(d, da + kk * k_step<A_MN>(), db + kk * k_step<B_MN>(), p.idesc, k > first || kk ? 1u : 0u);
+                    mma_commit(empty0 + 8 * stage);
+                    if (++stage == STAGES) stage = 0, phase ^= 1;
+                }
+                mma_commit(acc_full0 + 8 * b);
+                ++n;
+                if (k >= it.k1 || aborted()) break;
             }
-            mma_commit(acc_full0 + 8 * b);
         }
-    } else if (warp >= 4) {
+    }
+    } else {
+        if constexpr (LONG) more_registers<REGS_MANY>();
         const int q = warp & 3, half = (warp - 4) >> 2;
         const uint32_t leader_empty = at_leader(acc_empty0);
         const float factor = MODE == STORE ? out_factor(p) : 1.0f;
         int n = 0;
-        for (int i = pair; i < walk.items; i += n_pairs, ++n) {
-            const Item it = walk.at(p, i);
-            const int b = n & 1;
-            const bool ok = mbar_wait(acc_full0 + 8 * b, (uint32_t)((n >> 1) & 1)) && !aborted();
+        // The next accumulator: wait for it, or give it back.
+        auto take = [&]() -> bool {
+            const bool ok = mbar_wait(acc_full0 + 8 * (n & 1), (uint32_t)((n >> 1) & 1)) && !aborted();
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up(204);
-                break;
+                return false;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + b * TN + half * 128;
-            const int row = it.tm * TM + (int)rank * 128 + q * 32 + lane, col = it.tn * TN + half * 128;
-            if constexpr (MODE == ROWS)
-                rows_epilogue<SCALED>(p, at, row, live, col, 2 * it.tn + half);
-            else if constexpr (MODE == GRAD)
-                grad_epilogue<T, SCALED>(p, at, row, live, col);
-            else
-                store_epilogue(p, at, it.k1 > it.k0, row, M, col, it.split, factor);
+            return true;
+        };
+        auto give = [&] {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0)
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_empty + 8 * b)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_empty + 8 * (n & 1))
                              : "memory");
+            ++n;
+        };
+        const uint32_t mine = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
+        bool fine = true;
+        for (int i = pair; fine && i < walk.items; i += n_pairs) {
+            const Item it = walk.at(p, i);
+            const int row = it.tm * TM + (int)rank * 128 + q * 32 + lane, col = it.tn * TN + half * 128;
+            auto whole = [&](auto &&e) {
+                if constexpr (LONG) {
+                    float sum[4][32];
+                    fine = take();
+                    if (!fine) return;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(mine + (n & 1) * TN + c * 32, sum[c]);
+                    give();
+#pragma unroll 1
+                    for (int k = it.k0 + CHAIN; k < it.k1; k += CHAIN) {
+                        fine = take();
+                        if (!fine) return;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            float v[16];
+                            tmem_ld16(mine + (n & 1) * TN + c * 16, v);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sum[c / 2][c % 2 * 16 + j] += v[j];
+                        }
+                        give();
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) e.chunk(c * 32, sum[c]);
+                } else {
+                    fine = take();
+                    if (!fine) return;
+#pragma unroll 1
+                    for (int c = 0; c < 128; c += 32) {
+                        float v[32];
+                        tmem_ld32(mine + (n & 1) * TN + c, v);
+                        e.chunk(c, v);
+                    }
+                    give();
+                }
+                e.end();
+            };
+            if constexpr (MODE == ROWS)
+                whole(RowsEpilogue<SCALED>(p, row, live, col, 2 * it.tn + half));
+            else if constexpr (MODE == GRAD)
+                whole(GradEpilogue<T, SCALED>(p, row, live, col));
+            else
+                whole(StoreEpilogue<SCALED>(p, it.k1 > it.k0, row, M, col, it.split, factor));
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

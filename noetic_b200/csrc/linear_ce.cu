@@ -375,9 +375,9 @@ struct Maps {
     CUtensorMap a[2], b[2];
 };
 
-template <int MODE, class T, bool SCALED, bool A_MN, bool B_MN>
+template <int MODE, class T, bool SCALED, bool LONG, bool A_MN, bool B_MN>
 cudaError_t launch(const Maps &m, const Gemm &g, int sms, cudaStream_t st) {
-    auto *k = ce::gemm_k<MODE, T, SCALED, A_MN, B_MN>;
+    auto *k = ce::gemm_k<MODE, T, SCALED, LONG, A_MN, B_MN>;
     cudaError_t e = allow_shared(k, ce::SMEM_BYTES);
     if (e != cudaSuccess) return e;
     const int64_t items = (int64_t)((g.M + ce::TM - 1) / ce::TM) * ((g.N + ce::TN - 1) / ce::TN) * g.splits;
@@ -486,7 +486,7 @@ struct Call {
         g.part_ld = p.mp;
         g.zt = at<float>(p.zt);
         g.target = ix.target;
-        e = launch<ce::ROWS, P, SPLIT, false, false>(m, g, sms, st);
+        e = launch<ce::ROWS, P, SPLIT, true, false, false>(m, g, sms, st);
         if (e != cudaSuccess) return e;
         ce_join_k<<<(unsigned)((a.rows + 31) / 32), 256, 0, st>>>(a, ix.head, ix.row_of, g.part, p.mp, g.zt, p.tiles);
         return cudaGetLastError();
@@ -521,7 +521,7 @@ struct Call {
             g.g_part = p.mp * p.ldg;
             g.col0 = v0;
             g.g_scale = g_scale;
-            if (a.rows) e = launch<ce::GRAD, P, SPLIT, false, false>(mg, g, sms, st);
+            if (a.rows) e = launch<ce::GRAD, P, SPLIT, SPLIT, false, false>(mg, g, sms, st);
             if (e != cudaSuccess) return e;
             if (a.dx) {
                 Gemm c = gemm((int)a.rows, a.width, n, 0, false, true, p.dx_splits);
@@ -537,7 +537,7 @@ struct Call {
                 c.out_dtype = a.dtype;
                 c.out_row = ix.row_of;
                 c.out_scale = a.grad_scale / g_scale;
-                e = launch<ce::STORE, P, SPLIT, false, true>(mx, c, sms, st);
+                e = launch<ce::STORE, P, SPLIT, SPLIT, false, true>(mx, c, sms, st);
                 if (e == cudaSuccess && last && p.dx_splits > 1) e = reduce<T>(c, (int)a.rows, p.dx_splits);
                 if (e != cudaSuccess) return e;
             }
@@ -554,7 +554,7 @@ struct Call {
                 c.out_dtype = a.dw_dtype;
                 c.out_add = a.accumulate;
                 c.out_scale = a.grad_scale / g_scale;
-                e = launch<ce::STORE, P, SPLIT, true, true>(mw, c, sms, st);
+                e = launch<ce::STORE, P, SPLIT, SPLIT, true, true>(mw, c, sms, st);
                 if (e == cudaSuccess && p.dw_splits > 1)
                     e = a.dw_dtype == NK_F32 ? reduce<float>(c, n, p.dw_splits) : reduce<T>(c, n, p.dw_splits);
                 if (e != cudaSuccess) return e;
