@@ -13,8 +13,8 @@
 //               nothing is transposed in memory;
 //   warp 1      the leader's issues the MMAs, 4 to a K-block;
 //   warps 4-11  epilogue, from one of two accumulators while the other fills.
-// Every wait is bounded (1 s); where one runs out, the kernel records it, every
-// role leaves its loop, copies in flight are waited for and TMEM is freed.
+// Every wait is bounded (1 s); where one runs out, the kernel records it, the
+// roles leave their loops, copies in flight are waited for and TMEM is freed.
 #pragma once
 
 #include <cuda.h>
@@ -90,6 +90,15 @@ __device__ __forceinline__ uint64_t globaltimer() {
     uint64_t t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
+}
+
+// One lane of the warp.  (A branch on it tells the compiler that what follows is
+// one thread's; a branch on the lane's number does not, and costs the MMAs and copies
+// that it guards about 100 cycles each.)
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+    return r != 0;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -412,7 +421,6 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = (uint64_t *)(smem + STAGES * STAGE_BYTES);
     uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 4);
-    __shared__ int s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
@@ -420,7 +428,6 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     const uint32_t acc_full0 = smem_u32(&bars[2 * STAGES]), acc_empty0 = smem_u32(&bars[2 * STAGES + 2]);
 
     if (threadIdx.x == 0) {
-        s_abort = 0;
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full0 + 8 * s, 1);
             mbar_init(empty0 + 8 * s, 1);
@@ -447,82 +454,104 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     const int live = (int)p.head->live;
     const int M = p.live_dim == 0 ? live : p.M, K = p.live_dim == 1 ? live : p.K;
     const Walk walk(p, M, K);
-    auto aborted = [&] { return *(volatile int *)&s_abort != 0; };
-    auto give_up = [&](uint32_t code) {
-        atomicExch(&p.head->err, code);
-        s_abort = 1;
-    };
+    // A wait that ran out ends the role that waited; the others' waits on it run out too.
+    auto give_up = [&](uint32_t code) { atomicExch(&p.head->err, code); };
 
     if (warp < 4) {
-    if constexpr (LONG) fewer_registers<REGS_FEW>();
-    if (warp == 0 && lane == 0) {
-        int stage = 0, issued = 0;
-        uint32_t phase = 0;
-        const uint32_t leader_full = at_leader(full0);
-        for (int i = pair; i < walk.items && !aborted(); i += n_pairs) {
-            const Item it = walk.at(p, i);
-            const int m0 = it.tm * TM + (int)rank * 128, n0 = it.tn * TN + (int)rank * 128;
-            int seg = it.k0 / max(1, walk.kblocks), kb = it.k0 - seg * walk.kblocks;
-            for (int k = it.k0; k < it.k1; ++k) {
-                if (!mbar_wait(empty0 + 8 * stage, phase ^ 1)) give_up(201);
-                if (aborted()) break;
-                const uint32_t to = smem_u32(smem + stage * STAGE_BYTES), bar = leader_full + 8 * stage;
-                if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * STAGE_BYTES);
-                const CUtensorMap *ma = (p.sa >> seg) & 1 ? &mapA1 : &mapA0, *mb = (p.sb >> seg) & 1 ? &mapB1 : &mapB0;
-                if (A_MN) {
-                    tma_load(to, ma, bar, m0, kb * BK);
-                    tma_load(to + OPERAND_BYTES / 2, ma, bar, m0 + 64, kb * BK);
-                } else {
-                    tma_load(to, ma, bar, kb * BK, m0);
-                }
-                if (B_MN) {
-                    tma_load(to + OPERAND_BYTES, mb, bar, n0, p.b_row0 + kb * BK);
-                    tma_load(to + OPERAND_BYTES + OPERAND_BYTES / 2, mb, bar, n0 + 64, p.b_row0 + kb * BK);
-                } else {
-                    tma_load(to + OPERAND_BYTES, mb, bar, kb * BK, p.b_row0 + n0);
-                }
-                ++issued;
-                if (++stage == STAGES) stage = 0, phase ^= 1;
-                if (++kb == walk.kblocks) kb = 0, ++seg;
-            }
-        }
-        // A stage's copies have landed once its MMAs are done: wait for the last
-        // ones, so that none writes into shared memory after the CTA's end.
-        int s = 0;
-        uint32_t ph = 0;
-        for (int i = 0; i < issued; ++i) {
-            if (i >= issued - STAGES) mbar_wait(empty0 + 8 * s, ph);
-            if (++s == STAGES) s = 0, ph ^= 1;
-        }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        int stage = 0, n = 0;
-        uint32_t phase = 0;
-        for (int i = pair; i < walk.items && !aborted(); i += n_pairs) {
-            const Item it = walk.at(p, i);
-            for (int k = it.k0;;) {
-                const int end = LONG ? min(it.k1, k + CHAIN) : it.k1, first = k, b = n & 1;
-                if (!mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1))) give_up(202);
-                if (aborted()) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + b * TN;
-                for (; k < end; ++k) {
-                    if (!mbar_wait(full0 + 8 * stage, phase)) give_up(203);
-                    if (aborted()) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = smem_u32(smem + stage * STAGE_BYTES);
-                    const uint64_t da = smem_desc<A_MN>(at), db = smem_desc<B_MN>(at + OPERAND_BYTES);
-#pragma unroll
-                    for (int kk = 0; kk < BK / 16; ++kk)
-                        mma(d, da + kk * k_step<A_MN>(), db + kk * k_step<B_MN>(), p.idesc, k > first || kk ? 1u : 0u);
-                    mma_commit(empty0 + 8 * stage);
+        if constexpr (LONG) fewer_registers<REGS_FEW>();
+        if (warp == 0) {
+            const bool one = elect();
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            bool fine = true;
+            const uint32_t leader_full = at_leader(full0), ring = smem_u32(smem);
+            for (int i = pair; fine && i < walk.items; i += n_pairs) {
+                const Item it = walk.at(p, i);
+                const int m0 = it.tm * TM + (int)rank * 128, n0 = it.tn * TN + (int)rank * 128;
+                int seg = it.k0 / max(1, walk.kblocks), x = (it.k0 - seg * walk.kblocks) * BK;
+                for (int k = it.k0; k < it.k1; ++k) {
+                    fine = mbar_wait(empty0 + 8 * stage, phase ^ 1);
+                    if (!__all_sync(0xffffffffu, fine)) {
+                        if (one) give_up(201);
+                        fine = false;
+                        break;
+                    }
+                    if (one) {
+                        const uint32_t to = ring + stage * STAGE_BYTES, bar = leader_full + 8 * stage;
+                        const CUtensorMap *ma = (p.sa >> seg) & 1 ? &mapA1 : &mapA0, *mb = (p.sb >> seg) & 1 ? &mapB1 : &mapB0;
+                        if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * STAGE_BYTES);
+                        if (A_MN) {
+                            tma_load(to, ma, bar, m0, x);
+                            tma_load(to + OPERAND_BYTES / 2, ma, bar, m0 + 64, x);
+                        } else {
+                            tma_load(to, ma, bar, x, m0);
+                        }
+                        if (B_MN) {
+                            tma_load(to + OPERAND_BYTES, mb, bar, n0, p.b_row0 + x);
+                            tma_load(to + OPERAND_BYTES + OPERAND_BYTES / 2, mb, bar, n0 + 64, p.b_row0 + x);
+                        } else {
+                            tma_load(to + OPERAND_BYTES, mb, bar, x, p.b_row0 + n0);
+                        }
+                    }
+                    ++issued;
                     if (++stage == STAGES) stage = 0, phase ^= 1;
+                    x += BK;
+                    if (x >= K) x = 0, ++seg;
                 }
-                mma_commit(acc_full0 + 8 * b);
-                ++n;
-                if (k >= it.k1 || aborted()) break;
+            }
+            // A stage's copies have landed once its MMAs are done: wait for the last
+            // ones, so that none writes into shared memory after the CTA's end.
+            stage = issued % STAGES;
+            phase = (uint32_t)(issued / STAGES) & 1;
+            for (int i = 0; i < min(issued, STAGES); ++i) {
+                // (From the oldest of the last STAGES on: its number is issued - STAGES + i.)
+                const int at = issued < STAGES ? i : (stage + i) % STAGES;
+                const uint32_t ph = issued < STAGES ? 0u : (stage + i < STAGES ? phase ^ 1 : phase);
+                mbar_wait(empty0 + 8 * at, ph);
+            }
+        } else if (warp == 1 && rank == 0) {
+            const bool one = elect();
+            int stage = 0, n = 0;
+            uint32_t phase = 0;
+            bool fine = true;
+            const uint64_t da0 = smem_desc<A_MN>(smem_u32(smem)), db0 = smem_desc<B_MN>(smem_u32(smem) + OPERAND_BYTES);
+            for (int i = pair; fine && i < walk.items; i += n_pairs) {
+                const Item it = walk.at(p, i);
+                for (int k = it.k0;;) {
+                    const int end = LONG ? min(it.k1, k + CHAIN) : it.k1, b = n & 1;
+                    fine = mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1));
+                    if (!__all_sync(0xffffffffu, fine)) {
+                        if (one) give_up(202);
+                        fine = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t d = tmem + b * TN;
+                    uint32_t more = 0;
+                    for (; k < end; ++k) {
+                        fine = mbar_wait(full0 + 8 * stage, phase);
+                        if (!__all_sync(0xffffffffu, fine)) {
+                            if (one) give_up(203);
+                            fine = false;
+                            break;
+                        }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (one) {
+                            const uint64_t da = da0 + (uint64_t)(stage * (STAGE_BYTES >> 4)), db = db0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
+#pragma unroll
+                            for (int kk = 0; kk < BK / 16; ++kk)
+                                mma(d, da + kk * k_step<A_MN>(), db + kk * k_step<B_MN>(), p.idesc, kk ? 1u : more);
+                            mma_commit(empty0 + 8 * stage);
+                        }
+                        more = 1;
+                        if (++stage == STAGES) stage = 0, phase ^= 1;
+                    }
+                    if (one) mma_commit(acc_full0 + 8 * b);
+                    ++n;
+                    if (k >= it.k1 || !fine) break;
+                }
             }
         }
-    }
     } else {
         if constexpr (LONG) more_registers<REGS_MANY>();
         const int q = warp & 3, half = (warp - 4) >> 2;
@@ -531,7 +560,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
         int n = 0;
         // The next accumulator: wait for it, or give it back.
         auto take = [&]() -> bool {
-            const bool ok = mbar_wait(acc_full0 + 8 * (n & 1), (uint32_t)((n >> 1) & 1)) && !aborted();
+            const bool ok = mbar_wait(acc_full0 + 8 * (n & 1), (uint32_t)((n >> 1) & 1));
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up(204);
                 return false;
