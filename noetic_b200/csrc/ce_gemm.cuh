@@ -28,15 +28,16 @@ constexpr int TM = 256, TN = 256, BK = 64;  // a pair's tile
 constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * BK * 2;          // a CTA's half of A or B
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
 constexpr int THREADS = 384, EPI_WARPS = 8;
+constexpr int BOX_BYTES = 32 * 64 * 2;  // GRAD: 32 rows and 64 columns of G, on their way out
+constexpr int smem_bytes(bool boxes) { return STAGES * STAGE_BYTES + (boxes ? EPI_WARPS * BOX_BYTES : 0) + 1024 + 256; }
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint64_t WAIT_NS = 1000000000ull;
 // The tensor cores cut, not round, when they add to a sum, so a chain of products
 // is off by half a step of the sum for each 16 of K, all one way (measured: 1.7e-8
 // of a logit each).  Where f32 results depend on it (the loss; f32 gradients), a
 // chain ends after CHAIN K-blocks and the epilogue's registers add the chains up.
-constexpr int CHAIN = 4;
+constexpr int CHAIN = 8;
 constexpr int REGS_FEW = 64, REGS_MANY = 216;  // 4 warps and 8 of 32: within 384 * 168
 
 // What the first kernel of a call finds out, for the others (the workspace's head).
@@ -66,11 +67,9 @@ struct Gemm {
     int64_t part_ld;
     float *zt;
     const uint32_t *target;  // of each row that counts
-    // GRAD: G [row][ldg], and its second part ldg * Mp elements behind
+    // GRAD: G goes out through mapC0, its second part through mapC1
     const float2 *stats;     // of each row that counts
     const float *weight;     // of each row that counts, relative to the largest
-    void *g;
-    int64_t ldg, g_part;
     int col0;                // the piece's first token
     float g_scale;
     // STORE
@@ -174,35 +173,24 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         : "memory");
 }
 
-// 32 columns of this warp's 32 rows; every lane takes part.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    __syncwarp();
+// 32 columns of this warp's 32 rows; every lane takes part.  The values are there
+// after tmem_wait, which has to name them: the compiler knows of no other order.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]),
+          "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
+          "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]),
+          "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    __syncwarp();
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+template <int N>
+__device__ __forceinline__ void tmem_wait(float *v) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
 
 // A tile's piece: its row and column block and its K-blocks.
@@ -241,83 +229,111 @@ struct Walk {
 
 // ---------------------------------------------------------------- epilogues
 // A warp has 32 rows (lane = row) and 128 columns of its CTA's 128 x 256 sums, which
-// come 32 at a time, from TMEM or (LONG) from the registers that added them up.
+// come 64 at a time, from TMEM or (LONG) from the registers that added them up.
 // `row` counts rows that count (or tokens, in dw), `col` is the first column; every
-// lane of a warp calls chunk().
+// lane of a warp calls some().
 
-// The maximum and the sum of exponentials of 128 logits of a row.
+// The maximum and the sum of exponentials of 128 logits of a row.  The sum is kept
+// relative to a whole power of two near the first maximum: an exponential is then one
+// fma and one ex2, and 2^100 of room means that the power hardly ever moves.
 template <bool SCALED>
 struct RowsEpilogue {
     const Gemm &p;
     const int row, live, col, slot;
     const uint32_t t;
-    float m = -INFINITY, s = 0.0f;
+    float m = -INFINITY, s = 0.0f, power = -INFINITY;
     __device__ __forceinline__ RowsEpilogue(const Gemm &g, int r, int n, int c, int at)
         : p(g), row(r), live(n), col(c), slot(at), t(r < n ? g.target[r] : NO_TOKEN) {}
-    __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
+    __device__ __forceinline__ void some(int c, float *v) {
         if (col + c >= p.n_valid) return;  // warp-uniform
         if (SCALED) {
             const float xs = *p.x_scale, ws = *p.w_scale;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = v[j] * xs * ws;
+            for (int j = 0; j < 64; ++j) v[j] = v[j] * xs * ws;
         }
-        if (col + c + 32 > p.n_valid)
+        if (col + c + 64 > p.n_valid)
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 64; ++j)
                 if (col + c + j >= p.n_valid) v[j] = -INFINITY;
-        if (t - (uint32_t)(col + c) < 32u)
+        if (t - (uint32_t)(col + c) < 64u)
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 64; ++j)
                 if (t == (uint32_t)(col + c + j)) p.zt[row] = v[j];
-        float top = v[0];
+        float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
-        const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
-        s *= ex2((m - base) * LOG2E);
+        for (int j = 4; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], v[j]);
+        m = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        const float want = m * LOG2E;
+        if (want > power + 60.0f) {
+            const float now = rintf(want);
+            s *= ex2(power - now);  // (s is 0 before the first)
+            power = now;
+        }
+        const float base = power == -INFINITY ? 0.0f : power;
         float a[4] = {};
 #pragma unroll
-        for (int j = 0; j < 32; ++j) a[j & 3] += ex2((v[j] - base) * LOG2E);
+        for (int j = 0; j < 64; ++j) a[j & 3] += ex2(fmaf(v[j], LOG2E, -base));
         s += (a[0] + a[1]) + (a[2] + a[3]);
-        m = now;
     }
-    __device__ __forceinline__ void end() const {
+    __device__ __forceinline__ void end() {
+        // Relative to the maximum from here on (with the same log2(e), whose error so cancels).
+        if (m > -INFINITY) s *= ex2(fmaf(-m, LOG2E, power));
         if (row < live) p.part[(int64_t)slot * p.part_ld + row] = make_float2(m, s);
     }
 };
 
+__device__ __forceinline__ void store_box(const CUtensorMap *map, uint32_t from, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"((uint64_t)map), "r"(from),
+                 "r"(x), "r"(y)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
 // G = weight (exp(z - m - log s) - [t]) of 128 logits of a row; zeros where there
-// is no row or no token, since the products that follow read whole blocks.
+// is no row or no token, since the products that follow read whole blocks.  64
+// columns of the warp's 32 rows go out at once, as a box whose 16-byte places are
+// swizzled by row (a lane writing its own row to memory takes a line for each 16
+// bytes: 6.3 us a tile where the box takes 3.7).
 template <class T, bool SCALED>
 struct GradEpilogue {
     const Gemm &p;
+    const CUtensorMap *const map0, *const map1;
+    uint8_t *const box;
     const bool in;
-    const int col;
+    const int row0, col;
     const uint32_t t;
     const float2 st;
-    const float h;
-    T *const g;
-    __device__ __forceinline__ GradEpilogue(const Gemm &q, int row, int live, int c)
-        : p(q), in(row < live), col(c), t(in ? q.target[row] - (uint32_t)q.col0 : NO_TOKEN),
-          st(in ? q.stats[row] : make_float2(0.0f, 0.0f)), h(in ? q.weight[row] * q.g_scale : 0.0f),
-          g((T *)q.g + (int64_t)row * q.ldg + c) {}
-    __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
-        const float xs = SCALED ? *p.x_scale : 1.0f, ws = SCALED ? *p.w_scale : 1.0f;
-        const bool whole = in && col + c + 32 <= p.n_valid;
+    const float h, base;
+    __device__ __forceinline__ GradEpilogue(const Gemm &q, const CUtensorMap *a, const CUtensorMap *b, uint8_t *to, int row, int live,
+                                            int c)
+        : p(q), map0(a), map1(b), box(to), in(row < live), row0(row - (int)(threadIdx.x & 31)), col(c),
+          t(in ? q.target[row] - (uint32_t)q.col0 : NO_TOKEN), st(in ? q.stats[row] : make_float2(0.0f, 0.0f)),
+          h(in ? q.weight[row] * q.g_scale : 0.0f), base((st.x + st.y) * LOG2E) {}
+    __device__ __forceinline__ void some(int c, float *v) {
+        const int lane = threadIdx.x & 31;
+        if (SCALED) {
+            const float xs = *p.x_scale, ws = *p.w_scale;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            float z = v[j];
-            if (SCALED) z = z * xs * ws;
-            z = ex2(((z - st.x) - st.y) * LOG2E) * h;
-            v[j] = whole || (in && col + c + j < p.n_valid) ? z : 0.0f;
+            for (int j = 0; j < 64; ++j) v[j] = ex2(((v[j] * xs * ws - st.x) - st.y) * LOG2E) * h;
+        } else {
+            // (For 16 bits the fma's error, 2^-24 of the log-sum, is nothing.)
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = ex2(fmaf(v[j], LOG2E, -base)) * h;
         }
-        if (t - (uint32_t)(col + c) < 32u)
+        if (!in || col + c + 64 > p.n_valid)
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 64; ++j)
+                if (!in || col + c + j >= p.n_valid) v[j] = 0.0f;
+        if (t - (uint32_t)(col + c) < 64u)
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
                 if (t == (uint32_t)(col + c + j)) v[j] -= h;
 #pragma unroll
         for (int part = 0; part < (SCALED ? 2 : 1); ++part) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the box is free again
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
+            for (int j = 0; j < 64; j += 8) {
                 uint4 q;
                 T *o = reinterpret_cast<T *>(&q);
 #pragma unroll
@@ -325,20 +341,23 @@ struct GradEpilogue {
                     o[e] = from_f32<T>(v[j + e]);
                     if (SCALED) v[j + e] -= to_f32(o[e]);
                 }
-                *reinterpret_cast<uint4 *>(g + part * p.g_part + c + j) = q;
+                *reinterpret_cast<uint4 *>(box + lane * 128 + (((j >> 3) ^ (lane & 7)) << 4)) = q;
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) store_box(part ? map1 : map0, smem_u32(box), col + c, row0);
         }
     }
     __device__ __forceinline__ void end() const {}
 };
 
 template <class T>
-__device__ __forceinline__ void store_out(const Gemm &p, const float (&v)[32], int64_t at, int col) {
+__device__ __forceinline__ void store_out(const Gemm &p, const float *v, int64_t at, int col) {
     T *o = (T *)p.out + at + col;
     constexpr int PER = 16 / sizeof(T);
-    if (col + 32 <= p.n_valid && ((uintptr_t)o & 15) == 0) {
+    if (col + 64 <= p.n_valid && ((uintptr_t)o & 15) == 0) {
 #pragma unroll
-        for (int j = 0; j < 32; j += PER) {
+        for (int j = 0; j < 64; j += PER) {
             uint4 q;
             T *e = reinterpret_cast<T *>(&q);
             if (p.out_add) q = *reinterpret_cast<const uint4 *>(o + j);
@@ -348,7 +367,7 @@ __device__ __forceinline__ void store_out(const Gemm &p, const float (&v)[32], i
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 64; ++j)
             if (col + j < p.n_valid) o[j] = from_f32<T>(p.out_add ? v[j] + to_f32(o[j]) : v[j]);
     }
 }
@@ -364,32 +383,32 @@ __device__ __forceinline__ float out_factor(const Gemm &p) {
 template <bool F32>
 struct StoreEpilogue {
     const Gemm &p;
-    const bool some;  // K has anything: else the accumulator holds nothing
+    const bool any;  // K has anything: else the accumulator holds nothing
     const int row, rows, col;
     const float factor;
     float *const acc;
-    __device__ __forceinline__ StoreEpilogue(const Gemm &g, bool any, int r, int n, int c, int split, float f)
-        : p(g), some(any), row(r), rows(n), col(c), factor(f),
+    __device__ __forceinline__ StoreEpilogue(const Gemm &g, bool has, int r, int n, int c, int split, float f)
+        : p(g), any(has), row(r), rows(n), col(c), factor(f),
           acc(g.acc ? g.acc + (int64_t)split * g.acc_split + (int64_t)r * g.ld_acc + c : nullptr) {}
-    __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
+    __device__ __forceinline__ void some(int c, float *v) {
         if (col + c >= p.n_valid || row >= rows) return;
-        if (!some)
+        if (!any)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+            for (int j = 0; j < 64; ++j) v[j] = 0.0f;
         float *a = acc + c;
         if (p.add)
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
+            for (int j = 0; j < 64; j += 4) {
                 const float4 q = *reinterpret_cast<const float4 *>(a + j);
                 v[j] += q.x, v[j + 1] += q.y, v[j + 2] += q.z, v[j + 3] += q.w;
             }
         if (p.keep) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(a + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4 *>(a + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             return;
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= factor;
+        for (int j = 0; j < 64; ++j) v[j] *= factor;
         const int64_t at = (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld;
         if (F32 || p.out_dtype == 0)
             store_out<float>(p, v, at, col + c);
@@ -416,10 +435,12 @@ __device__ __forceinline__ void fewer_registers() {
 template <int MODE, class T, bool SCALED, bool LONG, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
-       const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ Gemm p) {
+       const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1,
+       const __grid_constant__ CUtensorMap mapC0, const __grid_constant__ CUtensorMap mapC1, const __grid_constant__ Gemm p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = (uint64_t *)(smem + STAGES * STAGE_BYTES);
+    uint8_t *boxes = smem + STAGES * STAGE_BYTES;
+    uint64_t *bars = (uint64_t *)(boxes + (MODE == GRAD ? EPI_WARPS * BOX_BYTES : 0));
     uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -561,7 +582,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
         // The next accumulator: wait for it, or give it back.
         auto take = [&]() -> bool {
             const bool ok = mbar_wait(acc_full0 + 8 * (n & 1), (uint32_t)((n >> 1) & 1));
-            if (!__all_sync(0xffffffffu, ok)) {
+            if (!__all_sync(0xffffffffu, ok)) {  // (every lane is here: the loads that follow are the warp's)
                 if (lane == 0) give_up(204);
                 return false;
             }
@@ -583,35 +604,41 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             const int row = it.tm * TM + (int)rank * 128 + q * 32 + lane, col = it.tn * TN + half * 128;
             auto whole = [&](auto &&e) {
                 if constexpr (LONG) {
-                    float sum[4][32];
+                    float sum[128];
                     fine = take();
                     if (!fine) return;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(mine + (n & 1) * TN + c * 32, sum[c]);
+                    for (int c = 0; c < 128; c += 32) tmem_ld32(mine + (n & 1) * TN + c, sum + c);
+                    tmem_wait<128>(sum);
                     give();
 #pragma unroll 1
                     for (int k = it.k0 + CHAIN; k < it.k1; k += CHAIN) {
                         fine = take();
                         if (!fine) return;
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            float v[16];
-                            tmem_ld16(mine + (n & 1) * TN + c * 16, v);
+                        for (int c = 0; c < 128; c += 64) {
+                            float v[64];
+                            tmem_ld32(mine + (n & 1) * TN + c, v);
+                            tmem_ld32(mine + (n & 1) * TN + c + 32, v + 32);
+                            tmem_wait<64>(v);
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) sum[c / 2][c % 2 * 16 + j] += v[j];
+                            for (int j = 0; j < 64; ++j) sum[c + j] += v[j];
                         }
                         give();
                     }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) e.chunk(c * 32, sum[c]);
+                    e.some(0, sum);
+                    e.some(64, sum + 64);
                 } else {
                     fine = take();
                     if (!fine) return;
 #pragma unroll 1
-                    for (int c = 0; c < 128; c += 32) {
-                        float v[32];
+                    for (int c = 0; c < 128; c += 64) {
+                        float v[64];
+                        __syncwarp();
                         tmem_ld32(mine + (n & 1) * TN + c, v);
-                        e.chunk(c, v);
+                        tmem_ld32(mine + (n & 1) * TN + c + 32, v + 32);
+                        tmem_wait<64>(v);
+                        e.some(c, v);
                     }
                     give();
                 }
@@ -620,10 +647,11 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             if constexpr (MODE == ROWS)
                 whole(RowsEpilogue<SCALED>(p, row, live, col, 2 * it.tn + half));
             else if constexpr (MODE == GRAD)
-                whole(GradEpilogue<T, SCALED>(p, row, live, col));
+                whole(GradEpilogue<T, SCALED>(p, &mapC0, &mapC1, boxes + (warp - 4) * BOX_BYTES, row, live, col));
             else
                 whole(StoreEpilogue<SCALED>(p, it.k1 > it.k0, row, M, col, it.split, factor));
         }
+        if (MODE == GRAD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();

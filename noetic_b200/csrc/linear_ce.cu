@@ -372,17 +372,18 @@ uint32_t instruction(bool bf16, bool a_mn, bool b_mn) {
 }
 
 struct Maps {
-    CUtensorMap a[2], b[2];
+    CUtensorMap a[2], b[2], c[2];
 };
 
 template <int MODE, class T, bool SCALED, bool LONG, bool A_MN, bool B_MN>
 cudaError_t launch(const Maps &m, const Gemm &g, int sms, cudaStream_t st) {
     auto *k = ce::gemm_k<MODE, T, SCALED, LONG, A_MN, B_MN>;
-    cudaError_t e = allow_shared(k, ce::SMEM_BYTES);
+    constexpr int shared = ce::smem_bytes(MODE == ce::GRAD);
+    cudaError_t e = allow_shared(k, shared);
     if (e != cudaSuccess) return e;
     const int64_t items = (int64_t)((g.M + ce::TM - 1) / ce::TM) * ((g.N + ce::TN - 1) / ce::TN) * g.splits;
     const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(sms / 2, items));
-    k<<<2 * pairs, ce::THREADS, ce::SMEM_BYTES, st>>>(m.a[0], m.a[1], m.b[0], m.b[1], g);
+    k<<<2 * pairs, ce::THREADS, shared, st>>>(m.a[0], m.a[1], m.b[0], m.b[1], m.c[0], m.c[1], g);
     return cudaGetLastError();
 }
 
@@ -477,7 +478,7 @@ struct Call {
     cudaError_t forward() {
         cudaError_t e = begin(false);
         if (e != cudaSuccess) return e;
-        Maps m;
+        Maps m{};
         if (!map_x(m.a, 128) || !map_w(m.b, 128)) return cudaErrorInvalidValue;
         Gemm g = gemm((int)a.rows, a.vocab, a.width, 0, false, false, 1);
         g.m_fast = 1;
@@ -502,8 +503,8 @@ struct Call {
     cudaError_t backward() {
         cudaError_t e = begin(true);
         if (e != cudaSuccess) return e;
-        Maps mg, mx, mw;
-        if (!map_x(mg.a, 128) || !map_w(mg.b, 128) || !map_g(mx.a, 128) || !map_w(mx.b, 64) || !map_g(mw.a, 64) || !map_x(mw.b, 64))
+        Maps mg{}, mx{}, mw{};
+        if (!map_x(mg.a, 128) || !map_w(mg.b, 128) || !map_g(mg.c, 32) || !map_g(mx.a, 128) || !map_w(mx.b, 64) || !map_g(mw.a, 64) || !map_x(mw.b, 64))
             return cudaErrorInvalidValue;
         const float g_scale = BF16 ? 1.0f : G_SCALE;
         for (int v0 = 0; v0 < a.vocab; v0 += p.piece) {
@@ -516,9 +517,6 @@ struct Call {
             g.target = ix.target;
             g.stats = ix.stats;
             g.weight = ix.weight;
-            g.g = at<P>(p.g);
-            g.ldg = p.ldg;
-            g.g_part = p.mp * p.ldg;
             g.col0 = v0;
             g.g_scale = g_scale;
             if (a.rows) e = launch<ce::GRAD, P, SPLIT, SPLIT, false, false>(mg, g, sms, st);
