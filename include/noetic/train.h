@@ -105,11 +105,11 @@ void nk_adamw_many_free(nk_adamw_many *many);
  * grad c:  c = grad_scale, or, where max_norm > 0 and the norm of all grad_scale
  * grad is larger, grad_scale max_norm / norm.  With f32 gradients and moments
  * and c = 1 a tensor's result is nk_adamw_step's, bit for bit.  cfg->decay is not
- * read (each tensor has its own).  8-bit moments are read, stepped in f32, used
- * for this step's val, and rounded to nearest afterwards with a new scale for
+ * read (each tensor has its own).  8-bit moments are read, stepped in f32 (with
+ * a few roundings of 2^-23), used for this step's val, and rounded to nearest afterwards with a new scale for
  * the block; a v above 0 does not become 0, and |m| is kept up to 2^100.
  * norm (nullable, device): receives the norm.  bad (nullable, device): becomes 1
- * where an element's gradient or value is not finite; that element's val and
+ * where an element's g or value is not finite; that element's val and
  * moments stay (8-bit moments: as far as the block's new scale holds them).
  * A norm that is not finite, with max_norm > 0: nothing changes, bad becomes 1.
  * A captured call repeats its cfg, grad_scale and max_norm in each replay. */

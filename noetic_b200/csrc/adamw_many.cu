@@ -24,7 +24,7 @@ constexpr float E4M3_TINY = 0.001953125f;  // 2^-9, the smallest number above 0
 // Blocks whose largest value is below this are stored as zeros: 448 / value
 // would leave f32's range (values like that come of gradients below 1e-30).
 constexpr float SCALE_MIN = 7.8886090522101181e-31f;  // 2^-100
-constexpr float ROOT_MAX = 1.8446742974197924e19f;    // the root of f32's largest value
+constexpr float V_MAX = 3e38f;
 constexpr float MOMENT_MAX = 1.2676506002282294e30f;  // 2^100: m / (1 - b1^t) stays in range
 
 // Four gradients from element 4 i on.
@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(256) adamw_norm_k(AdamwMany p, float grad_scal
 // element stays as it is.
 __device__ __forceinline__ bool adamw_element(float &val, float grad, float c, float &m, float &v, const AdamwParams &a,
                                               bool decay) {
-    if (!isfinite(grad) || !isfinite(val)) return false;
     const float g = __fmul_rn(grad, c);
+    if (!isfinite(g) || !isfinite(val)) return false;
     m = __fadd_rn(__fmul_rn(a.b1, m), __fmul_rn(__fsub_rn(1.0f, a.b1), g));
     v = __fadd_rn(__fmul_rn(a.b2, v), __fmul_rn(__fmul_rn(__fsub_rn(1.0f, a.b2), g), g));
     const float mh = __fmul_rn(m, a.inv_bc1), vh = __fmul_rn(v, a.inv_bc2);
@@ -191,10 +191,14 @@ __device__ __forceinline__ bool chunk_step32(const nk_adamw_tensor &t, const Ada
     return ok;
 }
 
-__device__ __forceinline__ float from_e4m3(uint8_t b) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
+// Two e4m3 numbers, exactly.
+__device__ __forceinline__ float2 from_e4m3(uint32_t two) {
+    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
 }
-__device__ __forceinline__ uint8_t to_e4m3(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+// To nearest, ties to even.
+__device__ __forceinline__ uint32_t to_e4m3(float lo, float hi) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -202,18 +206,41 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+__device__ __forceinline__ float rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rsqrt_fast(float x) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// What a block's steps need of the call, worked out once a thread.
+struct Step8 {
+    float c, b1, g1, b2, g2, inv_bc1, root_bc2, eps, lr, wd;
+    __device__ __forceinline__ Step8(const AdamwParams &a, float factor)
+        : c(factor), b1(a.b1), g1((1.0f - a.b1) * factor), b2(a.b2), g2(1.0f - a.b2), inv_bc1(a.inv_bc1),
+          root_bc2(sqrtf(a.inv_bc2)), eps(a.eps), lr(a.lr), wd(a.wd) {}
+};
+
 // A warp steps one block of up to 256 elements: lane l holds elements 4 l .. + 3
 // and 128 + 4 l .. + 3, so the block's largest |m| and sqrt(v) are two shuffles'
-// reductions and nothing is read twice.
+// reductions and nothing is read twice.  Correctly rounded roots and quotients, as
+// the 32-bit step has them, took 116 instructions an element and 2.4 TB/s; here one
+// root (a reciprocal root and Newton's step, within 2^-23) serves the update and the
+// moment, and the quotient is a product with a reciprocal: 2^-22 of an update, which
+// is below the rounding of val.
 template <class G>
-__device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t first, uint32_t n, const AdamwParams &a,
-                                            float c, bool decay, bool vec) {
+__device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t first, uint32_t n, const Step8 &a, float wd,
+                                            bool vec) {
     const int lane = threadIdx.x & 31;
     float *val = t.val + first;
     uint8_t *m = (uint8_t *)t.m + first, *v = (uint8_t *)t.v + first;
     const G *grad = (const G *)t.grad + first;
     const float ms = t.m_scale[first / NK_ADAMW_BLOCK], vs = t.v_scale[first / NK_ADAMW_BLOCK];
-    float pv[2][4], g[2][4], mv[2][4], rv[2][4];
+    float pv[2][4], g[2][4], rv[2][4];
     uint32_t mb[2], vb[2];
     vec &= n == NK_ADAMW_BLOCK;
 #pragma unroll
@@ -239,34 +266,49 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
     }
     bool ok = true;
     float top_m = 0.0f, top_r = 0.0f;
+    const float k1 = a.b1 * ms;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float mm = __fmul_rn(from_e4m3((uint8_t)(mb[h] >> (8 * e))), ms);
-            const float r = __fmul_rn(from_e4m3((uint8_t)(vb[h] >> (8 * e))), vs);
-            float vv = __fmul_rn(r, r);
-            ok &= adamw_element(pv[h][e], g[h][e], c, mm, vv, a, decay);
-            mv[h][e] = fminf(fmaxf(mm, -MOMENT_MAX), MOMENT_MAX);
-            rv[h][e] = fminf(__fsqrt_rn(vv), ROOT_MAX);
-            top_m = fmaxf(top_m, fabsf(mv[h][e]));
+            const float2 mc = from_e4m3(e < 2 ? mb[h] & 0xFFFFu : mb[h] >> 16), vc = from_e4m3(e < 2 ? vb[h] & 0xFFFFu : vb[h] >> 16);
+            const float mq = e & 1 ? mc.y : mc.x, r = (e & 1 ? vc.y : vc.x) * vs;
+            const float gc = g[h][e] * a.c;
+            const bool fine = fabsf(gc) < INFINITY && fabsf(pv[h][e]) < INFINITY;
+            ok &= fine;
+            float mm = fmaf(mq, k1, g[h][e] * a.g1);
+            const float v1 = fmaf(a.b2 * r, r, (a.g2 * gc) * gc), vv = fminf(v1, V_MAX);
+            // sqrt(vv); below 2^-126 (a gradient below 1e-18) it counts as 0.
+            const float q = rsqrt_fast(vv);
+            float u = vv * q;
+            u = fmaf(fmaf(-u, u, vv) * 0.5f, q, u);
+            u = vv < 1.1754944e-38f ? 0.0f : u;
+            // (A v beyond f32's range divides to 0.)
+            const float inv = v1 > V_MAX ? 0.0f : rcp(fmaxf(fmaf(u, a.root_bc2, a.eps), 1.1754944e-38f));
+            const float upd = fmaf(mm * a.inv_bc1, inv, wd * pv[h][e]);
+            pv[h][e] = fine ? fmaf(-a.lr, upd, pv[h][e]) : pv[h][e];
+            mm = fminf(fmaxf(mm, -MOMENT_MAX), MOMENT_MAX);
+            g[h][e] = fine ? mm : mq * ms;  // the new m
+            rv[h][e] = fine ? u : r;
+            top_m = fmaxf(top_m, fabsf(g[h][e]));
             top_r = fmaxf(top_r, rv[h][e]);
         }
     top_m = warp_max(top_m);
     top_r = warp_max(top_r);
-    const float km = top_m >= SCALE_MIN ? __fdiv_rn(E4M3_MAX, top_m) : 0.0f;
-    const float kr = top_r >= SCALE_MIN ? __fdiv_rn(E4M3_MAX, top_r) : 0.0f;
+    const float km = top_m >= SCALE_MIN ? __fdividef(E4M3_MAX, top_m) : 0.0f;
+    const float kr = top_r >= SCALE_MIN ? __fdividef(E4M3_MAX, top_r) : 0.0f;
+    // A root above 0 stays above 0: a later step divides by it.
+    const float least = kr > 0.0f ? E4M3_TINY : 0.0f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const uint32_t at = h * 128 + lane * 4;
-        uint32_t mo = 0, vo = 0;
+        float y[4], z[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float y = __fmul_rn(rv[h][e], kr);
-            mo |= (uint32_t)to_e4m3(__fmul_rn(mv[h][e], km)) << (8 * e);
-            // A root above 0 stays above 0: a later step divides by it.
-            vo |= (uint32_t)to_e4m3(rv[h][e] > 0.0f && kr > 0.0f ? fmaxf(y, E4M3_TINY) : 0.0f) << (8 * e);
+            y[e] = g[h][e] * km;
+            z[e] = rv[h][e] > 0.0f ? fmaxf(rv[h][e] * kr, least) : 0.0f;
         }
+        const uint32_t mo = to_e4m3(y[0], y[1]) | to_e4m3(y[2], y[3]) << 16, vo = to_e4m3(z[0], z[1]) | to_e4m3(z[2], z[3]) << 16;
         if (vec) {
             __stcs(reinterpret_cast<float4 *>(val + at), make_float4(pv[h][0], pv[h][1], pv[h][2], pv[h][3]));
             __stcs(reinterpret_cast<uint32_t *>(m + at), mo);
@@ -284,32 +326,33 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
         }
     }
     if (lane == 0) {
-        // (The scale of what was stored: 1 / k up to rounding, 0 for zeros.)
-        t.m_scale[first / NK_ADAMW_BLOCK] = km > 0.0f ? __fdiv_rn(top_m, E4M3_MAX) : 0.0f;
-        t.v_scale[first / NK_ADAMW_BLOCK] = kr > 0.0f ? __fdiv_rn(top_r, E4M3_MAX) : 0.0f;
+        // (The scale of what was stored, 0 for zeros.)
+        t.m_scale[first / NK_ADAMW_BLOCK] = km > 0.0f ? top_m * (1.0f / E4M3_MAX) : 0.0f;
+        t.v_scale[first / NK_ADAMW_BLOCK] = kr > 0.0f ? top_r * (1.0f / E4M3_MAX) : 0.0f;
     }
     return ok;
 }
 
 template <class G>
-__device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const AdamwChunk &ch, const AdamwParams &a,
-                                            float c, bool decay) {
+__device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const AdamwChunk &ch, const Step8 &a, bool decay) {
     const bool vec = aligned(t.val, 16) && aligned(t.m, 4) && aligned(t.v, 4) && aligned(t.grad, 4 * sizeof(G)) &&
                      (!t.copy || aligned(t.copy, 8));
+    const float wd = decay ? a.wd : 0.0f;
     bool ok = true;
     for (uint32_t b = (threadIdx.x >> 5) * NK_ADAMW_BLOCK; b < ch.n; b += (blockDim.x >> 5) * NK_ADAMW_BLOCK)
-        ok &= block_step8<G>(t, ch.first + b, min(ch.n - b, (uint32_t)NK_ADAMW_BLOCK), a, c, decay, vec);
+        ok &= block_step8<G>(t, ch.first + b, min(ch.n - b, (uint32_t)NK_ADAMW_BLOCK), a, wd, vec);
     return ok;
 }
 
 template <int BITS>
-__global__ void __launch_bounds__(256) adamw_many_k(AdamwMany p, uint32_t from, uint32_t to, AdamwParams a,
+__global__ void __launch_bounds__(256, BITS == 8 ? 4 : 6) adamw_many_k(AdamwMany p, uint32_t from, uint32_t to, AdamwParams a,
                                                     float grad_scale, bool with_clip, uint32_t *bad) {
     float c = grad_scale;
     if (with_clip) {
         if (p.clip[1] == 0.0f) return;
         c = p.clip[0];
     }
+    const Step8 a8(a, c);
     bool ok = true;
     for (uint32_t i = from + blockIdx.x; i < to; i += gridDim.x) {
         const AdamwChunk ch = p.chunks[i];
@@ -320,9 +363,9 @@ __global__ void __launch_bounds__(256) adamw_many_k(AdamwMany p, uint32_t from, 
                   : t.grad_dtype == NK_F16 ? chunk_step32<__half>(t, ch, a, c, decay)
                                            : chunk_step32<__nv_bfloat16>(t, ch, a, c, decay);
         } else {
-            ok &= t.grad_dtype == NK_F32   ? chunk_step8<float>(t, ch, a, c, decay)
-                  : t.grad_dtype == NK_F16 ? chunk_step8<__half>(t, ch, a, c, decay)
-                                           : chunk_step8<__nv_bfloat16>(t, ch, a, c, decay);
+            ok &= t.grad_dtype == NK_F32   ? chunk_step8<float>(t, ch, a8, decay)
+                  : t.grad_dtype == NK_F16 ? chunk_step8<__half>(t, ch, a8, decay)
+                                           : chunk_step8<__nv_bfloat16>(t, ch, a8, decay);
         }
     }
     if (!ok && bad) *bad = 1u;
