@@ -42,20 +42,32 @@ __device__ __forceinline__ void load4(const G *p, float (&g)[4]) {
 }
 
 // ---------------------------------------------------------------- norm
+// (Four vectors of 16 bytes to a thread at once: with 8 bytes the pass was at 2.4 TB/s.)
 template <class G>
 __device__ __forceinline__ double chunk_squares(const G *grad, uint32_t n, bool vec) {
+    constexpr uint32_t PER = 16 / sizeof(G);
     double s = 0.0;
-    uint32_t done = 0;
-    if (vec) {
-        done = n & ~3u;
-        for (uint32_t i = threadIdx.x * 4; i < done; i += blockDim.x * 4) {
-            float g[4];
-            load4(grad + i, g);
-            // (A group of four in f32, the groups in 64 bits.)
-            s += (double)(fmaf(g[0], g[0], g[1] * g[1]) + fmaf(g[2], g[2], g[3] * g[3]));
+    const uint32_t vectors = vec ? n / PER : 0;
+    const uint4 *p = reinterpret_cast<const uint4 *>(grad);
+    for (uint32_t i = threadIdx.x; i < vectors; i += 4 * blockDim.x) {
+        uint4 q[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) q[u] = i + u * blockDim.x < vectors ? __ldcs(p + i + u * blockDim.x) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            // (A vector in f32, the vectors in 64 bits.)
+            const G *g = reinterpret_cast<const G *>(&q[u]);
+            float a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (uint32_t e = 0; e < PER; e += 2) {
+                const float x = to_f32(g[e]), y = to_f32(g[e + 1]);
+                a = fmaf(x, x, a);
+                b = fmaf(y, y, b);
+            }
+            s += (double)(a + b);
         }
     }
-    for (uint32_t i = done + threadIdx.x; i < n; i += blockDim.x) {
+    for (uint32_t i = vectors * PER + threadIdx.x; i < n; i += blockDim.x) {
         const float g = to_f32(grad[i]);
         s += (double)(g * g);
     }
@@ -73,12 +85,14 @@ __device__ __forceinline__ double block_sum_d(double v, double *red) {
 
 __device__ __forceinline__ bool aligned(const void *p, uint32_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-// Each chunk's sum of squares to its own place; the block that finishes last
-// adds them in a fixed order, so the norm does not depend on scheduling.
+// Each block's sum of squares, of the chunks that its number gives it, to its own
+// place; the block that finishes last adds them in a fixed order, so the norm does
+// not depend on scheduling.
 __global__ void __launch_bounds__(256) adamw_norm_k(AdamwMany p, float grad_scale, float max_norm, float *norm,
                                                     uint32_t *bad) {
     __shared__ double red[32];
     __shared__ bool last;
+    double sum = 0.0;
     for (uint32_t c = blockIdx.x; c < p.n_chunks; c += gridDim.x) {
         const AdamwChunk ch = p.chunks[c];
         const nk_adamw_tensor &t = p.tensors[ch.tensor];
@@ -88,15 +102,16 @@ __global__ void __launch_bounds__(256) adamw_norm_k(AdamwMany p, float grad_scal
             s = chunk_squares(g, ch.n, aligned(g, 16));
         } else if (t.grad_dtype == NK_F16) {
             const __half *g = (const __half *)t.grad + ch.first;
-            s = chunk_squares(g, ch.n, aligned(g, 8));
+            s = chunk_squares(g, ch.n, aligned(g, 16));
         } else {
             const __nv_bfloat16 *g = (const __nv_bfloat16 *)t.grad + ch.first;
-            s = chunk_squares(g, ch.n, aligned(g, 8));
+            s = chunk_squares(g, ch.n, aligned(g, 16));
         }
-        s = block_sum_d(s, red);
-        if (threadIdx.x == 0) p.partial[c] = s;
+        sum += s;
     }
+    sum = block_sum_d(sum, red);
     if (threadIdx.x == 0) {
+        p.partial[blockIdx.x] = sum;
         __threadfence();
         last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
     }
@@ -104,7 +119,7 @@ __global__ void __launch_bounds__(256) adamw_norm_k(AdamwMany p, float grad_scal
     if (!last) return;
     __threadfence();
     double s = 0.0;
-    for (uint32_t c = threadIdx.x; c < p.n_chunks; c += blockDim.x) s += __ldcg(p.partial + c);
+    for (uint32_t c = threadIdx.x; c < gridDim.x; c += blockDim.x) s += __ldcg(p.partial + c);
     s = block_sum_d(s, red);
     if (threadIdx.x == 0) {
         const float all = (float)(sqrt(s) * fabs((double)grad_scale));
@@ -217,13 +232,38 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
     return r;
 }
 
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // What a block's steps need of the call, worked out once a thread.
 struct Step8 {
     float c, b1, g1, b2, g2, inv_bc1, root_bc2, eps, lr, wd;
     __device__ __forceinline__ Step8(const AdamwParams &a, float factor)
         : c(factor), b1(a.b1), g1((1.0f - a.b1) * factor), b2(a.b2), g2(1.0f - a.b2), inv_bc1(a.inv_bc1),
-          root_bc2(sqrtf(a.inv_bc2)), eps(a.eps), lr(a.lr), wd(a.wd) {}
+          root_bc2(sqrtf(a.inv_bc2)), eps(fmaxf(a.eps, 1.1754944e-38f)), lr(a.lr), wd(a.wd) {}
 };
+
+// A block of 256 elements on its way to a warp: copies into shared memory that
+// need no registers, so that each warp has STAGES8 - 1 blocks (2.5 KB each) in flight
+// while it works on one.  (With loads into registers instead the kernel waited for
+// memory 60% of its time: 88 us of 19M elements where this takes 64.)
+constexpr int STAGES8 = 3, WARPS8 = 8;
+struct __align__(16) Stage8 {
+    float val[NK_ADAMW_BLOCK];
+    uint32_t grad[NK_ADAMW_BLOCK];  // up to 4 bytes an element
+    uint32_t m[NK_ADAMW_BLOCK / 4], v[NK_ADAMW_BLOCK / 4];
+    float scale[4];  // of m and of v
+};
+
+__device__ __forceinline__ void copy16(void *to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(void *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
+__device__ __forceinline__ float grad_of(const void *grad, int dtype, uint64_t i) {
+    return dtype == NK_F32 ? ((const float *)grad)[i] : dtype == NK_F16 ? to_f32(((const __half *)grad)[i]) : to_f32(((const __nv_bfloat16 *)grad)[i]);
+}
 
 // A warp steps one block of up to 256 elements: lane l holds elements 4 l .. + 3
 // and 128 + 4 l .. + 3, so the block's largest |m| and sqrt(v) are two shuffles'
@@ -232,36 +272,30 @@ struct Step8 {
 // root (a reciprocal root and Newton's step, within 2^-23) serves the update and the
 // moment, and the quotient is a product with a reciprocal: 2^-22 of an update, which
 // is below the rounding of val.
-template <class G>
-__device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t first, uint32_t n, const Step8 &a, float wd,
-                                            bool vec) {
+//
+// The careful form: short blocks, tensors that start off 16 bytes, elements that are
+// not finite or beyond the range of what is stored.
+__device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t first, uint32_t n, AdamwParams params, float factor) {
     const int lane = threadIdx.x & 31;
+    const nk_adamw_tensor &t = *tp;
+    const Step8 a(params, factor);
+    const float wd = t.decay ? a.wd : 0.0f;
     float *val = t.val + first;
     uint8_t *m = (uint8_t *)t.m + first, *v = (uint8_t *)t.v + first;
-    const G *grad = (const G *)t.grad + first;
-    const float ms = t.m_scale[first / NK_ADAMW_BLOCK], vs = t.v_scale[first / NK_ADAMW_BLOCK];
-    float pv[2][4], g[2][4], rv[2][4];
+    float ms, vs, pv[2][4], g[2][4], rv[2][4];
     uint32_t mb[2], vb[2];
-    vec &= n == NK_ADAMW_BLOCK;
+    ms = t.m_scale[first / NK_ADAMW_BLOCK], vs = t.v_scale[first / NK_ADAMW_BLOCK];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const uint32_t at = h * 128 + lane * 4;
-        if (vec) {
-            const float4 q = __ldcs(reinterpret_cast<const float4 *>(val + at));
-            pv[h][0] = q.x, pv[h][1] = q.y, pv[h][2] = q.z, pv[h][3] = q.w;
-            load4(grad + at, g[h]);
-            mb[h] = __ldcs(reinterpret_cast<const uint32_t *>(m + at));
-            vb[h] = __ldcs(reinterpret_cast<const uint32_t *>(v + at));
-        } else {
-            mb[h] = vb[h] = 0;
+        mb[h] = vb[h] = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool in = at + e < n;
-                pv[h][e] = in ? val[at + e] : 0.0f;
-                g[h][e] = in ? to_f32(grad[at + e]) : 0.0f;
-                mb[h] |= in ? (uint32_t)m[at + e] << (8 * e) : 0u;
-                vb[h] |= in ? (uint32_t)v[at + e] << (8 * e) : 0u;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const bool in = at + e < n;
+            pv[h][e] = in ? val[at + e] : 0.0f;
+            g[h][e] = in ? grad_of(t.grad, t.grad_dtype, first + at + e) : 0.0f;
+            mb[h] |= in ? (uint32_t)m[at + e] << (8 * e) : 0u;
+            vb[h] |= in ? (uint32_t)v[at + e] << (8 * e) : 0u;
         }
     }
     bool ok = true;
@@ -284,7 +318,7 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
             u = fmaf(fmaf(-u, u, vv) * 0.5f, q, u);
             u = vv < 1.1754944e-38f ? 0.0f : u;
             // (A v beyond f32's range divides to 0.)
-            const float inv = v1 > V_MAX ? 0.0f : rcp(fmaxf(fmaf(u, a.root_bc2, a.eps), 1.1754944e-38f));
+            const float inv = v1 > V_MAX ? 0.0f : rcp(fmaf(u, a.root_bc2, a.eps));
             const float upd = fmaf(mm * a.inv_bc1, inv, wd * pv[h][e]);
             pv[h][e] = fine ? fmaf(-a.lr, upd, pv[h][e]) : pv[h][e];
             mm = fminf(fmaxf(mm, -MOMENT_MAX), MOMENT_MAX);
@@ -309,21 +343,14 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
             z[e] = rv[h][e] > 0.0f ? fmaxf(rv[h][e] * kr, least) : 0.0f;
         }
         const uint32_t mo = to_e4m3(y[0], y[1]) | to_e4m3(y[2], y[3]) << 16, vo = to_e4m3(z[0], z[1]) | to_e4m3(z[2], z[3]) << 16;
-        if (vec) {
-            __stcs(reinterpret_cast<float4 *>(val + at), make_float4(pv[h][0], pv[h][1], pv[h][2], pv[h][3]));
-            __stcs(reinterpret_cast<uint32_t *>(m + at), mo);
-            __stcs(reinterpret_cast<uint32_t *>(v + at), vo);
-            if (t.copy) store_copy4(t.copy, t.copy_dtype, first + at, pv[h]);
-        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (at + e < n) {
-                    val[at + e] = pv[h][e];
-                    m[at + e] = (uint8_t)(mo >> (8 * e));
-                    v[at + e] = (uint8_t)(vo >> (8 * e));
-                    if (t.copy) store_copy(t.copy, t.copy_dtype, first + at + e, pv[h][e]);
-                }
-        }
+        for (int e = 0; e < 4; ++e)
+            if (at + e < n) {
+                val[at + e] = pv[h][e];
+                m[at + e] = (uint8_t)(mo >> (8 * e));
+                v[at + e] = (uint8_t)(vo >> (8 * e));
+                if (t.copy) store_copy(t.copy, t.copy_dtype, first + at + e, pv[h][e]);
+            }
     }
     if (lane == 0) {
         // (The scale of what was stored, 0 for zeros.)
@@ -333,64 +360,220 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
     return ok;
 }
 
+// The same for a whole block in shared memory, two elements to an instruction.  What
+// is not finite, or out of range, shows in a sum of products with 0 and in the largest
+// moment; such a block, of which nothing is stored yet, goes to the careful form.
 template <class G>
-__device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const AdamwChunk &ch, const Step8 &a, bool decay) {
-    const bool vec = aligned(t.val, 16) && aligned(t.m, 4) && aligned(t.v, 4) && aligned(t.grad, 4 * sizeof(G)) &&
-                     (!t.copy || aligned(t.copy, 8));
-    const float wd = decay ? a.wd : 0.0f;
+__device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t first, const Stage8 &st, const Step8 &a, const AdamwParams &params,
+                                            float wd) {
+    const int lane = threadIdx.x & 31;
+    const float ms = st.scale[0], vs = st.scale[1];
+    const float2 k1 = both(a.b1 * ms), c = both(a.c), g1 = both(a.g1), b2 = both(-a.b2), g2 = both(-a.g2), zero = both(0.0f);
+    float2 pv[4], mv[4], root[4], strange = zero;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t at = h * 128 + lane * 4;
+        const float4 q = *reinterpret_cast<const float4 *>(&st.val[at]);
+        pv[2 * h] = make_float2(q.x, q.y);
+        pv[2 * h + 1] = make_float2(q.z, q.w);
+        float2 g[2];
+        if constexpr (sizeof(G) == 4) {
+            const float4 k = *reinterpret_cast<const float4 *>(&st.grad[at]);
+            g[0] = make_float2(k.x, k.y);
+            g[1] = make_float2(k.z, k.w);
+        } else {
+            const uint2 k = *reinterpret_cast<const uint2 *>(&st.grad[at / 2]);
+            const G *e = reinterpret_cast<const G *>(&k);
+            g[0] = make_float2(to_f32(e[0]), to_f32(e[1]));
+            g[1] = make_float2(to_f32(e[2]), to_f32(e[3]));
+        }
+        const uint32_t mb = st.m[at / 4], vb = st.v[at / 4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int o = 2 * h + i;
+            const float2 r = mul2(from_e4m3(i ? vb >> 16 : vb & 0xFFFFu), both(vs)), gc = mul2(g[i], c);
+            mv[o] = fma2(from_e4m3(i ? mb >> 16 : mb & 0xFFFFu), k1, mul2(g[i], g1));
+            const float2 nv = fma2(mul2(b2, r), r, mul2(mul2(g2, gc), gc));  // -v'
+            strange = fma2(mv[o], zero, strange);
+            strange = fma2(nv, zero, strange);
+            strange = fma2(pv[o], zero, strange);
+            const float2 s = make_float2(rsqrt_fast(-nv.x), rsqrt_fast(-nv.y));
+            float2 u = mul2(nv, s);  // -sqrt(v')
+            u = fma2(fma2(u, u, nv), mul2(s, both(0.5f)), u);
+            // (0 gave 0 times infinity.)
+            root[o] = make_float2(fmaxf(-u.x, 0.0f), fmaxf(-u.y, 0.0f));
+        }
+    }
+    float top_m = 0.0f, top_r = 0.0f;
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+        top_m = fmaxf(top_m, fmaxf(fabsf(mv[o].x), fabsf(mv[o].y)));
+        top_r = fmaxf(top_r, fmaxf(root[o].x, root[o].y));
+    }
+    top_m = warp_max(top_m);
+    top_r = warp_max(top_r);
+    if (__any_sync(0xffffffffu, !(strange.x + strange.y == 0.0f)) || top_m > MOMENT_MAX)
+        return careful_step8(&t, first, NK_ADAMW_BLOCK, params, a.c);
+    const float km = top_m >= SCALE_MIN ? __fdividef(E4M3_MAX, top_m) : 0.0f;
+    const float kr = top_r >= SCALE_MIN ? __fdividef(E4M3_MAX, top_r) : 0.0f;
+    const float least = kr > 0.0f ? E4M3_TINY : 0.0f;
+    const float2 root_bc2 = both(a.root_bc2), eps = both(a.eps), rate = both(-a.lr * a.inv_bc1), fade = both(-a.lr * wd);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t at = h * 128 + lane * 4;
+        uint32_t mo[2], vo[2];
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int o = 2 * h + i;
+            const float2 den = fma2(root[o], root_bc2, eps);
+            const float2 q = mul2(mv[o], make_float2(rcp(den.x), rcp(den.y)));
+            const float2 now = add2(pv[o], fma2(q, rate, mul2(fade, pv[o])));
+            p[2 * i] = now.x, p[2 * i + 1] = now.y;
+            const float2 y = mul2(mv[o], both(km)), z = mul2(root[o], both(kr)), big = mul2(root[o], both(1e25f));
+            mo[i] = to_e4m3(y.x, y.y);
+            // A root above 0 (then above 1e-19) stays above 0: a later step divides by it.
+            vo[i] = to_e4m3(fminf(fmaxf(z.x, least), big.x), fminf(fmaxf(z.y, least), big.y));
+        }
+        __stcs(reinterpret_cast<float4 *>(t.val + first + at), make_float4(p[0], p[1], p[2], p[3]));
+        __stcs(reinterpret_cast<uint32_t *>((uint8_t *)t.m + first + at), mo[0] | mo[1] << 16);
+        __stcs(reinterpret_cast<uint32_t *>((uint8_t *)t.v + first + at), vo[0] | vo[1] << 16);
+        if (t.copy) store_copy4(t.copy, t.copy_dtype, first + at, p);
+    }
+    if (lane == 0) {
+        // (The scale of what was stored, 0 for zeros.)
+        t.m_scale[first / NK_ADAMW_BLOCK] = km > 0.0f ? top_m * (1.0f / E4M3_MAX) : 0.0f;
+        t.v_scale[first / NK_ADAMW_BLOCK] = kr > 0.0f ? top_r * (1.0f / E4M3_MAX) : 0.0f;
+    }
+    return true;
+}
+
+// The copies of a whole block into a warp's stage.
+template <class G>
+__device__ __forceinline__ void issue8(const nk_adamw_tensor &t, uint64_t e, Stage8 &st) {
+    const int lane = threadIdx.x & 31;
+    copy16(&st.val[lane * 4], t.val + e + lane * 4);
+    copy16(&st.val[128 + lane * 4], t.val + e + 128 + lane * 4);
+    if constexpr (sizeof(G) == 4) {
+        copy16(&st.grad[lane * 4], (const G *)t.grad + e + lane * 4);
+        copy16(&st.grad[128 + lane * 4], (const G *)t.grad + e + 128 + lane * 4);
+    } else {
+        copy16(&st.grad[lane * 4], (const G *)t.grad + e + lane * 8);
+    }
+    if (lane < 16)
+        copy16(&st.m[lane * 4], (const uint8_t *)t.m + e + lane * 16);
+    else
+        copy16(&st.v[lane * 4 - 64], (const uint8_t *)t.v + e + lane * 16 - 256);
+    if (lane < 2) copy4(&st.scale[lane], (lane ? t.v_scale : t.m_scale) + e / NK_ADAMW_BLOCK);
+}
+
+// A warp's chunk, STAGES8 - 1 blocks ahead.
+template <class G>
+__device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const AdamwChunk &ch, const Step8 &a, const AdamwParams &params,
+                                            Stage8 *ring) {
+    const float wd = t.decay ? a.wd : 0.0f;
+    const bool vec = aligned(t.val, 16) && aligned(t.m, 16) && aligned(t.v, 16) && aligned(t.grad, 16) && (!t.copy || aligned(t.copy, 8));
+    const uint32_t whole = vec ? ch.n / NK_ADAMW_BLOCK : 0;
     bool ok = true;
-    for (uint32_t b = (threadIdx.x >> 5) * NK_ADAMW_BLOCK; b < ch.n; b += (blockDim.x >> 5) * NK_ADAMW_BLOCK)
-        ok &= block_step8<G>(t, ch.first + b, min(ch.n - b, (uint32_t)NK_ADAMW_BLOCK), a, wd, vec);
+#pragma unroll
+    for (uint32_t s = 0; s < STAGES8 - 1; ++s) {
+        if (s < whole) issue8<G>(t, ch.first + s * NK_ADAMW_BLOCK, ring[s]);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int from = 0, to = STAGES8 - 1;
+    for (uint32_t b = 0; b < whole; ++b) {
+        if (b + STAGES8 - 1 < whole) issue8<G>(t, ch.first + (b + STAGES8 - 1) * NK_ADAMW_BLOCK, ring[to]);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES8 - 1) : "memory");
+        __syncwarp();  // the other lanes' copies, too
+        ok &= block_step8<G>(t, ch.first + b * NK_ADAMW_BLOCK, ring[from], a, params, wd);
+        __syncwarp();  // (before the next copies into it)
+        from = from + 1 == STAGES8 ? 0 : from + 1;
+        to = to + 1 == STAGES8 ? 0 : to + 1;
+    }
+    for (uint32_t at = whole * NK_ADAMW_BLOCK; at < ch.n; at += NK_ADAMW_BLOCK)
+        ok &= careful_step8(&t, ch.first + at, min(ch.n - at, (uint32_t)NK_ADAMW_BLOCK), params, a.c);
     return ok;
 }
 
-template <int BITS>
-__global__ void __launch_bounds__(256, BITS == 8 ? 4 : 6) adamw_many_k(AdamwMany p, uint32_t from, uint32_t to, AdamwParams a,
-                                                    float grad_scale, bool with_clip, uint32_t *bad) {
+// 32-bit moments: a block of threads takes chunks block, block + blocks, ...
+__global__ void __launch_bounds__(256, 6) adamw32_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad) {
+    float c = grad_scale;
+    if (with_clip) {
+        if (p.clip[1] == 0.0f) return;
+        c = p.clip[0];
+    }
+    bool ok = true;
+    for (uint32_t i = blockIdx.x; i < p.n_chunks32; i += gridDim.x) {
+        const AdamwChunk ch = p.chunks[i];
+        const nk_adamw_tensor t = p.tensors[ch.tensor];
+        const bool decay = t.decay && a.wd != 0.0f;
+        ok &= t.grad_dtype == NK_F32   ? chunk_step32<float>(t, ch, a, c, decay)
+              : t.grad_dtype == NK_F16 ? chunk_step32<__half>(t, ch, a, c, decay)
+                                       : chunk_step32<__nv_bfloat16>(t, ch, a, c, decay);
+    }
+    if (!ok && bad) *bad = 1u;
+}
+
+// 8-bit moments: each warp takes chunks of its own, a ring of blocks ahead.
+__global__ void __launch_bounds__(32 * WARPS8, 3) adamw8_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad) {
+    extern __shared__ Stage8 rings[];
     float c = grad_scale;
     if (with_clip) {
         if (p.clip[1] == 0.0f) return;
         c = p.clip[0];
     }
     const Step8 a8(a, c);
+    Stage8 *ring = rings + (threadIdx.x >> 5) * STAGES8;
     bool ok = true;
-    for (uint32_t i = from + blockIdx.x; i < to; i += gridDim.x) {
-        const AdamwChunk ch = p.chunks[i];
-        const nk_adamw_tensor t = p.tensors[ch.tensor];
-        const bool decay = t.decay && a.wd != 0.0f;
-        if constexpr (BITS == 32) {
-            ok &= t.grad_dtype == NK_F32   ? chunk_step32<float>(t, ch, a, c, decay)
-                  : t.grad_dtype == NK_F16 ? chunk_step32<__half>(t, ch, a, c, decay)
-                                           : chunk_step32<__nv_bfloat16>(t, ch, a, c, decay);
-        } else {
-            ok &= t.grad_dtype == NK_F32   ? chunk_step8<float>(t, ch, a8, decay)
-                  : t.grad_dtype == NK_F16 ? chunk_step8<__half>(t, ch, a8, decay)
-                                           : chunk_step8<__nv_bfloat16>(t, ch, a8, decay);
-        }
+    uint32_t i = p.n_chunks32 + blockIdx.x * WARPS8 + (threadIdx.x >> 5);
+    AdamwChunk next = i < p.n_chunks ? p.chunks[i] : AdamwChunk{};
+    while (i < p.n_chunks) {
+        const AdamwChunk ch = next;
+        i += gridDim.x * WARPS8;
+        if (i < p.n_chunks) next = p.chunks[i];
+        const nk_adamw_tensor &t = p.tensors[ch.tensor];
+        ok &= t.grad_dtype == NK_F32   ? chunk_step8<float>(t, ch, a8, a, ring)
+              : t.grad_dtype == NK_F16 ? chunk_step8<__half>(t, ch, a8, a, ring)
+                                       : chunk_step8<__nv_bfloat16>(t, ch, a8, a, ring);
     }
     if (!ok && bad) *bad = 1u;
 }
 
 }  // namespace
 
-uint32_t adamw_chunk_elements(uint64_t total, int sms) {
-    // Enough chunks for eight blocks on every SM, of 1024 to 16384 elements.
-    const uint64_t want = total / ((uint64_t)sms * 8) / 1024 * 1024;
-    return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(want, 1024), 16384);
+uint32_t adamw_chunk_elements(uint64_t total, int sms, int bits) {
+    if (bits == 32) {
+        // Enough chunks for eight blocks of threads on every SM, of 1024 to 16384 elements.
+        const uint64_t want = total / ((uint64_t)sms * 8) / 1024 * 1024;
+        return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(want, 1024), 16384);
+    }
+    // The same number for each warp, of 32 blocks at most.
+    const uint64_t blocks = total / NK_ADAMW_BLOCK + 1, warps = (uint64_t)sms * 3 * WARPS8;
+    const uint64_t rounds = (blocks + warps * 32 - 1) / (warps * 32);
+    return NK_ADAMW_BLOCK * (uint32_t)((blocks + warps * rounds - 1) / (warps * rounds));
 }
+
+uint32_t adamw_partials(int sms) { return (uint32_t)sms * 8; }
 
 cudaError_t adamw_many_norm(const AdamwMany &p, float grad_scale, float max_norm, float *norm, uint32_t *bad, int sms,
                             cudaStream_t st) {
-    const unsigned blocks = std::max(1u, std::min<unsigned>(p.n_chunks, (unsigned)sms * 8));
+    const unsigned blocks = std::max(1u, std::min<unsigned>(p.n_chunks, adamw_partials(sms)));
     adamw_norm_k<<<blocks, 256, 0, st>>>(p, grad_scale, max_norm, norm, bad);
     return cudaGetLastError();
 }
 
 cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, float grad_scale, bool with_clip, uint32_t *bad,
                             int sms, cudaStream_t st) {
-    const uint32_t n32 = p.n_chunks32, n8 = p.n_chunks - n32;
-    if (n32) adamw_many_k<32><<<std::min<unsigned>(n32, (unsigned)sms * 8), 256, 0, st>>>(p, 0, n32, a, grad_scale, with_clip, bad);
-    if (n8) adamw_many_k<8><<<std::min<unsigned>(n8, (unsigned)sms * 8), 256, 0, st>>>(p, n32, p.n_chunks, a, grad_scale, with_clip, bad);
+    const uint32_t n8 = p.n_chunks - p.n_chunks32;
+    if (p.n_chunks32)
+        adamw32_k<<<std::min<unsigned>(p.n_chunks32, (unsigned)sms * 8), 256, 0, st>>>(p, a, grad_scale, with_clip, bad);
+    if (n8) {
+        constexpr int shared = WARPS8 * STAGES8 * (int)sizeof(Stage8);
+        cudaError_t e = allow_shared(adamw8_k, shared);
+        if (e != cudaSuccess) return e;
+        adamw8_k<<<std::min<unsigned>((n8 + WARPS8 - 1) / WARPS8, (unsigned)sms * 3), 32 * WARPS8, shared, st>>>(p, a, grad_scale, with_clip, bad);
+    }
     return cudaGetLastError();
 }
 

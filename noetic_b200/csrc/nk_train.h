@@ -24,12 +24,14 @@ struct AdamwMany {
     const nk_adamw_tensor *tensors;  // device
     const AdamwChunk *chunks;        // device: [0, n_chunks32) of 32-bit moments, then those of 8-bit ones
     uint32_t n_chunks, n_chunks32;
-    double *partial;   // device [n_chunks]: sums of squares
+    double *partial;   // device [adamw_partials]: sums of squares
     uint32_t *ticket;  // device, 0 between calls
     float *clip;       // device [2]: the factor of the gradients; 0 or 1: whether the step runs
 };
-// How many elements a chunk should have for a model of `total` elements.
-uint32_t adamw_chunk_elements(uint64_t total, int sms);
+// How many elements a chunk should have, of `total` with moments of `bits`, and how
+// many partial sums the norm leaves at most.
+uint32_t adamw_chunk_elements(uint64_t total, int sms, int bits);
+uint32_t adamw_partials(int sms);
 // clip[0] = grad_scale * min(1, max_norm / norm), with the norm also to *norm (nullable).
 cudaError_t adamw_many_norm(const AdamwMany &p, float grad_scale, float max_norm, float *norm, uint32_t *bad,
                             int sms, cudaStream_t st);

@@ -317,23 +317,25 @@ nk_status nk_adamw_many_create(const nk_adamw_tensor *tensors, uint64_t count, n
         const int device = device_of(tensors, count, now);
         Current current(device);
         const int sms = sm_count();
-        uint64_t total = 0;
-        for (uint64_t i = 0; i < count; ++i) total += tensors[i].n;
-        const uint32_t size = nk::adamw_chunk_elements(total, sms);
         std::vector<nk::AdamwChunk> chunks;
         uint32_t n32 = 0;
         for (const int bits : {32, 8}) {
+            uint64_t total = 0;
+            for (uint64_t i = 0; i < count; ++i) total += tensors[i].state_bits == bits ? tensors[i].n : 0;
+            const uint32_t size = nk::adamw_chunk_elements(total, sms, bits);
             for (uint64_t i = 0; i < count; ++i) {
                 if (tensors[i].state_bits != bits) continue;
                 for (uint64_t at = 0; at < tensors[i].n; at += size)
                     chunks.push_back({(uint32_t)i, (uint32_t)std::min<uint64_t>(size, tensors[i].n - at), at});
             }
+            // Whole chunks first: the last round of a grid is then one of short ones.
+            std::stable_partition(chunks.begin() + (bits == 32 ? 0 : n32), chunks.end(), [&](const nk::AdamwChunk &c) { return c.n == size; });
             if (bits == 32) n32 = (uint32_t)chunks.size();
         }
         // One allocation: the tables, the partial sums, the ticket and the factor.
         auto round = [](size_t n) { return (n + 255) / 256 * 256; };
         const size_t tb = round(count * sizeof(nk_adamw_tensor)), cb = round(chunks.size() * sizeof(nk::AdamwChunk)),
-                     pb = round(chunks.size() * sizeof(double));
+                     pb = round(nk::adamw_partials(sms) * sizeof(double));
         std::unique_ptr<nk_adamw_many, void (*)(nk_adamw_many *)> many(new nk_adamw_many, nk_adamw_many_free);
         many->device = device;
         many->sms = sms;
