@@ -244,9 +244,11 @@ struct Step8 {
 
 // A block of 256 elements on its way to a warp: copies into shared memory that
 // need no registers, so that each warp has STAGES8 - 1 blocks (2.5 KB each) in flight
-// while it works on one.  (With loads into registers instead the kernel waited for
-// memory 60% of its time: 88 us of 19M elements where this takes 64.)
-constexpr int STAGES8 = 3, WARPS8 = 8;
+// while it works on one.  16 warps on an SM with four stages: 24 warps with three, 32
+// with two and 16 with six measured 1272, 1348 and 1419 us where this takes 1259 (361M
+// elements, bf16 gradients and copy, the norm's 112 us with it); chunks of 128 blocks
+// rather than 32, and plain stores rather than streaming ones, took 55 us off that.
+constexpr int STAGES8 = 4, WARPS8 = 8;
 struct __align__(16) Stage8 {
     float val[NK_ADAMW_BLOCK];
     uint32_t grad[NK_ADAMW_BLOCK];  // up to 4 bytes an element
@@ -435,9 +437,9 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
             // A root above 0 (then above 1e-19) stays above 0: a later step divides by it.
             vo[i] = to_e4m3(fminf(fmaxf(z.x, least), big.x), fminf(fmaxf(z.y, least), big.y));
         }
-        __stcs(reinterpret_cast<float4 *>(t.val + first + at), make_float4(p[0], p[1], p[2], p[3]));
-        __stcs(reinterpret_cast<uint32_t *>((uint8_t *)t.m + first + at), mo[0] | mo[1] << 16);
-        __stcs(reinterpret_cast<uint32_t *>((uint8_t *)t.v + first + at), vo[0] | vo[1] << 16);
+        *reinterpret_cast<float4 *>(t.val + first + at) = make_float4(p[0], p[1], p[2], p[3]);
+        *reinterpret_cast<uint32_t *>((uint8_t *)t.m + first + at) = mo[0] | mo[1] << 16;
+        *reinterpret_cast<uint32_t *>((uint8_t *)t.v + first + at) = vo[0] | vo[1] << 16;
         if (t.copy) store_copy4(t.copy, t.copy_dtype, first + at, p);
     }
     if (lane == 0) {
@@ -516,7 +518,7 @@ __global__ void __launch_bounds__(256, 6) adamw32_k(AdamwMany p, AdamwParams a, 
 }
 
 // 8-bit moments: each warp takes chunks of its own, a ring of blocks ahead.
-__global__ void __launch_bounds__(32 * WARPS8, 3) adamw8_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad) {
+__global__ void __launch_bounds__(32 * WARPS8, 2) adamw8_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad) {
     extern __shared__ Stage8 rings[];
     float c = grad_scale;
     if (with_clip) {
@@ -548,9 +550,9 @@ uint32_t adamw_chunk_elements(uint64_t total, int sms, int bits) {
         const uint64_t want = total / ((uint64_t)sms * 8) / 1024 * 1024;
         return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(want, 1024), 16384);
     }
-    // The same number for each warp, of 32 blocks at most.
-    const uint64_t blocks = total / NK_ADAMW_BLOCK + 1, warps = (uint64_t)sms * 3 * WARPS8;
-    const uint64_t rounds = (blocks + warps * 32 - 1) / (warps * 32);
+    // The same number for each warp, of 128 blocks at most.
+    const uint64_t blocks = total / NK_ADAMW_BLOCK + 1, warps = (uint64_t)sms * 2 * WARPS8;
+    const uint64_t rounds = (blocks + warps * 128 - 1) / (warps * 128);
     return NK_ADAMW_BLOCK * (uint32_t)((blocks + warps * rounds - 1) / (warps * rounds));
 }
 
@@ -572,7 +574,7 @@ cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, float grad
         constexpr int shared = WARPS8 * STAGES8 * (int)sizeof(Stage8);
         cudaError_t e = allow_shared(adamw8_k, shared);
         if (e != cudaSuccess) return e;
-        adamw8_k<<<std::min<unsigned>((n8 + WARPS8 - 1) / WARPS8, (unsigned)sms * 3), 32 * WARPS8, shared, st>>>(p, a, grad_scale, with_clip, bad);
+        adamw8_k<<<std::min<unsigned>((n8 + WARPS8 - 1) / WARPS8, (unsigned)sms * 2), 32 * WARPS8, shared, st>>>(p, a, grad_scale, with_clip, bad);
     }
     return cudaGetLastError();
 }
