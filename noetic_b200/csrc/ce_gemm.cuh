@@ -69,7 +69,7 @@ struct Gemm {
     const uint32_t *target;  // of each row that counts
     // GRAD: G goes out through mapC0, its second part through mapC1
     const float2 *stats;     // of each row that counts
-    const float *weight;     // of each row that counts, relative to the largest
+    const float *weight;     // of each row that counts
     int col0;                // the piece's first token
     float g_scale;
     // STORE
@@ -308,7 +308,7 @@ struct GradEpilogue {
                                             int c)
         : p(q), map0(a), map1(b), box(to), in(row < live), row0(row - (int)(threadIdx.x & 31)), col(c),
           t(in ? q.target[row] - (uint32_t)q.col0 : NO_TOKEN), st(in ? q.stats[row] : make_float2(0.0f, 0.0f)),
-          h(in ? q.weight[row] * q.g_scale : 0.0f), base((st.x + st.y) * LOG2E) {}
+          h(in ? q.weight[row] / q.head->weight_max * q.g_scale : 0.0f), base((st.x + st.y) * LOG2E) {}
     __device__ __forceinline__ void some(int c, float *v) {
         const int lane = threadIdx.x & 31;
         if (SCALED) {

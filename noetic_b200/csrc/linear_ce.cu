@@ -32,42 +32,155 @@ constexpr float G_SCALE = 16384.0f;
 
 constexpr size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-// A block joins 32 rows' tiles, in a fixed order: lane = row, warps share the tiles.
+// A block joins the tiles of 8 rows, in a fixed order: 32 threads a row.  row_of null:
+// the rows are as the caller has them, and those without a token get zeros.
 __global__ void __launch_bounds__(256) ce_join_k(LinearCeArgs a, const Head *head, const uint32_t *row_of, const float2 *part,
                                                  int64_t part_ld, const float *zt, int tiles) {
-    __shared__ float red[8][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t i = (int64_t)blockIdx.x * 32 + lane;
-    const int64_t n = head->live;
-    if ((int64_t)blockIdx.x * 32 >= n) return;
-    const bool in = i < n;
-    const float2 *p = part + i;
+    __shared__ float2 red[8][33];
+    const int at = threadIdx.x & 7, slot = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = (int64_t)blockIdx.x * 8 + at, n = row_of ? (int64_t)head->live : a.rows;
+    if ((int64_t)blockIdx.x * 8 >= n) return;
     float m = -INFINITY, s = 0.0f;
-    if (in)
-        for (int t = warp; t < tiles; t += 8) {
-            const float2 q = p[t * part_ld];
+    if (i < n)
+        for (int t = slot; t < tiles; t += 32) {
+            const float2 q = part[t * part_ld + i];
             const float now = fmaxf(m, q.x), base = now == -INFINITY ? 0.0f : now;
             s = fmaf(q.y, ex2((q.x - base) * LOG2E), s * ex2((m - base) * LOG2E));
             m = now;
         }
-    red[warp][lane] = m;
+    red[at][slot] = make_float2(m, s);
     __syncthreads();
-    float top = red[0][lane];
+    // Warp w finishes row w.
+    const float2 q = red[warp][lane];
+    float top = q.x;
 #pragma unroll
-    for (int w = 1; w < 8; ++w) top = fmaxf(top, red[w][lane]);
-    __syncthreads();
-    red[warp][lane] = s * ex2((m - (top == -INFINITY ? 0.0f : top)) * LOG2E);
-    __syncthreads();
-    if (warp != 0 || !in) return;
-    s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) s += red[w][lane];
-    float ls = logf(s), loss = (top - zt[i]) + ls;
-    // Not a number, or a wait in the product ran out.
-    if (!(isfinite(loss) && isfinite(ls)) || head->err) top = ls = loss = NAN;
-    const int64_t row = row_of[i];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    s = warp_sum(q.y * ex2((q.x - (top == -INFINITY ? 0.0f : top)) * LOG2E));
+    const int64_t mine = (int64_t)blockIdx.x * 8 + warp;
+    if (lane != 0 || mine >= n) return;
+    const int64_t row = row_of ? row_of[mine] : mine;
+    float loss = 0.0f, ls = 0.0f;
+    if (row_of || a.targets[row] < (uint32_t)a.vocab) {
+        ls = logf(s);
+        loss = (top - zt[mine]) + ls;
+        // Not a number, or a wait in the product ran out.
+        if (!(isfinite(loss) && isfinite(ls)) || (head && head->err)) top = ls = loss = NAN;
+    } else {
+        top = 0.0f;
+    }
     if (a.loss) a.loss[row] = loss;
     if (a.stats) a.stats[2 * row] = top, a.stats[2 * row + 1] = ls;
+}
+
+// ---------------------------------------------------------------- few rows
+// Where the product is small the bound is reading w once (or launches): f32 fmas on
+// the CUDA cores, 8 rows of x in shared memory, and a warp that multiplies them with
+// COLS rows of w at a time, straight from memory.
+constexpr int FEW_WARPS = 8;
+constexpr int few_cols(int rows) { return rows >= 8 ? 4 : 8; }
+
+// N sums over the warp at once: lane l ends with that of value l % N (N a power of
+// two up to 32), for N - 1 + log2(32 / N) shuffles.
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = N / 2; h >= 1; h >>= 1) {
+        const bool up = lane & h;
+#pragma unroll
+        for (int i = 0; i < h; ++i) {
+            const float keep = up ? v[i + h] : v[i], give = up ? v[i] : v[i + h];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, h);
+        }
+    }
+    float s = v[0];
+#pragma unroll
+    for (int o = N; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
+template <class T, int R>
+__global__ void __launch_bounds__(32 * FEW_WARPS) ce_few_k(LinearCeArgs a, float2 *part, int64_t part_ld, float *zt) {
+    constexpr int COLS = few_cols(R), PER = 16 / (int)sizeof(T), N = R * COLS;
+    extern __shared__ __align__(16) float xs[];  // [R][width up to whole vectors]
+    __shared__ float2 red[FEW_WARPS][R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.width, whole = d / PER, ld = (d + PER - 1) / PER * PER;
+    const int64_t r0 = (int64_t)blockIdx.y * R;
+    for (int i = threadIdx.x; i < R * ld; i += 32 * FEW_WARPS) {
+        const int r = i / ld, k = i - r * ld;
+        // (A row without a token is not read.)
+        const bool in = k < d && r0 + r < a.rows && a.targets[r0 + r] < (uint32_t)a.vocab;
+        xs[i] = in ? to_f32(((const T *)a.x)[(r0 + r) * a.x_stride + k]) : 0.0f;
+    }
+    __syncthreads();
+    // The lane's own row and column of w among the N products.
+    const int mine = lane % N, my_row = mine / COLS, my_col = mine % COLS;
+    const uint32_t target = r0 + my_row < a.rows ? a.targets[r0 + my_row] : NO_TOKEN;
+    float m = -INFINITY, s = 0.0f;
+    const int step = gridDim.x * FEW_WARPS * COLS;
+    for (int v0 = (blockIdx.x * FEW_WARPS + warp) * COLS; v0 < a.vocab; v0 += step) {
+        float acc[N] = {};
+        const T *w[COLS];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) w[c] = (const T *)a.w + (int64_t)min(v0 + c, a.vocab - 1) * a.w_stride;
+        for (int u = lane; u < whole; u += 32) {
+            uint4 q[COLS];
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) q[c] = __ldg(reinterpret_cast<const uint4 *>(w[c] + u * PER));
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int e = 0; e < PER; e += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(&xs[r * ld + u * PER + e]);
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c) {
+                        const T *y = reinterpret_cast<const T *>(&q[c]) + e;
+                        float &t = acc[r * COLS + c];
+                        t = fmaf(x.x, to_f32(y[0]), t);
+                        t = fmaf(x.y, to_f32(y[1]), t);
+                        t = fmaf(x.z, to_f32(y[2]), t);
+                        t = fmaf(x.w, to_f32(y[3]), t);
+                    }
+                }
+        }
+        if (lane < d - whole * PER) {
+            const int k = whole * PER + lane;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) {
+                const float y = to_f32(w[c][k]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r * COLS + c] = fmaf(xs[r * ld + k], y, acc[r * COLS + c]);
+            }
+        }
+        const float z = warp_sums<N>(acc);
+        const int col = v0 + my_col;
+        if (col < a.vocab && lane < N) {
+            if ((uint32_t)col == target) zt[r0 + my_row] = z;
+            const float now = fmaxf(m, z), base = now == -INFINITY ? 0.0f : now;
+            s = fmaf(s, ex2((m - base) * LOG2E), ex2((z - base) * LOG2E));
+            m = now;
+        }
+    }
+    // The lanes of a row (COLS neighbours), then the warps.
+#pragma unroll
+    for (int o = COLS / 2; o >= 1; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        const float now = fmaxf(m, m2), base = now == -INFINITY ? 0.0f : now;
+        s = s * ex2((m - base) * LOG2E) + s2 * ex2((m2 - base) * LOG2E);
+        m = now;
+    }
+    if (lane < N && my_col == 0) red[warp][my_row] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x < R && r0 + threadIdx.x < a.rows) {
+        m = -INFINITY, s = 0.0f;
+        for (int w = 0; w < FEW_WARPS; ++w) {
+            const float2 q = red[w][threadIdx.x];
+            const float now = fmaxf(m, q.x), base = now == -INFINITY ? 0.0f : now;
+            s = s * ex2((m - base) * LOG2E) + q.y * ex2((q.x - base) * LOG2E);
+            m = now;
+        }
+        part[blockIdx.x * part_ld + r0 + threadIdx.x] = make_float2(m, s);
+    }
 }
 
 // ---------------------------------------------------------------- rows that count
@@ -77,61 +190,86 @@ struct Index {
     uint32_t *row_of, *place;  // the row of each that counts; the place of each row, or NO_TOKEN
     uint32_t *target;
     float2 *stats;   // backward
-    float *weight;   // backward: relative to the largest
+    float *weight;   // backward
 };
 
-// One block: each thread walks rows / 1024 of the rows, twice, around a prefix sum.
+// One block, 8192 rows at a time: a thread looks at 8, and a prefix sum of the warps'
+// counts gives each its place.  (Neighbouring threads take neighbouring rows: with 8
+// rows in a row to a thread this took 31 us of 8192 rows.)
 __global__ void __launch_bounds__(1024) ce_index_k(LinearCeArgs a, Index ix, bool backward) {
-    __shared__ uint32_t sums[32];
+    __shared__ uint32_t counts[8 * 32];
+    __shared__ uint32_t all;
     __shared__ float tops[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t per = (a.rows + 1023) / 1024, r0 = min(a.rows, tid * per), r1 = min(a.rows, r0 + per);
-    auto weight = [&](int64_t r) { return a.row_weight ? a.row_weight[r] : 1.0f; };
-    auto counts = [&](int64_t r) { return a.targets[r] < (uint32_t)a.vocab && (!backward || weight(r) != 0.0f); };
-    uint32_t n = 0;
+    uint32_t carry = 0;
     float top = 0.0f;
-    for (int64_t r = r0; r < r1; ++r)
-        if (counts(r)) {
-            ++n;
-            if (backward) top = fmaxf(top, fabsf(weight(r)));
-        }
-    uint32_t upto = n;
+    for (int64_t r0 = 0; r0 < a.rows; r0 += 8192) {
+        uint32_t t[8], votes[8];
+        float w[8];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int i = 0; i < 8; ++i) {
+            const int64_t r = r0 + i * 1024 + tid;
+            t[i] = r < a.rows ? a.targets[r] : NO_TOKEN;
+            w[i] = backward && a.row_weight && r < a.rows ? a.row_weight[r] : 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool counts_in = t[i] < (uint32_t)a.vocab && w[i] != 0.0f;
+            if (counts_in) top = fmaxf(top, fabsf(w[i]));
+            votes[i] = __ballot_sync(0xffffffffu, counts_in);
+            if (lane == 0) counts[i * 32 + warp] = __popc(votes[i]);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t n[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n[i] = counts[lane * 8 + i], sum += n[i];
+            uint32_t upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            uint32_t before = upto - sum;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) counts[lane * 8 + i] = before, before += n[i];
+            if (lane == 31) all = upto;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t r = r0 + i * 1024 + tid;
+            if (r >= a.rows) continue;
+            if (!(votes[i] >> lane & 1)) {
+                ix.place[r] = NO_TOKEN;
+                if (!backward) {
+                    if (a.loss) a.loss[r] = 0.0f;
+                    if (a.stats) a.stats[2 * r] = a.stats[2 * r + 1] = 0.0f;
+                }
+                continue;
+            }
+            const uint32_t at = carry + counts[i * 32 + warp] + __popc(votes[i] & ((1u << lane) - 1));
+            ix.place[r] = at;
+            ix.row_of[at] = (uint32_t)r;
+            ix.target[at] = t[i];
+            if (backward) {
+                ix.stats[at] = make_float2(a.in_stats[2 * r], a.in_stats[2 * r + 1]);
+                ix.weight[at] = w[i];
+            }
+        }
+        carry += all;
+        __syncthreads();
     }
-    if (lane == 31) sums[warp] = upto;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) tops[warp] = top;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-    top = 0.0f;
-    for (int w = 0; w < 32; ++w) {
-        if (w < warp) before += sums[w];
-        all += sums[w];
-        top = fmaxf(top, tops[w]);
+    if (warp == 0) {
+        top = tops[lane];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) *ix.head = Head{0u, carry, backward ? top : 1.0f, 0u, 0u};
     }
-    uint32_t at = before + upto - n;
-    for (int64_t r = r0; r < r1; ++r) {
-        if (!counts(r)) {
-            ix.place[r] = NO_TOKEN;
-            if (!backward) {
-                if (a.loss) a.loss[r] = 0.0f;
-                if (a.stats) a.stats[2 * r] = a.stats[2 * r + 1] = 0.0f;
-            }
-            continue;
-        }
-        ix.place[r] = at;
-        ix.row_of[at] = (uint32_t)r;
-        ix.target[at] = a.targets[r];
-        if (backward) {
-            ix.stats[at] = make_float2(a.in_stats[2 * r], a.in_stats[2 * r + 1]);
-            ix.weight[at] = __fdiv_rn(weight(r), top);
-        }
-        ++at;
-    }
-    if (tid == 0) *ix.head = Head{0u, all, backward ? top : 1.0f, 0u, 0u};
 }
 
 // The largest finite |x| of the rows that count (place not null), or of all.
@@ -308,6 +446,7 @@ struct Plan {
     int64_t mp = 0;      // rows, up to whole tiles
     int64_t dp = 0;      // columns of laid out rows
     bool split = false;  // f32: two parts
+    bool few = false;    // forward on the CUDA cores
     bool copy_w = false;
     int tiles = 0;       // partial results of a row
     int piece = 0;       // tokens of G at a time
@@ -317,11 +456,35 @@ struct Plan {
            dx = 0, dw = 0, bytes = 0;
 };
 
-// Pieces of K for a product of few tiles: as many as fill the pairs, each of 8
-// K-blocks at least.
+// Pieces of K for a product of few tiles, of 8 K-blocks at least: the number that
+// needs the fewest rounds of the pairs, where each piece more costs its sums' way to
+// memory and back (about 16 K-blocks' time).
 int pick_splits(int64_t tiles, int64_t kblocks, int pairs) {
-    const int64_t s = std::min<int64_t>(pairs / std::max<int64_t>(1, tiles), kblocks / 8);
-    return (int)std::max<int64_t>(1, s);
+    int best = 1;
+    double least = 1e300;
+    for (int s = 1; s <= 64 && kblocks / s >= 8; ++s) {
+        const double rounds = (double)((tiles * s + pairs - 1) / pairs);
+        const double cost = rounds * ((double)kblocks / s) + (s > 1 ? 16.0 * rounds : 0.0);
+        if (cost < least * 0.97) least = cost, best = s;
+    }
+    return best;
+}
+
+// Whether the forward call takes the few rows' kernel: w's rows in whole 16-byte units,
+// 8 of x within shared memory, and a product below what the other way's launches and
+// (f32) two more passes over w cost.  Measured (us, this and the other way):
+// FEW_FIGURES
+bool few_rows(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride) {
+    const int es = dtype == NK_F32 ? 4 : 2;
+    if (((uintptr_t)w & 15) != 0 || w_stride * es % 16 != 0 || width > 4096 || rows > 4096) return false;
+    const double products = (double)rows * width * vocab;
+    return dtype == NK_F32 ? products <= 6e8 : rows <= 4 || products <= 1e8;
+}
+int few_blocks(int64_t rows, int vocab) {
+    const int r = rows >= 8 ? 8 : rows > 2 ? 4 : (int)std::max<int64_t>(rows, 1);
+    const int64_t groups = (rows + r - 1) / r, cols = (int64_t)FEW_WARPS * few_cols(r);
+    // (148 SMs, three blocks on each; the workspace does not go by the device.)
+    return (int)std::max<int64_t>(1, std::min<int64_t>((vocab + cols - 1) / cols, 444 / groups));
 }
 
 Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride, bool backward) {
@@ -332,9 +495,14 @@ Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int
         return at;
     };
     p.mp = (int64_t)round_up((size_t)std::max<int64_t>(rows, 1), ce::TM);
-    p.dp = (int64_t)round_up((size_t)width, 8);
+    // Rows of whole 128-byte lines: boxes that straddle them make a product 30% slower
+    // (1000 columns: 275 us of 9472 x 16384 rows, and 210 with 1024).  A copy of w costs
+    // about as much as a third of the product with 1024 rows, or with 2048 where the
+    // product is the only one; below that, rows from 16 bytes on are taken as they are.
+    p.dp = (int64_t)round_up((size_t)width, 64);
     p.split = dtype == NK_F32;
-    p.copy_w = p.split || ((uintptr_t)w & 15) != 0 || w_stride % 8 != 0;
+    const bool lines = ((uintptr_t)w & 127) == 0 && w_stride % 64 == 0, units = ((uintptr_t)w & 15) == 0 && w_stride % 8 == 0;
+    p.copy_w = p.split || !units || (!lines && rows >= (backward ? 1024 : 2048));
     const size_t parts = p.split ? 2 : 1;
     p.head = room(sizeof(Head));
     p.scales = room(8);
@@ -344,6 +512,15 @@ Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int
     p.x = room((size_t)p.mp * p.dp * 2 * parts);
     if (p.copy_w) p.w = room((size_t)vocab * p.dp * 2 * parts);
     if (!backward) {
+        p.few = few_rows(dtype, rows, width, vocab, w, w_stride);
+        if (p.few) {
+            p.bytes = 0;
+            p.tiles = few_blocks(rows, vocab);
+            p.mp = rows;
+            p.part = room((size_t)rows * p.tiles * 8);
+            p.zt = room((size_t)rows * 4);
+            return p;
+        }
         p.tiles = 2 * ((vocab + ce::TN - 1) / ce::TN);
         p.part = room((size_t)p.mp * p.tiles * 8);
         p.zt = room((size_t)rows * 4);
@@ -475,7 +652,20 @@ struct Call {
         return g;
     }
 
+    template <int R>
+    cudaError_t few() {
+        auto *k = ce_few_k<T, R>;
+        const int shared = R * (int)round_up((size_t)a.width, 16 / sizeof(T)) * 4;
+        cudaError_t e = allow_shared(k, R * 4096 * 4);
+        if (e != cudaSuccess) return e;
+        k<<<dim3((unsigned)p.tiles, (unsigned)((a.rows + R - 1) / R)), 32 * FEW_WARPS, shared, st>>>(a, at<float2>(p.part), p.mp,
+                                                                                                      at<float>(p.zt));
+        ce_join_k<<<(unsigned)((a.rows + 7) / 8), 256, 0, st>>>(a, nullptr, nullptr, at<float2>(p.part), p.mp, at<float>(p.zt), p.tiles);
+        return cudaGetLastError();
+    }
+
     cudaError_t forward() {
+        if (p.few) return a.rows >= 8 ? few<8>() : a.rows > 2 ? few<4>() : a.rows == 2 ? few<2>() : few<1>();
         cudaError_t e = begin(false);
         if (e != cudaSuccess) return e;
         Maps m{};
@@ -489,7 +679,7 @@ struct Call {
         g.target = ix.target;
         e = launch<ce::ROWS, P, SPLIT, true, false, false>(m, g, sms, st);
         if (e != cudaSuccess) return e;
-        ce_join_k<<<(unsigned)((a.rows + 31) / 32), 256, 0, st>>>(a, ix.head, ix.row_of, g.part, p.mp, g.zt, p.tiles);
+        ce_join_k<<<(unsigned)((a.rows + 7) / 8), 256, 0, st>>>(a, ix.head, ix.row_of, g.part, p.mp, g.zt, p.tiles);
         return cudaGetLastError();
     }
 
