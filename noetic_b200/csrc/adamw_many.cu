@@ -90,6 +90,8 @@ __device__ __forceinline__ bool aligned(const void *p, uint32_t to) { return ((u
 // not depend on scheduling.
 __global__ void __launch_bounds__(256) adamw_norm_k(AdamwMany p, float grad_scale, float max_norm, float *norm,
                                                     uint32_t *bad) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ double red[32];
     __shared__ bool last;
     double sum = 0.0;
@@ -500,6 +502,8 @@ __device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const Adam
 
 // 32-bit moments: a block of threads takes chunks block, block + blocks, ...
 __global__ void __launch_bounds__(256, 6) adamw32_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad) {
+    pdl_trigger();
+    pdl_wait();
     float c = grad_scale;
     if (with_clip) {
         if (p.clip[1] == 0.0f) return;
@@ -519,6 +523,8 @@ __global__ void __launch_bounds__(256, 6) adamw32_k(AdamwMany p, AdamwParams a, 
 
 // 8-bit moments: each warp takes chunks of its own, a ring of blocks ahead.
 __global__ void __launch_bounds__(32 * WARPS8, 2) adamw8_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad) {
+    pdl_trigger();
+    pdl_wait();
     extern __shared__ Stage8 rings[];
     float c = grad_scale;
     if (with_clip) {
@@ -561,22 +567,25 @@ uint32_t adamw_partials(int sms) { return (uint32_t)sms * 8; }
 cudaError_t adamw_many_norm(const AdamwMany &p, float grad_scale, float max_norm, float *norm, uint32_t *bad, int sms,
                             cudaStream_t st) {
     const unsigned blocks = std::max(1u, std::min<unsigned>(p.n_chunks, adamw_partials(sms)));
-    adamw_norm_k<<<blocks, 256, 0, st>>>(p, grad_scale, max_norm, norm, bad);
-    return cudaGetLastError();
+    return pdl_launch(adamw_norm_k, dim3(blocks), dim3(256), 0, st, p, grad_scale, max_norm, norm, bad);
 }
 
 cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, float grad_scale, bool with_clip, uint32_t *bad,
                             int sms, cudaStream_t st) {
     const uint32_t n8 = p.n_chunks - p.n_chunks32;
-    if (p.n_chunks32)
-        adamw32_k<<<std::min<unsigned>(p.n_chunks32, (unsigned)sms * 8), 256, 0, st>>>(p, a, grad_scale, with_clip, bad);
+    if (p.n_chunks32) {
+        const cudaError_t e = pdl_launch(adamw32_k, dim3(std::min<unsigned>(p.n_chunks32, (unsigned)sms * 8)), dim3(256), 0, st, p, a,
+                                         grad_scale, with_clip, bad);
+        if (e != cudaSuccess) return e;
+    }
     if (n8) {
         constexpr int shared = WARPS8 * STAGES8 * (int)sizeof(Stage8);
         cudaError_t e = allow_shared(adamw8_k, shared);
         if (e != cudaSuccess) return e;
-        adamw8_k<<<std::min<unsigned>((n8 + WARPS8 - 1) / WARPS8, (unsigned)sms * 2), 32 * WARPS8, shared, st>>>(p, a, grad_scale, with_clip, bad);
+        return pdl_launch(adamw8_k, dim3(std::min<unsigned>((n8 + WARPS8 - 1) / WARPS8, (unsigned)sms * 2)), dim3(32 * WARPS8), shared, st,
+                          p, a, grad_scale, with_clip, bad);
     }
-    return cudaGetLastError();
+    return cudaSuccess;
 }
 
 }  // namespace nk

@@ -29,7 +29,7 @@ constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * BK * 2;          // a CTA's half of A or B
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int THREADS = 384, EPI_WARPS = 8;
-constexpr int BOX_BYTES = 32 * 64 * 2;  // GRAD: 32 rows and 64 columns of G, on their way out
+constexpr int BOX_BYTES = 4096;  // GRAD, STORE: 32 rows of 128 bytes on their way out
 constexpr int smem_bytes(bool boxes) { return STAGES * STAGE_BYTES + (boxes ? EPI_WARPS * BOX_BYTES : 0) + 1024 + 256; }
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint64_t WAIT_NS = 1000000000ull;
@@ -37,6 +37,7 @@ constexpr uint64_t WAIT_NS = 1000000000ull;
 // is off by half a step of the sum for each 16 of K, all one way (measured: 1.7e-8
 // of a logit each).  Where f32 results depend on it (the loss; f32 gradients), a
 // chain ends after CHAIN K-blocks and the epilogue's registers add the chains up.
+// (f32: the low parts' products come first, as one chain: they are 2^-11 of the sum.)
 constexpr int CHAIN = 8;
 constexpr int REGS_FEW = 64, REGS_MANY = 216;  // 4 warps and 8 of 32: within 384 * 168
 
@@ -192,6 +193,9 @@ __device__ __forceinline__ void tmem_wait(float *v) {
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
+
+// Where the chain from K-block k of an item on ends; `low`: K-blocks of the low parts.
+__device__ __forceinline__ int chain_end(int k, int k1, int low) { return min(k1, k < low ? low : k + CHAIN); }
 
 // A tile's piece: its row and column block and its K-blocks.
 struct Item {
@@ -351,24 +355,23 @@ struct GradEpilogue {
     __device__ __forceinline__ void end() const {}
 };
 
+// Four neighbouring columns of an output row.
 template <class T>
-__device__ __forceinline__ void store_out(const Gemm &p, const float *v, int64_t at, int col) {
+__device__ __forceinline__ void store_out(const Gemm &p, const float4 &x, int64_t at, int col) {
     T *o = (T *)p.out + at + col;
-    constexpr int PER = 16 / sizeof(T);
-    if (col + 64 <= p.n_valid && ((uintptr_t)o & 15) == 0) {
+    float v[4] = {x.x, x.y, x.z, x.w};
+    struct __align__(4 * sizeof(T)) Four {
+        T e[4];
+    } q;
+    if (col + 4 <= p.n_valid && ((uintptr_t)o & (4 * sizeof(T) - 1)) == 0) {
+        if (p.out_add) q = *reinterpret_cast<const Four *>(o);
 #pragma unroll
-        for (int j = 0; j < 64; j += PER) {
-            uint4 q;
-            T *e = reinterpret_cast<T *>(&q);
-            if (p.out_add) q = *reinterpret_cast<const uint4 *>(o + j);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) e[i] = from_f32<T>(p.out_add ? v[j + i] + to_f32(e[i]) : v[j + i]);
-            *reinterpret_cast<uint4 *>(o + j) = q;
-        }
+        for (int i = 0; i < 4; ++i) q.e[i] = from_f32<T>(p.out_add ? v[i] + to_f32(q.e[i]) : v[i]);
+        *reinterpret_cast<Four *>(o) = q;
     } else {
 #pragma unroll
-        for (int j = 0; j < 64; ++j)
-            if (col + j < p.n_valid) o[j] = from_f32<T>(p.out_add ? v[j] + to_f32(o[j]) : v[j]);
+        for (int i = 0; i < 4; ++i)
+            if (col + i < p.n_valid) o[i] = from_f32<T>(p.out_add ? v[i] + to_f32(o[i]) : v[i]);
     }
 }
 
@@ -379,43 +382,56 @@ __device__ __forceinline__ float out_factor(const Gemm &p) {
     return f;
 }
 
-// F32: the output is always f32 (f32 inputs).
+// Sums to memory, 32 columns of the warp's rows at a time, through its box so that 8
+// lanes write 128 bytes of a row (dw of 1531 rows: 99 us with a row to a lane).  F32:
+// the output is always f32 (f32 inputs).
 template <bool F32>
 struct StoreEpilogue {
     const Gemm &p;
+    float *const box;
     const bool any;  // K has anything: else the accumulator holds nothing
-    const int row, rows, col;
+    const int row0, rows, col;
     const float factor;
     float *const acc;
-    __device__ __forceinline__ StoreEpilogue(const Gemm &g, bool has, int r, int n, int c, int split, float f)
-        : p(g), any(has), row(r), rows(n), col(c), factor(f),
-          acc(g.acc ? g.acc + (int64_t)split * g.acc_split + (int64_t)r * g.ld_acc + c : nullptr) {}
-    __device__ __forceinline__ void some(int c, float *v) {
-        if (col + c >= p.n_valid || row >= rows) return;
-        if (!any)
+    __device__ __forceinline__ StoreEpilogue(const Gemm &g, uint8_t *to, bool has, int r, int n, int c, int split, float f)
+        : p(g), box((float *)to), any(has), row0(r - (int)(threadIdx.x & 31)), rows(n), col(c), factor(f),
+          acc(g.acc ? g.acc + (int64_t)split * g.acc_split + c : nullptr) {}
+    __device__ __forceinline__ void some(int c0, float *v) {
+        const int lane = threadIdx.x & 31;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = 0.0f;
-        float *a = acc + c;
-        if (p.add)
+        for (int h = 0; h < 64; h += 32) {
+            const int c = c0 + h;
+            if (col + c >= p.n_valid) return;  // warp-uniform
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                const float4 q = *reinterpret_cast<const float4 *>(a + j);
-                v[j] += q.x, v[j + 1] += q.y, v[j + 2] += q.z, v[j + 3] += q.w;
+            for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<float4 *>(box + lane * 32 + ((j >> 2) ^ (lane & 7)) * 4) =
+                    any ? make_float4(v[h + j], v[h + j + 1], v[h + j + 2], v[h + j + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            __syncwarp();
+            const int cc = c + (lane & 7) * 4;
+#pragma unroll 4
+            for (int r = lane >> 3; r < 32; r += 4) {
+                if (row0 + r >= rows) break;
+                float4 x = *reinterpret_cast<const float4 *>(box + r * 32 + ((lane & 7) ^ (r & 7)) * 4);
+                float4 *a = reinterpret_cast<float4 *>(acc + (int64_t)(row0 + r) * p.ld_acc + cc);
+                if (p.add) {
+                    const float4 q = *a;
+                    x.x += q.x, x.y += q.y, x.z += q.z, x.w += q.w;
+                }
+                if (p.keep) {
+                    *a = x;
+                    continue;
+                }
+                x.x *= factor, x.y *= factor, x.z *= factor, x.w *= factor;
+                const int64_t at = (p.out_row ? (int64_t)p.out_row[row0 + r] : row0 + r + p.out_row0) * p.out_ld;
+                if (F32 || p.out_dtype == 0)
+                    store_out<float>(p, x, at, col + cc);
+                else if (p.out_dtype == 1)
+                    store_out<__half>(p, x, at, col + cc);
+                else
+                    store_out<__nv_bfloat16>(p, x, at, col + cc);
             }
-        if (p.keep) {
-#pragma unroll
-            for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4 *>(a + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            return;
         }
-#pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] *= factor;
-        const int64_t at = (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld;
-        if (F32 || p.out_dtype == 0)
-            store_out<float>(p, v, at, col + c);
-        else if (p.out_dtype == 1)
-            store_out<__half>(p, v, at, col + c);
-        else
-            store_out<__nv_bfloat16>(p, v, at, col + c);
     }
     __device__ __forceinline__ void end() const {}
 };
@@ -440,7 +456,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *boxes = smem + STAGES * STAGE_BYTES;
-    uint64_t *bars = (uint64_t *)(boxes + (MODE == GRAD ? EPI_WARPS * BOX_BYTES : 0));
+    uint64_t *bars = (uint64_t *)(boxes + (MODE == ROWS ? 0 : EPI_WARPS * BOX_BYTES));
     uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -472,9 +488,12 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     pair_sync();  // both CTAs' barriers exist before either signals the other
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    pdl_trigger();
+    pdl_wait();  // (what the kernels before left is read from here on)
     const int live = (int)p.head->live;
     const int M = p.live_dim == 0 ? live : p.M, K = p.live_dim == 1 ? live : p.K;
     const Walk walk(p, M, K);
+    const int low = SCALED ? 2 * walk.kblocks : 0;
     // A wait that ran out ends the role that waited; the others' waits on it run out too.
     auto give_up = [&](uint32_t code) { atomicExch(&p.head->err, code); };
 
@@ -539,7 +558,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             for (int i = pair; fine && i < walk.items; i += n_pairs) {
                 const Item it = walk.at(p, i);
                 for (int k = it.k0;;) {
-                    const int end = LONG ? min(it.k1, k + CHAIN) : it.k1, b = n & 1;
+                    const int end = LONG ? chain_end(k, it.k1, low) : it.k1, b = n & 1;
                     fine = mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1));
                     if (!__all_sync(0xffffffffu, fine)) {
                         if (one) give_up(202);
@@ -612,7 +631,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
                     tmem_wait<128>(sum);
                     give();
 #pragma unroll 1
-                    for (int k = it.k0 + CHAIN; k < it.k1; k += CHAIN) {
+                    for (int k = chain_end(it.k0, it.k1, low); k < it.k1; k = chain_end(k, it.k1, low)) {
                         fine = take();
                         if (!fine) return;
 #pragma unroll
@@ -649,7 +668,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             else if constexpr (MODE == GRAD)
                 whole(GradEpilogue<T, SCALED>(p, &mapC0, &mapC1, boxes + (warp - 4) * BOX_BYTES, row, live, col));
             else
-                whole(StoreEpilogue<SCALED>(p, it.k1 > it.k0, row, M, col, it.split, factor));
+                whole(StoreEpilogue<SCALED>(p, boxes + (warp - 4) * BOX_BYTES, it.k1 > it.k0, row, M, col, it.split, factor));
         }
         if (MODE == GRAD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }

@@ -36,16 +36,26 @@ constexpr size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; 
 // the rows are as the caller has them, and those without a token get zeros.
 __global__ void __launch_bounds__(256) ce_join_k(LinearCeArgs a, const Head *head, const uint32_t *row_of, const float2 *part,
                                                  int64_t part_ld, const float *zt, int tiles) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ float2 red[8][33];
     const int at = threadIdx.x & 7, slot = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t i = (int64_t)blockIdx.x * 8 + at, n = row_of ? (int64_t)head->live : a.rows;
     if ((int64_t)blockIdx.x * 8 >= n) return;
     float m = -INFINITY, s = 0.0f;
     if (i < n)
-        for (int t = slot; t < tiles; t += 32) {
-            const float2 q = part[t * part_ld + i];
-            const float now = fmaxf(m, q.x), base = now == -INFINITY ? 0.0f : now;
-            s = fmaf(q.y, ex2((q.x - base) * LOG2E), s * ex2((m - base) * LOG2E));
+        for (int t0 = slot; t0 < tiles; t0 += 256) {
+            float2 q[8];  // (eight loads at once: one after the other they took most of the time)
+            float now = m;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                q[u] = t0 + 32 * u < tiles ? part[(t0 + 32 * u) * part_ld + i] : make_float2(-INFINITY, 0.0f);
+                now = fmaxf(now, q[u].x);
+            }
+            const float base = now == -INFINITY ? 0.0f : now;
+            s *= ex2((m - base) * LOG2E);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s = fmaf(q[u].y, ex2((q[u].x - base) * LOG2E), s);
             m = now;
         }
     red[at][slot] = make_float2(m, s);
@@ -100,7 +110,9 @@ __device__ __forceinline__ float warp_sums(float (&v)[N]) {
 }
 
 template <class T, int R>
-__global__ void __launch_bounds__(32 * FEW_WARPS) ce_few_k(LinearCeArgs a, float2 *part, int64_t part_ld, float *zt) {
+__global__ void __launch_bounds__(32 * FEW_WARPS, R <= 2 ? 4 : 2) ce_few_k(LinearCeArgs a, float2 *part, int64_t part_ld, float *zt) {
+    pdl_trigger();
+    pdl_wait();
     constexpr int COLS = few_cols(R), PER = 16 / (int)sizeof(T), N = R * COLS;
     extern __shared__ __align__(16) float xs[];  // [R][width up to whole vectors]
     __shared__ float2 red[FEW_WARPS][R];
@@ -197,6 +209,8 @@ struct Index {
 // counts gives each its place.  (Neighbouring threads take neighbouring rows: with 8
 // rows in a row to a thread this took 31 us of 8192 rows.)
 __global__ void __launch_bounds__(1024) ce_index_k(LinearCeArgs a, Index ix, bool backward) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ uint32_t counts[8 * 32];
     __shared__ uint32_t all;
     __shared__ float tops[32];
@@ -275,6 +289,8 @@ __global__ void __launch_bounds__(1024) ce_index_k(LinearCeArgs a, Index ix, boo
 // The largest finite |x| of the rows that count (place not null), or of all.
 __global__ void __launch_bounds__(256) ce_absmax_k(const float *x, int64_t stride, int64_t rows, int d, const uint32_t *place,
                                                    uint32_t *out) {
+    pdl_trigger();
+    pdl_wait();
     float top = 0.0f;
     const int lane = threadIdx.x & 31;
     const int64_t step = (int64_t)gridDim.x * 8;
@@ -284,12 +300,18 @@ __global__ void __launch_bounds__(256) ce_absmax_k(const float *x, int64_t strid
         int c = 0;
         if (((uintptr_t)p & 15) == 0) {
             c = d & ~3;
-            for (int i = lane * 4; i < c; i += 128) {
-                const float4 q = *reinterpret_cast<const float4 *>(p + i);
-                const float v[4] = {q.x, q.y, q.z, q.w};
+            for (int i0 = lane * 4; i0 < c; i0 += 1024) {
+                float4 q[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (isfinite(v[e])) top = fmaxf(top, fabsf(v[e]));
+                for (int u = 0; u < 8; ++u)
+                    q[u] = i0 + u * 128 < c ? *reinterpret_cast<const float4 *>(p + i0 + u * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (isfinite(v[e])) top = fmaxf(top, fabsf(v[e]));
+                }
             }
         }
         for (int i = c + lane; i < d; i += 32)
@@ -318,6 +340,8 @@ template <class T>
 __global__ void __launch_bounds__(256) ce_lay_out_k(const T *src, int64_t stride, int64_t rows, int d, const uint32_t *place,
                                                     const Head *head, void *dst, int64_t ld, int64_t part, int fill, int64_t room,
                                                     T *zero, int64_t zero_stride, const uint32_t *top, float *undo) {
+    pdl_trigger();
+    pdl_wait();
     const int lane = threadIdx.x & 31;
     const float scale = top ? part_scale(*top) : 1.0f;
     if (undo && blockIdx.x == 0 && threadIdx.x == 0) *undo = 1.0f / scale;
@@ -337,17 +361,36 @@ __global__ void __launch_bounds__(256) ce_lay_out_k(const T *src, int64_t stride
         const T *p = src + r * stride;
         if constexpr (sizeof(T) == 2) {
             T *o = (T *)dst + to * ld;
-            const bool vec = real && ((uintptr_t)p & 15) == 0;
-            for (int i = lane * 8; i < ld; i += 256) {
-                uint4 q = make_uint4(0, 0, 0, 0);
-                T *e = reinterpret_cast<T *>(&q);
-                if (vec && i + 8 <= d)
-                    q = *reinterpret_cast<const uint4 *>(p + i);
-                else if (real)
+            // A row that starts within a unit of 16 bytes is read in whole units (no more of
+            // them than it touches), each shifted together with the next lane's.
+            const uint32_t off = (uintptr_t)p & 15, units = (off + 2 * d + 15) / 16;
+            const uint4 *from = reinterpret_cast<const uint4 *>((uintptr_t)p - off);
+            for (int i0 = 0; i0 < ld; i0 += 256) {
+                const uint32_t u = i0 / 8 + lane;
+                uint4 q = real && u < units ? from[u] : make_uint4(0, 0, 0, 0);
+                if (off) {  // (the warp's one row)
+                    uint4 n;
+                    n.x = __shfl_down_sync(0xffffffffu, q.x, 1);
+                    n.y = __shfl_down_sync(0xffffffffu, q.y, 1);
+                    n.z = __shfl_down_sync(0xffffffffu, q.z, 1);
+                    n.w = __shfl_down_sync(0xffffffffu, q.w, 1);
+                    if (lane == 31) n = real && u + 1 < units ? from[u + 1] : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
+                    const uint32_t words = off / 4, bits = off % 4 * 8;
+                    uint32_t x[5];
+#pragma unroll
+                    for (int e = 0; e < 5; ++e) x[e] = words == 0 ? w[e] : words == 1 ? w[e + 1] : words == 2 ? w[e + 2] : e < 5 ? w[min(e + 3, 7)] : 0u;
+                    q = make_uint4(__funnelshift_r(x[0], x[1], bits), __funnelshift_r(x[1], x[2], bits), __funnelshift_r(x[2], x[3], bits),
+                                   __funnelshift_r(x[3], x[4], bits));
+                }
+                const int i = i0 + lane * 8;
+                if (i + 8 > d) {
+                    T *e = reinterpret_cast<T *>(&q);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (i + j < d) e[j] = p[i + j];
-                *reinterpret_cast<uint4 *>(o + i) = q;
+                        if (i + j >= d) e[j] = from_f32<T>(0.0f);
+                }
+                if (i < ld) *reinterpret_cast<uint4 *>(o + i) = q;
             }
         } else {
             __half *o = (__half *)dst + to * ld;
@@ -380,6 +423,8 @@ __global__ void __launch_bounds__(256) ce_lay_out_k(const T *src, int64_t stride
 // The sums of a product whose K was split, in their order, rounded on the way out.
 template <class T>
 __global__ void __launch_bounds__(256) ce_reduce_k(Gemm p, int rows_max, int splits) {
+    pdl_trigger();
+    pdl_wait();
     const int rows = p.live_dim == 0 ? (int)p.head->live : rows_max;
     const float factor = ce::out_factor(p);
     const int64_t n = (int64_t)rows * p.ld_acc / 4;
@@ -404,6 +449,8 @@ __global__ void __launch_bounds__(256) ce_reduce_k(Gemm p, int rows_max, int spl
 // Where a wait in a product ran out, no gradient is right: NaN.
 template <class T, class W>
 __global__ void ce_check_k(const Head *head, T *dx, int64_t rows, int64_t dxs, W *dw, int64_t vocab, int64_t dws, int d) {
+    pdl_trigger();
+    pdl_wait();
     if (head->err == 0) return;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (rows + vocab) * d; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / d;
@@ -483,8 +530,10 @@ bool few_rows(int dtype, int64_t rows, int width, int vocab, const void *w, int6
 int few_blocks(int64_t rows, int vocab) {
     const int r = rows >= 8 ? 8 : rows > 2 ? 4 : (int)std::max<int64_t>(rows, 1);
     const int64_t groups = (rows + r - 1) / r, cols = (int64_t)FEW_WARPS * few_cols(r);
-    // (148 SMs, three blocks on each; the workspace does not go by the device.)
-    return (int)std::max<int64_t>(1, std::min<int64_t>((vocab + cols - 1) / cols, 444 / groups));
+    // (148 SMs, four blocks on each; the workspace does not go by the device.)
+    const int64_t whole = (vocab + cols - 1) / cols, most = std::max<int64_t>(1, 592 * (groups > 1 ? 2 : 1) / groups);
+    const int64_t rounds = (whole + most - 1) / most;
+    return (int)((whole + rounds - 1) / rounds);
 }
 
 Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride, bool backward) {
@@ -552,18 +601,6 @@ struct Maps {
     CUtensorMap a[2], b[2], c[2];
 };
 
-template <int MODE, class T, bool SCALED, bool LONG, bool A_MN, bool B_MN>
-cudaError_t launch(const Maps &m, const Gemm &g, int sms, cudaStream_t st) {
-    auto *k = ce::gemm_k<MODE, T, SCALED, LONG, A_MN, B_MN>;
-    constexpr int shared = ce::smem_bytes(MODE == ce::GRAD);
-    cudaError_t e = allow_shared(k, shared);
-    if (e != cudaSuccess) return e;
-    const int64_t items = (int64_t)((g.M + ce::TM - 1) / ce::TM) * ((g.N + ce::TN - 1) / ce::TN) * g.splits;
-    const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(sms / 2, items));
-    k<<<2 * pairs, ce::THREADS, shared, st>>>(m.a[0], m.a[1], m.b[0], m.b[1], m.c[0], m.c[1], g);
-    return cudaGetLastError();
-}
-
 // T: the type of x and w; P: that of the parts the products take.
 template <class T, class P>
 struct Call {
@@ -588,6 +625,21 @@ struct Call {
         w_ld = p.copy_w ? p.dp : a.w_stride;
         w_cols = p.copy_w ? p.dp : a.width;
     }
+    cudaError_t err = cudaSuccess;  // the first launch's that failed: none follows it
+
+    template <class... K, class... A>
+    void go(void (*k)(K...), dim3 grid, int threads, int shared, A &&...args) {
+        if (err == cudaSuccess) err = pdl_launch(k, grid, dim3((unsigned)threads), (size_t)shared, st, args...);
+    }
+    template <int MODE, bool LONG, bool A_MN, bool B_MN>
+    void product(const Maps &m, const Gemm &g) {
+        auto *k = ce::gemm_k<MODE, P, SPLIT, LONG, A_MN, B_MN>;
+        constexpr int shared = ce::smem_bytes(MODE != ce::ROWS);
+        if (err == cudaSuccess) err = allow_shared(k, shared);
+        const int64_t items = (int64_t)((g.M + ce::TM - 1) / ce::TM) * ((g.N + ce::TN - 1) / ce::TN) * g.splits;
+        const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(sms / 2, items));
+        go(k, 2 * pairs, ce::THREADS, shared, m.a[0], m.a[1], m.b[0], m.b[1], m.c[0], m.c[1], g);
+    }
     template <class U>
     U *at(size_t o) const {
         return (U *)(ws + o);
@@ -596,22 +648,21 @@ struct Call {
 
     // The index, x and, where it has to be, w laid out.
     // (Zero rows follow the rows that count: up to a whole K-block of dw.)
-    cudaError_t begin(bool backward) {
-        ce_index_k<<<1, 1024, 0, st>>>(a, ix, backward);
+    void begin(bool backward) {
+        go(ce_index_k, 1, 1024, 0, a, ix, backward);
         uint32_t *tops = nullptr;
         if (SPLIT) {
             tops = &ix.head->x_max;
-            if (a.rows) ce_absmax_k<<<blocks(a.rows), 256, 0, st>>>((const float *)a.x, a.x_stride, a.rows, a.width, ix.place, tops);
-            ce_absmax_k<<<blocks(a.vocab), 256, 0, st>>>((const float *)a.w, a.w_stride, a.vocab, a.width, nullptr, tops + 1);
+            if (a.rows) go(ce_absmax_k, blocks(a.rows), 256, 0, (const float *)a.x, a.x_stride, a.rows, a.width, ix.place, tops);
+            go(ce_absmax_k, blocks(a.vocab), 256, 0, (const float *)a.w, a.w_stride, a.vocab, a.width, nullptr, tops + 1);
         }
-        ce_lay_out_k<T><<<blocks(a.rows + ce::TM), 256, 0, st>>>((const T *)a.x, a.x_stride, a.rows, a.width, ix.place, ix.head,
+        go(ce_lay_out_k<T>, blocks(a.rows + ce::TM), 256, 0, (const T *)a.x, a.x_stride, a.rows, a.width, ix.place, ix.head,
                                                                  at<void>(p.x), p.dp, p.mp * p.dp, ce::BK - 1, p.mp, (T *)a.dx, a.dx_stride,
                                                                  tops, SPLIT ? scales : nullptr);
         if (p.copy_w)
-            ce_lay_out_k<T><<<blocks(a.vocab), 256, 0, st>>>((const T *)a.w, a.w_stride, a.vocab, a.width, nullptr, nullptr,
+            go(ce_lay_out_k<T>, blocks(a.vocab), 256, 0, (const T *)a.w, a.w_stride, a.vocab, a.width, nullptr, nullptr,
                                                              at<void>(p.w), p.dp, (int64_t)a.vocab * p.dp, 0, 0, nullptr, 0,
                                                              tops ? tops + 1 : nullptr, SPLIT ? scales + 1 : nullptr);
-        return cudaGetLastError();
     }
 
     bool map_x(CUtensorMap (&m)[2], int box) const {
@@ -656,18 +707,16 @@ struct Call {
     cudaError_t few() {
         auto *k = ce_few_k<T, R>;
         const int shared = R * (int)round_up((size_t)a.width, 16 / sizeof(T)) * 4;
-        cudaError_t e = allow_shared(k, R * 4096 * 4);
-        if (e != cudaSuccess) return e;
-        k<<<dim3((unsigned)p.tiles, (unsigned)((a.rows + R - 1) / R)), 32 * FEW_WARPS, shared, st>>>(a, at<float2>(p.part), p.mp,
+        err = allow_shared(k, R * 4096 * 4);
+        go(k, dim3((unsigned)p.tiles, (unsigned)((a.rows + R - 1) / R)), 32 * FEW_WARPS, shared, a, at<float2>(p.part), p.mp,
                                                                                                       at<float>(p.zt));
-        ce_join_k<<<(unsigned)((a.rows + 7) / 8), 256, 0, st>>>(a, nullptr, nullptr, at<float2>(p.part), p.mp, at<float>(p.zt), p.tiles);
-        return cudaGetLastError();
+        go(ce_join_k, (unsigned)((a.rows + 7) / 8), 256, 0, a, nullptr, nullptr, at<float2>(p.part), p.mp, at<float>(p.zt), p.tiles);
+        return err;
     }
 
     cudaError_t forward() {
         if (p.few) return a.rows >= 8 ? few<8>() : a.rows > 2 ? few<4>() : a.rows == 2 ? few<2>() : few<1>();
-        cudaError_t e = begin(false);
-        if (e != cudaSuccess) return e;
+        begin(false);
         Maps m{};
         if (!map_x(m.a, 128) || !map_w(m.b, 128)) return cudaErrorInvalidValue;
         Gemm g = gemm((int)a.rows, a.vocab, a.width, 0, false, false, 1);
@@ -677,22 +726,19 @@ struct Call {
         g.part_ld = p.mp;
         g.zt = at<float>(p.zt);
         g.target = ix.target;
-        e = launch<ce::ROWS, P, SPLIT, true, false, false>(m, g, sms, st);
-        if (e != cudaSuccess) return e;
-        ce_join_k<<<(unsigned)((a.rows + 7) / 8), 256, 0, st>>>(a, ix.head, ix.row_of, g.part, p.mp, g.zt, p.tiles);
-        return cudaGetLastError();
+        product<ce::ROWS, true, false, false>(m, g);
+        go(ce_join_k, (unsigned)((a.rows + 7) / 8), 256, 0, a, ix.head, ix.row_of, g.part, p.mp, g.zt, p.tiles);
+        return err;
     }
 
     template <class O>
-    cudaError_t reduce(const Gemm &g, int rows, int splits) const {
+    void reduce(const Gemm &g, int rows, int splits) {
         const int64_t n = (int64_t)rows * g.ld_acc / 4;
-        ce_reduce_k<O><<<(unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, (int64_t)sms * 8)), 256, 0, st>>>(g, rows, splits);
-        return cudaGetLastError();
+        go(ce_reduce_k<O>, (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, (int64_t)sms * 8)), 256, 0, g, rows, splits);
     }
 
     cudaError_t backward() {
-        cudaError_t e = begin(true);
-        if (e != cudaSuccess) return e;
+        begin(true);
         Maps mg{}, mx{}, mw{};
         if (!map_x(mg.a, 128) || !map_w(mg.b, 128) || !map_g(mg.c, 32) || !map_g(mx.a, 128) || !map_w(mx.b, 64) || !map_g(mw.a, 64) || !map_x(mw.b, 64))
             return cudaErrorInvalidValue;
@@ -709,8 +755,7 @@ struct Call {
             g.weight = ix.weight;
             g.col0 = v0;
             g.g_scale = g_scale;
-            if (a.rows) e = launch<ce::GRAD, P, SPLIT, SPLIT, false, false>(mg, g, sms, st);
-            if (e != cudaSuccess) return e;
+            if (a.rows) product<ce::GRAD, SPLIT, false, false>(mg, g);
             if (a.dx) {
                 Gemm c = gemm((int)a.rows, a.width, n, 0, false, true, p.dx_splits);
                 c.b_row0 = v0;
@@ -725,9 +770,8 @@ struct Call {
                 c.out_dtype = a.dtype;
                 c.out_row = ix.row_of;
                 c.out_scale = a.grad_scale / g_scale;
-                e = launch<ce::STORE, P, SPLIT, SPLIT, false, true>(mx, c, sms, st);
-                if (e == cudaSuccess && last && p.dx_splits > 1) e = reduce<T>(c, (int)a.rows, p.dx_splits);
-                if (e != cudaSuccess) return e;
+                product<ce::STORE, SPLIT, false, true>(mx, c);
+                if (last && p.dx_splits > 1) reduce<T>(c, (int)a.rows, p.dx_splits);
             }
             if (a.dw) {
                 Gemm c = gemm(n, a.width, (int)a.rows, 1, true, true, p.dw_splits);
@@ -742,17 +786,20 @@ struct Call {
                 c.out_dtype = a.dw_dtype;
                 c.out_add = a.accumulate;
                 c.out_scale = a.grad_scale / g_scale;
-                e = launch<ce::STORE, P, SPLIT, SPLIT, true, true>(mw, c, sms, st);
-                if (e == cudaSuccess && p.dw_splits > 1)
-                    e = a.dw_dtype == NK_F32 ? reduce<float>(c, n, p.dw_splits) : reduce<T>(c, n, p.dw_splits);
-                if (e != cudaSuccess) return e;
+                product<ce::STORE, SPLIT, true, true>(mw, c);
+                if (p.dw_splits > 1) {
+                    if (a.dw_dtype == NK_F32)
+                        reduce<float>(c, n, p.dw_splits);
+                    else
+                        reduce<T>(c, n, p.dw_splits);
+                }
             }
         }
         if (a.dw_dtype == NK_F32)
-            ce_check_k<T, float><<<(unsigned)sms, 256, 0, st>>>(ix.head, (T *)a.dx, a.rows, a.dx_stride, (float *)a.dw, a.vocab, a.dw_stride, a.width);
+            go(ce_check_k<T, float>, (unsigned)sms, 256, 0, ix.head, (T *)a.dx, a.rows, a.dx_stride, (float *)a.dw, a.vocab, a.dw_stride, a.width);
         else
-            ce_check_k<T, T><<<(unsigned)sms, 256, 0, st>>>(ix.head, (T *)a.dx, a.rows, a.dx_stride, (T *)a.dw, a.vocab, a.dw_stride, a.width);
-        return cudaGetLastError();
+            go(ce_check_k<T, T>, (unsigned)sms, 256, 0, ix.head, (T *)a.dx, a.rows, a.dx_stride, (T *)a.dw, a.vocab, a.dw_stride, a.width);
+        return err;
     }
 };
 
