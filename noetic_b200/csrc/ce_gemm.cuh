@@ -355,23 +355,23 @@ struct GradEpilogue {
     __device__ __forceinline__ void end() const {}
 };
 
-// Four neighbouring columns of an output row.
+// Four neighbouring columns of an output row at o, of which `n` exist; vec: they do, and
+// o is a multiple of their size.
 template <class T>
-__device__ __forceinline__ void store_out(const Gemm &p, const float4 &x, int64_t at, int col) {
-    T *o = (T *)p.out + at + col;
-    float v[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ void store_out(T *o, const float4 &x, bool add, bool vec, int n) {
+    const float v[4] = {x.x, x.y, x.z, x.w};
     struct __align__(4 * sizeof(T)) Four {
         T e[4];
     } q;
-    if (col + 4 <= p.n_valid && ((uintptr_t)o & (4 * sizeof(T) - 1)) == 0) {
-        if (p.out_add) q = *reinterpret_cast<const Four *>(o);
+    if (vec) {
+        if (add) q = *reinterpret_cast<const Four *>(o);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q.e[i] = from_f32<T>(p.out_add ? v[i] + to_f32(q.e[i]) : v[i]);
+        for (int i = 0; i < 4; ++i) q.e[i] = from_f32<T>(add ? v[i] + to_f32(q.e[i]) : v[i]);
         *reinterpret_cast<Four *>(o) = q;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (col + i < p.n_valid) o[i] = from_f32<T>(p.out_add ? v[i] + to_f32(o[i]) : v[i]);
+            if (i < n) o[i] = from_f32<T>(add ? v[i] + to_f32(o[i]) : v[i]);
     }
 }
 
@@ -383,19 +383,39 @@ __device__ __forceinline__ float out_factor(const Gemm &p) {
 }
 
 // Sums to memory, 32 columns of the warp's rows at a time, through its box so that 8
-// lanes write 128 bytes of a row (dw of 1531 rows: 99 us with a row to a lane).  F32:
-// the output is always f32 (f32 inputs).
+// lanes write 128 bytes of a row; a lane's 8 rows (lane / 8 + 4 i) are taken from the
+// box together and go out together (one after the other they took 12 us a tile where
+// the MMAs of 1536 of K take 6.5).  F32: the output is always f32 (f32 inputs).
 template <bool F32>
 struct StoreEpilogue {
     const Gemm &p;
     float *const box;
     const bool any;  // K has anything: else the accumulator holds nothing
-    const int row0, rows, col;
+    const int col, rows;  // first column; how many of the warp's 32 rows exist
     const float factor;
     float *const acc;
+    int64_t out[8];  // where the lane's rows start in the output, in elements
     __device__ __forceinline__ StoreEpilogue(const Gemm &g, uint8_t *to, bool has, int r, int n, int c, int split, float f)
-        : p(g), box((float *)to), any(has), row0(r - (int)(threadIdx.x & 31)), rows(n), col(c), factor(f),
-          acc(g.acc ? g.acc + (int64_t)split * g.acc_split + c : nullptr) {}
+        : p(g), box((float *)to), any(has), col(c), rows(n - (r - (int)(threadIdx.x & 31))), factor(f),
+          acc(g.acc ? g.acc + (int64_t)split * g.acc_split + (int64_t)(r - (int)(threadIdx.x & 31) + ((threadIdx.x & 31) >> 3)) * g.ld_acc + c
+                    : nullptr) {
+        const int row0 = r - (int)(threadIdx.x & 31) + ((int)(threadIdx.x & 31) >> 3);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = min(row0 + 4 * i, n - 1);
+            out[i] = p.keep ? 0 : (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld;
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ void write(const float4 (&x)[8], int c) const {
+        const int lane = threadIdx.x & 31, left = p.n_valid - (col + c);
+        const bool vec = left >= 4 && (((uintptr_t)p.out | (uintptr_t)(p.out_ld * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
+        T *o = (T *)p.out + col + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((lane >> 3) + 4 * i < rows)
+                store_out<T>(o + out[i], make_float4(x[i].x * factor, x[i].y * factor, x[i].z * factor, x[i].w * factor), p.out_add != 0, vec, left);
+    }
     __device__ __forceinline__ void some(int c0, float *v) {
         const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -409,27 +429,30 @@ struct StoreEpilogue {
                     any ? make_float4(v[h + j], v[h + j + 1], v[h + j + 2], v[h + j + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
             __syncwarp();
             const int cc = c + (lane & 7) * 4;
-#pragma unroll 4
-            for (int r = lane >> 3; r < 32; r += 4) {
-                if (row0 + r >= rows) break;
-                float4 x = *reinterpret_cast<const float4 *>(box + r * 32 + ((lane & 7) ^ (r & 7)) * 4);
-                float4 *a = reinterpret_cast<float4 *>(acc + (int64_t)(row0 + r) * p.ld_acc + cc);
-                if (p.add) {
-                    const float4 q = *a;
-                    x.x += q.x, x.y += q.y, x.z += q.z, x.w += q.w;
-                }
-                if (p.keep) {
-                    *a = x;
-                    continue;
-                }
-                x.x *= factor, x.y *= factor, x.z *= factor, x.w *= factor;
-                const int64_t at = (p.out_row ? (int64_t)p.out_row[row0 + r] : row0 + r + p.out_row0) * p.out_ld;
-                if (F32 || p.out_dtype == 0)
-                    store_out<float>(p, x, at, col + cc);
-                else if (p.out_dtype == 1)
-                    store_out<__half>(p, x, at, col + cc);
-                else
-                    store_out<__nv_bfloat16>(p, x, at, col + cc);
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = (lane >> 3) + 4 * i;
+                x[i] = *reinterpret_cast<const float4 *>(box + r * 32 + ((lane & 7) ^ (r & 7)) * 4);
+            }
+            float *a = acc + cc;
+            if (p.add)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((lane >> 3) + 4 * i < rows) {
+                        const float4 q = *reinterpret_cast<const float4 *>(a + (int64_t)(4 * i) * p.ld_acc);
+                        x[i].x += q.x, x[i].y += q.y, x[i].z += q.z, x[i].w += q.w;
+                    }
+            if (p.keep) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((lane >> 3) + 4 * i < rows) *reinterpret_cast<float4 *>(a + (int64_t)(4 * i) * p.ld_acc) = x[i];
+            } else if (F32 || p.out_dtype == 0) {
+                write<float>(x, cc);
+            } else if (p.out_dtype == 1) {
+                write<__half>(x, cc);
+            } else {
+                write<__nv_bfloat16>(x, cc);
             }
         }
     }

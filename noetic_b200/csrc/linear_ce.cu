@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) ce_join_k(LinearCeArgs a, const Head *hea
 // the CUDA cores, 8 rows of x in shared memory, and a warp that multiplies them with
 // COLS rows of w at a time, straight from memory.
 constexpr int FEW_WARPS = 8;
-constexpr int few_cols(int rows) { return rows >= 8 ? 4 : 8; }
+constexpr int COLS = 4;
 
 // N sums over the warp at once: lane l ends with that of value l % N (N a power of
 // two up to 32), for N - 1 + log2(32 / N) shuffles.
@@ -113,16 +113,17 @@ template <class T, int R>
 __global__ void __launch_bounds__(32 * FEW_WARPS, R <= 2 ? 4 : 2) ce_few_k(LinearCeArgs a, float2 *part, int64_t part_ld, float *zt) {
     pdl_trigger();
     pdl_wait();
-    constexpr int COLS = few_cols(R), PER = 16 / (int)sizeof(T), N = R * COLS;
+    constexpr int PER = 16 / (int)sizeof(T), N = R * COLS;
     extern __shared__ __align__(16) float xs[];  // [R][width up to whole vectors]
     __shared__ float2 red[FEW_WARPS][R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.width, whole = d / PER, ld = (d + PER - 1) / PER * PER;
     const int64_t r0 = (int64_t)blockIdx.y * R;
-    for (int i = threadIdx.x; i < R * ld; i += 32 * FEW_WARPS) {
-        const int r = i / ld, k = i - r * ld;
+    for (int r = warp; r < R; r += FEW_WARPS) {
         // (A row without a token is not read.)
-        const bool in = k < d && r0 + r < a.rows && a.targets[r0 + r] < (uint32_t)a.vocab;
-        xs[i] = in ? to_f32(((const T *)a.x)[(r0 + r) * a.x_stride + k]) : 0.0f;
+        const bool in = r0 + r < a.rows && a.targets[r0 + r] < (uint32_t)a.vocab;
+        const T *x = (const T *)a.x + (r0 + r) * a.x_stride;
+#pragma unroll 8
+        for (int k = lane; k < ld; k += 32) xs[r * ld + k] = in && k < d ? to_f32(x[k]) : 0.0f;
     }
     __syncthreads();
     // The lane's own row and column of w among the N products.
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, R <= 2 ? 4 : 2) ce_few_k(Linea
         const T *w[COLS];
 #pragma unroll
         for (int c = 0; c < COLS; ++c) w[c] = (const T *)a.w + (int64_t)min(v0 + c, a.vocab - 1) * a.w_stride;
+#pragma unroll(R >= 8 ? 1 : 2)
         for (int u = lane; u < whole; u += 32) {
             uint4 q[COLS];
 #pragma unroll
@@ -529,9 +531,9 @@ bool few_rows(int dtype, int64_t rows, int width, int vocab, const void *w, int6
 }
 int few_blocks(int64_t rows, int vocab) {
     const int r = rows >= 8 ? 8 : rows > 2 ? 4 : (int)std::max<int64_t>(rows, 1);
-    const int64_t groups = (rows + r - 1) / r, cols = (int64_t)FEW_WARPS * few_cols(r);
-    // (148 SMs, four blocks on each; the workspace does not go by the device.)
-    const int64_t whole = (vocab + cols - 1) / cols, most = std::max<int64_t>(1, 592 * (groups > 1 ? 2 : 1) / groups);
+    const int64_t groups = (rows + r - 1) / r, cols = (int64_t)FEW_WARPS * COLS;
+    // (148 SMs, four blocks on each, or two of 8 rows: the workspace does not go by the device.)
+    const int64_t whole = (vocab + cols - 1) / cols, most = std::max<int64_t>(1, (groups > 1 ? 296 : 592) / groups);
     const int64_t rounds = (whole + most - 1) / most;
     return (int)((whole + rounds - 1) / rounds);
 }
