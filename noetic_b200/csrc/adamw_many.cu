@@ -217,6 +217,13 @@ __device__ __forceinline__ uint32_t to_e4m3(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// 448 / top, near enough to correctly rounded that hardly an element's place on the
+// grid of e4m3 moves by it.
+__device__ __forceinline__ float grid_scale(float top) {
+    const float r = __fdividef(1.0f, top), k = E4M3_MAX * r;
+    return fmaf(fmaf(-k, top, E4M3_MAX), r, k);
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -333,8 +340,8 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
         }
     top_m = warp_max(top_m);
     top_r = warp_max(top_r);
-    const float km = top_m >= SCALE_MIN ? __fdividef(E4M3_MAX, top_m) : 0.0f;
-    const float kr = top_r >= SCALE_MIN ? __fdividef(E4M3_MAX, top_r) : 0.0f;
+    const float km = top_m >= SCALE_MIN ? grid_scale(top_m) : 0.0f;
+    const float kr = top_r >= SCALE_MIN ? grid_scale(top_r) : 0.0f;
     // A root above 0 stays above 0: a later step divides by it.
     const float least = kr > 0.0f ? E4M3_TINY : 0.0f;
 #pragma unroll
@@ -418,8 +425,8 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
     top_r = warp_max(top_r);
     if (__any_sync(0xffffffffu, !(strange.x + strange.y == 0.0f)) || top_m > MOMENT_MAX)
         return careful_step8(&t, first, NK_ADAMW_BLOCK, params, a.c);
-    const float km = top_m >= SCALE_MIN ? __fdividef(E4M3_MAX, top_m) : 0.0f;
-    const float kr = top_r >= SCALE_MIN ? __fdividef(E4M3_MAX, top_r) : 0.0f;
+    const float km = top_m >= SCALE_MIN ? grid_scale(top_m) : 0.0f;
+    const float kr = top_r >= SCALE_MIN ? grid_scale(top_r) : 0.0f;
     const float least = kr > 0.0f ? E4M3_TINY : 0.0f;
     const float2 root_bc2 = both(a.root_bc2), eps = both(a.eps), rate = both(-a.lr * a.inv_bc1), fade = both(-a.lr * wd);
 #pragma unroll

@@ -61,7 +61,9 @@ struct Gemm {
     int m_fast, group_m;  // tile order: m first within groups of group_m row blocks, else n first
     int splits, kps;      // K-blocks (of all products) a piece of a tile takes
     Head *head;
-    const float *x_scale, *w_scale;  // f32: exact powers of two that undo the parts' scales (nullable)
+    // f32: exact powers of two that undo the parts' scales, one for each row of x and of w
+    // (ROWS), or one for each matrix (nullable in STORE)
+    const float *x_scale, *w_scale;
     int n_valid;                     // columns of C that exist
     // ROWS: part [2 tile + half][Mp] of (maximum, sum), zt [M]
     float2 *part;
@@ -251,9 +253,15 @@ struct RowsEpilogue {
     __device__ __forceinline__ void some(int c, float *v) {
         if (col + c >= p.n_valid) return;  // warp-uniform
         if (SCALED) {
-            const float xs = *p.x_scale, ws = *p.w_scale;
+            // (Scales of each row of x and w; those of w run on to whole tiles.)
+            const float xs = row < live ? p.x_scale[row] : 1.0f;
+            const float4 *ws = reinterpret_cast<const float4 *>(p.w_scale + col + c);
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = v[j] * xs * ws;
+            for (int j = 0; j < 64; j += 4) {
+                const float4 q = ws[j / 4];
+                v[j] = v[j] * xs * q.x, v[j + 1] = v[j + 1] * xs * q.y;
+                v[j + 2] = v[j + 2] * xs * q.z, v[j + 3] = v[j + 3] * xs * q.w;
+            }
         }
         if (col + c + 64 > p.n_valid)
 #pragma unroll

@@ -288,137 +288,173 @@ __global__ void __launch_bounds__(1024) ce_index_k(LinearCeArgs a, Index ix, boo
     }
 }
 
-// The largest finite |x| of the rows that count (place not null), or of all.
-__global__ void __launch_bounds__(256) ce_absmax_k(const float *x, int64_t stride, int64_t rows, int d, const uint32_t *place,
-                                                   uint32_t *out) {
-    pdl_trigger();
-    pdl_wait();
-    float top = 0.0f;
+// The largest finite |x| of a warp's row, on every lane.
+__device__ __forceinline__ float row_absmax(const float *p, int d) {
     const int lane = threadIdx.x & 31;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += step) {
-        if (place && place[r] == NO_TOKEN) continue;
-        const float *p = x + r * stride;
-        int c = 0;
-        if (((uintptr_t)p & 15) == 0) {
-            c = d & ~3;
-            for (int i0 = lane * 4; i0 < c; i0 += 1024) {
-                float4 q[8];
+    float top = 0.0f;
+    int c = 0;
+    if (((uintptr_t)p & 15) == 0) {
+        c = d & ~3;
+        for (int i0 = lane * 4; i0 < c; i0 += 1024) {
+            float4 q[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    q[u] = i0 + u * 128 < c ? *reinterpret_cast<const float4 *>(p + i0 + u * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < 8; ++u)
+                q[u] = i0 + u * 128 < c ? *reinterpret_cast<const float4 *>(p + i0 + u * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const float v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+            for (int u = 0; u < 8; ++u) {
+                const float v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (isfinite(v[e])) top = fmaxf(top, fabsf(v[e]));
-                }
+                for (int e = 0; e < 4; ++e)
+                    if (isfinite(v[e])) top = fmaxf(top, fabsf(v[e]));
             }
         }
-        for (int i = c + lane; i < d; i += 32)
-            if (isfinite(p[i])) top = fmaxf(top, fabsf(p[i]));
     }
+    for (int i = c + lane; i < d; i += 32)
+        if (isfinite(p[i])) top = fmaxf(top, fabsf(p[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+}
+
+// Rows to lay out for the products.
+struct Rows {
+    const void *src;
+    int64_t stride, rows;
+    const uint32_t *place;  // where each goes, or NO_TOKEN (nullable: its own place)
+    void *dst;
+    int64_t part;           // f32: from the high parts to the low ones, in elements
+    int fill;               // rows of zeros behind the last that has a place, within `room`
+    int64_t room;
+    void *zero;             // nullable: where rows without a place become zeros (dx)
+    int64_t zero_stride;
+    uint32_t *top;          // f32: bits of the largest finite number, for one scale; null: a scale for each row
+    float *undo;            // f32: what undoes the scale, or those of the rows
+};
+
+// f32: the largest finite number of the rows of x that count, and of w.
+__global__ void __launch_bounds__(256) ce_absmax_k(Rows x, Rows w, int d) {
+    pdl_trigger();
+    pdl_wait();
+    float top[2] = {0.0f, 0.0f};
+    const int64_t step = (int64_t)gridDim.x * 8;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < x.rows + w.rows; r += step) {
+        const bool of_w = r >= x.rows;
+        if (!of_w && x.place[r] == NO_TOKEN) continue;
+        const float t = row_absmax(of_w ? (const float *)w.src + (r - x.rows) * w.stride : (const float *)x.src + r * x.stride, d);
+        top[of_w] = fmaxf(top[of_w], t);
+    }
     // (Bits of numbers that are not negative are in their order; a maximum does not
     // depend on who comes first.)
-    if (lane == 0 && top > 0.0f) atomicMax(out, __float_as_uint(top));
+    if ((threadIdx.x & 31) == 0) {
+        if (top[0] > 0.0f) atomicMax(x.top, __float_as_uint(top[0]));
+        if (top[1] > 0.0f) atomicMax(w.top, __float_as_uint(top[1]));
+    }
 }
 
-// The power of two that brings the largest of a matrix to [2^14, 2^15).
-__device__ __forceinline__ float part_scale(uint32_t top) {
-    if (top == 0) return 1.0f;
-    const int e = 14 - ilogbf(__uint_as_float(top));
-    return exp2f((float)min(max(e, -120), 120));
+// The power of two that brings the largest of a matrix or a row to [2^14, 2^15).
+__device__ __forceinline__ float part_scale(float top) {
+    if (!(top > 0.0f)) return 1.0f;
+    return exp2f((float)min(max(14 - ilogbf(top), -120), 120));
 }
 
-// Rows as the products take them, from 16-byte boundaries and with zeros up to a
-// multiple of 8 columns: 16-bit rows as they are, f32 rows as two scaled f16 parts,
-// high and low, 22 bits together.  place: where each row goes (null: its own
-// place); `fill` rows behind the last become zeros, within `room` rows.  zero: rows that have no place
-// become zeros there (dx).
+// A warp's row: 16-bit elements as they are, f32 ones as two scaled f16 parts, high
+// and low, 22 bits together; from a 128-byte line on, zeros up to ld.
 template <class T>
-__global__ void __launch_bounds__(256) ce_lay_out_k(const T *src, int64_t stride, int64_t rows, int d, const uint32_t *place,
-                                                    const Head *head, void *dst, int64_t ld, int64_t part, int fill, int64_t room,
-                                                    T *zero, int64_t zero_stride, const uint32_t *top, float *undo) {
+__device__ __forceinline__ void lay_out_row(const Rows &j, const T *p, bool real, int64_t to, int d, int64_t ld) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (sizeof(T) == 2) {
+        T *o = (T *)j.dst + to * ld;
+        // A row that starts within a unit of 16 bytes is read in whole units (no more of
+        // them than it touches), each shifted together with the next lane's.
+        const uint32_t off = (uintptr_t)p & 15, units = (off + 2 * d + 15) / 16;
+        const uint4 *from = reinterpret_cast<const uint4 *>((uintptr_t)p - off);
+        for (int i0 = 0; i0 < ld; i0 += 256) {
+            const uint32_t u = i0 / 8 + lane;
+            uint4 q = real && u < units ? from[u] : make_uint4(0, 0, 0, 0);
+            if (off) {  // (the warp's one row)
+                uint4 n;
+                n.x = __shfl_down_sync(0xffffffffu, q.x, 1);
+                n.y = __shfl_down_sync(0xffffffffu, q.y, 1);
+                n.z = __shfl_down_sync(0xffffffffu, q.z, 1);
+                n.w = __shfl_down_sync(0xffffffffu, q.w, 1);
+                if (lane == 31) n = real && u + 1 < units ? from[u + 1] : make_uint4(0, 0, 0, 0);
+                const uint32_t w[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
+                const uint32_t words = off / 4, bits = off % 4 * 8;
+                uint32_t x[5];
+#pragma unroll
+                for (int e = 0; e < 5; ++e) x[e] = words == 0 ? w[e] : words == 1 ? w[e + 1] : words == 2 ? w[e + 2] : e < 5 ? w[min(e + 3, 7)] : 0u;
+                q = make_uint4(__funnelshift_r(x[0], x[1], bits), __funnelshift_r(x[1], x[2], bits), __funnelshift_r(x[2], x[3], bits),
+                               __funnelshift_r(x[3], x[4], bits));
+            }
+            const int i = i0 + lane * 8;
+            if (i + 8 > d) {
+                T *e = reinterpret_cast<T *>(&q);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (i + j >= d) e[j] = from_f32<T>(0.0f);
+            }
+            if (i < ld) *reinterpret_cast<uint4 *>(o + i) = q;
+        }
+    } else {
+        __half *o = (__half *)j.dst + to * ld;
+        // (With a scale of its own a row is read twice, the second time from the cache.)
+        const float scale = part_scale(j.top ? __uint_as_float(*j.top) : real ? row_absmax(p, d) : 0.0f);
+        if (!j.top && lane == 0) j.undo[to] = 1.0f / scale;
+        const bool vec = real && ((uintptr_t)p & 15) == 0;
+        for (int i = lane * 8; i < ld; i += 256) {
+            float v[8] = {};
+            if (vec && i + 8 <= d) {
+                const float4 a = *reinterpret_cast<const float4 *>(p + i), b = *reinterpret_cast<const float4 *>(p + i + 4);
+                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            } else if (real) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (i + e < d) v[e] = p[i + e];
+            }
+            uint4 hi, lo;
+            __half *h = reinterpret_cast<__half *>(&hi), *l = reinterpret_cast<__half *>(&lo);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = v[e] * scale;
+                h[e] = __float2half_rn(y);
+                l[e] = __float2half_rn(isfinite(y) ? y - __half2float(h[e]) : 0.0f);
+            }
+            *reinterpret_cast<uint4 *>(o + i) = hi;
+            *reinterpret_cast<uint4 *>(o + j.part + i) = lo;
+        }
+    }
+}
+
+// x (its rows that count, in their order, and rows of zeros behind them) and, where it
+// has to be laid out, w (else it has no rows here).
+template <class T>
+__global__ void __launch_bounds__(256) ce_lay_out_k(Rows x, Rows w, int d, int64_t ld, const Head *head) {
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31;
-    const float scale = top ? part_scale(*top) : 1.0f;
-    if (undo && blockIdx.x == 0 && threadIdx.x == 0) *undo = 1.0f / scale;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows + fill; r += step) {
-        const bool real = r < rows;
-        int64_t to = r;
-        if (place) {
-            if (real && place[r] == NO_TOKEN) {
-                if (zero)
-                    for (int i = lane; i < d; i += 32) zero[r * zero_stride + i] = from_f32<T>(0.0f);
+    if (sizeof(T) == 4 && blockIdx.x == 0 && threadIdx.x == 0 && x.top) {
+        *x.undo = 1.0f / part_scale(__uint_as_float(*x.top));
+        *w.undo = 1.0f / part_scale(__uint_as_float(*w.top));
+    }
+    const int64_t step = (int64_t)gridDim.x * 8, xs = x.rows + x.fill;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < xs + w.rows; r += step) {
+        if (r >= xs) {
+            lay_out_row<T>(w, (const T *)w.src + (r - xs) * w.stride, true, r - xs, d, ld);
+            continue;
+        }
+        const bool real = r < x.rows;
+        const T *p = (const T *)x.src + r * x.stride;
+        int64_t to = (int64_t)head->live + (r - x.rows);
+        if (real) {
+            const uint32_t place = x.place[r];
+            if (place == NO_TOKEN) {
+                if (x.zero)
+                    for (int i = lane; i < d; i += 32) ((T *)x.zero)[r * x.zero_stride + i] = from_f32<T>(0.0f);
                 continue;
             }
-            to = real ? (int64_t)place[r] : (int64_t)head->live + (r - rows);
-            if (to >= room) continue;
+            to = place;
         }
-        const T *p = src + r * stride;
-        if constexpr (sizeof(T) == 2) {
-            T *o = (T *)dst + to * ld;
-            // A row that starts within a unit of 16 bytes is read in whole units (no more of
-            // them than it touches), each shifted together with the next lane's.
-            const uint32_t off = (uintptr_t)p & 15, units = (off + 2 * d + 15) / 16;
-            const uint4 *from = reinterpret_cast<const uint4 *>((uintptr_t)p - off);
-            for (int i0 = 0; i0 < ld; i0 += 256) {
-                const uint32_t u = i0 / 8 + lane;
-                uint4 q = real && u < units ? from[u] : make_uint4(0, 0, 0, 0);
-                if (off) {  // (the warp's one row)
-                    uint4 n;
-                    n.x = __shfl_down_sync(0xffffffffu, q.x, 1);
-                    n.y = __shfl_down_sync(0xffffffffu, q.y, 1);
-                    n.z = __shfl_down_sync(0xffffffffu, q.z, 1);
-                    n.w = __shfl_down_sync(0xffffffffu, q.w, 1);
-                    if (lane == 31) n = real && u + 1 < units ? from[u + 1] : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
-                    const uint32_t words = off / 4, bits = off % 4 * 8;
-                    uint32_t x[5];
-#pragma unroll
-                    for (int e = 0; e < 5; ++e) x[e] = words == 0 ? w[e] : words == 1 ? w[e + 1] : words == 2 ? w[e + 2] : e < 5 ? w[min(e + 3, 7)] : 0u;
-                    q = make_uint4(__funnelshift_r(x[0], x[1], bits), __funnelshift_r(x[1], x[2], bits), __funnelshift_r(x[2], x[3], bits),
-                                   __funnelshift_r(x[3], x[4], bits));
-                }
-                const int i = i0 + lane * 8;
-                if (i + 8 > d) {
-                    T *e = reinterpret_cast<T *>(&q);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (i + j >= d) e[j] = from_f32<T>(0.0f);
-                }
-                if (i < ld) *reinterpret_cast<uint4 *>(o + i) = q;
-            }
-        } else {
-            __half *o = (__half *)dst + to * ld;
-            const bool vec = real && ((uintptr_t)p & 15) == 0;
-            for (int i = lane * 8; i < ld; i += 256) {
-                float v[8] = {};
-                if (vec && i + 8 <= d) {
-                    const float4 a = *reinterpret_cast<const float4 *>(p + i), b = *reinterpret_cast<const float4 *>(p + i + 4);
-                    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-                } else if (real) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (i + j < d) v[j] = p[i + j];
-                }
-                uint4 hi, lo;
-                __half *h = reinterpret_cast<__half *>(&hi), *l = reinterpret_cast<__half *>(&lo);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = v[j] * scale;
-                    h[j] = __float2half_rn(y);
-                    l[j] = __float2half_rn(isfinite(y) ? y - __half2float(h[j]) : 0.0f);
-                }
-                *reinterpret_cast<uint4 *>(o + i) = hi;
-                *reinterpret_cast<uint4 *>(o + part + i) = lo;
-            }
-        }
+        if (to < x.room) lay_out_row<T>(x, p, real, to, d, ld);
     }
 }
 
@@ -556,7 +592,7 @@ Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int
     p.copy_w = p.split || !units || (!lines && rows >= (backward ? 1024 : 2048));
     const size_t parts = p.split ? 2 : 1;
     p.head = room(sizeof(Head));
-    p.scales = room(8);
+    if (p.split) p.scales = room(((size_t)p.mp + round_up((size_t)vocab, ce::TN)) * 4);
     p.row_of = room((size_t)rows * 4);
     p.place = room((size_t)rows * 4);
     p.target = room((size_t)rows * 4);
@@ -652,19 +688,16 @@ struct Call {
     // (Zero rows follow the rows that count: up to a whole K-block of dw.)
     void begin(bool backward) {
         go(ce_index_k, 1, 1024, 0, a, ix, backward);
-        uint32_t *tops = nullptr;
-        if (SPLIT) {
-            tops = &ix.head->x_max;
-            if (a.rows) go(ce_absmax_k, blocks(a.rows), 256, 0, (const float *)a.x, a.x_stride, a.rows, a.width, ix.place, tops);
-            go(ce_absmax_k, blocks(a.vocab), 256, 0, (const float *)a.w, a.w_stride, a.vocab, a.width, nullptr, tops + 1);
+        Rows x{a.x, a.x_stride, a.rows, ix.place, at<void>(p.x), p.mp * p.dp, ce::BK - 1, p.mp, a.dx, a.dx_stride, nullptr, scales};
+        Rows w{a.w, a.w_stride, a.vocab, nullptr, at<void>(p.w), (int64_t)a.vocab * p.dp, 0, a.vocab, nullptr, 0, nullptr, scales + p.mp};
+        if (SPLIT && backward) {
+            // (dx and dw sum over tokens and rows: a scale for each matrix.)
+            x.top = &ix.head->x_max;
+            w.top = &ix.head->w_max;
+            go(ce_absmax_k, blocks(a.rows + a.vocab), 256, 0, x, w, a.width);
         }
-        go(ce_lay_out_k<T>, blocks(a.rows + ce::TM), 256, 0, (const T *)a.x, a.x_stride, a.rows, a.width, ix.place, ix.head,
-                                                                 at<void>(p.x), p.dp, p.mp * p.dp, ce::BK - 1, p.mp, (T *)a.dx, a.dx_stride,
-                                                                 tops, SPLIT ? scales : nullptr);
-        if (p.copy_w)
-            go(ce_lay_out_k<T>, blocks(a.vocab), 256, 0, (const T *)a.w, a.w_stride, a.vocab, a.width, nullptr, nullptr,
-                                                             at<void>(p.w), p.dp, (int64_t)a.vocab * p.dp, 0, 0, nullptr, 0,
-                                                             tops ? tops + 1 : nullptr, SPLIT ? scales + 1 : nullptr);
+        if (!p.copy_w) w.rows = 0;
+        go(ce_lay_out_k<T>, blocks(a.rows + w.rows + ce::BK), 256, 0, x, w, a.width, p.dp, ix.head);
     }
 
     bool map_x(CUtensorMap (&m)[2], int box) const {
@@ -723,7 +756,7 @@ struct Call {
         if (!map_x(m.a, 128) || !map_w(m.b, 128)) return cudaErrorInvalidValue;
         Gemm g = gemm((int)a.rows, a.vocab, a.width, 0, false, false, 1);
         g.m_fast = 1;
-        if (SPLIT) g.x_scale = scales, g.w_scale = scales + 1;
+        if (SPLIT) g.x_scale = scales, g.w_scale = scales + p.mp;
         g.part = at<float2>(p.part);
         g.part_ld = p.mp;
         g.zt = at<float>(p.zt);
@@ -751,7 +784,7 @@ struct Call {
             Gemm g = gemm((int)a.rows, n, a.width, 0, false, false, 1);
             g.m_fast = 1;
             g.b_row0 = v0;
-            if (SPLIT) g.x_scale = scales, g.w_scale = scales + 1;
+            if (SPLIT) g.x_scale = scales, g.w_scale = scales + p.mp;
             g.target = ix.target;
             g.stats = ix.stats;
             g.weight = ix.weight;
@@ -761,7 +794,7 @@ struct Call {
             if (a.dx) {
                 Gemm c = gemm((int)a.rows, a.width, n, 0, false, true, p.dx_splits);
                 c.b_row0 = v0;
-                if (SPLIT) c.w_scale = scales + 1;
+                if (SPLIT) c.w_scale = scales + p.mp;
                 c.acc = p.dx ? at<float>(p.dx) : nullptr;
                 c.ld_acc = p.ld_acc;
                 c.acc_split = p.mp * p.ld_acc;
