@@ -36,9 +36,11 @@ constexpr uint64_t WAIT_NS = 1000000000ull;
 // The tensor cores cut, not round, when they add to a sum, so a chain of products
 // is off by half a step of the sum for each 16 of K, all one way (measured: 1.7e-8
 // of a logit each).  Where f32 results depend on it (the loss; f32 gradients), a
-// chain ends after CHAIN K-blocks and the epilogue's registers add the chains up.
+// chain ends after a few K-blocks and the epilogue's registers add the chains up.
 // (f32: the low parts' products come first, as one chain: they are 2^-11 of the sum.)
-constexpr int CHAIN = 8;
+// Logits of f32 rows get the shortest chains: an error of the logit is one of p, and a
+// sure token's gradient is 1 - p.
+constexpr int chain_blocks(bool f32_logits) { return f32_logits ? 2 : 8; }
 constexpr int REGS_FEW = 64, REGS_MANY = 216;  // 4 warps and 8 of 32: within 384 * 168
 
 // What the first kernel of a call finds out, for the others (the workspace's head).
@@ -197,7 +199,10 @@ __device__ __forceinline__ void tmem_wait(float *v) {
 }
 
 // Where the chain from K-block k of an item on ends; `low`: K-blocks of the low parts.
-__device__ __forceinline__ int chain_end(int k, int k1, int low) { return min(k1, k < low ? low : k + CHAIN); }
+template <int CHAIN>
+__device__ __forceinline__ int chain_end(int k, int k1, int low) {
+    return min(k1, k < low ? low : k + CHAIN);
+}
 
 // A tile's piece: its row and column block and its K-blocks.
 struct Item {
@@ -478,7 +483,7 @@ __device__ __forceinline__ void fewer_registers() {
 }
 
 // T: the parts' type.  SCALED: f32 inputs, taken as two scaled f16 parts.  LONG:
-// chains of CHAIN K-blocks, added up in registers.
+// chains of a few K-blocks, added up in registers.
 template <int MODE, class T, bool SCALED, bool LONG, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
@@ -525,6 +530,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     const int M = p.live_dim == 0 ? live : p.M, K = p.live_dim == 1 ? live : p.K;
     const Walk walk(p, M, K);
     const int low = SCALED ? 2 * walk.kblocks : 0;
+    constexpr int CHAIN = chain_blocks(SCALED && MODE != STORE);
     // A wait that ran out ends the role that waited; the others' waits on it run out too.
     auto give_up = [&](uint32_t code) { atomicExch(&p.head->err, code); };
 
@@ -589,7 +595,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             for (int i = pair; fine && i < walk.items; i += n_pairs) {
                 const Item it = walk.at(p, i);
                 for (int k = it.k0;;) {
-                    const int end = LONG ? chain_end(k, it.k1, low) : it.k1, b = n & 1;
+                    const int end = LONG ? chain_end<CHAIN>(k, it.k1, low) : it.k1, b = n & 1;
                     fine = mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1));
                     if (!__all_sync(0xffffffffu, fine)) {
                         if (one) give_up(202);
@@ -662,7 +668,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
                     tmem_wait<128>(sum);
                     give();
 #pragma unroll 1
-                    for (int k = chain_end(it.k0, it.k1, low); k < it.k1; k = chain_end(k, it.k1, low)) {
+                    for (int k = chain_end<CHAIN>(it.k0, it.k1, low); k < it.k1; k = chain_end<CHAIN>(k, it.k1, low)) {
                         fine = take();
                         if (!fine) return;
 #pragma unroll

@@ -790,7 +790,7 @@ struct Call {
             g.weight = ix.weight;
             g.col0 = v0;
             g.g_scale = g_scale;
-            if (a.rows) product<ce::GRAD, SPLIT, false, false>(mg, g);
+            if (a.rows) product<ce::GRAD, true, false, false>(mg, g);
             if (a.dx) {
                 Gemm c = gemm((int)a.rows, a.width, n, 0, false, true, p.dx_splits);
                 c.b_row0 = v0;
