@@ -258,14 +258,14 @@ struct RowsEpilogue {
     __device__ __forceinline__ void some(int c, float *v) {
         if (col + c >= p.n_valid) return;  // warp-uniform
         if (SCALED) {
-            // (Scales of each row of x and w; those of w run on to whole tiles.)
+            // (Scales of each row of x and w; those of w run on to whole tiles.  Their
+            // product first: it leaves f32's range only where the logit does.)
             const float xs = row < live ? p.x_scale[row] : 1.0f;
             const float4 *ws = reinterpret_cast<const float4 *>(p.w_scale + col + c);
 #pragma unroll
             for (int j = 0; j < 64; j += 4) {
                 const float4 q = ws[j / 4];
-                v[j] = v[j] * xs * q.x, v[j + 1] = v[j + 1] * xs * q.y;
-                v[j + 2] = v[j + 2] * xs * q.z, v[j + 3] = v[j + 3] * xs * q.w;
+                v[j] *= xs * q.x, v[j + 1] *= xs * q.y, v[j + 2] *= xs * q.z, v[j + 3] *= xs * q.w;
             }
         }
         if (col + c + 64 > p.n_valid)
@@ -329,9 +329,9 @@ struct GradEpilogue {
     __device__ __forceinline__ void some(int c, float *v) {
         const int lane = threadIdx.x & 31;
         if (SCALED) {
-            const float xs = *p.x_scale, ws = *p.w_scale;
+            const float scale = *p.x_scale * *p.w_scale;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = ex2(((v[j] * xs * ws - st.x) - st.y) * LOG2E) * h;
+            for (int j = 0; j < 64; ++j) v[j] = ex2(((v[j] * scale - st.x) - st.y) * LOG2E) * h;
         } else {
             // (For 16 bits the fma's error, 2^-24 of the log-sum, is nothing.)
 #pragma unroll
@@ -389,6 +389,7 @@ __device__ __forceinline__ void store_out(T *o, const float4 &x, bool add, bool 
 }
 
 __device__ __forceinline__ float out_factor(const Gemm &p) {
+    if (p.head->err) return NAN;  // a wait in a product before this one ran out
     float f = p.out_scale * p.head->weight_max;
     if (p.x_scale) f *= *p.x_scale;
     if (p.w_scale) f *= *p.w_scale;
@@ -655,10 +656,13 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
         };
         const uint32_t mine = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
         bool fine = true;
-        for (int i = pair; fine && i < walk.items; i += n_pairs) {
+        for (int i = pair; i < walk.items; i += n_pairs) {
+            // (After a wait that ran out, sums become NaN: this item's and those that follow.)
+            if (MODE != STORE && !fine) break;
             const Item it = walk.at(p, i);
             const int row = it.tm * TM + (int)rank * 128 + q * 32 + lane, col = it.tn * TN + half * 128;
             auto whole = [&](auto &&e) {
+                if (MODE == STORE && !fine) return;
                 if constexpr (LONG) {
                     float sum[128];
                     fine = take();
@@ -704,8 +708,17 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
                 whole(RowsEpilogue<SCALED>(p, row, live, col, 2 * it.tn + half));
             else if constexpr (MODE == GRAD)
                 whole(GradEpilogue<T, SCALED>(p, &mapC0, &mapC1, boxes + (warp - 4) * BOX_BYTES, row, live, col));
-            else
-                whole(StoreEpilogue<SCALED>(p, boxes + (warp - 4) * BOX_BYTES, it.k1 > it.k0, row, M, col, it.split, factor));
+            else {
+                StoreEpilogue<SCALED> e(p, boxes + (warp - 4) * BOX_BYTES, it.k1 > it.k0, row, M, col, it.split, factor);
+                whole(e);
+                if (!fine) {
+                    float v[64];
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) v[j] = NAN;
+                    e.some(0, v);
+                    e.some(64, v);
+                }
+            }
         }
         if (MODE == GRAD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }

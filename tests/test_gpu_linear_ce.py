@@ -381,6 +381,106 @@ def test_calls_on_streams_and_graphs_side_by_side(nb, torch):
         c.check_backward(stats, 0.1, dx, dw)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_no_rows_set_dw_to_zero_and_negative_weights_count(nb, torch, dtype):
+    c = Case(torch, 65, 40, 260, dtype, seed=14)
+    _, stats = c.forward(nb)
+    c.weight[::2] *= -3.0
+    c.check_backward(stats, 0.5, *c.backward(nb, stats, 0.5))
+    c.check_backward(stats, -0.5, *c.backward(nb, stats, -0.5))
+    # grad_scale 0: zeros.
+    dx, dw = c.backward(nb, stats, 0.0)
+    assert (dx == 0).all() and (dw == 0).all()
+    none = Case(torch, 1, 40, 260, dtype, seed=15)
+    none.rows = 0
+    none.x, none.targets, none.weight = none.x[:0], none.targets[:0], None
+    _, dw = none.backward(nb, torch.zeros(0, 2, device="cuda"), want_dx=False)
+    assert (dw == 0).all()
+
+
+def test_f32_factors_far_apart(nb, torch):
+    """x and w whose products are ordinary, and whose sizes are the ends of f32's range."""
+    for rows in (40, 300):
+        c = Case(torch, rows, 96, 5000, "f32", seed=16)
+        for scale in (1e32, 1e-32):
+            c.x.mul_(scale)
+            c.w.div_(scale)
+            c.check_forward(*c.forward(nb))
+            c.x.div_(scale)
+            c.w.mul_(scale)
+        # Rows of very different sizes.
+        c.x[::2] *= 1e-12
+        c.w[::3] *= 1e-9
+        c.check_forward(*c.forward(nb))
+
+
+def test_two_host_threads_at_once(nb, torch):
+    import threading
+
+    cases = [Case(torch, 300 + 40 * i, 64 + 32 * i, 3000 + 500 * i, ["f32", "f16", "bf16", "bf16"][i], ignored=0.1, seed=40 + i)
+             for i in range(4)]
+    want = []
+    for c in cases:
+        loss, stats = c.forward(nb)
+        want.append((loss, stats, *c.backward(nb, stats, 0.1)))
+    rooms = [(c.workspace(nb, False), c.workspace(nb, True)) for c in cases]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            for _ in range(20):
+                with torch.cuda.stream(st):
+                    loss, stats = cases[i].forward(nb, rooms[i][0])
+                    got[i] = (loss, stats, *cases[i].backward(nb, stats, 0.1, room=rooms[i][1]))
+            st.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_a_training_step_end_to_end(nb, torch):
+    """Hidden rows, loss, gradients, a clipped AdamW step of the vocabulary matrix and its
+    16-bit copy, which the next loss reads: as a training program runs them, beside the
+    same steps in 64 bits with the copy rounded where the program rounds it."""
+    rows, d, V = 256, 64, 500
+    c = Case(torch, rows, d, V, "bf16", ignored=0.1, seed=50, weights=False)
+    val = c.w.float().clone()
+    w = val.to(torch.bfloat16)
+    c.w = w
+    dw = torch.zeros(V, d, device="cuda")
+    m, v = torch.zeros_like(dw), torch.zeros_like(dw)
+    norm = torch.zeros(1, device="cuda")
+    plan = nb.train.AdamwMany([nb.train.AdamwTensor(val=val.data_ptr(), grad=dw.data_ptr(), m=m.data_ptr(), v=v.data_ptr(),
+                                                    copy=w.data_ptr(), n=V * d, copy_dtype=2)])
+    n = int(c.live.sum())
+    v64, m64, s64 = val.double().clone(), m.double(), v.double()
+    for t in range(1, 6):
+        loss, stats = c.forward(nb)
+        c.check_forward(loss, stats)
+        dx, _ = c.backward(nb, stats, 1 / n, dw_dtype="f32", dw=dw.zero_())
+        c.check_backward(stats, 1 / n, dx, dw)
+        g = dw.double()
+        plan.step(lr=1e-2, t=t, max_norm=0.05, norm=norm.data_ptr())
+        g = g * min(1.0, 0.05 / float(g.norm()))
+        m64, s64 = 0.9 * m64 + 0.1 * g, 0.95 * s64 + 0.05 * g * g
+        v64 = v64 - 1e-2 * (m64 / (1 - 0.9**t)) / (torch.sqrt(s64 / (1 - 0.95**t)) + 1e-8)
+        # Five steps of at most lr each, 16 U of each, and the values' rounding; 0.9 and 0.95 are
+        # taken as f32, 2^-25 of them, which the corrections magnify by 1 / (1 - b) at most.
+        assert (val.double() - v64).abs().max() <= t * (1e-2 * 64 * U + U * float(val.abs().max()))
+        assert torch.equal(w, val.to(torch.bfloat16))
+
+
 def test_host_form_and_python_mirror(nb):
     rng = np.random.default_rng(0)
     x, w = rng.standard_normal((30, 50), np.float32), rng.standard_normal((90, 50), np.float32) * 0.3
