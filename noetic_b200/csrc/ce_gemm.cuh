@@ -72,7 +72,7 @@ struct Gemm {
     int64_t part_ld;
     float *zt;
     const uint32_t *target;  // of each row that counts
-    // GRAD: G goes out through mapC0, its second part through mapC1
+    // GRAD: G's parts go out through Products::c
     const float2 *stats;     // of each row that counts
     const float *weight;     // of each row that counts
     int col0;                // the piece's first token
@@ -210,8 +210,11 @@ struct Item {
 };
 
 struct Walk {
-    int mt, nt, total, kblocks, items;
-    __device__ __forceinline__ Walk(const Gemm &p, int M, int K) {
+    int mt, nt, total, kblocks, items, M, K;
+    __device__ __forceinline__ Walk() : mt(0), nt(0), total(0), kblocks(0), items(0), M(0), K(0) {}
+    __device__ __forceinline__ Walk(const Gemm &p, int live) {
+        M = p.live_dim == 0 ? live : p.M;
+        K = p.live_dim == 1 ? live : p.K;
         mt = (M + TM - 1) / TM;
         nt = (p.N + TN - 1) / TN;
         kblocks = (K + BK - 1) / BK;
@@ -236,6 +239,60 @@ struct Walk {
         }
         return it;
     }
+};
+
+// How the items of two products share the pairs, so that a last round of the one is
+// filled up with the other (dx 128 tiles of 256 K-blocks and dw 256 of 128 over 74
+// pairs: 896 K-blocks to a pair where each alone leaves 512 + 512).  The first's go
+// round robin; the second's to the pairs that have less, until all reach one level.
+// Pairs run the second's items in one order, so that neighbours share their operands.
+struct Deal {
+    int items[2], pairs, more;  // `more`: pairs that have one item of the first product more than the rest
+    int n[2];                   // of the second, for those pairs and for the rest
+    __host__ __device__ Deal(int items0, int cost0, int items1, int cost1, int pairs_) : pairs(pairs_) {
+        items[0] = items0;
+        items[1] = items1;
+        more = items0 % pairs;
+        const int q = items0 / pairs;
+        const long high = (long)(q + 1) * cost0, low = (long)q * cost0;
+        n[0] = n[1] = 0;
+        // The least level that has room for all; from one step of a class to the next.
+        long level = ((long)items0 * cost0 + (long)items1 * cost1 + pairs - 1) / pairs;
+        for (;;) {
+            n[0] = level > high ? (int)((level - high) / cost1) : 0;
+            n[1] = level > low ? (int)((level - low) / cost1) : 0;
+            if ((long)more * n[0] + (long)(pairs - more) * n[1] >= items1) break;
+            const long a = high + (long)(n[0] + 1) * cost1, b = low + (long)(n[1] + 1) * cost1;
+            level = more && a < b ? a : b;
+        }
+        if (n[1] < n[0]) n[1] = n[0];
+    }
+    // Item number i of a pair: the product and the item of it; false where there is none.
+    __host__ __device__ bool at(int pair, int i, int &which, int &item) const {
+        const int mine = items[0] / pairs + (pair < more);
+        which = i >= mine;
+        if (!which) {
+            item = i * pairs + pair;
+            return true;
+        }
+        const int s = i - mine, extra = n[1] - n[0];  // (first the pairs that have less of the first product)
+        if (pair < more) {
+            if (s >= n[0]) return false;
+            item = extra * (pairs - more) + s * pairs + pair;
+        } else {
+            if (s >= n[1]) return false;
+            item = s < extra ? s * (pairs - more) + pair - more : extra * (pairs - more) + (s - extra) * pairs + pair;
+        }
+        return item < items[1];
+    }
+};
+
+// What a launch computes: one product (the first), or in STORE two: dx, whose A is
+// K-major, and dw, whose A is MN-major (either can be empty).
+struct Products {
+    alignas(64) CUtensorMap a[2][2], b[2][2], c[2];  // [product][part]; c: G's parts
+    Gemm g[2];
+    int cost[2];  // K-blocks of an item, and what its end takes
 };
 
 // ---------------------------------------------------------------- epilogues
@@ -485,11 +542,9 @@ __device__ __forceinline__ void fewer_registers() {
 
 // T: the parts' type.  SCALED: f32 inputs, taken as two scaled f16 parts.  LONG:
 // chains of a few K-blocks, added up in registers.
-template <int MODE, class T, bool SCALED, bool LONG, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
-       const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1,
-       const __grid_constant__ CUtensorMap mapC0, const __grid_constant__ CUtensorMap mapC1, const __grid_constant__ Gemm p) {
+template <int MODE, class T, bool SCALED, bool LONG>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(const __grid_constant__ Products ps) {
+    constexpr bool B_MN = MODE == STORE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *boxes = smem + STAGES * STAGE_BYTES;
@@ -511,8 +566,8 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             mbar_init(acc_empty0 + 8 * b, 2 * EPI_WARPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&mapA0) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&mapB0) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&ps.a[0][0]) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&ps.b[0][0]) : "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -527,13 +582,16 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
     const uint32_t tmem = *tmem_slot;
     pdl_trigger();
     pdl_wait();  // (what the kernels before left is read from here on)
-    const int live = (int)p.head->live;
-    const int M = p.live_dim == 0 ? live : p.M, K = p.live_dim == 1 ? live : p.K;
-    const Walk walk(p, M, K);
-    const int low = SCALED ? 2 * walk.kblocks : 0;
+    Head *const head = ps.g[0].head;
+    const int live = (int)head->live;
+    const Walk walk0(ps.g[0], live), walk1 = MODE == STORE ? Walk(ps.g[1], live) : Walk();
+    const Deal deal(walk0.items, ps.cost[0], walk1.items, ps.cost[1], n_pairs);
+    // The pair's item number i.
+    int which = 0, item = 0;
+    auto next = [&](int i) { return deal.at(pair, i, which, item); };
     constexpr int CHAIN = chain_blocks(SCALED && MODE != STORE);
     // A wait that ran out ends the role that waited; the others' waits on it run out too.
-    auto give_up = [&](uint32_t code) { atomicExch(&p.head->err, code); };
+    auto give_up = [&](uint32_t code) { atomicExch(&head->err, code); };
 
     if (warp < 4) {
         if constexpr (LONG) fewer_registers<REGS_FEW>();
@@ -543,8 +601,10 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             uint32_t phase = 0;
             bool fine = true;
             const uint32_t leader_full = at_leader(full0), ring = smem_u32(smem);
-            for (int i = pair; fine && i < walk.items; i += n_pairs) {
-                const Item it = walk.at(p, i);
+            for (int i = 0; fine && next(i); ++i) {
+                const Gemm &p = ps.g[which];
+                const Walk walk = MODE == STORE && which ? walk1 : walk0;
+                const Item it = walk.at(p, item);
                 const int m0 = it.tm * TM + (int)rank * 128, n0 = it.tn * TN + (int)rank * 128;
                 int seg = it.k0 / max(1, walk.kblocks), x = (it.k0 - seg * walk.kblocks) * BK;
                 for (int k = it.k0; k < it.k1; ++k) {
@@ -556,9 +616,9 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
                     }
                     if (one) {
                         const uint32_t to = ring + stage * STAGE_BYTES, bar = leader_full + 8 * stage;
-                        const CUtensorMap *ma = (p.sa >> seg) & 1 ? &mapA1 : &mapA0, *mb = (p.sb >> seg) & 1 ? &mapB1 : &mapB0;
+                        const CUtensorMap *ma = &ps.a[which][(p.sa >> seg) & 1], *mb = &ps.b[which][(p.sb >> seg) & 1];
                         if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * STAGE_BYTES);
-                        if (A_MN) {
+                        if (MODE == STORE && which) {
                             tma_load(to, ma, bar, m0, x);
                             tma_load(to + OPERAND_BYTES / 2, ma, bar, m0 + 64, x);
                         } else {
@@ -574,7 +634,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
                     ++issued;
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                     x += BK;
-                    if (x >= K) x = 0, ++seg;
+                    if (x >= walk.K) x = 0, ++seg;
                 }
             }
             // A stage's copies have landed once its MMAs are done: wait for the last
@@ -592,9 +652,16 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             int stage = 0, n = 0;
             uint32_t phase = 0;
             bool fine = true;
-            const uint64_t da0 = smem_desc<A_MN>(smem_u32(smem)), db0 = smem_desc<B_MN>(smem_u32(smem) + OPERAND_BYTES);
-            for (int i = pair; fine && i < walk.items; i += n_pairs) {
-                const Item it = walk.at(p, i);
+            const uint64_t db0 = smem_desc<B_MN>(smem_u32(smem) + OPERAND_BYTES);
+            for (int i = 0; fine && next(i); ++i) {
+                const Gemm &p = ps.g[which];
+                const Walk walk = MODE == STORE && which ? walk1 : walk0;
+                const Item it = walk.at(p, item);
+                const int low = SCALED ? 2 * walk.kblocks : 0;
+                const bool a_mn = MODE == STORE && which;
+                const uint64_t da0 = a_mn ? smem_desc<true>(smem_u32(smem)) : smem_desc<false>(smem_u32(smem));
+                const uint64_t a_step = a_mn ? k_step<true>() : k_step<false>();
+                const uint32_t idesc = p.idesc;
                 for (int k = it.k0;;) {
                     const int end = LONG ? chain_end<CHAIN>(k, it.k1, low) : it.k1, b = n & 1;
                     fine = mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1));
@@ -618,7 +685,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
                             const uint64_t da = da0 + (uint64_t)(stage * (STAGE_BYTES >> 4)), db = db0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
 #pragma unroll
                             for (int kk = 0; kk < BK / 16; ++kk)
-                                mma(d, da + kk * k_step<A_MN>(), db + kk * k_step<B_MN>(), p.idesc, kk ? 1u : more);
+                                mma(d, da + kk * a_step, db + kk * k_step<B_MN>(), idesc, kk ? 1u : more);
                             mma_commit(empty0 + 8 * stage);
                         }
                         more = 1;
@@ -634,7 +701,7 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
         if constexpr (LONG) more_registers<REGS_MANY>();
         const int q = warp & 3, half = (warp - 4) >> 2;
         const uint32_t leader_empty = at_leader(acc_empty0);
-        const float factor = MODE == STORE ? out_factor(p) : 1.0f;
+        const float factor0 = MODE == STORE ? out_factor(ps.g[0]) : 1.0f, factor1 = MODE == STORE ? out_factor(ps.g[1]) : 1.0f;
         int n = 0;
         // The next accumulator: wait for it, or give it back.
         auto take = [&]() -> bool {
@@ -656,10 +723,13 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
         };
         const uint32_t mine = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
         bool fine = true;
-        for (int i = pair; i < walk.items; i += n_pairs) {
+        for (int i = 0; next(i); ++i) {
             // (After a wait that ran out, sums become NaN: this item's and those that follow.)
             if (MODE != STORE && !fine) break;
-            const Item it = walk.at(p, i);
+            const Gemm &p = ps.g[which];
+            const Walk walk = MODE == STORE && which ? walk1 : walk0;
+            const Item it = walk.at(p, item);
+            const int low = SCALED ? 2 * walk.kblocks : 0;
             const int row = it.tm * TM + (int)rank * 128 + q * 32 + lane, col = it.tn * TN + half * 128;
             auto whole = [&](auto &&e) {
                 if (MODE == STORE && !fine) return;
@@ -707,9 +777,9 @@ gemm_k(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtens
             if constexpr (MODE == ROWS)
                 whole(RowsEpilogue<SCALED>(p, row, live, col, 2 * it.tn + half));
             else if constexpr (MODE == GRAD)
-                whole(GradEpilogue<T, SCALED>(p, &mapC0, &mapC1, boxes + (warp - 4) * BOX_BYTES, row, live, col));
+                whole(GradEpilogue<T, SCALED>(p, &ps.c[0], &ps.c[1], boxes + (warp - 4) * BOX_BYTES, row, live, col));
             else {
-                StoreEpilogue<SCALED> e(p, boxes + (warp - 4) * BOX_BYTES, it.k1 > it.k0, row, M, col, it.split, factor);
+                StoreEpilogue<SCALED> e(p, boxes + (warp - 4) * BOX_BYTES, it.k1 > it.k0, row, walk.M, col, it.split, which ? factor1 : factor0);
                 whole(e);
                 if (!fine) {
                     float v[64];

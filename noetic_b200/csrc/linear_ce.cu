@@ -460,10 +460,8 @@ __global__ void __launch_bounds__(256) ce_lay_out_k(Rows x, Rows w, int d, int64
 
 // The sums of a product whose K was split, in their order, rounded on the way out.
 template <class T>
-__global__ void __launch_bounds__(256) ce_reduce_k(Gemm p, int rows_max, int splits) {
-    pdl_trigger();
-    pdl_wait();
-    const int rows = p.live_dim == 0 ? (int)p.head->live : rows_max;
+__device__ __forceinline__ void reduce(const Gemm &p, int splits) {
+    const int rows = p.live_dim == 0 ? (int)p.head->live : p.M;
     const float factor = ce::out_factor(p);
     const int64_t n = (int64_t)rows * p.ld_acc / 4;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -482,6 +480,13 @@ __global__ void __launch_bounds__(256) ce_reduce_k(Gemm p, int rows_max, int spl
         for (int j = 0; j < 4; ++j)
             if (col + j < p.n_valid) o[j] = from_f32<T>(p.out_add ? f[j] + to_f32(o[j]) : f[j]);
     }
+}
+template <class T, class W>
+__global__ void __launch_bounds__(256) ce_reduce_k(Gemm x, int x_splits, Gemm w, int w_splits) {
+    pdl_trigger();
+    pdl_wait();
+    if (x_splits) reduce<T>(x, x_splits);
+    if (w_splits) reduce<W>(w, w_splits);
 }
 
 // ---------------------------------------------------------------- host
@@ -524,18 +529,27 @@ struct Plan {
            dx = 0, dw = 0, bytes = 0;
 };
 
-// Pieces of K for a product of few tiles, of 8 K-blocks at least: the number that
-// needs the fewest rounds of the pairs, where each piece more costs its sums' way to
-// memory and back (about 16 K-blocks' time).
-int pick_splits(int64_t tiles, int64_t kblocks, int pairs) {
-    int best = 1;
+// An item's time in K-blocks: its own, or its sums' way out, which the next item's
+// K-blocks cover; and a piece's sums on their way to memory and back.
+constexpr int STORE_COST = 24, SPLIT_COST = 16;
+int item_cost(int64_t kblocks, bool split) { return (int)std::max<int64_t>(kblocks, STORE_COST) + 4 + (split ? SPLIT_COST : 0); }
+
+// Pieces of K for dx and dw, of 8 K-blocks at least: those that end first where the
+// two share the pairs (ce::Deal).
+void pick_splits(int64_t tx, int64_t kx, int64_t tw, int64_t kw, int pairs, int &sx, int &sw) {
+    static const int tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
     double least = 1e300;
-    for (int s = 1; s <= 64 && kblocks / s >= 8; ++s) {
-        const double rounds = (double)((tiles * s + pairs - 1) / pairs);
-        const double cost = rounds * ((double)kblocks / s) + (s > 1 ? 16.0 * rounds : 0.0);
-        if (cost < least * 0.97) least = cost, best = s;
-    }
-    return best;
+    sx = sw = 1;
+    for (const int i : tries)
+        for (const int j : tries) {
+            if ((i > 1 && (kx / i < 8 || tx * i > 4 * pairs)) || (j > 1 && (kw / j < 8 || tw * j > 4 * pairs))) continue;
+            const int cx = item_cost((kx + i - 1) / i, i > 1), cw = item_cost((kw + j - 1) / j, j > 1);
+            const ce::Deal d((int)(tx * i), cx, (int)(tw * j), cw, pairs);
+            const double q = (double)(tx * i / pairs);
+            const double a = d.more ? (q + 1) * cx + (double)d.n[0] * cw : 0.0, b = q * cx + (double)d.n[1] * cw;
+            const double cost = std::max(a, b);
+            if (cost < least * 0.97) least = cost, sx = i, sw = j;
+        }
 }
 
 // Whether the forward call takes the few rows' kernel: w's rows in whole 16-byte units,
@@ -605,8 +619,7 @@ Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int
     p.ld_acc = (int64_t)round_up((size_t)width, ce::TN);
     const int pairs = 74;
     const int64_t nt = p.ld_acc / ce::TN, segs = p.split ? 3 : 1;
-    p.dx_splits = pick_splits(p.mp / ce::TM * nt, p.ldg / ce::BK * segs, pairs);
-    p.dw_splits = pick_splits(p.ldg / ce::TN * nt, p.mp / ce::BK * segs, pairs);
+    pick_splits(p.mp / ce::TM * nt, p.ldg / ce::BK * segs, p.ldg / ce::TN * nt, p.mp / ce::BK * segs, pairs, p.dx_splits, p.dw_splits);
     if (p.dx_splits > 1 || p.piece < vocab) p.dx = room((size_t)p.dx_splits * p.mp * p.ld_acc * 4);
     if (p.dw_splits > 1) p.dw = room((size_t)p.dw_splits * p.ldg * p.ld_acc * 4);
     return p;
@@ -617,10 +630,6 @@ uint32_t instruction(bool bf16, bool a_mn, bool b_mn) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
            ((uint32_t)(ce::TN >> 3) << 17) | ((uint32_t)(ce::TM >> 4) << 24);
 }
-
-struct Maps {
-    CUtensorMap a[2], b[2], c[2];
-};
 
 // T: the type of x and w; P: that of the parts the products take.
 template <class T, class P>
@@ -652,14 +661,15 @@ struct Call {
     void go(void (*k)(K...), dim3 grid, int threads, int shared, A &&...args) {
         if (err == cudaSuccess) err = pdl_launch(k, grid, dim3((unsigned)threads), (size_t)shared, st, args...);
     }
-    template <int MODE, bool LONG, bool A_MN, bool B_MN>
-    void product(const Maps &m, const Gemm &g) {
-        auto *k = ce::gemm_k<MODE, P, SPLIT, LONG, A_MN, B_MN>;
+    template <int MODE, bool LONG>
+    void product(const ce::Products &ps) {
+        auto *k = ce::gemm_k<MODE, P, SPLIT, LONG>;
         constexpr int shared = ce::smem_bytes(MODE != ce::ROWS);
         if (err == cudaSuccess) err = allow_shared(k, shared);
-        const int64_t items = (int64_t)((g.M + ce::TM - 1) / ce::TM) * ((g.N + ce::TN - 1) / ce::TN) * g.splits;
+        int64_t items = 0;
+        for (const Gemm &g : ps.g) items += (int64_t)((g.M + ce::TM - 1) / ce::TM) * ((g.N + ce::TN - 1) / ce::TN) * g.splits;
         const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(sms / 2, items));
-        go(k, 2 * pairs, ce::THREADS, shared, m.a[0], m.a[1], m.b[0], m.b[1], m.c[0], m.c[1], g);
+        go(k, 2 * pairs, ce::THREADS, shared, ps);
     }
     template <class U>
     U *at(size_t o) const {
@@ -735,36 +745,34 @@ struct Call {
     cudaError_t forward() {
         if (p.few) return a.rows >= 8 ? few<8>() : a.rows > 2 ? few<4>() : a.rows == 2 ? few<2>() : few<1>();
         begin(false);
-        Maps m{};
-        if (!map_x(m.a, 128) || !map_w(m.b, 128)) return cudaErrorInvalidValue;
-        Gemm g = gemm((int)a.rows, a.vocab, a.width, 0, false, false, 1);
+        ce::Products ps{};
+        if (!map_x(ps.a[0], 128) || !map_w(ps.b[0], 128)) return cudaErrorInvalidValue;
+        Gemm &g = ps.g[0];
+        g = gemm((int)a.rows, a.vocab, a.width, 0, false, false, 1);
+        ps.cost[0] = ps.cost[1] = 1;
         g.m_fast = 1;
         if (SPLIT) g.x_scale = scales, g.w_scale = scales + p.mp;
         g.part = at<float2>(p.part);
         g.part_ld = p.mp;
         g.zt = at<float>(p.zt);
         g.target = ix.target;
-        product<ce::ROWS, true, false, false>(m, g);
+        product<ce::ROWS, true>(ps);
         go(ce_join_k, (unsigned)((a.rows + 7) / 8), 256, 0, a, ix.head, ix.row_of, g.part, p.mp, g.zt, p.tiles);
         return err;
     }
 
-    template <class O>
-    void reduce(const Gemm &g, int rows, int splits) {
-        const int64_t n = (int64_t)rows * g.ld_acc / 4;
-        go(ce_reduce_k<O>, (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, (int64_t)sms * 8)), 256, 0, g, rows, splits);
-    }
-
     cudaError_t backward() {
         begin(true);
-        Maps mg{}, mx{}, mw{};
-        if (!map_x(mg.a, 128) || !map_w(mg.b, 128) || !map_g(mg.c, 32) || !map_g(mx.a, 128) || !map_w(mx.b, 64) || !map_g(mw.a, 64) || !map_x(mw.b, 64))
+        ce::Products pg{}, ps{};
+        if (!map_x(pg.a[0], 128) || !map_w(pg.b[0], 128) || !map_g(pg.c, 32) || !map_g(ps.a[0], 128) || !map_w(ps.b[0], 64) ||
+            !map_g(ps.a[1], 64) || !map_x(ps.b[1], 64))
             return cudaErrorInvalidValue;
         const float g_scale = BF16 ? 1.0f : G_SCALE;
         for (int v0 = 0; v0 < a.vocab; v0 += p.piece) {
             const int n = std::min(p.piece, a.vocab - v0);
             const bool last = v0 + n == a.vocab;
-            Gemm g = gemm((int)a.rows, n, a.width, 0, false, false, 1);
+            Gemm &g = pg.g[0];
+            g = gemm((int)a.rows, n, a.width, 0, false, false, 1);
             g.m_fast = 1;
             g.b_row0 = v0;
             if (SPLIT) g.x_scale = scales, g.w_scale = scales + p.mp;
@@ -773,44 +781,45 @@ struct Call {
             g.weight = ix.weight;
             g.col0 = v0;
             g.g_scale = g_scale;
-            if (a.rows) product<ce::GRAD, true, false, false>(mg, g);
-            if (a.dx) {
-                Gemm c = gemm((int)a.rows, a.width, n, 0, false, true, p.dx_splits);
-                c.b_row0 = v0;
-                if (SPLIT) c.w_scale = scales + p.mp;
-                c.acc = p.dx ? at<float>(p.dx) : nullptr;
-                c.ld_acc = p.ld_acc;
-                c.acc_split = p.mp * p.ld_acc;
-                c.add = v0 != 0;
-                c.keep = !last || p.dx_splits > 1;
-                c.out = a.dx;
-                c.out_ld = a.dx_stride;
-                c.out_dtype = a.dtype;
-                c.out_row = ix.row_of;
-                c.out_scale = a.grad_scale / g_scale;
-                product<ce::STORE, SPLIT, false, true>(mx, c);
-                if (last && p.dx_splits > 1) reduce<T>(c, (int)a.rows, p.dx_splits);
-            }
-            if (a.dw) {
-                Gemm c = gemm(n, a.width, (int)a.rows, 1, true, true, p.dw_splits);
-                if (SPLIT) c.x_scale = scales;
-                c.acc = p.dw ? at<float>(p.dw) : nullptr;
-                c.ld_acc = p.ld_acc;
-                c.acc_split = p.ldg * p.ld_acc;
-                c.keep = p.dw_splits > 1;
-                c.out = a.dw;
-                c.out_ld = a.dw_stride;
-                c.out_row0 = v0;
-                c.out_dtype = a.dw_dtype;
-                c.out_add = a.accumulate;
-                c.out_scale = a.grad_scale / g_scale;
-                product<ce::STORE, SPLIT, true, true>(mw, c);
-                if (p.dw_splits > 1) {
-                    if (a.dw_dtype == NK_F32)
-                        reduce<float>(c, n, p.dw_splits);
-                    else
-                        reduce<T>(c, n, p.dw_splits);
-                }
+            pg.cost[0] = pg.cost[1] = 1;
+            if (a.rows) product<ce::GRAD, true>(pg);
+            Gemm &x = ps.g[0], &w = ps.g[1];
+            x = gemm(a.dx ? (int)a.rows : 0, a.width, n, a.dx ? 0 : 2, false, true, p.dx_splits);
+            x.b_row0 = v0;
+            if (SPLIT) x.w_scale = scales + p.mp;
+            x.acc = p.dx ? at<float>(p.dx) : nullptr;
+            x.ld_acc = p.ld_acc;
+            x.acc_split = p.mp * p.ld_acc;
+            x.add = v0 != 0;
+            x.keep = !last || p.dx_splits > 1;
+            x.out = a.dx;
+            x.out_ld = a.dx_stride;
+            x.out_dtype = a.dtype;
+            x.out_row = ix.row_of;
+            x.out_scale = a.grad_scale / g_scale;
+            w = gemm(a.dw ? n : 0, a.width, (int)a.rows, 1, true, true, p.dw_splits);
+            if (SPLIT) w.x_scale = scales;
+            w.acc = p.dw ? at<float>(p.dw) : nullptr;
+            w.ld_acc = p.ld_acc;
+            w.acc_split = p.ldg * p.ld_acc;
+            w.keep = p.dw_splits > 1;
+            w.out = a.dw;
+            w.out_ld = a.dw_stride;
+            w.out_row0 = v0;
+            w.out_dtype = a.dw_dtype;
+            w.out_add = a.accumulate;
+            w.out_scale = a.grad_scale / g_scale;
+            ps.cost[0] = item_cost(x.kps, p.dx_splits > 1);
+            ps.cost[1] = item_cost(w.kps, p.dw_splits > 1);
+            product<ce::STORE, SPLIT>(ps);
+            const int sx = a.dx && last && p.dx_splits > 1 ? p.dx_splits : 0, sw = a.dw && p.dw_splits > 1 ? p.dw_splits : 0;
+            if (sx || sw) {
+                const int64_t most = std::max<int64_t>(sx ? a.rows : 0, sw ? n : 0) * p.ld_acc / 4;
+                const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((most + 255) / 256, (int64_t)sms * 8));
+                if (a.dw_dtype == NK_F32)
+                    go(ce_reduce_k<T, float>, grid, 256, 0, x, sx, w, sw);
+                else
+                    go(ce_reduce_k<T, T>, grid, 256, 0, x, sx, w, sw);
             }
         }
         return err;
