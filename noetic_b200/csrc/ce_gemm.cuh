@@ -40,7 +40,7 @@ constexpr uint64_t WAIT_NS = 1000000000ull;
 // (f32: the low parts' products come first, as one chain: they are 2^-11 of the sum.)
 // Logits of f32 rows get the shortest chains: an error of the logit is one of p, and a
 // sure token's gradient is 1 - p.
-constexpr int chain_blocks(bool f32_logits) { return f32_logits ? 2 : 8; }
+constexpr int chain_blocks(bool f32_logits) { return f32_logits ? 4 : 8; }
 constexpr int REGS_FEW = 64, REGS_MANY = 216;  // 4 warps and 8 of 32: within 384 * 168
 
 // What the first kernel of a call finds out, for the others (the workspace's head).
@@ -425,24 +425,16 @@ struct GradEpilogue {
     __device__ __forceinline__ void end() const {}
 };
 
-// Four neighbouring columns of an output row at o, of which `n` exist; vec: they do, and
-// o is a multiple of their size.
-template <class T>
-__device__ __forceinline__ void store_out(T *o, const float4 &x, bool add, bool vec, int n) {
-    const float v[4] = {x.x, x.y, x.z, x.w};
-    struct __align__(4 * sizeof(T)) Four {
-        T e[4];
+// N neighbouring elements of an output row at o, which is a multiple of their size.
+template <class T, int N>
+__device__ __forceinline__ void store_out(T *o, const float (&v)[N], bool add) {
+    struct __align__(N * sizeof(T)) Some {
+        T e[N];
     } q;
-    if (vec) {
-        if (add) q = *reinterpret_cast<const Four *>(o);
+    if (add) q = *reinterpret_cast<const Some *>(o);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q.e[i] = from_f32<T>(add ? v[i] + to_f32(q.e[i]) : v[i]);
-        *reinterpret_cast<Four *>(o) = q;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < n) o[i] = from_f32<T>(add ? v[i] + to_f32(o[i]) : v[i]);
-    }
+    for (int i = 0; i < N; ++i) q.e[i] = from_f32<T>(add ? v[i] + to_f32(q.e[i]) : v[i]);
+    *reinterpret_cast<Some *>(o) = q;
 }
 
 __device__ __forceinline__ float out_factor(const Gemm &p) {
@@ -462,30 +454,74 @@ struct StoreEpilogue {
     const Gemm &p;
     float *const box;
     const bool any;  // K has anything: else the accumulator holds nothing
-    const int col, rows;  // first column; how many of the warp's 32 rows exist
+    const int col, row0, rows;  // first column; the warp's first row; how many of its 32 rows exist
     const float factor;
     float *const acc;
     int64_t out[8];  // where the lane's rows start in the output, in elements
     __device__ __forceinline__ StoreEpilogue(const Gemm &g, uint8_t *to, bool has, int r, int n, int c, int split, float f)
-        : p(g), box((float *)to), any(has), col(c), rows(n - (r - (int)(threadIdx.x & 31))), factor(f),
+        : p(g), box((float *)to), any(has), col(c), row0(r - (int)(threadIdx.x & 31)), rows(n - row0), factor(f),
           acc(g.acc ? g.acc + (int64_t)split * g.acc_split + (int64_t)(r - (int)(threadIdx.x & 31) + ((threadIdx.x & 31) >> 3)) * g.ld_acc + c
                     : nullptr) {
-        const int row0 = r - (int)(threadIdx.x & 31) + ((int)(threadIdx.x & 31) >> 3);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = min(row0 + 4 * i, n - 1);
-            out[i] = p.keep ? 0 : (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld;
-        }
+        for (int i = 0; i < 8; ++i) out[i] = p.keep ? 0 : start(((int)(threadIdx.x & 31) >> 3) + 4 * i);
     }
+    // Where the warp's row r starts in the output (beyond the last: as the last).
+    __device__ __forceinline__ int64_t start(int r) const {
+        const int row = row0 + max(min(r, rows - 1), -row0);
+        return (p.out_row ? (int64_t)p.out_row[row] : row + p.out_row0) * p.out_ld;
+    }
+    __device__ __forceinline__ float *at(int r, int c) const { return box + r * 32 + ((c >> 2) ^ (r & 7)) * 4 + (c & 3); }
+    // 32 columns from c on of the warp's rows, the lane's share of which is x.
     template <class T>
     __device__ __forceinline__ void write(const float4 (&x)[8], int c) const {
         const int lane = threadIdx.x & 31, left = p.n_valid - (col + c);
-        const bool vec = left >= 4 && (((uintptr_t)p.out | (uintptr_t)(p.out_ld * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
-        T *o = (T *)p.out + col + c;
+        const bool add = p.out_add != 0;
+        T *const o = (T *)p.out + col + c;
+        if (left >= 32 && (((uintptr_t)p.out | (uintptr_t)(p.out_ld * sizeof(T))) & (4 * sizeof(T) - 1)) == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if ((lane >> 3) + 4 * i < rows)
-                store_out<T>(o + out[i], make_float4(x[i].x * factor, x[i].y * factor, x[i].z * factor, x[i].w * factor), p.out_add != 0, vec, left);
+            for (int i = 0; i < 8; ++i)
+                if ((lane >> 3) + 4 * i < rows) {
+                    const float v[4] = {x[i].x * factor, x[i].y * factor, x[i].z * factor, x[i].w * factor};
+                    store_out<T, 4>(o + out[i] + (lane & 7) * 4, v, add);
+                }
+            return;
+        }
+        // Rows that start anywhere: through the box again, a row (of 16 bits: two rows, two
+        // elements to a lane from 4 bytes on) at a time, so that each sector is written once.
+        // (Four elements to a lane, one by one: 260 us of 65536 x 889 f16 where this takes ROWS_FIGURE.)
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = (lane >> 3) + 4 * i;
+            *reinterpret_cast<float4 *>(at(r, (lane & 7) * 4)) = make_float4(x[i].x * factor, x[i].y * factor, x[i].z * factor, x[i].w * factor);
+        }
+        __syncwarp();
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r) {
+                const float v[1] = {*at(r, lane)};
+                if (r < rows && lane < left) store_out<T, 1>(o + start(r) + lane, v, add);
+            }
+        } else {
+#pragma unroll 4
+            for (int r2 = 0; r2 < 16; ++r2) {
+                const int r = 2 * r2 + (lane >> 4), k = lane & 15;
+                T *const to = o + start(r);
+                const int odd = (int)((uintptr_t)to >> 1 & 1), first = 2 * k + odd, n = r < rows ? min(left, 32) : 0;
+                if (first + 1 < n) {
+                    const float v[2] = {*at(r, first), *at(r, first + 1)};
+                    store_out<T, 2>(to + first, v, add);
+                } else if (first < n) {
+                    const float v[1] = {*at(r, first)};
+                    store_out<T, 1>(to + first, v, add);
+                }
+                if (odd && k == 15 && n > 0) {
+                    const float v[1] = {*at(r, 0)};
+                    store_out<T, 1>(to, v, add);
+                }
+            }
+        }
+        __syncwarp();
     }
     __device__ __forceinline__ void some(int c0, float *v) {
         const int lane = threadIdx.x & 31;
@@ -519,11 +555,11 @@ struct StoreEpilogue {
                 for (int i = 0; i < 8; ++i)
                     if ((lane >> 3) + 4 * i < rows) *reinterpret_cast<float4 *>(a + (int64_t)(4 * i) * p.ld_acc) = x[i];
             } else if (F32 || p.out_dtype == 0) {
-                write<float>(x, cc);
+                write<float>(x, c);
             } else if (p.out_dtype == 1) {
-                write<__half>(x, cc);
+                write<__half>(x, c);
             } else {
-                write<__nv_bfloat16>(x, cc);
+                write<__nv_bfloat16>(x, c);
             }
         }
     }
@@ -752,7 +788,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
                             tmem_ld32(mine + (n & 1) * TN + c + 32, v + 32);
                             tmem_wait<64>(v);
 #pragma unroll
-                            for (int j = 0; j < 64; ++j) sum[c + j] += v[j];
+                            for (int j = 0; j < 64; j += 2) {
+                                const float2 t = add2(make_float2(sum[c + j], sum[c + j + 1]), make_float2(v[j], v[j + 1]));
+                                sum[c + j] = t.x;
+                                sum[c + j + 1] = t.y;
+                            }
                         }
                         give();
                     }

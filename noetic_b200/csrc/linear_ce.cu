@@ -368,32 +368,41 @@ __device__ __forceinline__ void lay_out_row(const Rows &j, const T *p, bool real
         // them than it touches), each shifted together with the next lane's.
         const uint32_t off = (uintptr_t)p & 15, units = (off + 2 * d + 15) / 16;
         const uint4 *from = reinterpret_cast<const uint4 *>((uintptr_t)p - off);
-        for (int i0 = 0; i0 < ld; i0 += 256) {
-            const uint32_t u = i0 / 8 + lane;
-            uint4 q = real && u < units ? from[u] : make_uint4(0, 0, 0, 0);
-            if (off) {  // (the warp's one row)
-                uint4 n;
-                n.x = __shfl_down_sync(0xffffffffu, q.x, 1);
-                n.y = __shfl_down_sync(0xffffffffu, q.y, 1);
-                n.z = __shfl_down_sync(0xffffffffu, q.z, 1);
-                n.w = __shfl_down_sync(0xffffffffu, q.w, 1);
-                if (lane == 31) n = real && u + 1 < units ? from[u + 1] : make_uint4(0, 0, 0, 0);
-                const uint32_t w[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
-                const uint32_t words = off / 4, bits = off % 4 * 8;
-                uint32_t x[5];
+        for (int i0 = 0; i0 < ld; i0 += 1024) {
+            uint4 q4[4];
 #pragma unroll
-                for (int e = 0; e < 5; ++e) x[e] = words == 0 ? w[e] : words == 1 ? w[e + 1] : words == 2 ? w[e + 2] : e < 5 ? w[min(e + 3, 7)] : 0u;
-                q = make_uint4(__funnelshift_r(x[0], x[1], bits), __funnelshift_r(x[1], x[2], bits), __funnelshift_r(x[2], x[3], bits),
-                               __funnelshift_r(x[3], x[4], bits));
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t u = i0 / 8 + 32 * k + lane;
+                q4[k] = real && u < units ? from[u] : make_uint4(0, 0, 0, 0);
             }
-            const int i = i0 + lane * 8;
-            if (i + 8 > d) {
-                T *e = reinterpret_cast<T *>(&q);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (i + j >= d) e[j] = from_f32<T>(0.0f);
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t u = i0 / 8 + 32 * k + lane;
+                uint4 q = q4[k];
+                if (off) {  // (the warp's one row)
+                    uint4 n;
+                    n.x = __shfl_down_sync(0xffffffffu, q.x, 1);
+                    n.y = __shfl_down_sync(0xffffffffu, q.y, 1);
+                    n.z = __shfl_down_sync(0xffffffffu, q.z, 1);
+                    n.w = __shfl_down_sync(0xffffffffu, q.w, 1);
+                    if (lane == 31) n = real && u + 1 < units ? from[u + 1] : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
+                    const uint32_t words = off / 4, bits = off % 4 * 8;
+                    uint32_t x[5];
+#pragma unroll
+                    for (int e = 0; e < 5; ++e) x[e] = words == 0 ? w[e] : words == 1 ? w[e + 1] : words == 2 ? w[e + 2] : w[min(e + 3, 7)];
+                    q = make_uint4(__funnelshift_r(x[0], x[1], bits), __funnelshift_r(x[1], x[2], bits), __funnelshift_r(x[2], x[3], bits),
+                                   __funnelshift_r(x[3], x[4], bits));
+                }
+                const int i = u * 8;
+                if (i + 8 > d) {
+                    T *e = reinterpret_cast<T *>(&q);
+#pragma unroll
+                    for (int t = 0; t < 8; ++t)
+                        if (i + t >= d) e[t] = from_f32<T>(0.0f);
+                }
+                if (i < ld) *reinterpret_cast<uint4 *>(o + i) = q;
             }
-            if (i < ld) *reinterpret_cast<uint4 *>(o + i) = q;
         }
     } else {
         __half *o = (__half *)j.dst + to * ld;
