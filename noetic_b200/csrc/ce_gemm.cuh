@@ -426,14 +426,14 @@ struct GradEpilogue {
 };
 
 // N neighbouring elements of an output row at o, which is a multiple of their size.
-template <class T, int N>
-__device__ __forceinline__ void store_out(T *o, const float (&v)[N], bool add) {
+template <class T, int N, bool ADD>
+__device__ __forceinline__ void store_out(T *o, const float (&v)[N]) {
     struct __align__(N * sizeof(T)) Some {
         T e[N];
     } q;
-    if (add) q = *reinterpret_cast<const Some *>(o);
+    if (ADD) q = *reinterpret_cast<const Some *>(o);
 #pragma unroll
-    for (int i = 0; i < N; ++i) q.e[i] = from_f32<T>(add ? v[i] + to_f32(q.e[i]) : v[i]);
+    for (int i = 0; i < N; ++i) q.e[i] = from_f32<T>(ADD ? v[i] + to_f32(q.e[i]) : v[i]);
     *reinterpret_cast<Some *>(o) = q;
 }
 
@@ -472,56 +472,42 @@ struct StoreEpilogue {
     }
     __device__ __forceinline__ float *at(int r, int c) const { return box + r * 32 + ((c >> 2) ^ (r & 7)) * 4 + (c & 3); }
     // 32 columns from c on of the warp's rows, the lane's share of which is x.
-    template <class T>
+    template <class T, bool ADD>
     __device__ __forceinline__ void write(const float4 (&x)[8], int c) const {
         const int lane = threadIdx.x & 31, left = p.n_valid - (col + c);
-        const bool add = p.out_add != 0;
         T *const o = (T *)p.out + col + c;
         if (left >= 32 && (((uintptr_t)p.out | (uintptr_t)(p.out_ld * sizeof(T))) & (4 * sizeof(T) - 1)) == 0) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if ((lane >> 3) + 4 * i < rows) {
                     const float v[4] = {x[i].x * factor, x[i].y * factor, x[i].z * factor, x[i].w * factor};
-                    store_out<T, 4>(o + out[i] + (lane & 7) * 4, v, add);
+                    store_out<T, 4, ADD>(o + out[i] + (lane & 7) * 4, v);
                 }
             return;
         }
-        // Rows that start anywhere: through the box again, a row (of 16 bits: two rows, two
-        // elements to a lane from 4 bytes on) at a time, so that each sector is written once.
-        // (Four elements to a lane, one by one: 260 us of 65536 x 889 f16 where this takes ROWS_FIGURE.)
+        // Rows that start anywhere: through the box again, a row at a time, an element to
+        // a lane.  (Pairs from 4 bytes on, with the odd ends apart, took 24 us a tile where
+        // this takes 14 and the aligned form 7.6, at 256 of K.)
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = (lane >> 3) + 4 * i;
-            *reinterpret_cast<float4 *>(at(r, (lane & 7) * 4)) = make_float4(x[i].x * factor, x[i].y * factor, x[i].z * factor, x[i].w * factor);
-        }
+        for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4 *>(at((lane >> 3) + 4 * i, (lane & 7) * 4)) = make_float4(x[i].x * factor, x[i].y * factor, x[i].z * factor, x[i].w * factor);
         __syncwarp();
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
+        if (lane < left) {
+#pragma unroll 8
+            for (int r = 0; r < min(rows, 32); ++r) {
                 const float v[1] = {*at(r, lane)};
-                if (r < rows && lane < left) store_out<T, 1>(o + start(r) + lane, v, add);
-            }
-        } else {
-#pragma unroll 4
-            for (int r2 = 0; r2 < 16; ++r2) {
-                const int r = 2 * r2 + (lane >> 4), k = lane & 15;
-                T *const to = o + start(r);
-                const int odd = (int)((uintptr_t)to >> 1 & 1), first = 2 * k + odd, n = r < rows ? min(left, 32) : 0;
-                if (first + 1 < n) {
-                    const float v[2] = {*at(r, first), *at(r, first + 1)};
-                    store_out<T, 2>(to + first, v, add);
-                } else if (first < n) {
-                    const float v[1] = {*at(r, first)};
-                    store_out<T, 1>(to + first, v, add);
-                }
-                if (odd && k == 15 && n > 0) {
-                    const float v[1] = {*at(r, 0)};
-                    store_out<T, 1>(to, v, add);
-                }
+                store_out<T, 1, ADD>(o + start(r) + lane, v);
             }
         }
         __syncwarp();
+    }
+    template <class T>
+    __device__ __forceinline__ void write(const float4 (&x)[8], int c) const {
+        if (p.out_add)
+            write<T, true>(x, c);
+        else
+            write<T, false>(x, c);
     }
     __device__ __forceinline__ void some(int c0, float *v) {
         const int lane = threadIdx.x & 31;
