@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256) adamw_norm_k(AdamwMany p, float grad_scal
         if (norm) *norm = all;
         if (max_norm > 0.0f) {
             const bool fine = isfinite(all);
-            p.clip[0] = all > max_norm ? grad_scale * __fdiv_rn(max_norm, all) : grad_scale;
+            p.clip[0] = all > max_norm ? __fmul_rn(grad_scale, __fmul_rn(max_norm, __frcp_rn(all))) : grad_scale;
             p.clip[1] = fine ? 1.0f : 0.0f;
             if (!fine && bad) *bad = 1u;
         }
@@ -217,11 +217,10 @@ __device__ __forceinline__ uint32_t to_e4m3(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
-// 448 / top, near enough to correctly rounded that hardly an element's place on the
-// grid of e4m3 moves by it.
+// 448 times the reciprocal of top (correctly rounded but for one in a million).
 __device__ __forceinline__ float grid_scale(float top) {
-    const float r = __fdividef(1.0f, top), k = E4M3_MAX * r;
-    return fmaf(fmaf(-k, top, E4M3_MAX), r, k);
+    const float r = __fdividef(1.0f, top);
+    return E4M3_MAX * fmaf(fmaf(-top, r, 1.0f), r, r);
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -243,11 +242,15 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
+// Two sums, each rounded, of products that are rounded: apart, since the assembler makes
+// one fma of a packed product and a packed sum.
+__device__ __forceinline__ float2 plus(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+
 // What a block's steps need of the call, worked out once a thread.
 struct Step8 {
     float c, b1, g1, b2, g2, inv_bc1, root_bc2, eps, lr, wd;
     __device__ __forceinline__ Step8(const AdamwParams &a, float factor)
-        : c(factor), b1(a.b1), g1((1.0f - a.b1) * factor), b2(a.b2), g2(1.0f - a.b2), inv_bc1(a.inv_bc1),
+        : c(factor), b1(a.b1), g1(1.0f - a.b1), b2(a.b2), g2(1.0f - a.b2), inv_bc1(a.inv_bc1),
           root_bc2(sqrtf(a.inv_bc2)), eps(fmaxf(a.eps, 1.1754944e-38f)), lr(a.lr), wd(a.wd) {}
 };
 
@@ -280,9 +283,13 @@ __device__ __forceinline__ float grad_of(const void *grad, int dtype, uint64_t i
 // and 128 + 4 l .. + 3, so the block's largest |m| and sqrt(v) are two shuffles'
 // reductions and nothing is read twice.  Correctly rounded roots and quotients, as
 // the 32-bit step has them, took 116 instructions an element and 2.4 TB/s; here one
-// root (a reciprocal root and Newton's step, within 2^-23) serves the update and the
-// moment, and the quotient is a product with a reciprocal: 2^-22 of an update, which
-// is below the rounding of val.
+// root (a reciprocal root and Newton's step, which rounds correctly but for one in a
+// million) serves the update and the moment, and the quotient is a product with a
+// reciprocal: 2^-22 of an update, which is below the rounding of val.  What the
+// moments are made of is rounded operation by operation, as in the 32-bit step: a
+// byte at the middle between two others then goes the same way wherever the formula
+// is computed, where an fma here sent one in a million the other way, and the next
+// step of such an element is an eighth longer or shorter.
 //
 // The careful form: short blocks, tensors that start off 16 bytes, elements that are
 // not finite or beyond the range of what is stored.
@@ -311,7 +318,6 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
     }
     bool ok = true;
     float top_m = 0.0f, top_r = 0.0f;
-    const float k1 = a.b1 * ms;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -321,8 +327,8 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
             const float gc = g[h][e] * a.c;
             const bool fine = fabsf(gc) < INFINITY && fabsf(pv[h][e]) < INFINITY;
             ok &= fine;
-            float mm = fmaf(mq, k1, g[h][e] * a.g1);
-            const float v1 = fmaf(a.b2 * r, r, (a.g2 * gc) * gc), vv = fminf(v1, V_MAX);
+            float mm = __fadd_rn(__fmul_rn(__fmul_rn(mq, ms), a.b1), __fmul_rn(gc, a.g1));
+            const float v1 = __fadd_rn(__fmul_rn(__fmul_rn(r, r), a.b2), __fmul_rn(__fmul_rn(gc, a.g2), gc)), vv = fminf(v1, V_MAX);
             // sqrt(vv); below 2^-126 (a gradient below 1e-18) it counts as 0.
             const float q = rsqrt_fast(vv);
             float u = vv * q;
@@ -379,7 +385,7 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
                                             float wd) {
     const int lane = threadIdx.x & 31;
     const float ms = st.scale[0], vs = st.scale[1];
-    const float2 k1 = both(a.b1 * ms), c = both(a.c), g1 = both(a.g1), b2 = both(-a.b2), g2 = both(-a.g2), zero = both(0.0f);
+    const float2 b1 = both(a.b1), c = both(a.c), g1 = both(a.g1), b2 = both(-a.b2), g2 = both(-a.g2), zero = both(0.0f);
     float2 pv[4], mv[4], root[4], strange = zero;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -403,8 +409,8 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
         for (int i = 0; i < 2; ++i) {
             const int o = 2 * h + i;
             const float2 r = mul2(from_e4m3(i ? vb >> 16 : vb & 0xFFFFu), both(vs)), gc = mul2(g[i], c);
-            mv[o] = fma2(from_e4m3(i ? mb >> 16 : mb & 0xFFFFu), k1, mul2(g[i], g1));
-            const float2 nv = fma2(mul2(b2, r), r, mul2(mul2(g2, gc), gc));  // -v'
+            mv[o] = plus(mul2(mul2(from_e4m3(i ? mb >> 16 : mb & 0xFFFFu), both(ms)), b1), mul2(gc, g1));
+            const float2 nv = plus(mul2(mul2(r, r), b2), mul2(mul2(gc, g2), gc));  // -v'
             strange = fma2(mv[o], zero, strange);
             strange = fma2(nv, zero, strange);
             strange = fma2(pv[o], zero, strange);

@@ -563,13 +563,17 @@ void pick_splits(int64_t tx, int64_t kx, int64_t tw, int64_t kw, int pairs, int 
 
 // Whether the forward call takes the few rows' kernel: w's rows in whole 16-byte units,
 // 8 of x within shared memory, and a product below what the other way's launches and
-// (f32) two more passes over w cost.  Measured (us, this and the other way):
-// FEW_FIGURES
+// (f32) its passes over w cost, about 12 us and 2.4 us a million elements of w where
+// the few rows' kernel makes 12.5 million products a us.  Measured (us, this and the
+// other way): f32 1 x 1024 x 32768 31 and 100, 16 rows 54 and 100, 32 rows 95 and 101,
+// 64 rows 168 and 101; 96 x 768 x 16384 99 and 45; 256 x 192 x 1024 13 and 26; 512 x
+// 512 x 1024 26 and 25; bf16 4 x 1024 x 32768 26 and 28, 8 rows 35 and 28; 256 x 192 x
+// 1024 13 and 18, 512 x 512 x 1024 29 and 18, 32 x 512 x 8192 17 and 18.
 bool few_rows(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride) {
     const int es = dtype == NK_F32 ? 4 : 2;
     if (((uintptr_t)w & 15) != 0 || w_stride * es % 16 != 0 || width > 4096 || rows > 4096) return false;
     const double products = (double)rows * width * vocab;
-    return dtype == NK_F32 ? products <= 6e8 : rows <= 4 || products <= 1e8;
+    return dtype == NK_F32 ? products <= 1.5e8 + 30.0 * width * vocab : rows <= 4 || products <= 1e8;
 }
 int few_blocks(int64_t rows, int vocab) {
     const int r = rows >= 8 ? 8 : rows > 2 ? 4 : (int)std::max<int64_t>(rows, 1);

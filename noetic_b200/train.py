@@ -124,7 +124,7 @@ class AdamwMany:
 
     def __init__(self, tensors):
         nb = _nb()
-        self.h = None
+        self.h, self._nb = None, None
         table = (NkAdamwTensor * len(tensors))(*[
             NkAdamwTensor(t.val, t.grad, t.m, t.v, t.m_scale, t.v_scale, t.copy, t.n, t.grad_dtype, t.copy_dtype,
                           t.state_bits, t.decay) for t in tensors])
@@ -147,7 +147,8 @@ class AdamwMany:
             self.h = None
 
     def __del__(self):
-        self.close()
+        if self._nb is not None and self._nb.lib is not None:  # (None as the interpreter ends)
+            self.close()
 
 
 def adamw_step_many(tensors, lr: float, t: int, b1: float = 0.9, b2: float = 0.95, eps: float = 1e-8, wd: float = 0.0,

@@ -179,6 +179,39 @@ def test_step(nb, torch, grad, bits, copy, shift):
         _same(torch, t, _want(torch, b, 1.0, HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, bits), copy)
 
 
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+def test_bytes_are_those_of_the_operations_one_by_one(nb, torch, grad):
+    """A byte at the middle between two others goes the way that the formula goes when each of its
+    operations is rounded; roots, one in a million of which the kernel rounds the other way, may
+    move one byte in a hundred thousand."""
+    s = Tensors(torch, [1 << 20, 3001], grad, 8, seed=12)
+    before = s.clone()
+    s.plan(nb).step(**HYPER)
+    torch.cuda.synchronize()
+    for t, b in zip(s.t, before):
+        n, blocks = b["n"], -(-b["n"] // 256)
+
+        def per(x):
+            return x.repeat_interleave(256)[:n]
+
+        g = b["grad"].float()
+        m = b["m"].view(torch.float8_e4m3fn).float() * per(b["m_scale"])
+        r = b["v"].view(torch.float8_e4m3fn).float() * per(b["v_scale"])
+        m = m * float(np.float32(0.9)) + g * float(np.float32(1) - np.float32(0.9))
+        v = r.square() * float(np.float32(0.95)) + (g * float(np.float32(1) - np.float32(0.95))) * g
+        for k, x in (("m", m), ("v", torch.sqrt(v))):
+            rows = torch.zeros(blocks * 256, device="cuda")
+            rows[:n] = x
+            top = rows.view(blocks, 256).abs().amax(1)
+            assert torch.equal(t[k + "_scale"], top * float(np.float32(1) / np.float32(448)))
+            y = x * per(torch.where(top > 0, (1.0 / top) * 448.0, 0.0))
+            if k == "v":
+                y = torch.where(x > 0, y.clamp(min=2.0**-9), y)
+            code = y.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+            away = int((t[k] != code).sum())
+            assert away <= (1e-5 * n if n > 1e5 else 0), (k, away)
+
+
 def test_32_bits_are_nk_adamw_step(nb, torch):
     s = Tensors(torch, SIZES, seed=3)
     other = s.clone()
@@ -210,7 +243,7 @@ def test_norm_and_clip(nb, torch, bits, grad, scale):
         assert abs(float(norm) - exact) <= 4 * 2.0**-24 * exact and int(bad) == 0
         c = np.float32(scale)
         if limit and float(norm) > np.float32(limit):
-            c = np.float32(scale) * (np.float32(limit) / np.float32(norm.cpu().numpy()[0]))
+            c = np.float32(scale) * (np.float32(limit) * (np.float32(1) / np.float32(norm.cpu().numpy()[0])))
         for t, b in zip(s.t, before):
             _same(torch, t, _want(torch, b, float(c), HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, bits))
         before = s.clone()
