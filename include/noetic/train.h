@@ -33,10 +33,11 @@ extern "C" {
  *                backward call needs
  * each nullable, not both.  A row whose target is no token is not read; its loss
  * and stats are 0.  A NaN or an infinity in a row of x makes the row's numbers
- * NaN, one in w those of every row.  Products of 16-bit elements are exact and
- * their sums f32; f32 elements count with 22 bits at least, relative to the
- * largest of their matrix.  (-infinity cannot mask a token here: a logit comes
- * from w.)
+ * NaN; one in w those of every row, unless it makes a logit -infinity, which can
+ * count as one of a token that is never chosen.  Products of 16-bit elements are
+ * exact and their sums f32; f32 elements count with 22 bits at least, relative to
+ * the largest of their row (for the gradients, of their matrix).  (-infinity cannot
+ * mask a token here: a logit comes from w.)
  * workspace: nk_linear_ce_workspace bytes, 256-byte aligned.  Should a wait
  * between parts of the kernel ever run out (it has a limit of seconds, for a
  * broken device), the loss is NaN. */
@@ -62,8 +63,9 @@ nk_status nk_linear_ce_workspace(int dtype, uint64_t rows, uint64_t width, uint6
  * nullable, not both; accumulate != 0 adds to dw (dx is set).  Rows whose target
  * is no token, or whose weight is 0, are not read, have dx = 0 and add nothing
  * to dw.  Each element of G is rounded once to the type of x (f32: 22 bits,
- * floor 2^-38) relative to the largest weight; sums are f32.  dx and dw must not
- * overlap x, w or each other. */
+ * floor 2^-38) relative to the largest finite weight; sums are f32.  A weight that
+ * is not finite breaks its row of dx, and dw.  dx and dw must not overlap x, w or
+ * each other. */
 nk_status nk_linear_ce_backward_device(const void *x, int dtype, uint64_t rows, uint64_t width, uint64_t x_stride,
                                        const void *w, uint64_t vocab, uint64_t w_stride, const uint32_t *targets,
                                        const float *stats, const float *row_weight, float grad_scale, void *dx,
@@ -106,8 +108,9 @@ void nk_adamw_many_free(nk_adamw_many *many);
  * grad is larger, grad_scale max_norm / norm.  With f32 gradients and moments
  * and c = 1 a tensor's result is nk_adamw_step's, bit for bit.  cfg->decay is not
  * read (each tensor has its own).  8-bit moments are read, stepped in f32 (with
- * a few roundings of 2^-23), used for this step's val, and rounded to nearest afterwards with a new scale for
- * the block; a v above 0 does not become 0, and |m| is kept up to 2^100.
+ * a few roundings of 2^-23), used for this step's val, and rounded to nearest
+ * afterwards with a new scale for the block; a v above 0 does not become 0, and
+ * |m| is kept up to 2^100.
  * norm (nullable, device): receives the norm.  bad (nullable, device): becomes 1
  * where an element's g or value is not finite; that element's val and
  * moments stay (8-bit moments: as far as the block's new scale holds them).

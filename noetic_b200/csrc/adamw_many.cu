@@ -64,12 +64,18 @@ __device__ __forceinline__ double chunk_squares(const G *grad, uint32_t n, bool 
                 a = fmaf(x, x, a);
                 b = fmaf(y, y, b);
             }
-            s += (double)(a + b);
+            // (Squares that leave f32's range: gradients above 4e18, or below 1e-16.)
+            if (a + b > 1e-30f && a + b < 1e37f) {
+                s += (double)(a + b);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < PER; ++e) s += (double)to_f32(g[e]) * (double)to_f32(g[e]);
+            }
         }
     }
     for (uint32_t i = vectors * PER + threadIdx.x; i < n; i += blockDim.x) {
-        const float g = to_f32(grad[i]);
-        s += (double)(g * g);
+        const double g = (double)to_f32(grad[i]);
+        s += g * g;
     }
     return s;
 }

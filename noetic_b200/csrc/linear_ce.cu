@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(1024) ce_index_k(LinearCeArgs a, Index ix, boo
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const bool counts_in = t[i] < (uint32_t)a.vocab && w[i] != 0.0f;
-            if (counts_in) top = fmaxf(top, fabsf(w[i]));
+            // (A weight that is not finite breaks its own row alone.)
+            if (counts_in && isfinite(w[i])) top = fmaxf(top, fabsf(w[i]));
             votes[i] = __ballot_sync(0xffffffffu, counts_in);
             if (lane == 0) counts[i * 32 + warp] = __popc(votes[i]);
         }

@@ -249,6 +249,28 @@ def test_norm_and_clip(nb, torch, bits, grad, scale):
         before = s.clone()
 
 
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+@pytest.mark.parametrize("factor", [1e25, 1e-25])
+def test_norm_of_gradients_whose_squares_leave_f32(nb, torch, grad, factor):
+    s = Tensors(torch, SIZES, grad, 32, seed=5)
+    for t in s.t:
+        t["grad"] *= factor
+        t["grad"][::3] = 0.0
+    before = s.clone()
+    plan = s.plan(nb)
+    norm = torch.zeros(1, device="cuda")
+    bad = torch.zeros(1, device="cuda", dtype=torch.int32)
+    exact = sum(float(t["grad"].double().square().sum()) for t in before) ** 0.5
+    plan.step(**HYPER, max_norm=1.0, norm=norm.data_ptr(), bad=bad.data_ptr())
+    torch.cuda.synchronize()
+    assert abs(float(norm) - exact) <= 4 * U * exact and int(bad) == 0
+    c = np.float32(1)
+    if factor > 1:
+        c = np.float32(1) / np.float32(norm.cpu().numpy()[0])
+    for t, b in zip(s.t, before):
+        _same(torch, t, _want(torch, b, float(c), HYPER["lr"], 7, 0.9, 0.95, 1e-8, 0.1, 32))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_elements_that_are_not_finite_stay(nb, torch, bits):
     s = Tensors(torch, [1000, 4096, 5], bits=bits, seed=5)

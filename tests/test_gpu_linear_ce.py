@@ -311,6 +311,20 @@ def test_broken_rows_leave_the_others_alone(nb, torch, dtype):
     assert torch.isnan(broken).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_weights_that_are_not_finite_break_their_rows(nb, torch, dtype):
+    c = Case(torch, 300, 128, 600, dtype, seed=13)
+    _, stats = c.forward(nb)
+    c.weight[[17, 211]] = 1.0
+    dx, _ = c.backward(nb, stats)
+    c.weight[17], c.weight[211] = INF, NAN
+    bad = torch.zeros(300, dtype=torch.bool, device="cuda")
+    bad[[17, 211]] = True
+    broken, dw = c.backward(nb, stats)
+    assert not torch.isfinite(broken[bad]).any() and torch.equal(broken[~bad], dx[~bad])
+    assert torch.isnan(dw).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_gradients_against_differences(nb, torch, dtype):
     """Along random directions, central differences of the 64-bit loss."""
