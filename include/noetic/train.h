@@ -75,6 +75,14 @@ nk_status nk_linear_ce_backward(const void *x, int dtype, uint64_t rows, uint64_
                                 const uint32_t *targets, const float *stats, const float *row_weight, float grad_scale,
                                 void *dx, void *dw, int dw_dtype, int accumulate, int device);
 
+/* Test control of the failure path, for the calls that this host thread makes from
+ * now on: in the product of the loss (1), of G (2) or of dx and dw (3) one copy is
+ * left out (0: none, the default), so that the waits for it run out, which are
+ * bounded at 2 ms then.  The call's loss, or what its gradients have from there on, is
+ * NaN, never a sum that lacks a product; the next call is as any other.  (Calls of few
+ * rows have no such product.) */
+nk_status nk_linear_ce_withhold(int product);
+
 /* Elements of a tensor that share a scale of the 8-bit moments. */
 #define NK_ADAMW_BLOCK 256u
 

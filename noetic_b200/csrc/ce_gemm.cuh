@@ -15,6 +15,8 @@
 //   warps 4-11  epilogue, from one of two accumulators while the other fills.
 // Every wait is bounded (1 s); where one runs out, the kernel records it, the
 // roles leave their loops, copies in flight are waited for and TMEM is freed.
+// Sums that miss a product are never handed on: the epilogue's own wait for them
+// runs out, and what it has to store becomes NaN.
 #pragma once
 
 #include <cuda.h>
@@ -33,6 +35,7 @@ constexpr int BOX_BYTES = 4096;  // GRAD, STORE: 32 rows of 128 bytes on their w
 constexpr int smem_bytes(bool boxes) { return STAGES * STAGE_BYTES + (boxes ? EPI_WARPS * BOX_BYTES : 0) + 1024 + 256; }
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint64_t WAIT_NS = 1000000000ull;
+constexpr uint64_t TEST_WAIT_NS = 2000000ull;  // of calls under nk_linear_ce_withhold
 // The tensor cores cut, not round, when they add to a sum, so a chain of products
 // is off by half a step of the sum for each 16 of K, all one way (measured: 1.7e-8
 // of a logit each).  Where f32 results depend on it (the loss; f32 gradients), a
@@ -135,11 +138,11 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_t limit) {
     if (mbar_try(bar, parity)) return true;
     const uint64_t t0 = globaltimer();
     while (!mbar_try(bar, parity))
-        if (globaltimer() - t0 > WAIT_NS) return false;
+        if (globaltimer() - t0 > limit) return false;
     return true;
 }
 
@@ -294,6 +297,8 @@ struct Products {
     alignas(64) CUtensorMap a[2][2], b[2][2], c[2];  // [product][part]; c: G's parts
     Gemm g[2];
     int cost[2];  // K-blocks of an item, and what its end takes
+    uint64_t wait_ns;  // bound of every wait
+    int withhold;      // test control: the last K-block of the first pair's first item is never brought
 };
 
 // ---------------------------------------------------------------- epilogues
@@ -630,8 +635,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
                 const Item it = walk.at(p, item);
                 const int m0 = it.tm * TM + (int)rank * 128, n0 = it.tn * TN + (int)rank * 128;
                 int seg = it.k0 / max(1, walk.kblocks), x = (it.k0 - seg * walk.kblocks) * BK;
-                for (int k = it.k0; k < it.k1; ++k) {
-                    fine = mbar_wait(empty0 + 8 * stage, phase ^ 1);
+                const bool hold = ps.withhold && pair == 0 && i == 0;
+                for (int k = it.k0; k < it.k1 - hold; ++k) {
+                    fine = mbar_wait(empty0 + 8 * stage, phase ^ 1, ps.wait_ns);
                     if (!__all_sync(0xffffffffu, fine)) {
                         if (one) give_up(201);
                         fine = false;
@@ -659,6 +665,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
                     x += BK;
                     if (x >= walk.K) x = 0, ++seg;
                 }
+                if (hold) fine = false;
             }
             // A stage's copies have landed once its MMAs are done: wait for the last
             // ones, so that none writes into shared memory after the CTA's end.
@@ -668,7 +675,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
                 // (From the oldest of the last STAGES on: its number is issued - STAGES + i.)
                 const int at = issued < STAGES ? i : (stage + i) % STAGES;
                 const uint32_t ph = issued < STAGES ? 0u : (stage + i < STAGES ? phase ^ 1 : phase);
-                mbar_wait(empty0 + 8 * at, ph);
+                mbar_wait(empty0 + 8 * at, ph, ps.wait_ns);
             }
         } else if (warp == 1 && rank == 0) {
             const bool one = elect();
@@ -687,7 +694,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
                 const uint32_t idesc = p.idesc;
                 for (int k = it.k0;;) {
                     const int end = LONG ? chain_end<CHAIN>(k, it.k1, low) : it.k1, b = n & 1;
-                    fine = mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1));
+                    fine = mbar_wait(acc_empty0 + 8 * b, (uint32_t)(((n >> 1) & 1) ^ 1), ps.wait_ns);
                     if (!__all_sync(0xffffffffu, fine)) {
                         if (one) give_up(202);
                         fine = false;
@@ -697,7 +704,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
                     const uint32_t d = tmem + b * TN;
                     uint32_t more = 0;
                     for (; k < end; ++k) {
-                        fine = mbar_wait(full0 + 8 * stage, phase);
+                        fine = mbar_wait(full0 + 8 * stage, phase, ps.wait_ns);
                         if (!__all_sync(0xffffffffu, fine)) {
                             if (one) give_up(203);
                             fine = false;
@@ -714,9 +721,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
                         more = 1;
                         if (++stage == STAGES) stage = 0, phase ^= 1;
                     }
+                    if (!fine) break;  // (not committed: the epilogue takes whole sums only)
                     if (one) mma_commit(acc_full0 + 8 * b);
                     ++n;
-                    if (k >= it.k1 || !fine) break;
+                    if (k >= it.k1) break;
                 }
             }
         }
@@ -728,7 +736,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
         int n = 0;
         // The next accumulator: wait for it, or give it back.
         auto take = [&]() -> bool {
-            const bool ok = mbar_wait(acc_full0 + 8 * (n & 1), (uint32_t)((n >> 1) & 1));
+            const bool ok = mbar_wait(acc_full0 + 8 * (n & 1), (uint32_t)((n >> 1) & 1), ps.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) {  // (every lane is here: the loads that follow are the warp's)
                 if (lane == 0) give_up(204);
                 return false;

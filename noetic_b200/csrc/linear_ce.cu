@@ -30,6 +30,9 @@ constexpr uint64_t PIECE_BYTES = 256ull << 20;  // of G
 // G is at most 1 before its scale: f16 keeps it down to 2^-38.
 constexpr float G_SCALE = 16384.0f;
 
+// nk_linear_ce_withhold: 1 + the Mode whose product's wait is to run out, or 0.
+thread_local int g_withhold = 0;
+
 constexpr size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 // A block joins the tiles of 8 rows, in a fixed order: 32 threads a row.  row_of null:
@@ -676,7 +679,9 @@ struct Call {
         if (err == cudaSuccess) err = pdl_launch(k, grid, dim3((unsigned)threads), (size_t)shared, st, args...);
     }
     template <int MODE, bool LONG>
-    void product(const ce::Products &ps) {
+    void product(ce::Products &ps) {
+        ps.wait_ns = g_withhold ? ce::TEST_WAIT_NS : ce::WAIT_NS;
+        ps.withhold = g_withhold == MODE + 1;
         auto *k = ce::gemm_k<MODE, P, SPLIT, LONG>;
         constexpr int shared = ce::smem_bytes(MODE != ce::ROWS);
         if (err == cudaSuccess) err = allow_shared(k, shared);
@@ -841,6 +846,8 @@ struct Call {
 };
 
 }  // namespace
+
+void linear_ce_withhold(int product) { g_withhold = product; }
 
 size_t linear_ce_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
                                  bool backward) {

@@ -58,6 +58,7 @@ struct LinearCeArgs {
 };
 size_t linear_ce_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
                                  bool backward);
+void linear_ce_withhold(int product);  // nk_linear_ce_withhold
 cudaError_t linear_ce(const LinearCeArgs &a, int sms, cudaStream_t st);
 cudaError_t linear_ce_backward(const LinearCeArgs &a, int sms, cudaStream_t st);
 

@@ -306,6 +306,13 @@ nk_status nk_linear_ce_backward(const void *x, int dtype, uint64_t rows, uint64_
     });
 }
 
+nk_status nk_linear_ce_withhold(int product) {
+    return guard("nk_linear_ce_withhold", [&] {
+        need(product >= 0 && product <= 3, "product must be 0 to 3");
+        nk::linear_ce_withhold(product);
+    });
+}
+
 nk_status nk_adamw_many_create(const nk_adamw_tensor *tensors, uint64_t count, nk_adamw_many **out) {
     return guard("nk_adamw_many_create", [&] {
         need(out, "null argument");

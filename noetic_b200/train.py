@@ -36,6 +36,7 @@ SIGNATURES = {
     "nk_linear_ce_backward_device": (_i32, [_P, _i32, _u64, _u64, _u64, _P, _u64, _u64, _P, _P, _P, _f32, _P, _u64, _P,
                                             _i32, _u64, _i32, _P, _u64, _P]),
     "nk_linear_ce_backward": (_i32, [_P, _i32, _u64, _u64, _P, _u64, _P, _P, _P, _f32, _P, _P, _i32, _i32, _i32]),
+    "nk_linear_ce_withhold": (_i32, [_i32]),
     "nk_adamw_many_create": (_i32, [C.POINTER(NkAdamwTensor), _u64, C.POINTER(_P)]),
     "nk_adamw_many_free": (None, [_P]),
     "nk_adamw_many_step_device": (_i32, [_P, _P, _f32, _f32, _P, _P, _P]),

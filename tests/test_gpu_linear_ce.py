@@ -531,3 +531,42 @@ def test_the_loss_is_that_of_the_logits(nb, torch):
                                                 None, _st(torch)))
     tol = 2 * c.dz().max() + (1000 / 32 + 200) * U + U * z.abs().max() * 4
     assert (loss + lp).abs().max() <= tol
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,width,vocab", [(600, 320, 1500), (300, 40, 5000)])
+def test_a_wait_that_runs_out_leaves_nan_and_never_a_part_of_a_sum(nb, torch, dtype, rows, width, vocab):
+    """A copy that never comes (a test control; the waits end after 2 ms): what is not the
+    right number is NaN, and the next calls are as they were."""
+    c = Case(torch, rows, width, vocab, dtype, ignored=0.1, seed=60)
+    loss, stats = c.forward(nb)
+    dx, dw = c.backward(nb, stats, 0.5)
+    hold = nb.lib().nk_linear_ce_withhold
+    assert hold(4) == nb.NK_ERR_INVALID and hold(-1) == nb.NK_ERR_INVALID
+    try:
+        nb._check(hold(1))
+        broken, _ = c.forward(nb)
+        if rows * width * vocab <= 1e8:  # (few products: a kernel without such waits)
+            assert torch.equal(broken, loss)
+        else:
+            assert torch.isnan(broken[c.live]).all() and (broken[~c.live] == 0).all()
+        nb._check(hold(2))
+        gx, gw = c.backward(nb, stats, 0.5)
+        assert torch.isnan(gx[c.live]).all() and torch.isnan(gw).all()
+        nb._check(hold(3))
+        for want_dx in (True, False):
+            for got, want in zip(c.backward(nb, stats, 0.5, want_dx=want_dx), (dx, dw)):
+                if got is None:
+                    continue
+                gone = torch.isnan(got)
+                assert torch.equal(got[~gone], want[~gone])
+                if (got.shape[0] == rows) == want_dx:
+                    # The first tile of the first product that is there.
+                    first = torch.nonzero(c.live)[:256, 0] if want_dx else slice(256)
+                    assert gone[first, :256].all()
+    finally:
+        nb._check(hold(0))
+    again, st = c.forward(nb)
+    assert torch.equal(again, loss) and torch.equal(st, stats)
+    for got, want in zip(c.backward(nb, stats, 0.5), (dx, dw)):
+        assert torch.equal(got, want)
