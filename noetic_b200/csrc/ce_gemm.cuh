@@ -38,8 +38,9 @@ constexpr uint64_t WAIT_NS = 1000000000ull;
 constexpr uint64_t TEST_WAIT_NS = 2000000ull;  // of calls under nk_linear_ce_withhold
 // The tensor cores cut, not round, when they add to a sum, so a chain of products
 // is off by half a step of the sum for each 16 of K, all one way (measured: 1.7e-8
-// of a logit each).  Where f32 results depend on it (the loss; f32 gradients), a
-// chain ends after a few K-blocks and the epilogue's registers add the chains up.
+// of a logit each).  Where f32 results depend on it (the loss; f32 gradients, an f32
+// dw of 16-bit rows too), and in 16-bit gradients of very many terms, a chain ends
+// after a few K-blocks and the epilogue's registers add the chains up.
 // (f32: the low parts' products come first, as one chain: they are 2^-11 of the sum.)
 // Logits of f32 rows get the shortest chains: an error of the logit is one of p, and a
 // sure token's gradient is 1 - p.  (8192 x 256 x 2369, gradients from exact statistics:
@@ -617,7 +618,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_k(c
     // The pair's item number i.
     int which = 0, item = 0;
     auto next = [&](int i) { return deal.at(pair, i, which, item); };
-    constexpr int CHAIN = chain_blocks(SCALED && MODE != STORE);
+    // (Gradients of 16-bit rows: as exact as their G makes them.  8192 x 1024 x 32768 with an f32 dw
+    // takes 1290 us with one chain, off by up to 2e-5, 1310 with chains of 32, 1400 of 16, 1420 of 8.)
+    constexpr int CHAIN = MODE == STORE && !SCALED ? 16 : chain_blocks(SCALED && MODE != STORE);
     // A wait that ran out ends the role that waited; the others' waits on it run out too.
     auto give_up = [&](uint32_t code) { atomicExch(&head->err, code); };
 

@@ -570,3 +570,26 @@ def test_a_wait_that_runs_out_leaves_nan_and_never_a_part_of_a_sum(nb, torch, dt
     assert torch.equal(again, loss) and torch.equal(st, stats)
     for got, want in zip(c.backward(nb, stats, 0.5), (dx, dw)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_f32_sums_of_many_rows_do_not_drift(nb, torch, dtype):
+    """dw in f32 of 65536 rows whose terms have one sign and one G: w = 0, so every p is what
+    the statistics say, a power of two.  A chain of 16 K-blocks passes a term through 64
+    additions that cut, and 5 (2 U each); 64 chains are added with U each; 4 U for the way
+    out.  (One chain over all rows cuts 4096 times: 2960 U of f16, all one way.)"""
+    rows, width, vocab = 65536, 2048, 2048
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = (1 + torch.rand(rows, width, generator=g, device="cuda")).to(_dt(torch, dtype))
+    w = torch.zeros(vocab, width, device="cuda", dtype=_dt(torch, dtype))
+    targets = torch.zeros(rows, device="cuda", dtype=torch.int32)
+    stats = torch.tensor([0.0, 11 * np.log(2.0)], device="cuda", dtype=torch.float32).repeat(rows, 1)
+    dw = torch.empty(vocab, width, device="cuda")
+    room = torch.empty(nb.train.linear_ce_workspace(CODE[dtype], rows, width, vocab, w.data_ptr(), width, True), device="cuda",
+                       dtype=torch.uint8)
+    nb._check(nb.lib().nk_linear_ce_backward_device(
+        _p(x), CODE[dtype], rows, width, width, _p(w), vocab, width, _p(targets), _p(stats), None, 1.0, None, 0, _p(dw), 0,
+        width, 0, _p(room), room.numel(), _st(torch)))
+    want = x.double().sum(0) / 2048
+    off = (dw[1:].double() - want) / want
+    assert float(off.abs().max()) <= (2 * (64 + 5) + 64 + 4) * U, float(off.abs().max()) / U
