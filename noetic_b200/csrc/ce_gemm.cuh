@@ -384,12 +384,14 @@ struct GradEpilogue {
     const int row0, col;
     const uint32_t t;
     const float2 st;
-    const float h, base;
+    const float h, base, hp;
     __device__ __forceinline__ GradEpilogue(const Gemm &q, const CUtensorMap *a, const CUtensorMap *b, uint8_t *to, int row, int live,
                                             int c)
         : p(q), map0(a), map1(b), box(to), in(row < live), row0(row - (int)(threadIdx.x & 31)), col(c),
           t(in ? q.target[row] - (uint32_t)q.col0 : NO_TOKEN), st(in ? q.stats[row] : make_float2(0.0f, 0.0f)),
-          h(in ? q.weight[row] / q.head->weight_max * q.g_scale : 0.0f), base((st.x + st.y) * LOG2E) {}
+          h(in ? weight() : 0.0f), base(st.x * LOG2E),
+          hp(h * ex2(-fmaf(st.y, LOG2E, fmaf(st.x, LOG2E, -base)))) {}
+    __device__ __forceinline__ float weight() const { return p.weight[row0 + (int)(threadIdx.x & 31)] / p.head->weight_max * p.g_scale; }
     __device__ __forceinline__ void some(int c, float *v) {
         const int lane = threadIdx.x & 31;
         if (SCALED) {
@@ -397,18 +399,21 @@ struct GradEpilogue {
 #pragma unroll
             for (int j = 0; j < 64; ++j) v[j] = ex2(((v[j] * scale - st.x) - st.y) * LOG2E) * h;
         } else {
-            // (For 16 bits the fma's error, 2^-24 of the log-sum, is nothing.)
+            // (One fma, whose error is of the distance to the maximum: what base lacks of it, and
+            // log s, are in hp.  With both in base, p was 8e-4 off at logits of 10^4.)
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = ex2(fmaf(v[j], LOG2E, -base)) * h;
+            for (int j = 0; j < 64; ++j) v[j] = ex2(fmaf(v[j], LOG2E, -base)) * hp;
         }
         if (!in || col + c + 64 > p.n_valid)
 #pragma unroll
             for (int j = 0; j < 64; ++j)
                 if (!in || col + c + j >= p.n_valid) v[j] = 0.0f;
-        if (t - (uint32_t)(col + c) < 64u)
+        if (t - (uint32_t)(col + c) < 64u) {
+            const float own = SCALED ? h : weight();  // (read again: a register more and the sums spill)
 #pragma unroll
             for (int j = 0; j < 64; ++j)
-                if (t == (uint32_t)(col + c + j)) v[j] -= h;
+                if (t == (uint32_t)(col + c + j)) v[j] -= own;
+        }
 #pragma unroll
         for (int part = 0; part < (SCALED ? 2 : 1); ++part) {
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the box is free again

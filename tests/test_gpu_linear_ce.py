@@ -593,3 +593,24 @@ def test_f32_sums_of_many_rows_do_not_drift(nb, torch, dtype):
     want = x.double().sum(0) / 2048
     off = (dw[1:].double() - want) / want
     assert float(off.abs().max()) <= (2 * (64 + 5) + 64 + 4) * U, float(off.abs().max()) / U
+
+
+@pytest.mark.parametrize("dtype,top", [("f16", 100.0), ("bf16", 256.0), ("f32", 100.0)])
+def test_probabilities_of_logits_far_from_zero(nb, torch, dtype, top):
+    """Rows of one number each, under logits that are all top^2, exactly; a row's log-sum is
+    what its statistics say.  dw is then G x, which shows each p: exp(-log sum), with the
+    roundings of log s (U of it) and of the exponential (2^-22), below 16 U, and G's own."""
+    rows, vocab = 64, 40
+    x = torch.diag(torch.full((rows,), top, device="cuda")).to(_dt(torch, dtype))
+    w = torch.full((vocab, rows), top, device="cuda").to(x.dtype)
+    ls = torch.linspace(1.0, 4.0, rows, device="cuda")
+    stats = torch.stack([torch.full_like(ls, top * top), ls], 1).contiguous()
+    targets = torch.zeros(rows, device="cuda", dtype=torch.int32)
+    dw = torch.empty(vocab, rows, device="cuda")
+    room = torch.empty(nb.train.linear_ce_workspace(CODE[dtype], rows, rows, vocab, w.data_ptr(), rows, True), device="cuda",
+                       dtype=torch.uint8)
+    nb._check(nb.lib().nk_linear_ce_backward_device(
+        _p(x), CODE[dtype], rows, rows, rows, _p(w), vocab, rows, _p(targets), _p(stats), None, 1.0, None, 0, _p(dw), 0, rows, 0,
+        _p(room), room.numel(), _st(torch)))
+    off = (dw[1:].double() / top) / torch.exp(-ls.double()) - 1
+    assert float(off.abs().max()) <= {"f16": 2.0**-11, "bf16": 2.0**-8, "f32": 2.0**-22}[dtype] + 20 * U, float(off.abs().max())
