@@ -412,7 +412,8 @@ nk_status nk_adamw_many_step(const nk_adamw_tensor *tensors, uint64_t count, con
             d.v = h.up((const char *)t.v, state) ? h.own.back() : nullptr;
             d.m_scale = h.up(t.m_scale, scales);
             d.v_scale = h.up(t.v_scale, scales);
-            d.copy = h.room<void>(t.n * 2, t.copy);
+            // (With what is there: a norm that is not finite leaves it.)
+            d.copy = h.up((const char *)t.copy, t.n * 2) ? h.own.back() : nullptr;
         }
         auto *flags = h.room<char>(8);
         cuda_check(cudaMemset(flags, 0, 8), "memset");

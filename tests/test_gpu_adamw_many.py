@@ -424,3 +424,19 @@ def test_host_form(nb, torch):
     grad[7] = np.nan
     with pytest.raises(nb.NoeticError):
         nb.adamw_step_many([dict(val=val, grad=grad, m=zero, v=zero)], lr=0.1, t=1)
+
+
+def test_host_form_leaves_everything_where_the_norm_is_not_finite(nb):
+    rng = np.random.default_rng(1)
+    a = {k: rng.standard_normal(700).astype(np.float32) for k in ("val", "grad", "m", "v")}
+    a["copy"] = rng.integers(0, 1 << 16, 700).astype(np.uint16)
+    a["grad"][5] = np.inf
+    before = {k: v.copy() for k, v in a.items()}
+    t = (nb.train.NkAdamwTensor * 1)(nb.train.NkAdamwTensor(
+        a["val"].ctypes.data, a["grad"].ctypes.data, a["m"].ctypes.data, a["v"].ctypes.data, None, None,
+        a["copy"].ctypes.data, 700, 0, 2, 32, 1))
+    cfg, norm = nb.NkAdamwCfg(0.1, 0.9, 0.95, 1e-8, 0.0, 1, 1), C.c_float()
+    assert nb.lib().nk_adamw_many_step(t, 1, C.byref(cfg), 1.0, 1.0, C.byref(norm), 0) == nb.NK_ERR_INVALID
+    assert norm.value == np.inf
+    for k, v in a.items():
+        assert v.tobytes() == before[k].tobytes(), k
