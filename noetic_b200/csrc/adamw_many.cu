@@ -298,7 +298,8 @@ __device__ __forceinline__ float grad_of(const void *grad, int dtype, uint64_t i
 // step of such an element is an eighth longer or shorter.
 //
 // The careful form: short blocks, tensors that start off 16 bytes, elements that are
-// not finite or beyond the range of what is stored.
+// not finite or beyond the range of what is stored.  Its operations are those of the other
+// form, so that an element's result does not depend on where it lies.
 __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t first, uint32_t n, AdamwParams params, float factor) {
     const int lane = threadIdx.x & 31;
     const nk_adamw_tensor &t = *tp;
@@ -342,8 +343,7 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
             u = vv < 1.1754944e-38f ? 0.0f : u;
             // (A v beyond f32's range divides to 0.)
             const float inv = v1 > V_MAX ? 0.0f : rcp(fmaf(u, a.root_bc2, a.eps));
-            const float upd = fmaf(mm * a.inv_bc1, inv, wd * pv[h][e]);
-            pv[h][e] = fine ? fmaf(-a.lr, upd, pv[h][e]) : pv[h][e];
+            pv[h][e] = fine ? pv[h][e] + fmaf(mm * inv, -a.lr * a.inv_bc1, -a.lr * wd * pv[h][e]) : pv[h][e];
             mm = fminf(fmaxf(mm, -MOMENT_MAX), MOMENT_MAX);
             g[h][e] = fine ? mm : mq * ms;  // the new m
             rv[h][e] = fine ? u : r;
