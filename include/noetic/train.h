@@ -120,7 +120,7 @@ void nk_adamw_many_free(nk_adamw_many *many);
  * afterwards with a new scale for the block; a v above 0 does not become 0, and
  * |m| is kept up to 2^100.
  * norm (nullable, device): receives the norm.  bad (nullable, device): becomes 1
- * where an element's g or value is not finite; that element's val and
+ * where an element's g, value or 8-bit moment is not finite; that element's val and
  * moments stay (8-bit moments: as far as the block's new scale holds them).
  * A norm that is not finite, with max_norm > 0: nothing changes, bad becomes 1.
  * A captured call repeats its cfg, grad_scale and max_norm in each replay. */

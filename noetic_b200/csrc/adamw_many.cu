@@ -331,8 +331,9 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
         for (int e = 0; e < 4; ++e) {
             const float2 mc = from_e4m3(e < 2 ? mb[h] & 0xFFFFu : mb[h] >> 16), vc = from_e4m3(e < 2 ? vb[h] & 0xFFFFu : vb[h] >> 16);
             const float mq = e & 1 ? mc.y : mc.x, r = (e & 1 ? vc.y : vc.x) * vs;
-            const float gc = g[h][e] * a.c;
-            const bool fine = fabsf(gc) < INFINITY && fabsf(pv[h][e]) < INFINITY;
+            // (A moment that is not finite stays so, and is no part of the block's scale.)
+            const float gc = g[h][e] * a.c, m0 = fabsf(mq * ms) < INFINITY ? mq * ms : NAN, r0 = fabsf(r) < INFINITY ? r : NAN;
+            const bool fine = fabsf(gc) < INFINITY && fabsf(pv[h][e]) < INFINITY && !isnan(m0) && !isnan(r0);
             ok &= fine;
             float mm = __fadd_rn(__fmul_rn(__fmul_rn(mq, ms), a.b1), __fmul_rn(gc, a.g1));
             const float v1 = __fadd_rn(__fmul_rn(__fmul_rn(r, r), a.b2), __fmul_rn(__fmul_rn(gc, a.g2), gc)), vv = fminf(v1, V_MAX);
@@ -345,8 +346,8 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
             const float inv = v1 > V_MAX ? 0.0f : rcp(fmaf(u, a.root_bc2, a.eps));
             pv[h][e] = fine ? pv[h][e] + fmaf(mm * inv, -a.lr * a.inv_bc1, -a.lr * wd * pv[h][e]) : pv[h][e];
             mm = fminf(fmaxf(mm, -MOMENT_MAX), MOMENT_MAX);
-            g[h][e] = fine ? mm : mq * ms;  // the new m
-            rv[h][e] = fine ? u : r;
+            g[h][e] = fine ? mm : m0;  // the new m
+            rv[h][e] = fine ? u : r0;
             top_m = fmaxf(top_m, fabsf(g[h][e]));
             top_r = fmaxf(top_r, rv[h][e]);
         }
@@ -363,7 +364,7 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             y[e] = g[h][e] * km;
-            z[e] = rv[h][e] > 0.0f ? fmaxf(rv[h][e] * kr, least) : 0.0f;
+            z[e] = rv[h][e] > 0.0f ? fmaxf(rv[h][e] * kr, least) : rv[h][e];
         }
         const uint32_t mo = to_e4m3(y[0], y[1]) | to_e4m3(y[2], y[3]) << 16, vo = to_e4m3(z[0], z[1]) | to_e4m3(z[2], z[3]) << 16;
 #pragma unroll

@@ -460,3 +460,31 @@ def test_8_bits_do_not_depend_on_where_a_tensor_lies(nb, torch, grad, copy):
             if i == 0 and a["n"] > 9:  # (whose moments stay, and may have been the block's largest)
                 keep = torch.arange(a["n"], device="cuda") != 9
                 assert torch.equal(a["val"][keep], c["val"][keep])
+
+
+@pytest.mark.parametrize("shift", [0, 3])
+def test_a_moment_that_is_not_finite_spoils_no_other(nb, torch, shift):
+    """A byte that is no number, or a block whose scale is infinite: those elements stay as they
+    are, `bad` says so, and all others go on as they would without them."""
+    s, ref = (Tensors(torch, [1000, 512], bits=8, shift=shift, seed=14) for _ in range(2))
+    for t in (s.t[0], ref.t[0]):
+        t["m"][7], t["v"][300] = 0, 1  # (nothing to the blocks' largest)
+    s.t[0]["m"][7] = 127
+    s.t[0]["v"][300] = 127
+    s.t[1]["m_scale"][1] = float("inf")
+    before = s.clone()
+    bad = torch.zeros(1, device="cuda", dtype=torch.int32)
+    for x, b in ((s, bad.data_ptr()), (ref, None)):
+        x.plan(nb).step(**HYPER, bad=b)
+    torch.cuda.synchronize()
+    assert int(bad) == 1
+    t, r = s.t[0], ref.t[0]
+    kept = torch.ones(1000, dtype=torch.bool, device="cuda")
+    kept[[7, 300]] = False
+    for k in ("val", "m", "v"):
+        assert torch.equal(t[k][kept], r[k][kept]), k
+    assert torch.equal(t["val"][~kept], before[0]["val"][~kept])
+    assert int(t["m"][7]) & 127 == 127 and int(t["v"][300]) & 127 == 127
+    assert torch.equal(t["m_scale"], r["m_scale"]) and torch.equal(t["v_scale"], r["v_scale"])
+    t, r = s.t[1], ref.t[1]
+    assert torch.equal(t["val"][:256], r["val"][:256]) and torch.equal(t["val"][256:], before[1]["val"][256:])
