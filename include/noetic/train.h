@@ -116,9 +116,14 @@ void nk_adamw_many_free(nk_adamw_many *many);
  * grad is larger, grad_scale max_norm / norm.  With f32 gradients and moments
  * and c = 1 a tensor's result is nk_adamw_step's, bit for bit.  cfg->decay is not
  * read (each tensor has its own).  8-bit moments are read, stepped in f32 (with
- * a few roundings of 2^-23), used for this step's val, and rounded to nearest
- * afterwards with a new scale for the block; a v above 0 does not become 0, and
- * |m| is kept up to 2^100.
+ * a few roundings of 2^-23), used for this step's val, and rounded afterwards with a
+ * new scale for the block; a v above 0 does not become 0, and |m| is kept up to
+ * 2^100.  A moment whose factor (b1, b2) is at most 0.95 is rounded to nearest; what
+ * it forgets in a step is then about half a step of the grid, and it follows its
+ * gradients as far as these, or the scale of its block, move it by more.  Above 0.95 it
+ * is rounded up or down in proportion to where it lies, so that the mean of m, or of v,
+ * is the formula's; which of the two goes by the element's number, val, g and cfg->t
+ * alone, so the same call on the same arrays gives the same bytes.
  * norm (nullable, device): receives the norm.  bad (nullable, device): becomes 1
  * where an element's g, value or 8-bit moment is not finite; that element's val and
  * moments stay (8-bit moments: as far as the block's new scale holds them).

@@ -223,6 +223,45 @@ __device__ __forceinline__ uint32_t to_e4m3(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// What the moments' rounding by chance takes from the call.
+struct Chance {
+    bool m, v;
+    uint32_t t;
+};
+// Above this factor a step forgets less than half a step of the grid (1/32 to 1/16 of a
+// value), so that to nearest a byte returns to where it was: roots whose gradients fell to
+// a tenth stood at 6.6 times the formula's after 600 steps at b2 = 0.99, and means of
+// gradients that turned round had not turned after 750 steps at b1 = 0.98.  Rounded up or
+// down in proportion they are at 1.00 and 0.04 off.  Below, noisy gradients move the block's
+// scale by enough (1.00 at b2 = 0.95), and to nearest is the more exact: 0.075 off where
+// chance is 0.107, and takes less time (361M elements, bf16 gradients and copy: 1245 us, by
+// chance 1570).
+constexpr float MOST_TO_NEAREST = 0.95f;
+
+// 24 bits of an element and a step, in [0, 1): odd multiples of it (2^32 by the golden
+// ratio, by sqrt 2 and by sqrt 3), folded.  `m`: another 24.
+__device__ __forceinline__ float chance_of(uint64_t element, uint32_t t, float val, float grad, bool m) {
+    uint32_t x = (uint32_t)element * 0x9E3779B9u + (uint32_t)(element >> 32) + t * 0x6A09E667u;
+    x ^= x >> 16;
+    x = (x ^ __float_as_uint(val)) * 0xBB67AE85u;
+    x ^= x >> 15;
+    x = (x + __float_as_uint(grad)) * 0x9E3779B9u;
+    x ^= x >> 16;
+    x *= 0x6A09E667u;
+    if (m) x = (x ^ x >> 13) * 0xBB67AE85u;
+    return (float)((x ^ x >> 15) & 0xFFFFFFu) * 5.9604645e-8f;
+}
+
+// One of the two numbers of the grid beside y >= 0, whose mean (SQUARE: whose square's mean)
+// is y's.
+template <bool SQUARE>
+__device__ __forceinline__ float by_chance(float y, float u) {
+    const uint32_t e = max(__float_as_uint(y) & 0x7F800000u, 121u << 23);  // (2^-6: below, one step)
+    const float step = __uint_as_float(e - (3u << 23)), q = y * __uint_as_float((257u << 23) - e), n = floorf(q), f = q - n;
+    const bool up = SQUARE ? u * (2.0f * n + 1.0f) < f * (q + n) : u < f;
+    return (up ? n + 1.0f : n) * step;
+}
+
 // 448 times the reciprocal of top (correctly rounded but for one in a million).
 __device__ __forceinline__ float grid_scale(float top) {
     const float r = __fdividef(1.0f, top);
@@ -300,14 +339,14 @@ __device__ __forceinline__ float grad_of(const void *grad, int dtype, uint64_t i
 // The careful form: short blocks, tensors that start off 16 bytes, elements that are
 // not finite or beyond the range of what is stored.  Its operations are those of the other
 // form, so that an element's result does not depend on where it lies.
-__device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t first, uint32_t n, AdamwParams params, float factor) {
+__device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t first, uint32_t n, AdamwParams params, float factor, Chance chance) {
     const int lane = threadIdx.x & 31;
     const nk_adamw_tensor &t = *tp;
     const Step8 a(params, factor);
     const float wd = t.decay ? a.wd : 0.0f;
     float *val = t.val + first;
     uint8_t *m = (uint8_t *)t.m + first, *v = (uint8_t *)t.v + first;
-    float ms, vs, pv[2][4], g[2][4], rv[2][4];
+    float ms, vs, pv[2][4], g[2][4], rv[2][4], um[2][4], uv[2][4];
     uint32_t mb[2], vb[2];
     ms = t.m_scale[first / NK_ADAMW_BLOCK], vs = t.v_scale[first / NK_ADAMW_BLOCK];
 #pragma unroll
@@ -333,6 +372,8 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
             const float mq = e & 1 ? mc.y : mc.x, r = (e & 1 ? vc.y : vc.x) * vs;
             // (A moment that is not finite stays so, and is no part of the block's scale.)
             const float gc = g[h][e] * a.c, m0 = fabsf(mq * ms) < INFINITY ? mq * ms : NAN, r0 = fabsf(r) < INFINITY ? r : NAN;
+            um[h][e] = chance.m ? chance_of(first + h * 128 + lane * 4 + e, chance.t, pv[h][e], gc, true) : 0.0f;
+            uv[h][e] = chance.v ? chance_of(first + h * 128 + lane * 4 + e, chance.t, pv[h][e], gc, false) : 0.0f;
             const bool fine = fabsf(gc) < INFINITY && fabsf(pv[h][e]) < INFINITY && !isnan(m0) && !isnan(r0);
             ok &= fine;
             float mm = __fadd_rn(__fmul_rn(__fmul_rn(mq, ms), a.b1), __fmul_rn(gc, a.g1));
@@ -365,6 +406,8 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
         for (int e = 0; e < 4; ++e) {
             y[e] = g[h][e] * km;
             z[e] = rv[h][e] > 0.0f ? fmaxf(rv[h][e] * kr, least) : rv[h][e];
+            if (chance.m) y[e] = copysignf(by_chance<false>(fabsf(y[e]), um[h][e]), y[e]);
+            if (chance.v) z[e] = by_chance<true>(z[e], uv[h][e]);
         }
         const uint32_t mo = to_e4m3(y[0], y[1]) | to_e4m3(y[2], y[3]) << 16, vo = to_e4m3(z[0], z[1]) | to_e4m3(z[2], z[3]) << 16;
 #pragma unroll
@@ -387,13 +430,13 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
 // The same for a whole block in shared memory, two elements to an instruction.  What
 // is not finite, or out of range, shows in a sum of products with 0 and in the largest
 // moment; such a block, of which nothing is stored yet, goes to the careful form.
-template <class G>
+template <class G, bool CHANCE>
 __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t first, const Stage8 &st, const Step8 &a, const AdamwParams &params,
-                                            float wd) {
+                                            float wd, const Chance &chance) {
     const int lane = threadIdx.x & 31;
     const float ms = st.scale[0], vs = st.scale[1];
     const float2 b1 = both(a.b1), c = both(a.c), g1 = both(a.g1), b2 = both(-a.b2), g2 = both(-a.g2), zero = both(0.0f);
-    float2 pv[4], mv[4], root[4], strange = zero;
+    float2 pv[4], mv[4], root[4], um[4], uv[4], strange = zero;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const uint32_t at = h * 128 + lane * 4;
@@ -416,6 +459,11 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
         for (int i = 0; i < 2; ++i) {
             const int o = 2 * h + i;
             const float2 r = mul2(from_e4m3(i ? vb >> 16 : vb & 0xFFFFu), both(vs)), gc = mul2(g[i], c);
+            if (CHANCE) {
+                const uint64_t e = first + at + 2 * i;
+                uv[o] = make_float2(chance_of(e, chance.t, pv[o].x, gc.x, false), chance_of(e + 1, chance.t, pv[o].y, gc.y, false));
+                if (chance.m) um[o] = make_float2(chance_of(e, chance.t, pv[o].x, gc.x, true), chance_of(e + 1, chance.t, pv[o].y, gc.y, true));
+            }
             mv[o] = plus(mul2(mul2(from_e4m3(i ? mb >> 16 : mb & 0xFFFFu), both(ms)), b1), mul2(gc, g1));
             const float2 nv = plus(mul2(mul2(r, r), b2), mul2(mul2(gc, g2), gc));  // -v'
             strange = fma2(mv[o], zero, strange);
@@ -437,7 +485,7 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
     top_m = warp_max(top_m);
     top_r = warp_max(top_r);
     if (__any_sync(0xffffffffu, !(strange.x + strange.y == 0.0f)) || top_m > MOMENT_MAX)
-        return careful_step8(&t, first, NK_ADAMW_BLOCK, params, a.c);
+        return careful_step8(&t, first, NK_ADAMW_BLOCK, params, a.c, chance);
     const float km = top_m >= SCALE_MIN ? grid_scale(top_m) : 0.0f;
     const float kr = top_r >= SCALE_MIN ? grid_scale(top_r) : 0.0f;
     const float least = kr > 0.0f ? E4M3_TINY : 0.0f;
@@ -454,10 +502,17 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
             const float2 q = mul2(mv[o], make_float2(rcp(den.x), rcp(den.y)));
             const float2 now = add2(pv[o], fma2(q, rate, mul2(fade, pv[o])));
             p[2 * i] = now.x, p[2 * i + 1] = now.y;
-            const float2 y = mul2(mv[o], both(km)), z = mul2(root[o], both(kr)), big = mul2(root[o], both(1e25f));
-            mo[i] = to_e4m3(y.x, y.y);
+            float2 y = mul2(mv[o], both(km)), z = mul2(root[o], both(kr));
+            const float2 big = mul2(root[o], both(1e25f));
             // A root above 0 (then above 1e-19) stays above 0: a later step divides by it.
-            vo[i] = to_e4m3(fminf(fmaxf(z.x, least), big.x), fminf(fmaxf(z.y, least), big.y));
+            z = make_float2(fminf(fmaxf(z.x, least), big.x), fminf(fmaxf(z.y, least), big.y));
+            if (CHANCE) {
+                if (chance.v) z = make_float2(by_chance<true>(z.x, uv[o].x), by_chance<true>(z.y, uv[o].y));
+                if (chance.m)
+                    y = make_float2(copysignf(by_chance<false>(fabsf(y.x), um[o].x), y.x), copysignf(by_chance<false>(fabsf(y.y), um[o].y), y.y));
+            }
+            mo[i] = to_e4m3(y.x, y.y);
+            vo[i] = to_e4m3(z.x, z.y);
         }
         *reinterpret_cast<float4 *>(t.val + first + at) = make_float4(p[0], p[1], p[2], p[3]);
         *reinterpret_cast<uint32_t *>((uint8_t *)t.m + first + at) = mo[0] | mo[1] << 16;
@@ -492,9 +547,9 @@ __device__ __forceinline__ void issue8(const nk_adamw_tensor &t, uint64_t e, Sta
 }
 
 // A warp's chunk, STAGES8 - 1 blocks ahead.
-template <class G>
+template <class G, bool CHANCE>
 __device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const AdamwChunk &ch, const Step8 &a, const AdamwParams &params,
-                                            Stage8 *ring) {
+                                            Stage8 *ring, const Chance &chance) {
     const float wd = t.decay ? a.wd : 0.0f;
     const bool vec = aligned(t.val, 16) && aligned(t.m, 16) && aligned(t.v, 16) && aligned(t.grad, 16) && (!t.copy || aligned(t.copy, 8));
     const uint32_t whole = vec ? ch.n / NK_ADAMW_BLOCK : 0;
@@ -510,13 +565,13 @@ __device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const Adam
         asm volatile("cp.async.commit_group;" ::: "memory");
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES8 - 1) : "memory");
         __syncwarp();  // the other lanes' copies, too
-        ok &= block_step8<G>(t, ch.first + b * NK_ADAMW_BLOCK, ring[from], a, params, wd);
+        ok &= block_step8<G, CHANCE>(t, ch.first + b * NK_ADAMW_BLOCK, ring[from], a, params, wd, chance);
         __syncwarp();  // (before the next copies into it)
         from = from + 1 == STAGES8 ? 0 : from + 1;
         to = to + 1 == STAGES8 ? 0 : to + 1;
     }
     for (uint32_t at = whole * NK_ADAMW_BLOCK; at < ch.n; at += NK_ADAMW_BLOCK)
-        ok &= careful_step8(&t, ch.first + at, min(ch.n - at, (uint32_t)NK_ADAMW_BLOCK), params, a.c);
+        ok &= careful_step8(&t, ch.first + at, min(ch.n - at, (uint32_t)NK_ADAMW_BLOCK), params, a.c, chance);
     return ok;
 }
 
@@ -541,8 +596,11 @@ __global__ void __launch_bounds__(256, 6) adamw32_k(AdamwMany p, AdamwParams a, 
     if (!ok && bad) *bad = 1u;
 }
 
-// 8-bit moments: each warp takes chunks of its own, a ring of blocks ahead.
-__global__ void __launch_bounds__(32 * WARPS8, 2) adamw8_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad) {
+// 8-bit moments: each warp takes chunks of its own, a ring of blocks ahead.  CHANCE: m's
+// or v's bytes are rounded by chance.
+template <bool CHANCE>
+__global__ void __launch_bounds__(32 * WARPS8, 2) adamw8_k(AdamwMany p, AdamwParams a, float grad_scale, bool with_clip, uint32_t *bad,
+                                                           Chance chance) {
     pdl_trigger();
     pdl_wait();
     extern __shared__ Stage8 rings[];
@@ -561,9 +619,9 @@ __global__ void __launch_bounds__(32 * WARPS8, 2) adamw8_k(AdamwMany p, AdamwPar
         i += gridDim.x * WARPS8;
         if (i < p.n_chunks) next = p.chunks[i];
         const nk_adamw_tensor &t = p.tensors[ch.tensor];
-        ok &= t.grad_dtype == NK_F32   ? chunk_step8<float>(t, ch, a8, a, ring)
-              : t.grad_dtype == NK_F16 ? chunk_step8<__half>(t, ch, a8, a, ring)
-                                       : chunk_step8<__nv_bfloat16>(t, ch, a8, a, ring);
+        ok &= t.grad_dtype == NK_F32   ? chunk_step8<float, CHANCE>(t, ch, a8, a, ring, chance)
+              : t.grad_dtype == NK_F16 ? chunk_step8<__half, CHANCE>(t, ch, a8, a, ring, chance)
+                                       : chunk_step8<__nv_bfloat16, CHANCE>(t, ch, a8, a, ring, chance);
     }
     if (!ok && bad) *bad = 1u;
 }
@@ -590,7 +648,7 @@ cudaError_t adamw_many_norm(const AdamwMany &p, float grad_scale, float max_norm
     return pdl_launch(adamw_norm_k, dim3(blocks), dim3(256), 0, st, p, grad_scale, max_norm, norm, bad);
 }
 
-cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, float grad_scale, bool with_clip, uint32_t *bad,
+cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, uint32_t t, float grad_scale, bool with_clip, uint32_t *bad,
                             int sms, cudaStream_t st) {
     const uint32_t n8 = p.n_chunks - p.n_chunks32;
     if (p.n_chunks32) {
@@ -600,10 +658,12 @@ cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, float grad
     }
     if (n8) {
         constexpr int shared = WARPS8 * STAGES8 * (int)sizeof(Stage8);
-        cudaError_t e = allow_shared(adamw8_k, shared);
+        const Chance chance{a.b1 > MOST_TO_NEAREST, a.b2 > MOST_TO_NEAREST, t};
+        auto *k = chance.m || chance.v ? adamw8_k<true> : adamw8_k<false>;
+        cudaError_t e = allow_shared(k, shared);
         if (e != cudaSuccess) return e;
-        return pdl_launch(adamw8_k, dim3(std::min<unsigned>((n8 + WARPS8 - 1) / WARPS8, (unsigned)sms * 2)), dim3(32 * WARPS8), shared, st,
-                          p, a, grad_scale, with_clip, bad);
+        return pdl_launch(k, dim3(std::min<unsigned>((n8 + WARPS8 - 1) / WARPS8, (unsigned)sms * 2)), dim3(32 * WARPS8), shared, st,
+                          p, a, grad_scale, with_clip, bad, chance);
     }
     return cudaSuccess;
 }

@@ -36,7 +36,8 @@ uint32_t adamw_partials(int sms);
 cudaError_t adamw_many_norm(const AdamwMany &p, float grad_scale, float max_norm, float *norm, uint32_t *bad,
                             int sms, cudaStream_t st);
 // with_clip: the factor and the decision come from p.clip; else the factor is grad_scale.
-cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, float grad_scale, bool with_clip, uint32_t *bad,
+// t: the step's counter, for what is rounded by chance.
+cudaError_t adamw_many_step(const AdamwMany &p, const AdamwParams &a, uint32_t t, float grad_scale, bool with_clip, uint32_t *bad,
                             int sms, cudaStream_t st);
 
 // ---- cross entropy from hidden rows (linear_ce.cu)

@@ -389,7 +389,7 @@ nk_status nk_adamw_many_step_device(nk_adamw_many *many, const nk_adamw_cfg *cfg
         Current current(many->device);
         if (norm || max_norm > 0.0f)
             cuda_check(nk::adamw_many_norm(many->plan, grad_scale, max_norm, norm, bad, many->sms, (cudaStream_t)stream), "launch");
-        cuda_check(nk::adamw_many_step(many->plan, a, grad_scale, max_norm > 0.0f, bad, many->sms, (cudaStream_t)stream), "launch");
+        cuda_check(nk::adamw_many_step(many->plan, a, (uint32_t)cfg->t, grad_scale, max_norm > 0.0f, bad, many->sms, (cudaStream_t)stream), "launch");
     });
 }
 

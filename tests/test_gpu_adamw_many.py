@@ -488,3 +488,108 @@ def test_a_moment_that_is_not_finite_spoils_no_other(nb, torch, shift):
     assert torch.equal(t["m_scale"], r["m_scale"]) and torch.equal(t["v_scale"], r["v_scale"])
     t, r = s.t[1], ref.t[1]
     assert torch.equal(t["val"][:256], r["val"][:256]) and torch.equal(t["val"][256:], before[1]["val"][256:])
+
+
+def _pair(torch, n, seed):
+    """The same tensor with 32-bit and with 8-bit moments, all zero."""
+    a, b = Tensors(torch, [n], seed=seed), Tensors(torch, [n], bits=8, seed=seed)
+    for s in (a, b):
+        for k in ("m", "v", "m_scale", "v_scale"):
+            if k in s.t[0]:
+                s.t[0][k].zero_()
+    b.t[0]["val"].copy_(a.t[0]["val"])
+    return a, b
+
+
+def _stored(torch, t, k):
+    return t[k].view(torch.float8_e4m3fn).double() * t[k + "_scale"].double().repeat_interleave(256)[:t["n"]]
+
+
+@pytest.mark.parametrize("noise", [1.0, 0.0])
+@pytest.mark.parametrize("b2,steps", [(0.98, 600), (0.99, 1200), (0.999, 5000)])
+def test_8_bit_roots_follow_gradients_that_shrink(nb, torch, b2, steps, noise):
+    """A third of the way in, half the elements' gradients fall to a tenth.  A stored v's mean
+    is the formula's; one element's is off by the roundings that it remembers: each at most a
+    step's square over 4, (1/8)^2 / 4 of v at a step that moves it that far, and a step's
+    share is (1 - b2) and the scale's: 30% of v an element (measured: 0.32).  25600 of them:
+    0.2%; 5% is far off that and far below what rounding to nearest does (4 to 90 times v)."""
+    n = 51200
+    a, b = _pair(torch, n, 20)
+    pa, pb = a.plan(nb), b.plan(nb)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    size = torch.exp(torch.randn(n, generator=g, device="cuda") - 6)
+    half = torch.arange(n, device="cuda") % 2 == 0
+    for step in range(1, steps + 1):
+        now = size * (torch.randn(n, generator=g, device="cuda") if noise else 1.0)
+        if step > steps // 3:
+            now[half] *= 0.1
+        for s, p in ((a, pa), (b, pb)):
+            s.t[0]["grad"].copy_(now)
+            p.step(**{**HYPER, "t": step, "b2": b2, "wd": 0.0})
+    torch.cuda.synchronize()
+    ratio = _stored(torch, b.t[0], "v").square() / a.t[0]["v"].double()
+    for which in (half, ~half):
+        assert abs(float(ratio[which].mean()) - 1) <= 0.05, (float(ratio[half].mean()), float(ratio[~half].mean()))
+
+
+@pytest.mark.parametrize("b1", [0.98, 0.99])
+def test_8_bit_means_follow_gradients_that_turn(nb, torch, b1):
+    """Gradients without noise, half of which turn round.  A stored m's mean is the formula's:
+    over 25600 elements the errors (at most 1/16 of m each, and 1 / sqrt(1 - b1^2) of that
+    remembered: 0.44) average to 0.3%; to nearest, m had not turned at all."""
+    n, steps = 51200, 1500
+    a, b = _pair(torch, n, 21)
+    pa, pb = a.plan(nb), b.plan(nb)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    size = torch.exp(torch.randn(n, generator=g, device="cuda") - 6)
+    half = torch.arange(n, device="cuda") % 2 == 0
+    for step in range(1, steps + 1):
+        for s, p in ((a, pa), (b, pb)):
+            s.t[0]["grad"].copy_(torch.where(half & (step > steps // 2), -size, size))
+            p.step(**{**HYPER, "t": step, "b1": b1, "wd": 0.0})
+    torch.cuda.synchronize()
+    ratio = _stored(torch, b.t[0], "m") / a.t[0]["m"].double()
+    for which in (half, ~half):
+        assert abs(float(ratio[which].mean()) - 1) <= 0.05, float(ratio[which].mean())
+
+
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+def test_rounding_by_chance_is_between_neighbours_in_proportion_and_repeats(nb, torch, grad):
+    n = 1 << 18
+    hyper = {**HYPER, "b1": 0.96, "b2": 0.97}
+    sets = [Tensors(torch, [n, 1000], grad, 8, shift=shift, seed=22) for shift in (0, 0, 3)]
+    for s in sets:
+        s.t[0]["val"].copy_(sets[0].t[0]["val"])
+        # (Roots that are not tiny: of those the floor moves the mean.  127 is no number.)
+        s.t[0]["v"].copy_((s.t[0]["v"] | 8).clamp(max=126))
+    before = sets[0].clone()
+    for s in sets:
+        s.plan(nb).step(**hyper)
+    torch.cuda.synchronize()
+    for i, t in enumerate(sets[0].t):
+        for o in sets[1:]:
+            assert all(torch.equal(t[k], o.t[i][k]) for k in ("val", "m", "v", "m_scale", "v_scale"))
+    t, want = sets[0].t[0], _want(torch, before[0], 1.0, HYPER["lr"], 7, 0.96, 0.97, 1e-8, 0.1, 8)
+    err = (t["val"].double() - want["val"]).abs()
+    assert (err <= U * want["val"].abs() + want["val_tol"]).all()
+    for k in ("m", "v"):
+        scale = t[k + "_scale"].double().repeat_interleave(256)
+        y, code = (want[k] / scale).abs(), t[k].view(torch.float8_e4m3fn).double()
+        assert ((code == 0) | (torch.sign(code) == torch.sign(want[k]))).all()
+        code = code.abs()
+        slack = 32 * U * y + want[k + "_tol"] / scale
+        # Within a step, and one of the two beside it where it is not on the grid itself.
+        step = torch.exp2(torch.floor(torch.log2(torch.maximum(y, code).clamp(min=2.0**-6))) - 3)
+        assert ((code - y).abs() < step + slack).all()
+        # The further of the two takes its share (what lies near the middle left out).
+        f = torch.frac(y / torch.exp2(torch.floor(torch.log2(y.clamp(min=2.0**-6))) - 3))
+        share = float(((code - y).abs() > step * 0.51).double().mean())
+        assert share > 0.5 * float(torch.minimum(f, 1 - f).mean()) > 0.01
+        # Its mean (the square's), over elements of one size: 6 deviations of at most half a step each.
+        for lo in (2.0**-7, 0.5, 3.0, 40.0, 200.0):
+            at = (y >= lo) & (y < 2 * lo)
+            if int(at.sum()) <= 500 and lo < 3.0:  # (v: none so small)
+                continue
+            d = code[at] - y[at] if k == "m" else (code[at].square() - y[at].square()) / (2 * y[at])
+            most = float(step[at].max()) / 2 * 1.1
+            assert abs(float(d.mean())) <= 6 * most / int(at.sum()) ** 0.5, (k, lo, float(d.mean()), most)
