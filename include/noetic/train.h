@@ -48,9 +48,13 @@ nk_status nk_linear_ce(const void *x, int dtype, uint64_t rows, uint64_t width, 
                        const uint32_t *targets, float *loss, float *stats, int device);
 
 /* The workspace of the call above (backward == 0) or below.  w: where the
- * matrix will be; what counts is its place within 16 bytes and its stride (one
+ * matrix will be; what counts is its place within 128 bytes and its stride.  One
  * that does not start its rows on 16-byte boundaries is copied, and so is an f32
- * one, as two 16-bit parts). */
+ * one, as two 16-bit parts.  One of 16 bits whose rows start on 16-byte but not on
+ * 128-byte boundaries is copied from 1024 rows on (2048 without gradients), if the
+ * workspace has the room that is asked for here; the size for a place on 128 bytes
+ * (256, say) does for it too, and the call is up to 30% slower then, with the same
+ * results. */
 nk_status nk_linear_ce_workspace(int dtype, uint64_t rows, uint64_t width, uint64_t vocab, const void *w,
                                  uint64_t w_stride, int backward, uint64_t *bytes);
 

@@ -592,7 +592,9 @@ int few_blocks(int64_t rows, int vocab) {
     return (int)((whole + rounds - 1) / rounds);
 }
 
-Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride, bool backward) {
+// lines_pay: w is copied where its rows start on 16-byte but not on 128-byte boundaries and
+// that pays.
+Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride, bool backward, bool lines_pay) {
     Plan p;
     auto room = [&](size_t n) {
         const size_t at = p.bytes;
@@ -607,7 +609,7 @@ Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int
     p.dp = (int64_t)round_up((size_t)width, 64);
     p.split = dtype == NK_F32;
     const bool lines = ((uintptr_t)w & 127) == 0 && w_stride % 64 == 0, units = ((uintptr_t)w & 15) == 0 && w_stride % 8 == 0;
-    p.copy_w = p.split || !units || (!lines && rows >= (backward ? 1024 : 2048));
+    p.copy_w = p.split || !units || (lines_pay && !lines && rows >= (backward ? 1024 : 2048));
     const size_t parts = p.split ? 2 : 1;
     p.head = room(sizeof(Head));
     if (p.split) p.scales = room(((size_t)p.mp + round_up((size_t)vocab, ce::TN)) * 4);
@@ -668,7 +670,7 @@ struct Call {
     int64_t w_ld, w_cols;
 
     Call(const LinearCeArgs &args, bool backward, int n_sms, cudaStream_t stream)
-        : a(args), p(make_plan(args.dtype, args.rows, args.width, args.vocab, args.w, args.w_stride, backward)), sms(n_sms), st(stream),
+        : a(args), p(make_plan(args.dtype, args.rows, args.width, args.vocab, args.w, args.w_stride, backward, args.copy_lines)), sms(n_sms), st(stream),
           ws((char *)args.workspace) {
         ix = {at<Head>(p.head), at<uint32_t>(p.row_of), at<uint32_t>(p.place), at<uint32_t>(p.target), at<float2>(p.stats), at<float>(p.weight)};
         scales = at<float>(p.scales);
@@ -857,8 +859,8 @@ struct Call {
 void linear_ce_withhold(int product) { g_withhold = product; }
 
 size_t linear_ce_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
-                                 bool backward) {
-    return make_plan(dtype, rows, width, vocab, w, w_stride, backward).bytes;
+                                 bool backward, bool copy_lines) {
+    return make_plan(dtype, rows, width, vocab, w, w_stride, backward, copy_lines).bytes;
 }
 
 cudaError_t linear_ce(const LinearCeArgs &a, int sms, cudaStream_t st) {

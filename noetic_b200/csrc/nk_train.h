@@ -56,9 +56,11 @@ struct LinearCeArgs {
     int64_t dx_stride, dw_stride;
     int dw_dtype, accumulate;
     void *workspace;
+    bool copy_lines;
 };
+// copy_lines: with room for a copy of a w that is not on 128-byte lines, where one pays.
 size_t linear_ce_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
-                                 bool backward);
+                                 bool backward, bool copy_lines);
 void linear_ce_withhold(int product);  // nk_linear_ce_withhold
 cudaError_t linear_ce(const LinearCeArgs &a, int sms, cudaStream_t st);
 cudaError_t linear_ce_backward(const LinearCeArgs &a, int sms, cudaStream_t st);

@@ -44,6 +44,21 @@ void check_linear_ce(int dtype, uint64_t rows, uint64_t width, uint64_t x_stride
     check_f32({targets});
 }
 
+// The bytes that a call takes of its workspace.  One without room for a copy of w that only
+// makes the call faster will do: the sizes for a w on 128-byte lines serve any on 16 bytes.
+uint64_t check_workspace(int dtype, uint64_t rows, uint64_t width, uint64_t vocab, const void *w, uint64_t w_stride, bool backward,
+                         const void *workspace, uint64_t have, bool &copy_lines) {
+    need(workspace, "null workspace");
+    check_aligned(workspace, 256, "workspace");
+    uint64_t bytes = 0;
+    for (const bool lines : {true, false}) {
+        copy_lines = lines;
+        bytes = nk::linear_ce_workspace_bytes(dtype, (int64_t)rows, (int)width, (int)vocab, w, (int64_t)w_stride, backward, lines);
+        if (have >= bytes) return bytes;
+    }
+    fail(NK_ERR_INVALID, "the workspace is smaller than nk_linear_ce_workspace says");
+}
+
 // ---------------------------------------------------------------- AdamW
 // AdamW::step's checks and bias corrections (optim.rs:35-47), on the host.
 nk::AdamwParams adamw_params(const nk_adamw_cfg *cfg, float grad_scale, float max_norm) {
@@ -165,7 +180,7 @@ nk_status nk_linear_ce_workspace(int dtype, uint64_t rows, uint64_t width, uint6
         const uint32_t some = 0;
         check_linear_ce(dtype, rows, width, width, vocab, w_stride, &some, w, &some);
         *bytes = nk::linear_ce_workspace_bytes(dtype, (int64_t)rows, (int)width, (int)vocab, w, (int64_t)w_stride,
-                                               backward != 0);
+                                               backward != 0, true);
     });
 }
 
@@ -177,11 +192,8 @@ nk_status nk_linear_ce_device(const void *x, int dtype, uint64_t rows, uint64_t 
         check_f32({loss, stats});
         if (rows == 0) return;
         need(loss || stats, "loss and stats are both null");
-        const uint64_t bytes = nk::linear_ce_workspace_bytes(dtype, (int64_t)rows, (int)width, (int)vocab, w,
-                                                             (int64_t)w_stride, false);
-        need(workspace, "null workspace");
-        check_aligned(workspace, 256, "workspace");
-        need(workspace_bytes >= bytes, "the workspace is smaller than nk_linear_ce_workspace says");
+        bool copy_lines = true;
+        const uint64_t bytes = check_workspace(dtype, rows, width, vocab, w, w_stride, false, workspace, workspace_bytes, copy_lines);
         const int es = elem_size(dtype);
         check_apart({{loss, rows * 4}, {stats, rows * 8}, {workspace, bytes}},
                     {matrix_span(x, rows, width, x_stride, es), matrix_span(w, vocab, width, w_stride, es), {targets, rows * 4}});
@@ -199,6 +211,7 @@ nk_status nk_linear_ce_device(const void *x, int dtype, uint64_t rows, uint64_t 
         a.loss = loss;
         a.stats = stats;
         a.workspace = workspace;
+        a.copy_lines = copy_lines;
         cuda_check(nk::linear_ce(a, sm_count(), (cudaStream_t)stream), "launch");
     });
 }
@@ -245,11 +258,8 @@ nk_status nk_linear_ce_backward_device(const void *x, int dtype, uint64_t rows, 
             check_aligned(dw, elem_size(dw_dtype), "dw");
         }
         if (rows == 0 && (!dw || accumulate)) return;
-        const uint64_t bytes = nk::linear_ce_workspace_bytes(dtype, (int64_t)rows, (int)width, (int)vocab, w,
-                                                             (int64_t)w_stride, true);
-        need(workspace, "null workspace");
-        check_aligned(workspace, 256, "workspace");
-        need(workspace_bytes >= bytes, "the workspace is smaller than nk_linear_ce_workspace says");
+        bool copy_lines = true;
+        const uint64_t bytes = check_workspace(dtype, rows, width, vocab, w, w_stride, true, workspace, workspace_bytes, copy_lines);
         const Span sx = matrix_span(x, rows, width, x_stride, es), sw = matrix_span(w, vocab, width, w_stride, es);
         check_apart({matrix_span(dx, rows, width, dx_stride, es), matrix_span(dw, vocab, width, dw_stride, dw ? elem_size(dw_dtype) : 0), {workspace, bytes}},
                     {sx, sw, {targets, rows * 4}, {stats, rows * 8}, {row_weight, rows * 4}});
@@ -276,6 +286,7 @@ nk_status nk_linear_ce_backward_device(const void *x, int dtype, uint64_t rows, 
         a.dw_dtype = dw_dtype;
         a.accumulate = accumulate != 0;
         a.workspace = workspace;
+        a.copy_lines = copy_lines;
         cuda_check(nk::linear_ce_backward(a, sm_count(), (cudaStream_t)stream), "launch");
     });
 }

@@ -48,7 +48,7 @@ def linear_ce_workspace(dtype: int, rows: int, width: int, vocab: int, w: int = 
                         backward: bool = False) -> int:
     """Bytes of workspace that ``nk_linear_ce_device`` (``backward``:
     ``nk_linear_ce_backward_device``) needs; ``w`` is the address of the
-    vocabulary matrix."""
+    vocabulary matrix, of which the place within 128 bytes counts."""
     nb = _nb()
     n = _u64()
     nb._check(nb.lib().nk_linear_ce_workspace(dtype, rows, width, vocab, w, width if w_stride is None else w_stride,

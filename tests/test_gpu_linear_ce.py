@@ -614,3 +614,22 @@ def test_probabilities_of_logits_far_from_zero(nb, torch, dtype, top):
         _p(room), room.numel(), _st(torch)))
     off = (dw[1:].double() / top) / torch.exp(-ls.double()) - 1
     assert float(off.abs().max()) <= {"f16": 2.0**-11, "bf16": 2.0**-8, "f32": 2.0**-22}[dtype] + 20 * U, float(off.abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_w_off_128_bytes_in_a_workspace_for_one_on_them(nb, torch, dtype):
+    """2100 rows, from which on such a w is copied where there is room: the same numbers without."""
+    rows, width, vocab = 2100, 192, 1100
+    c = Case(torch, rows, width, vocab, dtype, ignored=0.1, shift=8, seed=61)
+    assert c.w.data_ptr() % 128 == 16
+    room = [nb.train.linear_ce_workspace(CODE[dtype], rows, width, vocab, w, width, back) for w in (256, 272) for back in (False, True)]
+    assert room[0] < room[2] and room[1] < room[3]
+    loss, stats = c.forward(nb)
+    c.check_forward(loss, stats)
+    dx, dw = c.backward(nb, stats, 0.5)
+    c.check_backward(stats, 0.5, dx, dw)
+    small = [torch.full((n + 64,), 255, device="cuda", dtype=torch.uint8) for n in room[:2]]
+    got = c.forward(nb, small[0]) + c.backward(nb, stats, 0.5, room=small[1])
+    for a, b in zip(got, (loss, stats, dx, dw)):
+        assert torch.equal(a, b)
+    assert all((s[-64:] == 255).all() for s in small)

@@ -174,3 +174,26 @@ def test_python_mirror_refuses_shapes(nb):
                                                  m_scale=np.zeros(2), v_scale=np.zeros(1))], 0.1, 1)]:
         with pytest.raises(ValueError):
             bad()
+
+
+def _far(nb, name, rows, width, vocab, dtype, w, room):
+    """Whether a call is refused for its workspace.  (At these addresses there is nothing, and no
+    call gets as far as looking.)"""
+    a = dict(_calls(1 << 40)[name], dtype=dtype, rows=rows, width=width, x_stride=width, x=2 << 40, w=(3 << 40) + w, vocab=vocab,
+             w_stride=width, targets=4 << 40, stats=5 << 40, workspace=6 << 40, workspace_bytes=room)
+    a.update(dict(loss=7 << 40) if "loss" in a else dict(row_weight=None, dx=8 << 40, dx_stride=width, dw=9 << 40, dw_dtype=dtype,
+                                                         dw_stride=width))
+    st = _call(nb, name, a)
+    assert st != nb.NK_OK
+    return st == nb.NK_ERR_INVALID and "workspace" in nb.lib().nk_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,width,vocab", [(8192, 1024, 32768), (2048, 768, 16384), (1024, 72, 3000), (100, 64, 1000)])
+def test_a_workspace_serves_every_place_of_w_on_16_bytes(nb, dtype, rows, width, vocab):
+    for name, back in (("nk_linear_ce_device", False), ("nk_linear_ce_backward_device", True)):
+        n = [nb.train.linear_ce_workspace(dtype, rows, width, vocab, w=w, backward=back) for w in (256, 272, 320, 384)]
+        assert n[0] == n[3] <= n[1] == n[2]  # (its place within 128 bytes)
+        for w in (0, 16, 64, 112):
+            assert not _far(nb, name, rows, width, vocab, dtype, w, n[0])
+        assert _far(nb, name, rows, width, vocab, dtype, 16, 4096)
