@@ -47,7 +47,8 @@ nk_status nk_linear_ce_device(const void *x, int dtype, uint64_t rows, uint64_t 
 nk_status nk_linear_ce(const void *x, int dtype, uint64_t rows, uint64_t width, const void *w, uint64_t vocab,
                        const uint32_t *targets, float *loss, float *stats, int device);
 
-/* The workspace of the call above (backward == 0) or below.  w: where the
+/* The workspace of the call above (backward == 0) or below, with any number of rows up
+ * to `rows`.  w: where the
  * matrix will be; what counts is its place within 128 bytes and its stride.  One
  * that does not start its rows on 16-byte boundaries is copied, and so is an f32
  * one, as two 16-bit parts.  One of 16 bits whose rows start on 16-byte but not on

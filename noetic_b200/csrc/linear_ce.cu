@@ -546,6 +546,7 @@ struct Plan {
            dx = 0, dw = 0, bytes = 0;
 };
 
+constexpr int PAIRS = 74;  // of 148 SMs: the workspace does not go by the device
 // An item's time in K-blocks: its own, or its sums' way out, which the next item's
 // K-blocks cover; and a piece's sums on their way to memory and back.
 constexpr int STORE_COST = 24, SPLIT_COST = 16;
@@ -640,12 +641,35 @@ Plan make_plan(int dtype, int64_t rows, int width, int vocab, const void *w, int
     p.ldg = (int64_t)round_up((size_t)p.piece, ce::TN);
     p.g = room((size_t)p.mp * p.ldg * 2 * parts);
     p.ld_acc = (int64_t)round_up((size_t)width, ce::TN);
-    const int pairs = 74;
+    const int pairs = PAIRS;
     const int64_t nt = p.ld_acc / ce::TN, segs = p.split ? 3 : 1;
     pick_splits(p.mp / ce::TM * nt, p.ldg / ce::BK * segs, p.ldg / ce::TN * nt, p.mp / ce::BK * segs, pairs, p.dx_splits, p.dw_splits);
     if (p.dx_splits > 1 || p.piece < vocab) p.dx = room((size_t)p.dx_splits * p.mp * p.ld_acc * 4);
     if (p.dw_splits > 1) p.dw = room((size_t)p.dw_splits * p.ldg * p.ld_acc * 4);
     return p;
+}
+
+// What any call of up to `rows` rows takes at most.  Everything in a plan grows with the rows
+// but three things, which have bounds that do: G (PIECE_BYTES, or 1024 tokens of all rows), the
+// sums of a split dx or dw (256 x 256 sums of 4 items a pair at most, and no more splits than K
+// has 8 K-blocks for), and the few rows' partial results.
+size_t most_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride, bool backward) {
+    Plan p = make_plan(dtype, rows, width, vocab, w, w_stride, backward, true);
+    const auto whole = [](uint64_t n) { return round_up(n, 256); };
+    if (!backward) {
+        if (((uintptr_t)w & 15) != 0) return p.bytes;
+        const uint64_t cols = (uint64_t)(vocab + FEW_WARPS * COLS - 1) / (FEW_WARPS * COLS), some = std::min<int64_t>(rows, 4096);
+        const size_t few = whole(8 * std::min(some * cols, std::max(592 * std::min<uint64_t>(some, 8), some))) + whole(some * 4);
+        return std::max(p.bytes, few);
+    }
+    const uint64_t parts = p.split ? 2 : 1, segs = p.split ? 3 : 1, mp = (uint64_t)p.mp, tokens = round_up((size_t)vocab, ce::TN);
+    const uint64_t row = (uint64_t)p.ld_acc * 4, split = 4 * PAIRS * (uint64_t)ce::TM * ce::TN * 4;
+    const uint64_t kx = std::min<uint64_t>(tokens * segs / (8 * ce::BK), 64), kw = std::min<uint64_t>(mp * segs / (8 * ce::BK), 64);
+    const uint64_t g = std::min(mp * tokens * 2 * parts, std::max(PIECE_BYTES, mp * std::min<uint64_t>(tokens, 4 * ce::TN) * 2 * parts));
+    uint64_t dx = kx > 1 ? std::min(split, kx * mp * row) : 0;
+    if (p.piece < vocab) dx = std::max(dx, mp * row);
+    const uint64_t dw = kw > 1 ? std::min(split, kw * tokens * row) : 0;
+    return p.g + whole(g) + whole(dx) + whole(dw);
 }
 
 // Instruction descriptor: f32 sums, f16 or bf16 factors, 256 x 256, majors.
@@ -861,6 +885,10 @@ void linear_ce_withhold(int product) { g_withhold = product; }
 size_t linear_ce_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
                                  bool backward, bool copy_lines) {
     return make_plan(dtype, rows, width, vocab, w, w_stride, backward, copy_lines).bytes;
+}
+
+size_t linear_ce_most_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride, bool backward) {
+    return most_bytes(dtype, rows, width, vocab, w, w_stride, backward);
 }
 
 cudaError_t linear_ce(const LinearCeArgs &a, int sms, cudaStream_t st) {

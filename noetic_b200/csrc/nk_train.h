@@ -62,6 +62,9 @@ struct LinearCeArgs {
 size_t linear_ce_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
                                  bool backward, bool copy_lines);
 void linear_ce_withhold(int product);  // nk_linear_ce_withhold
+// What calls of up to `rows` rows take at most.
+size_t linear_ce_most_workspace_bytes(int dtype, int64_t rows, int width, int vocab, const void *w, int64_t w_stride,
+                                      bool backward);
 cudaError_t linear_ce(const LinearCeArgs &a, int sms, cudaStream_t st);
 cudaError_t linear_ce_backward(const LinearCeArgs &a, int sms, cudaStream_t st);
 

@@ -179,8 +179,7 @@ nk_status nk_linear_ce_workspace(int dtype, uint64_t rows, uint64_t width, uint6
         *bytes = 0;
         const uint32_t some = 0;
         check_linear_ce(dtype, rows, width, width, vocab, w_stride, &some, w, &some);
-        *bytes = nk::linear_ce_workspace_bytes(dtype, (int64_t)rows, (int)width, (int)vocab, w, (int64_t)w_stride,
-                                               backward != 0, true);
+        *bytes = nk::linear_ce_most_workspace_bytes(dtype, (int64_t)rows, (int)width, (int)vocab, w, (int64_t)w_stride, backward != 0);
     });
 }
 

@@ -47,7 +47,7 @@ SIGNATURES = {
 def linear_ce_workspace(dtype: int, rows: int, width: int, vocab: int, w: int = 256, w_stride: int | None = None,
                         backward: bool = False) -> int:
     """Bytes of workspace that ``nk_linear_ce_device`` (``backward``:
-    ``nk_linear_ce_backward_device``) needs; ``w`` is the address of the
+    ``nk_linear_ce_backward_device``) needs for up to ``rows`` rows; ``w`` is the address of the
     vocabulary matrix, of which the place within 128 bytes counts."""
     nb = _nb()
     n = _u64()

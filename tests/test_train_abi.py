@@ -197,3 +197,20 @@ def test_a_workspace_serves_every_place_of_w_on_16_bytes(nb, dtype, rows, width,
         for w in (0, 16, 64, 112):
             assert not _far(nb, name, rows, width, vocab, dtype, w, n[0])
         assert _far(nb, name, rows, width, vocab, dtype, 16, 4096)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("width,vocab", [(768, 16384), (333, 131072), (24, 37), (1, 1), (64, 1000), (2048, 131072), (4097, 5000),
+                                         (1024, 32768), (192, 300), (2304, 2048)])
+def test_a_workspace_serves_any_fewer_rows(nb, dtype, width, vocab):
+    rng = np.random.default_rng(width)
+    most = min(1 << 17, (1 << 37) // vocab)
+    sizes = sorted({1, 4, 5, 8, 9, 255, 256, 257, 1023, 1024, 2048, 4096, 4411, 5419, most,
+                    *np.exp(rng.uniform(0, np.log(most), 40)).astype(int).tolist()})
+    for name, back in (("nk_linear_ce_device", False), ("nk_linear_ce_backward_device", True)):
+        for w in (0, 16, 4):
+            n = [nb.train.linear_ce_workspace(dtype, rows, width, vocab, w=(3 << 40) + w, backward=back) for rows in sizes]
+            assert n == sorted(n)
+            for i, rows in enumerate(sizes):
+                for fewer in {rows, *sizes[max(0, i - 6):i], *rng.integers(1, rows + 1, 6).tolist()}:
+                    assert not _far(nb, name, fewer, width, vocab, dtype, w, n[i]), (rows, fewer, n[i])
