@@ -152,6 +152,15 @@ class AdamwMany:
             self.close()
 
 
+def _moment(a, kind, what):
+    """A copy of a moment: float32, or codes of 8 bits, which no other numbers stand for."""
+    a = np.asarray(a)
+    new = np.array(a, kind).reshape(-1)
+    if a.dtype != kind and (a.dtype == np.uint8 or (kind == np.uint8 and not np.array_equal(new, a.reshape(-1)))):
+        raise ValueError(f"{what}: codes of 8 bits need m_scale and v_scale, and scales need codes")
+    return new
+
+
 def adamw_step_many(tensors, lr: float, t: int, b1: float = 0.9, b2: float = 0.95, eps: float = 1e-8, wd: float = 0.0,
                     grad_scale: float = 1.0, max_norm: float = 0.0, device: int = 0):
     """One AdamW step over copies of all ``tensors``, each a dict of arrays ``val``,
@@ -168,7 +177,7 @@ def adamw_step_many(tensors, lr: float, t: int, b1: float = 0.9, b2: float = 0.9
         grad = np.ascontiguousarray(grad if grad.dtype in codes else grad.astype(np.float32)).reshape(-1)
         bits = 8 if t_in.get("m_scale") is not None else 32
         kind = np.uint8 if bits == 8 else np.float32
-        new = {"val": val, "m": np.array(t_in["m"], kind).reshape(-1), "v": np.array(t_in["v"], kind).reshape(-1)}
+        new = {"val": val, "m": _moment(t_in["m"], kind, "m"), "v": _moment(t_in["v"], kind, "v")}
         if bits == 8:
             blocks = -(-val.size // NK_ADAMW_BLOCK)
             for k in ("m_scale", "v_scale"):

@@ -214,3 +214,16 @@ def test_a_workspace_serves_any_fewer_rows(nb, dtype, width, vocab):
             for i, rows in enumerate(sizes):
                 for fewer in {rows, *sizes[max(0, i - 6):i], *rng.integers(1, rows + 1, 6).tolist()}:
                     assert not _far(nb, name, fewer, width, vocab, dtype, w, n[i]), (rows, fewer, n[i])
+
+
+def test_python_mirror_refuses_moments_of_another_kind_than_their_scales(nb):
+    """Values taken as codes lost their fractions, and codes taken as values their scales."""
+    def step(m, v, **scales):
+        z = np.zeros(4, np.float32)
+        return nb.adamw_step_many([dict(val=z, grad=z, m=m, v=v, **scales)], 0.1, 1)
+
+    values, codes, one = np.full(4, 0.3, np.float32), np.full(4, 90, np.uint8), np.ones(1, np.float32)
+    for m, v, scales in [(values, codes, True), (codes, values, True), (np.full(4, 300.0), codes, True), (-codes.astype(int), codes, True),
+                         (codes, values, False), (values, codes, False)]:
+        with pytest.raises(ValueError, match="codes"):
+            step(m, v, **(dict(m_scale=one, v_scale=one) if scales else {}))
