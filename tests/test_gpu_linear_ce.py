@@ -633,3 +633,66 @@ def test_w_off_128_bytes_in_a_workspace_for_one_on_them(nb, torch, dtype):
     for a, b in zip(got, (loss, stats, dx, dw)):
         assert torch.equal(a, b)
     assert all((s[-64:] == 255).all() for s in small)
+
+
+_TRIES = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64)
+
+
+def _up(n, to):
+    return -(-n // to) * to
+
+
+def _deal(items0, cost0, items1, cost1, pairs):
+    """How many items of the second product a pair with one more, or one less, of the first takes."""
+    more, q = items0 % pairs, items0 // pairs
+    high, low = (q + 1) * cost0, q * cost0
+    level = (items0 * cost0 + items1 * cost1 + pairs - 1) // pairs
+    while True:
+        n = [max(0, level - high) // cost1, max(0, level - low) // cost1]
+        if more * n[0] + (pairs - more) * n[1] >= items1:
+            return more, n[0], max(n)
+        a, b = high + (n[0] + 1) * cost1, low + (n[1] + 1) * cost1
+        level = a if more and a < b else b
+
+
+def _cuts(dtype, rows, width, vocab, pairs=74):
+    """(tokens of a piece, pieces of K of dx, of dw): the rule of a gradient call, restated."""
+    parts, segs = (2, 3) if dtype == "f32" else (1, 1)
+    mp = _up(max(rows, 1), 256)
+    piece = min(max((256 << 20) // 2 // parts // mp // 256 * 256, 1024), vocab)
+    ldg, nt = _up(piece, 256), _up(width, 256) // 256
+    tx, kx, tw, kw = mp // 256 * nt, ldg // 64 * segs, ldg // 256 * nt, mp // 64 * segs
+    least, best = 1e300, (1, 1)
+    for i in _TRIES:
+        for j in _TRIES:
+            if (i > 1 and (kx // i < 8 or tx * i > 4 * pairs)) or (j > 1 and (kw // j < 8 or tw * j > 4 * pairs)):
+                continue
+            cx, cw = max(-(-kx // i), 24) + 4 + 16 * (i > 1), max(-(-kw // j), 24) + 4 + 16 * (j > 1)
+            more, n0, n1 = _deal(tx * i, cx, tw * j, cw, pairs)
+            q = tx * i // pairs
+            cost = max((q + 1) * cx + n0 * cw if more else 0, q * cx + n1 * cw)
+            if cost < least * 0.97:
+                least, best = cost, (i, j)
+    return (piece, *best)
+
+
+@pytest.mark.parametrize("dtype,rows,width,vocab,want", [
+    ("bf16", 16384, 320, 19001, (8192, 1, 1)), ("f16", 12288, 768, 19001, (10752, 1, 1)), ("f32", 8192, 320, 19001, (8192, 1, 1)),
+    ("bf16", 18944, 512, 13001, (6912, 1, 4))])
+def test_pieces_whose_sums_stay_whole(nb, torch, dtype, rows, width, vocab, want):
+    """Several pieces of the vocabulary, the last one short, several column tiles, w read where it
+    stands (16 bits), and no piece of K for dx: its sums wait in one buffer and leave with the
+    last piece, as those of a large training batch do."""
+    assert _cuts(dtype, rows, width, vocab) == want and width % 64 == 0 and rows >= 1024
+    c = Case(torch, rows, width, vocab, dtype, ignored=0.05, seed=70)
+    assert c.w.data_ptr() % 128 == 0
+    loss, stats = c.forward(nb)
+    c.check_forward(loss, stats)
+    torch.cuda.empty_cache()
+    dx, dw = c.backward(nb, stats, 1 / rows)
+    c.check_backward(stats, 1 / rows, dx, dw)
+    base = torch.randn(vocab, width, device="cuda") / rows
+    torch.cuda.empty_cache()
+    dx, dw = c.backward(nb, stats, 1 / rows, dw_dtype="f32", dw=base.clone())
+    c.check_backward(stats, 1 / rows, dx, dw, base)
+    torch.cuda.empty_cache()
