@@ -268,12 +268,6 @@ __device__ __forceinline__ float grid_scale(float top) {
     return E4M3_MAX * fmaf(fmaf(-top, r, 1.0f), r, r);
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-
 __device__ __forceinline__ float rcp(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -312,13 +306,6 @@ struct __align__(16) Stage8 {
     uint32_t m[NK_ADAMW_BLOCK / 4], v[NK_ADAMW_BLOCK / 4];
     float scale[4];  // of m and of v
 };
-
-__device__ __forceinline__ void copy16(void *to, const void *from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy4(void *to, const void *from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
 
 __device__ __forceinline__ float grad_of(const void *grad, int dtype, uint64_t i) {
     return dtype == NK_F32 ? ((const float *)grad)[i] : dtype == NK_F16 ? to_f32(((const __half *)grad)[i]) : to_f32(((const __nv_bfloat16 *)grad)[i]);
@@ -392,8 +379,8 @@ __device__ __noinline__ bool careful_step8(const nk_adamw_tensor *tp, uint64_t f
             top_m = fmaxf(top_m, fabsf(g[h][e]));
             top_r = fmaxf(top_r, rv[h][e]);
         }
-    top_m = warp_max(top_m);
-    top_r = warp_max(top_r);
+    top_m = warp_max1(top_m);
+    top_r = warp_max1(top_r);
     const float km = top_m >= SCALE_MIN ? grid_scale(top_m) : 0.0f;
     const float kr = top_r >= SCALE_MIN ? grid_scale(top_r) : 0.0f;
     // A root above 0 stays above 0: a later step divides by it.
@@ -482,8 +469,8 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
         top_m = fmaxf(top_m, fmaxf(fabsf(mv[o].x), fabsf(mv[o].y)));
         top_r = fmaxf(top_r, fmaxf(root[o].x, root[o].y));
     }
-    top_m = warp_max(top_m);
-    top_r = warp_max(top_r);
+    top_m = warp_max1(top_m);
+    top_r = warp_max1(top_r);
     if (__any_sync(0xffffffffu, !(strange.x + strange.y == 0.0f)) || top_m > MOMENT_MAX)
         return careful_step8(&t, first, NK_ADAMW_BLOCK, params, a.c, chance);
     const float km = top_m >= SCALE_MIN ? grid_scale(top_m) : 0.0f;
@@ -531,19 +518,19 @@ __device__ __forceinline__ bool block_step8(const nk_adamw_tensor &t, uint64_t f
 template <class G>
 __device__ __forceinline__ void issue8(const nk_adamw_tensor &t, uint64_t e, Stage8 &st) {
     const int lane = threadIdx.x & 31;
-    copy16(&st.val[lane * 4], t.val + e + lane * 4);
-    copy16(&st.val[128 + lane * 4], t.val + e + 128 + lane * 4);
+    copy_async16(&st.val[lane * 4], t.val + e + lane * 4);
+    copy_async16(&st.val[128 + lane * 4], t.val + e + 128 + lane * 4);
     if constexpr (sizeof(G) == 4) {
-        copy16(&st.grad[lane * 4], (const G *)t.grad + e + lane * 4);
-        copy16(&st.grad[128 + lane * 4], (const G *)t.grad + e + 128 + lane * 4);
+        copy_async16(&st.grad[lane * 4], (const G *)t.grad + e + lane * 4);
+        copy_async16(&st.grad[128 + lane * 4], (const G *)t.grad + e + 128 + lane * 4);
     } else {
-        copy16(&st.grad[lane * 4], (const G *)t.grad + e + lane * 8);
+        copy_async16(&st.grad[lane * 4], (const G *)t.grad + e + lane * 8);
     }
     if (lane < 16)
-        copy16(&st.m[lane * 4], (const uint8_t *)t.m + e + lane * 16);
+        copy_async16(&st.m[lane * 4], (const uint8_t *)t.m + e + lane * 16);
     else
-        copy16(&st.v[lane * 4 - 64], (const uint8_t *)t.v + e + lane * 16 - 256);
-    if (lane < 2) copy4(&st.scale[lane], (lane ? t.v_scale : t.m_scale) + e / NK_ADAMW_BLOCK);
+        copy_async16(&st.v[lane * 4 - 64], (const uint8_t *)t.v + e + lane * 16 - 256);
+    if (lane < 2) copy_async4(&st.scale[lane], (lane ? t.v_scale : t.m_scale) + e / NK_ADAMW_BLOCK);
 }
 
 // A warp's chunk, STAGES8 - 1 blocks ahead.
@@ -557,13 +544,13 @@ __device__ __forceinline__ bool chunk_step8(const nk_adamw_tensor &t, const Adam
 #pragma unroll
     for (uint32_t s = 0; s < STAGES8 - 1; ++s) {
         if (s < whole) issue8<G>(t, ch.first + s * NK_ADAMW_BLOCK, ring[s]);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        copy_commit();
     }
     int from = 0, to = STAGES8 - 1;
     for (uint32_t b = 0; b < whole; ++b) {
         if (b + STAGES8 - 1 < whole) issue8<G>(t, ch.first + (b + STAGES8 - 1) * NK_ADAMW_BLOCK, ring[to]);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES8 - 1) : "memory");
+        copy_commit();
+        copy_wait<STAGES8 - 1>();
         __syncwarp();  // the other lanes' copies, too
         ok &= block_step8<G, CHANCE>(t, ch.first + b * NK_ADAMW_BLOCK, ring[from], a, params, wd, chance);
         __syncwarp();  // (before the next copies into it)
