@@ -67,9 +67,10 @@ nk_status nk_linear_ce_workspace(int dtype, uint64_t rows, uint64_t width, uint6
  * at a time.  dx (type of x) and dw (type of w, or f32: dw_dtype) are each
  * nullable, not both; accumulate != 0 adds to dw (dx is set).  Rows whose target
  * is no token, or whose weight is 0, are not read, have dx = 0 and add nothing
- * to dw.  Each element of G is rounded once to the type of x (f32: 22 bits,
- * floor 2^-38) relative to the largest finite weight; sums are f32.  A weight that
- * is not finite breaks its row of dx, and dw.  dx and dw must not overlap x, w or
+ * to dw.  Each element of G is rounded once to the type of x (f32: 22 bits) relative
+ * to the largest finite weight (f16 and f32: floor 2^-38 of it); sums are f32, and an
+ * f32 dw holds them.  A weight that is not finite breaks its row of dx, and dw.  After
+ * a wait that ran out, what is not right is NaN.  dx and dw must not overlap x, w or
  * each other. */
 nk_status nk_linear_ce_backward_device(const void *x, int dtype, uint64_t rows, uint64_t width, uint64_t x_stride,
                                        const void *w, uint64_t vocab, uint64_t w_stride, const uint32_t *targets,
@@ -122,8 +123,8 @@ void nk_adamw_many_free(nk_adamw_many *many);
  * and c = 1 a tensor's result is nk_adamw_step's, bit for bit.  cfg->decay is not
  * read (each tensor has its own).  8-bit moments are read, stepped in f32 (with
  * a few roundings of 2^-23), used for this step's val, and rounded afterwards with a
- * new scale for the block; a v above 0 does not become 0, and |m| is kept up to
- * 2^100.  A moment whose factor (b1, b2) is at most 0.95 is rounded to nearest; what
+ * new scale for the block; a v of 2^-126 or more does not become 0 (a smaller one
+ * counts as 0), and |m| is kept up to 2^100.  A moment whose factor (b1, b2) is at most 0.95 is rounded to nearest; what
  * it forgets in a step is then about half a step of the grid, and it follows its
  * gradients as far as these, or the scale of its block, move it by more.  Above 0.95 it
  * is rounded up or down in proportion to where it lies, so that the mean of m, or of v,

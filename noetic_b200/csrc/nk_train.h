@@ -13,8 +13,8 @@
 namespace nk {
 
 // ---- AdamW over many tensors (adamw_many.cu)
-// Part of a tensor: the 2^17 chunks of a large model are walked by a persistent
-// grid, so one launch serves tensors of any number and size.
+// Part of a tensor: a model's chunks (10 to 20 thousand of a large one) are walked by a
+// persistent grid, so one launch serves tensors of any number and size.
 struct AdamwChunk {
     uint32_t tensor, n;  // n <= the plan's chunk size
     uint64_t first;      // element, a multiple of NK_ADAMW_BLOCK
